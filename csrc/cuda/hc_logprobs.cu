@@ -1,0 +1,449 @@
+// Log probabilities of given tokens, entropies and most likely tokens of rows of logits; gradient of the logits.
+//
+// With m = max x and S = sum exp(x - m):  log p_i = x_i - m - log S,  H = log S - sum exp(x - m) (x - m) / S.
+// One pass over a row: every thread keeps a running maximum and, relative to it, the sum of exp(x - m) and of
+// exp(x - m) (x - m), which are rescaled when its maximum grows; the threads' triples are joined at the end.  When there
+// are few rows, a row is shared out among the blocks of a cluster, which join through shared memory of the cluster.
+//
+// Most likely tokens: value and index form one 64-bit key, so that no two are equal and the order is the one that the
+// header states.  Each thread knows its own maximum after the pass; from one per warp follows a bound that at least
+// `top` keys reach, and only the few threads whose maximum reaches it look at their logits again.  What they find is
+// ranked by counting.
+//
+// Both passes read and write each logit once and are bound by memory; exp and the arithmetic around it come close.
+#include <cooperative_groups.h>
+
+#include "hc_host.cuh"
+#include "hc_train.cuh"
+#include "homcomp_train.h"
+
+namespace hc {
+namespace dev {
+
+constexpr int kRowThreads = 512;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kMostTop = 64;
+constexpr int kCandidates = 2048;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kNothing = -200.0f;  // exp of this and of all below it is 0 in fp32
+
+struct LogprobParams {
+  const void* x;
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int64_t* top_tokens;
+  float* top_logprobs;
+  float* stats;
+  const float* d_logprobs;
+  const float* d_entropy;
+  void* dx;
+  int64_t rows, vocab, stride, dstride, ignore;
+  int top;
+  int cluster;
+};
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// the larger one, or NaN if one is NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+struct Softmax {
+  float m, s, t;  // maximum, sum of exp(x - m), sum of exp(x - m) (x - m)
+};
+// A sum of nothing has m = kLowest, s = t = 0.
+__device__ __forceinline__ Softmax join(const Softmax& a, const Softmax& b) {
+  const float m = fmaxf(a.m, b.m);
+  const float da = fmaxf(a.m - m, kNothing), db = fmaxf(b.m - m, kNothing);
+  const float fa = exp2_fast(da * kLog2e), fb = exp2_fast(db * kLog2e);
+  Softmax r;
+  r.m = m;
+  r.s = fmaf(a.s, fa, b.s * fb);
+  r.t = fmaf(fmaf(a.s, da, a.t), fa, fmaf(b.s, db, b.t) * fb);
+  return r;
+}
+__device__ __forceinline__ Softmax warp_join(Softmax v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Softmax u;
+    u.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+    u.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+    u.t = __shfl_xor_sync(0xffffffffu, v.t, o);
+    // the same operand first in both lanes, so that both get the same bits
+    v = (threadIdx.x & o) ? join(u, v) : join(v, u);
+  }
+  return v;
+}
+
+// Values in an order of whole numbers; 0 is below all.  -0 and +0 are equal.
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float v, int64_t index) {
+  return (uint64_t)ordered(v) << 32 | (0xffffffffu - (uint32_t)index);
+}
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max64(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Where a row begins within an aligned group: groups of eight values (16-bit types: 16 bytes, fp32: 32 bytes)
+template <typename T>
+__device__ __forceinline__ int place_of(const T* row) {
+  return (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) & 7u);
+}
+
+struct TopShared {
+  uint64_t list[kCandidates];
+  uint64_t warp_key[kRowWarps];
+  uint64_t bound;
+  uint64_t best[kMostTop];  // of this block, largest first; 0 where there are fewer
+  uint64_t last[kRowWarps];
+  int count;
+};
+
+// the `top` largest keys of the groups that this block has, into sh.best
+template <typename T>
+__device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, int shift, int64_t begin, int64_t end, float mine,
+                          int64_t where) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t groups = end - begin;
+  // this thread's largest key: in the group in which its maximum stood first
+  uint64_t key = 0;
+  if (where >= 0) {
+    float v[8];
+    load_group(row, where * 8 - shift, p.vocab, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t c = where * 8 - shift + j;
+      if (c >= 0 && c < p.vocab) key = max64(key, key_of(v[j], c));
+    }
+  }
+  // every warp's r-th largest; the (top / r)-th largest of those is reached by at least `top` keys
+  const int warps = (int)(groups < kRowThreads ? (groups + 31) / 32 : kRowWarps);
+  const int r = (p.top + warps - 1) / warps;
+  uint64_t k = key, best = 0;
+  for (int i = 0; i < r && i < 32; ++i) {
+    best = warp_max64(k);
+    if (k == best) k = 0;
+  }
+  if (r > 32) best = 0;
+  if (lane == 0) sh.warp_key[warp] = best;
+  if (threadIdx.x < kMostTop) sh.best[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  if (warp == 0) {
+    k = lane < kRowWarps ? sh.warp_key[lane] : 0;
+    for (int i = 0; i < (p.top + r - 1) / r; ++i) {
+      best = warp_max64(k);
+      if (k == best) k = 0;
+    }
+    if (lane == 0) sh.bound = best;
+  }
+  __syncthreads();
+  const uint64_t bound = sh.bound;
+  if (where >= 0 && ordered(mine) >= (uint32_t)(bound >> 32)) {
+    for (int64_t g = begin + threadIdx.x; g < end; g += kRowThreads) {
+      float v[8];
+      load_group(row, g * 8 - shift, p.vocab, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t c = g * 8 - shift + j;
+        const uint64_t one = key_of(v[j], c);
+        if (c >= 0 && c < p.vocab && one >= bound) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCandidates) sh.list[at] = one;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sh.count;
+  if (n <= kCandidates) {
+    for (int i = threadIdx.x; i < n; i += kRowThreads) {
+      const uint64_t one = sh.list[i];
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += sh.list[j] > one;
+      if (above < p.top) sh.best[above] = one;
+    }
+  } else {
+    // far more candidates than asked for (the largest logits all fell to a few threads): one search per token
+    uint64_t below = ~0ull;
+    for (int i = 0; i < p.top; ++i) {
+      uint64_t found = 0;
+      for (int64_t g = begin + threadIdx.x; g < end; g += kRowThreads) {
+        float v[8];
+        load_group(row, g * 8 - shift, p.vocab, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int64_t c = g * 8 - shift + j;
+          const uint64_t one = key_of(v[j], c);
+          if (c >= 0 && c < p.vocab && one < below) found = max64(found, one);
+        }
+      }
+      found = warp_max64(found);
+      if (lane == 0) sh.last[warp] = found;
+      __syncthreads();
+      found = 0;
+      for (int w = 0; w < kRowWarps; ++w) found = max64(found, sh.last[w]);
+      __syncthreads();
+      if (threadIdx.x == 0) sh.best[i] = found;
+      below = found;
+    }
+  }
+  __syncthreads();
+}
+
+// One row a block, or a cluster of p.cluster blocks for each row.
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kRowThreads) hc_logprob_kernel(const __grid_constant__ LogprobParams p) {
+  __shared__ Softmax warp_part[kRowWarps];
+  __shared__ Softmax block_part;
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  TopShared& sh = *reinterpret_cast<TopShared*>(dynamic);  // only there with kTop
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int part = blockIdx.x % p.cluster;
+  for (int64_t r = blockIdx.x / p.cluster; r < p.rows; r += gridDim.x / p.cluster) {
+    const int64_t token = p.tokens[r];
+    if (token == p.ignore) {  // the same for all threads of the cluster
+      if (part == 0) {
+        if (threadIdx.x == 0) {
+          p.logprobs[r] = 0.0f;
+          p.entropy[r] = 0.0f;
+          if (p.stats) p.stats[r * 3] = p.stats[r * 3 + 1] = p.stats[r * 3 + 2] = 0.0f;
+        }
+        if (kTop && threadIdx.x < p.top) {
+          p.top_tokens[r * p.top + threadIdx.x] = -1;
+          p.top_logprobs[r * p.top + threadIdx.x] = 0.0f;
+        }
+      }
+      continue;
+    }
+    const T* row = static_cast<const T*>(p.x) + r * p.stride;
+    const int shift = place_of(row);
+    const int64_t groups = (p.vocab + shift + 7) / 8;
+    const int64_t begin = groups * part / p.cluster, end = groups * (part + 1) / p.cluster;
+    Softmax a = {kLowest, 0.0f, 0.0f};
+    int64_t where = begin + threadIdx.x < end ? begin + threadIdx.x : -1;
+    for (int64_t g = begin + threadIdx.x; g < end; g += kRowThreads) {
+      float v[8];
+      const int64_t first = g * 8 - shift;
+      load_group(row, first, p.vocab, v);
+      if (first < 0 || first + 8 > p.vocab) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (first + j < 0 || first + j >= p.vocab) v[j] = -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+      if (top > a.m) {
+        const float d = fmaxf(a.m - top, kNothing), f = exp2_fast(d * kLog2e);
+        a.t = fmaf(a.s, d, a.t) * f;
+        a.s *= f;
+        a.m = top;
+        if (kTop) where = g;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = max_nan(v[j] - a.m, kNothing);
+        const float e = exp2_fast(d * kLog2e);
+        a.s += e;
+        a.t = fmaf(e, d, a.t);
+      }
+    }
+    const float mine = a.m;
+    a = warp_join(a);
+    if (lane == 0) warp_part[warp] = a;
+    __syncthreads();
+    if (warp == 0) {
+      a = lane < kRowWarps ? warp_part[lane] : Softmax{kLowest, 0.0f, 0.0f};
+      a = warp_join(a);
+      if (lane == 0) block_part = a;
+    }
+    if (kTop) block_top<T>(p, sh, row, shift, begin, end, mine, where);
+    if (p.cluster > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      if (part == 0) {
+        if (warp == 0) {
+          Softmax b = {kLowest, 0.0f, 0.0f};
+          if (lane < p.cluster) b = *cluster.map_shared_rank(&block_part, lane);
+          a = warp_join(b);
+        }
+        if (kTop) {
+          // the blocks' own largest, ranked together
+          const int n = p.cluster * p.top;
+          for (int i = threadIdx.x; i < n; i += kRowThreads) sh.list[i] = cluster.map_shared_rank(&sh, i / p.top)->best[i % p.top];
+          __syncthreads();
+          for (int i = threadIdx.x; i < n; i += kRowThreads) {
+            const uint64_t one = sh.list[i];
+            int above = 0;
+            for (int j = 0; j < n; ++j) above += sh.list[j] > one;
+            if (one && above < p.top) sh.best[above] = one;
+          }
+        }
+        if (warp == 0 && lane == 0) block_part = a;
+      }
+      cluster.sync();  // nobody leaves, or begins another row, before its part has been read
+    } else {
+      __syncthreads();
+    }
+    if (part == 0) {
+      const Softmax all = block_part;
+      const bool sound = all.s > 0.0f && all.s < INFINITY;  // no NaN, no +inf, something above -inf
+      const float log_s = logf(all.s);
+      if (threadIdx.x == 0) {
+        const float h = sound ? log_s - all.t / all.s : NAN;
+        p.logprobs[r] = sound && token >= 0 && token < p.vocab ? to_float(row[token]) - all.m - log_s : NAN;
+        p.entropy[r] = h;
+        if (p.stats) {
+          p.stats[r * 3] = sound ? all.m : NAN;
+          p.stats[r * 3 + 1] = log_s;
+          p.stats[r * 3 + 2] = h;
+        }
+      }
+      if (kTop && threadIdx.x < p.top) {
+        const uint64_t k = sh.best[threadIdx.x];
+        const int64_t i = 0xffffffffu - (uint32_t)k;
+        p.top_tokens[r * p.top + threadIdx.x] = sound ? i : -1;
+        p.top_logprobs[r * p.top + threadIdx.x] = sound ? to_float(row[i]) - all.m - log_s : NAN;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) hc_logprob_backward_kernel(const __grid_constant__ LogprobParams p) {
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const int64_t token = p.tokens[r];
+    const T* row = static_cast<const T*>(p.x) + r * p.stride;
+    T* out = static_cast<T*>(p.dx) + r * p.dstride;
+    const bool skip = token == p.ignore;
+    const int shift = place_of(row);
+    const bool same = place_of(out) == shift;
+    const int64_t groups = (p.vocab + shift + 7) / 8;
+    const bool lost = !skip && (token < 0 || token >= p.vocab);
+    const float m = skip ? 0.0f : lost ? NAN : p.stats[r * 3], log_s = p.stats[r * 3 + 1], h = p.stats[r * 3 + 2];
+    const float a = !skip && p.d_logprobs ? p.d_logprobs[r] : 0.0f, b = !skip && p.d_entropy ? p.d_entropy[r] : 0.0f;
+    for (int64_t g = (int64_t)blockIdx.y * kRowThreads + threadIdx.x; g < groups; g += (int64_t)gridDim.y * kRowThreads) {
+      const int64_t first = g * 8 - shift;
+      float v[8];
+      if (skip) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      } else {
+        load_group(row, first, p.vocab, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float l = max_nan(v[j] - m - log_s, kNothing);
+          const float e = exp2_fast(l * kLog2e);
+          const float pull = first + j == token ? a : 0.0f;
+          v[j] = fmaf(-e, fmaf(b, l + h, a), pull);
+        }
+      }
+      if (same) {
+        store_group(out, first, p.vocab, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (first + j >= 0 && first + j < p.vocab) out[first + j] = from_float<T>(v[j]);
+      }
+    }
+  }
+}
+
+}  // namespace dev
+
+namespace {
+
+bool logits_ok(const void* x, int type, size_t rows, size_t vocab, size_t stride) {
+  if (!element_type_ok(type) || vocab == 0 || vocab > 0x7fffffffu || stride < vocab || rows > (1ull << 40) || stride > (1ull << 40))
+    return false;
+  return rows == 0 || (x && reinterpret_cast<uintptr_t>(x) % element_bytes(type) == 0 && rows <= (1ull << 60) / stride);
+}
+
+// Blocks per row: as many as leave no SM idle, up to the eight of a portable cluster, while each has at least one group
+// of eight logits for every thread.
+int cluster_of(size_t rows, size_t vocab) {
+  const size_t sms = device_info().sms;
+  int c = 1;
+  while (c < 8 && rows * c * 2 <= 2 * sms && vocab / (size_t)(c * 2) >= dev::kRowThreads * 8 / 2) c *= 2;
+  return c;
+}
+
+template <typename T, bool kTop>
+cudaError_t run_logprobs(dev::LogprobParams p, cudaStream_t stream) {
+  p.cluster = cluster_of(p.rows, p.vocab);
+  const int64_t most = 0x7fffffff / 8;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)((p.rows < most ? p.rows : most) * p.cluster));
+  cfg.blockDim = dim3(dev::kRowThreads);
+  cfg.dynamicSmemBytes = kTop ? sizeof(dev::TopShared) : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  memset(&attr, 0, sizeof(attr));
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, dev::hc_logprob_kernel<T, kTop>, p);
+}
+
+template <typename F>
+cudaError_t by_type(int type, F f) {
+  return type == kF32 ? f(float()) : type == kBf16 ? f(__nv_bfloat16()) : f(__half());
+}
+
+}  // namespace
+}  // namespace hc
+
+extern "C" {
+
+int hc_token_logprobs(const void* logits, int type, size_t rows, size_t vocab, size_t stride, const int64_t* tokens,
+                      int64_t ignore, int top, float* logprobs, float* entropy, int64_t* top_tokens, float* top_logprobs,
+                      float* stats, hc_stream_t stream) {
+  if (!hc::logits_ok(logits, type, rows, vocab, stride)) return hc::kErrArgument;
+  if (top < 0 || top > hc::dev::kMostTop || (size_t)top > vocab) return hc::kErrArgument;
+  if (rows == 0) return hc::kOk;
+  if (!tokens || !logprobs || !entropy || (top && (!top_tokens || !top_logprobs))) return hc::kErrArgument;
+  hc::dev::LogprobParams p = {logits, tokens, logprobs, entropy, top_tokens, top_logprobs, stats, nullptr, nullptr, nullptr,
+                              (int64_t)rows, (int64_t)vocab, (int64_t)stride, 0, ignore, top, 1};
+  const cudaError_t e = hc::by_type(type, [&](auto t) {
+    return top ? hc::run_logprobs<decltype(t), true>(p, stream) : hc::run_logprobs<decltype(t), false>(p, stream);
+  });
+  return e == cudaSuccess ? hc::kOk : hc::kErrCuda;
+}
+
+int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t vocab, size_t stride,
+                               const int64_t* tokens, int64_t ignore, const float* stats, const float* dlogprobs,
+                               const float* dentropy, void* dlogits, size_t dstride, hc_stream_t stream) {
+  if (!hc::logits_ok(logits, type, rows, vocab, stride) || !hc::logits_ok(dlogits, type, rows, vocab, dstride)) return hc::kErrArgument;
+  if (rows == 0) return hc::kOk;
+  if (!tokens || !stats) return hc::kErrArgument;
+  hc::dev::LogprobParams p = {logits, tokens, nullptr, nullptr, nullptr, nullptr, const_cast<float*>(stats), dlogprobs, dentropy, dlogits,
+                              (int64_t)rows, (int64_t)vocab, (int64_t)stride, (int64_t)dstride, ignore, 0, 1};
+  const size_t parts = (vocab + 7 + 8 * hc::dev::kRowThreads - 1) / (8 * hc::dev::kRowThreads);
+  const unsigned y = (unsigned)(rows >= 1024 ? 1 : parts < 1 ? 1 : parts > 64 ? 64 : parts);
+  const dim3 grid((unsigned)(rows < 0x7fffffff ? rows : 0x7fffffff), y);
+  const cudaError_t e = hc::by_type(type, [&](auto t) {
+    hc::dev::hc_logprob_backward_kernel<decltype(t)><<<grid, hc::dev::kRowThreads, 0, stream>>>(p);
+    return cudaGetLastError();
+  });
+  return e == cudaSuccess ? hc::kOk : hc::kErrCuda;
+}
+
+}  // extern "C"

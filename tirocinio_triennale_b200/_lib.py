@@ -119,9 +119,10 @@ def cuda():
             lib = C.CDLL(str(path))
             _declare_cpu(lib)
             _declare_cuda(lib)
-            from . import _lib_ext
+            from . import _lib_ext, _lib_train
 
             _lib_ext.declare(lib)
+            _lib_train.declare(lib)
             _cuda = lib
     return _cuda
 

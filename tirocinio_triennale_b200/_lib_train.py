@@ -1,0 +1,25 @@
+"""Signatures of the training step's operators in libhomcomp_b200.so (csrc/include/homcomp_train.h)."""
+from __future__ import annotations
+
+import ctypes as C
+
+vp = C.c_void_p
+
+
+def declare(lib):
+    sz, f, i, l = C.c_size_t, C.c_float, C.c_int, C.c_int64
+    sizes = {
+        "hc_layer_norm_backward_bytes": [sz, sz],
+    }
+    sigs = {
+        "hc_layer_norm": [vp, i, vp, vp, i, vp, i, vp, sz, sz, f, vp],
+        "hc_layer_norm_backward": [vp, i, vp, i, vp, i, vp, vp, vp, vp, sz, sz, vp, sz, vp],
+        "hc_token_logprobs": [vp, i, sz, sz, sz, vp, l, i, vp, vp, vp, vp, vp, vp],
+        "hc_token_logprobs_backward": [vp, i, sz, sz, sz, vp, l, vp, vp, vp, vp, sz, vp],
+    }
+    for names, restype in ((sizes, sz), (sigs, i)):
+        for name, args in names.items():
+            fn = getattr(lib, name, None)
+            if fn is not None:
+                fn.restype = restype
+                fn.argtypes = args

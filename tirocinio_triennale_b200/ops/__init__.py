@@ -5,3 +5,5 @@ from .cpu_codec import (  # noqa: F401
 )
 from .codec import Codec  # noqa: F401
 from . import stream_io  # noqa: F401
+from .norm import layer_norm  # noqa: F401
+from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
