@@ -1,0 +1,324 @@
+// act(x W^T + b) + residual and its backward pass: the products are hc_gemm.cu's, here is what lies around them.
+#include "hc_gemm.cuh"
+#include "hc_host.cuh"
+#include "hc_train.cuh"
+#include "homcomp_train.h"
+
+namespace hc {
+namespace dev {
+
+// ---- a few rows -----------------------------------------------------------------------------------------------------
+// With up to eight rows the weights are read once and everything else is small: a warp takes two columns of the result,
+// its lanes go along the sum in groups of eight and add up all rows' products, in fp32, joined over the warp at the end.
+// Bound by reading W; the tensor cores would compute 128 rows for these few.
+struct FewRowsParams {
+  const void *x, *w, *bias, *residual;
+  void *out, *z;
+  int64_t ldx, ldw, ldr, ldo, ldz;
+  int64_t inner, width;
+  int rows, out_type, bias_type, activation;
+};
+
+__device__ __forceinline__ float act_value(float z, int kind) {
+  if (kind == kActNone) return z;
+  if (kind == kActRelu) return z > 0.0f ? z : z != z ? z : 0.0f;
+  const float u = kind == kActSilu ? z : 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
+  return z / (1.0f + __expf(-u));
+}
+__device__ __forceinline__ float act_slope(float z, int kind) {
+  if (kind == kActNone) return 1.0f;
+  if (kind == kActRelu) return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+  // d/dz of z sigmoid(v) = s + z s (1 - s) v'; where s (1 - s) is 0, z and v' may have left the range
+  const bool gelu = kind == kActGeluTanh;
+  const float v = gelu ? 1.5957691216057308f * fmaf(0.044715f * z * z, z, z) : z;
+  const float dv = gelu ? 1.5957691216057308f * fmaf(3.0f * 0.044715f * z, z, 1.0f) : 1.0f;
+  const float s = 1.0f / (1.0f + __expf(-v)), t = s * (1.0f - s);
+  return t > 0.0f ? fmaf(z * t, dv, s) : s;
+}
+
+template <typename T, int R, bool kVector>
+__global__ void __launch_bounds__(256) hc_few_rows_kernel(const __grid_constant__ FewRowsParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t first = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * 2;
+  if (first >= p.width) return;
+  const bool two = first + 1 < p.width;
+  const T* w0 = static_cast<const T*>(p.w) + first * p.ldw;
+  const T* w1 = two ? w0 + p.ldw : w0;
+  const T* x = static_cast<const T*>(p.x);
+  float sum[2][R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) sum[0][r] = sum[1][r] = 0.0f;
+  if (kVector) {
+    for (int64_t k = lane * 8; k < p.inner; k += 256) {
+      float a[8], b[8], v[8];
+      load8(w0 + k, a);
+      load8(w1 + k, b);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r < p.rows) {
+          load8(x + r * p.ldx + k, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum[0][r] = fmaf(v[j], a[j], sum[0][r]);
+            sum[1][r] = fmaf(v[j], b[j], sum[1][r]);
+          }
+        }
+      }
+    }
+  } else {
+    for (int64_t k = lane; k < p.inner; k += 32) {
+      const float a = to_float(w0[k]), b = to_float(w1[k]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r < p.rows) {
+          const float v = to_float(x[r * p.ldx + k]);
+          sum[0][r] = fmaf(v, a, sum[0][r]);
+          sum[1][r] = fmaf(v, b, sum[1][r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v = warp_sum(sum[c][r]);
+      const int64_t n = first + c;
+      if (lane == r && r < p.rows && n < p.width) {  // lane r stores row r
+        if (p.bias) v += param_at(p.bias, p.bias_type, n);
+        if (p.z) static_cast<T*>(p.z)[r * p.ldz + n] = from_float<T>(v);
+        v = act_value(v, p.activation);
+        if (p.residual) v += param_at(p.residual, p.out_type, r * p.ldr + n);
+        param_put(p.out, p.out_type, r * p.ldo + n, v);
+      }
+    }
+}
+
+// ---- rows of the backward pass ----------------------------------------------------------------------------------------
+// dz = dy act'(z), rounded for the products, and the sums of its columns.  A thread has eight columns, a block 256 and a
+// share of the rows.  Bound by memory.
+struct RowsBackwardParams {
+  const void *dy, *z;
+  void* dz;
+  float* partial;  // [share][width]
+  int64_t ldy, ldz, ldd, rows, width;
+  int activation, shares;
+};
+
+template <typename Y, typename T, bool kVector>
+__global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_constant__ RowsBackwardParams p) {
+  __shared__ float sums[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = blockIdx.x * 256ll + lane * 8;
+  float total[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) total[j] = 0.0f;
+  if (col < p.width) {
+    const bool whole = kVector && col + 8 <= p.width;
+    for (int64_t r = blockIdx.y * 8ll + warp; r < p.rows; r += p.shares * 8ll) {
+      const Y* dy = static_cast<const Y*>(p.dy) + r * p.ldy + col;
+      const T* z = static_cast<const T*>(p.z) + r * p.ldz + col;
+      T* dz = static_cast<T*>(p.dz) + r * p.ldd + col;
+      float g[8], a[8];
+      if (whole) {
+        load8(dy, g);
+        if (p.activation != kActNone) load8(z, a);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          g[j] = col + j < p.width ? to_float(dy[j]) : 0.0f;
+          a[j] = p.activation != kActNone && col + j < p.width ? to_float(z[j]) : 0.0f;
+        }
+      }
+      if (p.activation != kActNone) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] *= act_slope(a[j], p.activation);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) total[j] += g[j];
+      if (p.dz) {
+        if (whole) {
+          store8(dz, g);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (col + j < p.width) dz[j] = from_float<T>(g[j]);
+        }
+      }
+    }
+  }
+  if (!p.partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[warp][lane * 8 + j] = total[j];
+  __syncthreads();
+  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
+  if (c < p.width) p.partial[blockIdx.y * p.width + c] = s;
+}
+
+__global__ void __launch_bounds__(256) hc_rows_finish_kernel(const float* partial, int shares, int64_t width, void* out, int type) {
+  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
+  if (c >= width) return;
+  float s = 0.0f;
+  for (int i = 0; i < shares; ++i) s += partial[i * width + c];
+  param_put(out, type, c, s);
+}
+
+}  // namespace dev
+
+namespace {
+
+constexpr size_t kMostSize = (size_t)1 << 31;
+constexpr size_t kFewRows = 8;
+
+bool sizes_ok(size_t rows, size_t inner, size_t width) {
+  return inner > 0 && width > 0 && inner < kMostSize && width < kMostSize && rows < kMostSize;
+}
+bool stride_ok(size_t stride, size_t least) { return stride >= least && stride < ((size_t)1 << 32); }
+bool product_type(int type) { return type == kBf16 || type == kF16; }
+
+int shares_of(size_t rows, size_t width) {
+  const size_t sms = device_info().sms > 0 ? device_info().sms : 1;
+  const size_t strips = (width + 255) / 256, most = (rows + 31) / 32;
+  size_t shares = (sms * 4 + strips - 1) / strips;
+  if (shares > most) shares = most;
+  if (shares > 64) shares = 64;
+  return (int)(shares ? shares : 1);
+}
+
+template <typename T, int R>
+void few_rows_of(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((p.width + 15) / 16);
+  if (vector) dev::hc_few_rows_kernel<T, R, true><<<grid, 256, 0, stream>>>(p);
+  else dev::hc_few_rows_kernel<T, R, false><<<grid, 256, 0, stream>>>(p);
+}
+template <typename T>
+void few_rows(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
+  if (p.rows == 1) few_rows_of<T, 1>(p, vector, stream);
+  else if (p.rows == 2) few_rows_of<T, 2>(p, vector, stream);
+  else if (p.rows <= 4) few_rows_of<T, 4>(p, vector, stream);
+  else few_rows_of<T, 8>(p, vector, stream);
+}
+
+template <typename Y, typename T>
+void rows_backward(const dev::RowsBackwardParams& p, bool vector, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.width + 255) / 256), (unsigned)p.shares);
+  if (vector) dev::hc_rows_backward_kernel<Y, T, true><<<grid, 256, 0, stream>>>(p);
+  else dev::hc_rows_backward_kernel<Y, T, false><<<grid, 256, 0, stream>>>(p);
+}
+
+bool aligned_rows(const void* p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0; }
+
+}  // namespace
+}  // namespace hc
+
+extern "C" {
+
+int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
+              const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
+              int activation, size_t rows, size_t inner, size_t width, hc_stream_t stream) {
+  using namespace hc;
+  if (!product_type(type) || (out_type != kF32 && out_type != type) || !element_type_ok(bias_type)) return kErrArgument;
+  if (activation < kActNone || activation > kActSilu || !sizes_ok(rows, inner, width)) return kErrArgument;
+  if (!stride_ok(x_stride, inner) || !stride_ok(weight_stride, inner) || !stride_ok(out_stride, width)) return kErrArgument;
+  if ((residual && !stride_ok(residual_stride, width)) || (z && !stride_ok(z_stride, width))) return kErrArgument;
+  if (rows == 0) return kOk;
+  if (!x || !weight || !out) return kErrArgument;
+  if (rows <= kFewRows) {
+    const dev::FewRowsParams p = {x, weight, bias, residual, out, z, (int64_t)x_stride, (int64_t)weight_stride, (int64_t)residual_stride,
+                                  (int64_t)out_stride, (int64_t)z_stride, (int64_t)inner, (int64_t)width, (int)rows, out_type, bias_type, activation};
+    const bool vector = inner % 8 == 0 && aligned_rows(x, x_stride) && aligned_rows(weight, weight_stride);
+    if (type == kBf16) few_rows<__nv_bfloat16>(p, vector, stream);
+    else few_rows<__half>(p, vector, stream);
+    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+  }
+  if (!gemm_operand_ok(x, x_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
+  GemmCall c;
+  memset(&c, 0, sizeof(c));
+  c.mode = kGemmLinear;
+  c.type = type;
+  c.m = rows, c.n = width, c.k = inner, c.batch = 1;
+  c.a = {x, (int64_t)x_stride, 0, true};
+  c.b = {weight, (int64_t)weight_stride, 0, true};
+  c.out = {out, (int64_t)out_stride, 0};
+  c.out2 = {z, (int64_t)z_stride, 0};
+  c.in = {const_cast<void*>(residual), (int64_t)residual_stride, 0};
+  c.out_type = out_type;
+  c.bias = bias;
+  c.bias_type = bias_type;
+  c.activation = activation;
+  return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
+}
+
+size_t hc_linear_rows_backward_bytes(size_t rows, size_t width) {
+  return rows && width ? (size_t)hc::shares_of(rows, width) * width * sizeof(float) : 0;
+}
+
+int hc_linear_rows_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int type,
+                            void* dz, size_t dz_stride, void* dbias, int bias_type, size_t rows, size_t width, void* scratch,
+                            size_t scratch_bytes, hc_stream_t stream) {
+  using namespace hc;
+  if (!product_type(type) || (dy_type != kF32 && dy_type != type) || !element_type_ok(bias_type)) return kErrArgument;
+  if (activation < kActNone || activation > kActSilu || !sizes_ok(rows, 1, width) || !stride_ok(dy_stride, width)) return kErrArgument;
+  if ((dz && !stride_ok(dz_stride, width)) || (activation != kActNone && !stride_ok(z_stride, width))) return kErrArgument;
+  if (rows == 0) {
+    if (!dbias) return kOk;
+    return cudaMemsetAsync(dbias, 0, width * element_bytes(bias_type), stream) == cudaSuccess ? kOk : kErrCuda;
+  }
+  if (!dy || (activation != kActNone && !z)) return kErrArgument;
+  if (!dz && !dbias) return kOk;
+  if (dbias && (!scratch || scratch_bytes < hc_linear_rows_backward_bytes(rows, width))) return kErrArgument;
+  const dev::RowsBackwardParams p = {dy, z, dz, dbias ? static_cast<float*>(scratch) : nullptr, (int64_t)dy_stride, (int64_t)z_stride,
+                                     (int64_t)dz_stride, (int64_t)rows, (int64_t)width, activation, shares_of(rows, width)};
+  const bool vector = aligned_rows(dy, dy_stride) && (!dz || aligned_rows(dz, dz_stride)) && (activation == kActNone || aligned_rows(z, z_stride));
+  if (type == kBf16) {
+    if (dy_type == kF32) rows_backward<float, __nv_bfloat16>(p, vector, stream);
+    else rows_backward<__nv_bfloat16, __nv_bfloat16>(p, vector, stream);
+  } else {
+    if (dy_type == kF32) rows_backward<float, __half>(p, vector, stream);
+    else rows_backward<__half, __half>(p, vector, stream);
+  }
+  if (dbias) dev::hc_rows_finish_kernel<<<(unsigned)((width + 255) / 256), 256, 0, stream>>>(p.partial, p.shares, (int64_t)width, dbias, bias_type);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
+int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weight, size_t weight_stride, int type, void* dx,
+                             size_t dx_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream) {
+  using namespace hc;
+  if (!product_type(type) || !sizes_ok(rows, inner, width)) return kErrArgument;
+  if (!stride_ok(dz_stride, width) || !stride_ok(weight_stride, inner) || !stride_ok(dx_stride, inner)) return kErrArgument;
+  if (rows == 0) return kOk;
+  if (!dz || !weight || !dx || !gemm_operand_ok(dz, dz_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
+  GemmCall c;
+  memset(&c, 0, sizeof(c));
+  c.mode = kGemmLinear;
+  c.type = c.out_type = type;
+  c.m = rows, c.n = inner, c.k = width, c.batch = 1;
+  c.a = {dz, (int64_t)dz_stride, 0, true};
+  c.b = {weight, (int64_t)weight_stride, 0, false};
+  c.out = {dx, (int64_t)dx_stride, 0};
+  return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
+}
+
+int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, size_t x_stride, int type, void* dweight,
+                              size_t dweight_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream) {
+  using namespace hc;
+  if (!product_type(type) || !sizes_ok(rows, inner, width)) return kErrArgument;
+  if (!stride_ok(dz_stride, width) || !stride_ok(x_stride, inner) || !stride_ok(dweight_stride, inner) || !dweight) return kErrArgument;
+  if (rows == 0)
+    return cudaMemset2DAsync(dweight, dweight_stride * 2, 0, inner * 2, width, stream) == cudaSuccess ? kOk : kErrCuda;
+  if (!dz || !x || !gemm_operand_ok(dz, dz_stride) || !gemm_operand_ok(x, x_stride)) return kErrArgument;
+  GemmCall c;
+  memset(&c, 0, sizeof(c));
+  c.mode = kGemmLinear;
+  c.type = c.out_type = type;
+  c.m = width, c.n = inner, c.k = rows, c.batch = 1;
+  c.a = {dz, (int64_t)dz_stride, 0, false};
+  c.b = {x, (int64_t)x_stride, 0, false};
+  c.out = {dweight, (int64_t)dweight_stride, 0};
+  return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
+}
+
+}  // extern "C"

@@ -42,6 +42,42 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
                                const int64_t* tokens, int64_t ignore, const float* stats, const float* dlogprobs,
                                const float* dentropy, void* dlogits, size_t dstride, hc_stream_t stream);
 
+// ---- products ---------------------------------------------------------------------------------------------------------
+// Operands are bf16 or fp16 (`type` 1 or 2), sums fp32.  x [rows][inner], weight [width][inner], out [rows][width].
+// A product on the tensor cores reads its operands in 16-byte pieces: data 16-byte aligned, strides multiples of 8.
+// Results and what is added to them may lie anywhere.
+//
+// activation: 0 none, 1 GELU (tanh form), 2 ReLU, 3 SiLU.
+// out = act(x weight^T + bias) + residual; out_type 0 or `type`, residual (NULL: none) of out_type, bias (NULL: none)
+// of bias_type.  z: what the activation is applied to, of `type`, for the backward pass, or NULL.
+int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
+              const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
+              int activation, size_t rows, size_t inner, size_t width, hc_stream_t stream);
+// First part of the backward pass, over the rows of dy (dy_type 0 or `type`): dz = dy act'(z) of `type` (dz NULL: not
+// stored), dbias = the sums of its columns before rounding (NULL: not formed), in a fixed order.
+size_t hc_linear_rows_backward_bytes(size_t rows, size_t width);
+int hc_linear_rows_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int type,
+                            void* dz, size_t dz_stride, void* dbias, int bias_type, size_t rows, size_t width, void* scratch,
+                            size_t scratch_bytes, hc_stream_t stream);
+// dx = dz weight and dweight = dz^T x, of `type`
+int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weight, size_t weight_stride, int type, void* dx,
+                             size_t dx_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream);
+int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, size_t x_stride, int type, void* dweight,
+                              size_t dweight_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream);
+
+// ---- orthogonalised updates ---------------------------------------------------------------------------------------------
+// Newton-Schulz iteration: X = G / (|G| + eps); `steps` times X = a X + (b S + c S S) X with S = X X^T (or its mirror image
+// from the right where a matrix is taller than wide).  G: `batch` matrices [height][width] of `type`, rows `stride` and
+// matrices `batch_stride` elements apart; out: the same matrices in bf16 without gaps.  Products take fp16 operands; X
+// itself is carried in two fp16 numbers (22 bits), for what is rounded off it grows by up to `a` a step.
+size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
+int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
+                     int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);
+
+// The products' waits are bounded (2 s).  Synchronises the device and returns 3 if one of them ran out since the status
+// was last cleared, 0 if not.
+int hc_train_status(int clear);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,290 @@
+"""Products with bias, activation and residual, and their gradients, against the formulas in 64 bits.
+
+Tolerances count roundings.  u and h are half a step of fp32 and of the operands' type.  Products of 16-bit numbers are exact in
+fp32; a sum over k of them goes through at most k / 16 + 20 additions in a line, each off by at most a whole step (the tensor core
+need not round to nearest).  An activation's slope is at most 1.13, the slope's own slope at most 0.8 (ReLU apart).  Gradients see
+the argument of the activation rounded to the operands' type, and are themselves rounded to it before the products."""
+import ctypes as C
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from tirocinio_triennale_b200 import _lib, ops
+
+U = torch.finfo(torch.float32).eps / 2
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+ACT = {None: lambda z: z, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"), "relu": F.relu, "silu": F.silu}
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def least(t):
+    return 2.0 ** -25 if t == F16 else 1e-37  # half of the smallest number apart from 0
+
+
+def sums(k):
+    return (k / 16 + 20) * 2 * U
+
+
+def make(m, k, n, kind, seed=0, bias=F32, residual=None):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g).to(kind).cuda()
+    w = (torch.randn(n, k, generator=g) / k ** 0.5).to(kind).cuda()
+    b = None if bias is None else torch.randn(n, generator=g).to(bias).cuda()
+    r = None if residual is None else torch.randn(m, n, generator=g).to(residual).cuda()
+    dy = torch.randn(m, n, generator=g).to(kind if r is None else residual).cuda()
+    return x, w, b, r, dy
+
+
+def check(x, w, b, r, dy, act=None, out_dtype=None):
+    t = x.dtype
+    leaves = [None if v is None else v.detach().requires_grad_() for v in (x, w, b, r)]
+    y = ops.linear(leaves[0], leaves[1], leaves[2], activation=act, residual=leaves[3], out_dtype=out_dtype)
+    assert y.dtype == (r.dtype if r is not None else out_dtype or t) and y.shape == (*x.shape[:-1], w.shape[0])
+    assert torch.equal(y, ops.linear(x, w, b, activation=act, residual=r, out_dtype=out_dtype))
+    have = [i for i, v in enumerate(leaves) if v is not None]
+    grads = dict(zip(have, torch.autograd.grad(y, [leaves[i] for i in have], dy)))
+    m, k, n = x.numel() // x.shape[-1], x.shape[-1], w.shape[0]
+    X, W, D = x.double().reshape(m, k), w.double(), dy.double().reshape(m, n)
+    z = X @ W.t()
+    ez = sums(k) * (X.abs() @ W.abs().t())
+    if b is not None:
+        z = z + b.double()
+        ez = ez + U * z.abs()
+    z = z.requires_grad_()
+    a = ACT[act](z)
+    (slope,) = torch.autograd.grad(a.sum(), (z,))
+    a, z = a.detach(), z.detach()
+    want = a if r is None else a + r.double().reshape(m, n)
+    h = half_step(y.dtype)
+    room = 1.01 * (h * want.abs() + 1.13 * ez + 8 * U * (a.abs() + want.abs())) + least(y.dtype)
+    assert ((y.double().reshape(m, n) - want).abs() <= room).all()
+    h = half_step(t)
+    dz = D * slope
+    if act is None:
+        e = torch.zeros_like(dz)
+    else:
+        move = h * z.abs() + ez + least(t)
+        e = D.abs() * (0.8 * move + 8 * U)
+        if act == "relu":
+            e = torch.where(z.abs() <= move, D.abs(), 0.0)
+    if 2 in grads:
+        want = dz.sum(0)
+        assert grads[2].dtype == b.dtype
+        assert ((grads[2].double() - want).abs() <= 1.01 * (e.sum(0) + (m + 64) * U * (dz.abs() + e).sum(0) + half_step(b.dtype) * want.abs()) + least(b.dtype)).all()
+    if 3 in grads:
+        assert torch.equal(grads[3], dy)
+    e = e + h * dz.abs() + least(t)
+    for i, left, right, el in ((0, dz, W, e), (1, dz.t(), X, e.t())):
+        want = left @ right
+        room = el @ right.abs() + sums(left.shape[1]) * ((left.abs() + el) @ right.abs()) + h * want.abs() + least(t)
+        got = grads[i]
+        assert got.dtype == t and got.shape == (x, w)[i].shape
+        assert ((got.double().reshape(want.shape) - want).abs() <= 1.01 * room).all()
+
+
+SIZES = [(9, 8, 8), (16, 64, 64), (100, 72, 136), (128, 128, 256), (129, 130, 131), (200, 7, 1), (300, 1, 300), (130, 96, 257), (257, 1000, 520), (1000, 200, 2304), (640, 2048, 384), (64, 4096, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("kind", [BF16, F16])
+def test_sizes(m, k, n, kind):
+    check(*make(m, k, n, kind, m))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", range(1, 10))
+@pytest.mark.parametrize("k,n", [(768, 2304), (64, 17), (1001, 33), (5000, 100)])
+def test_few_rows(m, k, n):
+    check(*make(m, k, n, BF16, m, BF16, F32 if m % 2 else None))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu_tanh", "relu", "silu"])
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(5, 96, 50), (300, 264, 200), (77, 65, 129)])
+def test_activations(act, kind, m, k, n):
+    check(*make(m, k, n, kind, 1, kind), act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [F32, BF16])
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+@pytest.mark.parametrize("m,k,n", [(3, 64, 96), (130, 128, 100), (260, 64, 512), (50, 70, 33)])
+def test_residuals(residual, act, m, k, n):
+    check(*make(m, k, n, BF16, 2, None, residual), act)
+
+
+@pytest.mark.gpu
+def test_fp32_results():
+    x, w, b, _, dy = make(140, 192, 72, BF16, 3)
+    check(x, w, b, None, dy.float(), None, F32)
+    check(x, w, b, None, dy.float(), "silu", F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(150, 70, 90), (513, 200, 700), (1030, 65, 258), (4, 300, 40), (2000, 130, 520)])
+@pytest.mark.parametrize("kind", [BF16, F16])
+def test_whole_numbers_are_exact(m, k, n, kind):
+    """Small whole numbers: every sum is one that each type holds, so each element has one right value."""
+    g = torch.Generator().manual_seed(m)
+    some = lambda *s: (torch.randint(-1, 2, s, generator=g) * (torch.rand(*s, generator=g) < 0.2)).to(kind).cuda()  # noqa: E731
+    x, w, dy = some(m, k), some(n, k), some(m, n)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    y = ops.linear(*leaves)
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    for got, want in ((y, x.double() @ w.double().t()), (dx, dy.double() @ w.double()), (dw, dy.double().t() @ x.double())):
+        assert want.abs().max() <= 256 and torch.equal(got.double(), want)
+
+
+@pytest.mark.gpu
+def test_views_batches_and_gradients_with_gaps():
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn(3, 50, 400, generator=g).to(BF16).cuda()
+    w = torch.randn(120, 300, generator=g).to(BF16).cuda() / 17
+    for x in (wide[..., :300], wide[..., 1:301], wide[..., ::2][..., :100].repeat(1, 1, 3), wide[:, :, :300].transpose(0, 1), wide[:1, :1, 3:303], wide[:, :2, 3:303]):
+        for weight in (w, w.t().contiguous().t(), torch.cat([w, w], 1)[:, 7:307]):
+            dy = torch.randn(*x.shape[:-1], 120, generator=g).to(BF16).cuda()
+            check(x, weight, None, None, dy)
+    x = wide[0, :, :300].detach().requires_grad_()
+    (dx,) = torch.autograd.grad(ops.linear(x, w).sum(), (x,))  # the gradient of a sum has strides of 0
+    want = w.double().sum(0)
+    assert ((dx.double() - want).abs() <= half_step(BF16) * want.abs() + sums(120) * w.double().abs().sum(0)).all()
+    out = ops.linear(wide[0, :, :300], w, residual=torch.randn(50, 240, generator=g).cuda()[:, ::2])
+    assert out.shape == (50, 120) and out.dtype == F32
+    odd = ops.linear(wide[0, :, :300], w[:113])
+    assert odd.shape == (50, 113) and odd.stride(0) % 8 == 0
+
+
+@pytest.mark.gpu
+def test_rows_of_another_tensor_stay():
+    """Tiles that reach over the last row and column store nothing there."""
+    x, w, b, _, _ = make(130, 64, 100, BF16, 5)
+    lib = _lib.cuda()
+    for n, stride in ((100, 112), (99, 101)):
+        out = torch.full((133, stride), 7.0, dtype=BF16, device="cuda")
+        assert lib.hc_linear(x.data_ptr(), 64, w.data_ptr(), 64, 1, b.data_ptr(), 0, None, 0, out.data_ptr(), 1, stride, None, 0, 0, 130, 64, n,
+                             torch.cuda.current_stream().cuda_stream) == 0
+        assert (out[130:] == 7).all() and (out[:, n:] == 7).all()
+        assert torch.equal(out[:130, :n], ops.linear(x, w[:n], b[:n]))
+
+
+@pytest.mark.gpu
+def test_partial_gradients_and_no_rows():
+    x, w, b, r, dy = make(60, 80, 48, BF16, 6, F32, F32)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b, r)]
+    want = torch.autograd.grad(ops.linear(*leaves[:3], activation="silu", residual=leaves[3]), leaves, dy)
+    for k in range(4):
+        one = [v.detach().requires_grad_(i == k) for i, v in enumerate((x, w, b, r))]
+        got = torch.autograd.grad(ops.linear(*one[:3], activation="silu", residual=one[3]), (one[k],), dy)
+        assert torch.equal(got[0], want[k])
+    leaves = [x[:0].detach().requires_grad_(), w.detach().requires_grad_(), b.detach().requires_grad_()]
+    y = ops.linear(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy[:0].to(BF16))
+    assert y.shape == (0, 48) and dx.shape == (0, 80) and not dw.any() and not db.any()
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    x, w, b, _, dy = make(12, 40, 24, F16, 7)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    grads = torch.autograd.grad(ops.linear(*leaves, activation="gelu_tanh"), leaves, dy)
+    base = [v.double() for v in (x, w, b)]
+
+    def f(x, w, b):
+        return (F.gelu(x @ w.t() + b, approximate="tanh") * dy.double()).sum()
+
+    for k, at in ((0, (3, 5)), (0, (11, 39)), (1, (0, 0)), (1, (23, 7)), (2, (9,))):
+        ends = []
+        for s in (1e-4, -1e-4):
+            moved = [v.clone() for v in base]
+            moved[k][at] += s
+            ends.append(f(*moved))
+        # fp16: half a step 5e-4 of each of at most 40 terms of size 1 to 4, and of the result
+        assert abs((ends[0] - ends[1]) / 2e-4 - grads[k][at].double()) <= 0.03
+
+
+@pytest.mark.gpu
+def test_infinities_and_nan_stay_in_their_rows():
+    x, w, b, _, dy = make(200, 64, 96, BF16, 8)
+    x[5, 3], x[150, 60] = float("nan"), float("inf")
+    y = ops.linear(x, w, b)
+    bad = ~torch.isfinite(y).all(1)
+    assert bad.nonzero().flatten().tolist() == [5, 150] and torch.isnan(y[5]).all()
+    big = torch.tensor([[3e38], [-3e38], [0.0], [float("nan")]], device="cuda").to(BF16).expand(4, 16).contiguous()
+    one = torch.zeros(8, 16, device="cuda", dtype=BF16)
+    one[:, 0] = 1
+    for act in ("gelu_tanh", "silu", "relu"):
+        for rows in (4, 12):  # both kernels
+            v = big.repeat(rows // 4, 1).detach().requires_grad_()
+            y = ops.linear(v, one, activation=act)
+            (d,) = torch.autograd.grad(y, (v,), torch.ones_like(y))
+            assert (y[0] == big[0, 0]).all() and (y[1] == 0).all() and (y[2] == 0).all() and torch.isnan(y[3]).all()
+            assert float(d[0, 0]) == 8 and float(d[1, 0]) == 0 and float(d[2, 0]) == (0 if act == "relu" else 4) and torch.isnan(d[3, 0])
+
+
+@pytest.mark.gpu
+def test_same_bits_every_time_other_streams_and_graphs():
+    x, w, b, r, dy = make(700, 520, 328, BF16, 9, F32, F32)
+
+    def step():
+        leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+        y = ops.linear(*leaves, activation="gelu_tanh", residual=r)
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caught = step()
+    x.copy_(x.flip(0))
+    other = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(want, there))
+    assert all(torch.equal(p, q) for p, q in zip(other, caught))
+    assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+def test_refusals():
+    x, w = torch.zeros(4, 16, device="cuda", dtype=BF16), torch.zeros(8, 16, device="cuda", dtype=BF16)
+    for bad in (lambda: ops.linear(x.float(), w.float()), lambda: ops.linear(x, w.half()), lambda: ops.linear(x, w[:, :8]), lambda: ops.linear(x, w[0]),
+                lambda: ops.linear(x.cpu(), w), lambda: ops.linear(x, w, w[0]), lambda: ops.linear(x, w, activation="tanh"), lambda: ops.linear(x, w, residual=x),
+                lambda: ops.linear(x, w, residual=torch.zeros(4, 8, device="cuda", dtype=F16)), lambda: ops.linear(x, w, out_dtype=F16), lambda: ops.linear(x[:, :0], w[:, :0]),
+                lambda: ops.linear(x, w, residual=torch.zeros(4, 8, device="cuda"), out_dtype=BF16), lambda: ops.linear(x, w, torch.zeros(8))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_refusals_without_a_gpu():
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.linear(torch.ones(2, 8, dtype=BF16), torch.ones(3, 8, dtype=BF16))
+    lib = _lib.cuda()
+    p = C.c_void_p(4096)  # never read: every call below is refused before anything is launched
+    good = dict(x=p, xs=16, w=p, ws=16, type=1, b=None, bt=0, r=None, rs=0, out=p, ot=1, os=24, z=None, zs=0, act=0, m=32, k=16, n=24)
+
+    def forward(**kw):
+        return lib.hc_linear(*{**good, **kw}.values(), None)
+
+    for kw in (dict(type=0), dict(type=3), dict(ot=2), dict(bt=3), dict(act=4), dict(act=-1), dict(k=0), dict(n=0), dict(m=1 << 31), dict(xs=15), dict(ws=8), dict(os=23),
+               dict(r=p, rs=23), dict(z=p, zs=1), dict(x=None), dict(w=None), dict(out=None), dict(x=C.c_void_p(4098)), dict(xs=17), dict(ws=20), dict(w=C.c_void_p(4104))):
+        assert forward(**kw) == 4, kw
+    assert forward(m=0) == 0
+    rows = lambda **kw: lib.hc_linear_rows_backward(*{**dict(dy=p, t=1, s=24, z=p, zs=24, act=1, type=1, dz=p, ds=24, db=p, bt=0, m=32, n=24, sc=p, by=1 << 30), **kw}.values(), None)  # noqa: E731
+    for kw in (dict(t=2), dict(type=0), dict(s=23), dict(zs=23), dict(ds=23), dict(z=None), dict(dy=None), dict(sc=None), dict(by=8), dict(act=9), dict(n=0)):
+        assert rows(**kw) == 4, kw
+    assert rows(dz=None, db=None) == 0
+    for name in ("hc_linear_input_backward", "hc_linear_weight_backward"):
+        other = 16 if name.endswith("weight_backward") else 16
+        call = lambda **kw: getattr(lib, name)(*{**dict(dz=p, ds=24, o=p, os=other, type=1, out=p, outs=16, m=32, k=16, n=24), **kw}.values(), None)  # noqa: B023, E731
+        for kw in (dict(type=0), dict(ds=16), dict(ds=25), dict(os=15), dict(outs=8), dict(dz=None), dict(o=None), dict(out=None), dict(o=C.c_void_p(4100)), dict(k=0)):
+            assert call(**kw) == 4, (name, kw)

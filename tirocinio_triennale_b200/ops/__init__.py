@@ -7,3 +7,6 @@ from .codec import Codec  # noqa: F401
 from . import stream_io  # noqa: F401
 from .norm import layer_norm  # noqa: F401
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
+from .linear import linear  # noqa: F401
+from .orthogonalize import orthogonalize  # noqa: F401
+from ._train import train_status  # noqa: F401

@@ -58,3 +58,36 @@ def size(name: str, device: torch.device, *args) -> int:
 
 def wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def train_status(device=None, clear: bool = True) -> int:
+    """Synchronises and returns the sticky status of the products' kernels on a device (0 = ok, 3 = a wait ran out)."""
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        return int(_lib.cuda().hc_train_status(1 if clear else 0))
+
+
+def padded(n: int) -> int:
+    return (n + 7) // 8 * 8
+
+
+def empty_rows(rows: int, width: int, dtype, device) -> torch.Tensor:
+    """A matrix whose rows begin at 16-byte boundaries: with gaps where eight does not divide ``width``."""
+    t = torch.empty(rows, padded(width), dtype=dtype, device=device)
+    return t if t.shape[1] == width else t[:, :width]
+
+
+def row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else padded(t.shape[1])
+
+
+def rows_adjacent(t: torch.Tensor) -> bool:
+    """A matrix whose rows' elements are adjacent and whose rows do not overlap."""
+    return (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+
+
+def operand(t: torch.Tensor) -> torch.Tensor:
+    """A matrix as the products read it: rows of adjacent elements that begin at 16-byte boundaries; a copy if it is not so."""
+    if rows_adjacent(t) and row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return empty_rows(t.shape[0], t.shape[1], t.dtype, t.device).copy_(t)
