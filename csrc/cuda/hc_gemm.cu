@@ -5,6 +5,10 @@
 // tensor memory, two of them, so that a tile is stored while the next one is computed), four warps store.  An operand
 // may lie along the sum or across it: tile and descriptor differ, the data is not moved, so the products of a backward
 // pass need no transposed copies.
+//
+// Results leave through shared memory: a warp puts 32 rows of 128 bytes there (swizzled, so that no two of its threads
+// meet in a bank) and one TMA store takes them; what is added to a result comes in the same way, one piece ahead, and is
+// overwritten by the result in place.  Stored from registers, a row a thread, the projection 8192 x 2304 x 768 took 101 us.
 #include "hc_gemm.cuh"
 #include "hc_host.cuh"
 #include "hc_train.cuh"
@@ -20,6 +24,8 @@ constexpr uint64_t kGemmLimitNs = 2000ull * 1000 * 1000;
 
 struct GemmParams {
   CUtensorMap map_a, map_b;
+  CUtensorMap map_out, map_out2, map_in, map_in2;  // boxes of 32 rows of 128 bytes; of those that tma_* names
+  CUtensorMap map_mirror;                          // boxes of 64 rows of 32 values of a symmetric result
   int64_t m, n;
   int k_blocks;
   int tiles_m, tiles_n, tiles;  // of one matrix
@@ -34,21 +40,26 @@ struct GemmParams {
   int bias_type, activation;
   float ca, cb, cc;
   const float* scale;
-  int vector_out, vector_out2, vector_in, vector_in2;  // rows begin at 16 bytes
+  int tma_out, tma_out2, tma_in, tma_in2;              // moved by TMA: rows that begin at 16 bytes
 };
 
 __device__ unsigned int g_train_status;
 
+constexpr int kPiece = 4096;             // 32 rows of 128 bytes
+constexpr int kWarpStage = 4 * kPiece;   // two slots of two pieces for each storing warp
+
 template <int BN>
 struct GemmShape {
   static constexpr int kStage = kOperandA + BN * kBK * 2;
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kStages = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+  static constexpr int kSmem = kStages * kStage + 4 * kWarpStage + 1024;
   static constexpr int kColumns = 2 * BN;  // of tensor memory
 };
 
 struct GemmBarriers {
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drained;
+  uint64_t loaded[4][2];
+  alignas(16) float bias[4][64];
   uint32_t tmem;
   uint32_t gave_up;
 };
@@ -73,20 +84,26 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint3
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
-// 32 columns of this warp's 32 rows: thread i has row i
-__device__ __forceinline__ void tc_load32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of this warp's 32 rows: thread i has row i.  The values are there after tc_load_wait.
+__device__ __forceinline__ void tc_load32(uint32_t addr, float* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(addr));
+}
+__device__ __forceinline__ void tc_load_wait(float (&v)[64]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(v[i]));  // no use of a value moves in front of the wait
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, const void* src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z),
+               "r"(smem_u32(src))
+               : "memory");
 }
 
 // A wait that ends: with the barrier, after the limit, or because another role has given up.
@@ -143,112 +160,153 @@ __device__ __forceinline__ float activate(float z, int kind) {
   return z;
 }
 
-// 32 columns of one row
-template <typename T>
-__device__ __forceinline__ void read32(const T* p, int64_t count, bool vector, float (&v)[32]) {
-  if (vector && count >= 32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float w[8];
-      load8(p + i * 8, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i * 8 + j] = w[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = j < count ? to_float(p[j]) : 0.0f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void write32(T* p, int64_t count, bool vector, const float (&v)[32]) {
-  if (vector && count >= 32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = v[i * 8 + j];
-      store8(p + i * 8, w);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < count) p[j] = from_float<T>(v[j]);
-  }
-}
-__device__ __forceinline__ void write32_as(void* p, int type, int64_t at, int64_t count, bool vector, const float (&v)[32]) {
-  if (type == kF32) write32(static_cast<float*>(p) + at, count, vector, v);
-  else if (type == kBf16) write32(static_cast<__nv_bfloat16*>(p) + at, count, vector, v);
-  else write32(static_cast<__half*>(p) + at, count, vector, v);
-}
-__device__ __forceinline__ void read32_as(const void* p, int type, int64_t at, int64_t count, bool vector, float (&v)[32]) {
-  if (type == kF32) read32(static_cast<const float*>(p) + at, count, vector, v);
-  else if (type == kBf16) read32(static_cast<const __nv_bfloat16*>(p) + at, count, vector, v);
-  else read32(static_cast<const __half*>(p) + at, count, vector, v);
-}
-
 constexpr float kLow = 2048.0f;  // lo is held times this: as precise next to hi as fp16 can be
 
-// row, columns col .. col + 31 of matrix z
+// 16 bytes of row `lane` of a swizzled piece
+__device__ __forceinline__ uint4* piece_at(unsigned char* piece, int lane, int i) {
+  return reinterpret_cast<uint4*>(piece + lane * 128 + ((i ^ (lane & 7)) << 4));
+}
+__device__ __forceinline__ void unpack8(const uint4& w, int type, float (&v)[8]) {
+  if (type == kBf16) {
+    unpack2<__nv_bfloat16>(w.x, v[0], v[1]);
+    unpack2<__nv_bfloat16>(w.y, v[2], v[3]);
+    unpack2<__nv_bfloat16>(w.z, v[4], v[5]);
+    unpack2<__nv_bfloat16>(w.w, v[6], v[7]);
+  } else {
+    unpack2<__half>(w.x, v[0], v[1]);
+    unpack2<__half>(w.y, v[2], v[3]);
+    unpack2<__half>(w.z, v[4], v[5]);
+    unpack2<__half>(w.w, v[6], v[7]);
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float* v, int type) {
+  if (type == kBf16)
+    return make_uint4(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3]), pack2<__nv_bfloat16>(v[4], v[5]), pack2<__nv_bfloat16>(v[6], v[7]));
+  return make_uint4(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]), pack2<__half>(v[4], v[5]), pack2<__half>(v[6], v[7]));
+}
+
+// One piece of a result: 32 rows from `row0`, 64 columns from `col0` of matrix z, in v (thread i has row i).  `first` and
+// `second`: the slot's two pieces, with what TMA has brought for it; what TMA is to take away is put there.
 template <int MODE>
-__device__ __forceinline__ void gemm_finish(const GemmParams& p, int64_t z, int64_t row, int64_t col, float (&v)[32]) {
-  const int64_t count = row < p.m ? p.n - col : 0;
-  if (count <= 0) return;
-  const int64_t at = z * p.out.stride + row * p.out.ld + col;
+__device__ __forceinline__ void gemm_finish(const GemmParams& p, int64_t z, int64_t row0, int64_t col0, float (&v)[64], unsigned char* first,
+                                            unsigned char* second, float* bias, bool mirror) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = row0 + lane;
+  const int64_t count = row < p.m ? p.n - col0 : 0;  // columns of this row (may be over 64)
   if (MODE == kGemmLinear) {
     if (p.bias) {
+      bias[lane] = col0 + lane < p.n ? param_at(p.bias, p.bias_type, col0 + lane) : 0.0f;
+      bias[lane + 32] = col0 + lane + 32 < p.n ? param_at(p.bias, p.bias_type, col0 + lane + 32) : 0.0f;
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < count) v[j] += param_at(p.bias, p.bias_type, col + j);
+      for (int j = 0; j < 64; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + j);
+        v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+      }
+      __syncwarp();
     }
-    if (p.out2.data) write32_as(p.out2.data, p.type, row * p.out2.ld + col, count, p.vector_out2, v);
+    if (p.tma_out2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *piece_at(second, lane, i) = pack8(v + i * 8, p.type);
+    } else if (p.out2.data) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j)
+        if (j < count) param_put(p.out2.data, p.type, row * p.out2.ld + col0 + j, v[j]);
+    }
     if (p.activation != kActNone) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = activate(v[j], p.activation);
+      for (int j = 0; j < 64; ++j) v[j] = activate(v[j], p.activation);
     }
-    if (p.in.data) {
-      float r[32];
-      read32_as(p.in.data, p.out_type, row * p.in.ld + col, count, p.vector_in, r);
+    if (p.in.data && !p.tma_in) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] += r[j];
+      for (int j = 0; j < 64; ++j)
+        if (j < count) v[j] += param_at(p.in.data, p.out_type, row * p.in.ld + col0 + j);
     }
-    write32_as(p.out.data, p.out_type, at, count, p.vector_out, v);
-  } else if (MODE == kGemmUpdate) {
-    float hi[32], lo[32];
-    const int64_t from = z * p.in.stride + row * p.in.ld + col;
-    read32(static_cast<const __half*>(p.in.data) + from, count, p.vector_in, hi);
-    read32(static_cast<const __half*>(p.in2.data) + from, count, p.vector_in2, lo);
+    if (p.out_type == kF32) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = fmaf(p.ca, fmaf(lo[j], 1.0f / kLow, hi[j]), v[j]);
-    if (p.out2.data) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        hi[j] = to_float(__float2half_rn(v[j]));
-        lo[j] = (v[j] - hi[j]) * kLow;
+      for (int i = 0; i < 16; ++i) {
+        float4* at = reinterpret_cast<float4*>(piece_at(i < 8 ? first : second, lane, i & 7));
+        if (p.tma_in) {
+          const float4 r = *at;
+          v[i * 4] += r.x, v[i * 4 + 1] += r.y, v[i * 4 + 2] += r.z, v[i * 4 + 3] += r.w;
+        }
+        if (p.tma_out) *at = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
       }
-      write32(static_cast<__half*>(p.out.data) + at, count, p.vector_out, hi);
-      write32(static_cast<__half*>(p.out2.data) + at, count, p.vector_out2, lo);
     } else {
-      const float scale = p.scale[z];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= scale;
-      write32_as(p.out.data, p.out_type, at, count, p.vector_out, v);
+      for (int i = 0; i < 8; ++i) {
+        uint4* at = piece_at(first, lane, i);
+        if (p.tma_in) {
+          float r[8];
+          unpack8(*at, p.type, r);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i * 8 + j] += r[j];
+        }
+        if (p.tma_out) *at = pack8(v + i * 8, p.type);
+      }
+    }
+    if (!p.tma_out) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j)
+        if (j < count) param_put(p.out.data, p.out_type, row * p.out.ld + col0 + j, v[j]);
+    }
+  } else if (MODE == kGemmUpdate) {
+    const bool last = !p.out2.data;
+    const float scale = last ? p.scale[z] : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint4 *at = piece_at(first, lane, i), *at2 = piece_at(second, lane, i);
+      float hi[8], lo[8];
+      unpack8(*at, kF16, hi);
+      unpack8(*at2, kF16, lo);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i * 8 + j] = fmaf(p.ca, fmaf(lo[j], 1.0f / kLow, hi[j]), v[i * 8 + j]) * scale;
+      if (!last) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          hi[j] = to_float(__float2half_rn(v[i * 8 + j]));
+          lo[j] = (v[i * 8 + j] - hi[j]) * kLow;
+        }
+        *at = pack8(hi, kF16);
+        *at2 = pack8(lo, kF16);
+      } else if (p.tma_out) {
+        *at = pack8(v + i * 8, kBf16);
+      }
+    }
+    if (!p.tma_out) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j)
+        if (j < count) param_put(p.out.data, kBf16, z * p.out.stride + row * p.out.ld + col0 + j, v[j]);
     }
   } else {
-    if (col > row) return;  // the mirror image of another tile's
-    if (MODE == kGemmPoly) {
-      const float square = p.scale[z] * p.scale[z], c1 = p.cb * square, c2 = p.cc * square * square;
-      float q[32];
-      read32(static_cast<const __half*>(p.in.data) + z * p.in.stride + row * p.in.ld + col, count, p.vector_in, q);
+    const float square = MODE == kGemmPoly ? p.scale[z] * p.scale[z] : 0.0f, c1 = p.cb * square, c2 = p.cc * square * square;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = fmaf(c2, v[j], c1 * q[j]);
+    for (int i = 0; i < 8; ++i) {
+      uint4* at = piece_at(first, lane, i);
+      if (MODE == kGemmPoly) {
+        float q[8];
+        unpack8(*at, kF16, q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i * 8 + j] = fmaf(c2, v[i * 8 + j], c1 * q[j]);
+      }
+      *at = pack8(v + i * 8, kF16);
     }
-    __half* out = static_cast<__half*>(p.out.data);
-    const int64_t own = min(count, row - col + 1);
-    write32(out + at, own, p.vector_out, v);
+    if (mirror) {  // 64 rows of 32 values, not swizzled: the threads of a warp write neighbours
+      __half* t = reinterpret_cast<__half*>(second) + lane;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < count && col + j < row) out[z * p.out.stride + (col + j) * p.out.ld + row] = __float2half_rn(v[j]);
+      for (int j = 0; j < 64; ++j) t[j * 32] = __float2half_rn(v[j]);
+    }
   }
+}
+
+// brings what is added to the result at (row0, col0) into a slot
+template <int MODE>
+__device__ __forceinline__ void gemm_fetch(const GemmParams& p, int z, int row0, int col0, unsigned char* slot, uint64_t* bar) {
+  const bool both = MODE == kGemmUpdate || (MODE == kGemmLinear && p.out_type == kF32);
+  mbar_expect_tx(bar, both ? 2 * kPiece : kPiece);
+  tma_load_3d(slot, &p.map_in, col0, row0, z, bar);
+  if (MODE == kGemmUpdate) tma_load_3d(slot + kPiece, &p.map_in2, col0, row0, z, bar);
+  else if (both) tma_load_3d(slot + kPiece, &p.map_in, col0 + 32, row0, z, bar);
 }
 
 template <int BN, int MODE>
@@ -268,6 +326,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
       mbar_init(&sh.acc_empty[a], 4);
     }
     mbar_init(&sh.drained, 1);
+    for (int w = 0; w < 4; ++w) {
+      mbar_init(&sh.loaded[w][0], 1);
+      mbar_init(&sh.loaded[w][1], 1);
+    }
     sh.gave_up = 0;
     fence_mbar_init();
     tma_prefetch_map(&p.map_a);
@@ -361,23 +423,68 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
     }
   } else {
     int acc = 0;
-    uint32_t acc_phase = 0;
-    const int quarter = warp & 3;  // the rows of tensor memory that this warp can reach
+    uint32_t acc_phase = 0, uses = 0;  // pieces so far
+    const int quarter = warp & 3;      // the rows of tensor memory that this warp can reach
+    unsigned char* mine = stages + S::kStages * S::kStage + quarter * kWarpStage;
+    uint64_t* loaded = sh.loaded[quarter];
+    const bool fetches = MODE == kGemmPoly || MODE == kGemmUpdate || (MODE == kGemmLinear && p.tma_in);
+    constexpr bool kSymmetric = MODE == kGemmGram || MODE == kGemmPoly;
+    uint32_t fetched = 0;
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       const int z = t / p.tiles;
       int mi, ni;
       tile_place<BN, MODE>(p, t - z * p.tiles, mi, ni);
+      const int row0 = mi * kBM + quarter * 32, col0 = ni * BN;
+      // pieces of this warp that hold something (of a symmetric result: at the diagonal of blocks of 64, or below it)
+      int pieces = row0 < p.m ? (int)min((int64_t)(BN / 64), (p.n - col0 + 63) / 64) : 0;
+      if (kSymmetric && pieces) pieces = min(pieces, row0 / 64 - col0 / 64 + 1);
+      if (fetches && pieces > 0 && lane == 0) {
+        tma_wait_group_read<0>();
+        gemm_fetch<MODE>(p, z, row0, col0, mine + (uses & 1) * 2 * kPiece, &loaded[uses & 1]);
+        ++fetched;
+      }
       const bool ok = gemm_wait(&sh.acc_full[acc], acc_phase, sh);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const int64_t row = (int64_t)mi * kBM + quarter * 32 + lane;
+      bool good = true;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        float v[32];
+      for (int c = 0; c < pieces; ++c, ++uses) {
+        unsigned char* slot = mine + (uses & 1) * 2 * kPiece;
+        if (lane == 0) {
+          if (fetches) {
+            if (c + 1 < pieces) {
+              tma_wait_group_read<0>();
+              gemm_fetch<MODE>(p, z, row0, col0 + (c + 1) * 64, mine + ((uses + 1) & 1) * 2 * kPiece, &loaded[(uses + 1) & 1]);
+              ++fetched;
+            }
+          } else {
+            tma_wait_group_read<1>();
+          }
+        }
         __syncwarp();
-        tc_load32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + c, v);
-        gemm_finish<MODE>(p, z, row, (int64_t)ni * BN + c, v);
+        float v[64];
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + c * 64;
+        tc_load32(from, v);
+        tc_load32(from + 32, v + 32);
+        tc_load_wait(v);
+        if (fetches) good = __all_sync(0xffffffffu, gemm_wait(&loaded[uses & 1], (uses >> 1) & 1, sh));
+        if (!good) break;
+        const bool mirror = kSymmetric && (col0 + c * 64) / 64 < row0 / 64;
+        gemm_finish<MODE>(p, z, row0, col0 + c * 64, v, slot, slot + kPiece, sh.bias[quarter], mirror);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          const int col = col0 + c * 64;
+          if (p.tma_out) {
+            tma_store_3d(&p.map_out, col, row0, z, slot);
+            if (MODE == kGemmLinear && p.out_type == kF32 && col + 32 < p.n) tma_store_3d(&p.map_out, col + 32, row0, z, slot + kPiece);
+          }
+          if (p.tma_out2) tma_store_3d(&p.map_out2, col, row0, z, slot + kPiece);
+          if (mirror) tma_store_3d(&p.map_mirror, row0, col, z, slot + kPiece);
+          tma_commit_group();
+        }
       }
+      if (!good) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
@@ -385,6 +492,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
         acc = 0;
         acc_phase ^= 1;
       }
+    }
+    if (lane == 0) {
+      // what was fetched and not used (after a wait that ran out) lands before the CTA leaves, and all stores are done
+      for (; uses < fetched; ++uses) mbar_wait_bounded(&loaded[uses & 1], (uses >> 1) & 1, kGemmLimitNs);
+      tma_wait_group<0>();
     }
   }
   __syncthreads();
@@ -424,8 +536,21 @@ uint64_t descriptor(bool k_major) {
   return leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
-bool vector_side(const GemmSide& s, size_t bytes) {
-  return s.data && (reinterpret_cast<uintptr_t>(s.data) & 15u) == 0 && s.ld * bytes % 16 == 0 && s.stride * bytes % 16 == 0;
+// A map of boxes of 32 rows of 128 bytes (mirror: 64 rows of 32 values) of something beside the accumulator, if its rows
+// begin at 16 bytes.  TMA stores whole 16 bytes, also at the end of a row (seen on a B200): what it stores to has rows of
+// whole 16 bytes, or no more behind a row than rounds it up to eight values.
+bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall& c, bool stored, bool mirror = false) {
+  const size_t bytes = element_bytes(type);
+  if (stored && c.n * bytes % 16 && s.ld != (c.n + 7) / 8 * 8) return false;
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn || !s.data || (reinterpret_cast<uintptr_t>(s.data) & 15u) || s.ld * bytes % 16 || (c.batch > 1 && s.stride * bytes % 16)) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)c.n, (cuuint64_t)c.m, (cuuint64_t)c.batch};
+  cuuint64_t strides[2] = {(cuuint64_t)(s.ld * bytes), (cuuint64_t)((c.batch > 1 ? s.stride : s.ld) * bytes)};
+  cuuint32_t box[3] = {(cuuint32_t)(mirror ? 32 : 128 / bytes), mirror ? 64u : 32u, 1};
+  cuuint32_t step[3] = {1, 1, 1};
+  return fn(map, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int BN, int MODE>
@@ -478,11 +603,14 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
   p.cb = c.cb;
   p.cc = c.cc;
   p.scale = c.scale;
-  const size_t wide = MODE == kGemmLinear || (MODE == kGemmUpdate && !c.out2.data) ? element_bytes(c.out_type) : 2;
-  p.vector_out = vector_side(c.out, wide);
-  p.vector_out2 = vector_side(c.out2, 2);
-  p.vector_in = vector_side(c.in, MODE == kGemmLinear ? element_bytes(c.out_type) : 2);
-  p.vector_in2 = vector_side(c.in2, 2);
+  constexpr bool kLinear = MODE == kGemmLinear, kUpdate = MODE == kGemmUpdate;
+  p.tma_out = make_side_map(&p.map_out, c.out, c.out_type, c, true);
+  p.tma_out2 = c.out2.data && (kUpdate || (kLinear && c.out_type != kF32)) && make_side_map(&p.map_out2, c.out2, c.type, c, true);
+  p.tma_in = c.in.data && make_side_map(&p.map_in, c.in, kLinear ? c.out_type : kF16, c, false);
+  p.tma_in2 = kUpdate && make_side_map(&p.map_in2, c.in2, kF16, c, false);
+  // the iteration's own arrays lie as TMA wants them
+  if (!kLinear && ((MODE != kGemmGram && !p.tma_in) || (kUpdate && (!p.tma_in2 || (c.out2.data && (!p.tma_out || !p.tma_out2)))))) return cudaErrorInvalidValue;
+  if ((MODE == kGemmGram || MODE == kGemmPoly) && (!p.tma_out || !make_side_map(&p.map_mirror, c.out, kF16, c, true, true))) return cudaErrorInvalidValue;
   const cudaError_t e = set_smem(dev::hc_gemm_kernel<BN, MODE>, S::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t total = tiles * c.batch;

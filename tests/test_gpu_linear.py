@@ -174,6 +174,28 @@ def test_rows_of_another_tensor_stay():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(150, 100, 99), (40, 65, 257), (3, 100, 30), (300, 7, 9)])
+def test_what_lies_between_rows_is_not_read(m, k, n):
+    x, w, b, _, dy = make(m, k, n, BF16, 10, None)
+
+    def apart(t):
+        wide = torch.full((t.shape[0], (t.shape[1] + 8) // 8 * 8), float("nan"), dtype=t.dtype, device="cuda")
+        wide[:, :t.shape[1]] = t
+        return wide[:, :t.shape[1]]
+
+    leaves = [apart(x).requires_grad_(), apart(w).requires_grad_()]
+    y = ops.linear(*leaves, activation="silu")
+    got = (y, *torch.autograd.grad(y, leaves, apart(dy)))
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    y = ops.linear(*leaves, activation="silu")
+    assert all(torch.equal(p, q) for p, q in zip(got, (y, *torch.autograd.grad(y, leaves, dy))))
+    assert all(torch.isfinite(t).all() for t in got)
+    y = ops.linear(apart(x.detach()), apart(w.detach()).requires_grad_())
+    (dw,) = torch.autograd.grad(y, (y.grad_fn.next_functions[1][0].variable,), apart(dy))  # dy goes into the products as it is
+    assert torch.isfinite(dw).all()
+
+
+@pytest.mark.gpu
 def test_partial_gradients_and_no_rows():
     x, w, b, r, dy = make(60, 80, 48, BF16, 6, F32, F32)
     leaves = [v.detach().requires_grad_() for v in (x, w, b, r)]
