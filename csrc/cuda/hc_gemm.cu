@@ -1,13 +1,15 @@
 // out[m, n] = sum over k of a[m, k] b[n, k] on tcgen05 tensor cores, for the operators that are products.
 //
-// One CTA per SM goes through tiles of 128 x BN.  One thread brings the operands' tiles in by TMA (128-byte swizzle, 64
-// of the sum at a time, as many stages as shared memory holds), one issues the matrix instructions (fp32 accumulators in
-// tensor memory, two of them, so that a tile is stored while the next one is computed), four warps store.  An operand
-// may lie along the sum or across it: tile and descriptor differ, the data is not moved, so the products of a backward
-// pass need no transposed copies.
+// Two SMs work on a tile of 256 x BN together (or one on 128 x 64, for small results): each loads its 128 rows of the first
+// operand and one half of the second, and the matrix instruction reads both halves.  An SM loads 64 bytes a cycle at most,
+// which is what 256 x 256 takes at full rate (a tile of 128 x 256 on one SM takes 96: 8192 x 4096 x 8192 ran at 1.18 PFLOP/s).
+// One CTA per SM goes through tiles: one thread brings operands in by TMA (128-byte swizzle, 64 of the sum at a time, as many
+// stages as shared memory holds), one issues the matrix instructions (fp32 accumulators in tensor memory, two of them, so that
+// a tile is stored while the next one is computed), eight warps store.  An operand may lie along the sum or across it: boxes
+// and descriptors differ, the data is not moved, so the products of a backward pass need no transposed copies.
 //
-// Results leave through shared memory: a warp puts 32 rows of 128 bytes there (swizzled, so that no two of its threads
-// meet in a bank) and one TMA store takes them; what is added to a result comes in the same way, one piece ahead, and is
+// Results leave through shared memory: a warp puts 32 rows of 32 values there (swizzled, so that no two of its threads meet
+// in a bank) and one TMA store takes them; what is added to a result comes in the same way, one piece ahead, and is
 // overwritten by the result in place.  Stored from registers, a row a thread, the projection 8192 x 2304 x 768 took 101 us.
 #include "hc_gemm.cuh"
 #include "hc_host.cuh"
@@ -17,15 +19,16 @@
 namespace hc {
 namespace dev {
 
-constexpr int kBM = 128, kBK = 64;
-constexpr int kGemmThreads = 192;
+constexpr int kBM = 128, kBK = 64;  // rows of a CTA, part of the sum in a stage
+constexpr int kStoreWarps = 8;
+constexpr int kGemmThreads = 64 + 32 * kStoreWarps;
 constexpr int kOperandA = kBM * kBK * 2;
 constexpr uint64_t kGemmLimitNs = 2000ull * 1000 * 1000;
 
 struct GemmParams {
   CUtensorMap map_a, map_b;
-  CUtensorMap map_out, map_out2, map_in, map_in2;  // boxes of 32 rows of 128 bytes; of those that tma_* names
-  CUtensorMap map_mirror;                          // boxes of 64 rows of 32 values of a symmetric result
+  CUtensorMap map_out, map_out2, map_in, map_in2;  // boxes of 32 x 32 values; of those that tma_* names
+  CUtensorMap map_mirror;                          // the same of a symmetric result, without swizzle
   int64_t m, n;
   int k_blocks;
   int tiles_m, tiles_n, tiles;  // of one matrix
@@ -45,44 +48,80 @@ struct GemmParams {
 
 __device__ unsigned int g_train_status;
 
-constexpr int kPiece = 4096;             // 32 rows of 128 bytes
-constexpr int kWarpStage = 4 * kPiece;   // two slots of two pieces for each storing warp
+constexpr int kSlot = 4096;            // 32 x 32 values of 4 bytes, or two of 2 bytes
+constexpr int kWarpStage = 2 * kSlot;  // of each storing warp
 
-template <int BN>
+// kCtas: 2 work on a tile, or 1
+template <int BN, int kCtas>
 struct GemmShape {
-  static constexpr int kStage = kOperandA + BN * kBK * 2;
-  static constexpr int kStages = BN == 256 ? 3 : BN == 128 ? 5 : 6;
-  static constexpr int kSmem = kStages * kStage + 4 * kWarpStage + 1024;
+  static constexpr int kB = BN / kCtas;  // rows of the second operand in a CTA
+  static constexpr int kStage = kOperandA + kB * kBK * 2;
+  static constexpr int kStages = kStage > 24 * 1024 ? 5 : 6;
+  static constexpr int kSmem = kStages * kStage + kStoreWarps * kWarpStage + 1024;
   static constexpr int kColumns = 2 * BN;  // of tensor memory
+  static constexpr int kRows = kBM * kCtas;
 };
 
 struct GemmBarriers {
-  uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drained;
-  uint64_t loaded[4][2];
-  alignas(16) float bias[4][64];
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained;
+  uint64_t loaded[kStoreWarps][2];
+  alignas(16) float bias[kStoreWarps][32];
   uint32_t tmem;
   uint32_t gave_up;
 };
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
+// Addresses of the cluster's shared memory: a CTA's own are valid as they are.
+__device__ __forceinline__ uint32_t leader_address(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// bytes are counted at a barrier of this CTA or, in a pair, of the first one
+template <int kCtas>
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if (kCtas == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// arrives at the barrier, in a pair at both CTAs', when the matrix instructions so far are done
+template <int kCtas>
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  if (kCtas == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+template <int kCtas>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+  if (kCtas == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
 // 32 columns of this warp's 32 rows: thread i has row i.  The values are there after tc_load_wait.
 __device__ __forceinline__ void tc_load32(uint32_t addr, float* v) {
@@ -95,10 +134,10 @@ __device__ __forceinline__ void tc_load32(uint32_t addr, float* v) {
         "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void tc_load_wait(float (&v)[64]) {
+__device__ __forceinline__ void tc_load_wait(float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(v[i]));  // no use of a value moves in front of the wait
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));  // no use of a value moves in front of the wait
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, const void* src) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z),
@@ -127,12 +166,12 @@ __device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, GemmBa
 
 // Tile t of a matrix.  Symmetric results: only tiles that reach the diagonal or below it.  Others: 16 rows of tiles at a
 // time, so that the tiles at work share their operands in L2.
-template <int BN, int MODE>
+template <int BN, int kRows, int MODE>
 __device__ __forceinline__ void tile_place(const GemmParams& p, int t, int& mi, int& ni) {
   if (MODE == kGemmGram || MODE == kGemmPoly) {
     mi = 0;
     for (;;) {
-      int count = (mi * kBM + kBM - 1) / BN + 1;
+      int count = (mi * kRows + kRows - 1) / BN + 1;
       if (count > p.tiles_n) count = p.tiles_n;
       if (t < count) break;
       t -= count;
@@ -162,70 +201,68 @@ __device__ __forceinline__ float activate(float z, int kind) {
 
 constexpr float kLow = 2048.0f;  // lo is held times this: as precise next to hi as fp16 can be
 
-// 16 bytes of row `lane` of a swizzled piece
-__device__ __forceinline__ uint4* piece_at(unsigned char* piece, int lane, int i) {
-  return reinterpret_cast<uint4*>(piece + lane * 128 + ((i ^ (lane & 7)) << 4));
+// 16 bytes of row `lane` of a swizzled piece: rows of 128 bytes (fp32) or 64
+__device__ __forceinline__ float4* wide_at(unsigned char* piece, int lane, int i) {
+  return reinterpret_cast<float4*>(piece + lane * 128 + ((i ^ (lane & 7)) << 4));
 }
-__device__ __forceinline__ void unpack8(const uint4& w, int type, float (&v)[8]) {
-  if (type == kBf16) {
-    unpack2<__nv_bfloat16>(w.x, v[0], v[1]);
-    unpack2<__nv_bfloat16>(w.y, v[2], v[3]);
-    unpack2<__nv_bfloat16>(w.z, v[4], v[5]);
-    unpack2<__nv_bfloat16>(w.w, v[6], v[7]);
-  } else {
-    unpack2<__half>(w.x, v[0], v[1]);
-    unpack2<__half>(w.y, v[2], v[3]);
-    unpack2<__half>(w.z, v[4], v[5]);
-    unpack2<__half>(w.w, v[6], v[7]);
-  }
+__device__ __forceinline__ uint4* half_at(unsigned char* piece, int lane, int i) {
+  return reinterpret_cast<uint4*>(piece + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4));
 }
-__device__ __forceinline__ uint4 pack8(const float* v, int type) {
-  if (type == kBf16)
-    return make_uint4(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3]), pack2<__nv_bfloat16>(v[4], v[5]), pack2<__nv_bfloat16>(v[6], v[7]));
-  return make_uint4(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]), pack2<__half>(v[4], v[5]), pack2<__half>(v[6], v[7]));
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+  unpack2<T>(w.x, v[0], v[1]);
+  unpack2<T>(w.y, v[2], v[3]);
+  unpack2<T>(w.z, v[4], v[5]);
+  unpack2<T>(w.w, v[6], v[7]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+__device__ __forceinline__ uint4 pack8_as(const float* v, int type) {
+  return type == kBf16 ? pack8<__nv_bfloat16>(v) : pack8<__half>(v);
 }
 
-// One piece of a result: 32 rows from `row0`, 64 columns from `col0` of matrix z, in v (thread i has row i).  `first` and
-// `second`: the slot's two pieces, with what TMA has brought for it; what TMA is to take away is put there.
+// One piece of a result: 32 rows from `row0`, 32 columns from `col0` of matrix z, in v (thread i has row i).  `slot` has
+// what TMA has brought for it, and what TMA is to take away is put there; `bias`: of this thread's column.
 template <int MODE>
-__device__ __forceinline__ void gemm_finish(const GemmParams& p, int64_t z, int64_t row0, int64_t col0, float (&v)[64], unsigned char* first,
-                                            unsigned char* second, float* bias, bool mirror) {
+__device__ __forceinline__ void gemm_finish(const GemmParams& p, int z, int row0, int col0, float (&v)[32], unsigned char* slot, float bias,
+                                            float* shared_bias, bool mirror) {
   const int lane = threadIdx.x & 31;
   const int64_t row = row0 + lane;
-  const int64_t count = row < p.m ? p.n - col0 : 0;  // columns of this row (may be over 64)
+  const int64_t count = row < p.m ? p.n - col0 : 0;  // columns of this row (may be over 32)
+  unsigned char* second = slot + kSlot / 2;
   if (MODE == kGemmLinear) {
     if (p.bias) {
-      bias[lane] = col0 + lane < p.n ? param_at(p.bias, p.bias_type, col0 + lane) : 0.0f;
-      bias[lane + 32] = col0 + lane + 32 < p.n ? param_at(p.bias, p.bias_type, col0 + lane + 32) : 0.0f;
+      shared_bias[lane] = bias;
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 64; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(bias + j);
+      for (int j = 0; j < 32; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(shared_bias + j);
         v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
       }
-      __syncwarp();
     }
     if (p.tma_out2) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *piece_at(second, lane, i) = pack8(v + i * 8, p.type);
+      for (int i = 0; i < 4; ++i) *half_at(second, lane, i) = pack8_as(v + i * 8, p.type);
     } else if (p.out2.data) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
+      for (int j = 0; j < 32; ++j)
         if (j < count) param_put(p.out2.data, p.type, row * p.out2.ld + col0 + j, v[j]);
     }
     if (p.activation != kActNone) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j) v[j] = activate(v[j], p.activation);
+      for (int j = 0; j < 32; ++j) v[j] = activate(v[j], p.activation);
     }
     if (p.in.data && !p.tma_in) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
+      for (int j = 0; j < 32; ++j)
         if (j < count) v[j] += param_at(p.in.data, p.out_type, row * p.in.ld + col0 + j);
     }
     if (p.out_type == kF32) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float4* at = reinterpret_cast<float4*>(piece_at(i < 8 ? first : second, lane, i & 7));
+      for (int i = 0; i < 8; ++i) {
+        float4* at = wide_at(slot, lane, i);
         if (p.tma_in) {
           const float4 r = *at;
           v[i * 4] += r.x, v[i * 4 + 1] += r.y, v[i * 4 + 2] += r.z, v[i * 4 + 3] += r.w;
@@ -234,31 +271,32 @@ __device__ __forceinline__ void gemm_finish(const GemmParams& p, int64_t z, int6
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint4* at = piece_at(first, lane, i);
+      for (int i = 0; i < 4; ++i) {
+        uint4* at = half_at(slot, lane, i);
         if (p.tma_in) {
           float r[8];
-          unpack8(*at, p.type, r);
+          if (p.type == kBf16) unpack8<__nv_bfloat16>(*at, r);
+          else unpack8<__half>(*at, r);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[i * 8 + j] += r[j];
         }
-        if (p.tma_out) *at = pack8(v + i * 8, p.type);
+        if (p.tma_out) *at = pack8_as(v + i * 8, p.type);
       }
     }
     if (!p.tma_out) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
+      for (int j = 0; j < 32; ++j)
         if (j < count) param_put(p.out.data, p.out_type, row * p.out.ld + col0 + j, v[j]);
     }
   } else if (MODE == kGemmUpdate) {
     const bool last = !p.out2.data;
     const float scale = last ? p.scale[z] : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint4 *at = piece_at(first, lane, i), *at2 = piece_at(second, lane, i);
+    for (int i = 0; i < 4; ++i) {
+      uint4 *at = half_at(slot, lane, i), *at2 = half_at(second, lane, i);
       float hi[8], lo[8];
-      unpack8(*at, kF16, hi);
-      unpack8(*at2, kF16, lo);
+      unpack8<__half>(*at, hi);
+      unpack8<__half>(*at2, lo);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i * 8 + j] = fmaf(p.ca, fmaf(lo[j], 1.0f / kLow, hi[j]), v[i * 8 + j]) * scale;
       if (!last) {
@@ -267,34 +305,34 @@ __device__ __forceinline__ void gemm_finish(const GemmParams& p, int64_t z, int6
           hi[j] = to_float(__float2half_rn(v[i * 8 + j]));
           lo[j] = (v[i * 8 + j] - hi[j]) * kLow;
         }
-        *at = pack8(hi, kF16);
-        *at2 = pack8(lo, kF16);
+        *at = pack8<__half>(hi);
+        *at2 = pack8<__half>(lo);
       } else if (p.tma_out) {
-        *at = pack8(v + i * 8, kBf16);
+        *at = pack8<__nv_bfloat16>(v + i * 8);
       }
     }
     if (!p.tma_out) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
+      for (int j = 0; j < 32; ++j)
         if (j < count) param_put(p.out.data, kBf16, z * p.out.stride + row * p.out.ld + col0 + j, v[j]);
     }
   } else {
     const float square = MODE == kGemmPoly ? p.scale[z] * p.scale[z] : 0.0f, c1 = p.cb * square, c2 = p.cc * square * square;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint4* at = piece_at(first, lane, i);
+    for (int i = 0; i < 4; ++i) {
+      uint4* at = half_at(slot, lane, i);
       if (MODE == kGemmPoly) {
         float q[8];
-        unpack8(*at, kF16, q);
+        unpack8<__half>(*at, q);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i * 8 + j] = fmaf(c2, v[i * 8 + j], c1 * q[j]);
       }
-      *at = pack8(v + i * 8, kF16);
+      *at = pack8<__half>(v + i * 8);
     }
-    if (mirror) {  // 64 rows of 32 values, not swizzled: the threads of a warp write neighbours
+    if (mirror) {  // not swizzled: the threads of a warp write neighbours
       __half* t = reinterpret_cast<__half*>(second) + lane;
 #pragma unroll
-      for (int j = 0; j < 64; ++j) t[j * 32] = __float2half_rn(v[j]);
+      for (int j = 0; j < 32; ++j) t[j * 32] = __float2half_rn(v[j]);
     }
   }
 }
@@ -302,20 +340,21 @@ __device__ __forceinline__ void gemm_finish(const GemmParams& p, int64_t z, int6
 // brings what is added to the result at (row0, col0) into a slot
 template <int MODE>
 __device__ __forceinline__ void gemm_fetch(const GemmParams& p, int z, int row0, int col0, unsigned char* slot, uint64_t* bar) {
-  const bool both = MODE == kGemmUpdate || (MODE == kGemmLinear && p.out_type == kF32);
-  mbar_expect_tx(bar, both ? 2 * kPiece : kPiece);
-  tma_load_3d(slot, &p.map_in, col0, row0, z, bar);
-  if (MODE == kGemmUpdate) tma_load_3d(slot + kPiece, &p.map_in2, col0, row0, z, bar);
-  else if (both) tma_load_3d(slot + kPiece, &p.map_in, col0 + 32, row0, z, bar);
+  const bool whole = MODE == kGemmUpdate || (MODE == kGemmLinear && p.out_type == kF32);
+  mbar_expect_tx(bar, whole ? kSlot : kSlot / 2);
+  load_box<1>(slot, &p.map_in, col0, row0, z, smem_u32(bar));
+  if (MODE == kGemmUpdate) load_box<1>(slot + kSlot / 2, &p.map_in2, col0, row0, z, smem_u32(bar));
 }
 
-template <int BN, int MODE>
+template <int BN, int kCtas, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_constant__ GemmParams p) {
-  using S = GemmShape<BN>;
+  using S = GemmShape<BN, kCtas>;
   extern __shared__ unsigned char raw[];
   __shared__ GemmBarriers sh;
   unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kCtas == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair; the first one issues the matrix instructions
+  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -323,10 +362,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&sh.acc_full[a], 1);
-      mbar_init(&sh.acc_empty[a], 4);
+      mbar_init(&sh.acc_empty[a], kStoreWarps * kCtas);
     }
     mbar_init(&sh.drained, 1);
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kStoreWarps; ++w) {
       mbar_init(&sh.loaded[w][0], 1);
       mbar_init(&sh.loaded[w][1], 1);
     }
@@ -336,11 +375,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
     tma_prefetch_map(&p.map_b);
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(S::kColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if (kCtas == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(S::kColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(S::kColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (kCtas == 2) cluster_sync();  // the other CTA's barriers are there
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   const int total = p.tiles * p.batch;
@@ -351,10 +396,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
       uint32_t phase = 0;
       bool ok = true;
       int issued = 0;
-      for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+      for (int t = unit; ok && t < total; t += units) {
         const int z = t / p.tiles;
         int mi, ni;
-        tile_place<BN, MODE>(p, t - z * p.tiles, mi, ni);
+        tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
+        const int row = mi * S::kRows + rank * kBM, col = ni * BN + rank * S::kB;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!gemm_wait(&sh.empty[s], phase ^ 1, sh)) {
             ok = false;
@@ -362,16 +408,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
           }
           unsigned char* a = stages + s * S::kStage;
           unsigned char* b = a + kOperandA;
-          mbar_expect_tx(&sh.full[s], S::kStage);
+          const uint32_t bar = kCtas == 2 ? leader_address(&sh.full[s]) : smem_u32(&sh.full[s]);
+          if (rank == 0) mbar_expect_tx(&sh.full[s], S::kStage * kCtas);
           if (p.a_across) {
-            for (int i = 0; i < kBM / 64; ++i) tma_load_3d(a + i * 8192, &p.map_a, mi * kBM + i * 64, kb * kBK, z, &sh.full[s]);
+            for (int i = 0; i < kBM / 64; ++i) load_box<kCtas>(a + i * 8192, &p.map_a, row + i * 64, kb * kBK, z, bar);
           } else {
-            tma_load_3d(a, &p.map_a, kb * kBK, mi * kBM, z, &sh.full[s]);
+            load_box<kCtas>(a, &p.map_a, kb * kBK, row, z, bar);
           }
           if (p.b_across) {
-            for (int i = 0; i < BN / 64; ++i) tma_load_3d(b + i * 8192, &p.map_b, ni * BN + i * 64, kb * kBK, z, &sh.full[s]);
+            for (int i = 0; i < S::kB / 64; ++i) load_box<kCtas>(b + i * 8192, &p.map_b, col + i * 64, kb * kBK, z, bar);
           } else {
-            tma_load_3d(b, &p.map_b, kb * kBK, ni * BN, z, &sh.full[s]);
+            load_box<kCtas>(b, &p.map_b, kb * kBK, col, z, bar);
           }
           ++issued;
           if (++s == S::kStages) {
@@ -380,18 +427,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
           }
         }
       }
-      // copies in flight land before the CTA leaves
-      for (int back = 0; back < S::kStages && back < issued; ++back) {
-        const int i = issued - 1 - back;
-        mbar_wait_bounded(&sh.full[i % S::kStages], (i / S::kStages) & 1, kGemmLimitNs);
+      // Copies in flight land before the CTA leaves.  Those of a pair are counted at its first CTA; the second one leaves
+      // behind it, and after a wait that ran out, when they may differ in what they have issued, a millisecond later.
+      if (rank == 0) {
+        for (int back = 0; back < S::kStages && back < issued; ++back) {
+          const int i = issued - 1 - back;
+          mbar_wait_bounded(&sh.full[i % S::kStages], (i / S::kStages) & 1, kGemmLimitNs);
+        }
+      } else if (!ok) {
+        const long long t0 = clock64();
+        for (int i = 0; i < (1 << 22) && clock64() - t0 < 2000000; ++i) {
+        }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int s = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+      for (int t = unit; ok && t < total; t += units) {
         if (!gemm_wait(&sh.acc_empty[acc], acc_phase ^ 1, sh)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * BN;
@@ -404,90 +458,95 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
           const uint32_t a = smem_u32(stages + s * S::kStage);
           const uint64_t da = p.desc_a | (uint64_t)((a & 0x3ffff) >> 4), db = p.desc_b | (uint64_t)(((a + kOperandA) & 0x3ffff) >> 4);
 #pragma unroll
-          for (int i = 0; i < kBK / 16; ++i) tc_mma(d, da + i * p.step_a, db + i * p.step_b, p.idesc, kb > 0 || i > 0);
-          tc_commit(&sh.empty[s]);
+          for (int i = 0; i < kBK / 16; ++i) tc_mma<kCtas>(d, da + i * p.step_a, db + i * p.step_b, p.idesc, kb > 0 || i > 0);
+          tc_commit<kCtas>(&sh.empty[s]);
           if (++s == S::kStages) {
             s = 0;
             phase ^= 1;
           }
         }
-        tc_commit(&sh.acc_full[acc]);
+        tc_commit<kCtas>(&sh.acc_full[acc]);
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
       // so do the matrix instructions
-      tc_commit(&sh.drained);
+      tc_commit<kCtas>(&sh.drained);
       mbar_wait_bounded(&sh.drained, 0, kGemmLimitNs);
     }
   } else {
     int acc = 0;
     uint32_t acc_phase = 0, uses = 0;  // pieces so far
     const int quarter = warp & 3;      // the rows of tensor memory that this warp can reach
-    unsigned char* mine = stages + S::kStages * S::kStage + quarter * kWarpStage;
-    uint64_t* loaded = sh.loaded[quarter];
+    const int half = (warp - 2) >> 2;  // every second piece of 32 columns
+    unsigned char* mine = stages + S::kStages * S::kStage + (warp - 2) * kWarpStage;
+    uint64_t* loaded = sh.loaded[warp - 2];
+    float* shared_bias = sh.bias[warp - 2];
     const bool fetches = MODE == kGemmPoly || MODE == kGemmUpdate || (MODE == kGemmLinear && p.tma_in);
     constexpr bool kSymmetric = MODE == kGemmGram || MODE == kGemmPoly;
     uint32_t fetched = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    for (int t = unit; t < total; t += units) {
       const int z = t / p.tiles;
       int mi, ni;
-      tile_place<BN, MODE>(p, t - z * p.tiles, mi, ni);
-      const int row0 = mi * kBM + quarter * 32, col0 = ni * BN;
-      // pieces of this warp that hold something (of a symmetric result: at the diagonal of blocks of 64, or below it)
-      int pieces = row0 < p.m ? (int)min((int64_t)(BN / 64), (p.n - col0 + 63) / 64) : 0;
-      if (kSymmetric && pieces) pieces = min(pieces, row0 / 64 - col0 / 64 + 1);
-      if (fetches && pieces > 0 && lane == 0) {
-        tma_wait_group_read<0>();
-        gemm_fetch<MODE>(p, z, row0, col0, mine + (uses & 1) * 2 * kPiece, &loaded[uses & 1]);
-        ++fetched;
+      tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
+      const int row0 = mi * S::kRows + rank * kBM + quarter * 32, col0 = ni * BN;
+      // pieces of these rows that hold something (of a symmetric result: at the diagonal of blocks of 32, or below it)
+      int pieces = row0 < p.m ? (int)min((int64_t)(BN / 32), (p.n - col0 + 31) / 32) : 0;
+      if (kSymmetric && pieces) pieces = min(pieces, row0 / 32 - col0 / 32 + 1);
+      float bias = 0.0f;
+      if (half < pieces) {
+        if (fetches && lane == 0) {
+          tma_wait_group_read<0>();
+          gemm_fetch<MODE>(p, z, row0, col0 + half * 32, mine + (uses & 1) * kSlot, &loaded[uses & 1]);
+          ++fetched;
+        }
+        if (MODE == kGemmLinear && p.bias && col0 + half * 32 + lane < p.n) bias = param_at(p.bias, p.bias_type, col0 + half * 32 + lane);
       }
       const bool ok = gemm_wait(&sh.acc_full[acc], acc_phase, sh);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       bool good = true;
 #pragma unroll 1
-      for (int c = 0; c < pieces; ++c, ++uses) {
-        unsigned char* slot = mine + (uses & 1) * 2 * kPiece;
-        if (lane == 0) {
-          if (fetches) {
-            if (c + 1 < pieces) {
-              tma_wait_group_read<0>();
-              gemm_fetch<MODE>(p, z, row0, col0 + (c + 1) * 64, mine + ((uses + 1) & 1) * 2 * kPiece, &loaded[(uses + 1) & 1]);
-              ++fetched;
-            }
-          } else {
-            tma_wait_group_read<1>();
+      for (int c = half; c < pieces; c += 2, ++uses) {
+        const int col = col0 + c * 32;
+        unsigned char* slot = mine + (uses & 1) * kSlot;
+        float next_bias = 0.0f;
+        if (c + 2 < pieces) {
+          if (fetches && lane == 0) {
+            tma_wait_group_read<0>();
+            gemm_fetch<MODE>(p, z, row0, col + 64, mine + ((uses + 1) & 1) * kSlot, &loaded[(uses + 1) & 1]);
+            ++fetched;
           }
+          if (MODE == kGemmLinear && p.bias && col + 64 + lane < p.n) next_bias = param_at(p.bias, p.bias_type, col + 64 + lane);
         }
+        if (!fetches && lane == 0) tma_wait_group_read<1>();
         __syncwarp();
-        float v[64];
-        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + c * 64;
-        tc_load32(from, v);
-        tc_load32(from + 32, v + 32);
+        float v[32];
+        tc_load32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + c * 32, v);
         tc_load_wait(v);
         if (fetches) good = __all_sync(0xffffffffu, gemm_wait(&loaded[uses & 1], (uses >> 1) & 1, sh));
         if (!good) break;
-        const bool mirror = kSymmetric && (col0 + c * 64) / 64 < row0 / 64;
-        gemm_finish<MODE>(p, z, row0, col0 + c * 64, v, slot, slot + kPiece, sh.bias[quarter], mirror);
+        const bool mirror = kSymmetric && col / 32 < row0 / 32;
+        gemm_finish<MODE>(p, z, row0, col, v, slot, bias, shared_bias, mirror);
+        bias = next_bias;
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
-          const int col = col0 + c * 64;
-          if (p.tma_out) {
-            tma_store_3d(&p.map_out, col, row0, z, slot);
-            if (MODE == kGemmLinear && p.out_type == kF32 && col + 32 < p.n) tma_store_3d(&p.map_out, col + 32, row0, z, slot + kPiece);
-          }
-          if (p.tma_out2) tma_store_3d(&p.map_out2, col, row0, z, slot + kPiece);
-          if (mirror) tma_store_3d(&p.map_mirror, row0, col, z, slot + kPiece);
+          if (p.tma_out) tma_store_3d(&p.map_out, col, row0, z, slot);
+          if (p.tma_out2) tma_store_3d(&p.map_out2, col, row0, z, slot + kSlot / 2);
+          if (mirror) tma_store_3d(&p.map_mirror, row0, col, z, slot + kSlot / 2);
           tma_commit_group();
         }
       }
       if (!good) break;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(&sh.acc_empty[acc]);
+        else
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_address(&sh.acc_empty[acc])) : "memory");
+      }
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
@@ -500,10 +559,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
     }
   }
   __syncthreads();
+  if (kCtas == 2) cluster_sync();  // nobody leaves while the other one's memory is read or its barriers are used
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kColumns));
+    if (kCtas == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kColumns));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kColumns));
   }
 }
 
@@ -536,8 +597,7 @@ uint64_t descriptor(bool k_major) {
   return leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// A map of boxes of 32 rows of 128 bytes (mirror: 64 rows of 32 values) of something beside the accumulator, if its rows
-// begin at 16 bytes.  TMA stores whole 16 bytes, also at the end of a row (seen on a B200): what it stores to has rows of
+// A map of boxes of 32 x 32 values of something beside the accumulator, if its rows begin at 16 bytes.  TMA stores whole 16 bytes, also at the end of a row (seen on a B200): what it stores to has rows of
 // whole 16 bytes, or no more behind a row than rounds it up to eight values.
 bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall& c, bool stored, bool mirror = false) {
   const size_t bytes = element_bytes(type);
@@ -546,33 +606,39 @@ bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall
   if (!fn || !s.data || (reinterpret_cast<uintptr_t>(s.data) & 15u) || s.ld * bytes % 16 || (c.batch > 1 && s.stride * bytes % 16)) return false;
   cuuint64_t dims[3] = {(cuuint64_t)c.n, (cuuint64_t)c.m, (cuuint64_t)c.batch};
   cuuint64_t strides[2] = {(cuuint64_t)(s.ld * bytes), (cuuint64_t)((c.batch > 1 ? s.stride : s.ld) * bytes)};
-  cuuint32_t box[3] = {(cuuint32_t)(mirror ? 32 : 128 / bytes), mirror ? 64u : 32u, 1};
+  cuuint32_t box[3] = {32, 32, 1};
   cuuint32_t step[3] = {1, 1, 1};
   return fn(map, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-            s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+            s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, 
+            mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : type == kF32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, int MODE>
+// tiles of one matrix
+template <int MODE>
+int64_t count_tiles(const GemmCall& c, int rows, int bn) {
+  const int64_t tm = (c.m + rows - 1) / rows, tn = (c.n + bn - 1) / bn;
+  if (MODE != kGemmGram && MODE != kGemmPoly) return tm * tn;
+  int64_t tiles = 0;
+  for (int64_t i = 0; i < tm; ++i) {
+    const int64_t count = (i * rows + rows - 1) / bn + 1;
+    tiles += count < tn ? count : tn;
+  }
+  return tiles;
+}
+
+template <int BN, int kCtas, int MODE>
 cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
-  using S = dev::GemmShape<BN>;
+  using S = dev::GemmShape<BN, kCtas>;
   dev::GemmParams p;
   memset(&p, 0, sizeof(p));
   p.m = c.m;
   p.n = c.n;
   p.k_blocks = (int)((c.k + dev::kBK - 1) / dev::kBK);
-  p.tiles_m = (int)((c.m + dev::kBM - 1) / dev::kBM);
+  p.tiles_m = (int)((c.m + S::kRows - 1) / S::kRows);
   p.tiles_n = (int)((c.n + BN - 1) / BN);
   p.batch = (int)c.batch;
-  int64_t tiles = 0;
-  if (MODE == kGemmGram || MODE == kGemmPoly) {
-    for (int i = 0; i < p.tiles_m; ++i) {
-      const int count = (i * dev::kBM + dev::kBM - 1) / BN + 1;
-      tiles += count < p.tiles_n ? count : p.tiles_n;
-    }
-  } else {
-    tiles = (int64_t)p.tiles_m * p.tiles_n;
-  }
+  const int64_t tiles = count_tiles<MODE>(c, S::kRows, BN);
   if (tiles * c.batch > 0x7fffffff) return cudaErrorInvalidValue;
   p.tiles = (int)tiles;
   p.a_across = !c.a.k_major;
@@ -581,7 +647,7 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
                        c.a.k_major ? dev::kBM : dev::kBK))
     return cudaErrorInvalidValue;
   if (!make_matrix_map(&p.map_b, c.type, c.b.data, c.b.k_major ? c.k : c.n, c.b.k_major ? c.n : c.k, c.batch, c.b.ld, c.b.stride,
-                       c.b.k_major ? BN : dev::kBK))
+                       c.b.k_major ? S::kB : dev::kBK))
     return cudaErrorInvalidValue;
   p.desc_a = descriptor(c.a.k_major);
   p.desc_b = descriptor(c.b.k_major);
@@ -589,7 +655,7 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
   p.step_b = c.b.k_major ? 2 : 128;
   const uint32_t format = c.type == kBf16 ? 1u : 0u;
   p.idesc = 1u << 4 | format << 7 | format << 10 | (c.a.k_major ? 0u : 1u << 15) | (c.b.k_major ? 0u : 1u << 16) | (uint32_t)(BN / 8) << 17 |
-            (uint32_t)(dev::kBM / 16) << 24;
+            (uint32_t)(S::kRows / 16) << 24;
   p.out = c.out;
   p.out2 = c.out2;
   p.in = c.in;
@@ -611,33 +677,39 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
   // the iteration's own arrays lie as TMA wants them
   if (!kLinear && ((MODE != kGemmGram && !p.tma_in) || (kUpdate && (!p.tma_in2 || (c.out2.data && (!p.tma_out || !p.tma_out2)))))) return cudaErrorInvalidValue;
   if ((MODE == kGemmGram || MODE == kGemmPoly) && (!p.tma_out || !make_side_map(&p.map_mirror, c.out, kF16, c, true, true))) return cudaErrorInvalidValue;
-  const cudaError_t e = set_smem(dev::hc_gemm_kernel<BN, MODE>, S::kSmem);
+  const cudaError_t e = set_smem(dev::hc_gemm_kernel<BN, kCtas, MODE>, S::kSmem);
   if (e != cudaSuccess) return e;
-  const int64_t total = tiles * c.batch;
-  const int sms = device_info().sms;
-  dev::hc_gemm_kernel<BN, MODE><<<(int)(total < sms ? total : sms), dev::kGemmThreads, S::kSmem, stream>>>(p);
-  return cudaGetLastError();
+  const int64_t total = tiles * c.batch, units = device_info().sms / kCtas;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)((total < units ? total : units) * kCtas));
+  cfg.blockDim = dim3(dev::kGemmThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  memset(&attr, 0, sizeof(attr));
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kCtas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, dev::hc_gemm_kernel<BN, kCtas, MODE>, p);
 }
 
-// Width of a tile.  What a tile takes is its columns (the tensor core's time) and a constant for what does not shrink with
-// it (128 rows of the first operand are loaded for a tile of any width); the launch takes as long as the SM with the most tiles.
+// Which tile: the launch takes as long as the unit (a pair of SMs, or one) with the most tiles.  A stage of a tile costs the
+// cycles of the matrix instructions or those of loading it at 64 bytes a cycle, whichever are more; a tile some 1000 for its
+// start and its columns' stores.
 template <int MODE>
 cudaError_t run_gemm_mode(const GemmCall& c, cudaStream_t stream) {
-  const int64_t sms = device_info().sms > 0 ? device_info().sms : 1;
-  const int64_t tm = (c.m + 127) / 128 * c.batch;
-  int64_t best = 0;
-  int width = 0;
-  for (int bn = 256; bn >= 64; bn /= 2) {
-    const int64_t tiles = tm * ((c.n + bn - 1) / bn);
-    const int64_t cost = (tiles + sms - 1) / sms * (bn + 32);
-    if (width == 0 || cost < best) {
-      best = cost;
-      width = bn;
-    }
-  }
-  if (width == 256) return run_gemm<256, MODE>(c, stream);
-  if (width == 128) return run_gemm<128, MODE>(c, stream);
-  return run_gemm<64, MODE>(c, stream);
+  const int64_t sms = device_info().sms > 1 ? device_info().sms : 2, stages = (c.k + dev::kBK - 1) / dev::kBK;
+  const auto cost = [&](int bn, int ctas, int64_t cycles) {
+    const int64_t tiles = count_tiles<MODE>(c, dev::kBM * ctas, bn) * c.batch, units = sms / ctas;
+    return (tiles + units - 1) / units * (stages * cycles + 1000 + 4 * bn);
+  };
+  const int64_t big = cost(256, 2, 512), middle = cost(128, 2, 384), small = cost(64, 1, 384);
+  if (big <= middle && big <= small) return run_gemm<256, 2, MODE>(c, stream);
+  if (middle <= small) return run_gemm<128, 2, MODE>(c, stream);
+  return run_gemm<64, 1, MODE>(c, stream);
 }
 
 }  // namespace
