@@ -33,6 +33,7 @@ struct GemmParams {
   int k_blocks;
   int tiles_m, tiles_n, tiles;  // of one matrix
   int batch;
+  int parts;  // of the sum, in the place of a batch
   int a_across, b_across;  // the operand lies across the sum: boxes of 64 values across it
   uint32_t idesc;
   uint64_t desc_a, desc_b;    // without the address
@@ -186,12 +187,6 @@ __device__ __forceinline__ void tile_place(const GemmParams& p, int t, int& mi, 
   }
 }
 
-__device__ __forceinline__ float sigmoid(float v) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return r;
-}
 __device__ __forceinline__ float activate(float z, int kind) {
   if (kind == kActGeluTanh) return z * sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));  // (1 + tanh u) / 2 = sigmoid(2 u)
   if (kind == kActSilu) return z * sigmoid(z);
@@ -401,7 +396,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
         int mi, ni;
         tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
         const int row = mi * S::kRows + rank * kBM, col = ni * BN + rank * S::kB;
+        const int zz = p.parts > 1 ? 0 : z, k0 = p.parts > 1 ? z * p.k_blocks : 0;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
+          const int k = (k0 + kb) * kBK;
           if (!gemm_wait(&sh.empty[s], phase ^ 1, sh)) {
             ok = false;
             break;
@@ -411,14 +408,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
           const uint32_t bar = kCtas == 2 ? leader_address(&sh.full[s]) : smem_u32(&sh.full[s]);
           if (rank == 0) mbar_expect_tx(&sh.full[s], S::kStage * kCtas);
           if (p.a_across) {
-            for (int i = 0; i < kBM / 64; ++i) load_box<kCtas>(a + i * 8192, &p.map_a, row + i * 64, kb * kBK, z, bar);
+            for (int i = 0; i < kBM / 64; ++i) load_box<kCtas>(a + i * 8192, &p.map_a, row + i * 64, k, zz, bar);
           } else {
-            load_box<kCtas>(a, &p.map_a, kb * kBK, row, z, bar);
+            load_box<kCtas>(a, &p.map_a, k, row, zz, bar);
           }
           if (p.b_across) {
-            for (int i = 0; i < S::kB / 64; ++i) load_box<kCtas>(b + i * 8192, &p.map_b, col + i * 64, kb * kBK, z, bar);
+            for (int i = 0; i < S::kB / 64; ++i) load_box<kCtas>(b + i * 8192, &p.map_b, col + i * 64, k, zz, bar);
           } else {
-            load_box<kCtas>(b, &p.map_b, kb * kBK, col, z, bar);
+            load_box<kCtas>(b, &p.map_b, k, col, zz, bar);
           }
           ++issued;
           if (++s == S::kStages) {
@@ -628,13 +625,20 @@ int64_t count_tiles(const GemmCall& c, int rows, int bn) {
 }
 
 template <int BN, int kCtas, int MODE>
-cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
+cudaError_t run_gemm(const GemmCall& given, cudaStream_t stream) {
+  GemmCall c = given;
   using S = dev::GemmShape<BN, kCtas>;
   dev::GemmParams p;
   memset(&p, 0, sizeof(p));
   p.m = c.m;
   p.n = c.n;
   p.k_blocks = (int)((c.k + dev::kBK - 1) / dev::kBK);
+  const int64_t operands = c.batch;
+  p.parts = c.parts;
+  if (c.parts > 1) {
+    p.k_blocks = (p.k_blocks + c.parts - 1) / c.parts;  // what a part has behind the end of the sum reads as zeros
+    c.batch = c.parts;
+  }
   p.tiles_m = (int)((c.m + S::kRows - 1) / S::kRows);
   p.tiles_n = (int)((c.n + BN - 1) / BN);
   p.batch = (int)c.batch;
@@ -643,10 +647,10 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
   p.tiles = (int)tiles;
   p.a_across = !c.a.k_major;
   p.b_across = !c.b.k_major;
-  if (!make_matrix_map(&p.map_a, c.type, c.a.data, c.a.k_major ? c.k : c.m, c.a.k_major ? c.m : c.k, c.batch, c.a.ld, c.a.stride,
+  if (!make_matrix_map(&p.map_a, c.type, c.a.data, c.a.k_major ? c.k : c.m, c.a.k_major ? c.m : c.k, operands, c.a.ld, c.a.stride,
                        c.a.k_major ? dev::kBM : dev::kBK))
     return cudaErrorInvalidValue;
-  if (!make_matrix_map(&p.map_b, c.type, c.b.data, c.b.k_major ? c.k : c.n, c.b.k_major ? c.n : c.k, c.batch, c.b.ld, c.b.stride,
+  if (!make_matrix_map(&p.map_b, c.type, c.b.data, c.b.k_major ? c.k : c.n, c.b.k_major ? c.n : c.k, operands, c.b.ld, c.b.stride,
                        c.b.k_major ? S::kB : dev::kBK))
     return cudaErrorInvalidValue;
   p.desc_a = descriptor(c.a.k_major);
@@ -696,23 +700,53 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, dev::hc_gemm_kernel<BN, kCtas, MODE>, p);
 }
 
-// Which tile: the launch takes as long as the unit (a pair of SMs, or one) with the most tiles.  A stage of a tile costs the
-// cycles of the matrix instructions or those of loading it at 64 bytes a cycle, whichever are more; a tile some 1000 for its
-// start and its columns' stores.
+// Cycles that a launch takes: those of the unit (a pair of SMs, or one) with the most tiles.  A stage of a tile costs what the
+// matrix instructions take or what loading it takes at 64 bytes a cycle, whichever is more, a tile some 1000 for its start
+// and four for each of its columns.
+struct TileChoice {
+  int bn, ctas;
+  int64_t cost;
+};
+template <int MODE>
+TileChoice best_tile(const GemmCall& c, int parts) {
+  const int64_t sms = device_info().sms > 1 ? device_info().sms : 2, stages = ((c.k + dev::kBK - 1) / dev::kBK + parts - 1) / parts;
+  const int shapes[3][3] = {{256, 2, 512}, {128, 2, 384}, {64, 1, 384}};
+  TileChoice best = {0, 0, 0};
+  for (const auto& s : shapes) {
+    const int64_t tiles = count_tiles<MODE>(c, dev::kBM * s[1], s[0]) * c.batch * parts, units = sms / s[1];
+    const int64_t cost = (tiles + units - 1) / units * (stages * s[2] + 1000 + 4 * s[0]);
+    if (best.bn == 0 || cost < best.cost) best = {s[0], s[1], cost};
+  }
+  return best;
+}
+
 template <int MODE>
 cudaError_t run_gemm_mode(const GemmCall& c, cudaStream_t stream) {
-  const int64_t sms = device_info().sms > 1 ? device_info().sms : 2, stages = (c.k + dev::kBK - 1) / dev::kBK;
-  const auto cost = [&](int bn, int ctas, int64_t cycles) {
-    const int64_t tiles = count_tiles<MODE>(c, dev::kBM * ctas, bn) * c.batch, units = sms / ctas;
-    return (tiles + units - 1) / units * (stages * cycles + 1000 + 4 * bn);
-  };
-  const int64_t big = cost(256, 2, 512), middle = cost(128, 2, 384), small = cost(64, 1, 384);
-  if (big <= middle && big <= small) return run_gemm<256, 2, MODE>(c, stream);
-  if (middle <= small) return run_gemm<128, 2, MODE>(c, stream);
+  const TileChoice tile = best_tile<MODE>(c, c.parts > 1 ? c.parts : 1);
+  if (tile.bn == 256) return run_gemm<256, 2, MODE>(c, stream);
+  if (tile.bn == 128) return run_gemm<128, 2, MODE>(c, stream);
   return run_gemm<64, 1, MODE>(c, stream);
 }
 
 }  // namespace
+
+int gemm_parts(int64_t m, int64_t n, int64_t k) {
+  GemmCall c;
+  memset(&c, 0, sizeof(c));
+  c.m = m, c.n = n, c.k = k, c.batch = 1;
+  int best = 1;
+  int64_t least = best_tile<kGemmLinear>(c, 1).cost;
+  for (int parts = 2; parts <= 8; ++parts) {
+    if (k < parts * 1024) break;
+    // the parts are written and read once more, some 3000 bytes a cycle, by a launch that takes some 5000 cycles besides
+    const int64_t cost = best_tile<kGemmLinear>(c, parts).cost + 5000 + m * n * 8 * parts / 3000;
+    if (cost < least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  return best;
+}
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
   if (c.mode == kGemmLinear) return run_gemm_mode<kGemmLinear>(c, stream);

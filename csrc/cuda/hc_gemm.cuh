@@ -5,6 +5,14 @@
 #include <stdint.h>
 
 namespace hc {
+namespace dev {
+__device__ __forceinline__ float sigmoid(float v) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+}  // namespace dev
 
 enum GemmMode : int {
   kGemmLinear = 0,  // out = act(acc + bias) + residual; z = acc + bias
@@ -32,6 +40,7 @@ struct GemmCall {
   int mode;
   int type;  // of the operands
   int64_t m, n, k, batch;
+  int parts;  // over 1 (kGemmLinear without anything behind it, batch 1): as many results, each of a part of the sum, as a batch
   GemmOperand a, b;
   GemmSide out, out2;  // result; z, or lo
   GemmSide in, in2;    // residual, c1 or hi; lo
@@ -43,7 +52,8 @@ struct GemmCall {
   const float* scale;  // of each matrix of a batch (kGemmPoly, kGemmUpdate): X is that times what is stored
 };
 
-// status of the kernels: 3 after a wait that ran out, kept until it is cleared
+// Into how many parts the sum of a product with fp32 results is best shared out (1: none).
+int gemm_parts(int64_t m, int64_t n, int64_t k);
 cudaError_t launch_gemm(const GemmCall& call, cudaStream_t stream);
 bool gemm_operand_ok(const void* data, int64_t ld);
 

@@ -22,8 +22,7 @@ struct FewRowsParams {
 __device__ __forceinline__ float act_value(float z, int kind) {
   if (kind == kActNone) return z;
   if (kind == kActRelu) return z > 0.0f ? z : z != z ? z : 0.0f;
-  const float u = kind == kActSilu ? z : 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
-  return z / (1.0f + __expf(-u));
+  return z * sigmoid(kind == kActSilu ? z : 1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
 }
 __device__ __forceinline__ float act_slope(float z, int kind) {
   if (kind == kActNone) return 1.0f;
@@ -32,7 +31,7 @@ __device__ __forceinline__ float act_slope(float z, int kind) {
   const bool gelu = kind == kActGeluTanh;
   const float v = gelu ? 1.5957691216057308f * fmaf(0.044715f * z * z, z, z) : z;
   const float dv = gelu ? 1.5957691216057308f * fmaf(3.0f * 0.044715f * z, z, 1.0f) : 1.0f;
-  const float s = 1.0f / (1.0f + __expf(-v)), t = s * (1.0f - s);
+  const float s = sigmoid(v), t = s * (1.0f - s);
   return t > 0.0f ? fmaf(z * t, dv, s) : s;
 }
 
@@ -105,44 +104,51 @@ struct RowsBackwardParams {
   int activation, shares;
 };
 
-template <typename Y, typename T, bool kVector>
+template <typename Y, typename T, bool kVector, int kAct>
 __global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_constant__ RowsBackwardParams p) {
   __shared__ float sums[8][256];
+  constexpr int kAtOnce = 4;  // rows whose loads are under way together
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = blockIdx.x * 256ll + lane * 8;
+  const int64_t col = blockIdx.x * 256ll + lane * 8, step = p.shares * 8ll;
   float total[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) total[j] = 0.0f;
-  if (col < p.width) {
-    const bool whole = kVector && col + 8 <= p.width;
-    for (int64_t r = blockIdx.y * 8ll + warp; r < p.rows; r += p.shares * 8ll) {
+  const bool whole = kVector && col + 8 <= p.width;
+  for (int64_t r0 = blockIdx.y * 8ll + warp; r0 < p.rows && col < p.width; r0 += step * kAtOnce) {
+    float g[kAtOnce][8], a[kAtOnce][8];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t r = r0 + i * step;
       const Y* dy = static_cast<const Y*>(p.dy) + r * p.ldy + col;
       const T* z = static_cast<const T*>(p.z) + r * p.ldz + col;
-      T* dz = static_cast<T*>(p.dz) + r * p.ldd + col;
-      float g[8], a[8];
-      if (whole) {
-        load8(dy, g);
-        if (p.activation != kActNone) load8(z, a);
+      if (whole && r < p.rows) {
+        load8(dy, g[i]);
+        if (kAct != kActNone) load8(z, a[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          g[j] = col + j < p.width ? to_float(dy[j]) : 0.0f;
-          a[j] = p.activation != kActNone && col + j < p.width ? to_float(z[j]) : 0.0f;
+          const bool in = r < p.rows && col + j < p.width;
+          g[i][j] = in ? to_float(dy[j]) : 0.0f;
+          a[i][j] = kAct != kActNone && in ? to_float(z[j]) : 0.0f;
         }
       }
-      if (p.activation != kActNone) {
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= act_slope(a[j], p.activation);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t r = r0 + i * step;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (kAct != kActNone) g[i][j] *= act_slope(a[i][j], kAct);
+        total[j] += g[i][j];
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) total[j] += g[j];
-      if (p.dz) {
+      if (p.dz && r < p.rows) {
+        T* dz = static_cast<T*>(p.dz) + r * p.ldd + col;
         if (whole) {
-          store8(dz, g);
+          store8(dz, g[i]);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (col + j < p.width) dz[j] = from_float<T>(g[j]);
+            if (col + j < p.width) dz[j] = from_float<T>(g[i][j]);
         }
       }
     }
@@ -159,11 +165,43 @@ __global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_cons
 }
 
 __global__ void __launch_bounds__(256) hc_rows_finish_kernel(const float* partial, int shares, int64_t width, void* out, int type) {
-  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
-  if (c >= width) return;
+  __shared__ float sums[8][32];
+  const int64_t c = blockIdx.x * 32ll + (threadIdx.x & 31);
   float s = 0.0f;
-  for (int i = 0; i < shares; ++i) s += partial[i * width + c];
+  if (c < width)
+    for (int i = threadIdx.x >> 5; i < shares; i += 8) s += partial[i * width + c];
+  sums[threadIdx.x >> 5][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= width) return;
+  s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
   param_put(out, type, c, s);
+}
+
+// ---- products whose sum is shared out ---------------------------------------------------------------------------------
+// dW has few tiles and a long sum: parts of the sum go to different SMs, which leave fp32 matrices that are added here.
+template <typename T>
+__global__ void __launch_bounds__(256) hc_add_parts_kernel(const float* parts, int n, int64_t rows, int64_t width, int64_t ld, int64_t stride, T* out, int64_t ldo) {
+  const int64_t groups = (width + 7) / 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
+    const int64_t r = i / groups, c = (i - r * groups) * 8;
+    float s[8], v[8];
+    load8(parts + r * ld + c, s);
+    for (int k = 1; k < n; ++k) {
+      load8(parts + k * stride + r * ld + c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
+    T* to = out + r * ldo + c;
+    if (c + 8 <= width && ((reinterpret_cast<uintptr_t>(to) & 15u) == 0)) {
+      store8(to, s);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < width) to[j] = from_float<T>(s[j]);
+    }
+  }
 }
 
 }  // namespace dev
@@ -182,9 +220,9 @@ bool product_type(int type) { return type == kBf16 || type == kF16; }
 int shares_of(size_t rows, size_t width) {
   const size_t sms = device_info().sms > 0 ? device_info().sms : 1;
   const size_t strips = (width + 255) / 256, most = (rows + 31) / 32;
-  size_t shares = (sms * 4 + strips - 1) / strips;
+  size_t shares = sms * 4 / strips;
   if (shares > most) shares = most;
-  if (shares > 64) shares = 64;
+  if (shares > 128) shares = 128;
   return (int)(shares ? shares : 1);
 }
 
@@ -202,11 +240,18 @@ void few_rows(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
   else few_rows_of<T, 8>(p, vector, stream);
 }
 
+template <typename Y, typename T, int kAct>
+void rows_backward_of(const dev::RowsBackwardParams& p, bool vector, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.width + 255) / 256), (unsigned)p.shares);
+  if (vector) dev::hc_rows_backward_kernel<Y, T, true, kAct><<<grid, 256, 0, stream>>>(p);
+  else dev::hc_rows_backward_kernel<Y, T, false, kAct><<<grid, 256, 0, stream>>>(p);
+}
 template <typename Y, typename T>
 void rows_backward(const dev::RowsBackwardParams& p, bool vector, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.width + 255) / 256), (unsigned)p.shares);
-  if (vector) dev::hc_rows_backward_kernel<Y, T, true><<<grid, 256, 0, stream>>>(p);
-  else dev::hc_rows_backward_kernel<Y, T, false><<<grid, 256, 0, stream>>>(p);
+  if (p.activation == kActNone) rows_backward_of<Y, T, kActNone>(p, vector, stream);
+  else if (p.activation == kActGeluTanh) rows_backward_of<Y, T, kActGeluTanh>(p, vector, stream);
+  else if (p.activation == kActRelu) rows_backward_of<Y, T, kActRelu>(p, vector, stream);
+  else rows_backward_of<Y, T, kActSilu>(p, vector, stream);
 }
 
 bool aligned_rows(const void* p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0; }
@@ -280,7 +325,7 @@ int hc_linear_rows_backward(const void* dy, int dy_type, size_t dy_stride, const
     if (dy_type == kF32) rows_backward<float, __half>(p, vector, stream);
     else rows_backward<__half, __half>(p, vector, stream);
   }
-  if (dbias) dev::hc_rows_finish_kernel<<<(unsigned)((width + 255) / 256), 256, 0, stream>>>(p.partial, p.shares, (int64_t)width, dbias, bias_type);
+  if (dbias) dev::hc_rows_finish_kernel<<<(unsigned)((width + 31) / 32), 256, 0, stream>>>(p.partial, p.shares, (int64_t)width, dbias, bias_type);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
@@ -302,8 +347,16 @@ int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weigh
   return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
 }
 
+size_t hc_linear_weight_backward_bytes(size_t rows, size_t inner, size_t width) {
+  using namespace hc;
+  if (!sizes_ok(rows, inner, width) || rows == 0) return 0;
+  const int parts = gemm_parts((int64_t)width, (int64_t)inner, (int64_t)rows);
+  return parts > 1 ? (size_t)parts * width * ((inner + 7) / 8 * 8) * sizeof(float) : 0;
+}
+
 int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, size_t x_stride, int type, void* dweight,
-                              size_t dweight_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream) {
+                              size_t dweight_stride, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes,
+                              hc_stream_t stream) {
   using namespace hc;
   if (!product_type(type) || !sizes_ok(rows, inner, width)) return kErrArgument;
   if (!stride_ok(dz_stride, width) || !stride_ok(x_stride, inner) || !stride_ok(dweight_stride, inner) || !dweight) return kErrArgument;
@@ -318,6 +371,23 @@ int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, s
   c.a = {dz, (int64_t)dz_stride, 0, false};
   c.b = {x, (int64_t)x_stride, 0, false};
   c.out = {dweight, (int64_t)dweight_stride, 0};
+  const size_t need = hc_linear_weight_backward_bytes(rows, inner, width);
+  if (need) {
+    if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15u)) return kErrArgument;
+    const int64_t ld = (int64_t)(inner + 7) / 8 * 8, stride = (int64_t)width * ld;
+    c.parts = gemm_parts(c.m, c.n, c.k);
+    c.out_type = kF32;
+    c.out = {scratch, ld, stride};
+    if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
+    const int64_t groups = (int64_t)width * (ld / 8);
+    const unsigned grid = (unsigned)((groups + 255) / 256 < 2368 ? (groups + 255) / 256 : 2368);
+    const float* sums = static_cast<const float*>(scratch);
+    if (type == kBf16)
+      dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__nv_bfloat16*>(dweight), (int64_t)dweight_stride);
+    else
+      dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__half*>(dweight), (int64_t)dweight_stride);
+    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+  }
   return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
 }
 

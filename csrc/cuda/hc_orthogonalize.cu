@@ -23,20 +23,37 @@ struct ScaleParams {
   float growth;
   int64_t height, width, stride, batch_stride, ld;  // ld: of hi and lo
   int parts;
+  int lanes;  // threads of a block that share a row, a power of two
   float eps;
 };
 
-// sums of squares, in 64 bits: the entries may be anything that their type can hold
-template <typename T>
+// The values of one matrix in groups of eight, a block's share of them: f(row, column, values)
+template <typename T, bool kVector, typename F>
+__device__ __forceinline__ void for_groups(const ScaleParams& p, const T* g, F f) {
+  const int rows = kNormThreads / p.lanes, lane = threadIdx.x & (p.lanes - 1);
+  for (int64_t r = (int64_t)blockIdx.x * rows + threadIdx.x / p.lanes; r < p.height; r += (int64_t)p.parts * rows)
+#pragma unroll 4
+    for (int64_t c = lane * 8; c < p.width; c += p.lanes * 8) {
+      float v[8];
+      if (kVector) {
+        load8(g + r * p.stride + c, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < p.width ? to_float(g[r * p.stride + c + j]) : 0.0f;
+      }
+      f(r, c, v);
+    }
+}
+
+// Sums of squares, in 64 bits: the entries may be anything that their type can hold.  Bound by memory.
+template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) hc_square_sum_kernel(const __grid_constant__ ScaleParams p) {
   __shared__ double sums[kNormThreads / 32];
-  const T* g = static_cast<const T*>(p.g) + blockIdx.y * p.batch_stride;
   double s = 0.0;
-  for (int64_t r = blockIdx.x; r < p.height; r += p.parts)
-    for (int64_t c = threadIdx.x; c < p.width; c += kNormThreads) {
-      const double v = (double)to_float(g[r * p.stride + c]);
-      s = fma(v, v, s);
-    }
+  for_groups<T, kVector>(p, static_cast<const T*>(p.g) + blockIdx.y * p.batch_stride, [&](int64_t, int64_t, const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fma((double)v[j], (double)v[j], s);
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
@@ -47,31 +64,44 @@ __global__ void __launch_bounds__(kNormThreads) hc_square_sum_kernel(const __gri
   }
 }
 
-template <typename T>
+template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) hc_scale_kernel(const __grid_constant__ ScaleParams p) {
-  __shared__ double total;
+  __shared__ double factor;
+  __shared__ int exponent;
   if (threadIdx.x < 32) {
     double s = 0.0;
     for (int i = threadIdx.x; i < p.parts; i += 32) s += p.partial[(int64_t)blockIdx.y * p.parts + i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) total = s;
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(s), room = (norm / (norm + (double)p.eps)) * (double)p.growth;
+      int k = 0;
+      while (k < 126 && room * exp2((double)(k + 1)) <= 1.0) ++k;
+      factor = 1.0 / (norm + (double)p.eps);
+      exponent = k;
+      if (blockIdx.x == 0) p.scale[blockIdx.y] = exp2f((float)-k);
+    }
   }
   __syncthreads();
-  const double norm = sqrt(total), room = (norm / (norm + (double)p.eps)) * (double)p.growth;
-  int k = 0;
-  while (k < 126 && room * exp2((double)(k + 1)) <= 1.0) ++k;
-  const double scale = exp2((double)k) / (norm + (double)p.eps);
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.scale[blockIdx.y] = exp2f((float)-k);
-  const T* g = static_cast<const T*>(p.g) + blockIdx.y * p.batch_stride;
+  // 2^k / (norm + eps) as a number of 24 bits times a power of two: products with entries stay in the range of fp32, and
+  // are off by at most 1.5 2^-24
+  int e;
+  const float mantissa = (float)frexp(factor, &e);
+  const int up = e + exponent, first = up / 2, second = up - up / 2;
+  const float power1 = exp2f((float)max(-126, min(127, first))), power2 = exp2f((float)max(-126, min(127, second)));
   const int64_t at = (int64_t)blockIdx.y * p.height * p.ld;
-  for (int64_t r = blockIdx.x; r < p.height; r += gridDim.x)
-    for (int64_t c = threadIdx.x; c < p.width; c += kNormThreads) {
-      const float v = (float)((double)to_float(g[r * p.stride + c]) * scale);
-      const __half hi = __float2half_rn(v);
-      p.hi[at + r * p.ld + c] = hi;
-      p.lo[at + r * p.ld + c] = __float2half_rn((v - __half2float(hi)) * 2048.0f);
+  for_groups<T, kVector>(p, static_cast<const T*>(p.g) + blockIdx.y * p.batch_stride, [&](int64_t r, int64_t c, const float (&v)[8]) {
+    float hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = v[j] * power1 * mantissa * power2;
+      hi[j] = __half2float(__float2half_rn(x));
+      lo[j] = (x - hi[j]) * 2048.0f;
     }
+    // rows of hi and lo have room for whole groups
+    store8(p.hi + at + r * p.ld + c, hi);
+    store8(p.lo + at + r * p.ld + c, lo);
+  });
 }
 
 }  // namespace dev
@@ -80,6 +110,7 @@ namespace {
 
 struct Layout {
   int64_t ld, side, ld_side, parts;
+  int lanes;
   size_t x, s;  // bytes of one array of the size of X, and of S
   size_t total;
 };
@@ -89,7 +120,10 @@ Layout layout_of(size_t batch, size_t height, size_t width) {
   l.ld = (width + 7) / 8 * 8;
   l.side = height < width ? height : width;
   l.ld_side = (l.side + 7) / 8 * 8;
-  l.parts = height < 64 ? height : 64;
+  l.lanes = 1;
+  while (l.lanes < dev::kNormThreads && (size_t)l.lanes * 8 < width) l.lanes *= 2;
+  const size_t rows = dev::kNormThreads / l.lanes, most = (height + rows - 1) / rows, some = (1184 + batch - 1) / (batch ? batch : 1);
+  l.parts = most < some ? most : some;  // about eight blocks an SM
   l.x = round_up(batch * height * l.ld * 2);
   l.s = round_up(batch * l.side * l.ld_side * 2);
   l.total = round_up(batch * l.parts * 8) + round_up(batch * 4) + 3 * l.x + 2 * l.s;
@@ -101,11 +135,17 @@ bool matrices_ok(size_t batch, size_t height, size_t width) {
   return height > 0 && width > 0 && height < most && width < most && batch <= 65535;
 }
 
+template <typename T, bool kVector>
+void scale_of(const dev::ScaleParams& p, size_t batch, cudaStream_t stream) {
+  const dim3 grid((unsigned)p.parts, (unsigned)batch);
+  dev::hc_square_sum_kernel<T, kVector><<<grid, dev::kNormThreads, 0, stream>>>(p);
+  dev::hc_scale_kernel<T, kVector><<<grid, dev::kNormThreads, 0, stream>>>(p);
+}
 template <typename T>
 void scale(const dev::ScaleParams& p, size_t batch, cudaStream_t stream) {
-  dev::hc_square_sum_kernel<T><<<dim3((unsigned)p.parts, (unsigned)batch), dev::kNormThreads, 0, stream>>>(p);
-  const int64_t rows = p.height < 1024 ? p.height : 1024;
-  dev::hc_scale_kernel<T><<<dim3((unsigned)rows, (unsigned)batch), dev::kNormThreads, 0, stream>>>(p);
+  const bool vector = (reinterpret_cast<uintptr_t>(p.g) & 15u) == 0 && p.width % 8 == 0 && p.stride % 8 == 0 && (batch == 1 || p.batch_stride % 8 == 0);
+  if (vector) scale_of<T, true>(p, batch, stream);
+  else scale_of<T, false>(p, batch, stream);
 }
 
 }  // namespace
@@ -138,7 +178,7 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   float growth = 1.0f;
   for (int i = 0; i < steps; ++i) growth *= a > 1.0f || a < -1.0f ? (a < 0.0f ? -a : a) : 1.0f;
   const dev::ScaleParams p = {g, partial, static_cast<__half*>(hi[0]), static_cast<__half*>(lo), scales, growth, (int64_t)height, (int64_t)width, (int64_t)stride,
-                              (int64_t)batch_stride, l.ld, (int)l.parts, eps};
+                              (int64_t)batch_stride, l.ld, (int)l.parts, l.lanes, eps};
   if (type == kF32) scale<float>(p, batch, stream);
   else if (type == kBf16) scale<__nv_bfloat16>(p, batch, stream);
   else scale<__half>(p, batch, stream);

@@ -60,11 +60,14 @@ size_t hc_linear_rows_backward_bytes(size_t rows, size_t width);
 int hc_linear_rows_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int type,
                             void* dz, size_t dz_stride, void* dbias, int bias_type, size_t rows, size_t width, void* scratch,
                             size_t scratch_bytes, hc_stream_t stream);
-// dx = dz weight and dweight = dz^T x, of `type`
+// dx = dz weight and dweight = dz^T x, of `type`.  dweight has a long sum and may have few tiles: its scratch memory (there
+// may be none to give) holds fp32 sums of parts of the rows, which are added in a fixed order.
 int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weight, size_t weight_stride, int type, void* dx,
                              size_t dx_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream);
+size_t hc_linear_weight_backward_bytes(size_t rows, size_t inner, size_t width);
 int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, size_t x_stride, int type, void* dweight,
-                              size_t dweight_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream);
+                              size_t dweight_stride, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes,
+                              hc_stream_t stream);
 
 // ---- orthogonalised updates ---------------------------------------------------------------------------------------------
 // Newton-Schulz iteration: X = G / (|G| + eps); `steps` times X = a X + (b S + c S S) X with S = X X^T (or its mirror image

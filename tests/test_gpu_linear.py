@@ -86,7 +86,7 @@ def check(x, w, b, r, dy, act=None, out_dtype=None):
         assert ((got.double().reshape(want.shape) - want).abs() <= 1.01 * room).all()
 
 
-SIZES = [(9, 8, 8), (16, 64, 64), (100, 72, 136), (128, 128, 256), (129, 130, 131), (200, 7, 1), (300, 1, 300), (130, 96, 257), (257, 1000, 520), (1000, 200, 2304), (640, 2048, 384), (64, 4096, 64)]
+SIZES = [(9, 8, 8), (16, 64, 64), (100, 72, 136), (128, 128, 256), (129, 130, 131), (200, 7, 1), (300, 1, 300), (130, 96, 257), (257, 1000, 520), (1000, 200, 2304), (640, 2048, 384), (64, 4096, 64), (8200, 104, 312), (5003, 33, 77)]
 
 
 @pytest.mark.gpu
@@ -305,8 +305,7 @@ def test_refusals_without_a_gpu():
     for kw in (dict(t=2), dict(type=0), dict(s=23), dict(zs=23), dict(ds=23), dict(z=None), dict(dy=None), dict(sc=None), dict(by=8), dict(act=9), dict(n=0)):
         assert rows(**kw) == 4, kw
     assert rows(dz=None, db=None) == 0
-    for name in ("hc_linear_input_backward", "hc_linear_weight_backward"):
-        other = 16 if name.endswith("weight_backward") else 16
-        call = lambda **kw: getattr(lib, name)(*{**dict(dz=p, ds=24, o=p, os=other, type=1, out=p, outs=16, m=32, k=16, n=24), **kw}.values(), None)  # noqa: B023, E731
+    for name, more in (("hc_linear_input_backward", ()), ("hc_linear_weight_backward", (None, 0))):
+        call = lambda **kw: getattr(lib, name)(*{**dict(dz=p, ds=24, o=p, os=16, type=1, out=p, outs=16, m=32, k=16, n=24), **kw}.values(), *more, None)  # noqa: B023, E731
         for kw in (dict(type=0), dict(ds=16), dict(ds=25), dict(os=15), dict(outs=8), dict(dz=None), dict(o=None), dict(out=None), dict(o=C.c_void_p(4100)), dict(k=0)):
             assert call(**kw) == 4, (name, kw)

@@ -11,6 +11,7 @@ def declare(lib):
     sizes = {
         "hc_layer_norm_backward_bytes": [sz, sz],
         "hc_linear_rows_backward_bytes": [sz, sz],
+        "hc_linear_weight_backward_bytes": [sz, sz, sz],
         "hc_orthogonalize_bytes": [sz, sz, sz],
     }
     sigs = {
@@ -19,7 +20,7 @@ def declare(lib):
         "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp],
         "hc_linear_rows_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, i, sz, sz, vp, sz, vp],
         "hc_linear_input_backward": [vp, sz, vp, sz, i, vp, sz, sz, sz, sz, vp],
-        "hc_linear_weight_backward": [vp, sz, vp, sz, i, vp, sz, sz, sz, sz, vp],
+        "hc_linear_weight_backward": [vp, sz, vp, sz, i, vp, sz, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],
         "hc_train_status": [i],
         "hc_token_logprobs": [vp, i, sz, sz, sz, vp, l, i, vp, vp, vp, vp, vp, vp],

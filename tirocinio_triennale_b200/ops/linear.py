@@ -62,8 +62,10 @@ class _Linear(torch.autograd.Function):
         if want_w:
             dw = empty_rows(n, k, t, dev)
             a = operand(x)
+            need = size("hc_linear_weight_backward_bytes", dev, m, k, n)
+            scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             call("linear backward", "hc_linear_weight_backward", dev, dz.data_ptr(), row_stride(dz), a.data_ptr(), row_stride(a),
-                 TYPES[t], dw.data_ptr(), padded(k), m, k, n)
+                 TYPES[t], dw.data_ptr(), padded(k), m, k, n, ptr(scratch), need)
         return dx, dw, db, dy if want_r else None, None, None
 
 
