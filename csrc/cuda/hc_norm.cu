@@ -6,8 +6,9 @@
 //   h = (x - mean) rstd,  dx = rstd (w dy - mean(w dy) - h mean(w dy h)),  dw = sum dy h,  db = sum dy,
 // with the column sums of a thread's own columns in its registers over all rows that its block works on.  Rows whose
 // length eight does not divide begin at one of eight places within an aligned group; a block takes rows that begin at
-// the same place, so that its threads keep their columns (and their w) from row to row.  The sums of the blocks are
-// added by a second kernel in a fixed order.  Both passes are bound by memory.
+// the same place, so that its threads keep their columns, whose w and b wait in shared memory.  Where a block shares a row,
+// the next row is on its way while it works on this one.  The sums of the blocks are added by a second kernel in a fixed
+// order.  Both passes are bound by memory.
 #include "hc_host.cuh"
 #include "hc_train.cuh"
 #include "homcomp_train.h"
@@ -29,22 +30,105 @@ struct NormParams {
   int period;  // rows r, r + period, ... begin at the same place of an aligned group
 };
 
-// T threads a row, K groups of eight a thread; T = 32: one row a warp, 8 warps a block
+// Eight values as they lie in memory
+template <typename T>
+struct Raw {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+  }
+  __device__ __forceinline__ void load_some(const T* p, int64_t count) {
+    const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = (2 * j < count ? q[2 * j] : 0u) | (2 * j + 1 < count ? q[2 * j + 1] : 0u) << 16;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) unpack2<T>(w[j], v[2 * j], v[2 * j + 1]);
+  }
+  __device__ __forceinline__ void keep(int from, int to) {  // zeros outside of [from, to)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < from || j >= to) w[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+  }
+  // what was computed from the values is computed again behind this, not kept in registers
+  __device__ __forceinline__ void touch() { asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])::"memory"); }
+};
+template <>
+struct Raw<float> {
+  float w[8];
+  __device__ __forceinline__ void load(const float* p) { load8(p, w); }
+  __device__ __forceinline__ void load_some(const float* p, int64_t count) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = j < count ? p[j] : 0.0f;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = w[j];
+  }
+  __device__ __forceinline__ void keep(int from, int to) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < from || j >= to) w[j] = 0.0f;
+  }
+  __device__ __forceinline__ void touch() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("" : "+f"(w[j])::"memory");
+  }
+};
+// The group at `first` of a row whose first value is number `base` of `all`: whole, with the neighbouring rows' values, but
+// nothing behind the last one; what is not the row's reads as 0.
+template <typename T>
+__device__ __forceinline__ void take(Raw<T>& raw, const T* x, int64_t base, int first, int64_t width, int64_t all) {
+  if (first < width) {
+    if (base + first + 8 <= all) raw.load(x + base + first);
+    else raw.load_some(x + base + first, all - base - first);
+  }
+  if (first < 0 || first + 8 > width) raw.keep(max(-first, 0), (int)max(min(width - first, (int64_t)8), (int64_t)0));
+}
+
+template <int T>
+struct Team {
+  static constexpr int kThreads = T == 32 ? 128 : T;
+  static constexpr int kTeams = kThreads / T;
+  static constexpr int kBlocks = T == 32 ? 3 : 512 / T;  // that an SM holds at the least
+  static constexpr bool kAhead = T > 32;  // a row ahead; with a row a warp there are warps enough
+};
+
+// T threads a row, K groups of eight a thread
 template <typename X, typename Y, int T, int K>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) hc_norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(Team<T>::kThreads, Team<T>::kBlocks) hc_norm_kernel(const __grid_constant__ NormParams p) {
+  using G = Team<T>;
   __shared__ float2 shared[T / 32];
+  extern __shared__ __align__(16) float params[];  // w and b by place: [2][K * T * 8]
   const int lane = T == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t team = T == 32 ? blockIdx.x * 8ll + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t teams = T == 32 ? gridDim.x * 8ll : gridDim.x;
+  const int place = blockIdx.x % p.period;
+  const int64_t team = (int64_t)(blockIdx.x / p.period) * G::kTeams + (T == 32 ? threadIdx.x >> 5 : 0);
+  const int64_t step = (int64_t)(gridDim.x / p.period) * G::kTeams * p.period, all = p.rows * p.width;
+  const int shift = (int)(place * p.width & 7);
   const float inv = 1.0f / (float)p.width;
-  for (int64_t row = team; row < p.rows; row += teams) {
-    const int shift = (int)(row * p.width & 7);
-    const X* x = static_cast<const X*>(p.x) + row * p.width;
+  int64_t row = place + team * p.period;
+  Raw<X> raw[K], next[K];
+  if (row < p.rows)
+#pragma unroll
+    for (int k = 0; k < K; ++k) take(raw[k], static_cast<const X*>(p.x), row * p.width, (k * T + lane) * 8 - shift, p.width, all);
+  for (int i = threadIdx.x; i < K * T * 8; i += G::kThreads) {
+    const int64_t c = i - shift;
+    const bool in = c >= 0 && c < p.width;
+    params[i] = !in ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
+    params[K * T * 8 + i] = p.bias && in ? param_at(p.bias, p.param_type, c) : 0.0f;
+  }
+  __syncthreads();
+  for (; row < p.rows; row += step) {
+    if (G::kAhead && row + step < p.rows)
+#pragma unroll
+      for (int k = 0; k < K; ++k) take(next[k], static_cast<const X*>(p.x), (row + step) * p.width, (k * T + lane) * 8 - shift, p.width, all);
     float v[K][8];
     float sum = 0.0f, none = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      load_group(x, ((int64_t)k * T + lane) * 8 - shift, p.width, v[k]);
+      raw[k].values(v[k]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += v[k][j];
     }
@@ -53,13 +137,16 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) hc_norm_kernel(const __grid
     float squares = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t first = ((int64_t)k * T + lane) * 8 - shift;
+      const int first = (k * T + lane) * 8 - shift;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = first + j >= 0 && first + j < p.width ? v[k][j] - mean : 0.0f;
-        v[k][j] = c;
-        squares = fmaf(c, c, squares);
+      for (int j = 0; j < 8; ++j) v[k][j] -= mean;
+      if (first < 0 || first + 8 > p.width) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (first + j < 0 || first + j >= p.width) v[k][j] = 0.0f;
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) squares = fmaf(v[k][j], v[k][j], squares);
     }
     none = 0.0f;
     group_sum2<T>(squares, none, shared);
@@ -67,64 +154,85 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) hc_norm_kernel(const __grid
     Y* y = static_cast<Y*>(p.out) + row * p.width;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t first = ((int64_t)k * T + lane) * 8 - shift;
+      const int first = (k * T + lane) * 8 - shift;
+      if (first >= p.width) continue;
+      float w[8], b[8];
+      load8(params + (k * T + lane) * 8, w);
+      load8(params + K * T * 8 + (k * T + lane) * 8, b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t c = first + j;
-        const bool in = c >= 0 && c < p.width;
-        const float w = p.weight && in ? param_at(p.weight, p.param_type, c) : 1.0f;
-        const float b = p.bias && in ? param_at(p.bias, p.param_type, c) : 0.0f;
-        v[k][j] = fmaf(v[k][j] * rstd, w, b);
-      }
+      for (int j = 0; j < 8; ++j) v[k][j] = fmaf(v[k][j] * rstd, w[j], b[j]);
       store_group(y, first, p.width, v[k]);
     }
     if (p.stats && lane == 0) reinterpret_cast<float2*>(p.stats)[row] = make_float2(mean, rstd);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (G::kAhead) raw[k] = next[k];
+      else if (row + step < p.rows) take(raw[k], static_cast<const X*>(p.x), (row + step) * p.width, (k * T + lane) * 8 - shift, p.width, all);
+    }
   }
 }
 
 template <typename X, typename Y, int T, int K>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) hc_norm_backward_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(Team<T>::kThreads, Team<T>::kBlocks) hc_norm_backward_kernel(const __grid_constant__ NormParams p) {
+  using G = Team<T>;
   __shared__ float2 shared[T / 32];
-  constexpr int kTeams = T == 32 ? 8 : 1;
+  extern __shared__ __align__(16) float params[];  // w by place: [K * T * 8]; with a row a warp behind it the sums [2][K * 256]
   const int lane = T == 32 ? threadIdx.x & 31 : threadIdx.x;
   const int place = blockIdx.x % p.period;  // rows place, place + period, ... are shared out among the blocks of this place
-  const int64_t team = (int64_t)(blockIdx.x / p.period) * kTeams + (T == 32 ? threadIdx.x >> 5 : 0);
-  const int64_t teams = (int64_t)(gridDim.x / p.period) * kTeams;
+  const int64_t team = (int64_t)(blockIdx.x / p.period) * G::kTeams + (T == 32 ? threadIdx.x >> 5 : 0);
+  const int64_t step = (int64_t)(gridDim.x / p.period) * G::kTeams * p.period, all = p.rows * p.width;
   const int shift = (int)(place * p.width & 7);
   const float inv = 1.0f / (float)p.width;
-  float w[K][8], dw[K][8], db[K][8];
+  int64_t row = place + team * p.period;
+  Raw<X> x[K], next_x[K];
+  Raw<Y> dy[K], next_dy[K];
+  float2 st = make_float2(0.0f, 0.0f), next_st = st;
+  float dw[K][8], db[K][8];
+  if (row < p.rows) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      take(x[k], static_cast<const X*>(p.x), row * p.width, (k * T + lane) * 8 - shift, p.width, all);
+      take(dy[k], static_cast<const Y*>(p.dy), row * p.width, (k * T + lane) * 8 - shift, p.width, all);
+    }
+    st = reinterpret_cast<const float2*>(p.stats)[row];
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t c = ((int64_t)k * T + lane) * 8 - shift + j;
-      w[k][j] = c < 0 || c >= p.width ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
-      dw[k][j] = db[k][j] = 0.0f;
-    }
-  for (int64_t row = place + team * p.period; row < p.rows; row += teams * p.period) {
-    const X* x = static_cast<const X*>(p.x) + row * p.width;
-    const Y* dy = static_cast<const Y*>(p.dy) + row * p.width;
-    const float2 st = reinterpret_cast<const float2*>(p.stats)[row];
-    float h[K][8], g[K][8];
+    for (int j = 0; j < 8; ++j) dw[k][j] = db[k][j] = 0.0f;
+  for (int i = threadIdx.x; i < K * T * 8; i += G::kThreads) {
+    const int64_t c = i - shift;
+    params[i] = c < 0 || c >= p.width ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
+  }
+  __syncthreads();
+  for (; row < p.rows; row += step) {
+    const bool more = row + step < p.rows;
+    if (G::kAhead && more) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t first = ((int64_t)k * T + lane) * 8 - shift;
-      load_group(x, first, p.width, h[k]);
-      load_group(dy, first, p.width, g[k]);
+      for (int k = 0; k < K; ++k) {
+        take(next_x[k], static_cast<const X*>(p.x), (row + step) * p.width, (k * T + lane) * 8 - shift, p.width, all);
+        take(next_dy[k], static_cast<const Y*>(p.dy), (row + step) * p.width, (k * T + lane) * 8 - shift, p.width, all);
+      }
+      next_st = reinterpret_cast<const float2*>(p.stats)[row + step];
     }
+    // outside the row dy and w are 0, and nothing that is not a number there reaches a sum of other columns
     float a = 0.0f, b = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+      float h[8], g[8], w[8];
+      x[k].values(h);
+      dy[k].values(g);
+      load8(params + (k * T + lane) * 8, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        // outside the row g and w are 0 and h is whatever: nothing reaches a sum
-        h[k][j] = (h[k][j] - st.x) * st.y;
-        dw[k][j] = fmaf(g[k][j], h[k][j], dw[k][j]);
-        db[k][j] += g[k][j];
-        g[k][j] *= w[k][j];
-        a += g[k][j];
-        b = fmaf(g[k][j], h[k][j], b);
+        h[j] = (h[j] - st.x) * st.y;
+        dw[k][j] = fmaf(g[j], h[j], dw[k][j]);
+        db[k][j] += g[j];
+        g[j] *= w[j];
+        a += g[j];
+        b = fmaf(g[j], h[j], b);
       }
+    }
     if (p.out) {
       group_sum2<T>(a, b, shared);
       a *= inv;
@@ -132,18 +240,40 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) hc_norm_backward_kernel(con
       X* dx = static_cast<X*>(p.out) + row * p.width;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int64_t first = ((int64_t)k * T + lane) * 8 - shift;
+        const int first = (k * T + lane) * 8 - shift;
+        if (first >= p.width) continue;
+        float h[8], g[8], w[8];
+        x[k].touch();
+        dy[k].touch();
+        x[k].values(h);
+        dy[k].values(g);
+        load8(params + (k * T + lane) * 8, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[k][j] = st.y * (fmaf(-h[k][j], b, g[k][j]) - a);
-        store_group(dx, first, p.width, g[k]);
+        for (int j = 0; j < 8; ++j) g[j] = st.y * (fmaf(-(h[j] - st.x) * st.y, b, g[j] * w[j]) - a);
+        store_group(dx, first, p.width, g);
       }
+    }
+    if (G::kAhead) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        x[k] = next_x[k];
+        dy[k] = next_dy[k];
+      }
+      st = next_st;
+    } else if (more) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        take(x[k], static_cast<const X*>(p.x), (row + step) * p.width, (k * T + lane) * 8 - shift, p.width, all);
+        take(dy[k], static_cast<const Y*>(p.dy), (row + step) * p.width, (k * T + lane) * 8 - shift, p.width, all);
+      }
+      st = reinterpret_cast<const float2*>(p.stats)[row + step];
     }
   }
   if (!p.partial) return;
   float* mine = p.partial + (int64_t)blockIdx.x * 2 * p.width;
   if (T == 32) {  // the block's warps one after the other: a fixed order
-    extern __shared__ float sums[];  // [2][K * 256]
-    for (int warp = 0; warp < 8; ++warp) {
+    float* sums = params + K * 256;
+    for (int warp = 0; warp < G::kTeams; ++warp) {
       if ((threadIdx.x >> 5) == warp) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -156,7 +286,7 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) hc_norm_backward_kernel(con
       }
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < K * 256; i += 256) {
+    for (int i = threadIdx.x; i < K * 256; i += G::kThreads) {
       const int64_t c = ((int64_t)(i / 256) * 32 + (i & 31)) * 8 - shift + (i / 32) % 8;
       if (c < 0 || c >= p.width) continue;
       mine[c] = sums[i];
@@ -297,79 +427,91 @@ __global__ void __launch_bounds__(1024) hc_norm_finish_kernel(const float* parti
 namespace {
 
 constexpr int64_t kLongestInRegisters = 8192;
-constexpr int kBlocksPerSm = 4;
 
-// threads and groups of eight a thread for rows of `width` values (with one group more where rows begin anywhere)
+// Threads and groups of eight a thread for rows of `width` values (with one group more where rows begin anywhere): a warp while
+// three groups a thread do, then two groups a thread, which leaves room in the registers for the row ahead.
 struct Shape {
   int threads, groups;
 };
 Shape shape_of(size_t width) {
   const int need = (int)((width + 7) / 8) + (width % 8 ? 1 : 0);
-  if (need <= 128) return {32, (need + 31) / 32};
-  if (need <= 256) return {128, 2};
-  if (need <= 512) return {128, 4};
-  return {256, 4};
+  if (need <= 96) return {32, (need + 31) / 32};
+  return {need <= 256 ? 128 : need <= 384 ? 192 : need <= 512 ? 256 : need <= 768 ? 384 : 512, 2};
 }
 int period_of(size_t width) { return width % 8 == 0 ? 1 : width % 4 == 0 ? 2 : width % 2 == 0 ? 4 : 8; }
 bool in_registers(size_t width) { return width <= kLongestInRegisters - (width % 8 ? 8 : 0); }
 
-int backward_blocks(size_t rows, size_t width) {
+// Blocks: those that the SMs hold stay for all rows, a whole number of them for each place of an aligned group
+int norm_blocks(size_t rows, size_t width) {
   const int sms = device_info().sms > 0 ? device_info().sms : 1;
-  const int period = period_of(width);
   if (!in_registers(width)) return (int)(rows < 64 ? rows : 64);
-  const size_t teams = shape_of(width).threads == 32 ? 8 : 1;
-  size_t blocks = (rows + teams - 1) / teams;
-  const size_t most = (size_t)sms * (shape_of(width).threads == 256 ? 2 : shape_of(width).threads == 128 ? 4 : 2);
-  if (blocks > most) blocks = most;
-  return (int)((blocks + period - 1) / period * period);
+  const int period = period_of(width);
+  const Shape s = shape_of(width);
+  const size_t teams = s.threads == 32 ? 4 : 1, most = (size_t)sms * (s.threads == 32 ? 3 : 512 / s.threads) / period * period;
+  const size_t blocks = (rows + teams * period - 1) / (teams * period) * period;
+  return (int)(blocks < most ? blocks : most);
 }
 
 template <typename X, typename Y, int T, int K>
 cudaError_t run_forward(const dev::NormParams& p, cudaStream_t stream) {
-  const int64_t teams = T == 32 ? 8 : 1;
-  int64_t blocks = (p.rows + teams - 1) / teams;
-  if (blocks > 0x7fffffff) blocks = 0x7fffffff;
-  dev::hc_norm_kernel<X, Y, T, K><<<(unsigned)blocks, T == 32 ? 256 : T, 0, stream>>>(p);
+  constexpr int smem = 2 * K * T * 8 * 4;
+  if (smem > 40 * 1024) {  // with what the kernel has besides, 48 KB need no permission
+    const cudaError_t e = set_smem(dev::hc_norm_kernel<X, Y, T, K>, smem);
+    if (e != cudaSuccess) return e;
+  }
+  dev::hc_norm_kernel<X, Y, T, K><<<norm_blocks(p.rows, p.width), dev::Team<T>::kThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 template <typename X, typename Y, int T, int K>
 cudaError_t run_backward(const dev::NormParams& p, int blocks, cudaStream_t stream) {
-  dev::hc_norm_backward_kernel<X, Y, T, K><<<blocks, T == 32 ? 256 : T, T == 32 ? K * 2048 : 0, stream>>>(p);
+  constexpr int smem = K * T * 8 * 4 + (T == 32 ? K * 2048 : 0);
+  static_assert(smem <= 40 * 1024, "more needs the kernel's permission");
+  dev::hc_norm_backward_kernel<X, Y, T, K><<<blocks, dev::Team<T>::kThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
+// f with the threads and groups as constants
+template <typename F>
+cudaError_t by_shape(size_t width, F f) {
+  const Shape s = shape_of(width);
+  if (s.threads == 32) return s.groups == 1 ? f.template run<32, 1>() : s.groups == 2 ? f.template run<32, 2>() : f.template run<32, 3>();
+  if (s.threads == 128) return f.template run<128, 2>();
+  if (s.threads == 192) return f.template run<192, 2>();
+  if (s.threads == 256) return f.template run<256, 2>();
+  return s.threads == 384 ? f.template run<384, 2>() : f.template run<512, 2>();
+}
+template <typename X, typename Y>
+struct Forward {
+  const dev::NormParams& p;
+  cudaStream_t stream;
+  template <int T, int K>
+  cudaError_t run() {
+    return run_forward<X, Y, T, K>(p, stream);
+  }
+};
+template <typename X, typename Y>
+struct Backward {
+  const dev::NormParams& p;
+  int blocks;
+  cudaStream_t stream;
+  template <int T, int K>
+  cudaError_t run() {
+    return run_backward<X, Y, T, K>(p, blocks, stream);
+  }
+};
+
 template <typename X, typename Y>
 cudaError_t forward(const dev::NormParams& p, cudaStream_t stream) {
-  if (!in_registers(p.width)) {
-    dev::hc_norm_long_kernel<X, Y><<<(unsigned)(p.rows < 65536 ? p.rows : 65536), dev::kLong, 0, stream>>>(p);
-    return cudaGetLastError();
-  }
-  const Shape s = shape_of(p.width);
-  if (s.threads == 32) {
-    if (s.groups == 1) return run_forward<X, Y, 32, 1>(p, stream);
-    if (s.groups == 2) return run_forward<X, Y, 32, 2>(p, stream);
-    if (s.groups == 3) return run_forward<X, Y, 32, 3>(p, stream);
-    return run_forward<X, Y, 32, 4>(p, stream);
-  }
-  if (s.threads == 128) return s.groups == 2 ? run_forward<X, Y, 128, 2>(p, stream) : run_forward<X, Y, 128, 4>(p, stream);
-  return run_forward<X, Y, 256, 4>(p, stream);
+  if (in_registers(p.width)) return by_shape(p.width, Forward<X, Y>{p, stream});
+  dev::hc_norm_long_kernel<X, Y><<<(unsigned)(p.rows < 65536 ? p.rows : 65536), dev::kLong, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 template <typename X, typename Y>
 cudaError_t backward(const dev::NormParams& p, int blocks, cudaStream_t stream) {
-  if (!in_registers(p.width)) {
-    if (p.out) dev::hc_norm_long_dx_kernel<X, Y><<<(unsigned)(p.rows < 65536 ? p.rows : 65536), dev::kLong, 0, stream>>>(p);
-    if (p.partial) dev::hc_norm_long_sums_kernel<X, Y><<<dim3((unsigned)((p.width + 255) / 256), blocks), 256, 0, stream>>>(p);
-    return cudaGetLastError();
-  }
-  const Shape s = shape_of(p.width);
-  if (s.threads == 32) {
-    if (s.groups == 1) return run_backward<X, Y, 32, 1>(p, blocks, stream);
-    if (s.groups == 2) return run_backward<X, Y, 32, 2>(p, blocks, stream);
-    if (s.groups == 3) return run_backward<X, Y, 32, 3>(p, blocks, stream);
-    return run_backward<X, Y, 32, 4>(p, blocks, stream);
-  }
-  if (s.threads == 128) return s.groups == 2 ? run_backward<X, Y, 128, 2>(p, blocks, stream) : run_backward<X, Y, 128, 4>(p, blocks, stream);
-  return run_backward<X, Y, 256, 4>(p, blocks, stream);
+  if (in_registers(p.width)) return by_shape(p.width, Backward<X, Y>{p, blocks, stream});
+  if (p.out) dev::hc_norm_long_dx_kernel<X, Y><<<(unsigned)(p.rows < 65536 ? p.rows : 65536), dev::kLong, 0, stream>>>(p);
+  if (p.partial) dev::hc_norm_long_sums_kernel<X, Y><<<dim3((unsigned)((p.width + 255) / 256), blocks), 256, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 template <typename F>
@@ -398,13 +540,13 @@ int hc_layer_norm(const void* x, int x_type, const void* weight, const void* bia
   if (!hc::norm_arguments_ok(x, x_type, y, y_type, param_type, rows, width) || !(eps >= 0.0f)) return hc::kErrArgument;
   if (rows == 0) return hc::kOk;
   if (!x || !y) return hc::kErrArgument;
-  hc::dev::NormParams p = {x, nullptr, weight, bias, y, stats, nullptr, (int64_t)rows, (int64_t)width, eps, param_type, 1};
+  hc::dev::NormParams p = {x, nullptr, weight, bias, y, stats, nullptr, (int64_t)rows, (int64_t)width, eps, param_type, hc::period_of(width)};
   const cudaError_t e = hc::by_types(x_type, y_type, [&](auto a, auto b) { return hc::forward<decltype(a), decltype(b)>(p, stream); });
   return e == cudaSuccess ? hc::kOk : hc::kErrCuda;
 }
 
 size_t hc_layer_norm_backward_bytes(size_t rows, size_t width) {
-  return rows && width ? (size_t)hc::backward_blocks(rows, width) * 2 * width * sizeof(float) : 0;
+  return rows && width ? (size_t)hc::norm_blocks(rows, width) * 2 * width * sizeof(float) : 0;
 }
 
 int hc_layer_norm_backward(const void* dy, int y_type, const void* x, int x_type, const void* weight, int param_type,
@@ -420,7 +562,7 @@ int hc_layer_norm_backward(const void* dy, int y_type, const void* x, int x_type
   }
   if (!x || !dy || !stats) return hc::kErrArgument;
   if (!dx && !dweight) return hc::kOk;
-  const int blocks = hc::backward_blocks(rows, width);
+  const int blocks = hc::norm_blocks(rows, width);
   if (dweight && (!scratch || scratch_bytes < hc_layer_norm_backward_bytes(rows, width))) return hc::kErrArgument;
   hc::dev::NormParams p = {x, dy, weight, nullptr, dx, const_cast<float*>(stats), dweight ? static_cast<float*>(scratch) : nullptr,
                            (int64_t)rows, (int64_t)width, 0.0f, param_type, hc::period_of(width)};
