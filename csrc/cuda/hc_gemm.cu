@@ -764,5 +764,6 @@ extern "C" int hc_train_status(int clear) {
     const unsigned int zero = 0;
     if (cudaMemcpyToSymbol(hc::dev::g_train_status, &zero, sizeof(zero)) != cudaSuccess) return hc::kErrCuda;
   }
-  return (int)status;
+  const int norm = hc::norm_status(clear);
+  return status ? (int)status : norm;
 }

@@ -10,6 +10,7 @@ namespace hc {
 
 enum ElementType : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 inline size_t element_bytes(int type) { return type == kF32 ? 4 : 2; }
+int norm_status(int clear);  // of the layer norm's kernels (hc_norm.cu)
 inline bool element_type_ok(int type) { return type >= kF32 && type <= kF16; }
 
 namespace dev {
@@ -146,5 +147,35 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float2* shared) {
   }
 }
 
+// Two values at a time: one instruction for both
+struct Pair {
+  uint64_t w;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.w) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void parts(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.w)); }
+__device__ __forceinline__ float both(Pair p) {
+  float a, b;
+  parts(p, a, b);
+  return a + b;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+  return r;
+}
 }  // namespace dev
 }  // namespace hc

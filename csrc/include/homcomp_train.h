@@ -78,7 +78,7 @@ size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
 int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
                      int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 
-// The products' waits are bounded (2 s).  Synchronises the device and returns 3 if one of them ran out since the status
+// Waits of the products' and the norm's kernels are bounded (2 s).  Synchronises the device and returns 3 if one of them ran out since the status
 // was last cleared, 0 if not.
 int hc_train_status(int clear);
 
