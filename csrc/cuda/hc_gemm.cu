@@ -758,12 +758,6 @@ cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
 }  // namespace hc
 
 extern "C" int hc_train_status(int clear) {
-  unsigned int status = 0;
-  if (cudaMemcpyFromSymbol(&status, hc::dev::g_train_status, sizeof(status)) != cudaSuccess) return hc::kErrCuda;
-  if (clear && status) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbol(hc::dev::g_train_status, &zero, sizeof(zero)) != cudaSuccess) return hc::kErrCuda;
-  }
-  const int norm = hc::norm_status(clear);
-  return status ? (int)status : norm;
+  const int all[3] = {hc::take_status(hc::dev::g_train_status, clear), hc::norm_status(clear), hc::logprob_status(clear)};
+  return all[0] ? all[0] : all[1] ? all[1] : all[2];
 }

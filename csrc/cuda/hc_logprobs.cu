@@ -26,8 +26,8 @@
 namespace hc {
 namespace dev {
 
-constexpr int kRowThreads = 512;
-constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowThreads = 512;     // of a block that has a row, or a part of one
+constexpr int kStreamThreads = 128;  // of a block that has one row after the other
 constexpr int kMostTop = 64;
 constexpr int kCandidates = 2048;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -215,23 +215,23 @@ __device__ __forceinline__ Pair exp2_pair(Pair v) {
   return pair(exp2_fast(a), exp2_fast(b));
 }
 
-// The groups g, g + kRowThreads, ... of a row; what is not the row's, or from `end` on, is -inf.
-template <typename T>
+// The groups g, g + kThreads, ... of a row; what is not the row's, or from `end` on, is -inf.
+template <int kThreads, typename T>
 __device__ __forceinline__ void load_some(Logits<T> (&q)[kAtOnce], const T* row, int64_t g, int64_t end, int shift, int64_t vocab) {
-  const int64_t last = g + (kAtOnce - 1) * kRowThreads;
+  const int64_t last = g + (kAtOnce - 1) * kThreads;
   if (g * 8 >= shift && last < end && (last + 1) * 8 - shift <= vocab) {
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) q[i].load(row + (g + i * kRowThreads) * 8 - shift);
+    for (int i = 0; i < kAtOnce; ++i) q[i].load(row + (g + i * kThreads) * 8 - shift);
   } else {
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int64_t first = (g + i * kRowThreads) * 8 - shift;
+      const int64_t first = (g + i * kThreads) * 8 - shift;
       float v[8];
-      if (g + i * kRowThreads < end && first >= 0 && first + 8 <= vocab) {
+      if (g + i * kThreads < end && first >= 0 && first + 8 <= vocab) {
         q[i].load(row + first);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = g + i * kRowThreads < end && first + j >= 0 && first + j < vocab ? to_float(row[first + j]) : -INFINITY;
+        for (int j = 0; j < 8; ++j) v[j] = g + i * kThreads < end && first + j >= 0 && first + j < vocab ? to_float(row[first + j]) : -INFINITY;
         q[i].set(v);
       }
     }
@@ -240,34 +240,40 @@ __device__ __forceinline__ void load_some(Logits<T> (&q)[kAtOnce], const T* row,
 
 struct TopShared {
   uint64_t list[kCandidates];
-  uint64_t warp_key[kRowWarps];
+  uint64_t warp_key[kRowThreads / 32];
   uint64_t bound;
   uint64_t best[kMostTop];  // of this block, largest first; 0 where there are fewer
-  uint64_t last[kRowWarps];
+  uint64_t last[kRowThreads / 32];
   int count;
 };
 
-// the `top` largest keys of the groups that this block has, into sh.best
-template <typename T>
-__device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, int shift, int64_t begin, int64_t end, float mine,
+// The `top` largest keys of the groups of a row that this block has, into sh.best.  A thread has the groups begin + its number,
+// and every kThreads-th from there, and thread 0 also group 0 where `begin` is 1.  `mine`: its largest logit; `where`: the
+// first group of those among which that stood (the next ones of the thread, up to kAtOnce), -1 for a thread without groups.
+template <int kThreads, typename T>
+__device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, int shift, int64_t begin, int64_t end, bool first_too, float mine,
                           int64_t where) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t groups = end - begin;
-  // this thread's largest key: in the groups among which its maximum stood first
-  uint64_t key = 0;
-  for (int i = 0; i < kAtOnce && where >= 0; ++i) {
-    const int64_t g = where + i * kRowThreads;
-    if (g >= end) break;
-    float v[8];
-    load_group(row, g * 8 - shift, p.vocab, v);
+  const auto each_key = [&](int64_t from, int64_t to, auto f) {
+    for (int64_t g = from; g < to; g += kThreads) {
+      float v[8];
+      load_group(row, g * 8 - shift, p.vocab, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t c = g * 8 - shift + j;
-      if (c >= 0 && c < p.vocab) key = max64(key, key_of(v[j], c));
+      for (int j = 0; j < 8; ++j) {
+        const int64_t c = g * 8 - shift + j;
+        if (c >= 0 && c < p.vocab) f(key_of(v[j], c));
+      }
     }
-  }
+  };
+  const auto every_key = [&](auto f) {
+    if (first_too && threadIdx.x == 0) each_key(0, 1, f);
+    each_key(begin + threadIdx.x, end, f);
+  };
+  uint64_t key = 0;  // this thread's largest
+  if (where >= 0) each_key(where, where < begin ? where + 1 : min(end, where + kAtOnce * kThreads), [&](uint64_t one) { key = max64(key, one); });
   // every warp's r-th largest; the (top / r)-th largest of those is reached by at least `top` keys
-  const int warps = (int)(groups < kRowThreads ? (groups + 31) / 32 : kRowWarps);
+  const int warps = (int)max((int64_t)1, groups < kThreads ? (groups + 31) / 32 : (kThreads / 32));
   const int r = (p.top + warps - 1) / warps;
   uint64_t k = key, best = 0;
   for (int i = 0; i < r && i < 32; ++i) {
@@ -280,7 +286,7 @@ __device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, i
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
   if (warp == 0) {
-    k = lane < kRowWarps ? sh.warp_key[lane] : 0;
+    k = lane < (kThreads / 32) ? sh.warp_key[lane] : 0;
     for (int i = 0; i < (p.top + r - 1) / r; ++i) {
       best = warp_max64(k);
       if (k == best) k = 0;
@@ -290,24 +296,16 @@ __device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, i
   __syncthreads();
   const uint64_t bound = sh.bound;
   if (where >= 0 && ordered(mine) >= (uint32_t)(bound >> 32)) {
-    for (int64_t g = begin + threadIdx.x; g < end; g += kRowThreads) {
-      float v[8];
-      load_group(row, g * 8 - shift, p.vocab, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t c = g * 8 - shift + j;
-        const uint64_t one = key_of(v[j], c);
-        if (c >= 0 && c < p.vocab && one >= bound) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCandidates) sh.list[at] = one;
-        }
-      }
-    }
+    every_key([&](uint64_t one) {
+      if (one < bound) return;
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCandidates) sh.list[at] = one;
+    });
   }
   __syncthreads();
   const int n = sh.count;
   if (n <= kCandidates) {
-    for (int i = threadIdx.x; i < n; i += kRowThreads) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
       const uint64_t one = sh.list[i];
       int above = 0;
       for (int j = 0; j < n; ++j) above += sh.list[j] > one;
@@ -318,21 +316,14 @@ __device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, i
     uint64_t below = ~0ull;
     for (int i = 0; i < p.top; ++i) {
       uint64_t found = 0;
-      for (int64_t g = begin + threadIdx.x; g < end; g += kRowThreads) {
-        float v[8];
-        load_group(row, g * 8 - shift, p.vocab, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int64_t c = g * 8 - shift + j;
-          const uint64_t one = key_of(v[j], c);
-          if (c >= 0 && c < p.vocab && one < below) found = max64(found, one);
-        }
-      }
+      every_key([&](uint64_t one) {
+        if (one < below) found = max64(found, one);
+      });
       found = warp_max64(found);
       if (lane == 0) sh.last[warp] = found;
       __syncthreads();
       found = 0;
-      for (int w = 0; w < kRowWarps; ++w) found = max64(found, sh.last[w]);
+      for (int w = 0; w < (kThreads / 32); ++w) found = max64(found, sh.last[w]);
       __syncthreads();
       if (threadIdx.x == 0) sh.best[i] = found;
       below = found;
@@ -341,132 +332,292 @@ __device__ void block_top(const LogprobParams& p, TopShared& sh, const T* row, i
   __syncthreads();
 }
 
-// One row a block, or a cluster of p.cluster blocks for each row.
+// a row whose token is left out
+template <bool kTop>
+__device__ __forceinline__ void leave_out(const LogprobParams& p, int64_t r) {
+  if (threadIdx.x == 0) {
+    p.logprobs[r] = 0.0f;
+    p.entropy[r] = 0.0f;
+    if (p.stats) p.stats[r * 3] = p.stats[r * 3 + 1] = p.stats[r * 3 + 2] = 0.0f;
+  }
+  if (kTop && threadIdx.x < p.top) {
+    p.top_tokens[r * p.top + threadIdx.x] = -1;
+    p.top_logprobs[r * p.top + threadIdx.x] = 0.0f;
+  }
+}
+// a row whose sums are there
+template <typename T, bool kTop>
+__device__ __forceinline__ void store_row(const LogprobParams& p, int64_t r, int64_t token, const T* row, const Softmax& all, const uint64_t* best) {
+  const bool sound = all.s > 0.0f && all.s < INFINITY;  // no NaN, no +inf, something above -inf
+  const float log_s = logf(all.s);
+  if (threadIdx.x == 0) {
+    const float h = sound ? log_s - all.t / all.s : NAN;
+    p.logprobs[r] = sound && token >= 0 && token < p.vocab ? to_float(row[token]) - all.m - log_s : NAN;
+    p.entropy[r] = h;
+    if (p.stats) {
+      p.stats[r * 3] = sound ? all.m : NAN;
+      p.stats[r * 3 + 1] = log_s;
+      p.stats[r * 3 + 2] = h;
+    }
+  }
+  if (kTop && threadIdx.x < p.top) {
+    const int64_t i = 0xffffffffu - (uint32_t)best[threadIdx.x];
+    p.top_tokens[r * p.top + threadIdx.x] = sound ? i : -1;
+    p.top_logprobs[r * p.top + threadIdx.x] = sound ? to_float(row[i]) - all.m - log_s : NAN;
+  }
+}
+
+// A thread's sums so far, relative to m, which is near its maximum but not more than kSlack below it: it follows only then, for
+// in some thread of a warp the maximum grows nearly every time.  The maximum itself is `best`.
+constexpr float kSlack = 8.0f;
+template <typename T>
+struct Running {
+  float m, best;
+  Pair s, t;
+  uint32_t lowest;
+  __device__ __forceinline__ void clear() {
+    m = best = kLowest;
+    s = t = pair(0.0f, 0.0f);
+    lowest = 0;
+  }
+  // N more groups; whether the maximum has grown
+  template <int N>
+  __device__ __forceinline__ bool add(const Logits<T> (&q)[N]) {
+    const float top = Logits<T>::largest(q);
+    const bool more = top > best;
+    best = fmaxf(best, top);
+    if (top > m + kSlack || m == kLowest) {
+      const float d = fmaxf(m - best, kNothing), f = exp2_fast(d * kLog2e);
+      const Pair d2 = pair(d, d), f2 = pair(f, f);
+      t = fma2(s, d2, t) * f2;
+      s = s * f2;
+      m = best;
+      lowest = lowest_of<T>(best);
+    }
+    const Pair log2e = pair(kLog2e, kLog2e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      Pair d[4];
+      differences(q[i], m, lowest, d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const Pair e = exp2_pair(d[k] * log2e);
+        s = s + e;
+        t = fma2(e, d[k], t);
+      }
+    }
+    return more;
+  }
+  __device__ __forceinline__ Softmax sums() const { return join({m, both(s), both(t)}, {best, 0.0f, 0.0f}); }
+};
+
+// joins the threads' sums; in warp 0 every thread gets those of the block
+template <int kThreads>
+__device__ __forceinline__ Softmax block_join(Softmax a, Softmax* warp_part) {
+  a = warp_join(a);
+  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = a;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    a = threadIdx.x < kThreads / 32 ? warp_part[threadIdx.x] : Softmax{kLowest, 0.0f, 0.0f};
+    a = warp_join(a);
+  }
+  return a;
+}
+
+// Few rows: a cluster of p.cluster blocks for each, or one block.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kRowThreads) hc_logprob_kernel(const __grid_constant__ LogprobParams p) {
-  __shared__ Softmax warp_part[kRowWarps];
+  __shared__ Softmax warp_part[kRowThreads / 32];
   __shared__ Softmax block_part;
   extern __shared__ __align__(16) unsigned char dynamic[];
   TopShared& sh = *reinterpret_cast<TopShared*>(dynamic);  // only there with kTop
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = blockIdx.x % p.cluster;
-  for (int64_t r = blockIdx.x / p.cluster; r < p.rows; r += gridDim.x / p.cluster) {
-    const int64_t token = p.tokens[r];
-    if (token == p.ignore) {  // the same for all threads of the cluster
-      if (part == 0) {
-        if (threadIdx.x == 0) {
-          p.logprobs[r] = 0.0f;
-          p.entropy[r] = 0.0f;
-          if (p.stats) p.stats[r * 3] = p.stats[r * 3 + 1] = p.stats[r * 3 + 2] = 0.0f;
-        }
-        if (kTop && threadIdx.x < p.top) {
-          p.top_tokens[r * p.top + threadIdx.x] = -1;
-          p.top_logprobs[r * p.top + threadIdx.x] = 0.0f;
+  const int64_t r = blockIdx.x / p.cluster;
+  const int64_t token = p.tokens[r];
+  if (token == p.ignore) {  // the same for all threads of the cluster
+    if (part == 0) leave_out<kTop>(p, r);
+    return;
+  }
+  const T* row = static_cast<const T*>(p.x) + r * p.stride;
+  const int shift = place_of(row);
+  const int64_t groups = (p.vocab + shift + 7) / 8;
+  const int64_t begin = groups * part / p.cluster, end = groups * (part + 1) / p.cluster;
+  Running<T> run;
+  run.clear();
+  int64_t where = begin + threadIdx.x < end ? begin + threadIdx.x : -1;
+  for (int64_t g = begin + threadIdx.x; g < end; g += kAtOnce * kRowThreads) {
+    Logits<T> q[kAtOnce];
+    load_some<kRowThreads>(q, row, g, end, shift, p.vocab);
+    if (run.add(q) && kTop) where = g;
+  }
+  Softmax a = block_join<kRowThreads>(run.sums(), warp_part);
+  if (warp == 0 && lane == 0) block_part = a;
+  if (kTop) block_top<kRowThreads>(p, sh, row, shift, begin, end, false, run.best, where);
+  if (p.cluster > 1) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (part == 0) {
+      if (warp == 0) {
+        Softmax b = {kLowest, 0.0f, 0.0f};
+        if (lane < p.cluster) b = *cluster.map_shared_rank(&block_part, lane);
+        a = warp_join(b);
+      }
+      if (kTop) {
+        // the blocks' own largest, ranked together
+        const int n = p.cluster * p.top;
+        for (int i = threadIdx.x; i < n; i += kRowThreads) sh.list[i] = cluster.map_shared_rank(&sh, i / p.top)->best[i % p.top];
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kRowThreads) {
+          const uint64_t one = sh.list[i];
+          int above = 0;
+          for (int j = 0; j < n; ++j) above += sh.list[j] > one;
+          if (one && above < p.top) sh.best[above] = one;
         }
       }
+      if (warp == 0 && lane == 0) block_part = a;
+    }
+    cluster.sync();  // nobody leaves before its part has been read
+  } else {
+    __syncthreads();
+  }
+  if (part == 0) store_row<T, kTop>(p, r, token, row, block_part, sh.best);
+}
+
+// Many rows: a block stays and has one row after the other brought into a ring in shared memory, in pieces of 32 logits a thread
+// by bulk copies that do not wait for the end of a row.  What a row costs besides its logits, some 300 instructions a thread, is
+// kept small by few threads, and the SM filled by eight blocks (8192 x 50257 logits of bf16: 267 us with a block of 512 threads for
+// each row, 280 with two such blocks an SM and rings).
+template <typename T>
+constexpr int kPieceBytes = kAtOnce * 8 * (int)sizeof(T) * kStreamThreads;
+constexpr int kRing = 3;
+__device__ unsigned int g_logprob_status;
+
+template <typename T>
+struct Stream {  // what one thread knows to ask for the pieces
+  int64_t row, token;
+  int piece, pieces;
+  const T* from;
+  int64_t groups;  // whole ones that begin at `from`
+};
+template <typename T>
+__device__ __forceinline__ void whole_groups(const T* row, int64_t vocab, const T*& from, int64_t& groups) {
+  const int shift = place_of(row), skipped = shift ? 8 - shift : 0;
+  from = row + skipped;
+  groups = (vocab - skipped) / 8;
+}
+
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kStreamThreads, 8) hc_logprob_stream_kernel(const __grid_constant__ LogprobParams p) {
+  constexpr int kGroups = kAtOnce * kStreamThreads;
+  __shared__ Softmax warp_part[(kStreamThreads / 32)];
+  __shared__ Softmax block_part;
+  __shared__ uint64_t full[kRing], empty[kRing];
+  extern __shared__ __align__(128) unsigned char dynamic[];
+  TopShared& sh = *reinterpret_cast<TopShared*>(dynamic + kRing * kPieceBytes<T>);  // only there with kTop
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], (kStreamThreads / 32));
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  // Thread 0 asks for the pieces, kRing - 1 ahead of the one that is worked on.
+  Stream<T> ask;
+  ask.row = blockIdx.x;
+  ask.piece = ask.pieces = 0;
+  uint32_t asked = 0;
+  bool gave_up = false;
+  const auto ask_one = [&] {
+    while (ask.piece == ask.pieces) {  // the next row that is read
+      if (ask.pieces) ask.row += gridDim.x;
+      while (ask.row < p.rows && p.tokens[ask.row] == p.ignore) ask.row += gridDim.x;
+      if (ask.row >= p.rows) return;
+      whole_groups(static_cast<const T*>(p.x) + ask.row * p.stride, p.vocab, ask.from, ask.groups);
+      ask.pieces = (int)((ask.groups + kGroups - 1) / kGroups);
+      ask.piece = 0;
+    }
+    const int stage = asked % kRing;
+    if (asked >= kRing && !mbar_wait_bounded(&empty[stage], (asked / kRing - 1) & 1, 2000ull * 1000 * 1000)) gave_up = true;
+    const int64_t first = (int64_t)ask.piece * kGroups;
+    const uint32_t bytes = (uint32_t)min((int64_t)kGroups, ask.groups - first) * 8 * sizeof(T);
+    mbar_expect_tx(&full[stage], bytes);
+    bulk_load(dynamic + stage * kPieceBytes<T>, ask.from + first * 8, bytes, &full[stage]);
+    ++ask.piece;
+    ++asked;
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < kRing - 1; ++i) ask_one();
+  uint32_t used = 0;
+  int64_t token = blockIdx.x < p.rows ? p.tokens[blockIdx.x] : 0;
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const int64_t next_token = r + gridDim.x < p.rows ? p.tokens[r + gridDim.x] : 0;
+    if (token == p.ignore) {
+      leave_out<kTop>(p, r);
+      token = next_token;
       continue;
     }
     const T* row = static_cast<const T*>(p.x) + r * p.stride;
     const int shift = place_of(row);
-    const int64_t groups = (p.vocab + shift + 7) / 8;
-    const int64_t begin = groups * part / p.cluster, end = groups * (part + 1) / p.cluster;
-    Softmax a = {kLowest, 0.0f, 0.0f};
-    int64_t where = begin + threadIdx.x < end ? begin + threadIdx.x : -1;
-    Pair s2 = pair(0.0f, 0.0f), t2 = s2;
-    const Pair log2e = pair(kLog2e, kLog2e);
-    uint32_t lowest = lowest_of<T>(a.m);
-    for (int64_t g = begin + threadIdx.x; g < end; g += kAtOnce * kRowThreads) {
+    const T* from;
+    int64_t groups;
+    whole_groups(row, p.vocab, from, groups);
+    const int64_t all = (p.vocab + shift + 7) / 8;
+    const int skipped = shift ? 1 : 0;  // the groups that come through the ring are skipped, skipped + 1, ...
+    Running<T> run;
+    run.clear();
+    int64_t where = skipped + threadIdx.x < all ? skipped + threadIdx.x : -1;
+    // what lies before the first whole group, and behind the last one
+    for (int edge = 0; edge < 2; ++edge) {
+      const int64_t g = edge ? all - 1 : 0;
+      if (edge ? skipped + groups == all || threadIdx.x != (all - 1 - skipped) % kStreamThreads : !skipped || threadIdx.x) continue;
+      float v[8];
+      Logits<T> q[1];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = g * 8 + j >= shift && g * 8 + j - shift < p.vocab ? to_float(row[g * 8 + j - shift]) : -INFINITY;
+      q[0].set(v);
+      if (run.add(q) && kTop) where = g;
+    }
+    for (int64_t g0 = 0; g0 < groups; g0 += kGroups, ++used) {
+      if (threadIdx.x == 0) ask_one();
+      const int stage = used % kRing;
+      // after a wait that ran out the others are short (a copy may still be on its way); the status says that sums are wrong
+      if (!mbar_wait_bounded(&full[stage], (used / kRing) & 1, gave_up ? 1000ull * 1000 : 2000ull * 1000 * 1000)) gave_up = true;
+      const T* piece = reinterpret_cast<const T*>(dynamic + stage * kPieceBytes<T>);
       Logits<T> q[kAtOnce];
-      load_some(q, row, g, end, shift, p.vocab);
-      const float top = Logits<T>::largest(q);
-      if (top > a.m) {
-        const float d = fmaxf(a.m - top, kNothing), f = exp2_fast(d * kLog2e);
-        const Pair d2 = pair(d, d), f2 = pair(f, f);
-        t2 = fma2(s2, d2, t2) * f2;
-        s2 = s2 * f2;
-        a.m = top;
-        lowest = lowest_of<T>(top);
-        if (kTop) where = g;
-      }
+      const int64_t g = g0 + threadIdx.x;
+      if (g0 + kGroups <= groups) {
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        Pair d[4];
-        differences(q[i], a.m, lowest, d);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const Pair e = exp2_pair(d[k] * log2e);
-          s2 = s2 + e;
-          t2 = fma2(e, d[k], t2);
+        for (int i = 0; i < kAtOnce; ++i) q[i].load(piece + (threadIdx.x + i * kStreamThreads) * 8);
+        if (run.add(q) && kTop) where = skipped + g;
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kAtOnce; ++i) {
+          if (g + i * kStreamThreads >= groups) break;
+          Logits<T> one[1];
+          one[0].load(piece + (threadIdx.x + i * kStreamThreads) * 8);
+          if (run.add(one) && kTop) where = skipped + g + i * kStreamThreads;
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
     }
-    a.s = both(s2);
-    a.t = both(t2);
-    const float mine = a.m;
-    a = warp_join(a);
-    if (lane == 0) warp_part[warp] = a;
+    if (__any_sync(0xffffffffu, gave_up) && lane == 0) atomicMax(&g_logprob_status, 3u);
+    const Softmax a = block_join<kStreamThreads>(run.sums(), warp_part);
+    if (threadIdx.x == 0) block_part = a;
+    if (kTop) block_top<kStreamThreads>(p, sh, row, shift, skipped, all, skipped, run.best, where);
     __syncthreads();
-    if (warp == 0) {
-      a = lane < kRowWarps ? warp_part[lane] : Softmax{kLowest, 0.0f, 0.0f};
-      a = warp_join(a);
-      if (lane == 0) block_part = a;
-    }
-    if (kTop) block_top<T>(p, sh, row, shift, begin, end, mine, where);
-    if (p.cluster > 1) {
-      namespace cg = cooperative_groups;
-      cg::cluster_group cluster = cg::this_cluster();
-      cluster.sync();
-      if (part == 0) {
-        if (warp == 0) {
-          Softmax b = {kLowest, 0.0f, 0.0f};
-          if (lane < p.cluster) b = *cluster.map_shared_rank(&block_part, lane);
-          a = warp_join(b);
-        }
-        if (kTop) {
-          // the blocks' own largest, ranked together
-          const int n = p.cluster * p.top;
-          for (int i = threadIdx.x; i < n; i += kRowThreads) sh.list[i] = cluster.map_shared_rank(&sh, i / p.top)->best[i % p.top];
-          __syncthreads();
-          for (int i = threadIdx.x; i < n; i += kRowThreads) {
-            const uint64_t one = sh.list[i];
-            int above = 0;
-            for (int j = 0; j < n; ++j) above += sh.list[j] > one;
-            if (one && above < p.top) sh.best[above] = one;
-          }
-        }
-        if (warp == 0 && lane == 0) block_part = a;
-      }
-      cluster.sync();  // nobody leaves, or begins another row, before its part has been read
-    } else {
-      __syncthreads();
-    }
-    if (part == 0) {
-      const Softmax all = block_part;
-      const bool sound = all.s > 0.0f && all.s < INFINITY;  // no NaN, no +inf, something above -inf
-      const float log_s = logf(all.s);
-      if (threadIdx.x == 0) {
-        const float h = sound ? log_s - all.t / all.s : NAN;
-        p.logprobs[r] = sound && token >= 0 && token < p.vocab ? to_float(row[token]) - all.m - log_s : NAN;
-        p.entropy[r] = h;
-        if (p.stats) {
-          p.stats[r * 3] = sound ? all.m : NAN;
-          p.stats[r * 3 + 1] = log_s;
-          p.stats[r * 3 + 2] = h;
-        }
-      }
-      if (kTop && threadIdx.x < p.top) {
-        const uint64_t k = sh.best[threadIdx.x];
-        const int64_t i = 0xffffffffu - (uint32_t)k;
-        p.top_tokens[r * p.top + threadIdx.x] = sound ? i : -1;
-        p.top_logprobs[r * p.top + threadIdx.x] = sound ? to_float(row[i]) - all.m - log_s : NAN;
-      }
-    }
+    store_row<T, kTop>(p, r, token, row, block_part, sh.best);
+    token = next_token;
     __syncthreads();
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) hc_logprob_backward_kernel(const __grid_constant__ LogprobParams p) {
+__global__ void __launch_bounds__(kStreamThreads) hc_logprob_backward_kernel(const __grid_constant__ LogprobParams p) {
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const int64_t token = p.tokens[r];
     const T* row = static_cast<const T*>(p.x) + r * p.stride;
@@ -484,12 +635,12 @@ __global__ void __launch_bounds__(kRowThreads) hc_logprob_backward_kernel(const 
     const Pair first_term = pair(c0, c0), slope = pair(-b, -b);
     const uint32_t lowest = lowest_of<T>(m);
     const int64_t token_group = skip || lost ? -1 : (token + shift) / 8, token_place = (token + shift) % 8;
-    for (int64_t g = (int64_t)blockIdx.y * kAtOnce * kRowThreads + threadIdx.x; g < groups; g += (int64_t)gridDim.y * kAtOnce * kRowThreads) {
+    for (int64_t g = (int64_t)blockIdx.y * kAtOnce * kStreamThreads + threadIdx.x; g < groups; g += (int64_t)gridDim.y * kAtOnce * kStreamThreads) {
       Logits<T> q[kAtOnce];
-      if (!skip) load_some(q, row, g, groups, shift, p.vocab);
+      if (!skip) load_some<kStreamThreads>(q, row, g, groups, shift, p.vocab);
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
-        const int64_t group = g + i * kRowThreads, first = group * 8 - shift;
+        const int64_t group = g + i * kStreamThreads, first = group * 8 - shift;
         if (group >= groups) break;
         float v[8];
         if (skip) {
@@ -522,7 +673,7 @@ __global__ void __launch_bounds__(kRowThreads) hc_logprob_backward_kernel(const 
 namespace {
 
 bool logits_ok(const void* x, int type, size_t rows, size_t vocab, size_t stride) {
-  if (!element_type_ok(type) || vocab == 0 || vocab > 0x7fffffffu || stride < vocab || rows > (1ull << 40) || stride > (1ull << 40))
+  if (!element_type_ok(type) || vocab == 0 || vocab > 0x7fffffffu || stride < vocab || rows > 0x7fffffffu || stride > (1ull << 40))
     return false;
   return rows == 0 || (x && reinterpret_cast<uintptr_t>(x) % element_bytes(type) == 0 && rows <= (1ull << 60) / stride);
 }
@@ -538,11 +689,21 @@ int cluster_of(size_t rows, size_t vocab) {
 
 template <typename T, bool kTop>
 cudaError_t run_logprobs(dev::LogprobParams p, cudaStream_t stream) {
+  const int64_t sms = device_info().sms;
+  // A block for a row has its own start and end, which the ring does without; the ring wants some pieces a row and a row for
+  // each of its blocks.
+  if (p.rows >= 8 * sms && p.vocab >= 2 * dev::kPieceBytes<T> / (int64_t)sizeof(T)) {
+    const int smem = dev::kRing * dev::kPieceBytes<T> + (kTop ? (int)sizeof(dev::TopShared) : 0);
+    const cudaError_t e = set_smem(dev::hc_logprob_stream_kernel<T, kTop>, smem);
+    if (e != cudaSuccess) return e;
+    dev::hc_logprob_stream_kernel<T, kTop><<<(unsigned)(8 * sms), dev::kStreamThreads, smem, stream>>>(p);
+    return cudaGetLastError();
+  }
   p.cluster = cluster_of(p.rows, p.vocab);
-  const int64_t most = 0x7fffffff / 8;
+  if (p.rows > 0x7fffffff / p.cluster) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)((p.rows < most ? p.rows : most) * p.cluster));
+  cfg.gridDim = dim3((unsigned)(p.rows * p.cluster));
   cfg.blockDim = dim3(dev::kRowThreads);
   cfg.dynamicSmemBytes = kTop ? sizeof(dev::TopShared) : 0;
   cfg.stream = stream;
@@ -562,6 +723,9 @@ cudaError_t by_type(int type, F f) {
 }
 
 }  // namespace
+
+int logprob_status(int clear) { return take_status(dev::g_logprob_status, clear); }
+
 }  // namespace hc
 
 extern "C" {
@@ -589,11 +753,11 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
   if (!tokens || !stats) return hc::kErrArgument;
   hc::dev::LogprobParams p = {logits, tokens, nullptr, nullptr, nullptr, nullptr, const_cast<float*>(stats), dlogprobs, dentropy, dlogits,
                               (int64_t)rows, (int64_t)vocab, (int64_t)stride, (int64_t)dstride, ignore, 0, 1};
-  const size_t chunk = 8 * hc::dev::kAtOnce * hc::dev::kRowThreads, parts = (vocab + 7 + chunk - 1) / chunk;
-  const unsigned y = (unsigned)(rows >= 1024 ? 1 : parts < 1 ? 1 : parts > 64 ? 64 : parts);
+  const size_t chunk = 8 * hc::dev::kAtOnce * hc::dev::kStreamThreads, parts = (vocab + 7 + chunk - 1) / chunk;
+  const unsigned y = (unsigned)(rows >= 2048 ? 1 : parts < 1 ? 1 : parts > 64 ? 64 : parts);
   const dim3 grid((unsigned)(rows < 0x7fffffff ? rows : 0x7fffffff), y);
   const cudaError_t e = hc::by_type(type, [&](auto t) {
-    hc::dev::hc_logprob_backward_kernel<decltype(t)><<<grid, hc::dev::kRowThreads, 0, stream>>>(p);
+    hc::dev::hc_logprob_backward_kernel<decltype(t)><<<grid, hc::dev::kStreamThreads, 0, stream>>>(p);
     return cudaGetLastError();
   });
   return e == cudaSuccess ? hc::kOk : hc::kErrCuda;

@@ -619,13 +619,7 @@ bool norm_arguments_ok(const void* x, int x_type, const void* y, int y_type, int
 
 }  // namespace
 
-int norm_status(int clear) {
-  unsigned int status = 0;
-  if (cudaMemcpyFromSymbol(&status, dev::g_norm_status, sizeof(status)) != cudaSuccess) return kErrCuda;
-  const unsigned int zero = 0;
-  if (clear && status && cudaMemcpyToSymbol(dev::g_norm_status, &zero, sizeof(zero)) != cudaSuccess) return kErrCuda;
-  return (int)status;
-}
+int norm_status(int clear) { return take_status(dev::g_norm_status, clear); }
 
 }  // namespace hc
 

@@ -10,7 +10,17 @@ namespace hc {
 
 enum ElementType : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 inline size_t element_bytes(int type) { return type == kF32 ? 4 : 2; }
-int norm_status(int clear);  // of the layer norm's kernels (hc_norm.cu)
+// The status of the kernels of a source: 0, or 3 after a wait that ran out, kept until it is cleared.
+int norm_status(int clear);
+int logprob_status(int clear);
+template <typename S>
+int take_status(S& symbol, int clear) {
+  unsigned int status = 0;
+  if (cudaMemcpyFromSymbol(&status, symbol, sizeof(status)) != cudaSuccess) return 5;  // kErrCuda
+  const unsigned int zero = 0;
+  if (clear && status && cudaMemcpyToSymbol(symbol, &zero, sizeof(zero)) != cudaSuccess) return 5;
+  return (int)status;
+}
 inline bool element_type_ok(int type) { return type >= kF32 && type <= kF16; }
 
 namespace dev {
