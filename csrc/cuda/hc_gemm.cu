@@ -681,7 +681,8 @@ cudaError_t run_gemm(const GemmCall& given, cudaStream_t stream) {
   // the iteration's own arrays lie as TMA wants them
   if (!kLinear && ((MODE != kGemmGram && !p.tma_in) || (kUpdate && (!p.tma_in2 || (c.out2.data && (!p.tma_out || !p.tma_out2)))))) return cudaErrorInvalidValue;
   if ((MODE == kGemmGram || MODE == kGemmPoly) && (!p.tma_out || !make_side_map(&p.map_mirror, c.out, kF16, c, true, true))) return cudaErrorInvalidValue;
-  const cudaError_t e = set_smem(dev::hc_gemm_kernel<BN, kCtas, MODE>, S::kSmem);
+  static unsigned long long allowed = 0;
+  const cudaError_t e = allow_smem(dev::hc_gemm_kernel<BN, kCtas, MODE>, S::kSmem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t total = tiles * c.batch, units = device_info().sms / kCtas;
   cudaLaunchConfig_t cfg;

@@ -81,6 +81,20 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), int grid, int block, in
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// The same, asked once for each device: `done` is the kernel's own, one bit a device.  All sizes up to the most that a block may
+// have are allowed then.
+template <typename K>
+cudaError_t allow_smem(K kernel, int most, unsigned long long* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return cudaSuccess;
+  e = set_smem(kernel, most);
+  if (e == cudaSuccess) __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
+  return e;
+}
+
 // CTAs of `kernel` that one GPU holds at the same time, asked of the runtime once per device.  The
 // kernels are written for a grid that is resident as a whole (CTA i owns tile i, and every look-back
 // waits for tiles held by other CTAs of the grid), so the grid is cut to this number, never assumed.

@@ -694,7 +694,8 @@ cudaError_t run_logprobs(dev::LogprobParams p, cudaStream_t stream) {
   // each of its blocks.
   if (p.rows >= 8 * sms && p.vocab >= 2 * dev::kPieceBytes<T> / (int64_t)sizeof(T)) {
     const int smem = dev::kRing * dev::kPieceBytes<T> + (kTop ? (int)sizeof(dev::TopShared) : 0);
-    const cudaError_t e = set_smem(dev::hc_logprob_stream_kernel<T, kTop>, smem);
+    static unsigned long long allowed = 0;
+    const cudaError_t e = allow_smem(dev::hc_logprob_stream_kernel<T, kTop>, smem, &allowed);
     if (e != cudaSuccess) return e;
     dev::hc_logprob_stream_kernel<T, kTop><<<(unsigned)(8 * sms), dev::kStreamThreads, smem, stream>>>(p);
     return cudaGetLastError();

@@ -537,7 +537,8 @@ cudaError_t run_forward(dev::NormParams p, cudaStream_t stream) {
   using G = dev::Block<T, false>;
   const int smem = plan_rings(&p, sizeof(X), 0, G::kTeams, 2 * K * T * 8 * 4, 0);
   if (p.stages < 2) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = set_smem(dev::hc_norm_kernel<X, Y, T, K>, smem);
+  static unsigned long long allowed = 0;
+  const cudaError_t e = allow_smem(dev::hc_norm_kernel<X, Y, T, K>, dev::kNormSmem, &allowed);
   if (e != cudaSuccess) return e;
   dev::hc_norm_kernel<X, Y, T, K><<<norm_blocks<false>(p.rows, p.width), G::kThreads, smem, stream>>>(p);
   return cudaGetLastError();
@@ -547,7 +548,8 @@ cudaError_t run_backward(dev::NormParams p, int blocks, cudaStream_t stream) {
   using G = dev::Block<T, true>;
   const int smem = plan_rings(&p, sizeof(X), sizeof(Y), G::kTeams, K * T * 8 * 4, 2 * K * T * 8 * 4);
   if (p.stages < 2) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = set_smem(dev::hc_norm_backward_kernel<X, Y, T, K>, smem);
+  static unsigned long long allowed = 0;
+  const cudaError_t e = allow_smem(dev::hc_norm_backward_kernel<X, Y, T, K>, dev::kNormSmem, &allowed);
   if (e != cudaSuccess) return e;
   dev::hc_norm_backward_kernel<X, Y, T, K><<<blocks, G::kThreads, smem, stream>>>(p);
   return cudaGetLastError();

@@ -1,6 +1,8 @@
 """What the front ends of the training step's operators share: types, checks of tensors, calls."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -35,9 +37,19 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_functions = {}  # native functions by name
+
+
+def _function(name: str):
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.cuda(), name)
+    return fn
+
+
 def call(what: str, name: str, device: torch.device, *args):
     """The native function on the current stream of ``device``, with that device current."""
-    fn = getattr(_lib.cuda(), name)
+    fn = _functions.get(name) or _function(name)
     index = device.index
     if _current_device() == index:
         st = fn(*args, _raw_stream(index))
@@ -48,12 +60,15 @@ def call(what: str, name: str, device: torch.device, *args):
         _lib.check(st, what)
 
 
+@functools.lru_cache(maxsize=4096)
+def _size(name: str, index: int, *args) -> int:
+    with torch.cuda.device(index):
+        return _function(name)(*args)
+
+
 def size(name: str, device: torch.device, *args) -> int:
-    """A native function that says how much scratch memory a call needs."""
-    if _current_device() == device.index:
-        return getattr(_lib.cuda(), name)(*args)
-    with torch.cuda.device(device):
-        return getattr(_lib.cuda(), name)(*args)
+    """A native function that says how much scratch memory a call needs: it goes by sizes and the device alone."""
+    return _size(name, device.index, *args)
 
 
 def wants_grad(*tensors) -> bool:

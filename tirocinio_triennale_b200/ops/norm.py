@@ -10,7 +10,7 @@ from ._train import TYPES, call, floating, packed, ptr, size, vector, wants_grad
 def _forward(x, weight, bias, eps, out_dtype, keep):
     width = x.shape[-1]
     rows = x.numel() // width
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    y = torch.empty_like(x, dtype=out_dtype)
     stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if keep else None
     param = weight if weight is not None else bias
     call("layer_norm", "hc_layer_norm", x.device, x.data_ptr(), TYPES[x.dtype], ptr(weight), ptr(bias),
