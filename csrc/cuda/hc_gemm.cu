@@ -187,11 +187,10 @@ __device__ __forceinline__ void tile_place(const GemmParams& p, int t, int& mi, 
   }
 }
 
-__device__ __forceinline__ float activate(float z, int kind) {
-  if (kind == kActGeluTanh) return z * sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));  // (1 + tanh u) / 2 = sigmoid(2 u)
-  if (kind == kActSilu) return z * sigmoid(z);
-  if (kind == kActRelu) return z > 0.0f ? z : z != z ? z : 0.0f;
-  return z;
+template <int kAct>
+__device__ __forceinline__ void activate_all(float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) activate_pair<kAct>(v[j], v[j + 1]);
 }
 
 constexpr float kLow = 2048.0f;  // lo is held times this: as precise next to hi as fp16 can be
@@ -245,10 +244,9 @@ __device__ __forceinline__ void gemm_finish(const GemmParams& p, int z, int row0
       for (int j = 0; j < 32; ++j)
         if (j < count) param_put(p.out2.data, p.type, row * p.out2.ld + col0 + j, v[j]);
     }
-    if (p.activation != kActNone) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = activate(v[j], p.activation);
-    }
+    if (p.activation == kActGeluTanh) activate_all<kActGeluTanh>(v);
+    else if (p.activation == kActRelu) activate_all<kActRelu>(v);
+    else if (p.activation == kActSilu) activate_all<kActSilu>(v);
     if (p.in.data && !p.tma_in) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)

@@ -4,16 +4,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-namespace hc {
-namespace dev {
-__device__ __forceinline__ float sigmoid(float v) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return r;
-}
-}  // namespace dev
+#include "hc_train.cuh"
 
+namespace hc {
 enum GemmMode : int {
   kGemmLinear = 0,  // out = act(acc + bias) + residual; z = acc + bias
   kGemmGram = 1,    // out = acc, symmetric
@@ -21,6 +14,69 @@ enum GemmMode : int {
   kGemmUpdate = 3,  // x = a (hi + lo / 2048) + acc; out hi and lo again, or bf16
 };
 enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActRelu = 2, kActSilu = 3 };
+
+namespace dev {
+
+// Activations of two values at a time.  GELU (tanh form) and SiLU are z sigmoid(v), with v = 2 sqrt(2 / pi) (z + 0.044715 z^3)
+// or z; sigmoid(v) = 1 / (1 + e) with e = exp(-v), and one reciprocal, of the product of both sums, serves both values: exp and
+// reciprocal are what these functions cost.  z is raised to where e is 2^60 and the function within 1e-16 of 0, so that
+// the product stays in range.
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f * 1.5957691216057308f;
+constexpr float kGeluLeast = -7.5f, kSiluLeast = -41.5f;  // v = -41.6, -41.5
+
+__device__ __forceinline__ float act_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float act_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// sigmoid of both v, given v times -log2(e)
+__device__ __forceinline__ Pair sigmoid_pair(Pair exponent) {
+  float a, b, r;
+  parts(exponent, a, b);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(a));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(b));
+  a += 1.0f;
+  b += 1.0f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  return pair(b, a) * pair(r, r);
+}
+template <int kAct>
+__device__ __forceinline__ void activate_pair(float& x, float& y) {
+  if (kAct == kActRelu) {
+    x = act_max_nan(x, 0.0f);
+    y = act_max_nan(y, 0.0f);
+  } else if (kAct == kActGeluTanh || kAct == kActSilu) {
+    const float least = kAct == kActSilu ? kSiluLeast : kGeluLeast;
+    const Pair z = pair(act_max_nan(x, least), act_max_nan(y, least));
+    Pair v = z * pair(-kLog2E, -kLog2E);
+    if (kAct == kActGeluTanh) v = z * fma2(z * z, pair(-kGelu3 * kLog2E, -kGelu3 * kLog2E), pair(-kGelu1 * kLog2E, -kGelu1 * kLog2E));
+    parts(z * sigmoid_pair(v), x, y);
+  }
+}
+// g times the activation's slope at z: s + z s (1 - s) v'.  Beyond +-7.5 (41.5) it is 0 and 1 to within 1e-16.
+template <int kAct>
+__device__ __forceinline__ Pair slope_pair(Pair g, float x, float y) {
+  if (kAct == kActNone) return g;
+  if (kAct == kActRelu) return g * pair(x > 0.0f ? 1.0f : x != x ? x : 0.0f, y > 0.0f ? 1.0f : y != y ? y : 0.0f);
+  const float least = kAct == kActSilu ? kSiluLeast : kGeluLeast;
+  const Pair z = pair(act_min_nan(act_max_nan(x, least), -least), act_min_nan(act_max_nan(y, least), -least));
+  Pair v = z * pair(-kLog2E, -kLog2E), zdv = z;
+  if (kAct == kActGeluTanh) {
+    const Pair square = z * z;
+    v = z * fma2(square, pair(-kGelu3 * kLog2E, -kGelu3 * kLog2E), pair(-kGelu1 * kLog2E, -kGelu1 * kLog2E));
+    zdv = z * fma2(square, pair(3.0f * kGelu3, 3.0f * kGelu3), pair(kGelu1, kGelu1));
+  }
+  const Pair s = sigmoid_pair(v), minus = s * pair(-1.0f, -1.0f);
+  return g * fma2(zdv, fma2(minus, s, s), s);
+}
+
+}  // namespace dev
 
 // An operand is stored as rows of adjacent elements.  kMajor: its rows are those of the product (or its columns, for the
 // second operand) and lie along the sum; otherwise the sum runs over its rows.

@@ -20,19 +20,11 @@ struct FewRowsParams {
 };
 
 __device__ __forceinline__ float act_value(float z, int kind) {
-  if (kind == kActNone) return z;
-  if (kind == kActRelu) return z > 0.0f ? z : z != z ? z : 0.0f;
-  return z * sigmoid(kind == kActSilu ? z : 1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
-}
-__device__ __forceinline__ float act_slope(float z, int kind) {
-  if (kind == kActNone) return 1.0f;
-  if (kind == kActRelu) return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
-  // d/dz of z sigmoid(v) = s + z s (1 - s) v'; where s (1 - s) is 0, z and v' may have left the range
-  const bool gelu = kind == kActGeluTanh;
-  const float v = gelu ? 1.5957691216057308f * fmaf(0.044715f * z * z, z, z) : z;
-  const float dv = gelu ? 1.5957691216057308f * fmaf(3.0f * 0.044715f * z, z, 1.0f) : 1.0f;
-  const float s = sigmoid(v), t = s * (1.0f - s);
-  return t > 0.0f ? fmaf(z * t, dv, s) : s;
+  float other = 0.0f;
+  if (kind == kActGeluTanh) activate_pair<kActGeluTanh>(z, other);
+  else if (kind == kActRelu) activate_pair<kActRelu>(z, other);
+  else if (kind == kActSilu) activate_pair<kActSilu>(z, other);
+  return z;
 }
 
 template <typename T, int R, bool kVector>
@@ -110,9 +102,9 @@ __global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_cons
   constexpr int kAtOnce = 4;  // rows whose loads are under way together
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t col = blockIdx.x * 256ll + lane * 8, step = p.shares * 8ll;
-  float total[8];
+  Pair total[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) total[j] = 0.0f;
+  for (int j = 0; j < 4; ++j) total[j] = pair(0.0f, 0.0f);
   const bool whole = kVector && col + 8 <= p.width;
   for (int64_t r0 = blockIdx.y * 8ll + warp; r0 < p.rows && col < p.width; r0 += step * kAtOnce) {
     float g[kAtOnce][8], a[kAtOnce][8];
@@ -137,9 +129,10 @@ __global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_cons
     for (int i = 0; i < kAtOnce; ++i) {
       const int64_t r = r0 + i * step;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (kAct != kActNone) g[i][j] *= act_slope(a[i][j], kAct);
-        total[j] += g[i][j];
+      for (int j = 0; j < 4; ++j) {
+        const Pair v = slope_pair<kAct>(pair(g[i][2 * j], g[i][2 * j + 1]), a[i][2 * j], a[i][2 * j + 1]);
+        total[j] = total[j] + v;
+        parts(v, g[i][2 * j], g[i][2 * j + 1]);
       }
       if (p.dz && r < p.rows) {
         T* dz = static_cast<T*>(p.dz) + r * p.ldd + col;
@@ -155,7 +148,7 @@ __global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_cons
   }
   if (!p.partial) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sums[warp][lane * 8 + j] = total[j];
+  for (int j = 0; j < 4; ++j) parts(total[j], sums[warp][lane * 8 + 2 * j], sums[warp][lane * 8 + 2 * j + 1]);
   __syncthreads();
   const int64_t c = blockIdx.x * 256ll + threadIdx.x;
   float s = 0.0f;

@@ -49,11 +49,12 @@ __device__ __forceinline__ void for_groups(const ScaleParams& p, const T* g, F f
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) hc_square_sum_kernel(const __grid_constant__ ScaleParams p) {
   __shared__ double sums[kNormThreads / 32];
-  double s = 0.0;
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
   for_groups<T, kVector>(p, static_cast<const T*>(p.g) + blockIdx.y * p.batch_stride, [&](int64_t, int64_t, const float (&v)[8]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fma((double)v[j], (double)v[j], s);
+    for (int j = 0; j < 8; ++j) part[j & 3] = fma((double)v[j], (double)v[j], part[j & 3]);
   });
+  double s = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
@@ -104,6 +105,157 @@ __global__ void __launch_bounds__(kNormThreads) hc_scale_kernel(const __grid_con
   });
 }
 
+// ---- small matrices ---------------------------------------------------------------------------------------------------
+// The general form is three launches a step, whose work on a small matrix is less than their start.  Here one block takes a
+// matrix through all steps in shared memory, short side first, with warp-wide 16 x 8 x 16 matrix instructions: they need
+// neither tensor memory nor descriptors, and at this size what counts is the way from one product to the next.
+constexpr int kSmallThreads = 512;
+constexpr int kSmallTiles = 16;  // tiles of 16 x 8 of a warp at the most
+
+struct SmallParams {
+  const void* g;
+  __nv_bfloat16* out;
+  int64_t stride, batch_stride;
+  int height, width;  // of a matrix as it is given
+  int side, length;   // short and long side
+  int rows, pitch;    // short side rounded up to 16; halves from row to row of X
+  int s_pitch;        // of S and the polynomial
+  int steps;
+  float a, b, c, eps, growth;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const __half* p, bool transposed) {
+  const uint32_t at = smem_u32(p);
+  if (transposed)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two neighbouring tiles, 16 rows from `row` and 16 columns from `col`, of a product over k: the first operand's rows lie along
+// the sum; the second one is given as rows along it (kAcross: false) or as rows across it.
+template <bool kAcross>
+__device__ __forceinline__ void small_product(float (&d0)[4], float (&d1)[4], const __half* a, int a_pitch, const __half* b, int b_pitch, int row,
+                                              int col, int k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) d0[j] = d1[j] = 0.0f;
+  const __half* pa = a + (row + (lane & 15)) * a_pitch + (lane >> 4) * 8;
+  const __half* pb = kAcross ? b + (lane & 15) * b_pitch + col + (lane >> 4) * 8 : b + (col + (lane & 7) + (lane >> 4) * 8) * b_pitch + ((lane >> 3) & 1) * 8;
+  for (int i = 0; i < k; i += 16) {
+    uint32_t fa[4], fb[4];
+    ldmatrix4(fa, pa + i, false);
+    ldmatrix4(fb, pb + (kAcross ? i * b_pitch : i), kAcross);
+    mma16816(d0, fa, fb[0], fb[1]);
+    mma16816(d1, fa, fb[2], fb[3]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSmallThreads, 1) hc_newton_small_kernel(const __grid_constant__ SmallParams p) {
+  extern __shared__ __align__(16) __half small[];
+  __shared__ double sums[kSmallThreads / 32];
+  __half* hi = small;
+  __half* lo = hi + p.rows * p.pitch;
+  __half* s = lo + p.rows * p.pitch;
+  __half* q = s + p.rows * p.s_pitch;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool tall = p.height > p.width;
+  const T* g = static_cast<const T*>(p.g) + blockIdx.x * p.batch_stride;
+  const int count = p.height * p.width;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < count; i += kSmallThreads) {
+    const int r = i / p.width, c = i - r * p.width;
+    const double v = (double)to_float(g[r * p.stride + c]);
+    sum = fma(v, v, sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sums[warp] = sum;
+  for (int i = threadIdx.x; i < p.rows * p.pitch * 2; i += kSmallThreads) small[i] = __float2half_rn(0.0f);  // also what rounds X up
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < kSmallThreads / 32; ++w) sum += sums[w];
+  const double norm = sqrt(sum), room = (norm / (norm + (double)p.eps)) * (double)p.growth;
+  int k = 0;
+  while (k < 126 && room * exp2((double)(k + 1)) <= 1.0) ++k;
+  const float scale = exp2f((float)-k);
+  const double factor = exp2((double)k) / (norm + (double)p.eps);
+  for (int i = threadIdx.x; i < count; i += kSmallThreads) {
+    const int r = i / p.width, c = i - r * p.width;
+    const float v = (float)((double)to_float(g[r * p.stride + c]) * factor);
+    const __half h = __float2half_rn(v);
+    const int at = tall ? c * p.pitch + r : r * p.pitch + c;
+    hi[at] = h;
+    lo[at] = __float2half_rn((v - __half2float(h)) * 2048.0f);
+  }
+  __syncthreads();
+  const int row_tiles = p.rows / 16, s_tiles = row_tiles * row_tiles, length = (p.length + 15) / 16 * 16, x_tiles = row_tiles * (length / 16);
+  const int r0 = lane / 4, c0 = (lane & 3) * 2;  // of a thread's part of a tile: rows r0 and r0 + 8, columns c0 and c0 + 1
+  const float c1 = p.b * scale * scale, c2 = p.c * scale * scale * scale * scale;
+  for (int step = 0; step < p.steps; ++step) {
+    for (int t = warp; t < s_tiles; t += kSmallThreads / 32) {
+      const int row = t / row_tiles * 16, col = t % row_tiles * 16;
+      float d[2][4];
+      small_product<false>(d[0], d[1], hi, p.pitch, hi, p.pitch, row, col, length);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __half* to = s + (row + r0 + (j >> 1) * 8) * p.s_pitch + col + c0;
+        *reinterpret_cast<__half2*>(to + (j & 1) * 8) = __floats2half2_rn(d[j & 1][(j >> 1) * 2], d[j & 1][(j >> 1) * 2 + 1]);
+      }
+    }
+    __syncthreads();
+    for (int t = warp; t < s_tiles; t += kSmallThreads / 32) {
+      const int row = t / row_tiles * 16, col = t % row_tiles * 16;
+      float d[2][4];
+      small_product<false>(d[0], d[1], s, p.s_pitch, s, p.s_pitch, row, col, p.rows);  // S is its own mirror image
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = (row + r0 + (j >> 1) * 8) * p.s_pitch + col + c0 + (j & 1) * 8;
+        const float2 old = __half22float2(*reinterpret_cast<const __half2*>(s + at));
+        const float* v = d[j & 1] + (j >> 1) * 2;
+        *reinterpret_cast<__half2*>(q + at) = __floats2half2_rn(fmaf(c2, v[0], c1 * old.x), fmaf(c2, v[1], c1 * old.y));
+      }
+    }
+    __syncthreads();
+    float d[kSmallTiles][4];
+#pragma unroll
+    for (int i = 0; i < kSmallTiles / 2; ++i) {
+      const int t = warp + i * (kSmallThreads / 32);
+      if (t < x_tiles) small_product<true>(d[2 * i], d[2 * i + 1], q, p.s_pitch, hi, p.pitch, t % row_tiles * 16, t / row_tiles * 16, p.rows);
+    }
+    __syncthreads();  // nobody reads the old X any more
+    const bool last = step == p.steps - 1;
+#pragma unroll
+    for (int i = 0; i < kSmallTiles / 2; ++i) {
+      const int t = warp + i * (kSmallThreads / 32);
+      if (t >= x_tiles) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = t % row_tiles * 16 + r0 + (j >> 1) * 8, col = t / row_tiles * 16 + c0 + (j & 1) * 8, at = row * p.pitch + col;
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(hi + at)), l = __half22float2(*reinterpret_cast<const __half2*>(lo + at));
+        const float* v = d[2 * i + (j & 1)] + (j >> 1) * 2;
+        const float x0 = fmaf(p.a, fmaf(l.x, 1.0f / 2048.0f, h.x), v[0]), x1 = fmaf(p.a, fmaf(l.y, 1.0f / 2048.0f, h.y), v[1]);
+        if (last) {
+          __nv_bfloat16* out = p.out + (int64_t)blockIdx.x * count;
+          if (row < p.side && col < p.length) out[tall ? col * p.width + row : row * p.width + col] = __float2bfloat16_rn(x0 * scale);
+          if (row < p.side && col + 1 < p.length) out[tall ? (col + 1) * p.width + row : row * p.width + col + 1] = __float2bfloat16_rn(x1 * scale);
+        } else {
+          const __half2 nh = __floats2half2_rn(x0, x1);
+          const float2 f = __half22float2(nh);
+          *reinterpret_cast<__half2*>(hi + at) = nh;
+          *reinterpret_cast<__half2*>(lo + at) = __floats2half2_rn((x0 - f.x) * 2048.0f, (x1 - f.y) * 2048.0f);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
 }  // namespace dev
 
 namespace {
@@ -148,6 +300,35 @@ void scale(const dev::ScaleParams& p, size_t batch, cudaStream_t stream) {
   else scale_of<T, false>(p, batch, stream);
 }
 
+constexpr int kSmallSmem = 224 * 1024;
+
+// The form for small matrices: where its tiles fit a warp's registers and shared memory, and a block is done with a matrix
+// sooner than launches of the general form follow one another.  A step of that takes 14 us and some more for large matrices; a
+// block computes about 1.2 MFLOP a microsecond.
+bool small_plan(dev::SmallParams* p, size_t batch, size_t height, size_t width, int* smem) {
+  const int64_t side = height < width ? height : width, length = height < width ? width : height;
+  const int64_t rows = (side + 15) / 16 * 16, long_rows = (length + 15) / 16 * 16;
+  if (rows > 128 || rows / 16 * (long_rows / 16) > dev::kSmallThreads / 32 * (dev::kSmallTiles / 2)) return false;
+  // rows of 16 bytes more than a whole number of 32: eight rows of ldmatrix lie in different banks
+  p->pitch = (int)long_rows + 8;
+  p->s_pitch = (int)rows + 8;
+  *smem = (int)((2 * rows * p->pitch + 2 * rows * p->s_pitch) * 2);
+  if (*smem > kSmallSmem) return false;
+  const int64_t sms = device_info().sms > 0 ? device_info().sms : 1, waves = ((int64_t)batch + sms - 1) / sms;
+  const double flop = 2.0 * rows * rows * (2.0 * long_rows + rows);
+  if (waves * flop / 1.2e6 > 14.0) return false;
+  p->height = (int)height, p->width = (int)width, p->side = (int)side, p->length = (int)length, p->rows = (int)rows;
+  return true;
+}
+template <typename T>
+cudaError_t run_small(const dev::SmallParams& p, size_t batch, int smem, cudaStream_t stream) {
+  static unsigned long long allowed = 0;
+  const cudaError_t e = allow_smem(dev::hc_newton_small_kernel<T>, kSmallSmem, &allowed);
+  if (e != cudaSuccess) return e;
+  dev::hc_newton_small_kernel<T><<<(unsigned)batch, dev::kSmallThreads, smem, stream>>>(p);
+  return cudaGetLastError();
+}
+
 }  // namespace
 }  // namespace hc
 
@@ -166,6 +347,20 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   if (!g || !out || !scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u)) return kErrArgument;
   const Layout l = layout_of(batch, height, width);
   if (scratch_bytes < l.total) return kErrArgument;
+  float growth = 1.0f;
+  for (int i = 0; i < steps; ++i) growth *= a > 1.0f || a < -1.0f ? (a < 0.0f ? -a : a) : 1.0f;
+  dev::SmallParams small;
+  int smem = 0;
+  if (small_plan(&small, batch, height, width, &smem)) {
+    small.g = g;
+    small.out = static_cast<__nv_bfloat16*>(out);
+    small.stride = (int64_t)stride, small.batch_stride = (int64_t)batch_stride;
+    small.steps = steps;
+    small.a = a, small.b = b, small.c = c, small.eps = eps, small.growth = growth;
+    const cudaError_t e = type == kF32 ? run_small<float>(small, batch, smem, stream)
+                          : type == kBf16 ? run_small<__nv_bfloat16>(small, batch, smem, stream) : run_small<__half>(small, batch, smem, stream);
+    return e == cudaSuccess ? kOk : kErrCuda;
+  }
   unsigned char* at = static_cast<unsigned char*>(scratch);
   double* partial = reinterpret_cast<double*>(at);
   at += round_up(batch * l.parts * 8);
@@ -175,8 +370,6 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   void* lo = at + 2 * l.x;
   void* gram = at + 3 * l.x;
   void* poly = at + 3 * l.x + l.s;
-  float growth = 1.0f;
-  for (int i = 0; i < steps; ++i) growth *= a > 1.0f || a < -1.0f ? (a < 0.0f ? -a : a) : 1.0f;
   const dev::ScaleParams p = {g, partial, static_cast<__half*>(hi[0]), static_cast<__half*>(lo), scales, growth, (int64_t)height, (int64_t)width, (int64_t)stride,
                               (int64_t)batch_stride, l.ld, (int)l.parts, l.lanes, eps};
   if (type == kF32) scale<float>(p, batch, stream);

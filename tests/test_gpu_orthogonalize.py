@@ -41,7 +41,7 @@ def gaussian(*shape, seed=0):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("height,width", [(1, 1), (1, 64), (64, 1), (8, 8), (32, 48), (64, 192), (192, 64), (100, 100), (128, 128), (129, 130), (131, 129), (127, 600), (500, 75), (255, 257), (768, 768), (300, 1100), (1030, 260)])
+@pytest.mark.parametrize("height,width", [(1, 1), (1, 64), (64, 1), (8, 8), (32, 48), (64, 192), (192, 64), (100, 100), (128, 128), (129, 130), (131, 129), (127, 600), (500, 75), (255, 257), (16, 1000), (700, 33), (96, 340), (60, 2000), (768, 768), (300, 1100), (1030, 260)])
 def test_sizes(height, width):
     # a few rows or columns: the matrix is next to orthogonal already, few roundings average out
     check(gaussian(height, width, seed=height), ROOM if min(height, width) > 1 else 8e-3)
