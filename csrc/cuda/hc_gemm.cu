@@ -548,9 +548,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
       }
     }
     if (lane == 0) {
-      // what was fetched and not used (after a wait that ran out) lands before the CTA leaves, and all stores are done
+      // what was fetched and not used (after a wait that ran out) lands before the CTA leaves, and all stores have read what
+      // they take from its shared memory
       for (; uses < fetched; ++uses) mbar_wait_bounded(&loaded[uses & 1], (uses >> 1) & 1, kGemmLimitNs);
-      tma_wait_group<0>();
+      tma_wait_group_read<0>();
     }
   }
   __syncthreads();

@@ -108,20 +108,21 @@ __global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_cons
   const bool whole = kVector && col + 8 <= p.width;
   for (int64_t r0 = blockIdx.y * 8ll + warp; r0 < p.rows && col < p.width; r0 += step * kAtOnce) {
     float g[kAtOnce][8], a[kAtOnce][8];
+    if (whole && r0 + (kAtOnce - 1) * step < p.rows) {
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int64_t r = r0 + i * step;
-      const Y* dy = static_cast<const Y*>(p.dy) + r * p.ldy + col;
-      const T* z = static_cast<const T*>(p.z) + r * p.ldz + col;
-      if (whole && r < p.rows) {
-        load8(dy, g[i]);
-        if (kAct != kActNone) load8(z, a[i]);
-      } else {
+      for (int i = 0; i < kAtOnce; ++i) {
+        load8(static_cast<const Y*>(p.dy) + (r0 + i * step) * p.ldy + col, g[i]);
+        if (kAct != kActNone) load8(static_cast<const T*>(p.z) + (r0 + i * step) * p.ldz + col, a[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int64_t r = r0 + i * step;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = r < p.rows && col + j < p.width;
-          g[i][j] = in ? to_float(dy[j]) : 0.0f;
-          a[i][j] = kAct != kActNone && in ? to_float(z[j]) : 0.0f;
+          g[i][j] = in ? to_float(static_cast<const Y*>(p.dy)[r * p.ldy + col + j]) : 0.0f;
+          a[i][j] = kAct != kActNone && in ? to_float(static_cast<const T*>(p.z)[r * p.ldz + col + j]) : 0.0f;
         }
       }
     }

@@ -23,26 +23,36 @@ struct ScaleParams {
   float growth;
   int64_t height, width, stride, batch_stride, ld;  // ld: of hi and lo
   int parts;
-  int lanes;  // threads of a block that share a row, a power of two
   float eps;
 };
 
-// The values of one matrix in groups of eight, a block's share of them: f(row, column, values)
+// The values of one matrix in groups of eight, a block's share of them, four groups under way at a time: f(row, column, values)
 template <typename T, bool kVector, typename F>
 __device__ __forceinline__ void for_groups(const ScaleParams& p, const T* g, F f) {
-  const int rows = kNormThreads / p.lanes, lane = threadIdx.x & (p.lanes - 1);
-  for (int64_t r = (int64_t)blockIdx.x * rows + threadIdx.x / p.lanes; r < p.height; r += (int64_t)p.parts * rows)
-#pragma unroll 4
-    for (int64_t c = lane * 8; c < p.width; c += p.lanes * 8) {
-      float v[8];
-      if (kVector) {
-        load8(g + r * p.stride + c, v);
-      } else {
+  const uint32_t each = (uint32_t)((p.width + 7) / 8), step = gridDim.x * kNormThreads;
+  const int64_t groups = p.height * (int64_t)each;
+  for (int64_t i0 = blockIdx.x * kNormThreads + threadIdx.x; i0 < groups; i0 += 4ll * step) {
+    float v[4][8];
+    int64_t row[4], col[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < p.width ? to_float(g[r * p.stride + c + j]) : 0.0f;
-      }
-      f(r, c, v);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = i0 + (int64_t)i * step;
+      row[i] = groups <= 0xffffffffll ? (uint32_t)at / each : at / each;
+      col[i] = (at - row[i] * each) * 8;
     }
+    if (kVector && i0 + 3ll * step < groups) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load8(g + row[i] * p.stride + col[i], v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = i0 + (int64_t)i * step < groups && col[i] + j < p.width ? to_float(g[row[i] * p.stride + col[i] + j]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + (int64_t)i * step < groups) f(row[i], col[i], v[i]);
+  }
 }
 
 // Sums of squares, in 64 bits: the entries may be anything that their type can hold.  Bound by memory.
@@ -110,7 +120,6 @@ __global__ void __launch_bounds__(kNormThreads) hc_scale_kernel(const __grid_con
 // matrix through all steps in shared memory, short side first, with warp-wide 16 x 8 x 16 matrix instructions: they need
 // neither tensor memory nor descriptors, and at this size what counts is the way from one product to the next.
 constexpr int kSmallThreads = 512;
-constexpr int kSmallTiles = 16;  // tiles of 16 x 8 of a warp at the most
 
 struct SmallParams {
   const void* g;
@@ -142,16 +151,37 @@ template <bool kAcross>
 __device__ __forceinline__ void small_product(float (&d0)[4], float (&d1)[4], const __half* a, int a_pitch, const __half* b, int b_pitch, int row,
                                               int col, int k) {
   const int lane = threadIdx.x & 31;
+  // the next operands are on their way while one pair is multiplied, and two sums take turns; not unrolled further: with all
+  // tiles' loops in line the code outgrew the instruction cache (a step of 192 x 64: 6.0 us, 4.7 rolled up)
+  float e0[4], e1[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) d0[j] = d1[j] = 0.0f;
+  for (int j = 0; j < 4; ++j) d0[j] = d1[j] = e0[j] = e1[j] = 0.0f;
   const __half* pa = a + (row + (lane & 15)) * a_pitch + (lane >> 4) * 8;
   const __half* pb = kAcross ? b + (lane & 15) * b_pitch + col + (lane >> 4) * 8 : b + (col + (lane & 7) + (lane >> 4) * 8) * b_pitch + ((lane >> 3) & 1) * 8;
-  for (int i = 0; i < k; i += 16) {
-    uint32_t fa[4], fb[4];
-    ldmatrix4(fa, pa + i, false);
-    ldmatrix4(fb, pb + (kAcross ? i * b_pitch : i), kAcross);
-    mma16816(d0, fa, fb[0], fb[1]);
-    mma16816(d1, fa, fb[2], fb[3]);
+  const int b_step = kAcross ? 16 * b_pitch : 16, n = k / 16;
+  uint32_t fa[2][4], fb[2][4];
+  ldmatrix4(fa[0], pa, false);
+  ldmatrix4(fb[0], pb, kAcross);
+#pragma unroll 1
+  for (int i = 0; i < n; i += 2) {
+    if (i + 1 < n) {
+      ldmatrix4(fa[1], pa + (i + 1) * 16, false);
+      ldmatrix4(fb[1], pb + (i + 1) * b_step, kAcross);
+    }
+    mma16816(d0, fa[0], fb[0][0], fb[0][1]);
+    mma16816(d1, fa[0], fb[0][2], fb[0][3]);
+    if (i + 1 >= n) break;
+    if (i + 2 < n) {
+      ldmatrix4(fa[0], pa + (i + 2) * 16, false);
+      ldmatrix4(fb[0], pb + (i + 2) * b_step, kAcross);
+    }
+    mma16816(e0, fa[1], fb[1][0], fb[1][1]);
+    mma16816(e1, fa[1], fb[1][2], fb[1][3]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    d0[j] += e0[j];
+    d1[j] += e1[j];
   }
 }
 
@@ -161,22 +191,30 @@ __global__ void __launch_bounds__(kSmallThreads, 1) hc_newton_small_kernel(const
   __shared__ double sums[kSmallThreads / 32];
   __half* hi = small;
   __half* lo = hi + p.rows * p.pitch;
-  __half* s = lo + p.rows * p.pitch;
+  __half* next = lo + p.rows * p.pitch;  // hi of the next step
+  __half* s = next + p.rows * p.pitch;
   __half* q = s + p.rows * p.s_pitch;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool tall = p.height > p.width;
   const T* g = static_cast<const T*>(p.g) + blockIdx.x * p.batch_stride;
   const int count = p.height * p.width;
+  // thread t has the values t, t + kSmallThreads, ... of the matrix
+  const int rows_on = kSmallThreads / p.width, columns_on = kSmallThreads % p.width, r_first = threadIdx.x / p.width, c_first = threadIdx.x % p.width;
   double sum = 0.0;
+  int r = r_first, c = c_first;
+#pragma unroll 8
   for (int i = threadIdx.x; i < count; i += kSmallThreads) {
-    const int r = i / p.width, c = i - r * p.width;
     const double v = (double)to_float(g[r * p.stride + c]);
     sum = fma(v, v, sum);
+    r += rows_on;
+    c += columns_on;
+    if (c >= p.width) c -= p.width, ++r;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sums[warp] = sum;
-  for (int i = threadIdx.x; i < p.rows * p.pitch * 2; i += kSmallThreads) small[i] = __float2half_rn(0.0f);  // also what rounds X up
+  if (p.side % 16 || p.length % 16)  // what rounds X up
+    for (int i = threadIdx.x; i < p.rows * p.pitch * 3 / 2; i += kSmallThreads) reinterpret_cast<uint32_t*>(small)[i] = 0u;
   __syncthreads();
   sum = 0.0;
   for (int w = 0; w < kSmallThreads / 32; ++w) sum += sums[w];
@@ -185,13 +223,17 @@ __global__ void __launch_bounds__(kSmallThreads, 1) hc_newton_small_kernel(const
   while (k < 126 && room * exp2((double)(k + 1)) <= 1.0) ++k;
   const float scale = exp2f((float)-k);
   const double factor = exp2((double)k) / (norm + (double)p.eps);
+  r = r_first, c = c_first;
+#pragma unroll 8
   for (int i = threadIdx.x; i < count; i += kSmallThreads) {
-    const int r = i / p.width, c = i - r * p.width;
     const float v = (float)((double)to_float(g[r * p.stride + c]) * factor);
     const __half h = __float2half_rn(v);
     const int at = tall ? c * p.pitch + r : r * p.pitch + c;
     hi[at] = h;
     lo[at] = __float2half_rn((v - __half2float(h)) * 2048.0f);
+    r += rows_on;
+    c += columns_on;
+    if (c >= p.width) c -= p.width, ++r;
   }
   __syncthreads();
   const int row_tiles = p.rows / 16, s_tiles = row_tiles * row_tiles, length = (p.length + 15) / 16 * 16, x_tiles = row_tiles * (length / 16);
@@ -222,23 +264,16 @@ __global__ void __launch_bounds__(kSmallThreads, 1) hc_newton_small_kernel(const
       }
     }
     __syncthreads();
-    float d[kSmallTiles][4];
-#pragma unroll
-    for (int i = 0; i < kSmallTiles / 2; ++i) {
-      const int t = warp + i * (kSmallThreads / 32);
-      if (t < x_tiles) small_product<true>(d[2 * i], d[2 * i + 1], q, p.s_pitch, hi, p.pitch, t % row_tiles * 16, t / row_tiles * 16, p.rows);
-    }
-    __syncthreads();  // nobody reads the old X any more
     const bool last = step == p.steps - 1;
-#pragma unroll
-    for (int i = 0; i < kSmallTiles / 2; ++i) {
-      const int t = warp + i * (kSmallThreads / 32);
-      if (t >= x_tiles) continue;
+#pragma unroll 1
+    for (int t = warp; t < x_tiles; t += kSmallThreads / 32) {
+      float d[2][4];
+      small_product<true>(d[0], d[1], q, p.s_pitch, hi, p.pitch, t % row_tiles * 16, t / row_tiles * 16, p.rows);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = t % row_tiles * 16 + r0 + (j >> 1) * 8, col = t / row_tiles * 16 + c0 + (j & 1) * 8, at = row * p.pitch + col;
         const float2 h = __half22float2(*reinterpret_cast<const __half2*>(hi + at)), l = __half22float2(*reinterpret_cast<const __half2*>(lo + at));
-        const float* v = d[2 * i + (j & 1)] + (j >> 1) * 2;
+        const float* v = d[j & 1] + (j >> 1) * 2;
         const float x0 = fmaf(p.a, fmaf(l.x, 1.0f / 2048.0f, h.x), v[0]), x1 = fmaf(p.a, fmaf(l.y, 1.0f / 2048.0f, h.y), v[1]);
         if (last) {
           __nv_bfloat16* out = p.out + (int64_t)blockIdx.x * count;
@@ -247,11 +282,14 @@ __global__ void __launch_bounds__(kSmallThreads, 1) hc_newton_small_kernel(const
         } else {
           const __half2 nh = __floats2half2_rn(x0, x1);
           const float2 f = __half22float2(nh);
-          *reinterpret_cast<__half2*>(hi + at) = nh;
+          *reinterpret_cast<__half2*>(next + at) = nh;
           *reinterpret_cast<__half2*>(lo + at) = __floats2half2_rn((x0 - f.x) * 2048.0f, (x1 - f.y) * 2048.0f);
         }
       }
     }
+    __half* old = hi;
+    hi = next;
+    next = old;
     __syncthreads();
   }
 }
@@ -262,7 +300,6 @@ namespace {
 
 struct Layout {
   int64_t ld, side, ld_side, parts;
-  int lanes;
   size_t x, s;  // bytes of one array of the size of X, and of S
   size_t total;
 };
@@ -272,10 +309,9 @@ Layout layout_of(size_t batch, size_t height, size_t width) {
   l.ld = (width + 7) / 8 * 8;
   l.side = height < width ? height : width;
   l.ld_side = (l.side + 7) / 8 * 8;
-  l.lanes = 1;
-  while (l.lanes < dev::kNormThreads && (size_t)l.lanes * 8 < width) l.lanes *= 2;
-  const size_t rows = dev::kNormThreads / l.lanes, most = (height + rows - 1) / rows, some = (1184 + batch - 1) / (batch ? batch : 1);
-  l.parts = most < some ? most : some;  // about eight blocks an SM
+  // blocks: about eight an SM, and no more than have four groups a thread
+  const size_t most = (height * (width + 7) / 8 + 4 * dev::kNormThreads - 1) / (4 * dev::kNormThreads), some = (1184 + batch - 1) / (batch ? batch : 1);
+  l.parts = most < some ? most : some;
   l.x = round_up(batch * height * l.ld * 2);
   l.s = round_up(batch * l.side * l.ld_side * 2);
   l.total = round_up(batch * l.parts * 8) + round_up(batch * 4) + 3 * l.x + 2 * l.s;
@@ -308,12 +344,13 @@ constexpr int kSmallSmem = 224 * 1024;
 bool small_plan(dev::SmallParams* p, size_t batch, size_t height, size_t width, int* smem) {
   const int64_t side = height < width ? height : width, length = height < width ? width : height;
   const int64_t rows = (side + 15) / 16 * 16, long_rows = (length + 15) / 16 * 16;
-  if (rows > 128 || rows / 16 * (long_rows / 16) > dev::kSmallThreads / 32 * (dev::kSmallTiles / 2)) return false;
+  if (long_rows > 4096) return false;
   // rows of 16 bytes more than a whole number of 32: eight rows of ldmatrix lie in different banks
   p->pitch = (int)long_rows + 8;
   p->s_pitch = (int)rows + 8;
-  *smem = (int)((2 * rows * p->pitch + 2 * rows * p->s_pitch) * 2);
-  if (*smem > kSmallSmem) return false;
+  const int64_t bytes = (3 * rows * p->pitch + 2 * rows * p->s_pitch) * 2;
+  if (bytes > kSmallSmem) return false;
+  *smem = (int)bytes;
   const int64_t sms = device_info().sms > 0 ? device_info().sms : 1, waves = ((int64_t)batch + sms - 1) / sms;
   const double flop = 2.0 * rows * rows * (2.0 * long_rows + rows);
   if (waves * flop / 1.2e6 > 14.0) return false;
@@ -371,7 +408,7 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   void* gram = at + 3 * l.x;
   void* poly = at + 3 * l.x + l.s;
   const dev::ScaleParams p = {g, partial, static_cast<__half*>(hi[0]), static_cast<__half*>(lo), scales, growth, (int64_t)height, (int64_t)width, (int64_t)stride,
-                              (int64_t)batch_stride, l.ld, (int)l.parts, l.lanes, eps};
+                              (int64_t)batch_stride, l.ld, (int)l.parts, eps};
   if (type == kF32) scale<float>(p, batch, stream);
   else if (type == kBf16) scale<__nv_bfloat16>(p, batch, stream);
   else scale<__half>(p, batch, stream);
