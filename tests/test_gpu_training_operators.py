@@ -1,0 +1,172 @@
+"""The operators of the training step together: the model that runs through them, its gradients, the Muon update, the trainer."""
+import argparse
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from mp_util import run_ranks
+from tirocinio_triennale_b200 import ops
+from tirocinio_triennale_b200.models import GPT2, GPT2Config, Muon, muon_with_adamw
+from tirocinio_triennale_b200.models.muon import Optimizers
+
+
+def _pair(**kw):
+    cfg = GPT2Config.tiny()
+    for k, v in kw.items():
+        setattr(cfg, k, v)
+    torch.manual_seed(0)
+    plain = GPT2(cfg).cuda()
+    cfg = copy.copy(cfg)
+    cfg.fused = True
+    fused = GPT2(cfg).cuda()
+    fused.load_state_dict(plain.state_dict())
+    return plain.double(), fused
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [dict(), dict(d_model=96, n_head=3, vocab_size=1001, n_layer=1), dict(d_model=128, n_head=4, vocab_size=50257)])
+def test_model_through_the_operators(shape):
+    """Each of the two layers rounds some 8 tensors to bf16 on the way forward and as many on the way back, the head 4 and 4: 40
+    roundings of at most 2^-8 each, in relative 2-norm."""
+    plain, fused = _pair(**shape)
+    room = 40 * 2.0 ** -8
+    g = torch.Generator().manual_seed(1)
+    tok = torch.randint(0, plain.cfg.vocab_size, (3, 33), generator=g).cuda()
+    idx, targets = tok[:, :-1], tok[:, 1:].clone()
+    targets[0, :5] = -100
+    logits = fused(idx)
+    want = plain(idx)
+    assert logits.dtype == torch.bfloat16 and (logits.double() - want).norm() <= room * want.norm()
+    loss = fused(idx, targets)
+    loss.backward()
+    exact = F.cross_entropy(want.reshape(-1, want.shape[-1]), targets.reshape(-1))
+    exact.backward()
+    assert abs(loss.item() - exact.item()) <= room * exact.item()
+    for (name, p), q in zip(fused.named_parameters(), plain.parameters()):
+        assert p.grad.dtype == p.dtype == torch.float32 and p.grad.shape == p.shape
+        # a key's bias moves all scores of a query alike: its gradient is 0, and what stands there is rounding alone
+        scale = q.grad.norm() if not name.endswith("qkv.bias") else fused.blocks[0].qkv.weight.grad.double().norm()
+        assert (p.grad.double() - q.grad).norm() <= room * scale, name
+    assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+def test_model_in_a_graph():
+    """A step's forward and backward pass captured and replayed on other tokens gives what it gives outside."""
+    _, model = _pair()
+    tok = torch.randint(0, 257, (2, 33), generator=torch.Generator().manual_seed(2)).cuda()
+
+    def step():
+        model.zero_grad(set_to_none=True)
+        loss = model(tok[:, :-1], tok[:, 1:])
+        loss.backward()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    model.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caught = step()
+    tok.copy_(tok.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    grads = [p.grad.clone() for p in model.parameters()]
+    caught = caught.clone()
+    for p in model.parameters():
+        p.grad = None
+    assert torch.equal(step(), caught)
+    assert all((a - p.grad).norm() <= 1e-2 * a.norm() for a, p in zip(grads, model.parameters()))  # torch's attention may add in any order
+
+
+def _reference_step(p, g, m, lr, momentum, decay, nesterov):
+    m = momentum * m + g
+    u = g + momentum * m if nesterov else m
+    a, b, c = 3.4445, -4.7750, 2.0315
+    x = u / (u.norm() + 1e-7)
+    for _ in range(5):
+        s = x @ x.T
+        x = a * x + (b * s + c * s @ s) @ x
+    return p * (1 - lr * decay) - lr * max(1.0, p.shape[0] / p.shape[1]) ** 0.5 * x, m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_against_the_formulas(nesterov):
+    g = torch.Generator().manual_seed(3)
+    shapes = [(48, 96), (96, 48), (48, 96), (200, 130), (33, 7)]
+    params = [torch.nn.Parameter(torch.randn(*s, generator=g).cuda()) for s in shapes]
+    want = [(p.detach().double(), torch.zeros_like(p).double()) for p in params]
+    opt = Muon(params, lr=0.05, momentum=0.9, weight_decay=0.1, nesterov=nesterov)
+    for _ in range(3):
+        for i, p in enumerate(params):
+            p.grad = torch.randn(*shapes[i], generator=g).cuda()
+            want[i] = _reference_step(want[i][0], p.grad.double(), want[i][1], 0.05, 0.9, 0.1, nesterov)
+        opt.step()
+    for p, (w, m) in zip(params, want):
+        assert (opt.state[p]["momentum"].double() - m).norm() <= 1e-6 * m.norm()
+        # three updates, each within 5.7e-3 of its norm (that of the iteration's test) and of norm lr sqrt(rank) sqrt(height / width)
+        size = 3 * 0.05 * min(p.shape) ** 0.5 * max(1.0, p.shape[0] / p.shape[1]) ** 0.5 * 1.2
+        assert (p.detach().double() - w).norm() <= 8e-3 * size
+
+
+@pytest.mark.gpu
+def test_muon_with_adamw_state_and_refusals():
+    _, model = _pair()
+    opt = muon_with_adamw(model)
+    muon, adam = opt.optimizers
+    assert len(muon.param_groups[0]["params"]) == 8 and all(p.dim() == 2 for p in muon.param_groups[0]["params"])
+    held = {id(p) for o in (muon, adam) for gr in o.param_groups for p in gr["params"]}
+    assert held == {id(p) for p in model.parameters()} and id(model.wte.weight) in {id(p) for p in adam.param_groups[0]["params"]}
+    tok = torch.randint(0, 257, (2, 33), generator=torch.Generator().manual_seed(4)).cuda()
+    for _ in range(2):
+        opt.zero_grad()
+        model(tok[:, :-1], tok[:, 1:]).backward()
+        opt.step()
+    assert all(torch.isfinite(p).all() for p in model.parameters())
+    again = muon_with_adamw(model)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    p = muon.param_groups[0]["params"][0]
+    assert torch.equal(again.optimizers[0].state[p]["momentum"], muon.state[p]["momentum"])
+    with pytest.raises(ValueError):
+        again.load_state_dict(opt.state_dict()[:1])
+    opt.zero_grad()
+    opt.step()  # without gradients nothing moves
+
+
+def test_refusals_without_a_gpu():
+    with pytest.raises(ValueError):
+        Muon([torch.nn.Parameter(torch.zeros(3))])
+    with pytest.raises(ValueError):
+        Muon([torch.nn.Parameter(torch.zeros(3, 3))], momentum=1.0)
+    cfg = GPT2Config.tiny()
+    cfg.fused = True
+    with pytest.raises(ValueError, match="CUDA"):
+        GPT2(cfg)(torch.zeros(1, 4, dtype=torch.int64))
+    p = torch.nn.Parameter(torch.zeros(3, 3))
+    p.grad = torch.zeros(3, 3)
+    with pytest.raises(ValueError, match="CUDA"):
+        Optimizers(Muon([p])).step()
+
+
+def _trainer(rank, world):
+    from tirocinio_triennale_b200.models import train_dp
+
+    args = argparse.Namespace(model="tiny", steps=3, warmup=1, batch=2, seq=32, eb=1e-6, lr=1e-3, bucket_mb=0.05, cpu=False, save=None, resume=None,
+                              save_compressed_eb=0.0, fused=True, optimizer="muon", muon_lr=0.02)
+    for compressed in (True, False):
+        out = train_dp.run(args, compressed, rank, world, torch.device("cuda", 0))
+        assert out["steps_done"] == 4 and out["last_loss_rank0"] == out["last_loss_rank0"]
+        assert not compressed or out["compressed_calls"] > 0
+    assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+def test_trainer_with_the_operators_and_compressed_gradients():
+    run_ranks(_trainer, 1, backend="nccl")

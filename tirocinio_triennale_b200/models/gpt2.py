@@ -1,7 +1,12 @@
 """GPT-2-shaped decoder (12 layers, d_model 768, 12 heads, vocab 50257 for "small") used by the
 data-parallel benchmark: random-init weights, uniform random token ids.  Plain PyTorch modules
 (bf16 autocast, fused scaled-dot-product attention); the point of the benchmark is the gradient
-allreduce, which is this library's compressed collective."""
+allreduce, which is this library's compressed collective.
+
+With ``GPT2Config.fused`` the same weights run through this library's operators on a CUDA device:
+the residual stream stays float32, norms give bfloat16 rows to the products, bias, GELU and residual
+are added where a product is stored, and the loss takes one pass over the logits and one for their
+gradient (``ops.layer_norm``, ``ops.linear``, ``ops.token_logprobs``).  No autocast is needed."""
 from __future__ import annotations
 
 import math
@@ -10,6 +15,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .. import ops
 
 
 @dataclass
@@ -20,6 +27,7 @@ class GPT2Config:
     vocab_size: int = 50257
     seq_len: int = 1024
     dropout: float = 0.0
+    fused: bool = False  # this library's operators in place of torch's (CUDA, float32 weights, bfloat16 products)
 
     @staticmethod
     def small():
@@ -28,6 +36,14 @@ class GPT2Config:
     @staticmethod
     def tiny():
         return GPT2Config(n_layer=2, n_head=2, d_model=64, vocab_size=257, seq_len=32)
+
+
+def _norm(x, m: nn.LayerNorm):
+    return ops.layer_norm(x, m.weight, m.bias, eps=m.eps, out_dtype=torch.bfloat16)
+
+
+def _linear(x, m: nn.Linear, **kw):
+    return ops.linear(x, m.weight.to(torch.bfloat16), m.bias, **kw)
 
 
 class Block(nn.Module):
@@ -40,14 +56,18 @@ class Block(nn.Module):
         self.fc = nn.Linear(cfg.d_model, 4 * cfg.d_model)
         self.out = nn.Linear(4 * cfg.d_model, cfg.d_model)
         self.n_head = cfg.n_head
+        self.fused = cfg.fused
 
     def forward(self, x):
         B, T, C = x.shape
-        q, k, v = self.qkv(self.ln1(x)).split(C, dim=2)
+        q, k, v = (_linear(_norm(x, self.ln1), self.qkv) if self.fused else self.qkv(self.ln1(x))).split(C, dim=2)
         q = q.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
         k = k.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
         v = v.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        if self.fused:
+            x = _linear(a.transpose(1, 2).reshape(B, T, C), self.proj, residual=x)
+            return _linear(_linear(_norm(x, self.ln2), self.fc, activation="gelu_tanh"), self.out, residual=x)
         x = x + self.proj(a.transpose(1, 2).reshape(B, T, C))
         return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
 
@@ -78,6 +98,12 @@ class GPT2(nn.Module):
         x = self.wte(idx) + self.wpe(pos)
         for b in self.blocks:
             x = b(x)
+        if self.cfg.fused:
+            logits = ops.linear(_norm(x, self.ln_f), self.wte.weight.to(torch.bfloat16))
+            if targets is None:
+                return logits
+            kept = (targets != -100).sum()  # as cross_entropy leaves rows out
+            return -ops.token_logprobs(logits, targets).logprobs.sum() / kept
         logits = F.linear(self.ln_f(x), self.wte.weight)  # tied output embedding
         if targets is None:
             return logits

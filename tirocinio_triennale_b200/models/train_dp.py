@@ -8,6 +8,9 @@ library's compressed allreduce through the DDP communication hook, overlapped wi
 side stream, and (b) with plain NCCL.  Prints one JSON line with tokens/s of both runs and the loss
 gap after the last step.  Random-init weights, uniform random token ids (no dataset, no download).
 
+``--fused`` runs the model through this library's operators (layer norm, products with their epilogues, the
+loss over the logits); ``--optimizer muon`` orthogonalises the updates of the blocks' matrices.
+
 ``--save PATH`` writes model, optimiser, step count and the data generator's state after the last
 step (rank 0; one file per arm: PATH.compressed / PATH.nccl); ``--resume PATH`` continues from such
 files, bit for bit the run that was never interrupted.  ``--save-compressed-eb EB`` additionally
@@ -26,12 +29,14 @@ from torch.nn.parallel import DistributedDataParallel as DDP
 
 from ..parallel import CompressedHookState, compressed_allreduce_hook
 from .gpt2 import GPT2, GPT2Config
+from .muon import muon_with_adamw
 
 
 def run(args, compressed: bool, rank: int, world: int, device):
     torch.manual_seed(1234)
     cfg = GPT2Config.small() if args.model == "small" else GPT2Config.tiny()
     cfg.seq_len = args.seq
+    cfg.fused = getattr(args, "fused", False)
     model = GPT2(cfg).to(device)
     ddp = DDP(model, device_ids=[device.index] if device.type == "cuda" else None, bucket_cap_mb=args.bucket_mb,
               gradient_as_bucket_view=True)
@@ -39,7 +44,10 @@ def run(args, compressed: bool, rank: int, world: int, device):
     if compressed:
         state = CompressedHookState(eb=args.eb, max_bucket_elems=int(args.bucket_mb * 1.5 * 1024 * 1024 / 4) + (1 << 20))
         ddp.register_comm_hook(state, compressed_allreduce_hook)
-    opt = torch.optim.AdamW(ddp.parameters(), lr=args.lr, weight_decay=0.0, fused=device.type == "cuda")
+    if getattr(args, "optimizer", "adamw") == "muon":
+        opt = muon_with_adamw(model, lr=args.muon_lr, adam_lr=args.lr)
+    else:
+        opt = torch.optim.AdamW(ddp.parameters(), lr=args.lr, weight_decay=0.0, fused=device.type == "cuda")
     g = torch.Generator(device="cpu").manual_seed(100 + rank)
     arm = "compressed" if compressed else "nccl"
     start = 0
@@ -99,6 +107,9 @@ def main(argv=None):
     ap.add_argument("--seq", type=int, default=1024)
     ap.add_argument("--eb", type=float, default=1e-5)
     ap.add_argument("--lr", type=float, default=3e-4)
+    ap.add_argument("--fused", action="store_true", help="this library's operators in the model")
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"])
+    ap.add_argument("--muon-lr", type=float, default=0.02)
     ap.add_argument("--bucket-mb", type=float, default=25.0)
     ap.add_argument("--cpu", action="store_true", help="gloo + host-rank ring (functional check without GPUs)")
     ap.add_argument("--save", default=None, help="checkpoint prefix written after the last step")
@@ -106,6 +117,8 @@ def main(argv=None):
     ap.add_argument("--save-compressed-eb", type=float, default=0.0,
                     help="also write the weights as error-bounded streams with this absolute bound")
     args = ap.parse_args(argv)
+    if args.cpu and (args.fused or args.optimizer == "muon"):
+        ap.error("--fused and --optimizer muon need a GPU")
 
     rank = int(os.environ.get("RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))
