@@ -23,6 +23,7 @@ constexpr int kBM = 128, kBK = 64;  // rows of a CTA, part of the sum in a stage
 constexpr int kStoreWarps = 8;
 constexpr int kGemmThreads = 64 + 32 * kStoreWarps;
 constexpr int kOperandA = kBM * kBK * 2;
+constexpr int kGemmLinearWide = 4;  // kGemmLinear with a result in fp32
 constexpr uint64_t kGemmLimitNs = 2000ull * 1000 * 1000;
 
 struct GemmParams {
@@ -64,7 +65,7 @@ struct GemmShape {
 };
 
 struct GemmBarriers {
-  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained;
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained, stage_done, stage_go;
   uint64_t loaded[kStoreWarps][2];
   alignas(16) float bias[kStoreWarps][32];
   uint32_t tmem;
@@ -339,15 +340,275 @@ __device__ __forceinline__ void gemm_fetch(const GemmParams& p, int z, int row0,
   if (MODE == kGemmUpdate) load_box<1>(slot + kSlot / 2, &p.map_in2, col0, row0, z, smem_u32(bar));
 }
 
+// What the three roles carry from tile to tile (and, in a chain of products, from one to the next).
+struct Loading {
+  int s = 0, issued = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+};
+struct Multiplying {
+  int s = 0, acc = 0;
+  uint32_t phase = 0, acc_phase = 0;
+  bool ok = true;
+};
+struct Storing {
+  int acc = 0;
+  uint32_t acc_phase = 0, uses = 0;  // uses: pieces so far, which take the two slots in turn
+  uint32_t phases = 0;               // of the slots' barriers, a bit each
+  int on_their_way = 0;              // pieces that have been asked for and not been waited for
+  bool ok = true;
+};
+// A result in fp32 gets its sum in parts of 512: the tensor core does not round to nearest when it adds to an accumulator, and
+// what that loses over a whole sum (6e-6 of the result over 8192) is ten times what fp32 additions do.
+constexpr int kChunk = 8;  // stages
+
 template <int BN, int kCtas, int MODE>
-__global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_constant__ GemmParams p) {
+__device__ __forceinline__ void load_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* stages, Loading& st, int unit, int units, int rank) {
   using S = GemmShape<BN, kCtas>;
-  extern __shared__ unsigned char raw[];
-  __shared__ GemmBarriers sh;
-  unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int total = p.tiles * p.batch;
+  for (int t = unit; st.ok && t < total; t += units) {
+    const int z = t / p.tiles;
+    int mi, ni;
+    tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
+    const int row = mi * S::kRows + rank * kBM, col = ni * BN + rank * S::kB;
+    const int zz = p.parts > 1 ? 0 : z, k0 = p.parts > 1 ? z * p.k_blocks : 0;
+    for (int kb = 0; kb < p.k_blocks; ++kb) {
+      const int k = (k0 + kb) * kBK;
+      if (!gemm_wait(&sh.empty[st.s], st.phase ^ 1, sh)) {
+        st.ok = false;
+        break;
+      }
+      unsigned char* a = stages + st.s * S::kStage;
+      unsigned char* b = a + kOperandA;
+      const uint32_t bar = kCtas == 2 ? leader_address(&sh.full[st.s]) : smem_u32(&sh.full[st.s]);
+      if (rank == 0) mbar_expect_tx(&sh.full[st.s], S::kStage * kCtas);
+      if (p.a_across) {
+        for (int i = 0; i < kBM / 64; ++i) load_box<kCtas>(a + i * 8192, &p.map_a, row + i * 64, k, zz, bar);
+      } else {
+        load_box<kCtas>(a, &p.map_a, k, row, zz, bar);
+      }
+      if (p.b_across) {
+        for (int i = 0; i < S::kB / 64; ++i) load_box<kCtas>(b + i * 8192, &p.map_b, col + i * 64, k, zz, bar);
+      } else {
+        load_box<kCtas>(b, &p.map_b, k, col, zz, bar);
+      }
+      ++st.issued;
+      if (++st.s == S::kStages) {
+        st.s = 0;
+        st.phase ^= 1;
+      }
+    }
+  }
+}
+// Copies in flight land before the CTA leaves.  Those of a pair are counted at its first CTA; the second one leaves behind it,
+// and after a wait that ran out, when they may differ in what they have issued, a millisecond later.
+template <int BN, int kCtas>
+__device__ __forceinline__ void load_end(GemmBarriers& sh, const Loading& st, int rank) {
+  using S = GemmShape<BN, kCtas>;
+  if (rank == 0) {
+    for (int back = 0; back < S::kStages && back < st.issued; ++back) {
+      const int i = st.issued - 1 - back;
+      mbar_wait_bounded(&sh.full[i % S::kStages], (i / S::kStages) & 1, kGemmLimitNs);
+    }
+  } else if (!st.ok) {
+    const long long t0 = clock64();
+    for (int i = 0; i < (1 << 22) && clock64() - t0 < 2000000; ++i) {
+    }
+  }
+}
+
+template <int BN, int kCtas, int MODE>
+__device__ __forceinline__ void multiply_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* stages, Multiplying& st, uint32_t tmem, int unit, int units) {
+  using S = GemmShape<BN, kCtas>;
+  const int total = p.tiles * p.batch;
+  for (int t = unit; st.ok && t < total; t += units) {
+    for (int begin = 0; begin < p.k_blocks; begin += kChunk) {
+      const int end = MODE == kGemmLinearWide ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
+      if (!gemm_wait(&sh.acc_empty[st.acc], st.acc_phase ^ 1, sh)) {
+        st.ok = false;
+        return;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + st.acc * BN;
+      for (int kb = begin; kb < end; ++kb) {
+        if (!gemm_wait(&sh.full[st.s], st.phase, sh)) {
+          st.ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = smem_u32(stages + st.s * S::kStage);
+        const uint64_t da = p.desc_a | (uint64_t)((a & 0x3ffff) >> 4), db = p.desc_b | (uint64_t)(((a + kOperandA) & 0x3ffff) >> 4);
+#pragma unroll
+        for (int i = 0; i < kBK / 16; ++i) tc_mma<kCtas>(d, da + i * p.step_a, db + i * p.step_b, p.idesc, kb > begin || i > 0);
+        tc_commit<kCtas>(&sh.empty[st.s]);
+        if (++st.s == S::kStages) {
+          st.s = 0;
+          st.phase ^= 1;
+        }
+      }
+      tc_commit<kCtas>(&sh.acc_full[st.acc]);
+      if (++st.acc == 2) {
+        st.acc = 0;
+        st.acc_phase ^= 1;
+      }
+      if (!st.ok || end == p.k_blocks) break;
+    }
+  }
+}
+
+// the accumulator has been read
+template <int kCtas>
+__device__ __forceinline__ void release_accumulator(GemmBarriers& sh, Storing& st, int rank) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    if (rank == 0) mbar_arrive(&sh.acc_empty[st.acc]);
+    else
+      asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_address(&sh.acc_empty[st.acc])) : "memory");
+  }
+  if (++st.acc == 2) {
+    st.acc = 0;
+    st.acc_phase ^= 1;
+  }
+}
+
+template <int BN, int kCtas, int MODE>
+__device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* mine, Storing& st, uint32_t tmem, int unit, int units, int rank) {
+  using S = GemmShape<BN, kCtas>;
+  constexpr bool kWide = MODE == kGemmLinearWide, kLinear = MODE == kGemmLinear || kWide, kSymmetric = MODE == kGemmGram || MODE == kGemmPoly;
+  constexpr int kMode = kLinear ? kGemmLinear : MODE;
+  constexpr int kPieces = kWide ? (BN / 32 + 1) / 2 : 1;  // of a warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = kCtas == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair; the first one issues the matrix instructions
-  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
+  const int quarter = warp & 3;      // the rows of tensor memory that this warp can reach
+  const int half = (warp - 2) >> 2;  // every second piece of 32 columns
+  const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+  uint64_t* loaded = sh.loaded[warp - 2];
+  float* shared_bias = sh.bias[warp - 2];
+  const bool fetches = MODE == kGemmPoly || MODE == kGemmUpdate || (kLinear && p.tma_in);
+  const int total = p.tiles * p.batch;
+  for (int t = unit; t < total; t += units) {
+    const int z = t / p.tiles;
+    int mi, ni;
+    tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
+    const int row0 = mi * S::kRows + rank * kBM + quarter * 32, col0 = ni * BN;
+    // pieces of these rows that hold something (of a symmetric result: at the diagonal of blocks of 32, or below it)
+    int pieces = row0 < p.m ? (int)min((int64_t)(BN / 32), (p.n - col0 + 31) / 32) : 0;
+    if (kSymmetric && pieces) pieces = min(pieces, row0 / 32 - col0 / 32 + 1);
+    float bias = 0.0f;
+    if (half < pieces) {
+      if (fetches && lane == 0) {
+        tma_wait_group_read<0>();
+        gemm_fetch<kMode>(p, z, row0, col0 + half * 32, mine + (st.uses & 1) * kSlot, &loaded[st.uses & 1]);
+        ++st.on_their_way;
+      }
+      if (kLinear && p.bias && col0 + half * 32 + lane < p.n) bias = param_at(p.bias, p.bias_type, col0 + half * 32 + lane);
+    }
+    float sums[kPieces][32];
+    if (kWide) {
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sums[q][j] = 0.0f;
+      for (int begin = 0; begin < p.k_blocks; begin += kChunk) {
+        if (!__all_sync(0xffffffffu, gemm_wait(&sh.acc_full[st.acc], st.acc_phase, sh))) {
+          st.ok = false;
+          return;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q) {
+          if (half + 2 * q >= pieces) break;
+          float v[32];
+          __syncwarp();
+          tc_load32(lanes + st.acc * BN + (half + 2 * q) * 32, v);
+          tc_load_wait(v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sums[q][j] += v[j];
+        }
+        release_accumulator<kCtas>(sh, st, rank);
+      }
+    } else {
+      if (!__all_sync(0xffffffffu, gemm_wait(&sh.acc_full[st.acc], st.acc_phase, sh))) {
+        st.ok = false;
+        return;
+      }
+      tc_fence_after();
+    }
+    const auto piece = [&](int c, float (&v)[32]) {  // false: a wait ran out
+      const int col = col0 + c * 32;
+      unsigned char* slot = mine + (st.uses & 1) * kSlot;
+      float next_bias = 0.0f;
+      if (c + 2 < pieces) {
+        if (fetches && lane == 0) {
+          tma_wait_group_read<0>();
+          gemm_fetch<kMode>(p, z, row0, col + 64, mine + ((st.uses + 1) & 1) * kSlot, &loaded[(st.uses + 1) & 1]);
+          ++st.on_their_way;
+        }
+        if (kLinear && p.bias && col + 64 + lane < p.n) next_bias = param_at(p.bias, p.bias_type, col + 64 + lane);
+      }
+      if (!fetches && lane == 0) tma_wait_group_read<1>();
+      __syncwarp();
+      if (!kWide) {
+        tc_load32(lanes + st.acc * BN + c * 32, v);
+        tc_load_wait(v);
+      }
+      if (fetches) {
+        const uint32_t slot_number = st.uses & 1;
+        if (!__all_sync(0xffffffffu, gemm_wait(&loaded[slot_number], st.phases >> slot_number & 1, sh))) return false;
+        st.phases ^= 1u << slot_number;
+        --st.on_their_way;
+      }
+      const bool mirror = kSymmetric && col / 32 < row0 / 32;
+      gemm_finish<kMode>(p, z, row0, col, v, slot, bias, shared_bias, mirror);
+      bias = next_bias;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        if (p.tma_out) tma_store_3d(&p.map_out, col, row0, z, slot);
+        if (p.tma_out2) tma_store_3d(&p.map_out2, col, row0, z, slot + kSlot / 2);
+        if (mirror) tma_store_3d(&p.map_mirror, row0, col, z, slot + kSlot / 2);
+        tma_commit_group();
+      }
+      ++st.uses;
+      return true;
+    };
+    if (kWide) {
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q) {
+        if (half + 2 * q >= pieces) break;
+        if (!piece(half + 2 * q, sums[q])) {
+          st.ok = false;
+          return;
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int c = half; c < pieces; c += 2) {
+        if (!piece(c, sums[0])) {
+          st.ok = false;
+          return;
+        }
+      }
+      release_accumulator<kCtas>(sh, st, rank);
+    }
+  }
+}
+// what was fetched and not used (after a wait that ran out) lands before the CTA leaves, and all stores have read what they
+// take from its shared memory
+__device__ __forceinline__ void store_end(GemmBarriers& sh, Storing& st) {
+  if ((threadIdx.x & 31) != 0) return;
+  uint64_t* loaded = sh.loaded[(threadIdx.x >> 5) - 2];
+  for (; st.on_their_way > 0; --st.on_their_way, ++st.uses) {
+    mbar_wait_bounded(&loaded[st.uses & 1], st.phases >> (st.uses & 1) & 1, kGemmLimitNs);
+    st.phases ^= 1u << (st.uses & 1);
+  }
+  tma_wait_group_read<0>();
+}
+
+// barriers and tensor memory; by all threads
+template <int BN, int kCtas>
+__device__ __forceinline__ void gemm_begin(GemmBarriers& sh) {
+  using S = GemmShape<BN, kCtas>;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -358,16 +619,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
       mbar_init(&sh.acc_empty[a], kStoreWarps * kCtas);
     }
     mbar_init(&sh.drained, 1);
+    mbar_init(&sh.stage_done, kStoreWarps);
+    mbar_init(&sh.stage_go, 1);
     for (int w = 0; w < kStoreWarps; ++w) {
       mbar_init(&sh.loaded[w][0], 1);
       mbar_init(&sh.loaded[w][1], 1);
     }
     sh.gave_up = 0;
     fence_mbar_init();
-    tma_prefetch_map(&p.map_a);
-    tma_prefetch_map(&p.map_b);
   }
-  if (warp == 1) {
+  if (threadIdx.x >> 5 == 1) {
     if (kCtas == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(S::kColumns) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -380,188 +641,148 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_c
   __syncthreads();
   if (kCtas == 2) cluster_sync();  // the other CTA's barriers are there
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
-  const int total = p.tiles * p.batch;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      int issued = 0;
-      for (int t = unit; ok && t < total; t += units) {
-        const int z = t / p.tiles;
-        int mi, ni;
-        tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
-        const int row = mi * S::kRows + rank * kBM, col = ni * BN + rank * S::kB;
-        const int zz = p.parts > 1 ? 0 : z, k0 = p.parts > 1 ? z * p.k_blocks : 0;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          const int k = (k0 + kb) * kBK;
-          if (!gemm_wait(&sh.empty[s], phase ^ 1, sh)) {
-            ok = false;
-            break;
-          }
-          unsigned char* a = stages + s * S::kStage;
-          unsigned char* b = a + kOperandA;
-          const uint32_t bar = kCtas == 2 ? leader_address(&sh.full[s]) : smem_u32(&sh.full[s]);
-          if (rank == 0) mbar_expect_tx(&sh.full[s], S::kStage * kCtas);
-          if (p.a_across) {
-            for (int i = 0; i < kBM / 64; ++i) load_box<kCtas>(a + i * 8192, &p.map_a, row + i * 64, k, zz, bar);
-          } else {
-            load_box<kCtas>(a, &p.map_a, k, row, zz, bar);
-          }
-          if (p.b_across) {
-            for (int i = 0; i < S::kB / 64; ++i) load_box<kCtas>(b + i * 8192, &p.map_b, col + i * 64, k, zz, bar);
-          } else {
-            load_box<kCtas>(b, &p.map_b, k, col, zz, bar);
-          }
-          ++issued;
-          if (++s == S::kStages) {
-            s = 0;
-            phase ^= 1;
-          }
-        }
-      }
-      // Copies in flight land before the CTA leaves.  Those of a pair are counted at its first CTA; the second one leaves
-      // behind it, and after a wait that ran out, when they may differ in what they have issued, a millisecond later.
-      if (rank == 0) {
-        for (int back = 0; back < S::kStages && back < issued; ++back) {
-          const int i = issued - 1 - back;
-          mbar_wait_bounded(&sh.full[i % S::kStages], (i / S::kStages) & 1, kGemmLimitNs);
-        }
-      } else if (!ok) {
-        const long long t0 = clock64();
-        for (int i = 0; i < (1 << 22) && clock64() - t0 < 2000000; ++i) {
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int s = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int t = unit; ok && t < total; t += units) {
-        if (!gemm_wait(&sh.acc_empty[acc], acc_phase ^ 1, sh)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + acc * BN;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!gemm_wait(&sh.full[s], phase, sh)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a = smem_u32(stages + s * S::kStage);
-          const uint64_t da = p.desc_a | (uint64_t)((a & 0x3ffff) >> 4), db = p.desc_b | (uint64_t)(((a + kOperandA) & 0x3ffff) >> 4);
-#pragma unroll
-          for (int i = 0; i < kBK / 16; ++i) tc_mma<kCtas>(d, da + i * p.step_a, db + i * p.step_b, p.idesc, kb > 0 || i > 0);
-          tc_commit<kCtas>(&sh.empty[s]);
-          if (++s == S::kStages) {
-            s = 0;
-            phase ^= 1;
-          }
-        }
-        tc_commit<kCtas>(&sh.acc_full[acc]);
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
-      }
-      // so do the matrix instructions
-      tc_commit<kCtas>(&sh.drained);
-      mbar_wait_bounded(&sh.drained, 0, kGemmLimitNs);
-    }
-  } else {
-    int acc = 0;
-    uint32_t acc_phase = 0, uses = 0;  // pieces so far
-    const int quarter = warp & 3;      // the rows of tensor memory that this warp can reach
-    const int half = (warp - 2) >> 2;  // every second piece of 32 columns
-    unsigned char* mine = stages + S::kStages * S::kStage + (warp - 2) * kWarpStage;
-    uint64_t* loaded = sh.loaded[warp - 2];
-    float* shared_bias = sh.bias[warp - 2];
-    const bool fetches = MODE == kGemmPoly || MODE == kGemmUpdate || (MODE == kGemmLinear && p.tma_in);
-    constexpr bool kSymmetric = MODE == kGemmGram || MODE == kGemmPoly;
-    uint32_t fetched = 0;
-    for (int t = unit; t < total; t += units) {
-      const int z = t / p.tiles;
-      int mi, ni;
-      tile_place<BN, S::kRows, MODE>(p, t - z * p.tiles, mi, ni);
-      const int row0 = mi * S::kRows + rank * kBM + quarter * 32, col0 = ni * BN;
-      // pieces of these rows that hold something (of a symmetric result: at the diagonal of blocks of 32, or below it)
-      int pieces = row0 < p.m ? (int)min((int64_t)(BN / 32), (p.n - col0 + 31) / 32) : 0;
-      if (kSymmetric && pieces) pieces = min(pieces, row0 / 32 - col0 / 32 + 1);
-      float bias = 0.0f;
-      if (half < pieces) {
-        if (fetches && lane == 0) {
-          tma_wait_group_read<0>();
-          gemm_fetch<MODE>(p, z, row0, col0 + half * 32, mine + (uses & 1) * kSlot, &loaded[uses & 1]);
-          ++fetched;
-        }
-        if (MODE == kGemmLinear && p.bias && col0 + half * 32 + lane < p.n) bias = param_at(p.bias, p.bias_type, col0 + half * 32 + lane);
-      }
-      const bool ok = gemm_wait(&sh.acc_full[acc], acc_phase, sh);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      bool good = true;
-#pragma unroll 1
-      for (int c = half; c < pieces; c += 2, ++uses) {
-        const int col = col0 + c * 32;
-        unsigned char* slot = mine + (uses & 1) * kSlot;
-        float next_bias = 0.0f;
-        if (c + 2 < pieces) {
-          if (fetches && lane == 0) {
-            tma_wait_group_read<0>();
-            gemm_fetch<MODE>(p, z, row0, col + 64, mine + ((uses + 1) & 1) * kSlot, &loaded[(uses + 1) & 1]);
-            ++fetched;
-          }
-          if (MODE == kGemmLinear && p.bias && col + 64 + lane < p.n) next_bias = param_at(p.bias, p.bias_type, col + 64 + lane);
-        }
-        if (!fetches && lane == 0) tma_wait_group_read<1>();
-        __syncwarp();
-        float v[32];
-        tc_load32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + c * 32, v);
-        tc_load_wait(v);
-        if (fetches) good = __all_sync(0xffffffffu, gemm_wait(&loaded[uses & 1], (uses >> 1) & 1, sh));
-        if (!good) break;
-        const bool mirror = kSymmetric && col / 32 < row0 / 32;
-        gemm_finish<MODE>(p, z, row0, col, v, slot, bias, shared_bias, mirror);
-        bias = next_bias;
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-          if (p.tma_out) tma_store_3d(&p.map_out, col, row0, z, slot);
-          if (p.tma_out2) tma_store_3d(&p.map_out2, col, row0, z, slot + kSlot / 2);
-          if (mirror) tma_store_3d(&p.map_mirror, row0, col, z, slot + kSlot / 2);
-          tma_commit_group();
-        }
-      }
-      if (!good) break;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (rank == 0) mbar_arrive(&sh.acc_empty[acc]);
-        else
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_address(&sh.acc_empty[acc])) : "memory");
-      }
-      if (++acc == 2) {
-        acc = 0;
-        acc_phase ^= 1;
-      }
-    }
-    if (lane == 0) {
-      // what was fetched and not used (after a wait that ran out) lands before the CTA leaves, and all stores have read what
-      // they take from its shared memory
-      for (; uses < fetched; ++uses) mbar_wait_bounded(&loaded[uses & 1], (uses >> 1) & 1, kGemmLimitNs);
-      tma_wait_group_read<0>();
-    }
-  }
+}
+template <int BN, int kCtas>
+__device__ __forceinline__ void gemm_end(uint32_t tmem) {
+  using S = GemmShape<BN, kCtas>;
   __syncthreads();
   if (kCtas == 2) cluster_sync();  // nobody leaves while the other one's memory is read or its barriers are used
-  if (warp == 1) {
+  if (threadIdx.x >> 5 == 1) {
     __syncwarp();
     tc_fence_after();
     if (kCtas == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kColumns));
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kColumns));
   }
+}
+__device__ __forceinline__ unsigned char* gemm_stages(unsigned char* raw) {
+  return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+}
+
+template <int BN, int kCtas, int MODE>
+__global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_kernel(const __grid_constant__ GemmParams p) {
+  using S = GemmShape<BN, kCtas>;
+  extern __shared__ unsigned char raw[];
+  __shared__ GemmBarriers sh;
+  unsigned char* stages = gemm_stages(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kCtas == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair; the first one issues the matrix instructions
+  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&p.map_a);
+    tma_prefetch_map(&p.map_b);
+  }
+  gemm_begin<BN, kCtas>(sh);
+  const uint32_t tmem = sh.tmem;
+  if (warp == 0) {
+    if (lane == 0) {
+      Loading st;
+      load_tiles<BN, kCtas, MODE>(p, sh, stages, st, unit, units, rank);
+      load_end<BN, kCtas>(sh, st, rank);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      Multiplying st;
+      multiply_tiles<BN, kCtas, MODE>(p, sh, stages, st, tmem, unit, units);
+      // matrix instructions in flight are done before the CTA leaves, too
+      tc_commit<kCtas>(&sh.drained);
+      mbar_wait_bounded(&sh.drained, 0, kGemmLimitNs);
+    }
+  } else {
+    Storing st;
+    store_tiles<BN, kCtas, MODE>(p, sh, stages + S::kStages * S::kStage + (warp - 2) * kWarpStage, st, tmem, unit, units, rank);
+    store_end(sh, st);
+  }
+  gemm_end<BN, kCtas>(tmem);
+}
+
+// ---- all products of a Newton-Schulz iteration in one launch -----------------------------------------------------------
+// Each product needs all of the one before it, so the CTAs, which are all on the GPU (a cooperative launch), meet between them:
+// a CTA whose stores are complete adds one to a counter and waits, with a limit, until all have.
+struct ChainParams {
+  GemmParams gram[2], poly, update[2], last;
+  int steps;
+  unsigned int* arrived;  // 0 at the start
+};
+
+// by the loading thread, between product number `stage` and the next
+__device__ __forceinline__ bool meet(GemmBarriers& sh, unsigned int* arrived, int stage) {
+  if (!gemm_wait(&sh.stage_done, stage & 1, sh)) return false;
+  asm volatile("fence.proxy.async;" ::: "memory");
+  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
+  const unsigned int want = gridDim.x * (unsigned)(stage + 1);
+  const long long t0 = clock64();
+  for (uint32_t it = 0;; ++it) {
+    unsigned int n;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(arrived) : "memory");
+    if (n >= want) break;
+    if (*reinterpret_cast<volatile uint32_t*>(&sh.gave_up)) return false;
+    if (clock64() - t0 > (long long)kGemmLimitNs * 2 || it >= (1u << 28)) {
+      *reinterpret_cast<volatile uint32_t*>(&sh.gave_up) = 1;
+      atomicMax(&g_train_status, 3u);
+      return false;
+    }
+  }
+  asm volatile("fence.proxy.async;" ::: "memory");
+  mbar_arrive(&sh.stage_go);
+  return true;
+}
+
+template <int BN, int kCtas>
+__global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_chain_kernel(const __grid_constant__ ChainParams c) {
+  using S = GemmShape<BN, kCtas>;
+  extern __shared__ unsigned char raw[];
+  __shared__ GemmBarriers sh;
+  unsigned char* stages = gemm_stages(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kCtas == 2 ? (int)(blockIdx.x & 1) : 0;
+  const int unit = blockIdx.x / kCtas, units = gridDim.x / kCtas;
+  gemm_begin<BN, kCtas>(sh);
+  const uint32_t tmem = sh.tmem;
+  const int products = 3 * c.steps;
+  if (warp == 0) {
+    if (lane == 0) {
+      Loading st;
+      for (int i = 0; i < products && st.ok; ++i) {
+        const int step = i / 3;
+        if (i % 3 == 0) load_tiles<BN, kCtas, kGemmGram>(c.gram[step & 1], sh, stages, st, unit, units, rank);
+        else if (i % 3 == 1) load_tiles<BN, kCtas, kGemmPoly>(c.poly, sh, stages, st, unit, units, rank);
+        else load_tiles<BN, kCtas, kGemmUpdate>(step == c.steps - 1 ? c.last : c.update[step & 1], sh, stages, st, unit, units, rank);
+        if (st.ok && i + 1 < products) st.ok = meet(sh, c.arrived, i);
+      }
+      load_end<BN, kCtas>(sh, st, rank);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      Multiplying st;
+      for (int i = 0; i < products && st.ok; ++i) {
+        const int step = i / 3;
+        if (i % 3 == 0) multiply_tiles<BN, kCtas, kGemmGram>(c.gram[step & 1], sh, stages, st, tmem, unit, units);
+        else if (i % 3 == 1) multiply_tiles<BN, kCtas, kGemmPoly>(c.poly, sh, stages, st, tmem, unit, units);
+        else multiply_tiles<BN, kCtas, kGemmUpdate>(step == c.steps - 1 ? c.last : c.update[step & 1], sh, stages, st, tmem, unit, units);
+      }
+      tc_commit<kCtas>(&sh.drained);
+      mbar_wait_bounded(&sh.drained, 0, kGemmLimitNs);
+    }
+  } else {
+    Storing st;
+    unsigned char* mine = stages + S::kStages * S::kStage + (warp - 2) * kWarpStage;
+    for (int i = 0; i < products && st.ok; ++i) {
+      const int step = i / 3;
+      if (i % 3 == 0) store_tiles<BN, kCtas, kGemmGram>(c.gram[step & 1], sh, mine, st, tmem, unit, units, rank);
+      else if (i % 3 == 1) store_tiles<BN, kCtas, kGemmPoly>(c.poly, sh, mine, st, tmem, unit, units, rank);
+      else store_tiles<BN, kCtas, kGemmUpdate>(step == c.steps - 1 ? c.last : c.update[step & 1], sh, mine, st, tmem, unit, units, rank);
+      if (!st.ok || i + 1 == products) break;
+      if (lane == 0) {
+        tma_wait_group<0>();  // what this warp has stored is there
+        asm volatile("fence.proxy.async;" ::: "memory");
+        mbar_arrive(&sh.stage_done);
+      }
+      st.ok = __all_sync(0xffffffffu, gemm_wait(&sh.stage_go, i & 1, sh));
+      asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    store_end(sh, st);
+  }
+  gemm_end<BN, kCtas>(tmem);
 }
 
 }  // namespace dev
@@ -593,8 +814,9 @@ uint64_t descriptor(bool k_major) {
   return leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// A map of boxes of 32 x 32 values of something beside the accumulator, if its rows begin at 16 bytes.  TMA stores whole 16 bytes, also at the end of a row (seen on a B200): what it stores to has rows of
-// whole 16 bytes, or no more behind a row than rounds it up to eight values.
+// A map of boxes of 32 x 32 values of something beside the accumulator, if its rows begin at 16 bytes.  TMA stores whole 16
+// bytes, also at the end of a row (seen on a B200): what it stores to has rows of whole 16 bytes, or no more behind a row than
+// rounds it up to eight values.
 bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall& c, bool stored, bool mirror = false) {
   const size_t bytes = element_bytes(type);
   if (stored && c.n * bytes % 16 && s.ld != (c.n + 7) / 8 * 8) return false;
@@ -605,7 +827,7 @@ bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall
   cuuint32_t box[3] = {32, 32, 1};
   cuuint32_t step[3] = {1, 1, 1};
   return fn(map, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-            s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, 
+            s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
             mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : type == kF32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -624,10 +846,10 @@ int64_t count_tiles(const GemmCall& c, int rows, int bn) {
 }
 
 template <int BN, int kCtas, int MODE>
-cudaError_t run_gemm(const GemmCall& given, cudaStream_t stream) {
+cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   GemmCall c = given;
   using S = dev::GemmShape<BN, kCtas>;
-  dev::GemmParams p;
+  dev::GemmParams& p = *out;
   memset(&p, 0, sizeof(p));
   p.m = c.m;
   p.n = c.n;
@@ -672,7 +894,7 @@ cudaError_t run_gemm(const GemmCall& given, cudaStream_t stream) {
   p.cb = c.cb;
   p.cc = c.cc;
   p.scale = c.scale;
-  constexpr bool kLinear = MODE == kGemmLinear, kUpdate = MODE == kGemmUpdate;
+  constexpr bool kLinear = MODE == kGemmLinear || MODE == dev::kGemmLinearWide, kUpdate = MODE == kGemmUpdate;
   p.tma_out = make_side_map(&p.map_out, c.out, c.out_type, c, true);
   p.tma_out2 = c.out2.data && (kUpdate || (kLinear && c.out_type != kF32)) && make_side_map(&p.map_out2, c.out2, c.type, c, true);
   p.tma_in = c.in.data && make_side_map(&p.map_in, c.in, kLinear ? c.out_type : kF16, c, false);
@@ -680,24 +902,40 @@ cudaError_t run_gemm(const GemmCall& given, cudaStream_t stream) {
   // the iteration's own arrays lie as TMA wants them
   if (!kLinear && ((MODE != kGemmGram && !p.tma_in) || (kUpdate && (!p.tma_in2 || (c.out2.data && (!p.tma_out || !p.tma_out2)))))) return cudaErrorInvalidValue;
   if ((MODE == kGemmGram || MODE == kGemmPoly) && (!p.tma_out || !make_side_map(&p.map_mirror, c.out, kF16, c, true, true))) return cudaErrorInvalidValue;
-  static unsigned long long allowed = 0;
-  const cudaError_t e = allow_smem(dev::hc_gemm_kernel<BN, kCtas, MODE>, S::kSmem, &allowed);
-  if (e != cudaSuccess) return e;
-  const int64_t total = tiles * c.batch, units = device_info().sms / kCtas;
+  return cudaSuccess;
+}
+
+// a launch of pairs of CTAs, or of single ones
+template <int kCtas, typename K, typename P>
+cudaError_t launch_units(K kernel, const P& p, int64_t total, int smem, bool meeting, cudaStream_t stream) {
+  const int64_t units = device_info().sms / kCtas;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)((total < units ? total : units) * kCtas));
   cfg.blockDim = dim3(dev::kGemmThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  memset(&attr, 0, sizeof(attr));
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = kCtas;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, dev::hc_gemm_kernel<BN, kCtas, MODE>, p);
+  cudaLaunchAttribute attr[2];
+  memset(attr, 0, sizeof(attr));
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeCooperative;
+  attr[1].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = meeting ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int BN, int kCtas, int MODE>
+cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
+  using S = dev::GemmShape<BN, kCtas>;
+  dev::GemmParams p;
+  cudaError_t e = fill_params<BN, kCtas, MODE>(c, &p);
+  static unsigned long long allowed = 0;
+  if (e == cudaSuccess) e = allow_smem(dev::hc_gemm_kernel<BN, kCtas, MODE>, S::kSmem, &allowed);
+  if (e != cudaSuccess) return e;
+  return launch_units<kCtas>(dev::hc_gemm_kernel<BN, kCtas, MODE>, p, (int64_t)p.tiles * p.batch, S::kSmem, false, stream);
 }
 
 // Cycles that a launch takes: those of the unit (a pair of SMs, or one) with the most tiles.  A stage of a tile costs what the
@@ -728,6 +966,46 @@ cudaError_t run_gemm_mode(const GemmCall& c, cudaStream_t stream) {
   return run_gemm<64, 1, MODE>(c, stream);
 }
 
+// A chain's products with the same tiles.  A product ends with its slowest CTA; the next one begins some 2500 cycles later.
+TileChoice best_chain_tile(const GemmCall& gram, const GemmCall& poly, const GemmCall& update) {
+  const int64_t sms = device_info().sms > 1 ? device_info().sms : 2;
+  const int shapes[3][3] = {{256, 2, 512}, {128, 2, 384}, {64, 1, 384}};
+  TileChoice best = {0, 0, 0};
+  for (const auto& s : shapes) {
+    int64_t cost = 0;
+    const GemmCall* calls[3] = {&gram, &poly, &update};
+    for (int i = 0; i < 3; ++i) {
+      const GemmCall& c = *calls[i];
+      const int64_t tiles = (i < 2 ? count_tiles<kGemmGram>(c, dev::kBM * s[1], s[0]) : count_tiles<kGemmUpdate>(c, dev::kBM * s[1], s[0])) * c.batch;
+      const int64_t units = sms / s[1], stages = (c.k + dev::kBK - 1) / dev::kBK;
+      cost += (tiles + units - 1) / units * (stages * s[2] + 1000 + 4 * s[0]);
+    }
+    if (best.bn == 0 || cost < best.cost) best = {s[0], s[1], cost};
+  }
+  return best;
+}
+
+template <int BN, int kCtas>
+cudaError_t run_chain(const GemmChain& c, cudaStream_t stream) {
+  using S = dev::GemmShape<BN, kCtas>;
+  static_assert(sizeof(dev::ChainParams) <= 32000, "arguments of a kernel");
+  dev::ChainParams p;
+  cudaError_t e = cudaSuccess;
+  for (int i = 0; i < 2; ++i) {
+    if (e == cudaSuccess) e = fill_params<BN, kCtas, kGemmGram>(c.gram[i], &p.gram[i]);
+    if (e == cudaSuccess) e = fill_params<BN, kCtas, kGemmUpdate>(c.update[i], &p.update[i]);
+  }
+  if (e == cudaSuccess) e = fill_params<BN, kCtas, kGemmPoly>(c.poly, &p.poly);
+  if (e == cudaSuccess) e = fill_params<BN, kCtas, kGemmUpdate>(c.last, &p.last);
+  p.steps = c.steps;
+  p.arrived = c.arrived;
+  static unsigned long long allowed = 0;
+  if (e == cudaSuccess) e = allow_smem(dev::hc_gemm_chain_kernel<BN, kCtas>, S::kSmem, &allowed);
+  if (e != cudaSuccess) return e;
+  const int64_t total = (int64_t)p.last.tiles * p.last.batch;  // the product with the most tiles
+  return launch_units<kCtas>(dev::hc_gemm_chain_kernel<BN, kCtas>, p, total, S::kSmem, true, stream);
+}
+
 }  // namespace
 
 int gemm_parts(int64_t m, int64_t n, int64_t k) {
@@ -749,10 +1027,14 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
 }
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
-  if (c.mode == kGemmLinear) return run_gemm_mode<kGemmLinear>(c, stream);
-  if (c.mode == kGemmGram) return run_gemm_mode<kGemmGram>(c, stream);
-  if (c.mode == kGemmPoly) return run_gemm_mode<kGemmPoly>(c, stream);
-  return run_gemm_mode<kGemmUpdate>(c, stream);
+  return c.out_type == kF32 && c.parts <= 1 ? run_gemm_mode<dev::kGemmLinearWide>(c, stream) : run_gemm_mode<kGemmLinear>(c, stream);
+}
+
+cudaError_t launch_chain(const GemmChain& c, cudaStream_t stream) {
+  const TileChoice tile = best_chain_tile(c.gram[0], c.poly, c.update[0]);
+  if (tile.bn == 256) return run_chain<256, 2>(c, stream);
+  if (tile.bn == 128) return run_chain<128, 2>(c, stream);
+  return run_chain<64, 1>(c, stream);
 }
 
 }  // namespace hc

@@ -93,7 +93,6 @@ struct GemmSide {
   int64_t stride;
 };
 struct GemmCall {
-  int mode;
   int type;  // of the operands
   int64_t m, n, k, batch;
   int parts;  // over 1 (kGemmLinear without anything behind it, batch 1): as many results, each of a part of the sum, as a batch
@@ -110,7 +109,15 @@ struct GemmCall {
 
 // Into how many parts the sum of a product with fp32 results is best shared out (1: none).
 int gemm_parts(int64_t m, int64_t n, int64_t k);
+// act(a b + bias) + residual
 cudaError_t launch_gemm(const GemmCall& call, cudaStream_t stream);
+// The products of a Newton-Schulz iteration in one launch: step i takes gram[i % 2], poly and update[i % 2], the last one `last`.
+struct GemmChain {
+  GemmCall gram[2], poly, update[2], last;
+  int steps;
+  unsigned int* arrived;  // a word of device memory that is 0 when the launch begins
+};
+cudaError_t launch_chain(const GemmChain& chain, cudaStream_t stream);
 bool gemm_operand_ok(const void* data, int64_t ld);
 
 }  // namespace hc

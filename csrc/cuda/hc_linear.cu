@@ -276,7 +276,6 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   if (!gemm_operand_ok(x, x_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
   GemmCall c;
   memset(&c, 0, sizeof(c));
-  c.mode = kGemmLinear;
   c.type = type;
   c.m = rows, c.n = width, c.k = inner, c.batch = 1;
   c.a = {x, (int64_t)x_stride, 0, true};
@@ -332,7 +331,6 @@ int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weigh
   if (!dz || !weight || !dx || !gemm_operand_ok(dz, dz_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
   GemmCall c;
   memset(&c, 0, sizeof(c));
-  c.mode = kGemmLinear;
   c.type = c.out_type = type;
   c.m = rows, c.n = inner, c.k = width, c.batch = 1;
   c.a = {dz, (int64_t)dz_stride, 0, true};
@@ -359,7 +357,6 @@ int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, s
   if (!dz || !x || !gemm_operand_ok(dz, dz_stride) || !gemm_operand_ok(x, x_stride)) return kErrArgument;
   GemmCall c;
   memset(&c, 0, sizeof(c));
-  c.mode = kGemmLinear;
   c.type = c.out_type = type;
   c.m = width, c.n = inner, c.k = rows, c.batch = 1;
   c.a = {dz, (int64_t)dz_stride, 0, false};

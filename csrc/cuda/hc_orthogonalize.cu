@@ -1,6 +1,6 @@
 // Newton-Schulz iteration of a batch of matrices: X = G / (|G| + eps), then X = a X + (b S + c S S) X with S = X X^T, or
-// X = a X + X (b S + c S S) with S = X^T X where that is the smaller one.  Three products a step (hc_gemm.cu), of which
-// the first two give symmetric matrices and compute one half.
+// X = a X + X (b S + c S S) with S = X^T X where that is the smaller one.  Three products a step, of which the first two give
+// symmetric matrices and compute one half, all of them in one launch (hc_gemm.cu).
 //
 // Operands are fp16: 11 bits, and no entry of X, S or the polynomial leaves its range once |X| <= 1.  What is rounded off
 // X in directions that G hardly has would grow by `a` in every step (485 times in five); products with X carry none of it
@@ -20,6 +20,7 @@ struct ScaleParams {
   double* partial;  // [batch][parts]
   __half *hi, *lo;
   float* scale;  // [batch]: X = 2^-k (hi + lo / 2048)
+  unsigned int* arrived;
   float growth;
   int64_t height, width, stride, batch_stride, ld;  // ld: of hi and lo
   int parts;
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kNormThreads) hc_scale_kernel(const __grid_con
       factor = 1.0 / (norm + (double)p.eps);
       exponent = k;
       if (blockIdx.x == 0) p.scale[blockIdx.y] = exp2f((float)-k);
+      if (blockIdx.x == 0 && blockIdx.y == 0) *p.arrived = 0;
     }
   }
   __syncthreads();
@@ -116,8 +118,7 @@ __global__ void __launch_bounds__(kNormThreads) hc_scale_kernel(const __grid_con
 }
 
 // ---- small matrices ---------------------------------------------------------------------------------------------------
-// The general form is three launches a step, whose work on a small matrix is less than their start.  Here one block takes a
-// matrix through all steps in shared memory, short side first, with warp-wide 16 x 8 x 16 matrix instructions: they need
+// The general form has its CTAs meet after every product, and each of them starts loading then.  Here one block takes a matrix through all steps in shared memory, short side first, with warp-wide 16 x 8 x 16 matrix instructions: they need
 // neither tensor memory nor descriptors, and at this size what counts is the way from one product to the next.
 constexpr int kSmallThreads = 512;
 
@@ -314,7 +315,7 @@ Layout layout_of(size_t batch, size_t height, size_t width) {
   l.parts = most < some ? most : some;
   l.x = round_up(batch * height * l.ld * 2);
   l.s = round_up(batch * l.side * l.ld_side * 2);
-  l.total = round_up(batch * l.parts * 8) + round_up(batch * 4) + 3 * l.x + 2 * l.s;
+  l.total = round_up(batch * l.parts * 8) + round_up(batch * 4 + 4) + 3 * l.x + 2 * l.s;
   return l;
 }
 
@@ -402,12 +403,13 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   double* partial = reinterpret_cast<double*>(at);
   at += round_up(batch * l.parts * 8);
   float* scales = reinterpret_cast<float*>(at);
-  at += round_up(batch * 4);
+  unsigned int* arrived = reinterpret_cast<unsigned int*>(scales + batch);
+  at += round_up(batch * 4 + 4);
   void* hi[2] = {at, at + l.x};
   void* lo = at + 2 * l.x;
   void* gram = at + 3 * l.x;
   void* poly = at + 3 * l.x + l.s;
-  const dev::ScaleParams p = {g, partial, static_cast<__half*>(hi[0]), static_cast<__half*>(lo), scales, growth, (int64_t)height, (int64_t)width, (int64_t)stride,
+  const dev::ScaleParams p = {g, partial, static_cast<__half*>(hi[0]), static_cast<__half*>(lo), scales, arrived, growth, (int64_t)height, (int64_t)width, (int64_t)stride,
                               (int64_t)batch_stride, l.ld, (int)l.parts, eps};
   if (type == kF32) scale<float>(p, batch, stream);
   else if (type == kBf16) scale<__nv_bfloat16>(p, batch, stream);
@@ -415,44 +417,46 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   const bool wide = height <= width;
   const int64_t x_stride = (int64_t)height * l.ld, s_stride = l.side * l.ld_side;
-  for (int i = 0; i < steps; ++i) {
-    const GemmOperand x = {hi[i & 1], l.ld, x_stride, wide};  // along its rows, or (tall) down its columns
-    const GemmOperand s = {gram, l.ld_side, s_stride, true}, q = {poly, l.ld_side, s_stride, true};
-    GemmCall call;
-    memset(&call, 0, sizeof(call));
-    call.type = kF16;
-    call.batch = (int64_t)batch;
-    call.ca = a, call.cb = b, call.cc = c;
-    call.scale = scales;
-    call.mode = kGemmGram;
-    call.m = call.n = l.side;
-    call.k = wide ? width : height;
-    call.a = call.b = x;
-    call.out = {gram, l.ld_side, s_stride};
-    call.out_type = kF16;
-    if (launch_gemm(call, stream) != cudaSuccess) return kErrCuda;
-    call.mode = kGemmPoly;
-    call.k = l.side;
-    call.a = call.b = s;
-    call.in = call.out;
-    call.out = {poly, l.ld_side, s_stride};
-    if (launch_gemm(call, stream) != cudaSuccess) return kErrCuda;
-    const bool last = i == steps - 1;
-    call.mode = kGemmUpdate;
-    call.m = height;
-    call.n = width;
-    GemmOperand y = x;
-    y.k_major = !wide;
-    call.a = wide ? q : y;
-    call.b = wide ? y : q;
-    call.in = {hi[i & 1], l.ld, x_stride};
-    call.in2 = {lo, l.ld, x_stride};
-    call.out = last ? GemmSide{out, (int64_t)width, (int64_t)(height * width)} : GemmSide{hi[(i + 1) & 1], l.ld, x_stride};
-    call.out2 = last ? GemmSide{nullptr, 0, 0} : call.in2;
-    call.out_type = last ? kBf16 : kF16;
-    if (launch_gemm(call, stream) != cudaSuccess) return kErrCuda;
+  GemmChain chain;
+  memset(&chain, 0, sizeof(chain));
+  chain.steps = steps;
+  chain.arrived = arrived;
+  const GemmOperand s = {gram, l.ld_side, s_stride, true}, q = {poly, l.ld_side, s_stride, true};
+  GemmCall call;
+  memset(&call, 0, sizeof(call));
+  call.type = call.out_type = kF16;
+  call.batch = (int64_t)batch;
+  call.ca = a, call.cb = b, call.cc = c;
+  call.scale = scales;
+  chain.poly = call;
+  chain.poly.m = chain.poly.n = chain.poly.k = l.side;
+  chain.poly.a = chain.poly.b = s;
+  chain.poly.in = {gram, l.ld_side, s_stride};
+  chain.poly.out = {poly, l.ld_side, s_stride};
+  for (int i = 0; i < 2; ++i) {  // from hi[i] to the other one
+    GemmOperand x = {hi[i], l.ld, x_stride, wide};  // along its rows, or (tall) down its columns
+    chain.gram[i] = call;
+    chain.gram[i].m = chain.gram[i].n = l.side;
+    chain.gram[i].k = wide ? width : height;
+    chain.gram[i].a = chain.gram[i].b = x;
+    chain.gram[i].out = {gram, l.ld_side, s_stride};
+    x.k_major = !wide;
+    GemmCall& u = chain.update[i];
+    u = call;
+    u.m = height;
+    u.n = width;
+    u.k = l.side;
+    u.a = wide ? q : x;
+    u.b = wide ? x : q;
+    u.in = {hi[i], l.ld, x_stride};
+    u.in2 = u.out2 = {lo, l.ld, x_stride};
+    u.out = {hi[1 - i], l.ld, x_stride};
   }
-  return kOk;
+  chain.last = chain.update[(steps - 1) & 1];
+  chain.last.out = {out, (int64_t)width, (int64_t)(height * width)};
+  chain.last.out2 = {nullptr, 0, 0};
+  chain.last.out_type = kBf16;
+  return launch_chain(chain, stream) == cudaSuccess ? kOk : kErrCuda;
 }
 
 }  // extern "C"
