@@ -248,6 +248,20 @@ void rows_backward(const dev::RowsBackwardParams& p, bool vector, cudaStream_t s
   else rows_backward_of<Y, T, kActSilu>(p, vector, stream);
 }
 
+// scratch memory of a backward pass: sums of columns, sums of parts of the rows, dz
+struct BackwardLayout {
+  size_t sums, parts, total;
+};
+BackwardLayout backward_layout(size_t rows, size_t inner, size_t width, int keep_dz) {
+  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  const int parts = gemm_parts((int64_t)width, (int64_t)inner, (int64_t)rows);
+  BackwardLayout l;
+  l.sums = up((size_t)shares_of(rows, width) * width * sizeof(float));
+  l.parts = parts > 1 ? up((size_t)parts * width * ((inner + 7) / 8 * 8) * sizeof(float)) : 0;
+  l.total = l.sums + l.parts + (keep_dz ? up(rows * ((width + 7) / 8 * 8) * 2) : 0);
+  return l;
+}
+
 bool aligned_rows(const void* p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0; }
 
 }  // namespace
@@ -290,96 +304,86 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
 }
 
-size_t hc_linear_rows_backward_bytes(size_t rows, size_t width) {
-  return rows && width ? (size_t)hc::shares_of(rows, width) * width * sizeof(float) : 0;
+size_t hc_linear_backward_bytes(size_t rows, size_t inner, size_t width, int keep_dz) {
+  return hc::sizes_ok(rows, inner, width) && rows ? hc::backward_layout(rows, inner, width, keep_dz).total : 0;
 }
 
-int hc_linear_rows_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int type,
-                            void* dz, size_t dz_stride, void* dbias, int bias_type, size_t rows, size_t width, void* scratch,
-                            size_t scratch_bytes, hc_stream_t stream) {
+int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int keep_dz,
+                       const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, void* dx, size_t dx_stride,
+                       void* dweight, size_t dweight_stride, void* dbias, int bias_type, size_t rows, size_t inner, size_t width,
+                       void* scratch, size_t scratch_bytes, hc_stream_t stream) {
   using namespace hc;
   if (!product_type(type) || (dy_type != kF32 && dy_type != type) || !element_type_ok(bias_type)) return kErrArgument;
-  if (activation < kActNone || activation > kActSilu || !sizes_ok(rows, 1, width) || !stride_ok(dy_stride, width)) return kErrArgument;
-  if ((dz && !stride_ok(dz_stride, width)) || (activation != kActNone && !stride_ok(z_stride, width))) return kErrArgument;
+  if (activation < kActNone || activation > kActSilu || !sizes_ok(rows, inner, width) || !stride_ok(dy_stride, width)) return kErrArgument;
+  if (activation != kActNone && !stride_ok(z_stride, width)) return kErrArgument;
+  if ((dx && (!stride_ok(weight_stride, inner) || !stride_ok(dx_stride, inner))) || (dweight && (!stride_ok(x_stride, inner) || !stride_ok(dweight_stride, inner))))
+    return kErrArgument;
+  if (!keep_dz && (dx || dweight) && (activation != kActNone || dy_type != type)) return kErrArgument;
   if (rows == 0) {
-    if (!dbias) return kOk;
-    return cudaMemsetAsync(dbias, 0, width * element_bytes(bias_type), stream) == cudaSuccess ? kOk : kErrCuda;
+    cudaError_t e = dweight ? cudaMemset2DAsync(dweight, dweight_stride * 2, 0, inner * 2, width, stream) : cudaSuccess;
+    if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, width * element_bytes(bias_type), stream);
+    return e == cudaSuccess ? kOk : kErrCuda;
   }
+  if (!dx && !dweight && !dbias) return kOk;
   if (!dy || (activation != kActNone && !z)) return kErrArgument;
-  if (!dz && !dbias) return kOk;
-  if (dbias && (!scratch || scratch_bytes < hc_linear_rows_backward_bytes(rows, width))) return kErrArgument;
-  const dev::RowsBackwardParams p = {dy, z, dz, dbias ? static_cast<float*>(scratch) : nullptr, (int64_t)dy_stride, (int64_t)z_stride,
-                                     (int64_t)dz_stride, (int64_t)rows, (int64_t)width, activation, shares_of(rows, width)};
-  const bool vector = aligned_rows(dy, dy_stride) && (!dz || aligned_rows(dz, dz_stride)) && (activation == kActNone || aligned_rows(z, z_stride));
-  if (type == kBf16) {
-    if (dy_type == kF32) rows_backward<float, __nv_bfloat16>(p, vector, stream);
-    else rows_backward<__nv_bfloat16, __nv_bfloat16>(p, vector, stream);
-  } else {
-    if (dy_type == kF32) rows_backward<float, __half>(p, vector, stream);
-    else rows_backward<__half, __half>(p, vector, stream);
+  if ((dx && (!weight || !gemm_operand_ok(weight, weight_stride))) || (dweight && (!x || !gemm_operand_ok(x, x_stride)))) return kErrArgument;
+  const BackwardLayout l = backward_layout(rows, inner, width, keep_dz);
+  if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u) || scratch_bytes < l.total) return kErrArgument;
+  unsigned char* at = static_cast<unsigned char*>(scratch);
+  const bool products = dx || dweight;
+  const void* dz = keep_dz ? at + l.sums + l.parts : dy;
+  const size_t dz_stride = keep_dz ? (width + 7) / 8 * 8 : dy_stride;
+  if (products && !gemm_operand_ok(dz, dz_stride)) return kErrArgument;
+  if (dbias || (products && keep_dz)) {
+    const dev::RowsBackwardParams p = {dy, z, products && keep_dz ? const_cast<void*>(dz) : nullptr, dbias ? reinterpret_cast<float*>(at) : nullptr,
+                                       (int64_t)dy_stride, (int64_t)z_stride, (int64_t)dz_stride, (int64_t)rows, (int64_t)width, activation,
+                                       shares_of(rows, width)};
+    const bool vector = aligned_rows(dy, dy_stride) && (activation == kActNone || aligned_rows(z, z_stride));
+    if (type == kBf16) {
+      if (dy_type == kF32) rows_backward<float, __nv_bfloat16>(p, vector, stream);
+      else rows_backward<__nv_bfloat16, __nv_bfloat16>(p, vector, stream);
+    } else {
+      if (dy_type == kF32) rows_backward<float, __half>(p, vector, stream);
+      else rows_backward<__half, __half>(p, vector, stream);
+    }
+    if (dbias) dev::hc_rows_finish_kernel<<<(unsigned)((width + 31) / 32), 256, 0, stream>>>(p.partial, p.shares, (int64_t)width, dbias, bias_type);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   }
-  if (dbias) dev::hc_rows_finish_kernel<<<(unsigned)((width + 31) / 32), 256, 0, stream>>>(p.partial, p.shares, (int64_t)width, dbias, bias_type);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
-}
-
-int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weight, size_t weight_stride, int type, void* dx,
-                             size_t dx_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream) {
-  using namespace hc;
-  if (!product_type(type) || !sizes_ok(rows, inner, width)) return kErrArgument;
-  if (!stride_ok(dz_stride, width) || !stride_ok(weight_stride, inner) || !stride_ok(dx_stride, inner)) return kErrArgument;
-  if (rows == 0) return kOk;
-  if (!dz || !weight || !dx || !gemm_operand_ok(dz, dz_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
   GemmCall c;
   memset(&c, 0, sizeof(c));
   c.type = c.out_type = type;
-  c.m = rows, c.n = inner, c.k = width, c.batch = 1;
-  c.a = {dz, (int64_t)dz_stride, 0, true};
-  c.b = {weight, (int64_t)weight_stride, 0, false};
-  c.out = {dx, (int64_t)dx_stride, 0};
-  return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
-}
-
-size_t hc_linear_weight_backward_bytes(size_t rows, size_t inner, size_t width) {
-  using namespace hc;
-  if (!sizes_ok(rows, inner, width) || rows == 0) return 0;
-  const int parts = gemm_parts((int64_t)width, (int64_t)inner, (int64_t)rows);
-  return parts > 1 ? (size_t)parts * width * ((inner + 7) / 8 * 8) * sizeof(float) : 0;
-}
-
-int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, size_t x_stride, int type, void* dweight,
-                              size_t dweight_stride, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes,
-                              hc_stream_t stream) {
-  using namespace hc;
-  if (!product_type(type) || !sizes_ok(rows, inner, width)) return kErrArgument;
-  if (!stride_ok(dz_stride, width) || !stride_ok(x_stride, inner) || !stride_ok(dweight_stride, inner) || !dweight) return kErrArgument;
-  if (rows == 0)
-    return cudaMemset2DAsync(dweight, dweight_stride * 2, 0, inner * 2, width, stream) == cudaSuccess ? kOk : kErrCuda;
-  if (!dz || !x || !gemm_operand_ok(dz, dz_stride) || !gemm_operand_ok(x, x_stride)) return kErrArgument;
-  GemmCall c;
-  memset(&c, 0, sizeof(c));
-  c.type = c.out_type = type;
-  c.m = width, c.n = inner, c.k = rows, c.batch = 1;
-  c.a = {dz, (int64_t)dz_stride, 0, false};
-  c.b = {x, (int64_t)x_stride, 0, false};
-  c.out = {dweight, (int64_t)dweight_stride, 0};
-  const size_t need = hc_linear_weight_backward_bytes(rows, inner, width);
-  if (need) {
-    if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15u)) return kErrArgument;
-    const int64_t ld = (int64_t)(inner + 7) / 8 * 8, stride = (int64_t)width * ld;
-    c.parts = gemm_parts(c.m, c.n, c.k);
-    c.out_type = kF32;
-    c.out = {scratch, ld, stride};
+  c.batch = 1;
+  if (dx) {
+    c.m = rows, c.n = inner, c.k = width;
+    c.a = {dz, (int64_t)dz_stride, 0, true};
+    c.b = {weight, (int64_t)weight_stride, 0, false};
+    c.out = {dx, (int64_t)dx_stride, 0};
     if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
-    const int64_t groups = (int64_t)width * (ld / 8);
-    const unsigned grid = (unsigned)((groups + 255) / 256 < 2368 ? (groups + 255) / 256 : 2368);
-    const float* sums = static_cast<const float*>(scratch);
-    if (type == kBf16)
-      dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__nv_bfloat16*>(dweight), (int64_t)dweight_stride);
-    else
-      dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__half*>(dweight), (int64_t)dweight_stride);
-    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
   }
-  return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
+  if (dweight) {
+    c.m = width, c.n = inner, c.k = rows;
+    c.a = {dz, (int64_t)dz_stride, 0, false};
+    c.b = {x, (int64_t)x_stride, 0, false};
+    c.out = {dweight, (int64_t)dweight_stride, 0};
+    c.parts = gemm_parts(c.m, c.n, c.k);
+    const int64_t ld = (int64_t)(inner + 7) / 8 * 8, stride = (int64_t)width * ld;
+    float* sums = reinterpret_cast<float*>(at + l.sums);
+    if (c.parts > 1) {
+      c.out_type = kF32;
+      c.out = {sums, ld, stride};
+    }
+    if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
+    if (c.parts > 1) {
+      const int64_t groups = (int64_t)width * (ld / 8);
+      const unsigned grid = (unsigned)((groups + 255) / 256 < 2368 ? (groups + 255) / 256 : 2368);
+      if (type == kBf16)
+        dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__nv_bfloat16*>(dweight), (int64_t)dweight_stride);
+      else
+        dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__half*>(dweight), (int64_t)dweight_stride);
+      if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    }
+  }
+  return kOk;
 }
 
 }  // extern "C"

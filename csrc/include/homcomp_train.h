@@ -54,20 +54,15 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
               const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
               int activation, size_t rows, size_t inner, size_t width, hc_stream_t stream);
-// First part of the backward pass, over the rows of dy (dy_type 0 or `type`): dz = dy act'(z) of `type` (dz NULL: not
-// stored), dbias = the sums of its columns before rounding (NULL: not formed), in a fixed order.
-size_t hc_linear_rows_backward_bytes(size_t rows, size_t width);
-int hc_linear_rows_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int type,
-                            void* dz, size_t dz_stride, void* dbias, int bias_type, size_t rows, size_t width, void* scratch,
-                            size_t scratch_bytes, hc_stream_t stream);
-// dx = dz weight and dweight = dz^T x, of `type`.  dweight has a long sum and may have few tiles: its scratch memory (there
-// may be none to give) holds fp32 sums of parts of the rows, which are added in a fixed order.
-int hc_linear_input_backward(const void* dz, size_t dz_stride, const void* weight, size_t weight_stride, int type, void* dx,
-                             size_t dx_stride, size_t rows, size_t inner, size_t width, hc_stream_t stream);
-size_t hc_linear_weight_backward_bytes(size_t rows, size_t inner, size_t width);
-int hc_linear_weight_backward(const void* dz, size_t dz_stride, const void* x, size_t x_stride, int type, void* dweight,
-                              size_t dweight_stride, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes,
-                              hc_stream_t stream);
+// Backward pass: dz = dy act'(z), rounded to `type` for the products; dx = dz weight, dweight = dz^T x (of `type`) and dbias =
+// the sums of dz's columns before rounding (of bias_type), each NULL where it is not wanted.  dy is of dy_type, 0 or `type`.
+// keep_dz: dz is written to the scratch memory; 0 where dy itself is dz and a product can read it (no activation, dy of
+// `type`, its rows as operands have to lie).  Sums over rows are formed in a fixed order.
+size_t hc_linear_backward_bytes(size_t rows, size_t inner, size_t width, int keep_dz);
+int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void* z, size_t z_stride, int activation, int keep_dz,
+                       const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, void* dx, size_t dx_stride,
+                       void* dweight, size_t dweight_stride, void* dbias, int bias_type, size_t rows, size_t inner, size_t width,
+                       void* scratch, size_t scratch_bytes, hc_stream_t stream);
 
 // ---- orthogonalised updates ---------------------------------------------------------------------------------------------
 // Newton-Schulz iteration: X = G / (|G| + eps); `steps` times X = a X + (b S + c S S) X with S = X X^T (or its mirror image

@@ -303,11 +303,16 @@ def test_refusals_without_a_gpu():
                dict(r=p, rs=23), dict(z=p, zs=1), dict(x=None), dict(w=None), dict(out=None), dict(x=C.c_void_p(4098)), dict(xs=17), dict(ws=20), dict(w=C.c_void_p(4104))):
         assert forward(**kw) == 4, kw
     assert forward(m=0) == 0
-    rows = lambda **kw: lib.hc_linear_rows_backward(*{**dict(dy=p, t=1, s=24, z=p, zs=24, act=1, type=1, dz=p, ds=24, db=p, bt=0, m=32, n=24, sc=p, by=1 << 30), **kw}.values(), None)  # noqa: E731
-    for kw in (dict(t=2), dict(type=0), dict(s=23), dict(zs=23), dict(ds=23), dict(z=None), dict(dy=None), dict(sc=None), dict(by=8), dict(act=9), dict(n=0)):
-        assert rows(**kw) == 4, kw
-    assert rows(dz=None, db=None) == 0
-    for name, more in (("hc_linear_input_backward", ()), ("hc_linear_weight_backward", (None, 0))):
-        call = lambda **kw: getattr(lib, name)(*{**dict(dz=p, ds=24, o=p, os=16, type=1, out=p, outs=16, m=32, k=16, n=24), **kw}.values(), *more, None)  # noqa: B023, E731
-        for kw in (dict(type=0), dict(ds=16), dict(ds=25), dict(os=15), dict(outs=8), dict(dz=None), dict(o=None), dict(out=None), dict(o=C.c_void_p(4100)), dict(k=0)):
-            assert call(**kw) == 4, (name, kw)
+    good = dict(dy=p, dt=1, ds=24, z=p, zs=24, act=0, keep=1, x=p, xs=16, w=p, ws=16, type=1, dx=p, dxs=16, dw=p, dws=16, db=p, bt=0, m=32, k=16, n=24,
+                scratch=p, bytes=1 << 30)
+
+    def backward(**kw):
+        return lib.hc_linear_backward(*{**good, **kw}.values(), None)
+
+    odd = C.c_void_p(4104)
+    for kw in (dict(type=0), dict(dt=2), dict(bt=3), dict(act=4), dict(act=-1), dict(ds=23), dict(act=1, zs=23), dict(act=1, z=None), dict(act=1, keep=0), dict(dt=0, keep=0), dict(dy=None),
+               dict(xs=15), dict(ws=15), dict(dxs=8), dict(dws=8), dict(x=None), dict(w=None), dict(x=odd), dict(w=odd), dict(xs=17), dict(ws=20), dict(keep=0, dy=odd),
+               dict(keep=0, ds=25), dict(scratch=None), dict(scratch=odd), dict(bytes=8), dict(k=0), dict(n=0), dict(m=1 << 31)):
+        assert backward(**kw) == 4, kw
+    assert backward(dx=None, dw=None, db=None) == 0
+    assert lib.hc_linear_backward_bytes(0, 16, 24, 1) == 0

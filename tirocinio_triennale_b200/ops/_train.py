@@ -92,6 +92,10 @@ def empty_rows(rows: int, width: int, dtype, device) -> torch.Tensor:
     return t if t.shape[1] == width else t[:, :width]
 
 
+def any_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else padded(t.shape[1])
 
@@ -101,8 +105,10 @@ def rows_adjacent(t: torch.Tensor) -> bool:
     return (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
 
 
+def is_operand(t: torch.Tensor) -> bool:
+    """A matrix as the products read it: rows of adjacent elements that begin at 16-byte boundaries."""
+    return rows_adjacent(t) and row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0
+
+
 def operand(t: torch.Tensor) -> torch.Tensor:
-    """A matrix as the products read it: rows of adjacent elements that begin at 16-byte boundaries; a copy if it is not so."""
-    if rows_adjacent(t) and row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return empty_rows(t.shape[0], t.shape[1], t.dtype, t.device).copy_(t)
+    return t if is_operand(t) else empty_rows(t.shape[0], t.shape[1], t.dtype, t.device).copy_(t)

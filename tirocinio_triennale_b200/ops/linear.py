@@ -4,7 +4,8 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._train import (TYPES, call, empty_rows, floating, operand, padded, ptr, row_stride, rows_adjacent, size, vector, wants_grad)
+from ._train import (TYPES, any_stride, call, empty_rows, floating, is_operand, operand, padded, ptr, row_stride, rows_adjacent, size, vector,
+                     wants_grad)
 
 ACTIVATIONS = {None: 0, "gelu_tanh": 1, "relu": 2, "silu": 3}
 FEW_ROWS = 8  # up to here W is read by a kernel that takes rows that begin anywhere
@@ -17,13 +18,9 @@ def _forward(x, weight, bias, residual, act, out_dtype, keep):
     out = empty_rows(m, n, out_dtype, dev)
     z = empty_rows(m, n, x.dtype, dev) if keep and act else None
     call("linear", "hc_linear", dev, x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), TYPES[x.dtype], ptr(bias),
-         0 if bias is None else TYPES[bias.dtype], ptr(residual), 0 if residual is None else _any_stride(residual), out.data_ptr(),
+         0 if bias is None else TYPES[bias.dtype], ptr(residual), 0 if residual is None else any_stride(residual), out.data_ptr(),
          TYPES[out_dtype], padded(n), ptr(z), padded(n), act, m, k, n)
     return out, z
-
-
-def _any_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 class _Linear(torch.autograd.Function):
@@ -41,31 +38,21 @@ class _Linear(torch.autograd.Function):
         x, weight, z = ctx.saved_tensors
         (m, k), n, dev, t = x.shape, weight.shape[0], x.device, x.dtype
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        dz = g = dy if rows_adjacent(dy) else dy.contiguous()
-        # the rows are gone through where that has something to do: a slope, another type, rows that the products cannot read
-        as_is = not ctx.act and dy.dtype == t and operand(g) is g if m else True
-        through = (want_x or want_w) and not as_is
-        if through or want_b:
-            dz = empty_rows(m, n, t, dev) if through else g
-            db = torch.empty(n, dtype=ctx.bias_dtype, device=dev) if want_b else None
-            need = size("hc_linear_rows_backward_bytes", dev, m, n) if want_b else 0
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            call("linear backward", "hc_linear_rows_backward", dev, g.data_ptr(), TYPES[g.dtype], _any_stride(g), ptr(z), padded(n),
-                 ctx.act, TYPES[t], dz.data_ptr() if through else None, padded(n), ptr(db), 0 if db is None else TYPES[db.dtype], m, n,
-                 ptr(scratch), need)
-        if want_x:
-            dx = empty_rows(m, k, t, dev)
-            w = operand(weight)
-            call("linear backward", "hc_linear_input_backward", dev, dz.data_ptr(), row_stride(dz), w.data_ptr(), row_stride(w),
-                 TYPES[t], dx.data_ptr(), padded(k), m, k, n)
-        if want_w:
-            dw = empty_rows(n, k, t, dev)
-            a = operand(x)
-            need = size("hc_linear_weight_backward_bytes", dev, m, k, n)
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            call("linear backward", "hc_linear_weight_backward", dev, dz.data_ptr(), row_stride(dz), a.data_ptr(), row_stride(a),
-                 TYPES[t], dw.data_ptr(), padded(k), m, k, n, ptr(scratch), need)
+        if not (want_x or want_w or want_b):
+            return None, None, None, dy if want_r else None, None, None
+        g = dy if rows_adjacent(dy) else dy.contiguous()
+        # dz is written where dy itself is not what the products can read
+        keep = 1 if ctx.act or dy.dtype != t or not is_operand(g) else 0
+        dx = empty_rows(m, k, t, dev) if want_x else None
+        dw = empty_rows(n, k, t, dev) if want_w else None
+        db = torch.empty(n, dtype=ctx.bias_dtype, device=dev) if want_b else None
+        w = operand(weight) if want_x else weight
+        a = operand(x) if want_w else x
+        need = size("hc_linear_backward_bytes", dev, m, k, n, keep) if m else 0
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        call("linear backward", "hc_linear_backward", dev, g.data_ptr(), TYPES[g.dtype], any_stride(g), ptr(z), padded(n), ctx.act, keep,
+             a.data_ptr(), row_stride(a), w.data_ptr(), row_stride(w), TYPES[t], ptr(dx), padded(k), ptr(dw), padded(k), ptr(db),
+             0 if db is None else TYPES[db.dtype], m, k, n, ptr(scratch), need)
         return dx, dw, db, dy if want_r else None, None, None
 
 

@@ -6,7 +6,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._train import TYPES, call, floating, ptr, wants_grad
+from ._train import TYPES, any_stride, call, floating, ptr, wants_grad
 
 MOST_TOP = 64
 
@@ -26,13 +26,9 @@ def _forward(logits, tokens, top, ignore, keep):
     top_tokens = torch.empty(rows, top, dtype=torch.int64, device=dev) if top else None
     top_logprobs = torch.empty(rows, top, dtype=torch.float32, device=dev) if top else None
     stats = torch.empty(rows, 3, dtype=torch.float32, device=dev) if keep else None
-    call("token_logprobs", "hc_token_logprobs", dev, logits.data_ptr(), TYPES[logits.dtype], rows, vocab, _stride(logits),
+    call("token_logprobs", "hc_token_logprobs", dev, logits.data_ptr(), TYPES[logits.dtype], rows, vocab, any_stride(logits),
          tokens.data_ptr(), ignore, top, logprobs.data_ptr(), entropy.data_ptr(), ptr(top_tokens), ptr(top_logprobs), ptr(stats))
     return logprobs, entropy, top_tokens, top_logprobs, stats
-
-
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -55,7 +51,7 @@ class _TokenLogprobs(torch.autograd.Function):
         rows, vocab = logits.shape
         d_logprobs = None if d_logprobs is None else d_logprobs.contiguous()
         d_entropy = None if d_entropy is None else d_entropy.contiguous()
-        stride = _stride(logits)
+        stride = any_stride(logits)
         # rows that begin at the same places of 16-byte groups as the logits', so that both move in whole groups; a product
         # whose rows were padded to such groups gets its gradient padded alike
         at = vocab + (stride - vocab) % 8
