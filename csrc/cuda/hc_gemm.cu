@@ -870,7 +870,7 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.tiles_n = (int)((c.n + BN - 1) / BN);
   p.batch = (int)c.batch;
   const int64_t tiles = count_tiles<MODE>(c, S::kRows, BN);
-  if (tiles * c.batch > 0x7fffffff) return cudaErrorInvalidValue;
+  if (tiles * c.batch > 1 << 30) return cudaErrorInvalidValue;
   p.tiles = (int)tiles;
   p.a_across = !c.a.k_major;
   p.b_across = !c.b.k_major;
@@ -1048,6 +1048,7 @@ cudaError_t launch_chain(const GemmChain& c, cudaStream_t stream) {
 }  // namespace hc
 
 extern "C" int hc_train_status(int clear) {
+  if (cudaDeviceSynchronize() != cudaSuccess) return hc::kErrCuda;
   const int all[3] = {hc::take_status(hc::dev::g_train_status, clear), hc::norm_status(clear), hc::logprob_status(clear)};
   return all[0] ? all[0] : all[1] ? all[1] : all[2];
 }

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) hc_add_parts_kernel(const float* parts, i
 
 namespace {
 
-constexpr size_t kMostSize = (size_t)1 << 31;
+constexpr size_t kMostSize = (size_t)1 << 26;  // of each side: a tile's sum then stays far below the limit of a wait
 constexpr size_t kFewRows = 8;
 
 bool sizes_ok(size_t rows, size_t inner, size_t width) {

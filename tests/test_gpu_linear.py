@@ -299,7 +299,7 @@ def test_refusals_without_a_gpu():
     def forward(**kw):
         return lib.hc_linear(*{**good, **kw}.values(), None)
 
-    for kw in (dict(type=0), dict(type=3), dict(ot=2), dict(bt=3), dict(act=4), dict(act=-1), dict(k=0), dict(n=0), dict(m=1 << 31), dict(xs=15), dict(ws=8), dict(os=23),
+    for kw in (dict(type=0), dict(type=3), dict(ot=2), dict(bt=3), dict(act=4), dict(act=-1), dict(k=0), dict(n=0), dict(m=1 << 26), dict(xs=15), dict(ws=8), dict(os=23),
                dict(r=p, rs=23), dict(z=p, zs=1), dict(x=None), dict(w=None), dict(out=None), dict(x=C.c_void_p(4098)), dict(xs=17), dict(ws=20), dict(w=C.c_void_p(4104))):
         assert forward(**kw) == 4, kw
     assert forward(m=0) == 0
@@ -312,7 +312,7 @@ def test_refusals_without_a_gpu():
     odd = C.c_void_p(4104)
     for kw in (dict(type=0), dict(dt=2), dict(bt=3), dict(act=4), dict(act=-1), dict(ds=23), dict(act=1, zs=23), dict(act=1, z=None), dict(act=1, keep=0), dict(dt=0, keep=0), dict(dy=None),
                dict(xs=15), dict(ws=15), dict(dxs=8), dict(dws=8), dict(x=None), dict(w=None), dict(x=odd), dict(w=odd), dict(xs=17), dict(ws=20), dict(keep=0, dy=odd),
-               dict(keep=0, ds=25), dict(scratch=None), dict(scratch=odd), dict(bytes=8), dict(k=0), dict(n=0), dict(m=1 << 31)):
+               dict(keep=0, ds=25), dict(scratch=None), dict(scratch=odd), dict(bytes=8), dict(k=0), dict(n=0), dict(m=1 << 26)):
         assert backward(**kw) == 4, kw
     assert backward(dx=None, dw=None, db=None) == 0
     assert lib.hc_linear_backward_bytes(0, 16, 24, 1) == 0

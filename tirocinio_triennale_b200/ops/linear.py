@@ -94,6 +94,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if out_dtype not in (torch.float32, x.dtype):
         raise ValueError("linear: the result is float32 or of x's type")
     flat = x.reshape(-1, k)
+    if max(flat.shape[0], n, k) >= 1 << 26:
+        raise ValueError("linear: every side is below 2^26")
     if flat.shape[0] > FEW_ROWS:
         flat, weight = operand(flat), operand(weight)
     else:
