@@ -140,6 +140,18 @@ def test_muon_with_adamw_state_and_refusals():
     opt.step()  # without gradients nothing moves
 
 
+@pytest.mark.gpu
+def test_gradients_have_no_gradients():
+    x = torch.randn(20, 64, device="cuda", requires_grad=True)
+    t = torch.zeros(20, dtype=torch.int64, device="cuda")
+    h = x.detach().bfloat16().requires_grad_()
+    for y, leaf in ((ops.layer_norm(x), x), (ops.linear(h, h), h), (ops.token_logprobs(x, t).logprobs, x)):
+        (d,) = torch.autograd.grad(y.float().square().sum(), (leaf,), create_graph=True)
+        with pytest.raises(RuntimeError, match="no gradients of their own"):
+            d.sum().backward()
+        assert torch.isfinite(d).all()
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(ValueError):
         Muon([torch.nn.Parameter(torch.zeros(3))])

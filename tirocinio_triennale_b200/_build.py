@@ -144,6 +144,35 @@ def build_mpi(mpi_include: str | None = None, mpi_sources=(), mpi_link=(), force
     return lib
 
 
+def build_torch(force: bool = False) -> Path:
+    """``_homcomp_torch.so``: the training step's operators on torch tensors with their gradients (csrc/torch), compiled by g++
+    against the headers of the installed torch.  It is given the addresses of the library's functions when it is loaded."""
+    lib = LIBDIR / "_homcomp_torch.so"
+    src, header = CSRC / "torch" / "hc_torch.cpp", CSRC / "include" / "homcomp_train.h"
+    if not force and lib.exists() and lib.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+        return lib
+    import fcntl
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = str(Path(nvcc_path()).resolve().parent.parent / "include") if nvcc_path() else "/usr/local/cuda/include"
+    includes = [*cpp_extension.include_paths(), cuda, sysconfig.get_paths()["include"]]
+    LIBDIR.mkdir(parents=True, exist_ok=True)
+    with open(LIBDIR / ".build_torch.lock", "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if not force and lib.exists() and lib.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+            return lib
+        tmp = lib.with_suffix(".so.tmp%d" % os.getpid())
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_homcomp_torch",
+              "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I", str(CSRC / "include"),
+              *[a for i in includes for a in ("-isystem", i)], str(src), "-o", str(tmp),
+              *["-L" + p for p in cpp_extension.library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+        os.replace(tmp, lib)
+    return lib
+
+
 CLI_SOURCES = ["cli/homcomp_eval.cu", "cli/allreduce_threads.cu", "cli/compat_check.cu"]
 BINDIR = Path(__file__).resolve().parent / "bin"
 
@@ -169,5 +198,6 @@ if __name__ == "__main__":
     print(build_cuda(force="--force" in sys.argv, verbose="-v" in sys.argv))
     if "--timeline" in sys.argv:
         print(build_cuda(force="--force" in sys.argv, timeline=True))
+    print(build_torch(force="--force" in sys.argv))
     print(build_cli(force="--force" in sys.argv))
     print(build_mpi(force="--force" in sys.argv))
