@@ -7,8 +7,9 @@
 // twice from the ring, and has the column sums of a thread's own columns in its registers over all rows that its block
 // works on.  Rows whose length eight does not divide begin at one of eight places within an aligned group; a block takes rows
 // that begin at the same place, so that its threads keep their columns, whose w and b wait in shared memory.  The sums of the
-// blocks are added by a second kernel in a fixed order.  Both passes are bound by memory, and need some 60 KB an SM on their
-// way for that: with one row ahead in registers, 6001 x 5003 values of bf16 took 104 us forward and 109 us back.
+// blocks are added by a second kernel in a fixed order.  Both passes should be bound by memory (18 and 28 us for 6001 x 5003
+// values of bf16), which takes some 60 KB an SM on their way: with one row ahead in registers they took 104 and 109 us.  They take
+// 32 and 53 now, at 40 % of the issue slots of 16 warps an SM, which wait for shared memory and for their team.
 #include "hc_host.cuh"
 #include "hc_train.cuh"
 #include "homcomp_train.h"
@@ -33,11 +34,11 @@ struct NormParams {
 
 __device__ unsigned int g_norm_status;
 
-// A block stays on its SM for all rows; its teams of T threads share the parameters.  Forward needs few registers, and
-// its threads fill the SM; the column sums of the backward pass leave room for half as many.
-template <int T, bool kBackward>
+// A block stays on its SM for all rows; its teams of T threads share the parameters.  Forward with up to three groups a thread
+// needs few registers, and its threads fill the SM; with more, or the column sums of the backward pass, half as many do.
+template <int T, int K, bool kBackward>
 struct Block {
-  static constexpr int kThreads = kBackward ? 512 : 1024;
+  static constexpr int kThreads = kBackward || K > 3 ? 512 : 1024;
   static constexpr int kTeams = kThreads / T;
 };
 constexpr int kNormSmem = 220 * 1024;
@@ -51,16 +52,28 @@ __device__ __forceinline__ void load_pairs(const T* p, Pair (&v)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = pair(f[2 * j], f[2 * j + 1]);
 }
-template <typename T>
-__device__ __forceinline__ void store_pairs(T* row, int first, int64_t width, const Pair (&v)[4]) {
-  float f[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) parts(v[j], f[2 * j], f[2 * j + 1]);
-  store_group(row, first, width, f);
+// w and b wait in shared memory by place, in two halves: the first four of every group of eight, and the others.  (With eight
+// neighbours a thread, every second thread of a warp met another one's banks: 6001 x 5003 bf16 forward 37 us, 32 this way.)
+template <int kPlaces>
+__device__ __forceinline__ int param_place(int i) {
+  return (i >> 2 & 1) * (kPlaces / 2) + (i >> 3) * 4 + (i & 3);
+}
+template <int kPlaces>
+__device__ __forceinline__ void load_params(const float* params, int group, Pair (&v)[4]) {
+  const float4 a = reinterpret_cast<const float4*>(params)[group], b = reinterpret_cast<const float4*>(params + kPlaces / 2)[group];
+  v[0] = pair(a.x, a.y), v[1] = pair(a.z, a.w), v[2] = pair(b.x, b.y), v[3] = pair(b.z, b.w);
+}
+
+// Of a thread's K groups only the first one can begin before the row, and only the last one end behind it, or the one before that
+// where the row has no last one (it has a group less where it begins with a whole one).
+template <int K>
+__device__ __forceinline__ bool cut(int k, int first, int width) {
+  return (k == 0 && first < 0) || (k >= K - 2 && first + 8 > width);
 }
 // zeros in the places of values that are not in [0, width)
-__device__ __forceinline__ void keep_pairs(Pair (&v)[4], int first, int width) {
-  if (first >= 0 && first + 8 <= width) return;
+template <int K>
+__device__ __forceinline__ void keep_pairs(int k, Pair (&v)[4], int first, int width) {
+  if (!cut<K>(k, first, width)) return;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float a, b;
@@ -69,16 +82,43 @@ __device__ __forceinline__ void keep_pairs(Pair (&v)[4], int first, int width) {
     v[j] = pair(c >= 0 && c < width ? a : 0.0f, c + 1 >= 0 && c + 1 < width ? b : 0.0f);
   }
 }
+template <int K, typename T>
+__device__ __forceinline__ void store_pairs(int k, T* row, int first, int width, const Pair (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) parts(v[j], f[2 * j], f[2 * j + 1]);
+  if (!cut<K>(k, first, width)) {
+    store8(row + first, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (first + j >= 0 && first + j < width) row[first + j] = from_float<T>(f[j]);
+  }
+}
 
-// sums of two values over a team; the two buffers take turns, so that one barrier is enough
+// sum over a team; the two buffers take turns, so that one barrier is enough
 // `name`: of the team's hardware barrier, at which all of its threads come to every sum.
+template <int T>
+__device__ __forceinline__ float team_sum(float a, float2 (*shared)[T / 32], int name, int& turn) {
+  a = warp_sum(a);
+  if (T > 32) {
+    float* sums = reinterpret_cast<float*>(shared[turn]);
+    if ((threadIdx.x & 31) == 0) sums[(threadIdx.x >> 5) % (T / 32)] = a;
+    asm volatile("bar.sync %0, %1;" ::"r"(name), "n"(T) : "memory");
+    a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < T / 32; ++w) a += sums[w];
+    turn ^= 1;
+  }
+  return a;
+}
+// of two values
 template <int T>
 __device__ __forceinline__ void team_sum2(float& a, float& b, float2 (*shared)[T / 32], int name, int& turn) {
   a = warp_sum(a);
   b = warp_sum(b);
   if (T > 32) {
-    const int warp = (threadIdx.x >> 5) % (T / 32);
-    if ((threadIdx.x & 31) == 0) shared[turn][warp] = make_float2(a, b);
+    if ((threadIdx.x & 31) == 0) shared[turn][(threadIdx.x >> 5) % (T / 32)] = make_float2(a, b);
     asm volatile("bar.sync %0, %1;" ::"r"(name), "n"(T) : "memory");
     a = b = 0.0f;
 #pragma unroll
@@ -98,15 +138,15 @@ __device__ __forceinline__ uint32_t row_bytes(int64_t begin, int groups, int64_t
 }
 
 // A group of a row in the ring; what is not the row's reads as 0.
-template <typename T>
-__device__ __forceinline__ void take(const T* ring, int group, int first, int width, Pair (&v)[4]) {
-  if (first >= width) {
+template <int K, typename T>
+__device__ __forceinline__ void take(int k, const T* ring, int group, int first, int width, Pair (&v)[4]) {
+  if (k == K - 1 && first >= width) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = pair(0.0f, 0.0f);
     return;
   }
   load_pairs(ring + group * 8, v);
-  keep_pairs(v, first, width);
+  keep_pairs<K>(k, v, first, width);
 }
 
 // What the two kernels do alike: a team's rows come through its ring one after the other.  X, Y: what a row has of each type
@@ -174,9 +214,9 @@ struct Rows {
   }
 };
 
-template <typename X, typename Y, bool kBoth, int T>
+template <typename X, typename Y, bool kBoth, int T, int K>
 __device__ __forceinline__ Rows<X, Y, kBoth> rows_of(const NormParams& p, unsigned char* shared, int rings, uint64_t* bars) {
-  using G = Block<T, kBoth>;
+  using G = Block<T, K, kBoth>;
   Rows<X, Y, kBoth> q;
   const int place = blockIdx.x % p.period;  // rows place, place + period, ... are shared out among the blocks of this place
   const int mine = threadIdx.x / T;
@@ -203,20 +243,20 @@ __device__ __forceinline__ Rows<X, Y, kBoth> rows_of(const NormParams& p, unsign
 
 // T threads a row, K groups of eight a thread
 template <typename X, typename Y, int T, int K>
-__global__ void __launch_bounds__(Block<T, false>::kThreads, 1) hc_norm_kernel(const __grid_constant__ NormParams p) {
-  using G = Block<T, false>;
+__global__ void __launch_bounds__(Block<T, K, false>::kThreads, 1) hc_norm_kernel(const __grid_constant__ NormParams p) {
+  using G = Block<T, K, false>;
   __shared__ float2 shared[G::kTeams][2][T / 32];
   __shared__ uint64_t bars[G::kTeams * kMostStages];
   extern __shared__ __align__(16) float params[];  // w and b by place: [2][K * T * 8]; the rings
   const int lane = threadIdx.x % T, team = threadIdx.x / T;
-  auto q = rows_of<X, Y, false, T>(p, reinterpret_cast<unsigned char*>(params), 2 * K * T * 32, bars);
+  auto q = rows_of<X, Y, false, T, K>(p, reinterpret_cast<unsigned char*>(params), 2 * K * T * 32, bars);
   if (lane == 0) q.start();
 #pragma unroll 4
   for (int i = threadIdx.x; i < K * T * 8; i += G::kThreads) {
     const int64_t c = i - q.shift;
     const bool in = c >= 0 && c < p.width;
-    params[i] = !in ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
-    params[K * T * 8 + i] = p.bias && in ? param_at(p.bias, p.param_type, c) : 0.0f;
+    params[param_place<K * T * 8>(i)] = !in ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
+    params[K * T * 8 + param_place<K * T * 8>(i)] = p.bias && in ? param_at(p.bias, p.param_type, c) : 0.0f;
   }
   __syncthreads();
   const float inv = 1.0f / (float)p.width;
@@ -227,53 +267,48 @@ __global__ void __launch_bounds__(Block<T, false>::kThreads, 1) hc_norm_kernel(c
     Pair v[K][4], sum = pair(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      take(x, k * T + lane, (k * T + lane) * 8 - q.shift, width, v[k]);
+      take<K>(k, x, k * T + lane, (k * T + lane) * 8 - q.shift, width, v[k]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum = sum + v[k][j];
     }
-    float mean = both(sum), none = 0.0f;
-    team_sum2<T>(mean, none, shared[team], team + 1, turn);
+    const float mean = team_sum<T>(both(sum), shared[team], team + 1, turn) * inv;
     if (lane == 0) q.ask_next();
-    mean *= inv;
     const Pair minus = pair(-mean, -mean);
     Pair squares = pair(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[k][j] = v[k][j] + minus;
-      keep_pairs(v[k], (k * T + lane) * 8 - q.shift, width);
+      keep_pairs<K>(k, v[k], (k * T + lane) * 8 - q.shift, width);
 #pragma unroll
       for (int j = 0; j < 4; ++j) squares = fma2(v[k][j], v[k][j], squares);
     }
-    float var = both(squares);
-    none = 0.0f;
-    team_sum2<T>(var, none, shared[team], team + 1, turn);
-    const float rstd = 1.0f / sqrtf(fmaf(var, inv, p.eps));
+    const float rstd = rsqrtf(fmaf(team_sum<T>(both(squares), shared[team], team + 1, turn), inv, p.eps));
     const Pair scale = pair(rstd, rstd);
     Y* y = static_cast<Y*>(p.out) + q.row * p.width;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int first = (k * T + lane) * 8 - q.shift;
-      if (first >= width) continue;
+      if (k == K - 1 && first >= width) continue;
       Pair w[4], b[4];
-      load_pairs(params + (k * T + lane) * 8, w);
-      load_pairs(params + K * T * 8 + (k * T + lane) * 8, b);
+      load_params<K * T * 8>(params, k * T + lane, w);
+      load_params<K * T * 8>(params + K * T * 8, k * T + lane, b);
 #pragma unroll
       for (int j = 0; j < 4; ++j) b[j] = fma2(v[k][j] * scale, w[j], b[j]);
-      store_pairs(y, first, p.width, b);
+      store_pairs<K>(k, y, first, width, b);
     }
     if (p.stats && lane == 0) reinterpret_cast<float2*>(p.stats)[q.row] = make_float2(mean, rstd);
   }
 }
 
 template <typename X, typename Y, int T, int K>
-__global__ void __launch_bounds__(Block<T, true>::kThreads, 1) hc_norm_backward_kernel(const __grid_constant__ NormParams p) {
-  using G = Block<T, true>;
+__global__ void __launch_bounds__(Block<T, K, true>::kThreads, 1) hc_norm_backward_kernel(const __grid_constant__ NormParams p) {
+  using G = Block<T, K, true>;
   __shared__ float2 shared[G::kTeams][2][T / 32];
   __shared__ uint64_t bars[G::kTeams * kMostStages];
   extern __shared__ __align__(16) float params[];  // w by place: [K * T * 8]; the rings, whose place the sums [2][K * T * 8] take at last
   const int lane = threadIdx.x % T, team = threadIdx.x / T;
-  auto q = rows_of<X, Y, true, T>(p, reinterpret_cast<unsigned char*>(params), K * T * 32, bars);
+  auto q = rows_of<X, Y, true, T, K>(p, reinterpret_cast<unsigned char*>(params), K * T * 32, bars);
   if (lane == 0) q.start();
   Pair dw[K][4], db[K][4];
 #pragma unroll
@@ -283,7 +318,7 @@ __global__ void __launch_bounds__(Block<T, true>::kThreads, 1) hc_norm_backward_
 #pragma unroll 4
   for (int i = threadIdx.x; i < K * T * 8; i += G::kThreads) {
     const int64_t c = i - q.shift;
-    params[i] = c < 0 || c >= p.width ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
+    params[param_place<K * T * 8>(i)] = c < 0 || c >= p.width ? 0.0f : p.weight ? param_at(p.weight, p.param_type, c) : 1.0f;
   }
   __syncthreads();
   const float inv = 1.0f / (float)p.width;
@@ -301,9 +336,9 @@ __global__ void __launch_bounds__(Block<T, true>::kThreads, 1) hc_norm_backward_
     for (int k = 0; k < K; ++k) {
       const int first = (k * T + lane) * 8 - q.shift;
       Pair h[4], g[4], w[4];
-      take(x, k * T + lane, first, width, h);
-      take(dy, k * T + lane, first, width, g);
-      load_pairs(params + (k * T + lane) * 8, w);
+      take<K>(k, x, k * T + lane, first, width, h);
+      take<K>(k, dy, k * T + lane, first, width, g);
+      load_params<K * T * 8>(params, k * T + lane, w);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         h[j] = (h[j] + minus) * scale;
@@ -325,14 +360,14 @@ __global__ void __launch_bounds__(Block<T, true>::kThreads, 1) hc_norm_backward_
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int first = (k * T + lane) * 8 - q.shift;
-        if (first >= width) continue;
+        if (k == K - 1 && first >= width) continue;
         Pair h[4], g[4], w[4];
         load_pairs(x + (k * T + lane) * 8, h);
         load_pairs(dy + (k * T + lane) * 8, g);
-        load_pairs(params + (k * T + lane) * 8, w);
+        load_params<K * T * 8>(params, k * T + lane, w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) g[j] = fma2(g[j] * w[j], scale, fma2(h[j] + minus, slope, add));
-        store_pairs(dx, first, p.width, g);
+        store_pairs<K>(k, dx, first, width, g);
       }
     }
     st = next_st;
@@ -490,33 +525,39 @@ namespace {
 
 constexpr int64_t kLongestInRegisters = 8192;
 
-// Threads and groups of eight a thread for rows of `width` values (with one group more where rows begin anywhere): as few
-// groups as 128 threads need, then as many as the column sums leave registers for; long rows have two teams, for whose rings
-// there is room.  Forward a warp alone takes rows of up to three groups a thread, with no barrier in its sums (8192 x 768: 12.9 us,
-// 17.7 with 128 threads); back, where it would have 24 column sums a thread, it does not (24.1 us, 20.1 with 128 threads).
+// Threads and groups of eight a thread for rows of `width` values (with one group more where rows begin anywhere).  What a row
+// costs a warp besides its values, some 200 instructions, is shared by as few warps as the registers allow: up to five groups a
+// thread (6001 x 5003 bf16: with 256 threads a row and three groups 43 us forward and 55 us back, with 128 and five 37 and 54).
+// Forward a warp alone takes rows of up to three groups a thread, with no barrier in its sums (8192 x 768: 12.9 us, 17.7 with 128
+// threads); back, where it would have 24 column sums a thread and rings for 16 teams, it does not (24.1 us, 20.1).  Long rows
+// of wide types have fewer teams, for whose rings there is room.
 struct Shape {
   int threads, groups;
 };
-template <bool kBackward>
-Shape shape_of(size_t width) {
+constexpr int block_threads(bool backward, int groups) { return backward || groups > 3 ? 512 : 1024; }
+int ring_stages(bool backward, Shape s, size_t width, size_t bytes) {
+  const size_t groups = (width + 7) / 8 + (width % 8 ? 1 : 0), params = (size_t)s.groups * s.threads * 32 * (backward ? 1 : 2);
+  return (int)((dev::kNormSmem - params) / (block_threads(backward, s.groups) / s.threads) / (groups * 8 * bytes));
+}
+// bytes: of a value of x, and of dy in the backward pass
+Shape shape_of(bool backward, size_t width, size_t bytes) {
   const int need = (int)((width + 7) / 8) + (width % 8 ? 1 : 0);
-  if (!kBackward && need <= 96) return {32, (need + 31) / 32};
+  if (!backward && need <= 96) return {32, (need + 31) / 32};
   if (need <= 128) return {need <= 32 ? 32 : need <= 64 ? 64 : 128, 1};
-  if (need <= 384) return {128, (need + 127) / 128};
-  if (need <= 640) return {256, (need + 255) / 256};
-  return {512, 2};
+  const Shape one = {128, (need + 127) / 128}, two = {256, (need + 255) / 256};
+  if (need <= 640 && ring_stages(backward, one, width, bytes) >= 2) return one;
+  return ring_stages(backward, two, width, bytes) >= 2 ? two : Shape{512, 2};
 }
 int period_of(size_t width) { return width % 8 == 0 ? 1 : width % 4 == 0 ? 2 : width % 2 == 0 ? 4 : 8; }
 bool in_registers(size_t width) { return width <= kLongestInRegisters - (width % 8 ? 8 : 0); }
 
 // Blocks: one an SM, a whole number of them for each place of an aligned group, and no more than have a row for a team
-template <bool kBackward>
-int norm_blocks(size_t rows, size_t width) {
+int norm_blocks(size_t rows, size_t width, int teams) {
   const int sms = device_info().sms > 0 ? device_info().sms : 1;
   if (!in_registers(width)) return (int)(rows < 64 ? rows : 64);
   const int period = period_of(width);
-  const size_t teams = (kBackward ? 512 : 1024) / shape_of<kBackward>(width).threads, most = (size_t)(sms < period ? period : sms / period * period);
-  const size_t blocks = (rows + teams * period - 1) / (teams * period) * period;
+  const size_t most = (size_t)(sms < period ? period : sms / period * period);
+  const size_t blocks = (rows + (size_t)teams * period - 1) / ((size_t)teams * period) * period;
   return (int)(blocks < most ? blocks : most);
 }
 
@@ -534,39 +575,49 @@ int plan_rings(dev::NormParams* p, size_t x_bytes, size_t y_bytes, int teams, in
 
 template <typename X, typename Y, int T, int K>
 cudaError_t run_forward(dev::NormParams p, cudaStream_t stream) {
-  using G = dev::Block<T, false>;
+  using G = dev::Block<T, K, false>;
   const int smem = plan_rings(&p, sizeof(X), 0, G::kTeams, 2 * K * T * 8 * 4, 0);
   if (p.stages < 2) return cudaErrorInvalidConfiguration;
   static unsigned long long allowed = 0;
   const cudaError_t e = allow_smem(dev::hc_norm_kernel<X, Y, T, K>, dev::kNormSmem, &allowed);
   if (e != cudaSuccess) return e;
-  dev::hc_norm_kernel<X, Y, T, K><<<norm_blocks<false>(p.rows, p.width), G::kThreads, smem, stream>>>(p);
+  dev::hc_norm_kernel<X, Y, T, K><<<norm_blocks(p.rows, p.width, G::kTeams), G::kThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 template <typename X, typename Y, int T, int K>
-cudaError_t run_backward(dev::NormParams p, int blocks, cudaStream_t stream) {
-  using G = dev::Block<T, true>;
+cudaError_t run_backward(dev::NormParams p, int* blocks, cudaStream_t stream) {
+  using G = dev::Block<T, K, true>;
   const int smem = plan_rings(&p, sizeof(X), sizeof(Y), G::kTeams, K * T * 8 * 4, 2 * K * T * 8 * 4);
   if (p.stages < 2) return cudaErrorInvalidConfiguration;
   static unsigned long long allowed = 0;
   const cudaError_t e = allow_smem(dev::hc_norm_backward_kernel<X, Y, T, K>, dev::kNormSmem, &allowed);
   if (e != cudaSuccess) return e;
-  dev::hc_norm_backward_kernel<X, Y, T, K><<<blocks, G::kThreads, smem, stream>>>(p);
+  *blocks = norm_blocks(p.rows, p.width, G::kTeams);
+  dev::hc_norm_backward_kernel<X, Y, T, K><<<*blocks, G::kThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
 // f with the threads and groups as constants
 template <bool kBackward, typename F>
-cudaError_t by_shape(size_t width, F f) {
-  const Shape s = shape_of<kBackward>(width);
+cudaError_t by_shape(size_t width, size_t bytes, F f) {
+  const Shape s = shape_of(kBackward, width, bytes);
   if (s.threads == 32) {
     if (s.groups == 1) return f.template run<32, 1>();
     if constexpr (!kBackward) return s.groups == 2 ? f.template run<32, 2>() : f.template run<32, 3>();
   }
   if constexpr (kBackward)
     if (s.threads == 64) return f.template run<64, 1>();
-  if (s.threads == 128) return s.groups == 1 ? f.template run<128, 1>() : s.groups == 2 ? f.template run<128, 2>() : f.template run<128, 3>();
-  if (s.threads == 256) return s.groups == 2 ? f.template run<256, 2>() : f.template run<256, 3>();
+  if (s.threads == 128) {
+    if (s.groups == 1) return f.template run<128, 1>();
+    if (s.groups == 2) return f.template run<128, 2>();
+    if (s.groups == 3) return f.template run<128, 3>();
+    return s.groups == 4 ? f.template run<128, 4>() : f.template run<128, 5>();
+  }
+  if (s.threads == 256) {
+    if constexpr (kBackward)
+      if (s.groups == 2) return f.template run<256, 2>();
+    return s.groups == 3 ? f.template run<256, 3>() : f.template run<256, 4>();
+  }
   return f.template run<512, 2>();
 }
 template <typename X, typename Y>
@@ -581,7 +632,7 @@ struct Forward {
 template <typename X, typename Y>
 struct Backward {
   const dev::NormParams& p;
-  int blocks;
+  int* blocks;
   cudaStream_t stream;
   template <int T, int K>
   cudaError_t run() {
@@ -591,15 +642,16 @@ struct Backward {
 
 template <typename X, typename Y>
 cudaError_t forward(const dev::NormParams& p, cudaStream_t stream) {
-  if (in_registers(p.width)) return by_shape<false>(p.width, Forward<X, Y>{p, stream});
+  if (in_registers(p.width)) return by_shape<false>(p.width, sizeof(X), Forward<X, Y>{p, stream});
   dev::hc_norm_long_kernel<X, Y><<<(unsigned)(p.rows < 65536 ? p.rows : 65536), dev::kLong, 0, stream>>>(p);
   return cudaGetLastError();
 }
 template <typename X, typename Y>
-cudaError_t backward(const dev::NormParams& p, int blocks, cudaStream_t stream) {
-  if (in_registers(p.width)) return by_shape<true>(p.width, Backward<X, Y>{p, blocks, stream});
+cudaError_t backward(const dev::NormParams& p, int* blocks, cudaStream_t stream) {
+  if (in_registers(p.width)) return by_shape<true>(p.width, sizeof(X) + sizeof(Y), Backward<X, Y>{p, blocks, stream});
+  *blocks = norm_blocks(p.rows, p.width, 1);
   if (p.out) dev::hc_norm_long_dx_kernel<X, Y><<<(unsigned)(p.rows < 65536 ? p.rows : 65536), dev::kLong, 0, stream>>>(p);
-  if (p.partial) dev::hc_norm_long_sums_kernel<X, Y><<<dim3((unsigned)((p.width + 255) / 256), blocks), 256, 0, stream>>>(p);
+  if (p.partial) dev::hc_norm_long_sums_kernel<X, Y><<<dim3((unsigned)((p.width + 255) / 256), *blocks), 256, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
@@ -638,7 +690,7 @@ int hc_layer_norm(const void* x, int x_type, const void* weight, const void* bia
 }
 
 size_t hc_layer_norm_backward_bytes(size_t rows, size_t width) {
-  return rows && width ? (size_t)hc::norm_blocks<true>(rows, width) * 2 * width * sizeof(float) : 0;
+  return rows && width ? (size_t)hc::norm_blocks(rows, width, 1) * 2 * width * sizeof(float) : 0;
 }
 
 int hc_layer_norm_backward(const void* dy, int y_type, const void* x, int x_type, const void* weight, int param_type,
@@ -654,11 +706,11 @@ int hc_layer_norm_backward(const void* dy, int y_type, const void* x, int x_type
   }
   if (!x || !dy || !stats) return hc::kErrArgument;
   if (!dx && !dweight) return hc::kOk;
-  const int blocks = hc::norm_blocks<true>(rows, width);
+  int blocks = 0;  // at most as many as with a row a block
   if (dweight && (!scratch || scratch_bytes < hc_layer_norm_backward_bytes(rows, width))) return hc::kErrArgument;
   hc::dev::NormParams p = {x, dy, weight, nullptr, dx, const_cast<float*>(stats), dweight ? static_cast<float*>(scratch) : nullptr,
                            (int64_t)rows, (int64_t)width, 0.0f, param_type, hc::period_of(width), 0, 0, 0};
-  cudaError_t e = hc::by_types(x_type, y_type, [&](auto a, auto b) { return hc::backward<decltype(a), decltype(b)>(p, blocks, stream); });
+  cudaError_t e = hc::by_types(x_type, y_type, [&](auto a, auto b) { return hc::backward<decltype(a), decltype(b)>(p, &blocks, stream); });
   if (e == cudaSuccess && dweight) {
     hc::dev::hc_norm_finish_kernel<<<dim3((unsigned)((width + 31) / 32), 2), dim3(32, 32), 0, stream>>>(
         p.partial, blocks, (int64_t)width, dweight, dbias, param_type);
