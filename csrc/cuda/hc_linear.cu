@@ -97,7 +97,7 @@ struct RowsBackwardParams {
 };
 
 template <typename Y, typename T, bool kVector, int kAct>
-__global__ void __launch_bounds__(256) hc_rows_backward_kernel(const __grid_constant__ RowsBackwardParams p) {
+__global__ void __launch_bounds__(256, kAct == kActNone ? 3 : 2) hc_rows_backward_kernel(const __grid_constant__ RowsBackwardParams p) {
   __shared__ float sums[8][256];
   constexpr int kAtOnce = 4;  // rows whose loads are under way together
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -211,10 +211,11 @@ bool sizes_ok(size_t rows, size_t inner, size_t width) {
 bool stride_ok(size_t stride, size_t least) { return stride >= least && stride < ((size_t)1 << 32); }
 bool product_type(int type) { return type == kBf16 || type == kF16; }
 
-int shares_of(size_t rows, size_t width) {
+// As many blocks as the SMs hold at a time, two each (with an activation; three without), each with a share of the rows.
+int shares_of(size_t rows, size_t width, int activation) {
   const size_t sms = device_info().sms > 0 ? device_info().sms : 1;
   const size_t strips = (width + 255) / 256, most = (rows + 31) / 32;
-  size_t shares = sms * 4 / strips;
+  size_t shares = sms * (activation == kActNone ? 3 : 2) / strips;
   if (shares > most) shares = most;
   if (shares > 128) shares = 128;
   return (int)(shares ? shares : 1);
@@ -256,7 +257,7 @@ BackwardLayout backward_layout(size_t rows, size_t inner, size_t width, int keep
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   const int parts = gemm_parts((int64_t)width, (int64_t)inner, (int64_t)rows);
   BackwardLayout l;
-  l.sums = up((size_t)shares_of(rows, width) * width * sizeof(float));
+  l.sums = up((size_t)shares_of(rows, width, kActNone) * width * sizeof(float));  // the most there are
   l.parts = parts > 1 ? up((size_t)parts * width * ((inner + 7) / 8 * 8) * sizeof(float)) : 0;
   l.total = l.sums + l.parts + (keep_dz ? up(rows * ((width + 7) / 8 * 8) * 2) : 0);
   return l;
@@ -337,7 +338,7 @@ int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void
   if (dbias || (products && keep_dz)) {
     const dev::RowsBackwardParams p = {dy, z, products && keep_dz ? const_cast<void*>(dz) : nullptr, dbias ? reinterpret_cast<float*>(at) : nullptr,
                                        (int64_t)dy_stride, (int64_t)z_stride, (int64_t)dz_stride, (int64_t)rows, (int64_t)width, activation,
-                                       shares_of(rows, width)};
+                                       shares_of(rows, width, activation)};
     const bool vector = aligned_rows(dy, dy_stride) && (activation == kActNone || aligned_rows(z, z_stride));
     if (type == kBf16) {
       if (dy_type == kF32) rows_backward<float, __nv_bfloat16>(p, vector, stream);

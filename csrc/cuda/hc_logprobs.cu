@@ -97,6 +97,11 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ uint64_t key_of(float v, int64_t index) {
   return (uint64_t)ordered(v) << 32 | (0xffffffffu - (uint32_t)index);
 }
+// the value of a key (a zero without its sign)
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t b = (uint32_t)(key >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
 #pragma unroll
@@ -345,14 +350,14 @@ __device__ __forceinline__ void leave_out(const LogprobParams& p, int64_t r) {
     p.top_logprobs[r * p.top + threadIdx.x] = 0.0f;
   }
 }
-// a row whose sums are there
-template <typename T, bool kTop>
-__device__ __forceinline__ void store_row(const LogprobParams& p, int64_t r, int64_t token, const T* row, const Softmax& all, const uint64_t* best) {
+// a row whose sums are there; `logit`: of its token, for thread 0
+template <bool kTop>
+__device__ __forceinline__ void store_row(const LogprobParams& p, int64_t r, int64_t token, float logit, const Softmax& all, const uint64_t* best) {
   const bool sound = all.s > 0.0f && all.s < INFINITY;  // no NaN, no +inf, something above -inf
   const float log_s = logf(all.s);
   if (threadIdx.x == 0) {
     const float h = sound ? log_s - all.t / all.s : NAN;
-    p.logprobs[r] = sound && token >= 0 && token < p.vocab ? to_float(row[token]) - all.m - log_s : NAN;
+    p.logprobs[r] = sound && token >= 0 && token < p.vocab ? logit - all.m - log_s : NAN;
     p.entropy[r] = h;
     if (p.stats) {
       p.stats[r * 3] = sound ? all.m : NAN;
@@ -361,9 +366,10 @@ __device__ __forceinline__ void store_row(const LogprobParams& p, int64_t r, int
     }
   }
   if (kTop && threadIdx.x < p.top) {
-    const int64_t i = 0xffffffffu - (uint32_t)best[threadIdx.x];
+    const uint64_t key = best[threadIdx.x];
+    const int64_t i = 0xffffffffu - (uint32_t)key;
     p.top_tokens[r * p.top + threadIdx.x] = sound ? i : -1;
-    p.top_logprobs[r * p.top + threadIdx.x] = sound ? to_float(row[i]) - all.m - log_s : NAN;
+    p.top_logprobs[r * p.top + threadIdx.x] = sound ? value_of(key) - all.m - log_s : NAN;
   }
 }
 
@@ -435,21 +441,25 @@ __global__ void __launch_bounds__(kRowThreads) hc_logprob_kernel(const __grid_co
   const int part = blockIdx.x % p.cluster;
   const int64_t r = blockIdx.x / p.cluster;
   const int64_t token = p.tokens[r];
-  if (token == p.ignore) {  // the same for all threads of the cluster
-    if (part == 0) leave_out<kTop>(p, r);
-    return;
-  }
   const T* row = static_cast<const T*>(p.x) + r * p.stride;
   const int shift = place_of(row);
   const int64_t groups = (p.vocab + shift + 7) / 8;
   const int64_t begin = groups * part / p.cluster, end = groups * (part + 1) / p.cluster;
+  Logits<T> q[kAtOnce];
+  int64_t g = begin + threadIdx.x;
+  if (g < end) load_some<kRowThreads>(q, row, g, end, shift, p.vocab);  // on its way while the token comes
+  if (token == p.ignore) {  // the same for all threads of the cluster
+    if (part == 0) leave_out<kTop>(p, r);
+    return;
+  }
+  const float logit = part == 0 && threadIdx.x == 0 && token >= 0 && token < p.vocab ? to_float(row[token]) : 0.0f;
   Running<T> run;
   run.clear();
-  int64_t where = begin + threadIdx.x < end ? begin + threadIdx.x : -1;
-  for (int64_t g = begin + threadIdx.x; g < end; g += kAtOnce * kRowThreads) {
-    Logits<T> q[kAtOnce];
-    load_some<kRowThreads>(q, row, g, end, shift, p.vocab);
+  int64_t where = g < end ? g : -1;
+  for (; g < end;) {
     if (run.add(q) && kTop) where = g;
+    g += kAtOnce * kRowThreads;
+    if (g < end) load_some<kRowThreads>(q, row, g, end, shift, p.vocab);
   }
   Softmax a = block_join<kRowThreads>(run.sums(), warp_part);
   if (warp == 0 && lane == 0) block_part = a;
@@ -482,7 +492,7 @@ __global__ void __launch_bounds__(kRowThreads) hc_logprob_kernel(const __grid_co
   } else {
     __syncthreads();
   }
-  if (part == 0) store_row<T, kTop>(p, r, token, row, block_part, sh.best);
+  if (part == 0) store_row<kTop>(p, r, token, logit, block_part, sh.best);
 }
 
 // Many rows: a block stays and has one row after the other brought into a ring in shared memory, in pieces of 32 logits a thread
@@ -562,6 +572,7 @@ __global__ void __launch_bounds__(kStreamThreads, 8) hc_logprob_stream_kernel(co
     }
     const T* row = static_cast<const T*>(p.x) + r * p.stride;
     const int shift = place_of(row);
+    const float logit = threadIdx.x == 0 && token >= 0 && token < p.vocab ? to_float(row[token]) : 0.0f;
     const T* from;
     int64_t groups;
     whole_groups(row, p.vocab, from, groups);
@@ -610,7 +621,7 @@ __global__ void __launch_bounds__(kStreamThreads, 8) hc_logprob_stream_kernel(co
     if (threadIdx.x == 0) block_part = a;
     if (kTop) block_top<kStreamThreads>(p, sh, row, shift, skipped, all, skipped, run.best, where);
     __syncthreads();
-    store_row<T, kTop>(p, r, token, row, block_part, sh.best);
+    store_row<kTop>(p, r, token, logit, block_part, sh.best);
     token = next_token;
     __syncthreads();
   }
