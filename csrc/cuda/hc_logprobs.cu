@@ -689,12 +689,12 @@ bool logits_ok(const void* x, int type, size_t rows, size_t vocab, size_t stride
   return rows == 0 || (x && reinterpret_cast<uintptr_t>(x) % element_bytes(type) == 0 && rows <= (1ull << 60) / stride);
 }
 
-// Blocks per row: as many as leave no SM idle, up to the eight of a portable cluster, while each has at least one group
-// of eight logits for every thread.
+// Blocks per row: as many as have an SM each, up to the eight of a portable cluster, while each has at least one group of
+// eight logits for every other thread (37 rows of 50257: 12.9 us in clusters of eight, two blocks an SM, 10 us with a block a row).
 int cluster_of(size_t rows, size_t vocab) {
   const size_t sms = device_info().sms;
   int c = 1;
-  while (c < 8 && rows * c * 2 <= 2 * sms && vocab / (size_t)(c * 2) >= dev::kRowThreads * 8 / 2) c *= 2;
+  while (c < 8 && rows * c * 2 <= sms && vocab / (size_t)(c * 2) >= dev::kRowThreads * 8 / 2) c *= 2;
   return c;
 }
 
