@@ -8,9 +8,11 @@ namespace hc {
 namespace dev {
 
 // ---- a few rows -----------------------------------------------------------------------------------------------------
-// With up to eight rows the weights are read once and everything else is small: a warp takes two columns of the result,
-// its lanes go along the sum in groups of eight and add up all rows' products, in fp32, joined over the warp at the end.
-// Bound by reading W; the tensor cores would compute 128 rows for these few.
+// With up to sixteen rows the weights are read once and everything else is small, so the kernel is made for reading: sixteen
+// rows of W are a block's, its warps share the sum in stretches of 64, and each lane feeds mma.sync straight from 16-byte
+// loads of W and x, since any order of the sum will do as long as both operands have the same one.  Eight rows of x are the
+// n of one instruction; with three or four of them the instructions would take longer than the memory.  The tensor core's
+// own sum is taken up into fp32 every 16 stretches of a warp, as in the large products.
 struct FewRowsParams {
   const void *x, *w, *bias, *residual;
   void *out, *z;
@@ -27,62 +29,106 @@ __device__ __forceinline__ float act_value(float z, int kind) {
   return z;
 }
 
-template <typename T, int R, bool kVector>
-__global__ void __launch_bounds__(256) hc_few_rows_kernel(const __grid_constant__ FewRowsParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t first = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * 2;
-  if (first >= p.width) return;
-  const bool two = first + 1 < p.width;
-  const T* w0 = static_cast<const T*>(p.w) + first * p.ldw;
-  const T* w1 = two ? w0 + p.ldw : w0;
-  const T* x = static_cast<const T*>(p.x);
-  float sum[2][R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) sum[0][r] = sum[1][r] = 0.0f;
+// Eight elements of a lane for a step of 32 along the sum, as four words; zeros behind the end.
+template <typename T, bool kVector>
+__device__ __forceinline__ uint4 few_group(const T* row, int64_t k, int64_t end, int t) {
+  uint4 w = make_uint4(0, 0, 0, 0);
   if (kVector) {
-    for (int64_t k = lane * 8; k < p.inner; k += 256) {
-      float a[8], b[8], v[8];
-      load8(w0 + k, a);
-      load8(w1 + k, b);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r < p.rows) {
-          load8(x + r * p.ldx + k, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sum[0][r] = fmaf(v[j], a[j], sum[0][r]);
-            sum[1][r] = fmaf(v[j], b[j], sum[1][r]);
-          }
-        }
-      }
-    }
+    if (k + 8 * t < end) w = *reinterpret_cast<const uint4*>(row + k + 8 * t);
   } else {
-    for (int64_t k = lane; k < p.inner; k += 32) {
-      const float a = to_float(w0[k]), b = to_float(w1[k]);
+    // rows that start anywhere: single elements, a row's four lanes next to each other
+    uint32_t v[8];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r < p.rows) {
-          const float v = to_float(x[r * p.ldx + k]);
-          sum[0][r] = fmaf(v, a, sum[0][r]);
-          sum[1][r] = fmaf(v, b, sum[1][r]);
-        }
+    for (int j = 0; j < 8; ++j) v[j] = k + 4 * j + t < end ? *reinterpret_cast<const uint16_t*>(row + k + 4 * j + t) : 0u;
+    w = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void few_mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void few_mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kFewWarps = 16;  // at most, of a block
+constexpr int kFewSteps = 4;   // of 32 along the sum, whose loads are under way together
+
+template <typename T, int N, bool kVector>  // N: eights of rows
+__global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __grid_constant__ FewRowsParams p) {
+  __shared__ float parts[kFewWarps][N * 8][17];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t first = blockIdx.x * 16ll, last = p.width - 1;
+  const T* w0 = static_cast<const T*>(p.w) + (first + g < last ? first + g : last) * p.ldw;
+  const T* w1 = static_cast<const T*>(p.w) + (first + g + 8 < last ? first + g + 8 : last) * p.ldw;
+  const T* x[N];
+  int64_t end[N];  // of a row of x; a row that is not there ends before its start
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int row = n * 8 + g;
+    x[n] = static_cast<const T*>(p.x) + (row < p.rows ? row : 0) * p.ldx;
+    end[n] = row < p.rows ? p.inner : 0;
+  }
+  float sum[N][4], part[N][4];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[n][j] = part[n][j] = 0.0f;
+  int taken = 0;
+  for (int64_t k0 = warp * 64ll; k0 < p.inner; k0 += warps * 128ll) {
+    uint4 a[kFewSteps], b[kFewSteps], v[kFewSteps][N];
+#pragma unroll
+    for (int s = 0; s < kFewSteps; ++s) {
+      const int64_t k = k0 + (s >> 1) * (warps * 64ll) + (s & 1) * 32;
+      a[s] = few_group<T, kVector>(w0, k, p.inner, t);
+      b[s] = few_group<T, kVector>(w1, k, p.inner, t);
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[s][n] = few_group<T, kVector>(x[n], k, end[n], t);
+    }
+#pragma unroll
+    for (int s = 0; s < kFewSteps; ++s)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        few_mma<T>(part[n], a[s].x, b[s].x, a[s].y, b[s].y, v[s][n].x, v[s][n].y);
+        few_mma<T>(part[n], a[s].z, b[s].z, a[s].w, b[s].w, v[s][n].z, v[s][n].w);
       }
+    if (++taken == 8 || k0 + warps * 128ll >= p.inner) {
+      taken = 0;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum[n][j] += part[n][j];
+          part[n][j] = 0.0f;
+        }
     }
   }
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float v = warp_sum(sum[c][r]);
-      const int64_t n = first + c;
-      if (lane == r && r < p.rows && n < p.width) {  // lane r stores row r
-        if (p.bias) v += param_at(p.bias, p.bias_type, n);
-        if (p.z) static_cast<T*>(p.z)[r * p.ldz + n] = from_float<T>(v);
-        v = act_value(v, p.activation);
-        if (p.residual) v += param_at(p.residual, p.out_type, r * p.ldr + n);
-        param_put(p.out, p.out_type, r * p.ldo + n, v);
-      }
-    }
+    for (int j = 0; j < 4; ++j) parts[warp][n * 8 + 2 * t + (j & 1)][g + (j >> 1) * 8] = sum[n][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < N * 128; i += blockDim.x) {
+    const int r = i >> 4;
+    const int64_t n = first + (i & 15);
+    if (r >= p.rows || n >= p.width) continue;
+    float z = 0.0f;
+    for (int w = 0; w < warps; ++w) z += parts[w][r][i & 15];
+    if (p.bias) z += param_at(p.bias, p.bias_type, n);
+    if (p.z) static_cast<T*>(p.z)[r * p.ldz + n] = from_float<T>(z);
+    z = act_value(z, p.activation);
+    if (p.residual) z += param_at(p.residual, p.out_type, r * p.ldr + n);
+    param_put(p.out, p.out_type, r * p.ldo + n, z);
+  }
 }
 
 // ---- rows of the backward pass ----------------------------------------------------------------------------------------
@@ -203,7 +249,7 @@ __global__ void __launch_bounds__(256) hc_add_parts_kernel(const float* parts, i
 namespace {
 
 constexpr size_t kMostSize = (size_t)1 << 26;  // of each side: a tile's sum then stays far below the limit of a wait
-constexpr size_t kFewRows = 8;
+constexpr size_t kFewRows = 16;
 
 bool sizes_ok(size_t rows, size_t inner, size_t width) {
   return inner > 0 && width > 0 && inner < kMostSize && width < kMostSize && rows < kMostSize;
@@ -221,18 +267,18 @@ int shares_of(size_t rows, size_t width, int activation) {
   return (int)(shares ? shares : 1);
 }
 
-template <typename T, int R>
+template <typename T, int N>
 void few_rows_of(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
+  // eight warps a block; sixteen where that leaves SMs without a block and each warp has a step to go
   const unsigned grid = (unsigned)((p.width + 15) / 16);
-  if (vector) dev::hc_few_rows_kernel<T, R, true><<<grid, 256, 0, stream>>>(p);
-  else dev::hc_few_rows_kernel<T, R, false><<<grid, 256, 0, stream>>>(p);
+  const unsigned threads = (int)grid <= device_info().sms && p.inner >= 1024 ? 512 : 256;
+  if (vector) dev::hc_few_rows_kernel<T, N, true><<<grid, threads, 0, stream>>>(p);
+  else dev::hc_few_rows_kernel<T, N, false><<<grid, threads, 0, stream>>>(p);
 }
 template <typename T>
 void few_rows(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
-  if (p.rows == 1) few_rows_of<T, 1>(p, vector, stream);
-  else if (p.rows == 2) few_rows_of<T, 2>(p, vector, stream);
-  else if (p.rows <= 4) few_rows_of<T, 4>(p, vector, stream);
-  else few_rows_of<T, 8>(p, vector, stream);
+  if (p.rows <= 8) few_rows_of<T, 1>(p, vector, stream);
+  else few_rows_of<T, 2>(p, vector, stream);
 }
 
 template <typename Y, typename T, int kAct>
