@@ -946,7 +946,8 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
 
 // Cycles that a launch takes: those of the unit (a pair of SMs, or one) with the most tiles.  A stage of a tile costs what the
 // matrix instructions take or what loading it takes at 64 bytes a cycle, whichever is more, a tile some 1000 for its start
-// and four for each of its columns.
+// and four for each of its columns.  With a single row of tiles no SM finds in L2 what another one has read, and a stage is there
+// some 650 cycles after the one before it (64 rows, a sum of 8192: 44 us with 1024 columns, 47 with 8192).
 struct TileChoice {
   int bn, ctas;
   int64_t cost;
@@ -958,7 +959,8 @@ TileChoice best_tile(const GemmCall& c, int parts) {
   TileChoice best = {0, 0, 0};
   for (const auto& s : shapes) {
     const int64_t tiles = count_tiles<MODE>(c, dev::kBM * s[1], s[0]) * c.batch * parts, units = sms / s[1];
-    const int64_t cost = (tiles + units - 1) / units * (stages * s[2] + 1000 + 4 * s[0]);
+    const int stage = MODE == kGemmLinear && c.m <= dev::kBM * s[1] && s[2] < 650 ? 650 : s[2];
+    const int64_t cost = (tiles + units - 1) / units * (stages * stage + 1000 + 4 * s[0]);
     if (best.bn == 0 || cost < best.cost) best = {s[0], s[1], cost};
   }
   return best;
@@ -1020,8 +1022,8 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
   c.m = m, c.n = n, c.k = k, c.batch = 1;
   int best = 1;
   int64_t least = best_tile<kGemmLinear>(c, 1).cost;
-  for (int parts = 2; parts <= 8; ++parts) {
-    if (k < parts * 1024) break;
+  for (int parts = 2; parts <= 16; ++parts) {
+    if (k < parts * 256) break;
     // the parts are written and read once more, some 3000 bytes a cycle, by a launch that takes some 5000 cycles besides
     const int64_t cost = best_tile<kGemmLinear>(c, parts).cost + 5000 + m * n * 8 * parts / 3000;
     if (cost < least) {
@@ -1034,7 +1036,7 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
   // sums in parts cost 8 % at 8192 x 4096 x 8192 (392 us with a bf16 result, 403 with fp32, 437 with fp32 sums in parts)
-  const bool wide = c.out_type == kF32 && c.parts <= 1 && c.k > dev::kChunk * dev::kBK;
+  const bool wide = c.precise && c.k / (c.parts > 1 ? c.parts : 1) > dev::kChunk * dev::kBK;
   return wide ? run_gemm_mode<dev::kGemmLinearWide>(c, stream) : run_gemm_mode<kGemmLinear>(c, stream);
 }
 

@@ -96,6 +96,7 @@ struct GemmCall {
   int type;  // of the operands
   int64_t m, n, k, batch;
   int parts;  // over 1 (kGemmLinear without anything behind it, batch 1): as many results, each of a part of the sum, as a batch
+  bool precise;  // the sum is wanted with fp32's precision
   GemmOperand a, b;
   GemmSide out, out2;  // result; z, or lo
   GemmSide in, in2;    // residual, c1 or hi; lo
@@ -107,7 +108,7 @@ struct GemmCall {
   const float* scale;  // of each matrix of a batch (kGemmPoly, kGemmUpdate): X is that times what is stored
 };
 
-// Into how many parts the sum of a product with fp32 results is best shared out (1: none).
+// Into how many parts the sum of a product is best shared out (1: none).
 int gemm_parts(int64_t m, int64_t n, int64_t k);
 // act(a b + bias) + residual
 cudaError_t launch_gemm(const GemmCall& call, cudaStream_t stream);

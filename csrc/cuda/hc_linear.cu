@@ -220,27 +220,59 @@ __global__ void __launch_bounds__(256) hc_rows_finish_kernel(const float* partia
 }
 
 // ---- products whose sum is shared out ---------------------------------------------------------------------------------
-// dW has few tiles and a long sum: parts of the sum go to different SMs, which leave fp32 matrices that are added here.
-template <typename T>
-__global__ void __launch_bounds__(256) hc_add_parts_kernel(const float* parts, int n, int64_t rows, int64_t width, int64_t ld, int64_t stride, T* out, int64_t ldo) {
-  const int64_t groups = (width + 7) / 8;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
-    const int64_t r = i / groups, c = (i - r * groups) * 8;
+// A product with few tiles and a long sum gives parts of the sum to different SMs, which leave fp32 matrices; they are added
+// here, in the order of the sum, and what follows a product is done to them.
+struct JoinParams {
+  const float* parts;
+  int64_t ld, stride;  // rows of a part begin at 32 bytes
+  int count;
+  int64_t rows, width;
+  const void *bias, *residual;
+  void *out, *z;
+  int64_t ldr, ldo, ldz;
+  int type, out_type, bias_type, activation;
+};
+// the first `count` of eight values, from element i on
+__device__ __forceinline__ void join_put(void* base, int type, int64_t i, const float (&v)[8], int64_t count) {
+  unsigned char* to = static_cast<unsigned char*>(base) + i * (type == kF32 ? 4 : 2);
+  if (count >= 8 && (reinterpret_cast<uintptr_t>(to) & 15u) == 0) {
+    if (type == kF32) store8(reinterpret_cast<float*>(to), v);
+    else if (type == kBf16) store8(reinterpret_cast<__nv_bfloat16*>(to), v);
+    else store8(reinterpret_cast<__half*>(to), v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) param_put(base, type, i + j, v[j]);
+  }
+}
+__global__ void __launch_bounds__(256) hc_join_kernel(const __grid_constant__ JoinParams p) {
+  const int64_t groups = (p.width + 7) / 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < p.rows * groups; i += gridDim.x * 256ll) {
+    const int64_t r = i / groups, c = (i - r * groups) * 8, count = p.width - c;
+    const float* part = p.parts + r * p.ld + c;
     float s[8], v[8];
-    load8(parts + r * ld + c, s);
-    for (int k = 1; k < n; ++k) {
-      load8(parts + k * stride + r * ld + c, v);
+    load8(part, s);
+    for (int k = 1; k < p.count; ++k) {
+      load8(part + k * p.stride, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
     }
-    T* to = out + r * ldo + c;
-    if (c + 8 <= width && ((reinterpret_cast<uintptr_t>(to) & 15u) == 0)) {
-      store8(to, s);
-    } else {
+    if (p.bias) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j < width) to[j] = from_float<T>(s[j]);
+        if (j < count) s[j] += param_at(p.bias, p.bias_type, c + j);
     }
+    if (p.z) join_put(p.z, p.type, r * p.ldz + c, s, count);
+    if (p.activation != kActNone) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = act_value(s[j], p.activation);
+    }
+    if (p.residual) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < count) s[j] += param_at(p.residual, p.out_type, r * p.ldr + c + j);
+    }
+    join_put(p.out, p.out_type, r * p.ldo + c, s, count);
   }
 }
 
@@ -295,17 +327,48 @@ void rows_backward(const dev::RowsBackwardParams& p, bool vector, cudaStream_t s
   else rows_backward_of<Y, T, kActSilu>(p, vector, stream);
 }
 
-// scratch memory of a backward pass: sums of columns, sums of parts of the rows, dz
+size_t rounded(size_t v, size_t unit) { return (v + unit - 1) / unit * unit; }
+// scratch memory of a product: the parts of its sum
+size_t product_bytes(size_t m, size_t n, size_t k) {
+  const int parts = gemm_parts((int64_t)m, (int64_t)n, (int64_t)k);
+  return parts > 1 ? rounded((size_t)parts * m * rounded(n, 8) * sizeof(float), 256) : 0;
+}
+cudaError_t run_product(GemmCall c, void* scratch, cudaStream_t stream) {
+  c.precise = c.out_type == kF32;
+  const int parts = gemm_parts(c.m, c.n, c.k);
+  if (parts <= 1) return launch_gemm(c, stream);
+  dev::JoinParams p;
+  p.parts = static_cast<const float*>(scratch);
+  p.ld = (c.n + 7) / 8 * 8;
+  p.stride = c.m * p.ld;
+  p.count = parts;
+  p.rows = c.m, p.width = c.n;
+  p.bias = c.bias, p.residual = c.in.data, p.out = c.out.data, p.z = c.out2.data;
+  p.ldr = c.in.ld, p.ldo = c.out.ld, p.ldz = c.out2.ld;
+  p.type = c.type, p.out_type = c.out_type, p.bias_type = c.bias_type, p.activation = c.activation;
+  c.parts = parts;
+  c.out_type = kF32;
+  c.out = {scratch, p.ld, p.stride};
+  c.out2 = c.in = GemmSide{nullptr, 0, 0};
+  c.bias = nullptr;
+  c.activation = kActNone;
+  const cudaError_t e = launch_gemm(c, stream);
+  if (e != cudaSuccess) return e;
+  const int64_t blocks = (p.rows * (p.ld / 8) + 255) / 256;
+  dev::hc_join_kernel<<<(unsigned)(blocks < 2368 ? blocks : 2368), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+// scratch memory of a backward pass: sums of columns, parts of a product's sum, dz
 struct BackwardLayout {
   size_t sums, parts, total;
 };
 BackwardLayout backward_layout(size_t rows, size_t inner, size_t width, int keep_dz) {
-  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  const int parts = gemm_parts((int64_t)width, (int64_t)inner, (int64_t)rows);
   BackwardLayout l;
-  l.sums = up((size_t)shares_of(rows, width, kActNone) * width * sizeof(float));  // the most there are
-  l.parts = parts > 1 ? up((size_t)parts * width * ((inner + 7) / 8 * 8) * sizeof(float)) : 0;
-  l.total = l.sums + l.parts + (keep_dz ? up(rows * ((width + 7) / 8 * 8) * 2) : 0);
+  l.sums = rounded((size_t)shares_of(rows, width, kActNone) * width * sizeof(float), 256);  // the most there are
+  const size_t dx = product_bytes(rows, inner, width), dw = product_bytes(width, inner, rows);  // one after the other
+  l.parts = dx > dw ? dx : dw;
+  l.total = l.sums + l.parts + (keep_dz ? rounded(rows * rounded(width, 8) * 2, 256) : 0);
   return l;
 }
 
@@ -316,9 +379,13 @@ bool aligned_rows(const void* p, size_t stride) { return (reinterpret_cast<uintp
 
 extern "C" {
 
+size_t hc_linear_bytes(size_t rows, size_t inner, size_t width) {
+  return hc::sizes_ok(rows, inner, width) && rows > hc::kFewRows ? hc::product_bytes(rows, width, inner) : 0;
+}
+
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
               const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
-              int activation, size_t rows, size_t inner, size_t width, hc_stream_t stream) {
+              int activation, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes, hc_stream_t stream) {
   using namespace hc;
   if (!product_type(type) || (out_type != kF32 && out_type != type) || !element_type_ok(bias_type)) return kErrArgument;
   if (activation < kActNone || activation > kActSilu || !sizes_ok(rows, inner, width)) return kErrArgument;
@@ -335,6 +402,8 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
   }
   if (!gemm_operand_ok(x, x_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
+  const size_t need = product_bytes(rows, width, inner);
+  if (need && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u) || scratch_bytes < need)) return kErrArgument;
   GemmCall c;
   memset(&c, 0, sizeof(c));
   c.type = type;
@@ -348,7 +417,7 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   c.bias = bias;
   c.bias_type = bias_type;
   c.activation = activation;
-  return launch_gemm(c, stream) == cudaSuccess ? kOk : kErrCuda;
+  return run_product(c, scratch, stream) == cudaSuccess ? kOk : kErrCuda;
 }
 
 size_t hc_linear_backward_bytes(size_t rows, size_t inner, size_t width, int keep_dz) {
@@ -405,30 +474,14 @@ int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void
     c.a = {dz, (int64_t)dz_stride, 0, true};
     c.b = {weight, (int64_t)weight_stride, 0, false};
     c.out = {dx, (int64_t)dx_stride, 0};
-    if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
+    if (run_product(c, at + l.sums, stream) != cudaSuccess) return kErrCuda;
   }
   if (dweight) {
     c.m = width, c.n = inner, c.k = rows;
     c.a = {dz, (int64_t)dz_stride, 0, false};
     c.b = {x, (int64_t)x_stride, 0, false};
     c.out = {dweight, (int64_t)dweight_stride, 0};
-    c.parts = gemm_parts(c.m, c.n, c.k);
-    const int64_t ld = (int64_t)(inner + 7) / 8 * 8, stride = (int64_t)width * ld;
-    float* sums = reinterpret_cast<float*>(at + l.sums);
-    if (c.parts > 1) {
-      c.out_type = kF32;
-      c.out = {sums, ld, stride};
-    }
-    if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
-    if (c.parts > 1) {
-      const int64_t groups = (int64_t)width * (ld / 8);
-      const unsigned grid = (unsigned)((groups + 255) / 256 < 2368 ? (groups + 255) / 256 : 2368);
-      if (type == kBf16)
-        dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__nv_bfloat16*>(dweight), (int64_t)dweight_stride);
-      else
-        dev::hc_add_parts_kernel<<<grid, 256, 0, stream>>>(sums, c.parts, (int64_t)width, (int64_t)inner, ld, stride, static_cast<__half*>(dweight), (int64_t)dweight_stride);
-      if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-    }
+    if (run_product(c, at + l.sums, stream) != cudaSuccess) return kErrCuda;
   }
   return kOk;
 }

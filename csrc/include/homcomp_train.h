@@ -52,9 +52,11 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
 // activation: 0 none, 1 GELU (tanh form), 2 ReLU, 3 SiLU.
 // out = act(x weight^T + bias) + residual; out_type 0 or `type`, residual (NULL: none) of out_type, bias (NULL: none)
 // of bias_type.  z: what the activation is applied to, of `type`, for the backward pass, or NULL.
+// Scratch memory (hc_linear_bytes for the current device, 256-byte aligned) takes the parts of a sum that is shared out; 0: none.
+size_t hc_linear_bytes(size_t rows, size_t inner, size_t width);
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
               const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
-              int activation, size_t rows, size_t inner, size_t width, hc_stream_t stream);
+              int activation, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 // Backward pass: dz = dy act'(z), rounded to `type` for the products; dx = dz weight, dweight = dz^T x (of `type`) and dbias =
 // the sums of dz's columns before rounding (of bias_type), each NULL where it is not wanted.  dy is of dy_type, 0 or `type`.
 // keep_dz: dz is written to the scratch memory; 0 where dy itself is dz and a product can read it (no activation, dy of

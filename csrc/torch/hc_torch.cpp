@@ -32,6 +32,7 @@ struct Api {
   decltype(&hc_layer_norm_backward) layer_norm_backward;
   decltype(&hc_token_logprobs) token_logprobs;
   decltype(&hc_token_logprobs_backward) token_logprobs_backward;
+  decltype(&hc_linear_bytes) linear_bytes;
   decltype(&hc_linear) linear;
   decltype(&hc_linear_backward_bytes) linear_backward_bytes;
   decltype(&hc_linear_backward) linear_backward;
@@ -46,6 +47,7 @@ void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
   HC_BIND(layer_norm_backward);
   HC_BIND(token_logprobs);
   HC_BIND(token_logprobs_backward);
+  HC_BIND(linear_bytes);
   HC_BIND(linear);
   HC_BIND(linear_backward_bytes);
   HC_BIND(linear_backward);
@@ -193,7 +195,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
-constexpr int64_t kFewRows = 8;  // up to here W is read by a kernel that takes rows that begin anywhere
+constexpr int64_t kFewRows = 16;  // up to here W is read by a kernel that takes rows that begin anywhere
 
 Tensor linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t act, int out, at::IntArrayRef shape,
                       Tensor* z) {
@@ -201,8 +203,11 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bi
   const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
   Tensor y = empty_rows(m, n, x.options().dtype(scalar_of(out)), shape);
   if (z && act) *z = empty_rows(m, n, x.options());
+  const size_t need = api.linear_bytes(m, k, n);
+  const Tensor scratch = scratch_of(need, x);
   check(api.linear(x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), type_of(x), ptr(bias), type_of(bias), ptr(residual),
-                   residual ? any_stride(*residual) : 0, y.data_ptr(), out, padded(n), z ? ptr(*z) : nullptr, padded(n), (int)act, m, k, n, stream_of(x)),
+                   residual ? any_stride(*residual) : 0, y.data_ptr(), out, padded(n), z ? ptr(*z) : nullptr, padded(n), (int)act, m, k, n, ptr(scratch), need,
+                   stream_of(x)),
         "linear");
   return y;
 }

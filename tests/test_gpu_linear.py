@@ -97,7 +97,7 @@ def test_sizes(m, k, n, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", range(1, 10))
+@pytest.mark.parametrize("m", [*range(1, 10), 15, 16, 17])
 @pytest.mark.parametrize("k,n", [(768, 2304), (64, 17), (1001, 33), (5000, 100)])
 def test_few_rows(m, k, n):
     check(*make(m, k, n, BF16, m, BF16, F32 if m % 2 else None))
@@ -117,6 +117,17 @@ def test_activations(act, kind, m, k, n):
 @pytest.mark.parametrize("m,k,n", [(3, 64, 96), (130, 128, 100), (260, 64, 512), (50, 70, 33)])
 def test_residuals(residual, act, m, k, n):
     check(*make(m, k, n, BF16, 2, None, residual), act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,act,residual", [(BF16, None, F32), (F16, "gelu_tanh", None), (BF16, "silu", BF16), (BF16, "relu", None)])
+@pytest.mark.parametrize("m,k,n", [(33, 5000, 136), (130, 4104, 1000), (20, 3001, 77), (17, 8192, 8), (300, 6144, 200)])
+def test_long_sums_of_few_tiles(m, k, n, kind, act, residual):
+    """Sums that are shared out over the GPU, in either direction, with all that follows a product."""
+    assert _lib.cuda().hc_linear_bytes(m, k, n) > 0
+    check(*make(m, k, n, kind, m + n, kind, residual), act)
+    x, w, b, r, dy = make(m, n, k, kind, m, kind, residual)
+    check(x, w, b, r, dy, act)
 
 
 @pytest.mark.gpu
@@ -167,7 +178,7 @@ def test_rows_of_another_tensor_stay():
     lib = _lib.cuda()
     for n, stride in ((100, 112), (99, 101)):
         out = torch.full((133, stride), 7.0, dtype=BF16, device="cuda")
-        assert lib.hc_linear(x.data_ptr(), 64, w.data_ptr(), 64, 1, b.data_ptr(), 0, None, 0, out.data_ptr(), 1, stride, None, 0, 0, 130, 64, n,
+        assert lib.hc_linear(x.data_ptr(), 64, w.data_ptr(), 64, 1, b.data_ptr(), 0, None, 0, out.data_ptr(), 1, stride, None, 0, 0, 130, 64, n, None, 0,
                              torch.cuda.current_stream().cuda_stream) == 0
         assert (out[130:] == 7).all() and (out[:, n:] == 7).all()
         assert torch.equal(out[:130, :n], ops.linear(x, w[:n], b[:n]))
@@ -294,7 +305,7 @@ def test_refusals_without_a_gpu():
         ops.linear(torch.ones(2, 8, dtype=BF16), torch.ones(3, 8, dtype=BF16))
     lib = _lib.cuda()
     p = C.c_void_p(4096)  # never read: every call below is refused before anything is launched
-    good = dict(x=p, xs=16, w=p, ws=16, type=1, b=None, bt=0, r=None, rs=0, out=p, ot=1, os=24, z=None, zs=0, act=0, m=32, k=16, n=24)
+    good = dict(x=p, xs=16, w=p, ws=16, type=1, b=None, bt=0, r=None, rs=0, out=p, ot=1, os=24, z=None, zs=0, act=0, m=32, k=16, n=24, scratch=None, bytes=0)
 
     def forward(**kw):
         return lib.hc_linear(*{**good, **kw}.values(), None)

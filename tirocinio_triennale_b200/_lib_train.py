@@ -10,13 +10,14 @@ def declare(lib):
     sz, f, i, l = C.c_size_t, C.c_float, C.c_int, C.c_int64
     sizes = {
         "hc_layer_norm_backward_bytes": [sz, sz],
+        "hc_linear_bytes": [sz, sz, sz],
         "hc_linear_backward_bytes": [sz, sz, sz, i],
         "hc_orthogonalize_bytes": [sz, sz, sz],
     }
     sigs = {
         "hc_layer_norm": [vp, i, vp, vp, i, vp, i, vp, sz, sz, f, vp],
         "hc_layer_norm_backward": [vp, i, vp, i, vp, i, vp, vp, vp, vp, sz, sz, vp, sz, vp],
-        "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp],
+        "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp, sz, vp],
         "hc_linear_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, sz, i, vp, sz, vp, sz, vp, i, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],
         "hc_train_status": [i],
