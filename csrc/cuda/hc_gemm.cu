@@ -948,13 +948,14 @@ cudaError_t run_gemm(const GemmCall& c, cudaStream_t stream) {
 // matrix instructions take or what loading it takes at 64 bytes a cycle, whichever is more, a tile some 1000 for its start
 // and four for each of its columns.  With a single row of tiles no SM finds in L2 what another one has read, and a stage is there
 // some 650 cycles after the one before it (64 rows, a sum of 8192: 44 us with 1024 columns, 47 with 8192).
+int64_t sm_count() { return device_info().sms > 1 ? device_info().sms : 2; }
 struct TileChoice {
   int bn, ctas;
   int64_t cost;
 };
 template <int MODE>
-TileChoice best_tile(const GemmCall& c, int parts) {
-  const int64_t sms = device_info().sms > 1 ? device_info().sms : 2, stages = ((c.k + dev::kBK - 1) / dev::kBK + parts - 1) / parts;
+TileChoice best_tile(const GemmCall& c, int parts, int64_t sms) {
+  const int64_t stages = ((c.k + dev::kBK - 1) / dev::kBK + parts - 1) / parts;
   const int shapes[3][3] = {{256, 2, 512}, {128, 2, 384}, {64, 1, 384}};
   TileChoice best = {0, 0, 0};
   for (const auto& s : shapes) {
@@ -968,7 +969,7 @@ TileChoice best_tile(const GemmCall& c, int parts) {
 
 template <int MODE>
 cudaError_t run_gemm_mode(const GemmCall& c, cudaStream_t stream) {
-  const TileChoice tile = best_tile<MODE>(c, c.parts > 1 ? c.parts : 1);
+  const TileChoice tile = best_tile<MODE>(c, c.parts > 1 ? c.parts : 1, sm_count());
   if (tile.bn == 256) return run_gemm<256, 2, MODE>(c, stream);
   if (tile.bn == 128) return run_gemm<128, 2, MODE>(c, stream);
   return run_gemm<64, 1, MODE>(c, stream);
@@ -976,7 +977,7 @@ cudaError_t run_gemm_mode(const GemmCall& c, cudaStream_t stream) {
 
 // A chain's products with the same tiles.  A product ends with its slowest CTA; the next one begins some 2500 cycles later.
 TileChoice best_chain_tile(const GemmCall& gram, const GemmCall& poly, const GemmCall& update) {
-  const int64_t sms = device_info().sms > 1 ? device_info().sms : 2;
+  const int64_t sms = sm_count();
   const int shapes[3][3] = {{256, 2, 512}, {128, 2, 384}, {64, 1, 384}};
   TileChoice best = {0, 0, 0};
   for (const auto& s : shapes) {
@@ -1021,11 +1022,13 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
   memset(&c, 0, sizeof(c));
   c.m = m, c.n = n, c.k = k, c.batch = 1;
   int best = 1;
-  int64_t least = best_tile<kGemmLinear>(c, 1).cost;
+  if (k < 512) return 1;
+  const int64_t sms = sm_count();
+  int64_t least = best_tile<kGemmLinear>(c, 1, sms).cost;
   for (int parts = 2; parts <= 16; ++parts) {
     if (k < parts * 256) break;
     // the parts are written and read once more, some 3000 bytes a cycle, by a launch that takes some 5000 cycles besides
-    const int64_t cost = best_tile<kGemmLinear>(c, parts).cost + 5000 + m * n * 8 * parts / 3000;
+    const int64_t cost = best_tile<kGemmLinear>(c, parts, sms).cost + 5000 + m * n * 8 * parts / 3000;
     if (cost < least) {
       least = cost;
       best = parts;

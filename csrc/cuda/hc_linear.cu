@@ -11,8 +11,10 @@ namespace dev {
 // With up to sixteen rows the weights are read once and everything else is small, so the kernel is made for reading: sixteen
 // rows of W are a block's, its warps share the sum in stretches of 64, and each lane feeds mma.sync straight from 16-byte
 // loads of W and x, since any order of the sum will do as long as both operands have the same one.  Eight rows of x are the
-// n of one instruction; with three or four of them the instructions would take longer than the memory.  The tensor core's
-// own sum is taken up into fp32 every 16 stretches of a warp, as in the large products.
+// n of one instruction.  The tensor core's own sum is taken up into fp32 every 16 stretches of a warp, as in the large
+// products.  Bound by reading W: one row of 4096 -> 4096 takes 5.9 us (5.7 TB/s), of 8192 -> 8192 27 us (5.0 TB/s), with fp32
+// multiplications in place of mma.sync 8 rows took 39 and 143 us.  Rows of W that begin anywhere cost more loads (12.6 us for
+// 5001 -> 2049, 20 MB).
 struct FewRowsParams {
   const void *x, *w, *bias, *residual;
   void *out, *z;
@@ -29,20 +31,28 @@ __device__ __forceinline__ float act_value(float z, int kind) {
   return z;
 }
 
-// Eight elements of a lane for a step of 32 along the sum, as four words; zeros behind the end.
-template <typename T, bool kVector>
-__device__ __forceinline__ uint4 few_group(const T* row, int64_t k, int64_t end, int t) {
+// Eight 16-bit elements from p on, which may begin anywhere, with zeros from the `count`th on: the three words between an odd
+// element at either end, or the two at the end, shifted into place.
+__device__ __forceinline__ uint4 any_group(const uint16_t* p, int64_t count) {
   uint4 w = make_uint4(0, 0, 0, 0);
-  if (kVector) {
-    if (k + 8 * t < end) w = *reinterpret_cast<const uint4*>(row + k + 8 * t);
+  if (count >= 8) {
+    const bool odd = (reinterpret_cast<uintptr_t>(p) & 2u) != 0;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p + odd);
+    const uint32_t a = q[0], b = q[1], c = q[2], first = p[odd ? 0 : 6], last = p[7];
+    w = odd ? make_uint4(first | a << 16, __funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), c >> 16 | last << 16) : make_uint4(a, b, c, first | last << 16);
   } else {
-    // rows that start anywhere: single elements, a row's four lanes next to each other
     uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + 4 * j + t < end ? *reinterpret_cast<const uint16_t*>(row + k + 4 * j + t) : 0u;
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? p[j] : 0u;
     w = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
   }
   return w;
+}
+// Eight elements of a lane for a step of 32 along the sum; zeros behind the end.
+template <typename T, bool kVector>
+__device__ __forceinline__ uint4 few_group(const T* row, int64_t k, int64_t end, int t) {
+  if (!kVector) return any_group(reinterpret_cast<const uint16_t*>(row + k + 8 * t), end - k - 8 * t);
+  return k + 8 * t < end ? *reinterpret_cast<const uint4*>(row + k + 8 * t) : make_uint4(0, 0, 0, 0);
 }
 template <typename T>
 __device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -60,12 +70,12 @@ __device__ __forceinline__ void few_mma<__half>(float (&d)[4], uint32_t a0, uint
 }
 
 constexpr int kFewWarps = 16;  // at most, of a block
-constexpr int kFewSteps = 4;   // of 32 along the sum, whose loads are under way together
-
 template <typename T, int N, bool kVector>  // N: eights of rows
 __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __grid_constant__ FewRowsParams p) {
   __shared__ float parts[kFewWarps][N * 8][17];
+  constexpr int kSteps = 4;  // of 32 along the sum, whose loads are under way together
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t stride = warps * 32ll * kSteps;
   const int g = lane >> 2, t = lane & 3;
   const int64_t first = blockIdx.x * 16ll, last = p.width - 1;
   const T* w0 = static_cast<const T*>(p.w) + (first + g < last ? first + g : last) * p.ldw;
@@ -84,10 +94,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[n][j] = part[n][j] = 0.0f;
   int taken = 0;
-  for (int64_t k0 = warp * 64ll; k0 < p.inner; k0 += warps * 128ll) {
-    uint4 a[kFewSteps], b[kFewSteps], v[kFewSteps][N];
+  for (int64_t k0 = warp * 64ll; k0 < p.inner; k0 += stride) {
+    uint4 a[kSteps], b[kSteps], v[kSteps][N];
 #pragma unroll
-    for (int s = 0; s < kFewSteps; ++s) {
+    for (int s = 0; s < kSteps; ++s) {
       const int64_t k = k0 + (s >> 1) * (warps * 64ll) + (s & 1) * 32;
       a[s] = few_group<T, kVector>(w0, k, p.inner, t);
       b[s] = few_group<T, kVector>(w1, k, p.inner, t);
@@ -95,13 +105,13 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
       for (int n = 0; n < N; ++n) v[s][n] = few_group<T, kVector>(x[n], k, end[n], t);
     }
 #pragma unroll
-    for (int s = 0; s < kFewSteps; ++s)
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         few_mma<T>(part[n], a[s].x, b[s].x, a[s].y, b[s].y, v[s][n].x, v[s][n].y);
         few_mma<T>(part[n], a[s].z, b[s].z, a[s].w, b[s].w, v[s][n].z, v[s][n].w);
       }
-    if (++taken == 8 || k0 + warps * 128ll >= p.inner) {
+    if (++taken == 32 / kSteps || k0 + stride >= p.inner) {
       taken = 0;
 #pragma unroll
       for (int n = 0; n < N; ++n)
@@ -276,11 +286,23 @@ __global__ void __launch_bounds__(256) hc_join_kernel(const __grid_constant__ Jo
   }
 }
 
+// ---- rows that begin anywhere, as the products read them -----------------------------------------------------------------
+// Rows of 16-bit values, copied to rows that begin at 16 bytes, zeros behind their ends.  Bound by memory: a thread brings eight.
+__global__ void __launch_bounds__(256) hc_align_rows_kernel(const uint16_t* from, int64_t ld, int64_t rows, int64_t width, uint4* to, int64_t groups) {
+  const int64_t used = (width + 7) / 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * used; i += gridDim.x * 256ll) {
+    const int64_t r = i / used, c = i - r * used;
+    to[r * groups + c] = any_group(from + r * ld + c * 8, width - c * 8);
+  }
+}
+
 }  // namespace dev
 
 namespace {
 
 constexpr size_t kMostSize = (size_t)1 << 26;  // of each side: a tile's sum then stays far below the limit of a wait
+// Up to here the kernel for few rows: 8 us with 16 rows of 4096 -> 4096, 30 to 36 of 8192 -> 8192.  The large products take 16 and 37
+// with 17 rows; this kernel with four eights of rows took 16 to 18 and 88 to 108, for every block reads all of x.
 constexpr size_t kFewRows = 16;
 
 bool sizes_ok(size_t rows, size_t inner, size_t width) {
@@ -329,13 +351,11 @@ void rows_backward(const dev::RowsBackwardParams& p, bool vector, cudaStream_t s
 
 size_t rounded(size_t v, size_t unit) { return (v + unit - 1) / unit * unit; }
 // scratch memory of a product: the parts of its sum
-size_t product_bytes(size_t m, size_t n, size_t k) {
-  const int parts = gemm_parts((int64_t)m, (int64_t)n, (int64_t)k);
+size_t product_bytes(int parts, size_t m, size_t n) {
   return parts > 1 ? rounded((size_t)parts * m * rounded(n, 8) * sizeof(float), 256) : 0;
 }
-cudaError_t run_product(GemmCall c, void* scratch, cudaStream_t stream) {
+cudaError_t run_product(GemmCall c, int parts, void* scratch, cudaStream_t stream) {
   c.precise = c.out_type == kF32;
-  const int parts = gemm_parts(c.m, c.n, c.k);
   if (parts <= 1) return launch_gemm(c, stream);
   dev::JoinParams p;
   p.parts = static_cast<const float*>(scratch);
@@ -362,11 +382,14 @@ cudaError_t run_product(GemmCall c, void* scratch, cudaStream_t stream) {
 // scratch memory of a backward pass: sums of columns, parts of a product's sum, dz
 struct BackwardLayout {
   size_t sums, parts, total;
+  int dx_parts, dw_parts;
 };
 BackwardLayout backward_layout(size_t rows, size_t inner, size_t width, int keep_dz) {
   BackwardLayout l;
   l.sums = rounded((size_t)shares_of(rows, width, kActNone) * width * sizeof(float), 256);  // the most there are
-  const size_t dx = product_bytes(rows, inner, width), dw = product_bytes(width, inner, rows);  // one after the other
+  l.dx_parts = gemm_parts((int64_t)rows, (int64_t)inner, (int64_t)width);
+  l.dw_parts = gemm_parts((int64_t)width, (int64_t)inner, (int64_t)rows);
+  const size_t dx = product_bytes(l.dx_parts, rows, inner), dw = product_bytes(l.dw_parts, width, inner);  // one after the other
   l.parts = dx > dw ? dx : dw;
   l.total = l.sums + l.parts + (keep_dz ? rounded(rows * rounded(width, 8) * 2, 256) : 0);
   return l;
@@ -379,8 +402,20 @@ bool aligned_rows(const void* p, size_t stride) { return (reinterpret_cast<uintp
 
 extern "C" {
 
+int hc_align_rows(const void* from, size_t from_stride, size_t rows, size_t width, void* to, size_t to_stride, hc_stream_t stream) {
+  using namespace hc;
+  if (!stride_ok(from_stride, width) || !stride_ok(to_stride, width) || rows >= kMostSize || width >= kMostSize) return kErrArgument;
+  if (rows == 0 || width == 0) return kOk;
+  if (!from || !to || (reinterpret_cast<uintptr_t>(from) & 1u) || !gemm_operand_ok(to, (int64_t)to_stride)) return kErrArgument;
+  const size_t blocks = (rows * ((width + 7) / 8) + 255) / 256, most = (size_t)(device_info().sms > 0 ? device_info().sms : 1) * 8;
+  dev::hc_align_rows_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(
+      static_cast<const uint16_t*>(from), (int64_t)from_stride, (int64_t)rows, (int64_t)width, static_cast<uint4*>(to), (int64_t)to_stride / 8);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
 size_t hc_linear_bytes(size_t rows, size_t inner, size_t width) {
-  return hc::sizes_ok(rows, inner, width) && rows > hc::kFewRows ? hc::product_bytes(rows, width, inner) : 0;
+  return hc::sizes_ok(rows, inner, width) && rows > hc::kFewRows
+             ? hc::product_bytes(hc::gemm_parts((int64_t)rows, (int64_t)width, (int64_t)inner), rows, width) : 0;
 }
 
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
@@ -402,7 +437,8 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
   }
   if (!gemm_operand_ok(x, x_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
-  const size_t need = product_bytes(rows, width, inner);
+  const int parts = gemm_parts((int64_t)rows, (int64_t)width, (int64_t)inner);
+  const size_t need = product_bytes(parts, rows, width);
   if (need && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u) || scratch_bytes < need)) return kErrArgument;
   GemmCall c;
   memset(&c, 0, sizeof(c));
@@ -417,7 +453,7 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   c.bias = bias;
   c.bias_type = bias_type;
   c.activation = activation;
-  return run_product(c, scratch, stream) == cudaSuccess ? kOk : kErrCuda;
+  return run_product(c, parts, scratch, stream) == cudaSuccess ? kOk : kErrCuda;
 }
 
 size_t hc_linear_backward_bytes(size_t rows, size_t inner, size_t width, int keep_dz) {
@@ -474,14 +510,14 @@ int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void
     c.a = {dz, (int64_t)dz_stride, 0, true};
     c.b = {weight, (int64_t)weight_stride, 0, false};
     c.out = {dx, (int64_t)dx_stride, 0};
-    if (run_product(c, at + l.sums, stream) != cudaSuccess) return kErrCuda;
+    if (run_product(c, l.dx_parts, at + l.sums, stream) != cudaSuccess) return kErrCuda;
   }
   if (dweight) {
     c.m = width, c.n = inner, c.k = rows;
     c.a = {dz, (int64_t)dz_stride, 0, false};
     c.b = {x, (int64_t)x_stride, 0, false};
     c.out = {dweight, (int64_t)dweight_stride, 0};
-    if (run_product(c, at + l.sums, stream) != cudaSuccess) return kErrCuda;
+    if (run_product(c, l.dw_parts, at + l.sums, stream) != cudaSuccess) return kErrCuda;
   }
   return kOk;
 }

@@ -52,6 +52,8 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
 // activation: 0 none, 1 GELU (tanh form), 2 ReLU, 3 SiLU.
 // out = act(x weight^T + bias) + residual; out_type 0 or `type`, residual (NULL: none) of out_type, bias (NULL: none)
 // of bias_type.  z: what the activation is applied to, of `type`, for the backward pass, or NULL.
+// hc_align_rows copies rows of 16-bit values that begin anywhere to where a product can read them.
+int hc_align_rows(const void* from, size_t from_stride, size_t rows, size_t width, void* to, size_t to_stride, hc_stream_t stream);
 // Scratch memory (hc_linear_bytes for the current device, 256-byte aligned) takes the parts of a sum that is shared out; 0: none.
 size_t hc_linear_bytes(size_t rows, size_t inner, size_t width);
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,

@@ -32,6 +32,7 @@ struct Api {
   decltype(&hc_layer_norm_backward) layer_norm_backward;
   decltype(&hc_token_logprobs) token_logprobs;
   decltype(&hc_token_logprobs_backward) token_logprobs_backward;
+  decltype(&hc_align_rows) align_rows;
   decltype(&hc_linear_bytes) linear_bytes;
   decltype(&hc_linear) linear;
   decltype(&hc_linear_backward_bytes) linear_backward_bytes;
@@ -47,6 +48,7 @@ void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
   HC_BIND(layer_norm_backward);
   HC_BIND(token_logprobs);
   HC_BIND(token_logprobs_backward);
+  HC_BIND(align_rows);
   HC_BIND(linear_bytes);
   HC_BIND(linear);
   HC_BIND(linear_backward_bytes);
@@ -111,7 +113,14 @@ int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : padde
 bool rows_adjacent(const Tensor& t) { return (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
 // as the products read it: such rows that begin at 16-byte boundaries
 bool is_operand(const Tensor& t) { return rows_adjacent(t) && row_stride(t) % 8 == 0 && aligned(t); }
-Tensor operand(const Tensor& t) { return is_operand(t) ? t : empty_rows(t.size(0), t.size(1), t.options()).copy_(t); }
+Tensor operand(const Tensor& t) {
+  if (is_operand(t)) return t;
+  Tensor copy = empty_rows(t.size(0), t.size(1), t.options());
+  if (!rows_adjacent(t)) return copy.copy_(t);
+  const c10::cuda::CUDAGuard guard(t.device());
+  check(api.align_rows(t.data_ptr(), any_stride(t), t.size(0), t.size(1), copy.data_ptr(), padded(t.size(1)), stream_of(t)), "linear");
+  return copy;
+}
 Tensor adjacent(const Tensor& t) { return rows_adjacent(t) ? t : t.contiguous(); }
 Tensor matrix(const Tensor& t, int64_t width) { return t.dim() == 2 ? t : t.reshape({-1, width}); }
 

@@ -97,7 +97,7 @@ def test_sizes(m, k, n, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [*range(1, 10), 15, 16, 17])
+@pytest.mark.parametrize("m", [*range(1, 10), 15, 16, 17, 33])
 @pytest.mark.parametrize("k,n", [(768, 2304), (64, 17), (1001, 33), (5000, 100)])
 def test_few_rows(m, k, n):
     check(*make(m, k, n, BF16, m, BF16, F32 if m % 2 else None))
@@ -121,7 +121,7 @@ def test_residuals(residual, act, m, k, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,act,residual", [(BF16, None, F32), (F16, "gelu_tanh", None), (BF16, "silu", BF16), (BF16, "relu", None)])
-@pytest.mark.parametrize("m,k,n", [(33, 5000, 136), (130, 4104, 1000), (20, 3001, 77), (17, 8192, 8), (300, 6144, 200)])
+@pytest.mark.parametrize("m,k,n", [(33, 5000, 136), (130, 4104, 1000), (40, 3001, 77), (35, 8192, 8), (300, 6144, 200)])
 def test_long_sums_of_few_tiles(m, k, n, kind, act, residual):
     """Sums that are shared out over the GPU, in either direction, with all that follows a product."""
     assert _lib.cuda().hc_linear_bytes(m, k, n) > 0
@@ -169,6 +169,18 @@ def test_views_batches_and_gradients_with_gaps():
     assert out.shape == (50, 120) and out.dtype == F32
     odd = ops.linear(wide[0, :, :300], w[:113])
     assert odd.shape == (50, 113) and odd.stride(0) % 8 == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,stride,first", [(1, 1, 1, 0), (3, 7, 9, 1), (40, 65, 65, 3), (300, 1001, 1003, 5), (64, 96, 104, 0), (17, 8, 11, 2), (5, 4099, 4099, 7)])
+def test_rows_that_begin_anywhere(rows, width, stride, first):
+    """Copied whole, with zeros up to the next eight, and nothing behind those."""
+    src = torch.randint(-1000, 1000, (first + rows * stride,), dtype=torch.int16, device="cuda")
+    taken = src[first:].as_strided((rows, width), (stride, 1))
+    up = (width + 7) // 8 * 8
+    out = torch.full((rows + 1, up + 8), 77, dtype=torch.int16, device="cuda")
+    assert _lib.cuda().hc_align_rows(taken.data_ptr(), stride, rows, width, out.data_ptr(), up + 8, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out[:rows, :width], taken) and (out[:rows, width:up] == 0).all() and (out[:, up:] == 77).all() and (out[rows] == 77).all()
 
 
 @pytest.mark.gpu
@@ -314,6 +326,13 @@ def test_refusals_without_a_gpu():
                dict(r=p, rs=23), dict(z=p, zs=1), dict(x=None), dict(w=None), dict(out=None), dict(x=C.c_void_p(4098)), dict(xs=17), dict(ws=20), dict(w=C.c_void_p(4104))):
         assert forward(**kw) == 4, kw
     assert forward(m=0) == 0
+    long = dict(m=64, k=16384, xs=16384, ws=16384)
+    assert lib.hc_linear_bytes(64, 16384, 24) > 4096 and lib.hc_linear_bytes(16, 16384, 24) == 0
+    for kw in (dict(), dict(scratch=p, bytes=4096), dict(scratch=C.c_void_p(4104), bytes=1 << 30)):
+        assert forward(**long, **kw) == 4, kw
+    for kw in (dict(fs=15), dict(ts=15), dict(ts=20), dict(m=1 << 26), dict(k=1 << 26), dict(f=None), dict(t=None), dict(f=C.c_void_p(4097)), dict(t=C.c_void_p(4104))):
+        assert lib.hc_align_rows(*{**dict(f=p, fs=17, m=3, k=16, t=p, ts=16), **kw}.values(), None) == 4, kw
+    assert lib.hc_align_rows(p, 17, 0, 16, p, 16, None) == 0
     good = dict(dy=p, dt=1, ds=24, z=p, zs=24, act=0, keep=1, x=p, xs=16, w=p, ws=16, type=1, dx=p, dxs=16, dw=p, dws=16, db=p, bt=0, m=32, k=16, n=24,
                 scratch=p, bytes=1 << 30)
 

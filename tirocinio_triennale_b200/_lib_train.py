@@ -17,6 +17,7 @@ def declare(lib):
     sigs = {
         "hc_layer_norm": [vp, i, vp, vp, i, vp, i, vp, sz, sz, f, vp],
         "hc_layer_norm_backward": [vp, i, vp, i, vp, i, vp, vp, vp, vp, sz, sz, vp, sz, vp],
+        "hc_align_rows": [vp, sz, sz, sz, vp, sz, vp],
         "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp, sz, vp],
         "hc_linear_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, sz, i, vp, sz, vp, sz, vp, i, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],

@@ -31,7 +31,7 @@ def _load():
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
             names = ("hc_layer_norm", "hc_layer_norm_backward_bytes", "hc_layer_norm_backward", "hc_token_logprobs", "hc_token_logprobs_backward",
-                     "hc_linear_bytes", "hc_linear", "hc_linear_backward_bytes", "hc_linear_backward", "hc_orthogonalize_bytes", "hc_orthogonalize")
+                     "hc_align_rows", "hc_linear_bytes", "hc_linear", "hc_linear_backward_bytes", "hc_linear_backward", "hc_orthogonalize_bytes", "hc_orthogonalize")
             module.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in names})
             _module = module
     return _module
