@@ -101,11 +101,21 @@ Tensor packed(const Tensor& t) {
 OptTensor contiguous(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : t; }
 
 int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+// A tensor of shape (rows, width), or `shape`, whose rows are `apart` elements apart: not a view, which autograd would not let
+// be changed in place, but with memory for all of its last row.
+Tensor empty_apart(int64_t rows, int64_t width, int64_t apart, const at::TensorOptions& options, at::IntArrayRef shape = {}) {
+  Tensor t = at::empty({rows, apart}, options);
+  at::DimVector sizes(shape);
+  if (shape.empty()) sizes = {rows, width};
+  at::DimVector strides(sizes.size(), 1);
+  for (int64_t i = (int64_t)sizes.size() - 2, s = apart; i >= 0; s *= std::max<int64_t>(sizes[i], 1), --i) strides[i] = s;
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
+  return t;
+}
 // A matrix whose rows begin at 16-byte boundaries, with gaps where eight does not divide `width`; as `shape` where that is given
 Tensor empty_rows(int64_t rows, int64_t width, const at::TensorOptions& options, at::IntArrayRef shape = {}) {
   if (padded(width) == width) return shape.empty() ? at::empty({rows, width}, options) : at::empty(shape, options);
-  Tensor t = at::empty({rows, padded(width)}, options).narrow(1, 0, width);
-  return shape.size() > 2 || shape.size() == 1 ? t.view(shape) : t;
+  return empty_apart(rows, width, padded(width), options, shape);
 }
 int64_t any_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : padded(t.size(1)); }
@@ -264,7 +274,7 @@ struct Linear : Function<Linear> {
       const Tensor w = want_x ? operand(weight) : weight, a = want_w ? operand(x) : x;
       const size_t need = m ? api.linear_backward_bytes(m, k, n, keep) : 0;
       const Tensor scratch = scratch_of(need, x);
-      check(api.linear_backward(dy.data_ptr(), type_of(dy), any_stride(dy), ptr(z), padded(n), (int)act, keep, a.data_ptr(), row_stride(a), w.data_ptr(),
+      check(api.linear_backward(dy.data_ptr(), type_of(dy), row_stride(dy), ptr(z), padded(n), (int)act, keep, a.data_ptr(), row_stride(a), w.data_ptr(),
                                 row_stride(w), type_of(x), ptr(dx), padded(k), ptr(dw), padded(k), ptr(db), bias_type, m, k, n, ptr(scratch), need,
                                 stream_of(x)),
             "linear backward");
@@ -353,14 +363,13 @@ struct TokenLogprobs : Function<TokenLogprobs> {
     // rows that begin at the same places of 16-byte groups as the logits', so that both move in whole groups; a product whose
     // rows were padded to such groups gets its gradient padded alike
     const int64_t at = vocab + (stride - vocab) % 8;
-    Tensor d = at::empty({rows, at}, logits.options());
-    if (at != vocab) d = d.narrow(1, 0, vocab);
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const Tensor d = empty_apart(rows, vocab, at, logits.options(), shape);
     check(api.token_logprobs_backward(logits.data_ptr(), type_of(logits), rows, vocab, stride, static_cast<int64_t*>(tokens.data_ptr()),
                                       ctx->saved_data["ignore"].toInt(), static_cast<float*>(stats.data_ptr()), static_cast<float*>(ptr(a)),
                                       static_cast<float*>(ptr(b)), d.data_ptr(), at, stream_of(logits)),
           "token_logprobs backward");
-    const auto shape = ctx->saved_data["shape"].toIntVector();
-    return once({shape.size() == 2 ? d : d.view(shape), Tensor(), Tensor(), Tensor()}, graph);
+    return once({d, Tensor(), Tensor(), Tensor()}, graph);
   }
 };
 

@@ -101,6 +101,7 @@ def test_sizes(m, k, n, kind):
 @pytest.mark.parametrize("k,n", [(768, 2304), (64, 17), (1001, 33), (5000, 100)])
 def test_few_rows(m, k, n):
     check(*make(m, k, n, BF16, m, BF16, F32 if m % 2 else None))
+    check(*make(m, k, n, BF16, m, BF16, None if m % 2 else BF16))
 
 
 @pytest.mark.gpu
@@ -181,6 +182,28 @@ def test_rows_that_begin_anywhere(rows, width, stride, first):
     out = torch.full((rows + 1, up + 8), 77, dtype=torch.int16, device="cuda")
     assert _lib.cuda().hc_align_rows(taken.data_ptr(), stride, rows, width, out.data_ptr(), up + 8, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out[:rows, :width], taken) and (out[:rows, width:up] == 0).all() and (out[:, up:] == 77).all() and (out[rows] == 77).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(6,), (1,), (2, 3), ()])
+@pytest.mark.parametrize("n", [24, 33])
+def test_results_can_be_changed_in_place(shape, n):
+    x, w, b, _, _ = make(6, 40, n, BF16)
+    x = (x[0] if shape == () else x[:1] if shape == (1,) else x.reshape(*shape, 40)).requires_grad_()
+    y = ops.linear(x, w, b)
+    assert y.shape == (*shape, n)
+    before = y.detach().clone()
+    y.mul_(2.0)
+    y.sum().backward()
+    assert torch.equal(y.detach(), before * 2)
+    twice = torch.autograd.grad(ops.linear(x, w, b), x, torch.full_like(before, 2.0))[0]
+    assert torch.equal(x.grad, twice)
+
+
+@pytest.mark.gpu
+def test_long_sums_in_parts_with_fp32_results():
+    assert _lib.cuda().hc_linear_bytes(64, 8192, 4096) > 0
+    check(*make(64, 8192, 4096, BF16, 9, BF16, F32))
 
 
 @pytest.mark.gpu
