@@ -340,8 +340,8 @@ void scale(const dev::ScaleParams& p, size_t batch, cudaStream_t stream) {
 constexpr int kSmallSmem = 224 * 1024;
 
 // The form for small matrices: where its tiles fit a warp's registers and shared memory, and a block is done with a matrix
-// sooner than launches of the general form follow one another.  A step of that takes 14 us and some more for large matrices; a
-// block computes about 1.2 MFLOP a microsecond.
+// sooner than the general form goes through its three products.  A step of that takes 16 us and more; a block computes about
+// 1.2 MFLOP a microsecond (five steps of 1 x 128 x 128 take 66 us here, of 1 x 144 x 144 92; of 1 x 145 x 145, the general form, 100).
 bool small_plan(dev::SmallParams* p, size_t batch, size_t height, size_t width, int* smem) {
   const int64_t side = height < width ? height : width, length = height < width ? width : height;
   const int64_t rows = (side + 15) / 16 * 16, long_rows = (length + 15) / 16 * 16;
@@ -354,7 +354,7 @@ bool small_plan(dev::SmallParams* p, size_t batch, size_t height, size_t width, 
   *smem = (int)bytes;
   const int64_t sms = device_info().sms > 0 ? device_info().sms : 1, waves = ((int64_t)batch + sms - 1) / sms;
   const double flop = 2.0 * rows * rows * (2.0 * long_rows + rows);
-  if (waves * flop / 1.2e6 > 14.0) return false;
+  if (waves * flop / 1.2e6 > 16.0) return false;
   p->height = (int)height, p->width = (int)width, p->side = (int)side, p->length = (int)length, p->rows = (int)rows;
   return true;
 }
