@@ -46,6 +46,7 @@ struct GemmParams {
   float ca, cb, cc;
   const float* scale;
   int tma_out, tma_out2, tma_in, tma_in2;              // moved by TMA: rows that begin at 16 bytes
+  int wide_boxes;                                      // map_out and map_out2 are of boxes of 32 x 64 values
 };
 
 __device__ unsigned int g_train_status;
@@ -340,6 +341,31 @@ __device__ __forceinline__ void gemm_fetch(const GemmParams& p, int z, int row0,
   if (MODE == kGemmUpdate) load_box<1>(slot + kSlot / 2, &p.map_in2, col0, row0, z, smem_u32(bar));
 }
 
+// Half of a piece of 64 columns, which only TMA stores: 32 rows of 128 bytes in `out`, what the activation is applied to in `z`.
+__device__ __forceinline__ void gemm_finish_half(const GemmParams& p, float (&v)[32], int half, unsigned char* out, unsigned char* z, float bias,
+                                                 float* shared_bias) {
+  const int lane = threadIdx.x & 31;
+  if (p.bias) {
+    __syncwarp();
+    shared_bias[lane] = bias;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(shared_bias + j);
+      v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+    }
+  }
+  if (p.tma_out2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(wide_at(z, lane, half * 4 + i)) = pack8_as(v + i * 8, p.type);
+  }
+  if (p.activation == kActGeluTanh) activate_all<kActGeluTanh>(v);
+  else if (p.activation == kActRelu) activate_all<kActRelu>(v);
+  else if (p.activation == kActSilu) activate_all<kActSilu>(v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(wide_at(out, lane, half * 4 + i)) = pack8_as(v + i * 8, p.type);
+}
+
 // What the three roles carry from tile to tile (and, in a chain of products, from one to the next).
 struct Loading {
   int s = 0, issued = 0;
@@ -495,7 +521,7 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
     int pieces = row0 < p.m ? (int)min((int64_t)(BN / 32), (p.n - col0 + 31) / 32) : 0;
     if (kSymmetric && pieces) pieces = min(pieces, row0 / 32 - col0 / 32 + 1);
     float bias = 0.0f;
-    if (half < pieces) {
+    if (half < pieces && !(MODE == kGemmLinear && BN >= 128 && p.wide_boxes)) {
       if (fetches && lane == 0) {
         tma_wait_group_read<0>();
         gemm_fetch<kMode>(p, z, row0, col0 + half * 32, mine + (st.uses & 1) * kSlot, &loaded[st.uses & 1]);
@@ -587,6 +613,38 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
           return;
         }
       }
+    } else if (MODE == kGemmLinear && BN >= 128 && p.wide_boxes) {
+      // Half as many pieces and rows of boxes: what a piece costs besides its values (waits, the fence, the store's issue, some
+      // 1300 of 2200 cycles) is what bounds short sums (8192 x 64 -> 2304: 16.5 us instead of 23.3, 8192 x 768 -> 2304: 29 and 32).
+#pragma unroll 1
+      for (int c = half * 2; c < pieces; c += 4) {
+        const int col = col0 + c * 32;
+        float bias2[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (p.bias && col + h * 32 + lane < p.n) bias2[h] = param_at(p.bias, p.bias_type, col + h * 32 + lane);
+        unsigned char* slot = p.tma_out2 ? mine : mine + (st.uses & 1) * kSlot;
+        if (lane == 0) {
+          if (p.tma_out2) tma_wait_group_read<0>();
+          else tma_wait_group_read<1>();
+        }
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tc_load32(lanes + st.acc * BN + (c + h) * 32, sums[0]);
+          tc_load_wait(sums[0]);
+          gemm_finish_half(p, sums[0], h, slot, mine + kSlot, bias2[h], shared_bias);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&p.map_out, col, row0, z, slot);
+          if (p.tma_out2) tma_store_3d(&p.map_out2, col, row0, z, mine + kSlot);
+          tma_commit_group();
+        }
+        ++st.uses;
+      }
+      release_accumulator<kCtas>(sh, st, rank);
     } else {
 #pragma unroll 1
       for (int c = half; c < pieces; c += 2) {
@@ -820,21 +878,21 @@ uint64_t descriptor(bool k_major) {
   return leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// A map of boxes of 32 x 32 values of something beside the accumulator, if its rows begin at 16 bytes.  TMA stores whole 16
+// A map of boxes of 32 x 32 values (`wide`: 32 x 64 of 16 bits) of something beside the accumulator, if its rows begin at 16 bytes.  TMA stores whole 16
 // bytes, also at the end of a row (seen on a B200): what it stores to has rows of whole 16 bytes, or no more behind a row than
 // rounds it up to eight values.
-bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall& c, bool stored, bool mirror = false) {
+bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall& c, bool stored, bool mirror = false, bool wide = false) {
   const size_t bytes = element_bytes(type);
   if (stored && c.n * bytes % 16 && s.ld != (c.n + 7) / 8 * 8) return false;
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn || !s.data || (reinterpret_cast<uintptr_t>(s.data) & 15u) || s.ld * bytes % 16 || (c.batch > 1 && s.stride * bytes % 16)) return false;
   cuuint64_t dims[3] = {(cuuint64_t)c.n, (cuuint64_t)c.m, (cuuint64_t)c.batch};
   cuuint64_t strides[2] = {(cuuint64_t)(s.ld * bytes), (cuuint64_t)((c.batch > 1 ? s.stride : s.ld) * bytes)};
-  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t box[3] = {wide ? 64u : 32u, 32, 1};
   cuuint32_t step[3] = {1, 1, 1};
   return fn(map, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
             s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : type == kF32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : type == kF32 || wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -901,8 +959,10 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.cc = c.cc;
   p.scale = c.scale;
   constexpr bool kLinear = MODE == kGemmLinear || MODE == dev::kGemmLinearWide, kUpdate = MODE == kGemmUpdate;
-  p.tma_out = make_side_map(&p.map_out, c.out, c.out_type, c, true);
-  p.tma_out2 = c.out2.data && (kUpdate || (kLinear && c.out_type != kF32)) && make_side_map(&p.map_out2, c.out2, c.type, c, true);
+  if (MODE == kGemmLinear && BN >= 128 && c.out_type != kF32 && !c.in.data && make_side_map(&p.map_out, c.out, c.out_type, c, true, false, true))
+    p.wide_boxes = !c.out2.data || make_side_map(&p.map_out2, c.out2, c.type, c, true, false, true);
+  p.tma_out = p.wide_boxes || make_side_map(&p.map_out, c.out, c.out_type, c, true);
+  p.tma_out2 = c.out2.data && (kUpdate || (kLinear && c.out_type != kF32)) && (p.wide_boxes || make_side_map(&p.map_out2, c.out2, c.type, c, true));
   p.tma_in = c.in.data && make_side_map(&p.map_in, c.in, kLinear ? c.out_type : kF16, c, false);
   p.tma_in2 = kUpdate && make_side_map(&p.map_in2, c.in2, kF16, c, false);
   // the iteration's own arrays lie as TMA wants them
