@@ -428,6 +428,9 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   if ((residual && !stride_ok(residual_stride, width)) || (z && !stride_ok(z_stride, width))) return kErrArgument;
   if (rows == 0) return kOk;
   if (!x || !weight || !out) return kErrArgument;
+  if (!lies_at(x, 2) || !lies_at(weight, 2) || !lies_at(z, 2) || !lies_at(bias, element_bytes(bias_type)) || !lies_at(residual, element_bytes(out_type)) ||
+      !lies_at(out, element_bytes(out_type)))
+    return kErrArgument;
   if (rows <= kFewRows) {
     const dev::FewRowsParams p = {x, weight, bias, residual, out, z, (int64_t)x_stride, (int64_t)weight_stride, (int64_t)residual_stride,
                                   (int64_t)out_stride, (int64_t)z_stride, (int64_t)inner, (int64_t)width, (int)rows, out_type, bias_type, activation};
@@ -469,6 +472,8 @@ int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void
   if (activation < kActNone || activation > kActSilu || !sizes_ok(rows, inner, width) || !stride_ok(dy_stride, width)) return kErrArgument;
   if (activation != kActNone && !stride_ok(z_stride, width)) return kErrArgument;
   if ((dx && (!stride_ok(weight_stride, inner) || !stride_ok(dx_stride, inner))) || (dweight && (!stride_ok(x_stride, inner) || !stride_ok(dweight_stride, inner))))
+    return kErrArgument;
+  if (!lies_at(dy, element_bytes(dy_type)) || !lies_at(z, 2) || !lies_at(dx, 2) || !lies_at(dweight, 2) || !lies_at(dbias, element_bytes(bias_type)))
     return kErrArgument;
   if (!keep_dz && (dx || dweight) && (activation != kActNone || dy_type != type)) return kErrArgument;
   if (rows == 0) {

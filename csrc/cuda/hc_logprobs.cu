@@ -748,6 +748,9 @@ int hc_token_logprobs(const void* logits, int type, size_t rows, size_t vocab, s
   if (top < 0 || top > hc::dev::kMostTop || (size_t)top > vocab) return hc::kErrArgument;
   if (rows == 0) return hc::kOk;
   if (!tokens || !logprobs || !entropy || (top && (!top_tokens || !top_logprobs))) return hc::kErrArgument;
+  if (!hc::lies_at(tokens, 8) || !hc::lies_at(logprobs, 4) || !hc::lies_at(entropy, 4) || !hc::lies_at(top_tokens, 8) || !hc::lies_at(top_logprobs, 4) ||
+      !hc::lies_at(stats, 4))
+    return hc::kErrArgument;
   hc::dev::LogprobParams p = {logits, tokens, logprobs, entropy, top_tokens, top_logprobs, stats, nullptr, nullptr, nullptr,
                               (int64_t)rows, (int64_t)vocab, (int64_t)stride, 0, ignore, top, 1};
   const cudaError_t e = hc::by_type(type, [&](auto t) {
@@ -762,6 +765,7 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
   if (!hc::logits_ok(logits, type, rows, vocab, stride) || !hc::logits_ok(dlogits, type, rows, vocab, dstride)) return hc::kErrArgument;
   if (rows == 0) return hc::kOk;
   if (!tokens || !stats) return hc::kErrArgument;
+  if (!hc::lies_at(tokens, 8) || !hc::lies_at(stats, 4) || !hc::lies_at(dlogprobs, 4) || !hc::lies_at(dentropy, 4)) return hc::kErrArgument;
   hc::dev::LogprobParams p = {logits, tokens, nullptr, nullptr, nullptr, nullptr, const_cast<float*>(stats), dlogprobs, dentropy, dlogits,
                               (int64_t)rows, (int64_t)vocab, (int64_t)stride, (int64_t)dstride, ignore, 0, 1};
   const size_t chunk = 8 * hc::dev::kAtOnce * hc::dev::kStreamThreads, parts = (vocab + 7 + chunk - 1) / chunk;

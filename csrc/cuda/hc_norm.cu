@@ -684,6 +684,8 @@ int hc_layer_norm(const void* x, int x_type, const void* weight, const void* bia
   if (!hc::norm_arguments_ok(x, x_type, y, y_type, param_type, rows, width) || !(eps >= 0.0f)) return hc::kErrArgument;
   if (rows == 0) return hc::kOk;
   if (!x || !y) return hc::kErrArgument;
+  const size_t param = hc::element_bytes(param_type);
+  if (!hc::lies_at(weight, param) || !hc::lies_at(bias, param) || !hc::lies_at(stats, 8)) return hc::kErrArgument;
   hc::dev::NormParams p = {x, nullptr, weight, bias, y, stats, nullptr, (int64_t)rows, (int64_t)width, eps, param_type, hc::period_of(width), 0, 0, 0};
   const cudaError_t e = hc::by_types(x_type, y_type, [&](auto a, auto b) { return hc::forward<decltype(a), decltype(b)>(p, stream); });
   return e == cudaSuccess ? hc::kOk : hc::kErrCuda;
@@ -697,7 +699,10 @@ int hc_layer_norm_backward(const void* dy, int y_type, const void* x, int x_type
                            const float* stats, void* dx, void* dweight, void* dbias, size_t rows, size_t width,
                            void* scratch, size_t scratch_bytes, hc_stream_t stream) {
   if (!hc::norm_arguments_ok(x, x_type, dy, y_type, param_type, rows, width) || (!dweight != !dbias)) return hc::kErrArgument;
-  if (reinterpret_cast<uintptr_t>(dx) & 15u) return hc::kErrArgument;
+  const size_t param = hc::element_bytes(param_type);
+  if (!hc::lies_at(dx, 16) || !hc::lies_at(weight, param) || !hc::lies_at(dweight, param) || !hc::lies_at(dbias, param) || !hc::lies_at(stats, 8) ||
+      !hc::lies_at(scratch, 256))
+    return hc::kErrArgument;
   if (rows == 0) {
     if (!dweight) return hc::kOk;
     cudaError_t e = cudaMemsetAsync(dweight, 0, width * hc::element_bytes(param_type), stream);

@@ -382,7 +382,7 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   if (!element_type_ok(type) || !matrices_ok(batch, height, width) || stride < width || steps < 1 || steps > 100 || !(eps >= 0.0f)) return kErrArgument;
   if (stride > ((size_t)1 << 32) || batch_stride > ((size_t)1 << 56)) return kErrArgument;
   if (batch == 0) return kOk;
-  if (!g || !out || !scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u)) return kErrArgument;
+  if (!g || !out || !scratch || !lies_at(g, element_bytes(type)) || !lies_at(out, 2) || !lies_at(scratch, 256)) return kErrArgument;
   const Layout l = layout_of(batch, height, width);
   if (scratch_bytes < l.total) return kErrArgument;
   float growth = 1.0f;

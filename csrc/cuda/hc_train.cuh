@@ -10,6 +10,8 @@ namespace hc {
 
 enum ElementType : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 inline size_t element_bytes(int type) { return type == kF32 ? 4 : 2; }
+// nothing, or something that begins where elements of so many bytes may
+inline bool lies_at(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 // The status of the kernels of a source: 0, or 3 after a wait that ran out, kept until it is cleared.
 int norm_status(int clear);
 int logprob_status(int clear);

@@ -6,6 +6,8 @@
 // two graphs) need two of them.  All functions return 0 or a hc::Status code: 4 for arguments that the call does not
 // take, 5 for an error of the CUDA runtime.
 //
+// A pointer that does not begin where its elements may is refused.
+//
 // Types: 0 fp32, 1 bf16, 2 fp16.  Strides count elements from one row to the next; the elements of a row are adjacent.
 #pragma once
 #include <stddef.h>
@@ -20,7 +22,7 @@ typedef struct CUstream_st* hc_stream_t;  // same type as cudaStream_t
 // ---- layer norm ---------------------------------------------------------------------------------------------------
 // y = (x - mean(x)) * rstd * weight + bias over rows of `width` values, rstd = 1 / sqrt(var(x) + eps).
 // x, y (and dy, dx): `rows` rows, one after the other (stride = width), 16-byte aligned; weight / bias: NULL for 1 / 0.
-// stats: 2 floats a row (mean, rstd) for the backward pass, or NULL.
+// stats: 2 floats a row (mean, rstd), 8-byte aligned, for the backward pass, or NULL.
 int hc_layer_norm(const void* x, int x_type, const void* weight, const void* bias, int param_type, void* y, int y_type,
                   float* stats, size_t rows, size_t width, float eps, hc_stream_t stream);
 // dx, and dweight / dbias (both or neither; sums over the rows in fp32, in a fixed order).  dx may be NULL.

@@ -1,13 +1,14 @@
 """The operators of the training step together: the model that runs through them, its gradients, the Muon update, the trainer."""
 import argparse
 import copy
+import ctypes as C
 
 import pytest
 import torch
 import torch.nn.functional as F
 
 from mp_util import run_ranks
-from tirocinio_triennale_b200 import ops
+from tirocinio_triennale_b200 import _lib, ops
 from tirocinio_triennale_b200.models import GPT2, GPT2Config, Muon, muon_with_adamw
 from tirocinio_triennale_b200.models.muon import Optimizers
 
@@ -165,6 +166,31 @@ def test_refusals_without_a_gpu():
     p.grad = torch.zeros(3, 3)
     with pytest.raises(ValueError, match="CUDA"):
         Optimizers(Muon([p])).step()
+
+
+def test_pointers_between_elements_are_refused():
+    """Whatever a call reads or writes begins where its elements may; nothing below is launched."""
+    lib = _lib.cuda()
+    p, odd, half = (C.c_void_p(v) for v in (4096, 4097, 4098))
+    big = 1 << 30
+
+    def refused(name, good, **bad):
+        fn = getattr(lib, name)
+        for key, value in bad.items():
+            assert fn(*{**good, key: value}.values(), None) == 4, (name, key)
+
+    refused("hc_layer_norm", dict(x=p, xt=1, w=p, b=p, pt=0, y=p, yt=1, st=p, rows=4, width=16, eps=1e-5), w=half, b=half, st=half)
+    refused("hc_layer_norm_backward", dict(dy=p, yt=1, x=p, xt=1, w=p, pt=0, st=p, dx=p, dw=p, db=p, rows=4, width=16, scratch=p, bytes=big), w=half, st=half, dx=half, dw=half,
+            db=half, scratch=half)
+    refused("hc_linear", dict(x=p, xs=16, w=p, ws=16, type=1, b=p, bt=0, r=p, rs=24, out=p, ot=0, os=24, z=p, zs=24, act=1, m=3, k=16, n=24, scratch=None, bytes=0), x=odd, w=odd,
+            b=half, r=half, out=half, z=odd)
+    refused("hc_linear_backward", dict(dy=p, dt=0, ds=24, z=p, zs=24, act=1, keep=1, x=p, xs=16, w=p, ws=16, type=1, dx=p, dxs=16, dw=p, dws=16, db=p, bt=0, m=32, k=16, n=24,
+                                       scratch=p, bytes=big), dy=half, z=odd, dx=odd, dw=odd, db=half)
+    refused("hc_token_logprobs", dict(x=p, type=1, rows=4, vocab=16, stride=16, tokens=p, ignore=-100, top=2, lp=p, h=p, tt=p, tl=p, st=p), x=odd, tokens=half, lp=half, h=half, tt=half,
+            tl=half, st=half)
+    refused("hc_token_logprobs_backward", dict(x=p, type=1, rows=4, vocab=16, stride=16, tokens=p, ignore=-100, st=p, a=p, b=p, d=p, ds=16), x=odd, tokens=half, st=half, a=half, b=half,
+            d=odd)
+    refused("hc_orthogonalize", dict(g=p, type=0, batch=2, h=16, w=24, s=24, bs=384, out=p, steps=5, a=3.0, b=-4.0, c=2.0, eps=1e-7, scratch=p, bytes=big), g=half, out=odd)
 
 
 def _trainer(rank, world):
