@@ -207,6 +207,48 @@ def test_long_sums_in_parts_with_fp32_results():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(5, 512, 96), (16, 1001, 50), (64, 8192, 200), (300, 256, 130)])
+def test_a_row_of_nan_and_infinities_keeps_to_itself(m, k, n):
+    x, w, b, _, _ = make(m, k, n, BF16, 4)
+    clean = ops.linear(x, w, b, activation="silu")
+    bad = x.clone()
+    bad[1, 3], bad[2, 5] = float("nan"), float("inf")
+    out = ops.linear(bad, w, b, activation="silu")
+    assert out[1].isnan().all() and not out[2].isfinite().all()
+    keep = [i for i in range(m) if i not in (1, 2)]
+    assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.gpu
+def test_shared_sums_captured_and_on_two_streams():
+    """Each call has its own parts of a sum: two graphs and two streams at once give what one call gives."""
+    cases = [make(64, 8192, 256, BF16, 7), make(48, 6144, 512, BF16, 8)]
+    want = [ops.linear(x, w, b) for x, w, b, _, _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for (x, w, b, _, _), side in zip(cases, streams):
+            with torch.cuda.stream(side):
+                got.append(ops.linear(x, w, b))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, y) for g, y in zip(got, want))
+    graphs, outs = [], []
+    pool = torch.cuda.graph_pool_handle()
+    for x, w, b, _, _ in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(ops.linear(x, w, b))
+        graphs.append(graph)
+    for _ in range(2):
+        for (x, w, b, _, _), graph, out in zip(cases, graphs, outs):
+            x.neg_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ops.linear(x, w, b))
+
+
+@pytest.mark.gpu
 def test_rows_of_another_tensor_stay():
     """Tiles that reach over the last row and column store nothing there."""
     x, w, b, _, _ = make(130, 64, 100, BF16, 5)
