@@ -18,12 +18,12 @@ enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActRelu = 2, kActSilu =
 namespace dev {
 
 // Activations of two values at a time.  GELU (tanh form) and SiLU are z sigmoid(v), with v = 2 sqrt(2 / pi) (z + 0.044715 z^3)
-// or z; sigmoid(v) = 1 / (1 + e) with e = exp(-v), and one reciprocal, of the product of both sums, serves both values: exp and
-// reciprocal are what these functions cost.  z is raised to where e is 2^60 and the function within 1e-16 of 0, so that
-// the product stays in range.
+// or z; sigmoid(v) = 1 / (1 + e) with e = exp(-v).  Each value has its own exp and reciprocal: with one reciprocal for both, of
+// the product of their sums, a value's last bits depended on its neighbour, and a NaN made the neighbour one.  z is raised to where
+// e is about 2^60 and the function within 1e-16 of 0: minus infinity times 0 would not be a number.
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f * 1.5957691216057308f;
-constexpr float kGeluLeast = -7.5f, kSiluLeast = -41.5f;  // v = -41.6, -41.5
+constexpr float kGeluLeast = -7.5f, kSiluLeast = -41.5f;  // v = -42.1, -41.5
 
 __device__ __forceinline__ float act_max_nan(float a, float b) {
   float r;
@@ -37,14 +37,13 @@ __device__ __forceinline__ float act_min_nan(float a, float b) {
 }
 // sigmoid of both v, given v times -log2(e)
 __device__ __forceinline__ Pair sigmoid_pair(Pair exponent) {
-  float a, b, r;
+  float a, b;
   parts(exponent, a, b);
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(a));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(b));
-  a += 1.0f;
-  b += 1.0f;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
-  return pair(b, a) * pair(r, r);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(a + 1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(b + 1.0f));
+  return pair(a, b);
 }
 template <int kAct>
 __device__ __forceinline__ void activate_pair(float& x, float& y) {

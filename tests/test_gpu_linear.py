@@ -411,3 +411,65 @@ def test_refusals_without_a_gpu():
         assert backward(**kw) == 4, kw
     assert backward(dx=None, dw=None, db=None) == 0
     assert lib.hc_linear_backward_bytes(0, 16, 24, 1) == 0
+
+
+def _columns_apart(m, k, n, act, out_dtype, spoil):
+    """What a call gives in all columns but one, with that one spoilt and without."""
+    x, w, b, _, _ = make(m, k, n, BF16, 11)
+    dy = torch.randn(m, n, generator=torch.Generator().manual_seed(12)).to(out_dtype or BF16).cuda()
+    at = 5
+    keep = [i for i in range(n) if i != at]
+
+    def step():
+        leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+        y = ops.linear(*leaves, activation=act, out_dtype=out_dtype)
+        _, dw, db = torch.autograd.grad(y, leaves, dy)
+        return y.detach()[:, keep], dw[keep], db[keep], y.detach()[:, at]
+
+    clean = step()
+    spoil(w, b, at)
+    return clean, step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [None, "gelu_tanh", "silu", "relu"])
+@pytest.mark.parametrize("m,k,n", [(16, 96, 50), (17, 96, 50), (300, 264, 200), (64, 8192, 200), (1000, 64, 512)])
+@pytest.mark.parametrize("out_dtype", [None, F32])
+def test_a_column_of_nan_keeps_to_itself(m, k, n, act, out_dtype):
+    """A bad output unit (NaN in its bias or in its weights) is that unit's alone: every other column of the result, row of
+    the weights' gradient and element of the bias's has the bits that it has without it."""
+
+    def bias(w, b, at):
+        b[at] = float("nan")
+
+    def weight(w, b, at):
+        w[at, 3] = float("nan")
+
+    def infinite(w, b, at):
+        w[at] = 0  # inf - inf in every row
+        w[at, :2] = torch.tensor([float("inf"), -float("inf")])
+
+    for spoil in (bias, weight, infinite):
+        clean, got = _columns_apart(m, k, n, act, out_dtype, spoil)
+        assert not torch.isfinite(got[3]).all() and (spoil is infinite or torch.isnan(got[3]).all())
+        assert all(torch.isfinite(c).all() and torch.equal(c, g) for c, g in zip(clean[:3], got[:3]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
+@pytest.mark.parametrize("out_dtype", [None, F32])
+def test_a_value_does_not_depend_on_its_neighbour(act, out_dtype):
+    """Columns of which each second one is changed: the others keep their bits, as does their gradient."""
+    x, w, b, _, _ = make(300, 264, 200, BF16, 13)
+    dy = torch.randn(300, 200, generator=torch.Generator().manual_seed(14)).to(out_dtype or BF16).cuda()
+
+    def step(w, b):
+        leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+        y = ops.linear(*leaves, activation=act, out_dtype=out_dtype)
+        _, dw, db = torch.autograd.grad(y, leaves, dy)
+        return y.detach()[:, ::2], dw[::2], db[::2]
+
+    want = step(w, b)
+    w[1::2] *= 3
+    b[1::2] -= 2
+    assert all(torch.equal(p, q) for p, q in zip(want, step(w, b)))
