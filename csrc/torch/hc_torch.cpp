@@ -6,6 +6,9 @@
 // of homcomp_train.h, whose addresses it is given when it is loaded (so that it runs whichever build of the library is loaded).
 // It is built by g++ against torch's headers and links nothing of the library.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -69,6 +72,27 @@ int type_of(const OptTensor& t) { return t ? type_of(*t) : 0; }
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// The kernels run outside of torch's dispatcher: a tangent would be lost without a word, and a recording of a call would hold its
+// results' allocation and nothing that fills them.
+void not_recorded() {
+  bool recorded = at::tracer::impl::is_dispatch_enabled();
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (Modes::any_modes_set())
+    for (int8_t i = 0; i < static_cast<int8_t>(c10::impl::TorchDispatchModeKey::NUM_MODE_KEYS); ++i)
+      recorded = recorded || Modes::get_mode(static_cast<c10::impl::TorchDispatchModeKey>(i)).has_value();
+  TORCH_CHECK_NOT_IMPLEMENTED(!recorded, "the operators of a training step cannot be recorded (torch.jit.trace, make_fx, fake tensors)");
+}
+void ordinary(const char* name, const Tensor& t) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet others({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                        DispatchKey::FuncTorchVmapMode, DispatchKey::Batched, DispatchKey::ZeroTensor});
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.key_set().has_any(others), name, ": vmap, functional transforms and tensor subclasses are not implemented for the operators of a training step");
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
+                              ": forward-mode derivatives are not implemented for the operators of a training step");
+}
+void ordinary(const char* name, const OptTensor& t) {
+  if (t) ordinary(name, *t);
+}
 void floating(const char* name, const Tensor& t) {
   TORCH_CHECK_VALUE(type_of(t) != kNoType, name, ": expected a float32, bfloat16 or float16 tensor");
   TORCH_CHECK_VALUE(t.is_cuda(), name, ": expected a CUDA tensor");
@@ -178,6 +202,8 @@ struct LayerNorm : Function<LayerNorm> {
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+    not_recorded();
+    ordinary("gradient", grads[0]);
     const int64_t inputs = ctx->saved_data["inputs"].toInt();
     const int param_type = (int)ctx->saved_data["param_type"].toInt();
     const c10::cuda::CUDAGuard guard(x.device());
@@ -201,6 +227,10 @@ struct LayerNorm : Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int out) {
+  not_recorded();
+  ordinary("x", x);
+  ordinary("weight", weight);
+  ordinary("bias", bias);
   floating("x", x);
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm: x has no columns");
   if (out == kNoType) out = type_of(x);
@@ -264,6 +294,8 @@ struct Linear : Function<Linear> {
     const at::NoGradGuard no_grad;
     Tensor dx, dw, db;
     if (want_x || want_w || want_b) {
+      not_recorded();
+      ordinary("gradient", grads[0]);
       const Tensor dy = adjacent(matrix(grads[0], n));
       // dz is written where dy itself is not what the products can read
       const int keep = act || dy.scalar_type() != x.scalar_type() || !is_operand(dy);
@@ -284,6 +316,11 @@ struct Linear : Function<Linear> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t act, const OptTensor& residual, int out) {
+  not_recorded();
+  ordinary("x", x);
+  ordinary("weight", weight);
+  ordinary("bias", bias);
+  ordinary("residual", residual);
   floating("x", x);
   floating("weight", weight);
   beside("weight", weight, x);
@@ -355,6 +392,9 @@ struct TokenLogprobs : Function<TokenLogprobs> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
     if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    not_recorded();
+    for (int i = 0; i < 2; ++i)
+      if (grads[i].defined()) ordinary("gradient", grads[i]);
     const c10::cuda::CUDAGuard guard(logits.device());
     const bool graph = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
@@ -374,6 +414,9 @@ struct TokenLogprobs : Function<TokenLogprobs> {
 };
 
 std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top, int64_t ignore) {
+  not_recorded();
+  ordinary("logits", logits);
+  ordinary("tokens", tokens);
   floating("logits", logits);
   TORCH_CHECK_VALUE(logits.dim() > 0 && logits.size(-1) > 0, "token_logprobs: logits have no vocabulary");
   const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
@@ -391,6 +434,8 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor& lo
 
 // ---- orthogonalised updates -----------------------------------------------------------------------------------------
 Tensor orthogonalize(const Tensor& update, int64_t steps, double a, double b, double c, double eps) {
+  not_recorded();
+  ordinary("update", update);
   floating("update", update);
   TORCH_CHECK_VALUE(update.dim() >= 2 && update.size(-1) > 0 && update.size(-2) > 0, "orthogonalize: expected matrices, got shape ", update.sizes());
   TORCH_CHECK_VALUE(steps >= 1 && steps <= 100 && eps >= 0, "orthogonalize: 1 to 100 steps, eps not negative");

@@ -208,3 +208,63 @@ def _trainer(rank, world):
 @pytest.mark.gpu
 def test_trainer_with_the_operators_and_compressed_gradients():
     run_ranks(_trainer, 1, backend="nccl")
+
+
+def _calls(device):
+    """Every operator as a function of one of its tensors, with that tensor: name, function, tensor."""
+    f, h = torch.float32, torch.bfloat16
+    g = torch.Generator().manual_seed(5)
+    some = lambda *s, t=f: torch.randn(*s, generator=g).to(t).to(device)  # noqa: E731
+    x, w, b = some(6, 16), some(16), some(16)
+    xh, wh, bh, r = some(20, 16, t=h), some(24, 16, t=h), some(24), some(20, 24)
+    logits, tokens = some(5, 33), torch.arange(5, device=device)
+    return [("norm x", lambda v: ops.layer_norm(v, w, b), x), ("norm weight", lambda v: ops.layer_norm(x, v, b), w), ("norm bias", lambda v: ops.layer_norm(x, w, v), b),
+            ("linear x", lambda v: ops.linear(v, wh, bh, residual=r), xh), ("linear weight", lambda v: ops.linear(xh, v, bh, residual=r), wh),
+            ("linear bias", lambda v: ops.linear(xh, wh, v, residual=r), bh), ("linear residual", lambda v: ops.linear(xh, wh, bh, residual=v), r),
+            ("logits", lambda v: ops.token_logprobs(v, tokens).logprobs, logits), ("update", lambda v: ops.orthogonalize(v), some(8, 12))]
+
+
+def _refuses_what_it_cannot_do(device):
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for name, call, v in _calls(device):
+        with forward_ad.dual_level():
+            for leaf in (v.clone(), v.clone().requires_grad_()):
+                with pytest.raises(NotImplementedError, match="forward"):
+                    call(forward_ad.make_dual(leaf, torch.ones_like(v)))
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(call, (v,), check_trace=False)
+        for kind in ("real", "fake"):
+            with pytest.raises(NotImplementedError):
+                make_fx(call, tracing_mode=kind)(v)
+        for transformed in (lambda v=v: torch.vmap(call)(torch.stack([v, v])), lambda v=v: torch.func.jvp(call, (v,), (v,)), lambda v=v: torch.func.grad(lambda u: call(u).float().sum())(v)):
+            with pytest.raises(NotImplementedError):
+                transformed()
+
+
+def test_forward_mode_tracing_and_transforms_are_refused():
+    """A result made outside of torch's dispatcher has no tangent, and a recording of the call would hold an allocation that nothing fills."""
+    _refuses_what_it_cannot_do("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_tracing_and_transforms_are_refused_on_a_gpu():
+    _refuses_what_it_cannot_do("cuda")
+    assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+def test_gradients_with_a_tangent_are_refused():
+    """Forward mode over the backward pass: a Hessian-vector product, of which the gradient's tangent would be lost."""
+    import torch.autograd.forward_ad as forward_ad
+
+    for name, call, v in _calls("cuda"):
+        if name in ("update", "linear residual"):  # no gradient; one that is handed through
+            continue
+        leaf = v.clone().requires_grad_()
+        y = call(leaf)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.autograd.grad(y, leaf, dual)

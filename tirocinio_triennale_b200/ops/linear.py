@@ -19,7 +19,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     Everything behind the product happens before the result is stored.  For the backward pass of an activation its argument is
     kept in ``x``'s type, and the gradient is rounded to that type before it enters the products; gradients of ``x`` and ``weight``
     have their types, that of ``bias`` its own, summed in float32 in a fixed order.  Where eight does not divide ``width`` the
-    result's rows are kept apart so that they begin at 16-byte boundaries: it has gaps."""
+    result's rows are kept apart so that they begin at 16-byte boundaries: it has gaps.
+
+    Forward-mode derivatives, vmap and recorded (traced) calls raise NotImplementedError."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError("linear: activation is one of %s" % ", ".join(map(str, ACTIVATIONS)))

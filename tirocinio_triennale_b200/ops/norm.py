@@ -13,5 +13,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``x``: float32, bfloat16 or float16, any shape; ``weight`` and ``bias``: one value per column, both of one of these types.
     The result has ``x``'s type, or ``out_dtype``: a float32 residual stream can give bfloat16 rows to a product, which saves a
     conversion.  Of the two 16-bit types one call takes only one.  Statistics and sums are held in float32; the sums of the
-    gradients of ``weight`` and ``bias`` are formed in a fixed order.  Tensors with gaps are copied."""
+    gradients of ``weight`` and ``bias`` are formed in a fixed order.  Tensors with gaps are copied.
+
+    Forward-mode derivatives, vmap and recorded (traced) calls raise NotImplementedError."""
     return native().layer_norm(x, weight, bias, eps, type_code(out_dtype))
