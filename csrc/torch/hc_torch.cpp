@@ -93,6 +93,9 @@ void ordinary(const char* name, const Tensor& t) {
 void ordinary(const char* name, const OptTensor& t) {
   if (t) ordinary(name, *t);
 }
+// A view may stand for the negative of what lies in its memory (the imaginary part of a conjugate does; gradients may)
+Tensor held(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+OptTensor held(const OptTensor& t) { return t ? OptTensor(held(*t)) : t; }
 void floating(const char* name, const Tensor& t) {
   TORCH_CHECK_VALUE(type_of(t) != kNoType, name, ": expected a float32, bfloat16 or float16 tensor");
   TORCH_CHECK_VALUE(t.is_cuda(), name, ": expected a CUDA tensor");
@@ -213,7 +216,7 @@ struct LayerNorm : Function<LayerNorm> {
                want_b = (inputs & 2) && ctx->needs_input_grad((inputs & 1) ? 2 : 1), sums = want_w || want_b;
     const bool graph = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
-    const Tensor dy = packed(grads[0]);
+    const Tensor dy = packed(held(grads[0]));
     const Tensor dx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
     const at::TensorOptions params = x.options().dtype(scalar_of(param_type));
     const Tensor dw = sums ? at::empty({width}, params) : Tensor(), db = sums ? at::empty({width}, params) : Tensor();
@@ -226,11 +229,13 @@ struct LayerNorm : Function<LayerNorm> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int out) {
+Tensor layer_norm(const Tensor& x_, const OptTensor& weight_, const OptTensor& bias_, double eps, int out) {
   not_recorded();
-  ordinary("x", x);
-  ordinary("weight", weight);
-  ordinary("bias", bias);
+  ordinary("x", x_);
+  ordinary("weight", weight_);
+  ordinary("bias", bias_);
+  const Tensor x = held(x_);
+  const OptTensor weight = held(weight_), bias = held(bias_);
   floating("x", x);
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm: x has no columns");
   if (out == kNoType) out = type_of(x);
@@ -296,7 +301,7 @@ struct Linear : Function<Linear> {
     if (want_x || want_w || want_b) {
       not_recorded();
       ordinary("gradient", grads[0]);
-      const Tensor dy = adjacent(matrix(grads[0], n));
+      const Tensor dy = adjacent(matrix(held(grads[0]), n));
       // dz is written where dy itself is not what the products can read
       const int keep = act || dy.scalar_type() != x.scalar_type() || !is_operand(dy);
       const auto shape = ctx->saved_data["shape"].toIntVector();
@@ -315,12 +320,14 @@ struct Linear : Function<Linear> {
   }
 };
 
-Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t act, const OptTensor& residual, int out) {
+Tensor linear(const Tensor& x_, const Tensor& weight_, const OptTensor& bias_, int64_t act, const OptTensor& residual_, int out) {
   not_recorded();
-  ordinary("x", x);
-  ordinary("weight", weight);
-  ordinary("bias", bias);
-  ordinary("residual", residual);
+  ordinary("x", x_);
+  ordinary("weight", weight_);
+  ordinary("bias", bias_);
+  ordinary("residual", residual_);
+  const Tensor x = held(x_), weight = held(weight_);
+  const OptTensor bias = held(bias_), residual = held(residual_);
   floating("x", x);
   floating("weight", weight);
   beside("weight", weight, x);
@@ -399,7 +406,7 @@ struct TokenLogprobs : Function<TokenLogprobs> {
     const bool graph = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     const int64_t rows = logits.size(0), vocab = logits.size(1), stride = any_stride(logits);
-    const Tensor a = grads[0].defined() ? grads[0].contiguous() : Tensor(), b = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor a = grads[0].defined() ? held(grads[0]).contiguous() : Tensor(), b = grads[1].defined() ? held(grads[1]).contiguous() : Tensor();
     // rows that begin at the same places of 16-byte groups as the logits', so that both move in whole groups; a product whose
     // rows were padded to such groups gets its gradient padded alike
     const int64_t at = vocab + (stride - vocab) % 8;
@@ -413,10 +420,11 @@ struct TokenLogprobs : Function<TokenLogprobs> {
   }
 };
 
-std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top, int64_t ignore) {
+std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor& logits_, const Tensor& tokens_, int64_t top, int64_t ignore) {
   not_recorded();
-  ordinary("logits", logits);
-  ordinary("tokens", tokens);
+  ordinary("logits", logits_);
+  ordinary("tokens", tokens_);
+  const Tensor logits = held(logits_), tokens = held(tokens_);
   floating("logits", logits);
   TORCH_CHECK_VALUE(logits.dim() > 0 && logits.size(-1) > 0, "token_logprobs: logits have no vocabulary");
   const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
@@ -433,9 +441,10 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor& lo
 }
 
 // ---- orthogonalised updates -----------------------------------------------------------------------------------------
-Tensor orthogonalize(const Tensor& update, int64_t steps, double a, double b, double c, double eps) {
+Tensor orthogonalize(const Tensor& update_, int64_t steps, double a, double b, double c, double eps) {
   not_recorded();
-  ordinary("update", update);
+  ordinary("update", update_);
+  const Tensor update = held(update_);
   floating("update", update);
   TORCH_CHECK_VALUE(update.dim() >= 2 && update.size(-1) > 0 && update.size(-2) > 0, "orthogonalize: expected matrices, got shape ", update.sizes());
   TORCH_CHECK_VALUE(steps >= 1 && steps <= 100 && eps >= 0, "orthogonalize: 1 to 100 steps, eps not negative");

@@ -268,3 +268,23 @@ def test_gradients_with_a_tangent_are_refused():
             dual = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
             with pytest.raises(NotImplementedError, match="forward"):
                 torch.autograd.grad(y, leaf, dual)
+
+
+@pytest.mark.gpu
+def test_views_that_are_the_negative_of_what_lies_there():
+    """The imaginary part of a conjugate is such a view; so can gradients be."""
+    for name, call, v in _calls("cuda"):
+        want = call((-v).contiguous())
+        assert torch.equal(call(torch._neg_view(v)), want), name
+        if name == "update":
+            continue
+        leaf = v.clone().requires_grad_()
+        y = call(leaf)
+        dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(6)).to(y.dtype).cuda()
+        (want,) = torch.autograd.grad(y, leaf, -dy, retain_graph=True)
+        (got,) = torch.autograd.grad(y, leaf, torch._neg_view(dy))
+        assert torch.equal(got, want), name
+        leaf = torch._neg_view(v.clone()).requires_grad_()
+        (got,) = torch.autograd.grad(call(leaf), leaf, dy)
+        leaf = (-v).requires_grad_()
+        assert torch.equal(got, torch.autograd.grad(call(leaf), leaf, dy)[0]), name
