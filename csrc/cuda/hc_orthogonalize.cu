@@ -6,6 +6,8 @@
 // X in directions that G hardly has would grow by `a` in every step (485 times in five); products with X carry none of it
 // there, only the term a X does, so that term takes X from two fp16 numbers, hi and lo / 2048.  A matrix whose norm is far
 // below eps stays small: it is held times 2^k, with k from what its norm can grow to in `steps`, and S counts 2^-2k.
+#include <math.h>
+
 #include "hc_gemm.cuh"
 #include "hc_host.cuh"
 #include "hc_train.cuh"
@@ -337,6 +339,35 @@ void scale(const dev::ScaleParams& p, size_t batch, cudaStream_t stream) {
   else scale_of<T, false>(p, batch, stream);
 }
 
+// What `steps` steps do to a singular value that starts in [0, 1]: with s its square, a step takes it to |a + b s + c s s| times
+// itself.  `growth`: at most how many times as large one of them gets (X of a small norm is held times 2^k by it).  False if X, S
+// or the polynomial may leave the range of fp16 in which they are held: if a product begins with a singular value above 244, or with a
+// b s + c s s above 60000.  The coefficients that the iteration is used with keep all of them below 4.
+bool iteration_ok(int steps, double a, double b, double c, float* growth) {
+  constexpr double kMost = 60000.0;
+  *growth = 1.0f;
+  double most = 1.0;  // the largest singular value there can be
+  for (int i = 0; i < steps; ++i) {
+    const double end = most * most;
+    // largest absolute values over s in [0, end]: at the ends, or where a derivative is 0
+    const auto factor = [&](double s) { return fabs(a + s * (b + s * c)); };
+    const auto poly = [&](double s) { return fabs(s * (b + s * c)); };
+    const auto value = [&](double s) { return sqrt(s) * factor(s); };
+    double f = fmax(factor(0.0), factor(end)), q = poly(end), v = value(end);
+    const double middle = -b / (2.0 * c);  // of both parabolas
+    if (middle > 0.0 && middle < end) f = fmax(f, factor(middle)), q = fmax(q, poly(middle));
+    const double root = 9.0 * b * b - 20.0 * a * c;  // a + 3 b s + 5 c s s = 0
+    for (int sign = -1; sign <= 1; sign += 2) {
+      const double s = c != 0.0 ? (-3.0 * b + sign * sqrt(root)) / (10.0 * c) : -a / (3.0 * b);
+      if (s > 0.0 && s < end) v = fmax(v, value(s));
+    }
+    if (!(end <= kMost) || !(q <= kMost) || !(f < INFINITY)) return false;
+    if (f > 1.0) *growth *= (float)f;
+    most = v;
+  }
+  return true;
+}
+
 constexpr int kSmallSmem = 224 * 1024;
 
 // The form for small matrices: where its tiles fit a warp's registers and shared memory, and a block is done with a matrix
@@ -381,12 +412,12 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
   using namespace hc;
   if (!element_type_ok(type) || !matrices_ok(batch, height, width) || stride < width || steps < 1 || steps > 100 || !(eps >= 0.0f)) return kErrArgument;
   if (stride > ((size_t)1 << 32) || batch_stride > ((size_t)1 << 56)) return kErrArgument;
+  float growth;
+  if (!iteration_ok(steps, a, b, c, &growth)) return kErrArgument;
   if (batch == 0) return kOk;
   if (!g || !out || !scratch || !lies_at(g, element_bytes(type)) || !lies_at(out, 2) || !lies_at(scratch, 256)) return kErrArgument;
   const Layout l = layout_of(batch, height, width);
   if (scratch_bytes < l.total) return kErrArgument;
-  float growth = 1.0f;
-  for (int i = 0; i < steps; ++i) growth *= a > 1.0f || a < -1.0f ? (a < 0.0f ? -a : a) : 1.0f;
   dev::SmallParams small;
   int smem = 0;
   if (small_plan(&small, batch, height, width, &smem)) {

@@ -75,7 +75,8 @@ int hc_linear_backward(const void* dy, int dy_type, size_t dy_stride, const void
 // Newton-Schulz iteration: X = G / (|G| + eps); `steps` times X = a X + (b S + c S S) X with S = X X^T (or its mirror image
 // from the right where a matrix is taller than wide).  G: `batch` matrices [height][width] of `type`, rows `stride` and
 // matrices `batch_stride` elements apart; out: the same matrices in bf16 without gaps.  Products take fp16 operands; X
-// itself is carried in two fp16 numbers (22 bits), for what is rounded off it grows by up to `a` a step.
+// itself is carried in two fp16 numbers (22 bits), for what is rounded off it grows by up to `a` a step.  Coefficients that could
+// take a singular value in [0, 1], in all steps but the last, above 244, or b s + c s s of its square s above 60000, are refused.
 size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
 int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
                      int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);

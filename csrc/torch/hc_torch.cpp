@@ -457,9 +457,10 @@ Tensor orthogonalize(const Tensor& update_, int64_t steps, double a, double b, d
   Tensor out = at::empty(update.sizes(), update.options().dtype(at::kBFloat16));
   const size_t need = api.orthogonalize_bytes(batch, height, width);
   const Tensor scratch = scratch_of(need, g);
-  check(api.orthogonalize(g.data_ptr(), type_of(g), batch, height, width, height > 1 ? g.stride(1) : width, batch > 1 ? g.stride(0) : 0, out.data_ptr(), (int)steps,
-                          (float)a, (float)b, (float)c, (float)eps, ptr(scratch), need, stream_of(g)),
-        "orthogonalize");
+  const int status = api.orthogonalize(g.data_ptr(), type_of(g), batch, height, width, height > 1 ? g.stride(1) : width, batch > 1 ? g.stride(0) : 0, out.data_ptr(),
+                                       (int)steps, (float)a, (float)b, (float)c, (float)eps, ptr(scratch), need, stream_of(g));
+  TORCH_CHECK_VALUE(status != 4, "orthogonalize: coefficients (", a, ", ", b, ", ", c, ") may carry the iteration beyond the range of float16 in ", steps, " steps");
+  check(status, "orthogonalize");
   return out;
 }
 

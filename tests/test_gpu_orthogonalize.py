@@ -169,3 +169,29 @@ def test_refusals_without_a_gpu():
         assert call(**kw) == 4, kw
     assert call(batch=0) == 0 and lib.hc_orthogonalize_bytes(0, 4, 4) == 0
     assert lib.hc_orthogonalize_bytes(12, 2304, 768) >= 12 * (3 * 2304 * 768 + 2 * 768 * 768) * 2
+
+
+GROWING = [((3.0, 0.0, 0.0), 12), ((2.0, 1.0, 0.0), 4), ((-3.0, 0.0, 0.0), 12), ((1.0, 0.0, 300.0), 2), ((1.0, 70000.0, 0.0), 1), ((float("nan"), 0.0, 0.0), 2), ((1.0, float("inf"), 0.0), 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 60), (200, 300), (300, 200)])
+def test_iterations_that_leave_the_range_of_their_operands(shape):
+    """X, S and the polynomial are held in fp16: coefficients that may carry them beyond it are refused, those that do not give what the formula gives."""
+    g = gaussian(*shape, seed=9)
+    for coefficients, steps in GROWING:
+        with pytest.raises(ValueError, match="float16"):
+            ops.orthogonalize(g, steps=steps, coefficients=coefficients)
+    for coefficients, steps in (((3.0, 0.0, 0.0), 5), ((-3.0, 0.0, 0.0), 4), ((1.0, 60000.0, 0.0), 1), ((2.0, 1.0, 0.0), 3)):
+        got, want = ops.orthogonalize(g, steps=steps, coefficients=coefficients).double(), reference(g, steps, coefficients)
+        # A step's result has, in units of r above, the rounding of X as an operand of either product with S (2), of S and of the polynomial: 4 r in the terms
+        # with S, and moves with X by the polynomial's slope over its value, 3 at most where there is no S S term: (4 + 3 (4 + 3 4)) r = 52 r over three steps, and bf16.
+        assert torch.linalg.matrix_norm(got - want) <= (52 * 2.0 ** -11 / 3 ** 0.5 + 2.3e-3) * torch.linalg.matrix_norm(want)
+
+
+def test_coefficients_refused_without_a_gpu():
+    lib = _lib.cuda()
+    p = C.c_void_p(4096)  # never read: every call below is refused before anything is launched
+    for (a, b, c), steps in GROWING:
+        for h, w in ((16, 24), (400, 300)):
+            assert lib.hc_orthogonalize(p, 0, 2, h, w, w, h * w, p, steps, a, b, c, 1e-7, p, 1 << 30, None) == 4, (a, b, c, steps)

@@ -14,7 +14,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
 
     ``update``: float32, bfloat16 or float16 of shape (..., height, width); every matrix by itself, all of them in the same launches.
     The result is bfloat16 of the same shape.  Products take float16 operands and sum in float32, and X itself is carried to 22
-    bits between the steps, so that directions that ``update`` hardly has gain nothing from rounding.  No gradient.
+    bits between the steps, so that directions that ``update`` hardly has gain nothing from rounding.  Coefficients
+    with which the iteration may leave float16's range on its way raise ValueError (those in use stay far within it).  No gradient.
 
     Forward-mode derivatives, vmap and recorded (traced) calls raise NotImplementedError."""
     if len(coefficients) != 3:
