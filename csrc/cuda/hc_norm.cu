@@ -667,7 +667,7 @@ cudaError_t by_types(int x, int y, F f) {
 bool norm_arguments_ok(const void* x, int x_type, const void* y, int y_type, int param_type, size_t rows, size_t width) {
   if (!element_type_ok(x_type) || !element_type_ok(y_type) || !element_type_ok(param_type)) return false;
   if (x_type != kF32 && y_type != kF32 && x_type != y_type) return false;
-  if (width == 0 || width > (1u << 30) || rows > (1ull << 40) || rows * width > (1ull << 60)) return false;
+  if (width == 0 || width > (1u << 30) || rows > (1ull << 40) || rows > (1ull << 60) / width) return false;
   return rows == 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
 }
 

@@ -323,7 +323,7 @@ Layout layout_of(size_t batch, size_t height, size_t width) {
 
 bool matrices_ok(size_t batch, size_t height, size_t width) {
   const size_t most = (size_t)1 << 24;
-  return height > 0 && width > 0 && height < most && width < most && batch <= 65535;
+  return height > 0 && width > 0 && height < most && width < most && batch <= 65535 && batch <= ((size_t)1 << 48) / (height * width);
 }
 
 template <typename T, bool kVector>

@@ -210,3 +210,12 @@ def test_refusals_without_a_gpu():
     back = lambda dw, db, dx=p, s=p, n=1 << 30: lib.hc_layer_norm_backward(p, 0, p, 0, None, 0, p, dx, dw, db, 4, 16, s, n, None)  # noqa: E731
     assert back(p, None) == 4 and back(None, p) == 4 and back(p, p, s=None) == 4 and back(p, p, n=8) == 4 and back(None, None, C.c_void_p(4100)) == 4
     assert back(None, None, None) == 0
+
+
+def test_sizes_that_wrap_are_refused():
+    """rows x width beyond 2^60 is refused also where 64 bits count it from 0 again."""
+    lib = _lib.cuda()
+    p = C.c_void_p(4096)  # never read: every call below is refused before anything is launched
+    for rows, width in ((1 << 40, 1 << 24), (1 << 40, 1 << 30), (1 << 39, (1 << 25) + 8), (1 << 37, 1 << 27)):
+        assert lib.hc_layer_norm(p, 0, None, None, 0, p, 0, None, rows, width, 1e-5, None) == 4
+        assert lib.hc_layer_norm_backward(p, 0, p, 0, None, 0, p, p, None, None, rows, width, None, 0, None) == 4

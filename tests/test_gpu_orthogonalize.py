@@ -195,3 +195,14 @@ def test_coefficients_refused_without_a_gpu():
     for (a, b, c), steps in GROWING:
         for h, w in ((16, 24), (400, 300)):
             assert lib.hc_orthogonalize(p, 0, 2, h, w, w, h * w, p, steps, a, b, c, 1e-7, p, 1 << 30, None) == 4, (a, b, c, steps)
+
+
+def test_sizes_whose_memory_no_number_holds():
+    """Scratch memory of more bytes than 64 bits count is refused, not counted anew from 0."""
+    lib = _lib.cuda()
+    p = C.c_void_p(4096)
+    for batch, h, w in ((65535, 1 << 23, 1 << 23), (65535, (1 << 24) - 1, (1 << 24) - 1), (65535, 5305712, 5305712)):
+        assert lib.hc_orthogonalize_bytes(batch, h, w) == 0
+        assert lib.hc_orthogonalize(p, 0, batch, h, w, w, 0, p, 5, 3.0, -4.0, 2.0, 1e-7, p, (1 << 64) - 1, None) == 4
+    # a matrix that a GPU holds is still counted
+    assert lib.hc_orthogonalize_bytes(1, 1 << 16, 1 << 16) >= 5 * (1 << 33)
