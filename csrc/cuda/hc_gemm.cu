@@ -385,8 +385,11 @@ struct Storing {
   bool ok = true;
 };
 // A result in fp32 gets its sum in parts of 1024: the tensor core does not round to nearest when it adds to an accumulator, and
-// what that loses over a whole sum (6e-6 of the result over 8192) is ten times what fp32 additions do.
+// what that loses over a whole sum (6e-6 of the result over 8192) is ten times what fp32 additions do.  Where all terms are
+// positive it loses 6.5e-9 of the result a term (3.4e-3 over 2^19), so 16-bit results get theirs in parts, too, where what
+// is lost would come to more than a quarter of half the result's step: 5.3e-5 and 2.1e-4 at the lengths below.
 constexpr int kChunk = 16;  // stages
+constexpr int64_t kLongF16 = 8192, kLongBf16 = 32768;
 
 template <int BN, int kCtas, int MODE>
 __device__ __forceinline__ void load_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* stages, Loading& st, int unit, int units, int rank) {
@@ -1099,7 +1102,8 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
   // sums in parts cost 8 % at 8192 x 4096 x 8192 (392 us with a bf16 result, 403 with fp32, 437 with fp32 sums in parts)
-  const bool wide = c.precise && c.k / (c.parts > 1 ? c.parts : 1) > dev::kChunk * dev::kBK;
+  const int64_t length = c.k / (c.parts > 1 ? c.parts : 1);
+  const bool wide = length > (c.precise ? dev::kChunk * dev::kBK : c.type == kF16 ? dev::kLongF16 : dev::kLongBf16);
   return wide ? run_gemm_mode<dev::kGemmLinearWide>(c, stream) : run_gemm_mode<kGemmLinear>(c, stream);
 }
 

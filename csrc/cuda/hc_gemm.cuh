@@ -95,7 +95,7 @@ struct GemmCall {
   int type;  // of the operands
   int64_t m, n, k, batch;
   int parts;  // over 1 (kGemmLinear without anything behind it, batch 1): as many results, each of a part of the sum, as a batch
-  bool precise;  // the sum is wanted with fp32's precision
+  bool precise;  // the sum is wanted with fp32's precision, not only with that of a 16-bit result of `type`
   GemmOperand a, b;
   GemmSide out, out2;  // result; z, or lo
   GemmSide in, in2;    // residual, c1 or hi; lo

@@ -473,3 +473,39 @@ def test_a_value_does_not_depend_on_its_neighbour(act, out_dtype):
     w[1::2] *= 3
     b[1::2] -= 2
     assert all(torch.equal(p, q) for p, q in zip(want, step(w, b)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", ["rows", "inner"])
+def test_very_long_sums_of_16_bit_results(side):
+    """Positive terms, 2^23 of them in fp16, where half a step of the result is 2^-12 to 2^-11 of it.  A stretch of 1024 terms goes through 64 + 20
+    additions of the tensor core, each off by at most a whole step of fp32, 2 U; the sums of stretches are added in fp32, each addition off by U, 512 of
+    them in a line in each of the 16 parts of so long a sum, and then the parts: at most (168 + 512 + 16) U = 4.2e-5 of the result."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    some = lambda *s: (0.5 + 0.5 * torch.rand(*s, device="cuda", generator=g)).to(F16)  # noqa: E731
+    long = 1 << 23
+    if side == "rows":
+        x, w, dy = some(long, 8), some(16, 8).requires_grad_(), some(long, 16) * 2.0 ** -8
+        got = torch.autograd.grad(ops.linear(x, w), w, dy)[0]
+        want = dy.double().t() @ x.double()
+    else:
+        x, w = some(20, long), some(8, long) * 2.0 ** -8
+        got = ops.linear(x, w)
+        want = x.double() @ w.double().t()
+    assert want.min() > 1000 and want.max() < 60000
+    assert ((got.double() - want).abs() <= (half_step(F16) + 4.2e-5) * want).all()
+    # What is lost to an accumulator that is cut off lies on one side; a rounding to nearest is 0.29 of a step off, on either side: five of its standard deviations.
+    step = torch.finfo(F16).eps * 2.0 ** torch.floor(torch.log2(want))
+    assert abs(float(((got.double() - want) / step).mean())) <= 0.29 * 5 / want.numel() ** 0.5 + 4.2e-5 * 2 / torch.finfo(F16).eps
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,k", [(F16, 8200), (F16, 20001), (BF16, 40008)])
+@pytest.mark.parametrize("act,residual", [(None, None), ("gelu_tanh", None), ("silu", "same")])
+def test_long_sums_of_many_tiles_in_16_bits(kind, k, act, residual):
+    """Sums in stretches with everything that follows a product, the argument that is kept among it, and rows that TMA does not store.  Enough tiles that
+    no sum is shared out."""
+    for m, n in ((2300, 2040), (2190, 2043)):
+        assert _lib.cuda().hc_linear_bytes(m, k, n) == 0
+        x, w, b, r, dy = make(m, k, n, kind, 16, kind, kind if residual else None)
+        check(x, w, b, r, dy, act)
