@@ -24,6 +24,7 @@ constexpr int kStoreWarps = 8;
 constexpr int kGemmThreads = 64 + 32 * kStoreWarps;
 constexpr int kOperandA = kBM * kBK * 2;
 constexpr int kGemmLinearWide = 4;  // kGemmLinear whose sums are formed in parts
+constexpr int kGemmGramWide = 5;    // kGemmGram, the same
 constexpr uint64_t kGemmLimitNs = 2000ull * 1000 * 1000;
 
 struct GemmParams {
@@ -171,7 +172,7 @@ __device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, GemmBa
 // time, so that the tiles at work share their operands in L2.
 template <int BN, int kRows, int MODE>
 __device__ __forceinline__ void tile_place(const GemmParams& p, int t, int& mi, int& ni) {
-  if (MODE == kGemmGram || MODE == kGemmPoly) {
+  if (MODE == kGemmGram || MODE == kGemmGramWide || MODE == kGemmPoly) {
     mi = 0;
     for (;;) {
       int count = (mi * kRows + kRows - 1) / BN + 1;
@@ -452,7 +453,7 @@ __device__ __forceinline__ void multiply_tiles(const GemmParams& p, GemmBarriers
   const int total = p.tiles * p.batch;
   for (int t = unit; st.ok && t < total; t += units) {
     for (int begin = 0; begin < p.k_blocks; begin += kChunk) {
-      const int end = MODE == kGemmLinearWide ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
+      const int end = MODE == kGemmLinearWide || MODE == kGemmGramWide ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
       if (!gemm_wait(&sh.acc_empty[st.acc], st.acc_phase ^ 1, sh)) {
         st.ok = false;
         return;
@@ -504,8 +505,9 @@ __device__ __forceinline__ void release_accumulator(GemmBarriers& sh, Storing& s
 template <int BN, int kCtas, int MODE>
 __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* mine, Storing& st, uint32_t tmem, int unit, int units, int rank) {
   using S = GemmShape<BN, kCtas>;
-  constexpr bool kWide = MODE == kGemmLinearWide, kLinear = MODE == kGemmLinear || kWide, kSymmetric = MODE == kGemmGram || MODE == kGemmPoly;
-  constexpr int kMode = kLinear ? kGemmLinear : MODE;
+  constexpr bool kWide = MODE == kGemmLinearWide || MODE == kGemmGramWide, kLinear = MODE == kGemmLinear || MODE == kGemmLinearWide;
+  constexpr bool kSymmetric = MODE == kGemmGram || MODE == kGemmGramWide || MODE == kGemmPoly;
+  constexpr int kMode = MODE == kGemmLinearWide ? kGemmLinear : MODE == kGemmGramWide ? kGemmGram : MODE;
   constexpr int kPieces = kWide ? (BN / 32 + 1) / 2 : 1;  // of a warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3;      // the rows of tensor memory that this warp can reach
@@ -794,9 +796,10 @@ __device__ __forceinline__ bool meet(GemmBarriers& sh, unsigned int* arrived, in
   return true;
 }
 
-template <int BN, int kCtas>
+template <int BN, int kCtas, bool kLong>  // kLong: the long side is beyond kLongF16
 __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_chain_kernel(const __grid_constant__ ChainParams c) {
   using S = GemmShape<BN, kCtas>;
+  constexpr int kGram = kLong ? kGemmGramWide : kGemmGram;
   extern __shared__ unsigned char raw[];
   __shared__ GemmBarriers sh;
   unsigned char* stages = gemm_stages(raw);
@@ -811,7 +814,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_chain_kernel(const __
       Loading st;
       for (int i = 0; i < products && st.ok; ++i) {
         const int step = i / 3;
-        if (i % 3 == 0) load_tiles<BN, kCtas, kGemmGram>(c.gram[step & 1], sh, stages, st, unit, units, rank);
+        if (i % 3 == 0) load_tiles<BN, kCtas, kGram>(c.gram[step & 1], sh, stages, st, unit, units, rank);
         else if (i % 3 == 1) load_tiles<BN, kCtas, kGemmPoly>(c.poly, sh, stages, st, unit, units, rank);
         else load_tiles<BN, kCtas, kGemmUpdate>(step == c.steps - 1 ? c.last : c.update[step & 1], sh, stages, st, unit, units, rank);
         if (st.ok && i + 1 < products) st.ok = meet(sh, c.arrived, i);
@@ -823,7 +826,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_chain_kernel(const __
       Multiplying st;
       for (int i = 0; i < products && st.ok; ++i) {
         const int step = i / 3;
-        if (i % 3 == 0) multiply_tiles<BN, kCtas, kGemmGram>(c.gram[step & 1], sh, stages, st, tmem, unit, units);
+        if (i % 3 == 0) multiply_tiles<BN, kCtas, kGram>(c.gram[step & 1], sh, stages, st, tmem, unit, units);
         else if (i % 3 == 1) multiply_tiles<BN, kCtas, kGemmPoly>(c.poly, sh, stages, st, tmem, unit, units);
         else multiply_tiles<BN, kCtas, kGemmUpdate>(step == c.steps - 1 ? c.last : c.update[step & 1], sh, stages, st, tmem, unit, units);
       }
@@ -835,7 +838,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) hc_gemm_chain_kernel(const __
     unsigned char* mine = stages + S::kStages * S::kStage + (warp - 2) * kWarpStage;
     for (int i = 0; i < products && st.ok; ++i) {
       const int step = i / 3;
-      if (i % 3 == 0) store_tiles<BN, kCtas, kGemmGram>(c.gram[step & 1], sh, mine, st, tmem, unit, units, rank);
+      if (i % 3 == 0) store_tiles<BN, kCtas, kGram>(c.gram[step & 1], sh, mine, st, tmem, unit, units, rank);
       else if (i % 3 == 1) store_tiles<BN, kCtas, kGemmPoly>(c.poly, sh, mine, st, tmem, unit, units, rank);
       else store_tiles<BN, kCtas, kGemmUpdate>(step == c.steps - 1 ? c.last : c.update[step & 1], sh, mine, st, tmem, unit, units, rank);
       if (!st.ok || i + 1 == products) break;
@@ -1057,8 +1060,8 @@ TileChoice best_chain_tile(const GemmCall& gram, const GemmCall& poly, const Gem
   return best;
 }
 
-template <int BN, int kCtas>
-cudaError_t run_chain(const GemmChain& c, cudaStream_t stream) {
+template <int BN, int kCtas, bool kLong>
+cudaError_t run_chain_of(const GemmChain& c, cudaStream_t stream) {
   using S = dev::GemmShape<BN, kCtas>;
   static_assert(sizeof(dev::ChainParams) <= 32000, "arguments of a kernel");
   dev::ChainParams p;
@@ -1072,10 +1075,15 @@ cudaError_t run_chain(const GemmChain& c, cudaStream_t stream) {
   p.steps = c.steps;
   p.arrived = c.arrived;
   static unsigned long long allowed = 0;
-  if (e == cudaSuccess) e = allow_smem(dev::hc_gemm_chain_kernel<BN, kCtas>, S::kSmem, &allowed);
+  if (e == cudaSuccess) e = allow_smem(dev::hc_gemm_chain_kernel<BN, kCtas, kLong>, S::kSmem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t total = (int64_t)p.last.tiles * p.last.batch;  // the product with the most tiles
-  return launch_units<kCtas>(dev::hc_gemm_chain_kernel<BN, kCtas>, p, total, S::kSmem, true, stream);
+  return launch_units<kCtas>(dev::hc_gemm_chain_kernel<BN, kCtas, kLong>, p, total, S::kSmem, true, stream);
+}
+// S sums the long side, and its diagonal is all positive; the other sums are as long as the short side, which memory bounds.
+template <int BN, int kCtas>
+cudaError_t run_chain(const GemmChain& c, cudaStream_t stream) {
+  return c.gram[0].k > dev::kLongF16 ? run_chain_of<BN, kCtas, true>(c, stream) : run_chain_of<BN, kCtas, false>(c, stream);
 }
 
 }  // namespace

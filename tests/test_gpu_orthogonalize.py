@@ -206,3 +206,10 @@ def test_sizes_whose_memory_no_number_holds():
         assert lib.hc_orthogonalize(p, 0, batch, h, w, w, 0, p, 5, 3.0, -4.0, 2.0, 1e-7, p, (1 << 64) - 1, None) == 4
     # a matrix that a GPU holds is still counted
     assert lib.hc_orthogonalize_bytes(1, 1 << 16, 1 << 16) >= 5 * (1 << 33)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("height,width", [(32, 1 << 22), (1 << 20, 64), (700, 70001), (20000, 260)])
+def test_long_sides(height, width):
+    """S is a sum over the long side, of positive terms in its diagonal; its precision does not go with the length."""
+    check(torch.randn(height, width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(10)))
