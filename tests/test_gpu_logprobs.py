@@ -256,3 +256,61 @@ def test_refusals_without_a_gpu():
     for kw in (dict(st=None), dict(tokens=None), dict(dx=None), dict(ds=15), dict(type=5)):
         assert back(**kw) == 4, kw
     assert back(rows=0) == 0
+
+
+# From 1184 rows and a vocabulary of 8192 up, blocks stay and rows stream through them.
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [8192, 8193, 12301])
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("top", [0, 20])
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_rows(vocab, kind, top, masked):
+    x, t, a, b = make(1200, vocab, kind, vocab, masked)
+    t[700:1190] = IGNORED  # blocks that skip rows, some at their first one
+    check(x, t, a, b, top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad", [1, 3, 8, 102])
+def test_many_rows_apart(pad):
+    g = torch.Generator().manual_seed(pad)
+    wide = torch.randn(2500, 8197 + pad, generator=g).to(BF16).cuda()
+    t = torch.randint(0, 8197, (2500,), generator=g).cuda()
+    a, b = torch.randn(2500, generator=g).cuda(), torch.randn(2500, generator=g).cuda()
+    check(wide[:, :8197], t, a, b, 3)
+    check(wide[:, pad:], t, a, b, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+def test_many_rows_of_which_some_have_no_distribution(kind):
+    x, t, a, b = make(1300, 8201, kind, 5)
+    want = ops.token_logprobs(x, t, top=4)
+    bad = {0: math.nan, 7: math.inf, 650: math.nan, 1299: -math.inf}
+    x[0, 0], x[7, 8200], x[650, 4000], x[1299] = math.nan, math.inf, math.nan, -math.inf
+    low = torch.finfo(kind).min
+    x[20], x[21, 1:] = low, low
+    t[20], t[21] = 3, 0
+    leaf = x.detach().requires_grad_()
+    r = ops.token_logprobs(leaf, t, top=4)
+    (dx,) = torch.autograd.grad((r.logprobs, r.entropy), (leaf,), (a, b))
+    rows = list(bad)
+    assert torch.isnan(r.logprobs[rows]).all() and torch.isnan(r.entropy[rows]).all() and (r.top_tokens[rows] == -1).all() and torch.isnan(dx[rows]).all()
+    keep = [i for i in range(1300) if i not in bad and i not in (20, 21)]
+    for p, q in zip(r, want):
+        assert torch.equal(p[keep], q[keep])
+    check(x[[i for i in range(1300) if i not in bad]], t[[i for i in range(1300) if i not in bad]], a[:1296], b[:1296], 4)
+
+
+@pytest.mark.gpu
+def test_largest_logits_at_one_thread_of_many_rows():
+    """The same where rows stream: the groups of a thread are 128 groups apart, and 40 of the threads have all that counts."""
+    vocab = 65536
+    x = torch.zeros(1190, vocab, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    for thread in range(40):
+        at = (torch.arange(thread * 8, vocab, 1024)[:, None] + torch.arange(8)).reshape(-1)
+        x[:, at.cuda()] = 5 + torch.rand(1190, at.numel(), generator=g).cuda()
+    t = torch.arange(1190, device="cuda")
+    one = torch.ones(1190, device="cuda")
+    check(x, t, one, one, 64)
