@@ -288,3 +288,39 @@ def test_views_that_are_the_negative_of_what_lies_there():
         (got,) = torch.autograd.grad(call(leaf), leaf, dy)
         leaf = (-v).requires_grad_()
         assert torch.equal(got, torch.autograd.grad(call(leaf), leaf, dy)[0]), name
+
+
+def _trainer_with_status(rank, world, status, prefix):
+    import os
+
+    from tirocinio_triennale_b200.models import train_dp
+
+    asked = []
+
+    def train_status(device=None, clear=True):
+        asked.append(device)
+        return status if rank == world - 1 else 0  # of one rank; all of them end
+
+    train_dp.train_status = train_status
+    model = train_dp.GPT2
+
+    def plain(cfg):  # the operators need a GPU; what is tested is what the trainer makes of their status
+        cfg = copy.copy(cfg)
+        cfg.fused = False
+        return model(cfg)
+
+    train_dp.GPT2 = plain
+    args = argparse.Namespace(model="tiny", steps=2, warmup=1, batch=2, seq=16, eb=1e-6, lr=1e-3, bucket_mb=0.05, cpu=True, save=prefix, resume=None, save_compressed_eb=0.0,
+                              fused=True, optimizer="adamw", muon_lr=0.02)
+    if status:
+        with pytest.raises(RuntimeError, match="operators"):
+            train_dp.run(args, True, rank, world, torch.device("cpu"))
+    else:
+        train_dp.run(args, True, rank, world, torch.device("cpu"))
+    assert asked and os.path.exists("%s.compressed.rank%d" % (prefix, rank)) == (status == 0)
+
+
+@pytest.mark.parametrize("world", [1, 2])
+@pytest.mark.parametrize("status", [0, 3])
+def test_a_wait_that_ran_out_ends_the_trainer_on_all_ranks(status, world, tmp_path):
+    run_ranks(_trainer_with_status, world, backend="gloo", args=(status, str(tmp_path / "ck")))

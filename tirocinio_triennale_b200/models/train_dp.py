@@ -27,9 +27,18 @@ import torch
 import torch.distributed as dist
 from torch.nn.parallel import DistributedDataParallel as DDP
 
+from ..ops import train_status
 from ..parallel import CompressedHookState, compressed_allreduce_hook
 from .gpt2 import GPT2, GPT2Config
 from .muon import muon_with_adamw
+
+
+def _check_operators(device):
+    """Raises on all ranks if a wait of the operators' kernels ran out on one of them: what it left in gradients or weights is wrong."""
+    status = torch.tensor([train_status(device)], device=device)
+    dist.all_reduce(status, op=dist.ReduceOp.MAX)
+    if int(status):
+        raise RuntimeError("the operators of the training step report status %d: results of this run are not to be used" % int(status))
 
 
 def run(args, compressed: bool, rank: int, world: int, device):
@@ -76,6 +85,8 @@ def run(args, compressed: bool, rank: int, world: int, device):
         torch.cuda.synchronize()
     dist.barrier()
     dt = time.perf_counter() - t0
+    if cfg.fused or getattr(args, "optimizer", "adamw") == "muon":
+        _check_operators(device)  # before anything of the run is reported or saved
     last = torch.stack(losses[-5:]).float().mean()
     dist.all_reduce(last)
     out = {"tokens_per_s": args.steps * args.batch * args.seq * world / dt, "final_loss": float(last) / world,
