@@ -324,3 +324,30 @@ def _trainer_with_status(rank, world, status, prefix):
 @pytest.mark.parametrize("status", [0, 3])
 def test_a_wait_that_ran_out_ends_the_trainer_on_all_ranks(status, world, tmp_path):
     run_ranks(_trainer_with_status, world, backend="gloo", args=(status, str(tmp_path / "ck")))
+
+
+def test_a_module_built_for_another_torch_is_built_anew(tmp_path, monkeypatch):
+    """What the native front end was compiled against is in its name; another torch's classes lie differently."""
+    from tirocinio_triennale_b200 import _build
+
+    monkeypatch.setattr(_build, "LIBDIR", tmp_path)
+    made = []
+
+    def run(cmd):
+        made.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return ""
+
+    monkeypatch.setattr(_build, "_run", run)
+    lib = _build.build_torch()
+    assert lib.exists() and len(made) == 1
+    assert _build.build_torch() == lib and len(made) == 1
+    monkeypatch.setattr(torch, "__version__", "9.9.9+cu999")
+    other = _build.build_torch()
+    assert _build.build_torch() == other != lib and len(made) == 2
+    monkeypatch.undo()
+    monkeypatch.setattr(_build, "LIBDIR", tmp_path)
+    monkeypatch.setattr(_build, "_run", run)
+    assert _build.build_torch() == lib and len(made) == 2
+    lib.unlink()
+    assert _build.build_torch() == lib and len(made) == 3

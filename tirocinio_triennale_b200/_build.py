@@ -145,16 +145,18 @@ def build_mpi(mpi_include: str | None = None, mpi_sources=(), mpi_link=(), force
 
 
 def build_torch(force: bool = False) -> Path:
-    """``_homcomp_torch.so``: the training step's operators on torch tensors with their gradients (csrc/torch), compiled by g++
-    against the headers of the installed torch.  It is given the addresses of the library's functions when it is loaded."""
-    lib = LIBDIR / "_homcomp_torch.so"
+    """``_homcomp_torch.<torch>.<python>.so``: the training step's operators on torch tensors with their gradients (csrc/torch), compiled
+    by g++ against the headers of the installed torch.  It is given the addresses of the library's functions when it is loaded.  The
+    torch and the Python that it was built for are in its name, so that with others it is built anew."""
+    import torch
+
+    lib = LIBDIR / ("_homcomp_torch.torch-%s.%s.so" % (torch.__version__, sys.implementation.cache_tag))
     src, header = CSRC / "torch" / "hc_torch.cpp", CSRC / "include" / "homcomp_train.h"
     if not force and lib.exists() and lib.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
         return lib
     import fcntl
     import sysconfig
 
-    import torch
     from torch.utils import cpp_extension
 
     cuda = str(Path(nvcc_path()).resolve().parent.parent / "include") if nvcc_path() else "/usr/local/cuda/include"
