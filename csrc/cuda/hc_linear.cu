@@ -303,7 +303,7 @@ namespace {
 constexpr size_t kMostSize = (size_t)1 << 26;  // of each side: a tile's sum then stays far below the limit of a wait
 // Up to here the kernel for few rows: 8 us with 16 rows of 4096 -> 4096, 30 to 36 of 8192 -> 8192.  The large products take 16 and 37
 // with 17 rows; this kernel with four eights of rows took 16 to 18 and 88 to 108, for every block reads all of x.
-constexpr size_t kFewRows = 16;
+constexpr size_t kFewRows = HC_LINEAR_FEW_ROWS;
 
 bool sizes_ok(size_t rows, size_t inner, size_t width) {
   return inner > 0 && width > 0 && inner < kMostSize && width < kMostSize && rows < kMostSize;
@@ -331,6 +331,7 @@ void few_rows_of(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) 
 }
 template <typename T>
 void few_rows(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
+  static_assert(kFewRows <= 16, "two eights of rows");
   if (p.rows <= 8) few_rows_of<T, 1>(p, vector, stream);
   else few_rows_of<T, 2>(p, vector, stream);
 }

@@ -47,7 +47,9 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
 // ---- products ---------------------------------------------------------------------------------------------------------
 // Operands are bf16 or fp16 (`type` 1 or 2), sums fp32.  x [rows][inner], weight [width][inner], out [rows][width], each side
 // below 2^26.
-// A product on the tensor cores reads its operands in 16-byte pieces: data 16-byte aligned, strides multiples of 8.
+#define HC_LINEAR_FEW_ROWS 16
+// A product of more than HC_LINEAR_FEW_ROWS rows, and the products of a backward pass, read their operands in 16-byte pieces: data
+// 16-byte aligned, strides multiples of 8.  Fewer rows, and their weights, may begin anywhere.
 // Results and what is added to them may lie anywhere.  Where a result's stride is its width rounded up to eight, what lies
 // behind its rows is padding and may be overwritten; behind rows of any other stride nothing is.
 //

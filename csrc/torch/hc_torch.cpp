@@ -249,8 +249,6 @@ Tensor layer_norm(const Tensor& x_, const OptTensor& weight_, const OptTensor& b
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
-constexpr int64_t kFewRows = 16;  // up to here W is read by a kernel that takes rows that begin anywhere
-
 Tensor linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t act, int out, at::IntArrayRef shape,
                       Tensor* z) {
   const c10::cuda::CUDAGuard guard(x.device());
@@ -266,7 +264,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bi
   return y;
 }
 // operands as the call with m rows reads them
-Tensor for_rows(const Tensor& t, int64_t m) { return m > kFewRows ? operand(t) : adjacent(t); }
+Tensor for_rows(const Tensor& t, int64_t m) { return m > HC_LINEAR_FEW_ROWS ? operand(t) : adjacent(t); }
 
 struct Linear : Function<Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& given, const Tensor& given_weight, const OptTensor& bias, const OptTensor& residual, int64_t act,
