@@ -351,3 +351,14 @@ def test_a_module_built_for_another_torch_is_built_anew(tmp_path, monkeypatch):
     assert _build.build_torch() == lib and len(made) == 2
     lib.unlink()
     assert _build.build_torch() == lib and len(made) == 3
+
+
+def test_muon_with_adamw_where_one_of_them_has_nothing():
+    """A model without linear layers, and one of nothing but their matrices."""
+    one = muon_with_adamw(torch.nn.LayerNorm(8))
+    assert [type(o) for o in one.optimizers] == [torch.optim.AdamW]
+    other = muon_with_adamw(torch.nn.Linear(8, 8, bias=False), lr=0.5)
+    assert [type(o) for o in other.optimizers] == [Muon] and other.optimizers[0].param_groups[0]["lr"] == 0.5
+    other.load_state_dict(other.state_dict())
+    with pytest.raises(ValueError):
+        one.load_state_dict([])

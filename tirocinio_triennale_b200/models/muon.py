@@ -57,7 +57,7 @@ class Muon(torch.optim.Optimizer):
 
 
 class Optimizers:
-    """Several optimisers that step together."""
+    """Several optimisers that step together.  A learning-rate scheduler takes one of ``optimizers``."""
 
     def __init__(self, *optimizers):
         self.optimizers = optimizers
@@ -81,11 +81,15 @@ class Optimizers:
 
 
 def muon_with_adamw(model: torch.nn.Module, lr: float = 0.02, adam_lr: float = 3e-4, momentum: float = 0.95, weight_decay: float = 0.0) -> Optimizers:
-    """Muon for the matrices of ``model``'s linear layers, AdamW for everything else."""
+    """Muon for the matrices of ``model``'s linear layers, AdamW for everything else; one of them alone where the other has nothing."""
     matrices = {id(m.weight) for m in model.modules() if isinstance(m, torch.nn.Linear)}
     embedded = {id(m.weight) for m in model.modules() if isinstance(m, torch.nn.Embedding)}  # also where they are the output's
     matrices -= embedded
     params = list(model.parameters())
-    return Optimizers(Muon([p for p in params if id(p) in matrices], lr=lr, momentum=momentum, weight_decay=weight_decay),
-                      torch.optim.AdamW([p for p in params if id(p) not in matrices], lr=adam_lr, weight_decay=weight_decay,
-                                        fused=all(p.is_cuda for p in params)))
+    turned, others = [p for p in params if id(p) in matrices], [p for p in params if id(p) not in matrices]
+    optimizers = []
+    if turned:
+        optimizers.append(Muon(turned, lr=lr, momentum=momentum, weight_decay=weight_decay))
+    if others:
+        optimizers.append(torch.optim.AdamW(others, lr=adam_lr, weight_decay=weight_decay, fused=all(p.is_cuda for p in params)))
+    return Optimizers(*optimizers)
