@@ -388,9 +388,10 @@ struct Storing {
 // A result in fp32 gets its sum in parts of 1024: the tensor core does not round to nearest when it adds to an accumulator, and
 // what that loses over a whole sum (6e-6 of the result over 8192) is ten times what fp32 additions do.  Where all terms are
 // positive it loses 6.5e-9 of the result a term (3.4e-3 over 2^19), so 16-bit results get theirs in parts, too, where what
-// is lost would come to more than a quarter of half the result's step: 5.3e-5 and 2.1e-4 at the lengths below.
+// is lost would come to more than a quarter of half the result's step (2^-14, 2^-11): 5.3e-5 and 4.3e-4 at the lengths below.
+// Of tiles of 256 x 256 a thread then has 128 sums, and keeps 216 bytes outside of its 168 registers.
 constexpr int kChunk = 16;  // stages
-constexpr int64_t kLongF16 = 8192, kLongBf16 = 32768;
+constexpr int64_t kLongF16 = 8192, kLongBf16 = 65536;
 
 template <int BN, int kCtas, int MODE>
 __device__ __forceinline__ void load_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* stages, Loading& st, int unit, int units, int rank) {
@@ -1109,7 +1110,8 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
 }
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
-  // sums in parts cost 8 % at 8192 x 4096 x 8192 (392 us with a bf16 result, 403 with fp32, 437 with fp32 sums in parts)
+  // sums in parts cost 8 % at 8192 x 4096 x 8192 (392 us with a bf16 result, 403 with fp32, 437 with fp32 sums in parts), 6 % at
+  // 4096 x 4096 x 16384 in fp16 (432 and 458 us)
   const int64_t length = c.k / (c.parts > 1 ? c.parts : 1);
   const bool wide = length > (c.precise ? dev::kChunk * dev::kBK : c.type == kF16 ? dev::kLongF16 : dev::kLongBf16);
   return wide ? run_gemm_mode<dev::kGemmLinearWide>(c, stream) : run_gemm_mode<kGemmLinear>(c, stream);
