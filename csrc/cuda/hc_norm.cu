@@ -527,7 +527,8 @@ constexpr int64_t kLongestInRegisters = 8192;
 
 // Threads and groups of eight a thread for rows of `width` values (with one group more where rows begin anywhere).  What a row
 // costs a warp besides its values, some 200 instructions, is shared by as few warps as the registers allow: up to five groups a
-// thread (6001 x 5003 bf16: with 256 threads a row and three groups 43 us forward and 55 us back, with 128 and five 37 and 54).
+// thread (6001 x 5003 bf16: with 256 threads a row and three groups 43 us forward and 55 us back, with 128 and five 37 and 54, although
+// the backward pass then has 36 to 112 bytes more to a thread than its 128 registers hold).
 // Forward a warp alone takes rows of up to three groups a thread, with no barrier in its sums (8192 x 768: 12.9 us, 17.7 with 128
 // threads); back, where it would have 24 column sums a thread and rings for 16 teams, it does not (24.1 us, 20.1).  Long rows
 // of wide types have fewer teams, for whose rings there is room.

@@ -6,7 +6,8 @@
 // two graphs) need two of them.  All functions return 0 or a hc::Status code: 4 for arguments that the call does not
 // take, 5 for an error of the CUDA runtime.
 //
-// A pointer that does not begin where its elements may is refused.
+// A pointer that does not begin where its elements may is refused.  What a call writes does not overlap what it reads, its scratch memory
+// or its other results.
 //
 // Types: 0 fp32, 1 bf16, 2 fp16.  Strides count elements from one row to the next; the elements of a row are adjacent.
 #pragma once
@@ -45,7 +46,8 @@ int hc_token_logprobs_backward(const void* logits, int type, size_t rows, size_t
                                const float* dentropy, void* dlogits, size_t dstride, hc_stream_t stream);
 
 // ---- products ---------------------------------------------------------------------------------------------------------
-// Operands are bf16 or fp16 (`type` 1 or 2), sums fp32.  x [rows][inner], weight [width][inner], out [rows][width], each side
+// Operands are bf16 or fp16 (`type` 1 or 2), sums fp32, in the tensor core over up to 1024 terms for fp32 results and up to 8192 (fp16) or 65536
+// (bf16) for 16-bit ones, whose rounding is four times and more what that loses.  x [rows][inner], weight [width][inner], out [rows][width], each side
 // below 2^26.
 #define HC_LINEAR_FEW_ROWS 16
 // A product of more than HC_LINEAR_FEW_ROWS rows, and the products of a backward pass, read their operands in 16-byte pieces: data
@@ -63,7 +65,8 @@ size_t hc_linear_bytes(size_t rows, size_t inner, size_t width);
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
               const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
               int activation, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes, hc_stream_t stream);
-// Backward pass: dz = dy act'(z), rounded to `type` for the products; dx = dz weight, dweight = dz^T x (of `type`) and dbias =
+// Backward pass: dz = dy act'(z), rounded to `type` for the products (fp16: infinite beyond 65504, 0 below 3e-8, also where dy is fp32; a loss
+// is scaled accordingly); dx = dz weight, dweight = dz^T x (of `type`) and dbias =
 // the sums of dz's columns before rounding (of bias_type), each NULL where it is not wanted.  dy is of dy_type, 0 or `type`.
 // keep_dz: dz is written to the scratch memory; 0 where dy itself is dz and a product can read it (no activation, dy of
 // `type`, its rows as operands have to lie).  Sums over rows are formed in a fixed order.
@@ -83,8 +86,8 @@ size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
 int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
                      int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 
-// Waits of the products' and the norm's kernels are bounded (2 s).  Synchronises the device and returns 3 if one of them ran out since the status
-// was last cleared, 0 if not.
+// The kernels' waits are bounded (2 s).  Where one ran out the call's results are wrong.  Synchronises the device and returns 3 if that
+// happened since the status was last cleared, 0 if not.
 int hc_train_status(int clear);
 
 #ifdef __cplusplus

@@ -24,7 +24,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ign
     gradient (None where ``top`` is 0; at most 64).  ``-logprobs.sum() / count`` is the cross-entropy loss.
 
     Rows whose token is ``ignore_index`` are not read: 0 for both numbers, -1 for their tokens, a gradient of 0.  Logits of -inf
-    are tokens that cannot come: they add nothing and get a gradient of 0.  A row that has a NaN or +inf, or nothing above -inf,
+    are tokens that cannot come: they add nothing and get a gradient of 0 (the row's own token: that of its log probability).  A row that has a NaN or +inf, or nothing above -inf,
     gives NaN and tokens of -1; a token outside the vocabulary gives NaN for its log probability and its row of the gradient.
 
     Forward-mode derivatives, vmap and recorded (traced) calls raise NotImplementedError."""
