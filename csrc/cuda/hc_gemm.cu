@@ -46,6 +46,7 @@ struct GemmParams {
   int bias_type, activation;
   float ca, cb, cc;
   const float* scale;
+  const unsigned int* most;
   int tma_out, tma_out2, tma_in, tma_in2;              // moved by TMA: rows that begin at 16 bytes
   int wide_boxes;                                      // map_out and map_out2 are of boxes of 32 x 64 values
 };
@@ -230,6 +231,11 @@ __device__ __forceinline__ void gemm_finish(const GemmParams& p, int z, int row0
   const int64_t count = row < p.m ? p.n - col0 : 0;  // columns of this row (may be over 32)
   unsigned char* second = slot + kSlot / 2;
   if (MODE == kGemmLinear) {
+    if (p.most) {
+      const float power = gradient_power(p.most, -1);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= power;
+    }
     if (p.bias) {
       shared_bias[lane] = bias;
       __syncwarp();
@@ -346,6 +352,11 @@ __device__ __forceinline__ void gemm_fetch(const GemmParams& p, int z, int row0,
 __device__ __forceinline__ void gemm_finish_half(const GemmParams& p, float (&v)[32], int half, unsigned char* out, unsigned char* z, float bias,
                                                  float* shared_bias) {
   const int lane = threadIdx.x & 31;
+  if (p.most) {
+    const float power = gradient_power(p.most, -1);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= power;
+  }
   if (p.bias) {
     __syncwarp();
     shared_bias[lane] = bias;
@@ -965,6 +976,7 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.cb = c.cb;
   p.cc = c.cc;
   p.scale = c.scale;
+  p.most = c.most;
   constexpr bool kLinear = MODE == kGemmLinear || MODE == dev::kGemmLinearWide, kUpdate = MODE == kGemmUpdate;
   if (MODE == kGemmLinear && BN >= 128 && c.out_type != kF32 && !c.in.data && make_side_map(&p.map_out, c.out, c.out_type, c, true, false, true))
     p.wide_boxes = !c.out2.data || make_side_map(&p.map_out2, c.out2, c.type, c, true, false, true);

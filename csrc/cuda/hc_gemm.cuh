@@ -75,6 +75,14 @@ __device__ __forceinline__ Pair slope_pair(Pair g, float x, float y) {
   return g * fma2(zdv, fma2(minus, s, s), s);
 }
 
+// fp16 products take an fp32 gradient times 2^k (sign 1), and their results times 2^-k (sign -1), with k from the bits of the largest
+// finite |gradient|, which comes to [2^13, 2^14): times a slope it stays in range, and 2^-38 of it is still a number.
+__device__ __forceinline__ float gradient_power(const unsigned int* most, int sign) {
+  const int exponent = (int)(*most >> 23);
+  const int k = *most ? min(127 + 13 - exponent, 100) : 0;  // from -114
+  return __int_as_float((127 + sign * k) << 23);
+}
+
 }  // namespace dev
 
 // An operand is stored as rows of adjacent elements.  kMajor: its rows are those of the product (or its columns, for the
@@ -105,6 +113,7 @@ struct GemmCall {
   int activation;
   float ca, cb, cc;
   const float* scale;  // of each matrix of a batch (kGemmPoly, kGemmUpdate): X is that times what is stored
+  const unsigned int* most;  // kGemmLinear without anything behind it: see gradient_power, whose inverse the result is taken times; or NULL
 };
 
 // Into how many parts the sum of a product is best shared out (1: none).

@@ -65,8 +65,8 @@ size_t hc_linear_bytes(size_t rows, size_t inner, size_t width);
 int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const void* bias, int bias_type,
               const void* residual, size_t residual_stride, void* out, int out_type, size_t out_stride, void* z, size_t z_stride,
               int activation, size_t rows, size_t inner, size_t width, void* scratch, size_t scratch_bytes, hc_stream_t stream);
-// Backward pass: dz = dy act'(z), rounded to `type` for the products (fp16: infinite beyond 65504, 0 below 3e-8, also where dy is fp32; a loss
-// is scaled accordingly); dx = dz weight, dweight = dz^T x (of `type`) and dbias =
+// Backward pass: dz = dy act'(z), rounded to `type` for the products (of an fp32 dy and fp16 operands times a power of two, which its largest
+// finite value gives, and which the results are freed of); dx = dz weight, dweight = dz^T x (of `type`) and dbias =
 // the sums of dz's columns before rounding (of bias_type), each NULL where it is not wanted.  dy is of dy_type, 0 or `type`.
 // keep_dz: dz is written to the scratch memory; 0 where dy itself is dz and a product can read it (no activation, dy of
 // `type`, its rows as operands have to lie).  Sums over rows are formed in a fixed order.

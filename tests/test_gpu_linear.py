@@ -509,3 +509,85 @@ def test_long_sums_of_many_tiles_in_16_bits(kind, k, act, residual):
         assert _lib.cuda().hc_linear_bytes(m, k, n) == 0
         x, w, b, r, dy = make(m, k, n, kind, 16, kind, kind if residual else None)
         check(x, w, b, r, dy, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(5, 96, 50), (300, 264, 200), (77, 65, 129), (40, 200, 6144), (2500, 64, 96)])
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+@pytest.mark.parametrize("dy_size,operand_size", [(2.0 ** -30, 2.0 ** 10), (2.0 ** 24, 2.0 ** -12), (2.0 ** 100, 2.0 ** -14), (2.0 ** -126, 1.0), (1.0, 1.0), (0.0, 1.0)])
+def test_fp32_gradients_beyond_fp16(m, k, n, act, dy_size, operand_size):
+    """An fp32 gradient enters fp16 products times a power of two, which takes its largest value to 2^13 at least: what is rounded there is 2^-11 of a value,
+    or 2^-25 2^-13 of the largest one.  Only what fp16 does not hold of the result itself is infinite or 0."""
+    g = torch.Generator().manual_seed(m)
+    x, w, b = (torch.randn(*s, generator=g).to(F16).cuda() for s in ((m, k), (n, k), (n,)))
+    dy = (torch.randn(m, n, generator=g) * dy_size).cuda()
+    grown = [(x * operand_size).to(F16).requires_grad_(), (w * operand_size).to(F16).requires_grad_(), b.requires_grad_()]
+    y = ops.linear(*grown, activation=act, out_dtype=F32)
+    got = torch.autograd.grad(y, grown, dy)
+    X, W, B = (v.detach().double() for v in grown)
+    z = X @ W.t() + B
+    ez = sums(k) * (X.abs() @ W.abs().t()) + U * z.abs()
+    D = dy.double()
+    if act is None:
+        dz, e = D, torch.zeros_like(D)
+    else:
+        z = z.requires_grad_()
+        (slope,) = torch.autograd.grad(ACT[act](z).sum(), (z,))
+        z = z.detach()
+        dz, e = D * slope, D.abs() * (0.8 * (half_step(F16) * z.abs() + ez + least(F16)) + 8 * U)
+    e = e + half_step(F16) * dz.abs() + 2.0 ** -38 * D.abs().max()
+    for have, left, right, el in ((got[0], dz, W, e), (got[1], dz.t(), X, e.t())):
+        want = left @ right
+        room = 1.01 * (el @ right.abs() + sums(left.shape[1]) * ((left.abs() + el) @ right.abs()) + half_step(F16) * want.abs()) + least(F16)
+        clear = want.abs() + room < 65500
+        assert torch.isfinite(have[clear]).all() and ((have.double() - want).abs() <= room)[clear].all()
+        assert torch.isinf(have[want.abs() - room > 65540]).all()
+        if dy_size == 0.0:
+            assert not have.any()
+    want = dz.sum(0)
+    room = 1.01 * (e.sum(0) + (m + 64) * U * (dz.abs() + e).sum(0) + half_step(F16) * want.abs()) + least(F16)
+    clear = want.abs() + room < 65500
+    assert ((got[2].double() - want).abs() <= room)[clear].all()
+
+
+@pytest.mark.gpu
+def test_fp32_gradients_beyond_fp16_that_are_not_finite():
+    """What is infinite or not a number in one row, and one column, has no part in the power that the others are taken times."""
+    g = torch.Generator().manual_seed(3)
+    x, w = torch.randn(200, 64, generator=g).to(F16).cuda().requires_grad_(), (torch.randn(96, 64, generator=g) * 2.0 ** 8).to(F16).cuda().requires_grad_()
+    dy = (torch.randn(200, 96, generator=g) * 2.0 ** -28).cuda()
+    dy[7, 9] = 0.0
+    clean = torch.autograd.grad(ops.linear(x, w, out_dtype=F32), (x, w), dy)
+    assert clean[0].any(1).all()
+    for bad in (float("inf"), float("nan")):
+        dy[7, 9] = bad
+        dx, dw = torch.autograd.grad(ops.linear(x, w, out_dtype=F32), (x, w), dy)
+        rows, columns = [i for i in range(200) if i != 7], [i for i in range(96) if i != 9]
+        assert torch.equal(dx[rows], clean[0][rows]) and torch.equal(dw[columns], clean[1][columns])
+        assert not torch.isfinite(dx[7]).all() and not torch.isfinite(dw[9]).all()
+
+
+@pytest.mark.gpu
+def test_fp32_gradients_of_any_size_in_a_graph():
+    """The power of two is found anew in every replay."""
+    g = torch.Generator().manual_seed(4)
+    x, w = torch.randn(200, 64, generator=g).to(F16).cuda(), torch.randn(96, 64, generator=g).to(F16).cuda()
+    dy = torch.randn(200, 96, generator=g).cuda()
+    wide = torch.randn(200, 130, generator=g).cuda()[:, 3:99]  # rows with gaps
+
+    def step():
+        leaves = [v.detach().requires_grad_() for v in (x, w)]
+        y = ops.linear(*leaves, out_dtype=F32)
+        return (*torch.autograd.grad(y, leaves, dy, retain_graph=True), *torch.autograd.grad(y, leaves, wide))
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caught = step()
+    for size in (2.0 ** 20, 2.0 ** -40, 2.0 ** 10):
+        dy.mul_(size)
+        wide.mul_(size)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(p, q) for p, q in zip(caught, want)) and want[0].any()

@@ -17,8 +17,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     float32 or ``x``'s type, and the result has its type; without one the result has ``x``'s type or ``out_dtype`` (float32).
 
     Everything behind the product happens before the result is stored.  For the backward pass of an activation its argument is
-    kept in ``x``'s type, and the gradient, also a float32 one, is rounded to that type before it enters the products (float16 holds 6e-8 to
-    65504: the loss is scaled for it); gradients of ``x`` and ``weight``
+    kept in ``x``'s type, and the gradient is rounded to that type before it enters the products (a float32 one, where that
+    type is float16, times a power of two that brings its largest value into range); gradients of ``x`` and ``weight``
     have their types, that of ``bias`` its own, summed in float32 in a fixed order.  Where eight does not divide ``width`` the
     result's rows are kept apart so that they begin at 16-byte boundaries: it has gaps.
 
