@@ -62,7 +62,11 @@ __device__ __forceinline__ void activate_pair(float& x, float& y) {
 template <int kAct>
 __device__ __forceinline__ Pair slope_pair(Pair g, float x, float y) {
   if (kAct == kActNone) return g;
-  if (kAct == kActRelu) return g * pair(x > 0.0f ? 1.0f : x != x ? x : 0.0f, y > 0.0f ? 1.0f : y != y ? y : 0.0f);
+  if (kAct == kActRelu) {  // chosen, not multiplied: an infinite g has no part where the slope is 0
+    float a, b;
+    parts(g, a, b);
+    return pair(x > 0.0f ? a : x != x ? x : 0.0f, y > 0.0f ? b : y != y ? y : 0.0f);
+  }
   const float least = kAct == kActSilu ? kSiluLeast : kGeluLeast;
   const Pair z = pair(act_min_nan(act_max_nan(x, least), -least), act_min_nan(act_max_nan(y, least), -least));
   Pair v = z * pair(-kLog2E, -kLog2E), zdv = z;

@@ -591,3 +591,20 @@ def test_fp32_gradients_of_any_size_in_a_graph():
         torch.cuda.synchronize()
         want = step()
         assert all(torch.equal(p, q) for p, q in zip(caught, want)) and want[0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(5, 64, 40), (300, 264, 200)])
+@pytest.mark.parametrize("out_dtype", [None, F32])
+def test_infinite_gradients_of_what_relu_leaves_out(m, k, n, out_dtype):
+    """Where its argument is not above 0 nothing depends on the result, whatever the gradient is there."""
+    x, w, b, _, _ = make(m, k, n, BF16, 17)
+    dy = torch.randn(m, n, generator=torch.Generator().manual_seed(18)).to(out_dtype or BF16).cuda()
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    y = ops.linear(*leaves, activation="relu", out_dtype=out_dtype)
+    off = y.detach() == 0
+    assert off.any() and not off.all()
+    want = torch.autograd.grad(y, leaves, torch.where(off, 0.0, dy), retain_graph=True)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        got = torch.autograd.grad(y, leaves, torch.where(off, bad, dy), retain_graph=True)
+        assert all(torch.isfinite(p).all() and torch.equal(p, q) for p, q in zip(want, got))

@@ -17,7 +17,8 @@ class Muon(torch.optim.Optimizer):
     """``m = momentum m + g``, ``u = g + momentum m`` (or ``m`` without ``nesterov``), and then
     ``p = p (1 - lr weight_decay) - lr sqrt(max(1, height / width)) orthogonalize(u)``.
 
-    Parameters: matrices on a CUDA device.  The momentum has the gradient's type."""
+    Parameters: matrices on a CUDA device.  The momentum has the gradient's type, as in torch's own optimisers: float32 for float32 weights, which the
+    trainer's are."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5):
         if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
