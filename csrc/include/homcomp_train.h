@@ -86,6 +86,30 @@ size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
 int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
                      int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 
+// ---- AdamW ------------------------------------------------------------------------------------------------------------------
+// One step over `count` tensors (a list in host memory, read before the call returns; no two of its tensors overlap):
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr decay) - (m / (sqrt(v) / sqrt(1 - b2^step) + eps)) lr / (1 - b1^step)
+// All parameters are of param_type, all gradients of grad_type: the same, or param_type fp32.  They may begin anywhere; 16-byte
+// alignment is faster.
+// bits 32: the moments are fp32, `scales` is not used.  bits 8: a byte each, and `scales` has 2 floats for every 256 values, the largest |m|
+// and the largest sqrt(v) among them (8-byte aligned).  m is a sign, 4 bits of exponent and 3 of fraction relative to its largest, sqrt(v) 4 and 4 bits; all zeros
+// is the state to begin with.  Both are rounded up or down at random, by a hash of the value's number, the tensor's `number`, step and seed.
+// A block that gets a value which is not finite becomes NaN as a whole; one whose largest value is below 2^-100 is held as zeros.
+// lr_at, step_at: where they are in device memory (float, int64), so that a captured call goes on counting; NULL: `lr` and `step` (from 1).
+typedef struct hc_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scales;
+  size_t n;
+  uint32_t number;
+} hc_adamw_tensor;
+int hc_adamw(const hc_adamw_tensor* tensors, size_t count, int param_type, int grad_type, int bits, double lr, const float* lr_at, double beta1, double beta2,
+             double eps, double weight_decay, int64_t step, const int64_t* step_at, uint64_t seed, hc_stream_t stream);
+// What moments in 8 bits stand for: n values of m and of v, the first of them the first of a block.
+int hc_adamw_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const float* scales, size_t n, float* m, float* v, hc_stream_t stream);
+
 // The kernels' waits are bounded (2 s).  Where one ran out the call's results are wrong.  Synchronises the device and returns 3 if that
 // happened since the status was last cleared, 0 if not.
 int hc_train_status(int clear);

@@ -15,9 +15,11 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <string>
 #include <tuple>
 #include <unordered_map>
+#include <vector>
 
 #include "homcomp_train.h"
 
@@ -42,6 +44,8 @@ struct Api {
   decltype(&hc_linear_backward) linear_backward;
   decltype(&hc_orthogonalize_bytes) orthogonalize_bytes;
   decltype(&hc_orthogonalize) orthogonalize;
+  decltype(&hc_adamw) adamw;
+  decltype(&hc_adamw_values) adamw_values;
 } api;
 
 void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
@@ -58,6 +62,8 @@ void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
   HC_BIND(linear_backward);
   HC_BIND(orthogonalize_bytes);
   HC_BIND(orthogonalize);
+  HC_BIND(adamw);
+  HC_BIND(adamw_values);
 #undef HC_BIND
 }
 
@@ -462,6 +468,144 @@ Tensor orthogonalize(const Tensor& update_, int64_t steps, double a, double b, d
   return out;
 }
 
+// ---- AdamW ------------------------------------------------------------------------------------------------------------
+constexpr int64_t kAdamBlock = 256;  // values that share a scale
+struct Stretch {
+  uintptr_t begin, end;
+  bool written;
+};
+void add_stretch(std::vector<Stretch>& all, const Tensor& t, bool written) {
+  const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel()) all.push_back({at, at + t.numel() * t.element_size(), written});
+}
+// whether something that is written lies where something else is written or read
+bool any_overlap(std::vector<Stretch>& all) {
+  std::sort(all.begin(), all.end(), [](const Stretch& a, const Stretch& b) { return a.begin < b.begin; });
+  uintptr_t end = 0, written_end = 0;
+  for (const Stretch& s : all) {
+    if (s.begin < written_end || (s.written && s.begin < end)) return true;
+    end = std::max(end, s.end);
+    if (s.written) written_end = std::max(written_end, s.end);
+  }
+  return false;
+}
+void changed_in_place(const char* name, size_t i, const Tensor& t, const Tensor& p, at::ScalarType type) {
+  TORCH_CHECK_VALUE(t.device() == p.device(), name, "[", i, "] is on ", t.device(), ", not on ", p.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == type, name, "[", i, "] is of type ", t.scalar_type(), ", not ", type);
+  TORCH_CHECK_VALUE(!t.is_neg() && !t.is_conj(), name, "[", i, "]: expected a tensor that is what lies in its memory");
+}
+// the values of both lie in the same order
+bool same_order(const Tensor& t, const Tensor& p) {
+  if (!t.sizes().equals(p.sizes())) return false;
+  if (t.is_contiguous() && p.is_contiguous()) return true;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) != p.stride(d)) return false;
+  return true;
+}
+void one_value(const char* name, const Tensor& t, at::ScalarType type, const Tensor& p) {
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.numel() == 1 && t.device() == p.device(), "adamw_step: ", name, " is a number or one value of type ", type, " on ", p.device());
+}
+
+void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs,
+                const std::optional<std::vector<Tensor>>& scales, double lr, const OptTensor& lr_at, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                const OptTensor& step_at, uint64_t seed) {
+  not_recorded();
+  const size_t count = params.size();
+  TORCH_CHECK_VALUE(grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count && (!scales || scales->size() == count),
+                    "adamw_step: lists of different lengths: ", count, " parameters, ", grads.size(), " gradients, ", exp_avgs.size(), " and ", exp_avg_sqs.size(), " moments");
+  TORCH_CHECK_VALUE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw_step: betas are from 0 to below 1");
+  TORCH_CHECK_VALUE(eps >= 0 && weight_decay >= 0 && (lr_at || lr >= 0), "adamw_step: lr, eps and weight_decay are not negative");
+  TORCH_CHECK_VALUE(step_at || step >= 1, "adamw_step: steps count from 1");
+  if (!count) return;
+  const Tensor& first = params[0];
+  floating("params[0]", first);
+  if (lr_at) one_value("lr", *lr_at, at::kFloat, first);
+  if (step_at) one_value("step", *step_at, at::kLong, first);
+  const c10::cuda::CUDAGuard guard(first.device());
+  const at::NoGradGuard no_grad;
+  const at::ScalarType state = scales ? at::kByte : at::kFloat;
+  std::vector<Stretch> stretches;
+  stretches.reserve(5 * count + 2);
+  std::vector<Tensor> copies;  // of gradients that lie in another order
+  struct Kind {
+    int param, grad;
+    std::vector<hc_adamw_tensor> tensors;
+  };
+  std::vector<Kind> kinds;
+  for (size_t i = 0; i < count; ++i) {
+    const Tensor& p = params[i];
+    ordinary("params", p);
+    ordinary("grads", grads[i]);
+    TORCH_CHECK_VALUE(p.layout() == at::kStrided && grads[i].layout() == at::kStrided, "adamw_step: expected dense tensors");
+    floating("params", p);
+    floating("grads", grads[i]);
+    changed_in_place("params", i, p, first, p.scalar_type());
+    TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "params[", i, "] has gaps");
+    TORCH_CHECK_VALUE(grads[i].device() == p.device() && grads[i].sizes().equals(p.sizes()), "grads[", i, "] of shape ", grads[i].sizes(), " on ", grads[i].device(), " for a parameter of shape ",
+                      p.sizes(), " on ", p.device());
+    TORCH_CHECK_VALUE(grads[i].scalar_type() == p.scalar_type() || p.scalar_type() == at::kFloat, "grads[", i, "] is of type ", grads[i].scalar_type(), ", its parameter ", p.scalar_type());
+    changed_in_place("exp_avgs", i, exp_avgs[i], first, state);
+    changed_in_place("exp_avg_sqs", i, exp_avg_sqs[i], first, state);
+    TORCH_CHECK_VALUE(same_order(exp_avgs[i], p) && same_order(exp_avg_sqs[i], p), "exp_avgs[", i, "], exp_avg_sqs[", i, "]: expected the shape and strides of the parameter");
+    Tensor g = held(grads[i]);
+    if (!same_order(g, p)) {
+      g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
+      copies.push_back(g);
+    } else if (!g.is_same(grads[i])) {
+      copies.push_back(g);
+    }
+    const int64_t n = p.numel();
+    if (scales) {
+      const Tensor& s = (*scales)[i];
+      changed_in_place("scales", i, s, first, at::kFloat);
+      TORCH_CHECK_VALUE(s.is_contiguous() && s.dim() == 2 && s.size(1) == 2 && s.size(0) == (n + kAdamBlock - 1) / kAdamBlock && reinterpret_cast<uintptr_t>(s.data_ptr()) % 8 == 0, "scales[", i,
+                        "]: expected two values for every ", kAdamBlock, " of the ", n, " parameters, got shape ", s.sizes());
+      add_stretch(stretches, s, true);
+    }
+    add_stretch(stretches, p, true);
+    add_stretch(stretches, exp_avgs[i], true);
+    add_stretch(stretches, exp_avg_sqs[i], true);
+    add_stretch(stretches, g, false);
+    const int pt = type_of(p), gt = type_of(g);
+    auto kind = std::find_if(kinds.begin(), kinds.end(), [&](const Kind& k) { return k.param == pt && k.grad == gt; });
+    if (kind == kinds.end()) kind = kinds.insert(kinds.end(), Kind{pt, gt, {}});
+    kind->tensors.push_back({p.data_ptr(), g.data_ptr(), exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr(), scales ? static_cast<float*>((*scales)[i].data_ptr()) : nullptr, (size_t)n, (uint32_t)i});
+  }
+  if (lr_at) add_stretch(stretches, *lr_at, false);
+  if (step_at) add_stretch(stretches, *step_at, false);
+  TORCH_CHECK_VALUE(!any_overlap(stretches), "adamw_step: tensors overlap, or one is in the lists twice");
+  for (const Kind& k : kinds)
+    check(api.adamw(k.tensors.data(), k.tensors.size(), k.param, k.grad, scales ? 8 : 32, lr, static_cast<float*>(ptr(lr_at)), beta1, beta2, eps, weight_decay, step,
+                    static_cast<int64_t*>(ptr(step_at)), seed, stream_of(first)),
+          "adamw_step");
+  for (size_t i = 0; i < count; ++i) {  // whoever kept one of them for a backward pass is told
+    params[i].unsafeGetTensorImpl()->bump_version();
+    exp_avgs[i].unsafeGetTensorImpl()->bump_version();
+    exp_avg_sqs[i].unsafeGetTensorImpl()->bump_version();
+    if (scales) (*scales)[i].unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+std::tuple<Tensor, Tensor> adamw_values(const Tensor& exp_avg, const Tensor& exp_avg_sq, const Tensor& scales) {
+  not_recorded();
+  ordinary("exp_avg", exp_avg);
+  ordinary("exp_avg_sq", exp_avg_sq);
+  ordinary("scales", scales);
+  TORCH_CHECK_VALUE(exp_avg.is_cuda() && exp_avg.scalar_type() == at::kByte && exp_avg.is_non_overlapping_and_dense(), "adamw_values: expected moments of type uint8 on a CUDA device, without gaps");
+  changed_in_place("exp_avg_sq", 0, exp_avg_sq, exp_avg, at::kByte);
+  changed_in_place("scales", 0, scales, exp_avg, at::kFloat);
+  TORCH_CHECK_VALUE(same_order(exp_avg_sq, exp_avg), "adamw_values: moments of different shapes or strides");
+  const int64_t n = exp_avg.numel();
+  TORCH_CHECK_VALUE(scales.is_contiguous() && scales.dim() == 2 && scales.size(1) == 2 && scales.size(0) == (n + kAdamBlock - 1) / kAdamBlock && reinterpret_cast<uintptr_t>(scales.data_ptr()) % 8 == 0,
+                    "adamw_values: expected two scales for every ", kAdamBlock, " of ", n, " values, got shape ", scales.sizes());
+  const c10::cuda::CUDAGuard guard(exp_avg.device());
+  Tensor m = at::empty_strided(exp_avg.sizes(), exp_avg.strides(), exp_avg.options().dtype(at::kFloat)), v = at::empty_like(m);
+  check(api.adamw_values(static_cast<uint8_t*>(exp_avg.data_ptr()), static_cast<uint8_t*>(exp_avg_sq.data_ptr()), static_cast<float*>(scales.data_ptr()), (size_t)n,
+                         static_cast<float*>(m.data_ptr()), static_cast<float*>(v.data_ptr()), stream_of(exp_avg)),
+        "adamw_values");
+  return {m, v};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -470,4 +614,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear);
   m.def("token_logprobs", &token_logprobs);
   m.def("orthogonalize", &orthogonalize);
+  m.def("adamw_step", &adamw_step);
+  m.def("adamw_values", &adamw_values);
 }

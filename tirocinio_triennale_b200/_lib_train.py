@@ -7,7 +7,7 @@ vp = C.c_void_p
 
 
 def declare(lib):
-    sz, f, i, l = C.c_size_t, C.c_float, C.c_int, C.c_int64
+    sz, f, d, i, l = C.c_size_t, C.c_float, C.c_double, C.c_int, C.c_int64
     sizes = {
         "hc_layer_norm_backward_bytes": [sz, sz],
         "hc_linear_bytes": [sz, sz, sz],
@@ -21,6 +21,8 @@ def declare(lib):
         "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp, sz, vp],
         "hc_linear_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, sz, i, vp, sz, vp, sz, vp, i, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],
+        "hc_adamw": [vp, sz, i, i, i, d, vp, d, d, d, d, l, vp, C.c_uint64, vp],
+        "hc_adamw_values": [vp, vp, vp, sz, vp, vp, vp],
         "hc_train_status": [i],
         "hc_token_logprobs": [vp, i, sz, sz, sz, vp, l, i, vp, vp, vp, vp, vp, vp],
         "hc_token_logprobs_backward": [vp, i, sz, sz, sz, vp, l, vp, vp, vp, vp, sz, vp],

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from .adamw import AdamW
 
 
 class Muon(torch.optim.Optimizer):
@@ -81,8 +82,11 @@ class Optimizers:
             o.load_state_dict(s)
 
 
-def muon_with_adamw(model: torch.nn.Module, lr: float = 0.02, adam_lr: float = 3e-4, momentum: float = 0.95, weight_decay: float = 0.0) -> Optimizers:
-    """Muon for the matrices of ``model``'s linear layers, AdamW for everything else; one of them alone where the other has nothing."""
+def muon_with_adamw(model: torch.nn.Module, lr: float = 0.02, adam_lr: float = 3e-4, momentum: float = 0.95, weight_decay: float = 0.0,
+                    adam_bits: int | None = None) -> Optimizers:
+    """Muon for the matrices of ``model``'s linear layers, AdamW for everything else; one of them alone where the other has nothing.
+
+    ``adam_bits``: None for torch's AdamW, 32 or 8 for this library's with moments of so many bits."""
     matrices = {id(m.weight) for m in model.modules() if isinstance(m, torch.nn.Linear)}
     embedded = {id(m.weight) for m in model.modules() if isinstance(m, torch.nn.Embedding)}  # also where they are the output's
     matrices -= embedded
@@ -91,6 +95,8 @@ def muon_with_adamw(model: torch.nn.Module, lr: float = 0.02, adam_lr: float = 3
     optimizers = []
     if turned:
         optimizers.append(Muon(turned, lr=lr, momentum=momentum, weight_decay=weight_decay))
-    if others:
+    if others and adam_bits is not None:
+        optimizers.append(AdamW(others, lr=adam_lr, weight_decay=weight_decay, bits=adam_bits))
+    elif others:
         optimizers.append(torch.optim.AdamW(others, lr=adam_lr, weight_decay=weight_decay, fused=all(p.is_cuda for p in params)))
     return Optimizers(*optimizers)

@@ -9,7 +9,7 @@ side stream, and (b) with plain NCCL.  Prints one JSON line with tokens/s of bot
 gap after the last step.  Random-init weights, uniform random token ids (no dataset, no download).
 
 ``--fused`` runs the model through this library's operators (layer norm, products with their epilogues, the
-loss over the logits); ``--optimizer muon`` orthogonalises the updates of the blocks' matrices.
+loss over the logits); ``--optimizer muon`` orthogonalises the updates of the blocks' matrices; ``--adam-bits`` takes this library's AdamW, with moments in 32 or 8 bits.
 
 ``--save PATH`` writes model, optimiser, step count and the data generator's state after the last
 step (rank 0; one file per arm: PATH.compressed / PATH.nccl); ``--resume PATH`` continues from such
@@ -29,6 +29,7 @@ from torch.nn.parallel import DistributedDataParallel as DDP
 
 from ..ops import train_status
 from ..parallel import CompressedHookState, compressed_allreduce_hook
+from .adamw import AdamW
 from .gpt2 import GPT2, GPT2Config
 from .muon import muon_with_adamw
 
@@ -53,8 +54,11 @@ def run(args, compressed: bool, rank: int, world: int, device):
     if compressed:
         state = CompressedHookState(eb=args.eb, max_bucket_elems=int(args.bucket_mb * 1.5 * 1024 * 1024 / 4) + (1 << 20))
         ddp.register_comm_hook(state, compressed_allreduce_hook)
+    adam_bits = getattr(args, "adam_bits", None)
     if getattr(args, "optimizer", "adamw") == "muon":
-        opt = muon_with_adamw(model, lr=args.muon_lr, adam_lr=args.lr)
+        opt = muon_with_adamw(model, lr=args.muon_lr, adam_lr=args.lr, adam_bits=adam_bits)
+    elif adam_bits is not None:
+        opt = AdamW(ddp.parameters(), lr=args.lr, weight_decay=0.0, bits=adam_bits)
     else:
         opt = torch.optim.AdamW(ddp.parameters(), lr=args.lr, weight_decay=0.0, fused=device.type == "cuda")
     g = torch.Generator(device="cpu").manual_seed(100 + rank)
@@ -120,6 +124,7 @@ def main(argv=None):
     ap.add_argument("--lr", type=float, default=3e-4)
     ap.add_argument("--fused", action="store_true", help="this library's operators in the model")
     ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"])
+    ap.add_argument("--adam-bits", type=int, default=None, choices=[8, 32], help="this library's AdamW with moments of so many bits, in place of torch's")
     ap.add_argument("--muon-lr", type=float, default=0.02)
     ap.add_argument("--bucket-mb", type=float, default=25.0)
     ap.add_argument("--cpu", action="store_true", help="gloo + host-rank ring (functional check without GPUs)")
@@ -128,8 +133,8 @@ def main(argv=None):
     ap.add_argument("--save-compressed-eb", type=float, default=0.0,
                     help="also write the weights as error-bounded streams with this absolute bound")
     args = ap.parse_args(argv)
-    if args.cpu and (args.fused or args.optimizer == "muon"):
-        ap.error("--fused and --optimizer muon need a GPU")
+    if args.cpu and (args.fused or args.optimizer == "muon" or args.adam_bits is not None):
+        ap.error("--fused, --optimizer muon and --adam-bits need a GPU")
 
     rank = int(os.environ.get("RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))
