@@ -25,6 +25,7 @@ constexpr int kGemmThreads = 64 + 32 * kStoreWarps;
 constexpr int kOperandA = kBM * kBK * 2;
 constexpr int kGemmLinearWide = 4;  // kGemmLinear whose sums are formed in parts
 constexpr int kGemmGramWide = 5;    // kGemmGram, the same
+constexpr int kGemmLossSumsWide = 8;  // kGemmLossSums, the same
 constexpr uint64_t kGemmLimitNs = 2000ull * 1000 * 1000;
 
 struct GemmParams {
@@ -47,6 +48,7 @@ struct GemmParams {
   float ca, cb, cc;
   const float* scale;
   const unsigned int* most;
+  GemmLoss loss;
   int tma_out, tma_out2, tma_in, tma_in2;              // moved by TMA: rows that begin at 16 bytes
   int wide_boxes;                                      // map_out and map_out2 are of boxes of 32 x 64 values
 };
@@ -378,6 +380,48 @@ __device__ __forceinline__ void gemm_finish_half(const GemmParams& p, float (&v)
   for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(wide_at(out, lane, half * 4 + i)) = pack8_as(v + i * 8, p.type);
 }
 
+__device__ __forceinline__ float power2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// 32 logits of a row from column `col` on, of which `count` are of the vocabulary, taken up into the row's largest logit and the sum of
+// exponentials relative to it.  A NaN, or an infinite logit, makes the sum NaN; a row of -inf alone has a sum of 0.
+__device__ __forceinline__ void loss_take(float (&v)[32], int64_t count, int64_t token, float& most, float& sum, float* picked) {
+  if (count < 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = j < count ? v[j] : -INFINITY;
+  }
+  if (token >= 0 && token < 32 && token < count) {
+    // by the bits of its number (a comparison with each of the 32 becomes an array in local memory)
+    float w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = token & 1 ? v[2 * j + 1] : v[2 * j];
+#pragma unroll
+    for (int bit = 1; bit < 5; ++bit)
+#pragma unroll
+      for (int j = 0; j < 16 >> bit; ++j) w[j] = token >> bit & 1 ? w[2 * j + 1] : w[2 * j];
+    *picked = w[0];
+  }
+  float top = fmaxf(v[0], v[1]);
+#pragma unroll
+  for (int j = 2; j < 32; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));
+  if (top > most) {
+    sum = most == -INFINITY ? sum : sum * power2((most - top) * kLog2E);
+    most = top;
+  }
+  const float ref = most == -INFINITY ? 0.0f : -most;
+  Pair total = pair(0.0f, 0.0f);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float a, b;
+    parts((pair(v[j], v[j + 1]) + pair(ref, ref)) * pair(kLog2E, kLog2E), a, b);
+    total = total + pair(power2(a), power2(b));
+  }
+  sum += both(total);
+}
+
 // What the three roles carry from tile to tile (and, in a chain of products, from one to the next).
 struct Loading {
   int s = 0, issued = 0;
@@ -465,7 +509,7 @@ __device__ __forceinline__ void multiply_tiles(const GemmParams& p, GemmBarriers
   const int total = p.tiles * p.batch;
   for (int t = unit; st.ok && t < total; t += units) {
     for (int begin = 0; begin < p.k_blocks; begin += kChunk) {
-      const int end = MODE == kGemmLinearWide || MODE == kGemmGramWide ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
+      const int end = MODE == kGemmLinearWide || MODE == kGemmGramWide || MODE == kGemmLossSumsWide ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
       if (!gemm_wait(&sh.acc_empty[st.acc], st.acc_phase ^ 1, sh)) {
         st.ok = false;
         return;
@@ -517,7 +561,8 @@ __device__ __forceinline__ void release_accumulator(GemmBarriers& sh, Storing& s
 template <int BN, int kCtas, int MODE>
 __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* mine, Storing& st, uint32_t tmem, int unit, int units, int rank) {
   using S = GemmShape<BN, kCtas>;
-  constexpr bool kWide = MODE == kGemmLinearWide || MODE == kGemmGramWide, kLinear = MODE == kGemmLinear || MODE == kGemmLinearWide;
+  constexpr bool kWide = MODE == kGemmLinearWide || MODE == kGemmGramWide || MODE == kGemmLossSumsWide, kLinear = MODE == kGemmLinear || MODE == kGemmLinearWide;
+  constexpr bool kLossSums = MODE == kGemmLossSums || MODE == kGemmLossSumsWide;
   constexpr bool kSymmetric = MODE == kGemmGram || MODE == kGemmGramWide || MODE == kGemmPoly;
   constexpr int kMode = MODE == kGemmLinearWide ? kGemmLinear : MODE == kGemmGramWide ? kGemmGram : MODE;
   constexpr int kPieces = kWide ? (BN / 32 + 1) / 2 : 1;  // of a warp
@@ -576,6 +621,79 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
         return;
       }
       tc_fence_after();
+    }
+    if constexpr (kLossSums) {
+      // thread i has row i: its largest logit and sum over this warp's pieces of the tile
+      const int64_t row = row0 + lane;
+      const int64_t token = row < p.m ? p.loss.tokens[row] - p.loss.first : -1;
+      float most = -INFINITY, sum = 0.0f;
+      if constexpr (kWide) {
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q) {
+          const int col = col0 + (half + 2 * q) * 32;
+          if (half + 2 * q < pieces) loss_take(sums[q], p.n - col, token - col, most, sum, p.loss.picked + row);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = half; c < pieces; c += 2) {
+          __syncwarp();
+          tc_load32(lanes + st.acc * BN + c * 32, sums[0]);
+          tc_load_wait(sums[0]);
+          loss_take(sums[0], p.n - col0 - c * 32, token - col0 - c * 32, most, sum, p.loss.picked + row);
+        }
+        release_accumulator<kCtas>(sh, st, rank);
+      }
+      if (row < p.m) p.loss.sums[(int64_t)(ni * 2 + half) * p.m + row] = make_float2(most, sum);
+      continue;
+    }
+    if constexpr (MODE == kGemmLossGrad) {
+      const int64_t row = row0 + lane;
+      const bool in = row < p.m;
+      const int64_t given = in ? p.loss.tokens[row] : p.loss.ignore, token = given - p.loss.first;
+      const bool kept = given != p.loss.ignore;
+      const float less = kept ? -p.loss.lse[row] : 0.0f;
+      float weight = kept ? p.loss.weight[row] : 0.0f;
+      if (p.most) weight *= gradient_power(p.most, 1);
+      constexpr int kPer = BN >= 128 ? 2 : 1;  // pieces of a box
+#pragma unroll 1
+      for (int c = half * kPer; c < pieces; c += 2 * kPer) {
+        unsigned char* slot = mine + (st.uses & 1) * kSlot;
+        if (lane == 0) tma_wait_group_read<1>();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) {
+          float(&v)[32] = sums[0];
+          tc_load32(lanes + st.acc * BN + (c + h) * 32, v);
+          tc_load_wait(v);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float a, b;
+            parts((pair(v[j], v[j + 1]) + pair(less, less)) * pair(kLog2E, kLog2E), a, b);
+            parts(pair(power2(a), power2(b)) * pair(weight, weight), v[j], v[j + 1]);
+          }
+          const int64_t at = token - (col0 + (c + h) * 32);
+          if (at >= 0 && at < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = j == (int)at ? v[j] - weight : v[j];
+          }
+          if (!kept) {  // also where the row's logits are no numbers
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *(kPer == 2 ? reinterpret_cast<uint4*>(wide_at(slot, lane, h * 4 + i)) : half_at(slot, lane, i)) = pack8_as(v + i * 8, p.type);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&p.map_out, col0 + c * 32, row0, 0, slot);
+          tma_commit_group();
+        }
+        ++st.uses;
+      }
+      release_accumulator<kCtas>(sh, st, rank);
+      continue;
     }
     const auto piece = [&](int c, float (&v)[32]) {  // false: a wait ran out
       const int col = col0 + c * 32;
@@ -977,6 +1095,9 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.cc = c.cc;
   p.scale = c.scale;
   p.most = c.most;
+  p.loss = c.loss;
+  if (MODE == kGemmLossSums || MODE == dev::kGemmLossSumsWide) return cudaSuccess;
+  if (MODE == kGemmLossGrad) return make_side_map(&p.map_out, c.out, c.type, c, true, false, BN >= 128) ? cudaSuccess : cudaErrorInvalidValue;
   constexpr bool kLinear = MODE == kGemmLinear || MODE == dev::kGemmLinearWide, kUpdate = MODE == kGemmUpdate;
   if (MODE == kGemmLinear && BN >= 128 && c.out_type != kF32 && !c.in.data && make_side_map(&p.map_out, c.out, c.out_type, c, true, false, true))
     p.wide_boxes = !c.out2.data || make_side_map(&p.map_out2, c.out2, c.type, c, true, false, true);
@@ -1039,7 +1160,7 @@ TileChoice best_tile(const GemmCall& c, int parts, int64_t sms) {
   TileChoice best = {0, 0, 0};
   for (const auto& s : shapes) {
     const int64_t tiles = count_tiles<MODE>(c, dev::kBM * s[1], s[0]) * c.batch * parts, units = sms / s[1];
-    const int stage = MODE == kGemmLinear && c.m <= dev::kBM * s[1] && s[2] < 650 ? 650 : s[2];
+    const int stage = MODE != kGemmGram && MODE != kGemmPoly && MODE != kGemmUpdate && c.m <= dev::kBM * s[1] && s[2] < 650 ? 650 : s[2];
     const int64_t cost = (tiles + units - 1) / units * (stages * stage + 1000 + 4 * s[0]);
     if (best.bn == 0 || cost < best.cost) best = {s[0], s[1], cost};
   }
@@ -1120,6 +1241,26 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
   }
   return best;
 }
+
+int64_t gemm_cost(int64_t m, int64_t n, int64_t k) {
+  GemmCall c;
+  memset(&c, 0, sizeof(c));
+  c.m = m, c.n = n, c.k = k, c.batch = 1;
+  return best_tile<kGemmLinear>(c, 1, sm_count()).cost;
+}
+
+int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k) {
+  GemmCall c;
+  memset(&c, 0, sizeof(c));
+  c.m = m, c.n = n, c.k = k, c.batch = 1;
+  const int bn = best_tile<kGemmLossSums>(c, 1, sm_count()).bn;
+  return (n + bn - 1) / bn * 2;
+}
+
+cudaError_t launch_loss_sums(const GemmCall& c, cudaStream_t stream) {
+  return c.k > dev::kChunk * dev::kBK ? run_gemm_mode<dev::kGemmLossSumsWide>(c, stream) : run_gemm_mode<kGemmLossSums>(c, stream);
+}
+cudaError_t launch_loss_grad(const GemmCall& c, cudaStream_t stream) { return run_gemm_mode<kGemmLossGrad>(c, stream); }
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
   // sums in parts cost 8 % at 8192 x 4096 x 8192 (392 us with a bf16 result, 403 with fp32, 437 with fp32 sums in parts), 6 % at

@@ -12,6 +12,8 @@ enum GemmMode : int {
   kGemmGram = 1,    // out = acc, symmetric
   kGemmPoly = 2,    // out = b c1 + c acc, symmetric (c1: the operand itself)
   kGemmUpdate = 3,  // x = a (hi + lo / 2048) + acc; out hi and lo again, or bf16
+  kGemmLossSums = 6,  // acc are logits: each row's largest and sum of exponentials, over stretches of columns; the logit of the row's token
+  kGemmLossGrad = 7,  // out = weight (exp(acc - lse) - [the row's token])
 };
 enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActRelu = 2, kActSilu = 3 };
 
@@ -103,6 +105,16 @@ struct GemmSide {
   int64_t ld;
   int64_t stride;
 };
+// of the products that form logits
+struct GemmLoss {
+  const int64_t* tokens;  // a row's token; `ignore`: a row that has none
+  int64_t ignore;
+  int64_t first;       // the vocabulary's number of column 0
+  float2* sums;        // [stretch][row]: the largest logit of a stretch of columns and the sum of exp(logit - that); gemm_loss_stretches
+  float* picked;       // the token's logit
+  const float* lse;    // of a row
+  const float* weight;
+};
 struct GemmCall {
   int type;  // of the operands
   int64_t m, n, k, batch;
@@ -118,10 +130,17 @@ struct GemmCall {
   float ca, cb, cc;
   const float* scale;  // of each matrix of a batch (kGemmPoly, kGemmUpdate): X is that times what is stored
   const unsigned int* most;  // kGemmLinear without anything behind it: see gradient_power, whose inverse the result is taken times; or NULL
+  GemmLoss loss;             // kGemmLossSums, kGemmLossGrad
 };
 
 // Into how many parts the sum of a product is best shared out (1: none).
 int gemm_parts(int64_t m, int64_t n, int64_t k);
+// What a call's time is reckoned to be, in cycles, as a single part.
+int64_t gemm_cost(int64_t m, int64_t n, int64_t k);
+// stretches of columns of kGemmLossSums, two a tile
+int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k);
+cudaError_t launch_loss_sums(const GemmCall& call, cudaStream_t stream);
+cudaError_t launch_loss_grad(const GemmCall& call, cudaStream_t stream);
 // act(a b + bias) + residual
 cudaError_t launch_gemm(const GemmCall& call, cudaStream_t stream);
 // The products of a Newton-Schulz iteration in one launch: step i takes gram[i % 2], poly and update[i % 2], the last one `last`.

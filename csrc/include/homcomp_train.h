@@ -86,6 +86,23 @@ size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
 int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
                      int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 
+// ---- cross entropy from hidden rows ------------------------------------------------------------------------------------
+// loss_i = log sum_v exp(x_i . w_v) - x_i . w_token, without the logits ever being stored: x [rows][inner], weight [vocab][inner], both of `type` (1 or 2), as operands
+// of a product lie (16-byte aligned, strides multiples of 8), sides below 2^26; sums in the tensor core over up to 1024 terms.
+// reduction: 0 none (loss: a value a row), 1 sum, 2 mean over the rows that have a token (loss: one value; NaN where there are none).  A row whose token is `ignore`
+// gives 0 and a gradient of 0, whatever it holds, and enters dweight times 0; a token outside the vocabulary gives NaN, in the gradient in all of dweight.
+// stats: rows + 1 floats for the backward pass.  Scratch memory, 256-byte aligned: hc_linear_cross_entropy_bytes for the current device.
+size_t hc_linear_cross_entropy_bytes(size_t rows, size_t inner, size_t vocab);
+int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const int64_t* tokens, int64_t ignore, int reduction, float* loss,
+                            float* stats, size_t rows, size_t inner, size_t vocab, void* scratch, size_t scratch_bytes, hc_stream_t stream);
+// dx = G weight and dweight = G^T x (of `type`, each NULL where it is not wanted) with G = a (p - 1[token]); a: dloss (fp32) of the row, or dloss[0], over the count for a mean.
+// G is formed for a piece of the vocabulary at a time, in 16 bits (of fp16 times a power of two that the largest |a| gives), in scratch memory of at most 256 MiB or 1024 columns;
+// dx is summed in fp32.  Where a result's stride is its width rounded up to eight, what lies behind its rows may be overwritten.
+size_t hc_linear_cross_entropy_backward_bytes(size_t rows, size_t inner, size_t vocab);
+int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const int64_t* tokens, int64_t ignore, int reduction,
+                                     const float* stats, const float* dloss, void* dx, size_t dx_stride, void* dweight, size_t dweight_stride, size_t rows, size_t inner, size_t vocab,
+                                     void* scratch, size_t scratch_bytes, hc_stream_t stream);
+
 // ---- AdamW ------------------------------------------------------------------------------------------------------------------
 // One step over `count` tensors (a list in host memory, read before the call returns; no two of its tensors overlap):
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr decay) - (m / (sqrt(v) / sqrt(1 - b2^step) + eps)) lr / (1 - b1^step)

@@ -44,6 +44,10 @@ struct Api {
   decltype(&hc_linear_backward) linear_backward;
   decltype(&hc_orthogonalize_bytes) orthogonalize_bytes;
   decltype(&hc_orthogonalize) orthogonalize;
+  decltype(&hc_linear_cross_entropy_bytes) linear_cross_entropy_bytes;
+  decltype(&hc_linear_cross_entropy) linear_cross_entropy;
+  decltype(&hc_linear_cross_entropy_backward_bytes) linear_cross_entropy_backward_bytes;
+  decltype(&hc_linear_cross_entropy_backward) linear_cross_entropy_backward;
   decltype(&hc_adamw) adamw;
   decltype(&hc_adamw_values) adamw_values;
 } api;
@@ -62,6 +66,10 @@ void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
   HC_BIND(linear_backward);
   HC_BIND(orthogonalize_bytes);
   HC_BIND(orthogonalize);
+  HC_BIND(linear_cross_entropy_bytes);
+  HC_BIND(linear_cross_entropy);
+  HC_BIND(linear_cross_entropy_backward_bytes);
+  HC_BIND(linear_cross_entropy_backward);
   HC_BIND(adamw);
   HC_BIND(adamw_values);
 #undef HC_BIND
@@ -468,6 +476,77 @@ Tensor orthogonalize(const Tensor& update_, int64_t steps, double a, double b, d
   return out;
 }
 
+// ---- cross entropy from hidden rows ---------------------------------------------------------------------------------------
+enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
+// x and weight as the products read them
+Tensor loss_forward(const Tensor& x, const Tensor& weight, const Tensor& tokens, int64_t ignore, int reduction, at::IntArrayRef shape, Tensor* stats) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
+  const at::TensorOptions f = x.options().dtype(at::kFloat);
+  Tensor loss = reduction == kNone ? at::empty(shape, f) : at::empty({}, f);
+  *stats = at::empty({m + 1}, f);
+  const size_t need = api.linear_cross_entropy_bytes(m, k, n);
+  const Tensor scratch = scratch_of(need, x);
+  check(api.linear_cross_entropy(x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), type_of(x), static_cast<int64_t*>(tokens.data_ptr()), ignore, reduction,
+                                 static_cast<float*>(loss.data_ptr()), static_cast<float*>(stats->data_ptr()), m, k, n, ptr(scratch), need, stream_of(x)),
+        "linear_cross_entropy");
+  return loss;
+}
+
+struct LinearCrossEntropy : Function<LinearCrossEntropy> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& given, const Tensor& given_weight, const Tensor& given_tokens, int64_t ignore, int64_t reduction) {
+    const Tensor x = operand(matrix(given, given_weight.size(1))), weight = operand(given_weight), tokens = given_tokens.contiguous();
+    Tensor stats;
+    Tensor loss = loss_forward(x, weight, tokens, ignore, (int)reduction, given_tokens.sizes(), &stats);
+    ctx->save_for_backward({x, weight, tokens, stats});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["shape"] = given.sizes().vec();
+    return loss;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &tokens = saved[2], &stats = saved[3];
+    not_recorded();
+    ordinary("gradient", grads[0]);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
+    const bool graph = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
+    const Tensor dloss = held(grads[0]).contiguous();
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = empty_rows(m, k, x.options(), ctx->saved_data["shape"].toIntVector());
+    if (ctx->needs_input_grad(1)) dw = empty_rows(n, k, x.options());
+    const size_t need = api.linear_cross_entropy_backward_bytes(m, k, n);
+    const Tensor scratch = scratch_of(need, x);
+    check(api.linear_cross_entropy_backward(x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), type_of(x), static_cast<int64_t*>(tokens.data_ptr()),
+                                            ctx->saved_data["ignore"].toInt(), (int)ctx->saved_data["reduction"].toInt(), static_cast<float*>(stats.data_ptr()),
+                                            static_cast<float*>(dloss.data_ptr()), ptr(dx), padded(k), ptr(dw), padded(k), m, k, n, ptr(scratch), need, stream_of(x)),
+          "linear_cross_entropy backward");
+    return once({dx, dw, Tensor(), Tensor(), Tensor()}, graph);
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& x_, const Tensor& weight_, const Tensor& tokens_, int64_t ignore, int reduction) {
+  not_recorded();
+  ordinary("x", x_);
+  ordinary("weight", weight_);
+  ordinary("targets", tokens_);
+  const Tensor x = held(x_), weight = held(weight_), tokens = held(tokens_);
+  floating("x", x);
+  floating("weight", weight);
+  beside("weight", weight, x);
+  TORCH_CHECK_VALUE(type_of(x) != 0 && type_of(weight) == type_of(x), "linear_cross_entropy: x and weight are both bfloat16 or both float16, got ", x.scalar_type(), " and ", weight.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() > 0 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.numel() > 0, "linear_cross_entropy: no product of x ", x.sizes(), " and weight ", weight.sizes());
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.device() == x.device(), "linear_cross_entropy: expected int64 targets on the device of x");
+  TORCH_CHECK_VALUE(tokens.sizes().equals(x.sizes().slice(0, x.dim() - 1)), "linear_cross_entropy: targets of shape ", tokens.sizes(), " for x of shape ", x.sizes());
+  const int64_t n = weight.size(0), k = weight.size(1), m = x.numel() / k;
+  TORCH_CHECK_VALUE(std::max(m, std::max(n, k)) < (1 << 26), "linear_cross_entropy: every side is below 2^26");
+  if (at::GradMode::is_enabled() && (wants(x) || wants(weight))) return LinearCrossEntropy::apply(x, weight, tokens, ignore, (int64_t)reduction);
+  Tensor stats;
+  return loss_forward(operand(matrix(x, k)), operand(weight), tokens.contiguous(), ignore, reduction, tokens.sizes(), &stats);
+}
+
 // ---- AdamW ------------------------------------------------------------------------------------------------------------
 constexpr int64_t kAdamBlock = 256;  // values that share a scale
 struct Stretch {
@@ -614,6 +693,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear);
   m.def("token_logprobs", &token_logprobs);
   m.def("orthogonalize", &orthogonalize);
+  m.def("linear_cross_entropy", &linear_cross_entropy);
   m.def("adamw_step", &adamw_step);
   m.def("adamw_values", &adamw_values);
 }

@@ -13,6 +13,8 @@ def declare(lib):
         "hc_linear_bytes": [sz, sz, sz],
         "hc_linear_backward_bytes": [sz, sz, sz, i],
         "hc_orthogonalize_bytes": [sz, sz, sz],
+        "hc_linear_cross_entropy_bytes": [sz, sz, sz],
+        "hc_linear_cross_entropy_backward_bytes": [sz, sz, sz],
     }
     sigs = {
         "hc_layer_norm": [vp, i, vp, vp, i, vp, i, vp, sz, sz, f, vp],
@@ -21,6 +23,8 @@ def declare(lib):
         "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp, sz, vp],
         "hc_linear_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, sz, i, vp, sz, vp, sz, vp, i, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],
+        "hc_linear_cross_entropy": [vp, sz, vp, sz, i, vp, l, i, vp, vp, sz, sz, sz, vp, sz, vp],
+        "hc_linear_cross_entropy_backward": [vp, sz, vp, sz, i, vp, l, i, vp, vp, vp, sz, vp, sz, sz, sz, sz, vp, sz, vp],
         "hc_adamw": [vp, sz, i, i, i, d, vp, d, d, d, d, l, vp, C.c_uint64, vp],
         "hc_adamw_values": [vp, vp, vp, sz, vp, vp, vp],
         "hc_train_status": [i],

@@ -28,6 +28,7 @@ class GPT2Config:
     seq_len: int = 1024
     dropout: float = 0.0
     fused: bool = False  # this library's operators in place of torch's (CUDA, float32 weights, bfloat16 products)
+    logits: bool = True  # fused: the loss from the logits, or from the last hidden rows without them (``ops.linear_cross_entropy``)
 
     @staticmethod
     def small():
@@ -98,6 +99,8 @@ class GPT2(nn.Module):
         x = self.wte(idx) + self.wpe(pos)
         for b in self.blocks:
             x = b(x)
+        if self.cfg.fused and targets is not None and not self.cfg.logits:
+            return ops.linear_cross_entropy(_norm(x, self.ln_f), self.wte.weight.to(torch.bfloat16), targets)
         if self.cfg.fused:
             logits = ops.linear(_norm(x, self.ln_f), self.wte.weight.to(torch.bfloat16))
             if targets is None:
