@@ -11,8 +11,11 @@
 // Results leave through shared memory: a warp puts 32 rows of 32 values there (swizzled, so that no two of its threads meet
 // in a bank) and one TMA store takes them; what is added to a result comes in the same way, one piece ahead, and is
 // overwritten by the result in place.  Stored from registers, a row a thread, the projection 8192 x 2304 x 768 took 101 us.
+#include <initializer_list>
+
 #include "hc_gemm.cuh"
 #include "hc_host.cuh"
+#include "hc_tensor.cuh"
 #include "hc_train.cuh"
 #include "homcomp_train.h"
 
@@ -101,8 +104,6 @@ __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int 
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // arrives at the barrier, in a pair at both CTAs', when the matrix instructions so far are done
 template <int kCtas>
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -129,22 +130,6 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
         : "memory");
-}
-// 32 columns of this warp's 32 rows: thread i has row i.  The values are there after tc_load_wait.
-__device__ __forceinline__ void tc_load32(uint32_t addr, float* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
-        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
-        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(addr));
-}
-__device__ __forceinline__ void tc_load_wait(float (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));  // no use of a value moves in front of the wait
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, const void* src) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z),
@@ -214,10 +199,6 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
   unpack2<T>(w.y, v[2], v[3]);
   unpack2<T>(w.z, v[4], v[5]);
   unpack2<T>(w.w, v[6], v[7]);
-}
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* v) {
-  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 __device__ __forceinline__ uint4 pack8_as(const float* v, int type) {
   return type == kBf16 ? pack8<__nv_bfloat16>(v) : pack8<__half>(v);
@@ -378,12 +359,6 @@ __device__ __forceinline__ void gemm_finish_half(const GemmParams& p, float (&v)
   else if (p.activation == kActSilu) activate_all<kActSilu>(v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(wide_at(out, lane, half * 4 + i)) = pack8_as(v + i * 8, p.type);
-}
-
-__device__ __forceinline__ float power2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
 }
 
 // 32 logits of a row from column `col` on, of which `count` are of the vocabulary, taken up into the row's largest logit and the sum of
@@ -996,15 +971,13 @@ namespace {
 // boxes of 64 x `box_rows` of a batch of row-major matrices of 16-bit values; outside of a matrix zeros are read
 bool make_matrix_map(CUtensorMap* map, int type, const void* base, int64_t inner, int64_t rows, int64_t batch, int64_t ld, int64_t stride,
                      int box_rows) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return false;
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)batch};
   cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(batch > 1 ? stride : ld) * 2};
   cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
   cuuint32_t step[3] = {1, 1, 1};
-  return fn(map, type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                      step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // Shared memory descriptor without its address: 128-byte swizzle; eight rows of 128 bytes are 1024 bytes, and 64 values
@@ -1020,16 +993,15 @@ uint64_t descriptor(bool k_major) {
 bool make_side_map(CUtensorMap* map, const GemmSide& s, int type, const GemmCall& c, bool stored, bool mirror = false, bool wide = false) {
   const size_t bytes = element_bytes(type);
   if (stored && c.n * bytes % 16 && s.ld != (c.n + 7) / 8 * 8) return false;
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn || !s.data || (reinterpret_cast<uintptr_t>(s.data) & 15u) || s.ld * bytes % 16 || (c.batch > 1 && s.stride * bytes % 16)) return false;
+  if (!s.data || (reinterpret_cast<uintptr_t>(s.data) & 15u) || s.ld * bytes % 16 || (c.batch > 1 && s.stride * bytes % 16)) return false;
   cuuint64_t dims[3] = {(cuuint64_t)c.n, (cuuint64_t)c.m, (cuuint64_t)c.batch};
   cuuint64_t strides[2] = {(cuuint64_t)(s.ld * bytes), (cuuint64_t)((c.batch > 1 ? s.stride : s.ld) * bytes)};
   cuuint32_t box[3] = {wide ? 64u : 32u, 32, 1};
   cuuint32_t step[3] = {1, 1, 1};
-  return fn(map, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+  return encode_tiled(map, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
             s.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
             mirror ? CU_TENSOR_MAP_SWIZZLE_NONE : type == kF32 || wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // tiles of one matrix
@@ -1281,6 +1253,7 @@ cudaError_t launch_chain(const GemmChain& c, cudaStream_t stream) {
 
 extern "C" int hc_train_status(int clear) {
   if (cudaDeviceSynchronize() != cudaSuccess) return hc::kErrCuda;
-  const int all[3] = {hc::take_status(hc::dev::g_train_status, clear), hc::norm_status(clear), hc::logprob_status(clear)};
-  return all[0] ? all[0] : all[1] ? all[1] : all[2];
+  int worst = 0;
+  for (int status : {hc::take_status(hc::dev::g_train_status, clear), hc::norm_status(clear), hc::logprob_status(clear), hc::attention_status(clear)}) worst = worst ? worst : status;
+  return worst;
 }

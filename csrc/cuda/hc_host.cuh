@@ -24,18 +24,31 @@ inline EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
+// A tensor map.  The call needs the device's context to be current, which it is not in a thread that has called nothing of the runtime yet that needs one
+// (torch's autograd thread, with its memory from the cache): made current then, and tried again.
+template <typename... Args>
+bool encode_tiled(Args... args) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  CUresult r = fn(args...);
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+    r = fn(args...);
+  }
+  return r == CUDA_SUCCESS;
+}
+
 // 2-D view {32, rows} of a 4-byte-element array, box {32, box_rows}, 128-byte swizzle
 inline bool make_rows_map(CUtensorMap* map, const void* base, uint64_t rows, int box_rows) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn || rows == 0 || (reinterpret_cast<uintptr_t>(base) & 15u)) return false;
+  if (rows == 0 || (reinterpret_cast<uintptr_t>(base) & 15u)) return false;
   cuuint64_t dims[2] = {(cuuint64_t)kBlock, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)kBlock * 4};
   cuuint32_t box[2] = {(cuuint32_t)kBlock, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 struct DeviceInfo {

@@ -15,6 +15,7 @@ inline bool lies_at(const void* p, size_t bytes) { return reinterpret_cast<uintp
 // The status of the kernels of a source: 0, or 3 after a wait that ran out, kept until it is cleared.
 int norm_status(int clear);
 int logprob_status(int clear);
+int attention_status(int clear);
 template <typename S>
 int take_status(S& symbol, int clear) {
   unsigned int status = 0;

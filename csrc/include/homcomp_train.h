@@ -86,6 +86,28 @@ size_t hc_orthogonalize_bytes(size_t batch, size_t height, size_t width);
 int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_t width, size_t stride, size_t batch_stride, void* out,
                      int steps, float a, float b, float c, float eps, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 
+// ---- attention ---------------------------------------------------------------------------------------------------------------
+// Causal attention of `queries` positions, the last ones of `keys`: query i stands at p = i + keys - queries and sees key j if j <= p and (p - j < window or j < sinks)
+// (window 0: all up to p).  Softmax of scale q k^T over what is seen, times v; a query that sees nothing (p < 0) gives 0.  q (batch, heads, queries, head_size), k and v (batch, kv_heads, keys,
+// head_size), where heads / kv_heads query heads share a key's head; both of `type` (1 or 2).  head_size: a multiple of 8 up to 128; lengths below 2^24, batch times heads
+// below 2^24, scale above 0.
+// A tensor's values are adjacent, 16-byte aligned; its strides, multiples of 8 elements and at least head_size, are its own.
+// out and the gradients: (batch, position, head, head_size) without gaps, 16-byte aligned.
+// stats: hc_attention_stats floats for the backward pass, 16-byte aligned, or NULL.  Scratch memory, 256-byte aligned, of hc_attention_bytes (0: none).
+// A key or value that is not finite may show in any query of its sequence and head, also in one that does not see it.
+typedef struct hc_heads {
+  const void* data;
+  size_t batch, head, position;  // elements from one to the next
+} hc_heads;
+size_t hc_attention_stats(size_t batch, size_t heads, size_t queries);
+size_t hc_attention_bytes(size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size, size_t window, size_t sinks);
+int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float* stats, size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size,
+                 size_t window, size_t sinks, float scale, void* scratch, size_t scratch_bytes, hc_stream_t stream);
+// dq, and dk and dv (both or neither): of `type`, from `out` and `stats` of the forward pass.  Probabilities and their gradients are rounded to `type` for the products.
+size_t hc_attention_backward_bytes(size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size);
+int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k, hc_heads v, int type, const float* stats, void* dq, void* dk, void* dv, size_t batch, size_t heads,
+                          size_t kv_heads, size_t queries, size_t keys, size_t head_size, size_t window, size_t sinks, float scale, void* scratch, size_t scratch_bytes, hc_stream_t stream);
+
 // ---- cross entropy from hidden rows ------------------------------------------------------------------------------------
 // loss_i = log sum_v exp(x_i . w_v) - x_i . w_token, without the logits ever being stored: x [rows][inner], weight [vocab][inner], both of `type` (1 or 2), as operands
 // of a product lie (16-byte aligned, strides multiples of 8), sides below 2^26; sums in the tensor core over up to 1024 terms.

@@ -16,6 +16,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 #include <tuple>
 #include <unordered_map>
@@ -44,6 +45,11 @@ struct Api {
   decltype(&hc_linear_backward) linear_backward;
   decltype(&hc_orthogonalize_bytes) orthogonalize_bytes;
   decltype(&hc_orthogonalize) orthogonalize;
+  decltype(&hc_attention_stats) attention_stats;
+  decltype(&hc_attention_bytes) attention_bytes;
+  decltype(&hc_attention) attention;
+  decltype(&hc_attention_backward_bytes) attention_backward_bytes;
+  decltype(&hc_attention_backward) attention_backward;
   decltype(&hc_linear_cross_entropy_bytes) linear_cross_entropy_bytes;
   decltype(&hc_linear_cross_entropy) linear_cross_entropy;
   decltype(&hc_linear_cross_entropy_backward_bytes) linear_cross_entropy_backward_bytes;
@@ -66,6 +72,11 @@ void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
   HC_BIND(linear_backward);
   HC_BIND(orthogonalize_bytes);
   HC_BIND(orthogonalize);
+  HC_BIND(attention_stats);
+  HC_BIND(attention_bytes);
+  HC_BIND(attention);
+  HC_BIND(attention_backward_bytes);
+  HC_BIND(attention_backward);
   HC_BIND(linear_cross_entropy_bytes);
   HC_BIND(linear_cross_entropy);
   HC_BIND(linear_cross_entropy_backward_bytes);
@@ -476,6 +487,92 @@ Tensor orthogonalize(const Tensor& update_, int64_t steps, double a, double b, d
   return out;
 }
 
+// ---- attention ----------------------------------------------------------------------------------------------------------
+// as the kernels read it: adjacent values at 16-byte boundaries, no two of its rows in one place
+Tensor heads_of(const Tensor& t) {
+  bool ok = aligned(t) && (t.stride(3) == 1 || t.size(3) == 1);
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) >= t.size(3) && t.stride(i) % 8 == 0 && t.stride(i) < (int64_t(1) << 38)));
+  return ok ? t : packed(t);
+}
+hc_heads heads_at(const Tensor& t) { return {t.data_ptr(), (size_t)t.stride(0), (size_t)t.stride(1), (size_t)t.stride(2)}; }
+// (batch, heads, positions, values), lying as (batch, positions, heads, values)
+Tensor empty_heads(const Tensor& like, const Tensor& options) {
+  return at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, options.options()).transpose(1, 2);
+}
+Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, Tensor* stats) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t b = q.size(0), h = q.size(1), kv = k.size(1), m = q.size(2), n = k.size(2), d = q.size(3);
+  Tensor out = empty_heads(q, q);
+  if (stats) *stats = at::empty({(int64_t)api.attention_stats(b, h, m)}, q.options().dtype(at::kFloat));
+  const size_t need = api.attention_bytes(b, h, kv, m, n, d, window, sinks);
+  const Tensor scratch = scratch_of(need, q);
+  check(api.attention(heads_at(q), heads_at(k), heads_at(v), type_of(q), out.data_ptr(), stats ? static_cast<float*>(stats->data_ptr()) : nullptr, b, h, kv, m, n, d, window, sinks, (float)scale,
+                      ptr(scratch), need, stream_of(q)),
+        "attention");
+  return out;
+}
+
+struct Attention : Function<Attention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks, double scale) {
+    const Tensor q = heads_of(q_), k = heads_of(k_), v = heads_of(v_);
+    Tensor stats;
+    Tensor out = attention_forward(q, k, v, window, sinks, scale, &stats);
+    ctx->save_for_backward({q, k, v, out, stats});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &stats = saved[4];
+    not_recorded();
+    ordinary("gradient", grads[0]);
+    const c10::cuda::CUDAGuard guard(q.device());
+    const bool graph = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
+    const int64_t b = q.size(0), h = q.size(1), kv = k.size(1), m = q.size(2), n = k.size(2), d = q.size(3);
+    const Tensor dout = heads_of(held(grads[0]));
+    const bool want_k = ctx->needs_input_grad(1), want_v = ctx->needs_input_grad(2), both = want_k || want_v;
+    const Tensor dq = ctx->needs_input_grad(0) ? empty_heads(q, q) : Tensor(), dk = both ? empty_heads(k, k) : Tensor(), dv = both ? empty_heads(v, v) : Tensor();
+    const size_t need = api.attention_backward_bytes(b, h, kv, m, n, d);
+    const Tensor scratch = scratch_of(need, q);
+    check(api.attention_backward(heads_at(dout), out.data_ptr(), heads_at(q), heads_at(k), heads_at(v), type_of(q), static_cast<float*>(stats.data_ptr()), ptr(dq), ptr(dk), ptr(dv), b, h, kv, m, n, d,
+                                 ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(), (float)ctx->saved_data["scale"].toDouble(), ptr(scratch), need, stream_of(q)),
+          "attention backward");
+    return once({dq, want_k ? dk : Tensor(), want_v ? dv : Tensor(), Tensor(), Tensor(), Tensor()}, graph);
+  }
+};
+
+Tensor attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks, std::optional<double> given) {
+  not_recorded();
+  ordinary("q", q_);
+  ordinary("k", k_);
+  ordinary("v", v_);
+  const Tensor q = held(q_), k = held(k_), v = held(v_);
+  floating("q", q);
+  floating("k", k);
+  floating("v", v);
+  beside("k", k, q);
+  beside("v", v, q);
+  TORCH_CHECK_VALUE(type_of(q) != 0 && type_of(k) == type_of(q) && type_of(v) == type_of(q), "attention: q, k and v are all bfloat16 or all float16, got ", q.scalar_type(), ", ", k.scalar_type(), " and ",
+                    v.scalar_type());
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && k.sizes().equals(v.sizes()) && q.size(0) == k.size(0) && q.size(3) == k.size(3), "attention: no attention of q ", q.sizes(), " to k ", k.sizes(), " and v ",
+                    v.sizes());
+  const int64_t d = q.size(3), h = q.size(1), kv = k.size(1);
+  TORCH_CHECK_VALUE(d >= 8 && d <= 128 && d % 8 == 0, "attention: the head size is a multiple of 8 up to 128, got ", d);
+  TORCH_CHECK_VALUE(kv > 0 && h > 0 && h % kv == 0, "attention: ", h, " query heads do not share ", kv, " key heads");
+  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0, "attention: window and sinks are not negative");
+  const double scale = given ? *given : 1.0 / std::sqrt((double)d);
+  TORCH_CHECK_VALUE(scale > 0 && (float)scale > 0 && std::isfinite((float)scale), "attention: scale is above 0");
+  constexpr int64_t most = int64_t(1) << 24;
+  TORCH_CHECK_VALUE(q.size(2) < most && k.size(2) < most && q.size(0) < most && h < (1 << 15) && q.size(0) * h < most &&
+                        q.size(0) * h * ((q.size(2) + 127) / 128 + (k.size(2) + 127) / 128) < (int64_t(1) << 30),
+                    "attention: too many positions or heads: q ", q.sizes(), ", k ", k.sizes());
+  if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v))) return Attention::apply(q, k, v, window, sinks, scale);
+  return attention_forward(heads_of(q), heads_of(k), heads_of(v), window, sinks, scale, nullptr);
+}
+
 // ---- cross entropy from hidden rows ---------------------------------------------------------------------------------------
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
 // x and weight as the products read them
@@ -693,6 +790,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear);
   m.def("token_logprobs", &token_logprobs);
   m.def("orthogonalize", &orthogonalize);
+  m.def("attention", &attention);
   m.def("linear_cross_entropy", &linear_cross_entropy);
   m.def("adamw_step", &adamw_step);
   m.def("adamw_values", &adamw_values);

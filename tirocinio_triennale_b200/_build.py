@@ -24,7 +24,7 @@ CPU_SOURCES = ["cpu/hc_cpu_codec.cpp", "cpu/hc_cpu_ring.cpp"]
 CUDA_SOURCES = ["cuda/hc_kernels.cu", "cuda/hc_encode.cu", "cuda/hc_decode.cu", "cuda/hc_api.cu", "cuda/hc_ring.cu", "cuda/hc_compat.cu", "cuda/hc_noalloc.cu",
                 "cuda/hc_host_staged.cu", "cuda/hc_multicast.cu", "cuda/hc_norm.cu", "cuda/hc_logprobs.cu",
                 "cuda/hc_gemm.cu", "cuda/hc_linear.cu", "cuda/hc_orthogonalize.cu",
-                "cuda/hc_adamw.cu", "cuda/hc_loss.cu"]
+                "cuda/hc_adamw.cu", "cuda/hc_loss.cu", "cuda/hc_attention.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-ffp-contract=off", "--fmad=false",

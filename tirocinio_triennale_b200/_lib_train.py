@@ -6,6 +6,12 @@ import ctypes as C
 vp = C.c_void_p
 
 
+class Heads(C.Structure):
+    """hc_heads: a tensor of (batch, head, position, value) with its strides."""
+
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_size_t), ("head", C.c_size_t), ("position", C.c_size_t)]
+
+
 def declare(lib):
     sz, f, d, i, l = C.c_size_t, C.c_float, C.c_double, C.c_int, C.c_int64
     sizes = {
@@ -13,6 +19,9 @@ def declare(lib):
         "hc_linear_bytes": [sz, sz, sz],
         "hc_linear_backward_bytes": [sz, sz, sz, i],
         "hc_orthogonalize_bytes": [sz, sz, sz],
+        "hc_attention_stats": [sz, sz, sz],
+        "hc_attention_bytes": [sz] * 8,
+        "hc_attention_backward_bytes": [sz] * 6,
         "hc_linear_cross_entropy_bytes": [sz, sz, sz],
         "hc_linear_cross_entropy_backward_bytes": [sz, sz, sz],
     }
@@ -23,6 +32,8 @@ def declare(lib):
         "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp, sz, vp],
         "hc_linear_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, sz, i, vp, sz, vp, sz, vp, i, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],
+        "hc_attention": [Heads, Heads, Heads, i, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, f, vp, sz, vp],
+        "hc_attention_backward": [Heads, vp, Heads, Heads, Heads, i, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, f, vp, sz, vp],
         "hc_linear_cross_entropy": [vp, sz, vp, sz, i, vp, l, i, vp, vp, sz, sz, sz, vp, sz, vp],
         "hc_linear_cross_entropy_backward": [vp, sz, vp, sz, i, vp, l, i, vp, vp, vp, sz, vp, sz, sz, sz, sz, vp, sz, vp],
         "hc_adamw": [vp, sz, i, i, i, d, vp, d, d, d, d, l, vp, C.c_uint64, vp],

@@ -28,6 +28,9 @@ class GPT2Config:
     seq_len: int = 1024
     dropout: float = 0.0
     fused: bool = False  # this library's operators in place of torch's (CUDA, float32 weights, bfloat16 products)
+    attention: str = "torch"  # fused: torch's attention, or "own", this library's (``ops.attention``)
+    window: int | None = None  # positions that a token sees, itself the last of them (None: all before it)
+    sinks: int = 0  # with a window: first tokens that stay visible
     logits: bool = True  # fused: the loss from the logits, or from the last hidden rows without them (``ops.linear_cross_entropy``)
 
     @staticmethod
@@ -58,6 +61,19 @@ class Block(nn.Module):
         self.out = nn.Linear(4 * cfg.d_model, cfg.d_model)
         self.n_head = cfg.n_head
         self.fused = cfg.fused
+        if cfg.attention not in ("torch", "own") or cfg.attention == "own" and not cfg.fused:
+            raise ValueError("GPT2: attention is \"torch\", or with fused \"own\"")
+        self.own_attention = cfg.attention == "own"
+        self.window, self.sinks = cfg.window, cfg.sinks
+
+    def attend(self, q, k, v):
+        if self.own_attention:
+            return ops.attention(q, k, v, window=self.window, sinks=self.sinks)
+        if self.window is None:
+            return F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        p = torch.arange(q.shape[2], device=q.device)
+        back = p[:, None] - p[None, :]
+        return F.scaled_dot_product_attention(q, k, v, attn_mask=(back >= 0) & ((back < self.window) | (p[None, :] < self.sinks)))
 
     def forward(self, x):
         B, T, C = x.shape
@@ -65,7 +81,7 @@ class Block(nn.Module):
         q = q.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
         k = k.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
         v = v.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
-        a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        a = self.attend(q, k, v)
         if self.fused:
             x = _linear(a.transpose(1, 2).reshape(B, T, C), self.proj, residual=x)
             return _linear(_linear(_norm(x, self.ln2), self.fc, activation="gelu_tanh"), self.out, residual=x)

@@ -47,6 +47,7 @@ def run(args, compressed: bool, rank: int, world: int, device):
     cfg = GPT2Config.small() if args.model == "small" else GPT2Config.tiny()
     cfg.seq_len = args.seq
     cfg.fused = getattr(args, "fused", False)
+    cfg.attention, cfg.window, cfg.sinks = getattr(args, "attention", "torch"), getattr(args, "window", None), getattr(args, "sinks", 0)
     cfg.logits = not getattr(args, "no_logits", False)
     model = GPT2(cfg).to(device)
     ddp = DDP(model, device_ids=[device.index] if device.type == "cuda" else None, bucket_cap_mb=args.bucket_mb,
@@ -124,6 +125,9 @@ def main(argv=None):
     ap.add_argument("--eb", type=float, default=1e-5)
     ap.add_argument("--lr", type=float, default=3e-4)
     ap.add_argument("--fused", action="store_true", help="this library's operators in the model")
+    ap.add_argument("--attention", default="torch", choices=["torch", "own"], help="with --fused: torch's attention or this library's")
+    ap.add_argument("--window", type=int, default=None, help="positions that a token sees (all before it)")
+    ap.add_argument("--sinks", type=int, default=0, help="with --window: first tokens that stay visible")
     ap.add_argument("--no-logits", action="store_true", help="with --fused: the loss from the last hidden rows, a piece of the vocabulary at a time")
     ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"])
     ap.add_argument("--adam-bits", type=int, default=None, choices=[8, 32], help="this library's AdamW with moments of so many bits, in place of torch's")
@@ -137,8 +141,8 @@ def main(argv=None):
     args = ap.parse_args(argv)
     if args.cpu and (args.fused or args.optimizer == "muon" or args.adam_bits is not None):
         ap.error("--fused, --optimizer muon and --adam-bits need a GPU")
-    if args.no_logits and not args.fused:
-        ap.error("--no-logits needs --fused")
+    if not args.fused and (args.no_logits or args.attention == "own"):
+        ap.error("--no-logits and --attention own need --fused")
 
     rank = int(os.environ.get("RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))

@@ -9,6 +9,7 @@ from .norm import layer_norm  # noqa: F401
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from .linear import linear  # noqa: F401
 from .orthogonalize import orthogonalize  # noqa: F401
+from .attention import attention  # noqa: F401
 from .loss import linear_cross_entropy  # noqa: F401
 from .adamw import adamw_step, adamw_values  # noqa: F401
 from ._train import train_status  # noqa: F401
