@@ -31,9 +31,8 @@
 namespace hc {
 namespace dev {
 
-constexpr int kTile = 128;  // queries, keys
-constexpr int kAttnWarps = 8;  // with a row a thread
-constexpr int kAttnThreads = 64 + 32 * kAttnWarps;
+constexpr int kTile = 128;  // rows of a tile, one a thread
+constexpr int kStep = 64;   // columns that are worked on at a time
 constexpr uint64_t kAttnLimitNs = 2000ull * 1000 * 1000;
 constexpr float kSlack = 8.0f;  // powers of two that a score may be above its row's reference
 
@@ -43,21 +42,28 @@ template <int kD>
 struct AttnShape {
   static constexpr int kBoxes = kD / 64;          // of 64 values, 128 bytes
   static constexpr int kBytes = kTile * kD * 2;   // of a tile
-  static constexpr int kForwardStages = kD == 128 ? 4 : 8;  // tiles of keys or values
-  static constexpr int kForwardSmem = (2 + kForwardStages) * kBytes + 1024;
-  static constexpr int kQStages = kD == 128 ? 2 : 4, kDoStages = kD == 128 ? 2 : 4;
-  static constexpr int kKvSmem = (2 + kQStages + kDoStages) * kBytes + kQStages * 1024 + 1024;
-  static constexpr int kKStages = kD == 128 ? 3 : 5, kVStages = kD == 128 ? 2 : 4;
-  static constexpr int kQSmem = (2 + kKStages + kVStages) * kBytes + 1024;
+  static constexpr int kStepBytes = kStep * kD * 2;
+  // Heads of up to 64 values: two CTAs an SM, with half of the tensor memory each.
+  static constexpr int kResident = kD == 128 ? 1 : 2;
+  static constexpr int kColumns = 512 / kResident;
+  static constexpr int kSlots = kD == 128 ? 2 : 1;  // forward: steps of scores of a tile
+  static constexpr int kForwardStages = kD == 128 ? 10 : 8;  // steps of keys or of values
+  static constexpr int kForwardSmem = 2 * kBytes + kForwardStages * kStepBytes + 1024;
+  static constexpr int kForwardThreads = 32 * (4 + 8);
+  static constexpr int kGroups = kD == 128 ? 2 : 1;  // backward: of eight warps, which take the steps in turn
+  static constexpr int kStages = 4;                  // backward: a step of both streams, and what belongs to its queries
+  static constexpr int kBackwardSmem = 2 * kBytes + kStages * (2 * kStepBytes + 512) + 1024;
+  static constexpr int kBackwardThreads = 32 * (4 + 8 * kGroups);
 };
 
 struct AttnParams {
-  CUtensorMap q, k, v, dout;
+  CUtensorMap q, k, v, dout;                          // in steps of 64 positions (forward, q: tiles)
+  CUtensorMap q_tile, k_tile, v_tile, dout_tile;  // in tiles of 128 (backward)
   void* o;
   float* less;      // [batch heads][rows]: minus the logarithm (base 2) of a query's sum of exponentials, for the backward pass
   float* part_o;    // [split][query of all][head size], of the CTAs that share the keys out
   float* part_less;
-  const float* delta;  // as `less`
+  float* delta;  // as `less`
   void *dq, *dk, *dv;
   const unsigned int* most;  // bits of max|dO_i|, max|V_j| (fp16)
   int64_t less_ld;
@@ -69,8 +75,8 @@ struct AttnParams {
 };
 
 struct AttnBarriers {
-  uint64_t full[8], empty[8], more_full[4], more_empty[4];
-  uint64_t first, s_full[2], p_ready[2], done[2], s_read, dp_full[2], ds_ready[2], drained;
+  uint64_t full[16], empty[16], first, drained, met;
+  uint64_t s_full[4], p_ready[4], done[4], dp_full[2], ds_ready[2], ds_done[2];
   uint32_t tmem, gave_up;
 };
 
@@ -124,40 +130,53 @@ __device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, int x
 __device__ __forceinline__ void load_floats(void* dst, const float* src, int bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-// a tile: 128 rows from t on
-template <int kD>
-__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int t, int h, int b, uint64_t* bar) {
+// kRows rows from t on
+template <int kD, int kRows>
+__device__ __forceinline__ void load_rows(unsigned char* dst, const CUtensorMap* map, int t, int h, int b, uint64_t* bar) {
 #pragma unroll
-  for (int i = 0; i < AttnShape<kD>::kBoxes; ++i) load_4d(dst + i * kTile * 128, map, i * 64, t, h, b, bar);
+  for (int i = 0; i < AttnShape<kD>::kBoxes; ++i) load_4d(dst + i * kRows * 128, map, i * 64, t, h, b, bar);
 }
 
-__device__ __forceinline__ void attn_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void attn_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// The matrix instructions' warp runs as a whole, so that the compiler keeps descriptors and addresses in uniform registers, which these instructions take them from, and one
+// lane of it issues.  With one lane in all of its code an instruction cost 130 to 290 cycles, several times what the tensor cores take for it.
+__device__ __forceinline__ bool elected() {
+  uint32_t is;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
+}
+__device__ __forceinline__ void attn_commit(uint64_t* bar) {
+  if (elected()) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void attn_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  if (elected())
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
 // the first operand in tensor memory: rows in lanes, two values of the sum in a column
 __device__ __forceinline__ void attn_mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+  if (elected())
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
-// Descriptors of a tile, 128-byte swizzle.  Along: the sum runs along its rows of 128 bytes (eight rows are 1024 bytes).  Across: the sum runs
+// Descriptors of a tile or a step, 128-byte swizzle.  Along: the sum runs along its rows of 128 bytes (eight rows are 1024 bytes).  Across: the sum runs
 // over its rows, 64 values across it are a box.
 __device__ __forceinline__ uint64_t along(const unsigned char* tile) {
   return (uint64_t)((smem_u32(tile) & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 / 16) << 32 | 1ull << 46 | 2ull << 61;
 }
-__device__ __forceinline__ uint64_t across(const unsigned char* tile) {
-  return (uint64_t)((smem_u32(tile) & 0x3ffff) >> 4) | (uint64_t)(kTile * 128 / 16) << 16 | (uint64_t)(1024 / 16) << 32 | 1ull << 46 | 2ull << 61;
+__device__ __forceinline__ uint64_t across(const unsigned char* step) {
+  return (uint64_t)((smem_u32(step) & 0x3ffff) >> 4) | (uint64_t)(kStep * 128 / 16) << 16 | (uint64_t)(1024 / 16) << 32 | 1ull << 46 | 2ull << 61;
 }
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t operand_format() {
@@ -167,83 +186,87 @@ template <typename T>
 __device__ __forceinline__ uint32_t attn_idesc(int n, bool b_across) {
   return 1u << 4 | operand_format<T>() << 7 | operand_format<T>() << 10 | (b_across ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(kTile / 16) << 24;
 }
-// d = a b^T over the head's values: both tiles along the sum
+// d = a b^T over the head's values, of a tile and a step
 template <typename T, int kD>
 __device__ __forceinline__ void scores(uint32_t d, const unsigned char* a, const unsigned char* b) {
   const uint64_t da = along(a), db = along(b);
-  const uint32_t idesc = attn_idesc<T>(kTile, false);
+  const uint32_t idesc = attn_idesc<T>(kStep, false);
 #pragma unroll
-  for (int i = 0; i < kD / 16; ++i) {
-    const uint32_t at = (i / 4) * (kTile * 128 / 16) + (i % 4) * 2;
-    attn_mma(d, da + at, db + at, idesc, i > 0);
-  }
+  for (int i = 0; i < kD / 16; ++i) attn_mma(d, da + (i / 4) * (kTile * 128 / 16) + (i % 4) * 2, db + (i / 4) * (kStep * 128 / 16) + (i % 4) * 2, idesc, i > 0);
 }
-// d (+)= p b, p in tensor memory; its second 64 columns of the sum begin `second` columns behind the first
+// d (+)= p b, p in tensor memory, its second 32 values of the sum `second` columns behind the first, b a step
 template <typename T, int kD>
 __device__ __forceinline__ void weighted(uint32_t d, uint32_t p, int second, const unsigned char* b, bool add) {
   const uint64_t db = across(b);
   const uint32_t idesc = attn_idesc<T>(kD, true);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) attn_mma_from_tmem(d, p + (i / 4) * second + (i % 4) * 8, db + i * 128, idesc, add || i > 0);
+  for (int i = 0; i < kStep / 16; ++i) attn_mma_from_tmem(d, p + i / 2 * second + i % 2 * 8, db + i * 128, idesc, add || i > 0);
 }
 
 // ---- what is seen ------------------------------------------------------------------------------------------------------------
-// the tiles of keys that positions p0 to p1 see: those of the first tokens, then a stretch
-struct KeyTiles {
+// the steps of keys that positions p0 to p1 see: those of the first tokens, then a stretch
+struct KeySteps {
   int sinks, low, count;
-  __device__ __forceinline__ int at(int e) const { return e < sinks ? e : low + e - sinks; }
+  __device__ __forceinline__ int at(int e) const { return (e < sinks ? e : low + e - sinks) * kStep; }
 };
-__device__ __forceinline__ KeyTiles key_tiles(const AttnParams& p, int p0, int p1) {
-  KeyTiles t = {0, 0, 0};
+__device__ __forceinline__ KeySteps key_steps(const AttnParams& p, int p0, int p1) {
+  KeySteps t = {0, 0, 0};
   if (p1 < 0) return t;
   const int lowest = p0 - p.window + 1;
-  t.low = lowest > 0 ? lowest / kTile : 0;
-  t.sinks = min((min(p.sinks, p1 + 1) + kTile - 1) / kTile, t.low);
-  t.count = t.sinks + p1 / kTile - t.low + 1;
+  t.low = lowest > 0 ? lowest / kStep : 0;
+  t.sinks = min((min(p.sinks, p1 + 1) + kStep - 1) / kStep, t.low);
+  t.count = t.sinks + p1 / kStep - t.low + 1;
   return t;
 }
-__device__ __forceinline__ bool any_seen(const AttnParams& p, int p0, int p1, int k0) { return k0 <= p1 && (k0 + kTile - 1 > p0 - p.window || k0 < p.sinks); }
-__device__ __forceinline__ bool all_seen(const AttnParams& p, int p0, int p1, int k0) { return k0 + kTile - 1 <= p0 && (p1 - k0 < p.window || k0 + kTile <= p.sinks); }
+// of a step of keys from k0 on
+__device__ __forceinline__ bool any_seen(const AttnParams& p, int p0, int p1, int k0) { return k0 <= p1 && (k0 + kStep - 1 > p0 - p.window || k0 < p.sinks); }
+// of `keys` keys from k0 on
+__device__ __forceinline__ bool all_seen(const AttnParams& p, int p0, int p1, int k0, int keys) { return k0 + keys - 1 <= p0 && (p1 - k0 < p.window || k0 + keys <= p.sinks); }
 
-// barriers and tensor memory; by all threads
-__device__ __forceinline__ void attn_begin(AttnBarriers& sh, int ready_warps) {
+// of the 32 columns from `at` on those from `low` up to below `high`, and those below `sinks`, as bits
+__device__ __forceinline__ uint32_t ones_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen_bits(int low, int high, int sinks, int at) { return ones_below(high - at) & (~ones_below(low - at) | ones_below(sinks - at)); }
+
+// barriers and tensor memory; by all threads.  `rows`: warps that work on a step, `released`: roles that have to be done with a stage.
+template <int kColumns>
+__device__ __forceinline__ void attn_begin(AttnBarriers& sh, int warps, int rows, int released) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 1);
-    }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&sh.more_full[i], 1);
-      mbar_init(&sh.more_empty[i], 1);
+      mbar_init(&sh.empty[i], released);
     }
     mbar_init(&sh.first, 1);
-    mbar_init(&sh.s_read, kAttnWarps);
-    mbar_init(&sh.drained, 1);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(&sh.drained, 2);
+    mbar_init(&sh.met, warps);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_ready[i], ready_warps);
+      mbar_init(&sh.p_ready[i], rows);
       mbar_init(&sh.done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.dp_full[i], 1);
-      mbar_init(&sh.ds_ready[i], kAttnWarps);
+      mbar_init(&sh.ds_ready[i], rows);
+      mbar_init(&sh.ds_done[i], 1);
     }
     sh.gave_up = 0;
     fence_mbar_init();
   }
   if (threadIdx.x >> 5 == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
 }
+template <int kColumns>
 __device__ __forceinline__ void attn_end(uint32_t tmem) {
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x >> 5 == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns));
   }
 }
 __device__ __forceinline__ unsigned char* attn_tiles(unsigned char* raw) {
@@ -256,11 +279,11 @@ __device__ __forceinline__ void warp_arrives(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// A row's values, `factor` times what tensor memory has, from `to` on.  `there`, the same for all of a warp: tensor memory has them; `none`: zeros.
-template <typename O, int kD>
+// kCount of a row's values, `factor` times what tensor memory has, from `to` on; `d`: how many the row has from there.  `there`, the same for all of a warp: tensor memory has them; `none`: zeros.
+template <typename O, int kCount>
 __device__ __forceinline__ void store_row(uint32_t from, O* to, int d, float factor, bool in, bool there, bool none) {
 #pragma unroll
-  for (int c = 0; c < kD; c += 32) {
+  for (int c = 0; c < kCount; c += 32) {
     float v[32];
     if (there) {
       __syncwarp();
@@ -280,17 +303,25 @@ __device__ __forceinline__ void store_row(uint32_t from, O* to, int d, float fac
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// Tensor memory: scores of the two tiles of queries at 0 and 128 (the probabilities in their first 64 columns), O at 256 and 384.
+// the largest of three, which is one instruction
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two tiles of queries, with four warps and a warp that issues their matrix instructions each.  Tensor memory: one or two steps of scores of each tile (the probabilities in their first 32
+// columns), then O of both.  With two steps the next one's scores are formed while a step is worked on; heads of up to 64 values have one, and two CTAs on an SM.
 template <typename T, int kD>
-__global__ void __launch_bounds__(kAttnThreads, 1) hc_attention_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>::kResident) hc_attention_kernel(const __grid_constant__ AttnParams p) {
   using S = AttnShape<kD>;
-  constexpr int kStages = S::kForwardStages;
+  constexpr int kStages = S::kForwardStages, kSlots = S::kSlots, kO = 2 * kSlots * kStep;
   constexpr float kBias = operand_format<T>() ? 0.0f : 6.0f;  // probabilities are held times 2^6 in fp16: at most 2^14
   extern __shared__ unsigned char raw[];
   __shared__ AttnBarriers sh;
   unsigned char* tiles = attn_tiles(raw);
   unsigned char* ring = tiles + 2 * S::kBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // the blocks of queries that see most come first
   const int heads = p.packed ? p.kv_heads : p.heads;
   int64_t at = blockIdx.x;
@@ -309,97 +340,76 @@ __global__ void __launch_bounds__(kAttnThreads, 1) hc_attention_kernel(const __g
     p0[q] = p.off + i0;
     p1[q] = there ? p.off + (p.packed ? p.tq - 1 : i1) : -1;
   }
-  const KeyTiles list = key_tiles(p, p0[0], max(p1[0], p1[1]));
+  const KeySteps list = key_steps(p, p0[0], max(p1[0], p1[1]));
   const int e0 = (int)((int64_t)list.count * split / p.splits), e1 = (int)((int64_t)list.count * (split + 1) / p.splits);
-  attn_begin(sh, kAttnWarps / 2);
-  const uint32_t tmem = sh.tmem;
+  attn_begin<S::kColumns>(sh, 8, 4, 2);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   if (warp == 0) {
-    if (lane == 0) {
-      Ring<kStages> r;
-      bool ok = true;
-      const bool second = !p.packed && first + kTile < p.tq;
-      if (e0 < e1) {
-        if (p.packed) {
-          mbar_expect_tx(&sh.first, p.packed * 128 * S::kBoxes);
-          for (int i = 0; i < S::kBoxes; ++i) load_4d(tiles + i * kTile * 128, &p.q, i * 64, 0, head * p.group, b, &sh.first);
-        } else {
-          mbar_expect_tx(&sh.first, second ? 2 * S::kBytes : S::kBytes);
-          load_tile<kD>(tiles, &p.q, first, head, b, &sh.first);
-          if (second) load_tile<kD>(tiles + S::kBytes, &p.q, first + kTile, head, b, &sh.first);
-        }
-      }
-      for (int e = e0; ok && e < e1; ++e) {
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!attn_wait(&sh.empty[r.s], r.phase ^ 1, sh)) {
-            ok = false;
-            break;
-          }
-          mbar_expect_tx(&sh.full[r.s], S::kBytes);
-          load_tile<kD>(ring + r.s * S::kBytes, kv ? &p.v : &p.k, list.at(e) * kTile, kv_head, b, &sh.full[r.s]);
-          r.next();
-        }
-      }
-      ring_end(sh.full, r);
-      if (e0 < e1) mbar_wait_bounded(&sh.first, 0, kAttnLimitNs);
-    }
-  } else if (warp == 1) {
     if (lane == 0 && e0 < e1) {
+      Ring<kStages> r;
+      const bool second = !p.packed && first + kTile < p.tq;
+      if (p.packed) {
+        mbar_expect_tx(&sh.first, p.packed * 128 * S::kBoxes);
+        for (int i = 0; i < S::kBoxes; ++i) load_4d(tiles + i * kTile * 128, &p.q, i * 64, 0, head * p.group, b, &sh.first);
+      } else {
+        mbar_expect_tx(&sh.first, second ? 2 * S::kBytes : S::kBytes);
+        load_rows<kD, kTile>(tiles, &p.q, first, head, b, &sh.first);
+        if (second) load_rows<kD, kTile>(tiles + S::kBytes, &p.q, first + kTile, head, b, &sh.first);
+      }
+      const auto load = [&](const CUtensorMap* map, int e) {
+        if (!attn_wait(&sh.empty[r.s], r.phase ^ 1, sh)) return false;
+        mbar_expect_tx(&sh.full[r.s], S::kStepBytes);
+        load_rows<kD, kStep>(ring + r.s * S::kStepBytes, map, list.at(e), kv_head, b, &sh.full[r.s]);
+        r.next();
+        return true;
+      };
+      // in the order in which they are used
+      bool ok = true;
+      for (int e = e0; ok && e < min(e0 + kSlots, e1); ++e) ok = load(&p.k, e);
+      for (int e = e0; ok && e < e1; ++e) ok = load(&p.v, e) && (e + kSlots >= e1 || load(&p.k, e + kSlots));
+      ring_end(sh.full, r);
+      mbar_wait_bounded(&sh.first, 0, kAttnLimitNs);
+    }
+  } else if (warp <= 2) {
+    if (e0 < e1) {
+      const int q = warp - 1;
       Ring<kStages> r;  // of what is waited for next
-      int scored[2] = {0, 0}, summed[2] = {0, 0};
-      const auto score = [&](int q, int e, const unsigned char* k) {
-        if (!any_seen(p, p0[q], p1[q], list.at(e) * kTile)) return true;
-        if (scored[q] && !attn_wait(&sh.done[q], (scored[q] - 1) & 1, sh)) return false;  // the probabilities that lie there have been read
-        tc_fence_after();
-        scores<T, kD>(tmem + q * kTile, tiles + q * S::kBytes, k);
-        attn_commit(&sh.s_full[q]);
-        ++scored[q];
-        return true;
-      };
-      const auto sum = [&](int q, int e, const unsigned char* v) {
-        if (!any_seen(p, p0[q], p1[q], list.at(e) * kTile)) return true;
-        if (!attn_wait(&sh.p_ready[q], summed[q] & 1, sh)) return false;
-        tc_fence_after();
-        weighted<T, kD>(tmem + 256 + q * kTile, tmem + q * kTile, 32, v, summed[q] > 0);
-        attn_commit(&sh.done[q]);
-        ++summed[q];
-        return true;
-      };
-      bool ok = attn_wait(&sh.first, 0, sh) && attn_wait(&sh.full[r.s], r.phase, sh);
-      if (ok) {
-        tc_fence_after();
-        const unsigned char* k = ring + r.s * S::kBytes;
-        ok = score(0, e0, k) && score(1, e0, k);
+      int scored = 0, summed = 0;
+      const auto score = [&](int e) {
+        if (!attn_wait_all(&sh.full[r.s], r.phase, sh)) return false;
+        if (any_seen(p, p0[q], p1[q], list.at(e))) {
+          const int n = scored++, slot = q * kSlots + n % kSlots;
+          if (n >= kSlots && !attn_wait_all(&sh.done[slot], (n / kSlots - 1) & 1, sh)) return false;  // the probabilities that lie there have been read
+          tc_fence_after();
+          scores<T, kD>(tmem + slot * kStep, tiles + q * S::kBytes, ring + r.s * S::kStepBytes);
+          attn_commit(&sh.s_full[slot]);
+        }
         attn_commit(&sh.empty[r.s]);
         r.next();
-      }
-      for (int e = e0; ok && e < e1; ++e) {
-        if (!attn_wait(&sh.full[r.s], r.phase, sh)) break;
-        tc_fence_after();
-        const int v_stage = r.s;
-        const unsigned char* v = ring + v_stage * S::kBytes;
-        r.next();
-        if (!sum(0, e, v)) break;
-        const bool more = e + 1 < e1;
-        const unsigned char* k = ring + r.s * S::kBytes;
-        if (more) {
-          if (!attn_wait(&sh.full[r.s], r.phase, sh)) break;
+        return true;
+      };
+      const auto sum = [&](int e) {
+        if (!attn_wait_all(&sh.full[r.s], r.phase, sh)) return false;
+        if (any_seen(p, p0[q], p1[q], list.at(e))) {
+          const int n = summed++, slot = q * kSlots + n % kSlots;
+          if (!attn_wait_all(&sh.p_ready[slot], (n / kSlots) & 1, sh)) return false;
           tc_fence_after();
-          if (!score(0, e + 1, k)) break;
+          weighted<T, kD>(tmem + kO + q * kD, tmem + slot * kStep, 16, ring + r.s * S::kStepBytes, n > 0);
+          attn_commit(&sh.done[slot]);
         }
-        if (!sum(1, e, v)) break;
-        attn_commit(&sh.empty[v_stage]);
-        if (more) {
-          if (!score(1, e + 1, k)) break;
-          attn_commit(&sh.empty[r.s]);
-          r.next();
-        }
-      }
+        attn_commit(&sh.empty[r.s]);
+        r.next();
+        return true;
+      };
+      bool ok = attn_wait_all(&sh.first, 0, sh);
+      for (int e = e0; ok && e < min(e0 + kSlots, e1); ++e) ok = score(e);
+      for (int e = e0; ok && e < e1; ++e) ok = sum(e) && (e + kSlots >= e1 || score(e + kSlots));
       attn_commit(&sh.drained);  // matrix instructions in flight are done before the CTA leaves
-      mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
+      if (lane == 0) mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
     }
-  } else {
-    const int quarter = warp & 3, q = (warp - 2) >> 2, row = quarter * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + q * kTile, o_at = lanes + 256 + q * kTile;
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, q = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), o_at = lanes + kO + q * kD;
     const int i = p.packed ? row % p.tq : first + q * kTile + row;
     const bool in = p.packed ? q == 0 && row < p.packed : i < p.tq;
     const bool some = __any_sync(0xffffffffu, in);
@@ -408,81 +418,92 @@ __global__ void __launch_bounds__(kAttnThreads, 1) hc_attention_kernel(const __g
     float most = -INFINITY, sum = 0.0f, ref = 0.0f;
     int taken = 0;
     bool ok = true;
-    for (int e = e0; e < e1; ++e) {
-      const int k0 = list.at(e) * kTile;
+    for (int e = e0; ok && e < e1; ++e) {
+      const int k0 = list.at(e);
       if (!any_seen(p, p0[q], p1[q], k0)) continue;
-      if (!attn_wait_all(&sh.s_full[q], taken & 1, sh)) {
-        ok = false;
-        break;
-      }
+      const int slot = q * kSlots + taken % kSlots;
+      const uint32_t s_at = lanes + slot * kStep;
+      ok = attn_wait_all(&sh.s_full[slot], (taken / kSlots) & 1, sh);
+      if (!ok) break;
       tc_fence_after();
       if (some) {
-        float v[4][32];
+        // where the registers do not hold all of a row's scores they are read twice
+        constexpr int kHeld = kD == 128 ? 2 : 1;
+        float v[kHeld][32], tops[4];
+        const bool whole = all_seen(p, p0[q], p1[q], k0, kStep);
+        const int high = position + 1 - k0, low = position - p.window + 1 - k0, sinks = min(p.sinks - k0, high);
+        const auto read = [&](int c, float(&w)[32]) {
+          tc_load32(s_at + c * 32, w);
+          tc_load_wait(w);
+          if (!whole) {
+            const uint32_t seen = seen_bits(low, high, sinks, c * 32);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tc_load32(s_at + c * 32, v[c]);
+            for (int j = 0; j < 32; ++j) w[j] = seen >> j & 1 ? w[j] : -INFINITY;
+          }
+        };
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tc_load_wait(v[c]);
-        if (!all_seen(p, p0[q], p1[q], k0)) {
-          const int high = position - k0, low = position - p.window + 1 - k0, sinks = p.sinks - k0;
+        for (int c = 0; c < 2; ++c) {
+          float(&w)[32] = v[c % kHeld];
+          read(c, w);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int h = 0; h < 2; ++h) {
+            float& m = tops[c * 2 + h];
+            m = fmaxf(w[h * 16], w[h * 16 + 1]);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int n = c * 32 + j;
-              if (n > high || (n < low && n >= sinks)) v[c][j] = -INFINITY;
-            }
+            for (int j = 2; j < 16; j += 2) m = max3(m, w[h * 16 + j], w[h * 16 + j + 1]);
+          }
         }
-        float tops[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tops[c] = fmaxf(v[c][0], v[c][1]);
-#pragma unroll
-          for (int j = 2; j < 32; j += 2) tops[c] = fmaxf(tops[c], fmaxf(v[c][j], v[c][j + 1]));
-        }
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
         const bool grows = top > most + slack;
-        float factor = 1.0f;
-        if (grows) {
-          factor = power2((most - top) * p.scale2);
-          most = top;
-          ref = top * p.scale2 - kBias;
-          sum *= factor;
-        }
-        if (taken && __any_sync(0xffffffffu, grows)) {
+        if (__any_sync(0xffffffffu, grows)) {
+          float factor = 1.0f;
+          if (grows) {
+            factor = power2((most - top) * p.scale2);
+            most = top;
+            ref = top * p.scale2 - kBias;
+            sum *= factor;
+          }
+          if (taken) {
+            // O has everything up to the step before
+            ok = attn_wait_all(&sh.done[q * kSlots + (taken - 1) % kSlots], ((taken - 1) / kSlots) & 1, sh);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 32) {
+              float o[32];
+              tc_load32(o_at + c, o);
+              tc_load_wait(o);
 #pragma unroll
-          for (int c = 0; c < kD; c += 32) {
-            float o[32];
-            __syncwarp();
-            tc_load32(o_at + c, o);
-            tc_load_wait(o);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] *= factor;
-            tc_store32(o_at + c, o);
+              for (int j = 0; j < 32; ++j) o[j] *= factor;
+              tc_store32(o_at + c, o);
+            }
           }
         }
         const Pair scale = pair(p.scale2, p.scale2), less = pair(-ref, -ref);
-        Pair total = pair(0.0f, 0.0f);
+        Pair total[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
+          float(&w)[32] = v[c % kHeld];
+          if (kHeld == 1) read(c, w);
           uint32_t words[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             float x, y;
-            parts(fma2(pair(v[c][j], v[c][j + 1]), scale, less), x, y);
+            parts(fma2(pair(w[j], w[j + 1]), scale, less), x, y);
             x = power2(x);
             y = power2(y);
-            total = total + pair(x, y);
+            total[j / 2 % 2] = total[j / 2 % 2] + pair(x, y);
             words[j / 2] = pack2<T>(x, y);
           }
           tc_store16(s_at + c * 16, words);
         }
-        sum += both(total);
+        sum += both(total[0] + total[1]);
         tc_store_wait();
       }
       ++taken;
-      warp_arrives(&sh.p_ready[q]);
+      warp_arrives(&sh.p_ready[slot]);
     }
-    if (ok && taken && !attn_wait_all(&sh.done[q], (taken - 1) & 1, sh)) ok = false;
+    if (ok && e0 < e1) ok = attn_wait_all(&sh.drained, 0, sh);
     if (ok && some) {
       tc_fence_after();
       const bool none = sum == 0.0f;  // (a NaN is not)
@@ -498,7 +519,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) hc_attention_kernel(const __g
       }
     }
   }
-  attn_end(tmem);
+  attn_end<S::kColumns>(tmem);
 }
 
 // Joins the results of CTAs that shared the keys out: a warp a query and head.
@@ -611,347 +632,267 @@ __device__ __forceinline__ float ds_power(const unsigned int* most, int sign) {
   return __int_as_float((127 + sign * k) << 23);
 }
 
-// dK and dV of a tile of keys.  Tensor memory: scores (keys in lanes, queries in columns) at 0, dO V^T at 128, dV at 256, dK at 384.  The two halves of the warps have 64
-// queries each, whose probabilities lie at the beginning of their own 64 columns.
-template <typename T, int kD>
-__global__ void __launch_bounds__(kAttnThreads, 1) hc_attention_dkv_kernel(const __grid_constant__ AttnParams p) {
+// The backward pass of a tile of 128 keys (kKeys: dV = P^T dO, dK = scale dS^T Q; a stream of queries, 64 at a time) or of 128 queries (dQ = scale dS K; a stream of keys).  The tile
+// lies in lanes, the stream in columns.  Eight warps work on a step, four on each half of its columns; with heads of more than 64 values two groups of eight take the steps in turn, with smaller ones
+// two CTAs are on an SM, so that exponentials, multiplications and the tensor cores' work overlap.  One warp issues the products that form scores, one those that sum.
+// Tensor memory: scores of the groups' steps, then dO V^T (P and dS at the beginning of each half's 32 columns), then the two sums.
+//
+// delta from the rounded O, whose probabilities were rounded too, is wrong by some 2^-9 of itself, and all of a row's dS with it: half of the error of dQ and dK (1024 x 1024, 2.8e-3 of dQ's norm, where
+// all other roundings come to 2.5e-3).  The rows of dS sum to 0, so the sum of what they are instead is what delta lacks: r = sum_j P (dP - delta).  The queries' pass finds r on
+// its way, sums P K beside dS K, and gives dQ = scale (dS K - r P K); delta + r goes to the keys' pass, which comes behind it.
+template <typename T, int kD, bool kKeys>
+__global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>::kResident) hc_attention_backward_kernel(const __grid_constant__ AttnParams p) {
   using S = AttnShape<kD>;
-  constexpr int kQ = S::kQStages, kDo = S::kDoStages;
-  constexpr float kBias = operand_format<T>() ? 0.0f : 14.0f;  // probabilities are held times 2^14 in fp16
+  constexpr int kStages = S::kStages, kStageBytes = 2 * S::kStepBytes, kGroups = S::kGroups, kParts = 2 * kGroups;
+  constexpr int kDp = kGroups * kStep, kSum1 = 2 * kDp, kSum2 = kSum1 + kD;  // columns of tensor memory
+  constexpr bool kF16 = operand_format<T>() == 0;
   extern __shared__ unsigned char raw[];
   __shared__ AttnBarriers sh;
-  unsigned char *k_tile = attn_tiles(raw), *v_tile = k_tile + S::kBytes, *q_ring = v_tile + S::kBytes, *do_ring = q_ring + kQ * S::kBytes;
-  float* sides = reinterpret_cast<float*>(do_ring + kDo * S::kBytes);  // of a stage of queries: less, delta
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float lacking[kParts][kTile];
+  unsigned char *tile1 = attn_tiles(raw), *tile2 = tile1 + S::kBytes, *ring = tile2 + S::kBytes;
+  float* sides = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // of a step of queries: less, delta
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int heads = kKeys ? p.kv_heads : p.heads;
   int64_t at = blockIdx.x;
-  const int head = (int)(at % p.kv_heads);
-  at /= p.kv_heads;
-  const int b = (int)(at % p.batch), block = (int)(at / p.batch);
-  const int k0 = block * kTile, k1 = min(k0 + kTile, p.tk) - 1;
-  // the queries that see one of them, in tiles
-  const int i_first = max(k0 - p.off, 0), i_last = k0 < p.sinks ? p.tq - 1 : (int)min((int64_t)p.tq - 1, (int64_t)k1 + p.window - 1 - p.off);
-  const int t_first = i_first / kTile, tiles = i_first <= i_last ? i_last / kTile - t_first + 1 : 0, count = tiles * p.group;
-  attn_begin(sh, kAttnWarps);
-  const uint32_t tmem = sh.tmem;
+  const int head = (int)(at % heads);
+  at /= heads;
+  const int b = (int)(at % p.batch), block = kKeys ? (int)(at / p.batch) : p.blocks - 1 - (int)(at / p.batch);
+  const int t0 = block * kTile;  // the tile's first row
+  // the stream: queries that see one of the keys, head after head; or the keys that the queries see
+  const int q_first = max(t0 - p.off, 0) / kStep,
+            q_last = t0 < p.sinks ? p.tq - 1 : (int)min((int64_t)p.tq - 1, (int64_t)min(t0 + kTile, p.tk) - 1 + p.window - 1 - p.off);
+  const int q_steps = q_last >= max(t0 - p.off, 0) ? q_last / kStep - q_first + 1 : 0;
+  const int p0 = p.off + t0, p1 = p.off + min(t0 + kTile, p.tq) - 1;
+  const KeySteps list = kKeys ? KeySteps{0, 0, 0} : key_steps(p, p0, p1);
+  const int count = kKeys ? q_steps * p.group : list.count;
+  attn_begin<S::kColumns>(sh, 8 * kGroups, 8, 1);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   if (warp == 0) {
     if (lane == 0 && count) {
-      Ring<kQ> rq;
-      Ring<kDo> rd;
+      Ring<kStages> r;
       mbar_expect_tx(&sh.first, 2 * S::kBytes);
-      load_tile<kD>(k_tile, &p.k, k0, head, b, &sh.first);
-      load_tile<kD>(v_tile, &p.v, k0, head, b, &sh.first);
+      load_rows<kD, kTile>(tile1, kKeys ? &p.k_tile : &p.q_tile, t0, head, b, &sh.first);
+      load_rows<kD, kTile>(tile2, kKeys ? &p.v_tile : &p.dout_tile, t0, head, b, &sh.first);
+      int h = kKeys ? head * p.group : head / p.group, step = 0;
       for (int e = 0; e < count; ++e) {
-        const int h = head * p.group + e / tiles, i0 = (t_first + e % tiles) * kTile;
-        const int64_t side = ((int64_t)b * p.heads + h) * p.less_ld + i0;
-        if (!attn_wait(&sh.empty[rq.s], rq.phase ^ 1, sh)) break;
-        mbar_expect_tx(&sh.full[rq.s], S::kBytes + 1024);
-        load_tile<kD>(q_ring + rq.s * S::kBytes, &p.q, i0, h, b, &sh.full[rq.s]);
-        load_floats(sides + rq.s * 256, p.less + side, 512, &sh.full[rq.s]);
-        load_floats(sides + rq.s * 256 + 128, p.delta + side, 512, &sh.full[rq.s]);
-        rq.next();
-        if (!attn_wait(&sh.more_empty[rd.s], rd.phase ^ 1, sh)) break;
-        mbar_expect_tx(&sh.more_full[rd.s], S::kBytes);
-        load_tile<kD>(do_ring + rd.s * S::kBytes, &p.dout, i0, h, b, &sh.more_full[rd.s]);
-        rd.next();
+        if (!attn_wait(&sh.empty[r.s], r.phase ^ 1, sh)) break;
+        const int at0 = kKeys ? (q_first + step) * kStep : list.at(e);
+        unsigned char* to = ring + r.s * kStageBytes;
+        mbar_expect_tx(&sh.full[r.s], kStageBytes + (kKeys ? 512 : 0));
+        load_rows<kD, kStep>(to, kKeys ? &p.q : &p.k, at0, h, b, &sh.full[r.s]);
+        load_rows<kD, kStep>(to + S::kStepBytes, kKeys ? &p.dout : &p.v, at0, h, b, &sh.full[r.s]);
+        if (kKeys) {
+          const int64_t side = ((int64_t)b * p.heads + h) * p.less_ld + at0;
+          load_floats(sides + r.s * 128, p.less + side, 256, &sh.full[r.s]);
+          load_floats(sides + r.s * 128 + 64, p.delta + side, 256, &sh.full[r.s]);
+          if (++step == q_steps) {
+            step = 0;
+            ++h;
+          }
+        }
+        r.next();
       }
-      ring_end(sh.full, rq);
-      ring_end(sh.more_full, rd);
+      ring_end(sh.full, r);
       mbar_wait_bounded(&sh.first, 0, kAttnLimitNs);
     }
-  } else if (warp == 1) {
-    if (lane == 0 && count) {
-      Ring<kQ> rq;   // of the tile whose scores come next
-      Ring<kDo> rd;
-      const auto score = [&] {  // of the next tile of queries
-        if (!attn_wait(&sh.full[rq.s], rq.phase, sh)) return false;
-        tc_fence_after();
-        scores<T, kD>(tmem, k_tile, q_ring + rq.s * S::kBytes);
-        attn_commit(&sh.s_full[0]);
-        return true;
-      };
-      const auto second = [&] {
-        if (!attn_wait(&sh.more_full[rd.s], rd.phase, sh)) return false;
-        tc_fence_after();
-        scores<T, kD>(tmem + kTile, v_tile, do_ring + rd.s * S::kBytes);
-        attn_commit(&sh.dp_full[0]);
-        return true;
-      };
-      if (attn_wait(&sh.first, 0, sh) && score() && second()) {
-        for (int e = 0; e < count; ++e) {
-          const uint32_t turn = e & 1;
-          const int sq = rq.s, sd = rd.s;
-          if (!attn_wait(&sh.p_ready[0], turn, sh)) break;
+  } else if (warp <= 2) {
+    if (count) {
+      // a step's place in the ring; what is waited for the k-th time has parity k & 1
+      const auto stage = [&](int e) { return ring + e % kStages * kStageBytes; };
+      bool ok = true;
+      if (warp == 1) {
+        ok = attn_wait_all(&sh.first, 0, sh);
+        for (int e = 0; ok && e < count; ++e) {
+          const int g = e % kGroups;
+          const uint32_t before = (e / kGroups - 1) & 1;
+          ok = attn_wait_all(&sh.full[e % kStages], (e / kStages) & 1, sh) && (e < kGroups || attn_wait_all(&sh.done[g], before, sh));
+          if (!ok) break;
           tc_fence_after();
-          weighted<T, kD>(tmem + 256, tmem, 64, do_ring + sd * S::kBytes, e > 0);
-          attn_commit(&sh.done[0]);
-          attn_commit(&sh.more_empty[sd]);
-          rq.next();
-          rd.next();
-          if (e + 1 < count && (!attn_wait(&sh.done[0], turn, sh) || !score())) break;
-          if (!attn_wait(&sh.ds_ready[0], turn, sh)) break;
+          scores<T, kD>(tmem + g * kStep, tile1, stage(e));
+          attn_commit(&sh.s_full[g]);
+          ok = e < kGroups || attn_wait_all(&sh.ds_done[g], before, sh);
+          if (!ok) break;
           tc_fence_after();
-          weighted<T, kD>(tmem + 384, tmem + kTile, 64, q_ring + sq * S::kBytes, e > 0);
-          attn_commit(&sh.done[1]);
-          attn_commit(&sh.empty[sq]);
-          if (e + 1 < count && (!attn_wait(&sh.done[1], turn, sh) || !second())) break;
+          scores<T, kD>(tmem + kDp + g * kStep, tile2, stage(e) + S::kStepBytes);
+          attn_commit(&sh.dp_full[g]);
         }
+      } else {
+        const auto second_sum = [&](int e) {
+          const int g = e % kGroups;
+          if (!attn_wait_all(&sh.ds_ready[g], (e / kGroups) & 1, sh)) return false;
+          tc_fence_after();
+          weighted<T, kD>(tmem + kSum2, tmem + kDp + g * kStep, 32, stage(e), e > 0);
+          attn_commit(&sh.ds_done[g]);
+          attn_commit(&sh.empty[e % kStages]);  // all four products of the step are done then
+          return true;
+        };
+        for (int e = 0; ok && e < count; ++e) {
+          const int g = e % kGroups;
+          ok = attn_wait_all(&sh.full[e % kStages], (e / kStages) & 1, sh) && attn_wait_all(&sh.p_ready[g], (e / kGroups) & 1, sh);
+          if (!ok) break;
+          tc_fence_after();
+          weighted<T, kD>(tmem + kSum1, tmem + g * kStep, 32, stage(e) + (kKeys ? S::kStepBytes : 0), e > 0);
+          attn_commit(&sh.done[g]);
+          ok = e < kGroups - 1 || second_sum(e - (kGroups - 1));
+        }
+        for (int e = count - min(kGroups - 1, count); ok && e < count; ++e) ok = second_sum(e);
       }
       attn_commit(&sh.drained);
-      mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
+      if (lane == 0) mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
     }
-  } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, j = k0 + quarter * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + half * 64, dp_at = lanes + kTile + half * 64;
-    const float power = operand_format<T>() ? 1.0f : ds_power(p.most, 1), back = operand_format<T>() ? 1.0f : ds_power(p.most, -1);
-    const float gain = operand_format<T>() ? 1.0f : power * (1.0f / 16384.0f);
-    const Pair scale = pair(p.scale2, p.scale2), bias = pair(kBias, kBias);
-    Ring<kQ> rq;
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, part = (warp - 4) >> 2, g = part >> 1, half = part & 1, row = quarter * 32 + lane, t = t0 + row;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + g * kStep + half * 32, dp_at = s_at + kDp;
+    constexpr float kBias = kF16 && kKeys ? 14.0f : 0.0f;  // P^T is held times 2^14 in fp16 (what P K is for needs no more than a few bits)
+    const float power = kF16 ? ds_power(p.most, 1) : 1.0f, back = kF16 ? ds_power(p.most, -1) : 1.0f;
+    const Pair gain = pair(power * (kBias ? 1.0f / 16384.0f : 1.0f), power * (kBias ? 1.0f / 16384.0f : 1.0f));
+    const Pair scale = pair(p.scale2, p.scale2), minus = pair(-1.0f, -1.0f), bias = pair(kBias, kBias);
+    const bool in = t < (kKeys ? p.tk : p.tq);
+    const int64_t side = ((int64_t)b * p.heads + head) * p.less_ld + t;
+    float delta = 0.0f;
+    Pair less = pair(-INFINITY, -INFINITY), delta2 = pair(0.0f, 0.0f), lacks = pair(0.0f, 0.0f);
+    if (!kKeys && in) {
+      delta = p.delta[side];
+      less = pair(p.less[side], p.less[side]);
+      delta2 = pair(delta, delta);
+    }
+    int step = g;
+    if (kKeys)
+      while (q_steps && step >= q_steps) step -= q_steps;
     bool ok = true;
-    for (int e = 0; e < count; ++e) {
-      const uint32_t turn = e & 1;
-      const int i0 = (t_first + e % tiles) * kTile;
-      const float* less = sides + rq.s * 256 + half * 64;
-      if (!attn_wait_all(&sh.full[rq.s], rq.phase, sh) || !attn_wait_all(&sh.s_full[0], turn, sh)) {
+    for (int e = g; e < count; e += kGroups) {
+      const uint32_t turn = (e / kGroups) & 1;
+      const float* side_at = sides + e % kStages * 128 + half * 32;
+      if ((kKeys && !attn_wait_all(&sh.full[e % kStages], (e / kStages) & 1, sh)) || !attn_wait_all(&sh.s_full[g], turn, sh)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      float v[2][32];
-      tc_load32(s_at, v[0]);
-      tc_load32(s_at + 32, v[1]);
-      tc_load_wait(v[0]);
-      tc_load_wait(v[1]);
-      const int pa = p.off + i0, pb = p.off + min(i0 + kTile, p.tq) - 1;
-      const bool whole = all_seen(p, pa, pb, k0) && i0 + kTile <= p.tq;
-      // the columns (queries) that see this row's key
-      const int low = j - pa - half * 64;
-      const int high = min(p.tq - i0, (int)min((int64_t)kTile, j < p.sinks ? (int64_t)kTile : (int64_t)j + p.window - pa)) - half * 64;
+      float v[32];
+      tc_load32(s_at, v);
+      // what this row sees, or is seen by
+      bool whole;
+      uint32_t seen;
+      if (kKeys) {
+        const int i0 = (q_first + step) * kStep, pa = p.off + i0;
+        whole = i0 + kStep <= p.tq && all_seen(p, pa, pa + kStep - 1, t0, kTile);
+        const int high = min(p.tq - i0, (int)min((int64_t)kStep, t < p.sinks ? (int64_t)kStep : (int64_t)t + p.window - pa));
+        seen = seen_bits(t - pa, high, 0, half * 32);
+        step += kGroups;
+        while (step >= q_steps) step -= q_steps;
+      } else {
+        const int k0 = list.at(e), position = p.off + t, high = position - k0 + 1;
+        whole = all_seen(p, p0, p1, k0, kStep);
+        seen = seen_bits(position - p.window + 1 - k0, high, min(p.sinks - k0, high), half * 32);
+      }
+      tc_load_wait(v);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t words[16];
-#pragma unroll
-        for (int n = 0; n < 32; n += 4) {
-          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(less + c * 32 + n);
-          Pair l0 = {l.x}, l1 = {l.y};
-          if (!operand_format<T>()) {
+      for (int n = 0; n < 32; n += 4) {
+        Pair l0 = less, l1 = less;
+        if (kKeys) {
+          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(side_at + n);
+          l0 = Pair{l.x};
+          l1 = Pair{l.y};
+          if (kBias) {
             l0 = l0 + bias;
             l1 = l1 + bias;
           }
-          parts(fma2(pair(v[c][n], v[c][n + 1]), scale, l0), v[c][n], v[c][n + 1]);
-          parts(fma2(pair(v[c][n + 2], v[c][n + 3]), scale, l1), v[c][n + 2], v[c][n + 3]);
         }
-#pragma unroll
-        for (int n = 0; n < 32; ++n) v[c][n] = power2(v[c][n]);
-        if (!whole) {
-#pragma unroll
-          for (int n = 0; n < 32; ++n)
-            if (c * 32 + n < low || c * 32 + n >= high) v[c][n] = 0.0f;
-        }
-#pragma unroll
-        for (int n = 0; n < 32; n += 2) words[n / 2] = pack2<T>(v[c][n], v[c][n + 1]);
-        tc_store16(s_at + c * 16, words);
+        parts(fma2(pair(v[n], v[n + 1]), scale, l0), v[n], v[n + 1]);
+        parts(fma2(pair(v[n + 2], v[n + 3]), scale, l1), v[n + 2], v[n + 3]);
       }
+#pragma unroll
+      for (int n = 0; n < 32; ++n) v[n] = power2(v[n]);
+      if (!whole) {
+#pragma unroll
+        for (int n = 0; n < 32; ++n) v[n] = seen >> n & 1 ? v[n] : 0.0f;
+      }
+      uint32_t words[16];
+#pragma unroll
+      for (int n = 0; n < 32; n += 2) words[n / 2] = pack2<T>(v[n], v[n + 1]);
+      tc_store16(s_at, words);
       tc_store_wait();
-      warp_arrives(&sh.p_ready[0]);
-      if (!attn_wait_all(&sh.dp_full[0], turn, sh)) {
+      warp_arrives(&sh.p_ready[g]);
+      if (!attn_wait_all(&sh.dp_full[g], turn, sh)) {
         ok = false;
         break;
       }
       tc_fence_after();
+      float d[32];
+      tc_load32(dp_at, d);
+      tc_load_wait(d);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float g[32];
-        __syncwarp();
-        tc_load32(dp_at + c * 32, g);
-        tc_load_wait(g);
-        uint32_t words[16];
-#pragma unroll
-        for (int n = 0; n < 32; n += 4) {
-          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(less + 128 + c * 32 + n);
-          const Pair minus = pair(-1.0f, -1.0f);
-          Pair a = fma2(Pair{l.x}, minus, pair(g[n], g[n + 1])), w = fma2(Pair{l.y}, minus, pair(g[n + 2], g[n + 3]));
-          Pair pa2 = pair(v[c][n], v[c][n + 1]), pb2 = pair(v[c][n + 2], v[c][n + 3]);
-          if (!operand_format<T>()) {
-            pa2 = pa2 * pair(gain, gain);
-            pb2 = pb2 * pair(gain, gain);
-          }
-          parts(a * pa2, g[n], g[n + 1]);
-          parts(w * pb2, g[n + 2], g[n + 3]);
+      for (int n = 0; n < 32; n += 4) {
+        Pair l0 = delta2, l1 = delta2;
+        if (kKeys) {
+          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(side_at + 64 + n);
+          l0 = Pair{l.x};
+          l1 = Pair{l.y};
         }
-        if (!whole) {  // also where a query that does not see the key, or is none, has no number
-#pragma unroll
-          for (int n = 0; n < 32; ++n)
-            if (c * 32 + n < low || c * 32 + n >= high) g[n] = 0.0f;
+        Pair x = fma2(l0, minus, pair(d[n], d[n + 1])) * pair(v[n], v[n + 1]), y = fma2(l1, minus, pair(d[n + 2], d[n + 3])) * pair(v[n + 2], v[n + 3]);
+        if (kF16) {
+          x = x * gain;
+          y = y * gain;
         }
-#pragma unroll
-        for (int n = 0; n < 32; n += 2) words[n / 2] = pack2<T>(g[n], g[n + 1]);
-        tc_store16(dp_at + c * 16, words);
+        parts(x, d[n], d[n + 1]);
+        parts(y, d[n + 2], d[n + 3]);
       }
+      if (!whole) {  // also where one that is not seen, or a query that is none, has no number
+#pragma unroll
+        for (int n = 0; n < 32; ++n) d[n] = seen >> n & 1 ? d[n] : 0.0f;
+      }
+#pragma unroll
+      for (int n = 0; n < 32; n += 2) {
+        if (!kKeys) lacks = lacks + pair(d[n], d[n + 1]);
+        words[n / 2] = pack2<T>(d[n], d[n + 1]);
+      }
+      tc_store16(dp_at, words);
       tc_store_wait();
-      warp_arrives(&sh.ds_ready[0]);
-      rq.next();
+      warp_arrives(&sh.ds_ready[g]);
     }
-    if (ok && count) ok = attn_wait_all(&sh.done[0], (count - 1) & 1, sh) && attn_wait_all(&sh.done[1], (count - 1) & 1, sh);
-    if (ok) {
+    if (ok && count) ok = attn_wait_all(&sh.drained, 0, sh);
+    if (ok && kKeys) {
       tc_fence_after();
-      // the first half of the warps stores dV, the second dK
-      T* to = static_cast<T*>(half ? p.dk : p.dv) + (((int64_t)b * p.tk + j) * p.kv_heads + head) * p.d;
-      const float factor = half ? p.scale * back : operand_format<T>() ? 1.0f : 1.0f / 16384.0f;
-      store_row<T, kD>(lanes + 256 + half * kTile, to, p.d, factor, j < p.tk, count > 0, false);
+      // 64 of the columns of dV and dK each
+      const bool second = part * 64 >= kD;
+      const int c = part * 64 % kD;
+      T* to = static_cast<T*>(second ? p.dk : p.dv) + (((int64_t)b * p.tk + t) * p.kv_heads + head) * p.d + c;
+      store_row<T, 64>(lanes + kSum1 + part * 64, to, p.d - c, second ? p.scale * back : kF16 ? 1.0f / 16384.0f : 1.0f, in, count > 0, false);
+    }
+    if (ok && !kKeys) {
+      lacking[part][row] = both(lacks) * back;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.met);
+      ok = attn_wait_all(&sh.met, 0, sh);
+      float r = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) r += lacking[k][row];
+      if (ok && in && part == 0) p.delta[side] = delta + r;
+      tc_fence_after();
+      // 32 of the columns each
+      static_assert(kParts * 32 == kD, "a part's columns");
+      const int c = part * 32;
+      float x[32], y[32];
+      if (count) {
+        tc_load32(lanes + kSum1 + c, x);
+        tc_load32(lanes + kSum2 + c, y);
+        tc_load_wait(x);
+        tc_load_wait(y);
+      }
+      if (ok && in && p.dq) {
+        T* to = static_cast<T*>(p.dq) + (((int64_t)b * p.tq + t) * p.heads + head) * p.d + c;
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          if (c + j >= p.d) continue;
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = count ? p.scale * (y[j + k] * back - r * x[j + k]) : 0.0f;
+          store8(to + j, v);
+        }
+      }
     }
   }
-  attn_end(tmem);
-}
-
-// dQ of a tile of queries.  Tensor memory: scores (queries in lanes) at 0, dO V^T at 128 and 256 in turn, dQ at 384.
-template <typename T, int kD>
-__global__ void __launch_bounds__(kAttnThreads, 1) hc_attention_dq_kernel(const __grid_constant__ AttnParams p) {
-  using S = AttnShape<kD>;
-  constexpr int kK = S::kKStages, kV = S::kVStages;
-  extern __shared__ unsigned char raw[];
-  __shared__ AttnBarriers sh;
-  unsigned char *q_tile = attn_tiles(raw), *do_tile = q_tile + S::kBytes, *k_ring = do_tile + S::kBytes, *v_ring = k_ring + kK * S::kBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t at = blockIdx.x;
-  const int head = (int)(at % p.heads);
-  at /= p.heads;
-  const int b = (int)(at % p.batch), block = p.blocks - 1 - (int)(at / p.batch);
-  const int i0 = block * kTile, p0 = p.off + i0, p1 = p.off + min(i0 + kTile, p.tq) - 1;
-  const KeyTiles list = key_tiles(p, p0, p1);
-  const int count = list.count;
-  attn_begin(sh, kAttnWarps);
-  const uint32_t tmem = sh.tmem;
-  if (warp == 0) {
-    if (lane == 0 && count) {
-      Ring<kK> rk;
-      Ring<kV> rv;
-      mbar_expect_tx(&sh.first, 2 * S::kBytes);
-      load_tile<kD>(q_tile, &p.q, i0, head, b, &sh.first);
-      load_tile<kD>(do_tile, &p.dout, i0, head, b, &sh.first);
-      for (int e = 0; e < count; ++e) {
-        const int k0 = list.at(e) * kTile;
-        if (!attn_wait(&sh.empty[rk.s], rk.phase ^ 1, sh)) break;
-        mbar_expect_tx(&sh.full[rk.s], S::kBytes);
-        load_tile<kD>(k_ring + rk.s * S::kBytes, &p.k, k0, head / p.group, b, &sh.full[rk.s]);
-        rk.next();
-        if (!attn_wait(&sh.more_empty[rv.s], rv.phase ^ 1, sh)) break;
-        mbar_expect_tx(&sh.more_full[rv.s], S::kBytes);
-        load_tile<kD>(v_ring + rv.s * S::kBytes, &p.v, k0, head / p.group, b, &sh.more_full[rv.s]);
-        rv.next();
-      }
-      ring_end(sh.full, rk);
-      ring_end(sh.more_full, rv);
-      mbar_wait_bounded(&sh.first, 0, kAttnLimitNs);
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && count) {
-      Ring<kK> rk, used;  // of the tile whose scores come next; of the one whose dS comes next
-      Ring<kV> rv;
-      const auto score = [&](int e) {
-        if (!attn_wait(&sh.full[rk.s], rk.phase, sh)) return false;
-        if (e && !attn_wait(&sh.s_read, (e - 1) & 1, sh)) return false;
-        tc_fence_after();
-        scores<T, kD>(tmem, q_tile, k_ring + rk.s * S::kBytes);
-        attn_commit(&sh.s_full[0]);
-        rk.next();
-        if (!attn_wait(&sh.more_full[rv.s], rv.phase, sh)) return false;
-        if (e >= 2 && !attn_wait(&sh.done[e & 1], (e / 2 - 1) & 1, sh)) return false;
-        tc_fence_after();
-        scores<T, kD>(tmem + (1 + (e & 1)) * kTile, do_tile, v_ring + rv.s * S::kBytes);
-        attn_commit(&sh.dp_full[e & 1]);
-        attn_commit(&sh.more_empty[rv.s]);
-        rv.next();
-        return true;
-      };
-      if (attn_wait(&sh.first, 0, sh) && score(0)) {
-        for (int e = 0; e < count; ++e) {
-          if (e + 1 < count && !score(e + 1)) break;
-          if (!attn_wait(&sh.ds_ready[e & 1], (e / 2) & 1, sh)) break;
-          tc_fence_after();
-          weighted<T, kD>(tmem + 384, tmem + (1 + (e & 1)) * kTile, 64, k_ring + used.s * S::kBytes, e > 0);
-          attn_commit(&sh.done[e & 1]);
-          attn_commit(&sh.empty[used.s]);
-          used.next();
-        }
-      }
-      attn_commit(&sh.drained);
-      mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
-    }
-  } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, i = i0 + quarter * 32 + lane, position = p.off + i;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + half * 64;
-    const float power = operand_format<T>() ? 1.0f : ds_power(p.most, 1), back = operand_format<T>() ? 1.0f : ds_power(p.most, -1);
-    const bool in = i < p.tq;
-    const int64_t side = ((int64_t)b * p.heads + head) * p.less_ld + i;
-    const float less = in ? p.less[side] : -INFINITY, delta = in ? p.delta[side] : 0.0f;
-    const Pair scale = pair(p.scale2, p.scale2), less2 = pair(less, less), delta2 = pair(-delta, -delta), gain = pair(power, power);
-    bool ok = true;
-    for (int e = 0; e < count; ++e) {
-      const int k0 = list.at(e) * kTile;
-      if (!attn_wait_all(&sh.s_full[0], e & 1, sh)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float v[2][32];
-      tc_load32(s_at, v[0]);
-      tc_load32(s_at + 32, v[1]);
-      tc_load_wait(v[0]);
-      tc_load_wait(v[1]);
-      warp_arrives(&sh.s_read);
-      const bool whole = all_seen(p, p0, p1, k0);
-      const int high = position - k0 - half * 64, low = position - p.window + 1 - k0 - half * 64, sinks = p.sinks - k0 - half * 64;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int n = 0; n < 32; n += 2) {
-          float x, y;
-          parts(fma2(pair(v[c][n], v[c][n + 1]), scale, less2), x, y);
-          v[c][n] = power2(x);
-          v[c][n + 1] = power2(y);
-        }
-      }
-      if (!attn_wait_all(&sh.dp_full[e & 1], (e / 2) & 1, sh)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t dp_at = lanes + (1 + (e & 1)) * kTile + half * 64;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float g[32];
-        __syncwarp();
-        tc_load32(dp_at + c * 32, g);
-        tc_load_wait(g);
-        uint32_t words[16];
-#pragma unroll
-        for (int n = 0; n < 32; n += 2) {
-          Pair a = (pair(g[n], g[n + 1]) + delta2) * pair(v[c][n], v[c][n + 1]);
-          if (!operand_format<T>()) a = a * gain;
-          parts(a, g[n], g[n + 1]);
-        }
-        if (!whole) {
-#pragma unroll
-          for (int n = 0; n < 32; ++n) {
-            const int m = c * 32 + n;
-            if (m > high || (m < low && m >= sinks)) g[n] = 0.0f;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 32; n += 2) words[n / 2] = pack2<T>(g[n], g[n + 1]);
-        tc_store16(dp_at + c * 16, words);
-      }
-      tc_store_wait();
-      warp_arrives(&sh.ds_ready[e & 1]);
-    }
-    if (ok && count) ok = attn_wait_all(&sh.done[(count - 1) & 1], ((count - 1) / 2) & 1, sh);
-    if (ok && !half) {
-      tc_fence_after();
-      T* to = static_cast<T*>(p.dq) + (((int64_t)b * p.tq + i) * p.heads + head) * p.d;
-      store_row<T, kD>(lanes + 384, to, p.d, p.scale * back, in, count > 0, false);
-    }
-  }
-  attn_end(tmem);
+  attn_end<S::kColumns>(tmem);
 }
 
 }  // namespace dev
@@ -1031,7 +972,7 @@ cudaError_t run_forward(const dev::AttnParams& p, const Plan& plan, cudaStream_t
   cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t ctas = (int64_t)p.batch * (p.packed ? p.kv_heads : p.heads) * p.blocks * p.splits;
-  dev::hc_attention_kernel<T, kD><<<(unsigned)ctas, dev::kAttnThreads, smem, stream>>>(p);
+  dev::hc_attention_kernel<T, kD><<<(unsigned)ctas, dev::AttnShape<kD>::kForwardThreads, smem, stream>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess || plan.splits == 1) return e;
   const int64_t queries = (int64_t)p.batch * p.heads * p.tq;
@@ -1042,9 +983,9 @@ cudaError_t run_forward(const dev::AttnParams& p, const Plan& plan, cudaStream_t
 template <typename T, int kD>
 cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_heads& v, const void* o, float* delta, unsigned int* most, cudaStream_t stream) {
   static unsigned long long allowed_kv = 0, allowed_q = 0;
-  using S = dev::AttnShape<kD>;
-  cudaError_t e = allow_smem(dev::hc_attention_dkv_kernel<T, kD>, S::kKvSmem, &allowed_kv);
-  if (e == cudaSuccess) e = allow_smem(dev::hc_attention_dq_kernel<T, kD>, S::kQSmem, &allowed_q);
+  constexpr int smem = dev::AttnShape<kD>::kBackwardSmem;
+  cudaError_t e = allow_smem(dev::hc_attention_backward_kernel<T, kD, true>, smem, &allowed_kv);
+  if (e == cudaSuccess) e = allow_smem(dev::hc_attention_backward_kernel<T, kD, false>, smem, &allowed_q);
   if (e != cudaSuccess) return e;
   constexpr int kLanes = kD / 8;
   const int64_t most_blocks = attn_sms() * 8;
@@ -1056,13 +997,12 @@ cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_head
         static_cast<const T*>(v.data), (int64_t)v.batch, (int64_t)v.head, (int64_t)v.position, p.batch, p.kv_heads, p.tk, p.d, most + 1);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
+  // dq or not: the keys' pass needs the delta that this one completes
+  p.blocks = (p.tq + dev::kTile - 1) / dev::kTile;
+  dev::hc_attention_backward_kernel<T, kD, false><<<(unsigned)((int64_t)p.batch * p.heads * p.blocks), dev::AttnShape<kD>::kBackwardThreads, smem, stream>>>(p);
   if (p.dk) {
     p.blocks = (p.tk + dev::kTile - 1) / dev::kTile;
-    dev::hc_attention_dkv_kernel<T, kD><<<(unsigned)((int64_t)p.batch * p.kv_heads * p.blocks), dev::kAttnThreads, S::kKvSmem, stream>>>(p);
-  }
-  if (p.dq) {
-    p.blocks = (p.tq + dev::kTile - 1) / dev::kTile;
-    dev::hc_attention_dq_kernel<T, kD><<<(unsigned)((int64_t)p.batch * p.heads * p.blocks), dev::kAttnThreads, S::kQSmem, stream>>>(p);
+    dev::hc_attention_backward_kernel<T, kD, true><<<(unsigned)((int64_t)p.batch * p.kv_heads * p.blocks), dev::AttnShape<kD>::kBackwardThreads, smem, stream>>>(p);
   }
   return cudaGetLastError();
 }
@@ -1116,7 +1056,7 @@ int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float*
     p.part_less = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + up(rows * plan.splits * head_size * sizeof(float), 256));
   }
   if (!make_head_map(&p.q, type, q, head_size, queries, heads, batch, plan.packed ? (int)queries : dev::kTile, plan.packed ? p.group : 1) ||
-      !make_head_map(&p.k, type, k, head_size, keys, kv_heads, batch, dev::kTile, 1) || !make_head_map(&p.v, type, v, head_size, keys, kv_heads, batch, dev::kTile, 1))
+      !make_head_map(&p.k, type, k, head_size, keys, kv_heads, batch, dev::kStep, 1) || !make_head_map(&p.v, type, v, head_size, keys, kv_heads, batch, dev::kStep, 1))
     return kErrArgument;
   cudaError_t e;
   if (type == kBf16) e = head_size <= 64 ? run_forward<__nv_bfloat16, 64>(p, plan, stream) : run_forward<__nv_bfloat16, 128>(p, plan, stream);
@@ -1157,8 +1097,10 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
   p.delta = delta;
   p.most = most;
   p.dq = dq, p.dk = dk, p.dv = dv;
-  if (!make_head_map(&p.q, type, q, head_size, queries, heads, batch, dev::kTile, 1) || !make_head_map(&p.dout, type, dout, head_size, queries, heads, batch, dev::kTile, 1) ||
-      !make_head_map(&p.k, type, k, head_size, keys, kv_heads, batch, dev::kTile, 1) || !make_head_map(&p.v, type, v, head_size, keys, kv_heads, batch, dev::kTile, 1))
+  const auto map = [&](CUtensorMap* m, const hc_heads& t, size_t length, size_t of, int rows) { return make_head_map(m, type, t, head_size, length, of, batch, rows, 1); };
+  if (!map(&p.q, q, queries, heads, dev::kStep) || !map(&p.q_tile, q, queries, heads, dev::kTile) || !map(&p.dout, dout, queries, heads, dev::kStep) ||
+      !map(&p.dout_tile, dout, queries, heads, dev::kTile) || !map(&p.k, k, keys, kv_heads, dev::kStep) || !map(&p.k_tile, k, keys, kv_heads, dev::kTile) ||
+      !map(&p.v, v, keys, kv_heads, dev::kStep) || !map(&p.v_tile, v, keys, kv_heads, dev::kTile))
     return kErrArgument;
   cudaError_t e;
   if (type == kBf16) e = head_size <= 64 ? run_backward<__nv_bfloat16, 64>(p, dout, v, out, delta, most, stream) : run_backward<__nv_bfloat16, 128>(p, dout, v, out, delta, most, stream);
