@@ -13,7 +13,7 @@
 // Forward: two tiles of queries share their keys, so that the tensor cores work on one while the other's exponentials are taken, which bound it up to heads of
 // 64 (16 a cycle and SM).  The reference that exponentials are taken relative to follows a row's largest score when that is more than 2^8 above it; only then is O
 // taken times a factor.  Few queries (with all heads of a key's head at most 128 rows, a new token of each text for one) are one tile, and the keys are shared
-// out to several CTAs, whose results a second kernel joins: bound by reading keys and values.
+// out to the CTAs of a cluster, which join their results over its shared memory: bound by reading keys and values.
 // Backward: dK and dV in a kernel whose CTA has a tile of keys and goes through the queries, dQ in one whose CTA has a tile of queries.  That forms the scores twice (7 products instead of 5), and
 // needs no atomic additions, whose order would change the result, and no array of partial dQ.
 //
@@ -33,6 +33,7 @@ namespace dev {
 
 constexpr int kTile = 128;  // rows of a tile, one a thread
 constexpr int kStep = 64;   // columns that are worked on at a time
+constexpr int kMostSplits = 8;  // CTAs of a cluster
 constexpr uint64_t kAttnLimitNs = 2000ull * 1000 * 1000;
 constexpr float kSlack = 8.0f;  // powers of two that a score may be above its row's reference
 
@@ -47,7 +48,7 @@ struct AttnShape {
   static constexpr int kResident = kD == 128 ? 1 : 2;
   static constexpr int kColumns = 512 / kResident;
   static constexpr int kSlots = kD == 128 ? 2 : 1;  // forward: steps of scores of a tile
-  static constexpr int kForwardStages = kD == 128 ? 10 : 8;  // steps of keys or of values
+  static constexpr int kForwardStages = kD == 128 ? 10 : 8;  // steps, half of them of keys and half of values
   static constexpr int kForwardSmem = 2 * kBytes + kForwardStages * kStepBytes + 1024;
   static constexpr int kForwardThreads = 32 * (4 + 8);
   static constexpr int kGroups = kD == 128 ? 2 : 1;  // backward: of eight warps, which take the steps in turn
@@ -61,8 +62,6 @@ struct AttnParams {
   CUtensorMap q_tile, k_tile, v_tile, dout_tile;  // in tiles of 128 (backward)
   void* o;
   float* less;      // [batch heads][rows]: minus the logarithm (base 2) of a query's sum of exponentials, for the backward pass
-  float* part_o;    // [split][query of all][head size], of the CTAs that share the keys out
-  float* part_less;
   float* delta;  // as `less`
   void *dq, *dk, *dv;
   const unsigned int* most;  // bits of max|dO_i|, max|V_j| (fp16)
@@ -70,7 +69,7 @@ struct AttnParams {
   int batch, heads, kv_heads, group, tq, tk, d, off, window, sinks;
   int packed;   // rows of the one tile that holds the queries of all heads of a key's head, or 0
   int blocks;   // of queries, or of keys
-  int splits;
+  int splits;   // CTAs of a cluster that share the keys (forward) or the heads (dK and dV) of a tile
   float scale, scale2;  // scale2: times log2(e)
 };
 
@@ -148,11 +147,11 @@ __device__ __forceinline__ bool elected() {
       : "=r"(is));
   return is != 0;
 }
-__device__ __forceinline__ void attn_commit(uint64_t* bar) {
-  if (elected()) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void attn_commit(bool leader, uint64_t* bar) {
+  if (leader) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void attn_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  if (elected())
+__device__ __forceinline__ void attn_mma(bool leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  if (leader)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.u32 p, %4, 0;\n\t"
@@ -161,8 +160,8 @@ __device__ __forceinline__ void attn_mma(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 // the first operand in tensor memory: rows in lanes, two values of the sum in a column
-__device__ __forceinline__ void attn_mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  if (elected())
+__device__ __forceinline__ void attn_mma_from_tmem(bool leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  if (leader)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.u32 p, %4, 0;\n\t"
@@ -186,21 +185,40 @@ template <typename T>
 __device__ __forceinline__ uint32_t attn_idesc(int n, bool b_across) {
   return 1u << 4 | operand_format<T>() << 7 | operand_format<T>() << 10 | (b_across ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(kTile / 16) << 24;
 }
-// d = a b^T over the head's values, of a tile and a step
+// d = a b^T over the head's values, of a tile and a step (their descriptors along the sum)
 template <typename T, int kD>
-__device__ __forceinline__ void scores(uint32_t d, const unsigned char* a, const unsigned char* b) {
-  const uint64_t da = along(a), db = along(b);
+__device__ __forceinline__ void scores(bool leader, uint32_t d, uint64_t a, uint64_t b) {
   const uint32_t idesc = attn_idesc<T>(kStep, false);
 #pragma unroll
-  for (int i = 0; i < kD / 16; ++i) attn_mma(d, da + (i / 4) * (kTile * 128 / 16) + (i % 4) * 2, db + (i / 4) * (kStep * 128 / 16) + (i % 4) * 2, idesc, i > 0);
+  for (int i = 0; i < kD / 16; ++i) attn_mma(leader, d, a + (i / 4) * (kTile * 128 / 16) + (i % 4) * 2, b + (i / 4) * (kStep * 128 / 16) + (i % 4) * 2, idesc, i > 0);
 }
-// d (+)= p b, p in tensor memory, its second 32 values of the sum `second` columns behind the first, b a step
+// d (+)= p b, p in tensor memory, its second 32 values of the sum `second` columns behind the first, b a step (its descriptor across the sum)
 template <typename T, int kD>
-__device__ __forceinline__ void weighted(uint32_t d, uint32_t p, int second, const unsigned char* b, bool add) {
-  const uint64_t db = across(b);
+__device__ __forceinline__ void weighted(bool leader, uint32_t d, uint32_t p, int second, uint64_t b, bool add) {
   const uint32_t idesc = attn_idesc<T>(kD, true);
 #pragma unroll
-  for (int i = 0; i < kStep / 16; ++i) attn_mma_from_tmem(d, p + i / 2 * second + i % 2 * 8, db + i * 128, idesc, add || i > 0);
+  for (int i = 0; i < kStep / 16; ++i) attn_mma_from_tmem(leader, d, p + i / 2 * second + i % 2 * 8, b + i * 128, idesc, add || i > 0);
+}
+
+// ---- clusters -----------------------------------------------------------------------------------------------------------------
+// All threads of all CTAs of a cluster come to both of these, in any case; `all`: the cluster's size.
+__device__ __forceinline__ void cluster_meet(int all) {
+  if (all > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 peer_load4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float peer_load(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
 }
 
 // ---- what is seen ------------------------------------------------------------------------------------------------------------
@@ -218,8 +236,20 @@ __device__ __forceinline__ KeySteps key_steps(const AttnParams& p, int p0, int p
   t.count = t.sinks + p1 / kStep - t.low + 1;
   return t;
 }
-// of a step of keys from k0 on
-__device__ __forceinline__ bool any_seen(const AttnParams& p, int p0, int p1, int k0) { return k0 <= p1 && (k0 + kStep - 1 > p0 - p.window || k0 < p.sinks); }
+// Which of a list's steps positions p0 to p1, some of those that it was made for, see something of: those below `first`, and from `from` up to below `to`.
+struct StepsSeen {
+  int first, from, to;
+  __device__ __forceinline__ bool has(int e) const { return e < first || (e >= from && e < to); }
+};
+__device__ __forceinline__ StepsSeen steps_seen(const AttnParams& p, const KeySteps& list, int p0, int p1) {
+  if (p1 < 0) return {0, 0, 0};
+  const int shift = list.sinks - list.low, lowest = p0 - p.window + 1;
+  StepsSeen s;
+  s.to = p1 / kStep + shift + 1;
+  s.from = (lowest > 0 ? lowest / kStep : 0) + shift;
+  s.first = min(max(list.sinks, (p.sinks + kStep - 1) / kStep + shift), s.to);
+  return s;
+}
 // of `keys` keys from k0 on
 __device__ __forceinline__ bool all_seen(const AttnParams& p, int p0, int p1, int k0, int keys) { return k0 + keys - 1 <= p0 && (p1 - k0 < p.window || k0 + keys <= p.sinks); }
 
@@ -321,6 +351,11 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
   __shared__ AttnBarriers sh;
   unsigned char* tiles = attn_tiles(raw);
   unsigned char* ring = tiles + 2 * S::kBytes;
+  // what the CTAs of a cluster join lies where the operands were
+  constexpr int kRow = kD + 4;  // floats from row to row, so that neighbours' pieces do not meet in a bank
+  static_assert(2 * kTile * (kRow + 1) * 4 <= S::kForwardSmem - 1024, "room for the parts");
+  float *joined = reinterpret_cast<float*>(tiles), *part_less = joined + 2 * kTile * kRow;
+  const bool shared = p.packed || p.splits > 1;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // the blocks of queries that see most come first
   const int heads = p.packed ? p.kv_heads : p.heads;
@@ -336,17 +371,19 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
   int p0[2], p1[2];
   for (int q = 0; q < 2; ++q) {
     const int i0 = first + q * kTile, i1 = min(i0 + kTile, p.tq) - 1;
-    const bool there = i0 <= i1 && (q == 0 || !p.packed);
-    p0[q] = p.off + i0;
-    p1[q] = there ? p.off + (p.packed ? p.tq - 1 : i1) : -1;
+    p0[q] = p.packed ? p.off : p.off + i0;
+    p1[q] = p.packed ? p.off + p.tq - 1 : i0 <= i1 ? p.off + i1 : -1;
   }
   const KeySteps list = key_steps(p, p0[0], max(p1[0], p1[1]));
   const int e0 = (int)((int64_t)list.count * split / p.splits), e1 = (int)((int64_t)list.count * (split + 1) / p.splits);
-  attn_begin<S::kColumns>(sh, 8, 4, 2);
+  // One tile of queries is worked on twice, with every second step of the keys each.
+  attn_begin<S::kColumns>(sh, 8, 4, p.packed ? 1 : 2);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  constexpr int kRing = kStages / 2;  // of keys; behind it that of values
+  unsigned char* v_ring = ring + kRing * S::kStepBytes;
   if (warp == 0) {
     if (lane == 0 && e0 < e1) {
-      Ring<kStages> r;
+      Ring<kRing> rk, rv;
       const bool second = !p.packed && first + kTile < p.tq;
       if (p.packed) {
         mbar_expect_tx(&sh.first, p.packed * 128 * S::kBoxes);
@@ -356,72 +393,85 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
         load_rows<kD, kTile>(tiles, &p.q, first, head, b, &sh.first);
         if (second) load_rows<kD, kTile>(tiles + S::kBytes, &p.q, first + kTile, head, b, &sh.first);
       }
-      const auto load = [&](const CUtensorMap* map, int e) {
-        if (!attn_wait(&sh.empty[r.s], r.phase ^ 1, sh)) return false;
-        mbar_expect_tx(&sh.full[r.s], S::kStepBytes);
-        load_rows<kD, kStep>(ring + r.s * S::kStepBytes, map, list.at(e), kv_head, b, &sh.full[r.s]);
-        r.next();
-        return true;
-      };
-      // in the order in which they are used
-      bool ok = true;
-      for (int e = e0; ok && e < min(e0 + kSlots, e1); ++e) ok = load(&p.k, e);
-      for (int e = e0; ok && e < e1; ++e) ok = load(&p.v, e) && (e + kSlots >= e1 || load(&p.k, e + kSlots));
-      ring_end(sh.full, r);
+      for (int e = e0; e < e1; ++e) {
+        const int k0 = list.at(e);
+        if (!attn_wait(&sh.empty[rk.s], rk.phase ^ 1, sh)) break;
+        mbar_expect_tx(&sh.full[rk.s], S::kStepBytes);
+        load_rows<kD, kStep>(ring + rk.s * S::kStepBytes, &p.k, k0, kv_head, b, &sh.full[rk.s]);
+        rk.next();
+        if (!attn_wait(&sh.empty[8 + rv.s], rv.phase ^ 1, sh)) break;
+        mbar_expect_tx(&sh.full[8 + rv.s], S::kStepBytes);
+        load_rows<kD, kStep>(v_ring + rv.s * S::kStepBytes, &p.v, k0, kv_head, b, &sh.full[8 + rv.s]);
+        rv.next();
+      }
+      ring_end(sh.full, rk);
+      ring_end(sh.full + 8, rv);
       mbar_wait_bounded(&sh.first, 0, kAttnLimitNs);
     }
   } else if (warp <= 2) {
     if (e0 < e1) {
-      const int q = warp - 1;
-      Ring<kStages> r;  // of what is waited for next
+      const int q = warp - 1, by = p.packed ? 2 : 1;
+      const bool leader = elected();
+      const StepsSeen seen = p.packed ? StepsSeen{e1, 0, 0} : steps_seen(p, list, p0[q], p1[q]);
+      const uint64_t q_at = along(tiles + (p.packed ? 0 : q * S::kBytes)), k_at = along(ring), v_at = across(v_ring);
+      constexpr int kUnits = S::kStepBytes / 16;
       int scored = 0, summed = 0;
+      Ring<kRing> rk, rv;
+      const int start = p.packed ? e0 + ((e0 ^ q) & 1) : e0;  // its first step
+      if (start != e0) {
+        rk.next();
+        rv.next();
+      }
       const auto score = [&](int e) {
-        if (!attn_wait_all(&sh.full[r.s], r.phase, sh)) return false;
-        if (any_seen(p, p0[q], p1[q], list.at(e))) {
+        if (!attn_wait_all(&sh.full[rk.s], rk.phase, sh)) return false;
+        if (seen.has(e)) {
           const int n = scored++, slot = q * kSlots + n % kSlots;
           if (n >= kSlots && !attn_wait_all(&sh.done[slot], (n / kSlots - 1) & 1, sh)) return false;  // the probabilities that lie there have been read
           tc_fence_after();
-          scores<T, kD>(tmem + slot * kStep, tiles + q * S::kBytes, ring + r.s * S::kStepBytes);
-          attn_commit(&sh.s_full[slot]);
+          scores<T, kD>(leader, tmem + slot * kStep, q_at, k_at + rk.s * kUnits);
+          attn_commit(leader, &sh.s_full[slot]);
         }
-        attn_commit(&sh.empty[r.s]);
-        r.next();
+        attn_commit(leader, &sh.empty[rk.s]);
+        rk.next();
+        if (by == 2) rk.next();
         return true;
       };
       const auto sum = [&](int e) {
-        if (!attn_wait_all(&sh.full[r.s], r.phase, sh)) return false;
-        if (any_seen(p, p0[q], p1[q], list.at(e))) {
+        if (!attn_wait_all(&sh.full[8 + rv.s], rv.phase, sh)) return false;
+        if (seen.has(e)) {
           const int n = summed++, slot = q * kSlots + n % kSlots;
           if (!attn_wait_all(&sh.p_ready[slot], (n / kSlots) & 1, sh)) return false;
           tc_fence_after();
-          weighted<T, kD>(tmem + kO + q * kD, tmem + slot * kStep, 16, ring + r.s * S::kStepBytes, n > 0);
-          attn_commit(&sh.done[slot]);
+          weighted<T, kD>(leader, tmem + kO + q * kD, tmem + slot * kStep, 16, v_at + rv.s * kUnits, n > 0);
+          attn_commit(leader, &sh.done[slot]);
         }
-        attn_commit(&sh.empty[r.s]);
-        r.next();
+        attn_commit(leader, &sh.empty[8 + rv.s]);
+        rv.next();
+        if (by == 2) rv.next();
         return true;
       };
       bool ok = attn_wait_all(&sh.first, 0, sh);
-      for (int e = e0; ok && e < min(e0 + kSlots, e1); ++e) ok = score(e);
-      for (int e = e0; ok && e < e1; ++e) ok = sum(e) && (e + kSlots >= e1 || score(e + kSlots));
-      attn_commit(&sh.drained);  // matrix instructions in flight are done before the CTA leaves
+      int ahead = start;  // the next step whose scores are formed
+      for (int n = 0; ok && n < kSlots && ahead < e1; ++n, ahead += by) ok = score(ahead);
+      for (int e = start; ok && e < e1; e += by, ahead += by) ok = sum(e) && (ahead >= e1 || score(ahead));
+      attn_commit(leader, &sh.drained);  // matrix instructions in flight are done before the CTA leaves
       if (lane == 0) mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3, q = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), o_at = lanes + kO + q * kD;
     const int i = p.packed ? row % p.tq : first + q * kTile + row;
-    const bool in = p.packed ? q == 0 && row < p.packed : i < p.tq;
+    const bool in = p.packed ? row < p.packed : i < p.tq;
     const bool some = __any_sync(0xffffffffu, in);
     const int h = p.packed ? head * p.group + row / p.tq : head, position = p.off + i;
     const float slack = kSlack / p.scale2;
     float most = -INFINITY, sum = 0.0f, ref = 0.0f;
     int taken = 0;
     bool ok = true;
-    for (int e = e0; ok && e < e1; ++e) {
-      const int k0 = list.at(e);
-      if (!any_seen(p, p0[q], p1[q], k0)) continue;
-      const int slot = q * kSlots + taken % kSlots;
+    const StepsSeen seen_steps = p.packed ? StepsSeen{e1, 0, 0} : steps_seen(p, list, p0[q], p1[q]);
+    for (int e = p.packed ? e0 + ((e0 ^ q) & 1) : e0; ok && e < e1; e += p.packed ? 2 : 1) {
+      if (!seen_steps.has(e)) continue;
+      const int k0 = list.at(e), slot = q * kSlots + taken % kSlots;
       const uint32_t s_at = lanes + slot * kStep;
       ok = attn_wait_all(&sh.s_full[slot], (taken / kSlots) & 1, sh);
       if (!ok) break;
@@ -509,56 +559,58 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
       const bool none = sum == 0.0f;  // (a NaN is not)
       const float factor = none ? 0.0f : 1.0f / sum;
       const int64_t head_at = (int64_t)b * p.heads + h;
-      if (p.part_o) {
-        const int64_t all = (int64_t)p.batch * p.heads * p.tq, query = head_at * p.tq + i;
-        store_row<float, kD>(o_at, p.part_o + (split * all + query) * p.d, p.d, factor, in, taken > 0, none);
-        if (in) p.part_less[split * all + query] = none ? INFINITY : -(ref + log2f(sum));
+      if (shared) {
+        store_row<float, kD>(o_at, joined + (q * kTile + row) * kRow, kD, factor, in, taken > 0, none);
+        if (in) part_less[q * kTile + row] = none ? INFINITY : -(ref + log2f(sum));
       } else {
         store_row<T, kD>(o_at, static_cast<T*>(p.o) + (((int64_t)b * p.tq + i) * p.heads + h) * p.d, p.d, factor, in, taken > 0, none);
         if (in && p.less) p.less[head_at * p.less_ld + i] = none ? -INFINITY : -(ref + log2f(sum));
       }
     }
+    if (!ok && shared && in) part_less[q * kTile + row] = __int_as_float(0x7fc00000);  // a wait ran out: no numbers
   }
   attn_end<S::kColumns>(tmem);
-}
-
-// Joins the results of CTAs that shared the keys out: a warp a query and head.
-template <typename T>
-__global__ void __launch_bounds__(256) hc_attention_join_kernel(const float* part_o, const float* part_less, int splits, int64_t queries, int tq, int heads, int d, T* o, float* less,
-                                                                int64_t less_ld) {
-  const int lane = threadIdx.x & 31;
-  const int64_t query = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  if (query >= queries) return;
-  // minus a split's logarithm, +inf where it has seen nothing: the least of them is the reference
-  float least = INFINITY;
-  bool bad = false;
-  for (int s = lane; s < splits; s += 32) {
-    const float v = part_less[s * queries + query];
-    least = fminf(least, v);
-    bad = bad || v != v;
-  }
+  if (!shared) return;
+  // O = sum of the parts' O times 2^(their logarithm), over the sum of those; four columns of a row a thread, the rows' pieces go round the CTAs
+  cluster_meet(p.splits);
+  const int halves = p.packed ? 2 : 1, rows = p.packed ? p.packed : min(2 * kTile, p.tq - first), all = p.splits * halves;
+  for (int n = threadIdx.x * p.splits + split; n < rows * (kD / 4); n += S::kForwardThreads * p.splits) {
+    const int row = n / (kD / 4), c = n % (kD / 4) * 4;
+    const auto lies = [&](int k) { return row + (p.packed ? k % 2 * kTile : 0); };  // part k's row in its CTA
+    const auto rank = [&](int k) { return p.packed ? k / 2 : k; };
+    float least = INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float theirs[2 * kMostSplits];  // loads are on their way together
+    bool bad = false;
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, k));
-  bad = __any_sync(0xffffffffu, bad);
-  const bool none = least == INFINITY && !bad;
-  float sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; !none && s < splits; ++s) {
-    const float theirs = part_less[s * queries + query];
-    const float weight = theirs == INFINITY ? 0.0f : exp2f(least - theirs);
-    sum += weight;
-    if (lane * 4 < d && theirs != INFINITY) {
-      const float4 w = *reinterpret_cast<const float4*>(part_o + (s * queries + query) * d + lane * 4);
-      v[0] += weight * w.x, v[1] += weight * w.y, v[2] += weight * w.z, v[3] += weight * w.w;
+    for (int k = 0; k < 2 * kMostSplits; ++k) theirs[k] = k < all ? peer_load(peer_address(part_less + lies(k), rank(k))) : INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2 * kMostSplits; ++k) {
+      least = fminf(least, theirs[k]);
+      bad = bad || theirs[k] != theirs[k];
     }
+    const bool none = least == INFINITY && !bad;
+#pragma unroll
+    for (int k0 = 0; k0 < 2 * kMostSplits; k0 += 4) {
+      if (k0 >= all) break;
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = k0 + k < all ? peer_load4(peer_address(joined + lies(k0 + k) * kRow + c, rank(k0 + k))) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (theirs[k0 + k] == INFINITY) continue;
+        const float weight = power2(least - theirs[k0 + k]);
+        sum += weight;
+        v[0] += weight * x[k].x, v[1] += weight * x[k].y, v[2] += weight * x[k].z, v[3] += weight * x[k].w;
+      }
+    }
+    const float factor = none ? 0.0f : 1.0f / sum;
+    const int i = p.packed ? row % p.tq : first + row, h = p.packed ? head * p.group + row / p.tq : head;
+    if (c < p.d)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (((int64_t)b * p.tq + i) * p.heads + h) * p.d + c) =
+          make_uint2(pack2<T>(v[0] * factor, v[1] * factor), pack2<T>(v[2] * factor, v[3] * factor));
+    if (c == 0 && p.less) p.less[((int64_t)b * p.heads + h) * p.less_ld + i] = none ? -INFINITY : least - log2f(sum);
   }
-  const float factor = none ? 0.0f : 1.0f / sum;
-  const int64_t head = query / tq, b = head / heads;
-  const int i = (int)(query - head * tq);
-  if (lane * 4 < d) {
-    uint2 w = make_uint2(pack2<T>(v[0] * factor, v[1] * factor), pack2<T>(v[2] * factor, v[3] * factor));
-    *reinterpret_cast<uint2*>(o + ((b * tq + i) * heads + head % heads) * d + lane * 4) = w;
-  }
-  if (less && lane == 0) less[head * less_ld + i] = none ? -INFINITY : bad ? least + __int_as_float(0x7fc00000) : least - log2f(sum);
+  cluster_meet(p.splits);  // nobody leaves while its shared memory is read
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
@@ -651,9 +703,15 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   __shared__ float lacking[kParts][kTile];
   unsigned char *tile1 = attn_tiles(raw), *tile2 = tile1 + S::kBytes, *ring = tile2 + S::kBytes;
   float* sides = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // of a step of queries: less, delta
+  // what the CTAs of a cluster join lies where the operands were: dV and dK side by side
+  constexpr int kRow = 2 * kD + 4;
+  static_assert(kTile * kRow * 4 <= S::kBackwardSmem - 1024, "room for the parts");
+  float* joined = reinterpret_cast<float*>(tile1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int heads = kKeys ? p.kv_heads : p.heads;
   int64_t at = blockIdx.x;
+  const int rank = kKeys ? (int)(at % p.splits) : 0;  // in a cluster that shares a tile of keys' query heads out
+  if (kKeys) at /= p.splits;
   const int head = (int)(at % heads);
   at /= heads;
   const int b = (int)(at % p.batch), block = kKeys ? (int)(at / p.batch) : p.blocks - 1 - (int)(at / p.batch);
@@ -664,7 +722,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   const int q_steps = q_last >= max(t0 - p.off, 0) ? q_last / kStep - q_first + 1 : 0;
   const int p0 = p.off + t0, p1 = p.off + min(t0 + kTile, p.tq) - 1;
   const KeySteps list = kKeys ? KeySteps{0, 0, 0} : key_steps(p, p0, p1);
-  const int count = kKeys ? q_steps * p.group : list.count;
+  const int own_heads = p.group / p.splits, count = kKeys ? q_steps * own_heads : list.count;
   attn_begin<S::kColumns>(sh, 8 * kGroups, 8, 1);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   if (warp == 0) {
@@ -673,7 +731,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
       mbar_expect_tx(&sh.first, 2 * S::kBytes);
       load_rows<kD, kTile>(tile1, kKeys ? &p.k_tile : &p.q_tile, t0, head, b, &sh.first);
       load_rows<kD, kTile>(tile2, kKeys ? &p.v_tile : &p.dout_tile, t0, head, b, &sh.first);
-      int h = kKeys ? head * p.group : head / p.group, step = 0;
+      int h = kKeys ? head * p.group + rank * own_heads : head / p.group, step = 0;
       for (int e = 0; e < count; ++e) {
         if (!attn_wait(&sh.empty[r.s], r.phase ^ 1, sh)) break;
         const int at0 = kKeys ? (q_first + step) * kStep : list.at(e);
@@ -697,8 +755,10 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     }
   } else if (warp <= 2) {
     if (count) {
-      // a step's place in the ring; what is waited for the k-th time has parity k & 1
-      const auto stage = [&](int e) { return ring + e % kStages * kStageBytes; };
+      // what is waited for the k-th time has parity k & 1
+      const bool leader = elected();
+      constexpr int kUnits = kStageBytes / 16, kSecond = S::kStepBytes / 16;
+      const uint64_t tile1_at = along(tile1), tile2_at = along(tile2), ring_along = along(ring), ring_across = across(ring);
       bool ok = true;
       if (warp == 1) {
         ok = attn_wait_all(&sh.first, 0, sh);
@@ -708,22 +768,22 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
           ok = attn_wait_all(&sh.full[e % kStages], (e / kStages) & 1, sh) && (e < kGroups || attn_wait_all(&sh.done[g], before, sh));
           if (!ok) break;
           tc_fence_after();
-          scores<T, kD>(tmem + g * kStep, tile1, stage(e));
-          attn_commit(&sh.s_full[g]);
+          scores<T, kD>(leader, tmem + g * kStep, tile1_at, ring_along + e % kStages * kUnits);
+          attn_commit(leader, &sh.s_full[g]);
           ok = e < kGroups || attn_wait_all(&sh.ds_done[g], before, sh);
           if (!ok) break;
           tc_fence_after();
-          scores<T, kD>(tmem + kDp + g * kStep, tile2, stage(e) + S::kStepBytes);
-          attn_commit(&sh.dp_full[g]);
+          scores<T, kD>(leader, tmem + kDp + g * kStep, tile2_at, ring_along + e % kStages * kUnits + kSecond);
+          attn_commit(leader, &sh.dp_full[g]);
         }
       } else {
         const auto second_sum = [&](int e) {
           const int g = e % kGroups;
           if (!attn_wait_all(&sh.ds_ready[g], (e / kGroups) & 1, sh)) return false;
           tc_fence_after();
-          weighted<T, kD>(tmem + kSum2, tmem + kDp + g * kStep, 32, stage(e), e > 0);
-          attn_commit(&sh.ds_done[g]);
-          attn_commit(&sh.empty[e % kStages]);  // all four products of the step are done then
+          weighted<T, kD>(leader, tmem + kSum2, tmem + kDp + g * kStep, 32, ring_across + e % kStages * kUnits, e > 0);
+          attn_commit(leader, &sh.ds_done[g]);
+          attn_commit(leader, &sh.empty[e % kStages]);  // all four products of the step are done then
           return true;
         };
         for (int e = 0; ok && e < count; ++e) {
@@ -731,13 +791,13 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
           ok = attn_wait_all(&sh.full[e % kStages], (e / kStages) & 1, sh) && attn_wait_all(&sh.p_ready[g], (e / kGroups) & 1, sh);
           if (!ok) break;
           tc_fence_after();
-          weighted<T, kD>(tmem + kSum1, tmem + g * kStep, 32, stage(e) + (kKeys ? S::kStepBytes : 0), e > 0);
-          attn_commit(&sh.done[g]);
+          weighted<T, kD>(leader, tmem + kSum1, tmem + g * kStep, 32, ring_across + e % kStages * kUnits + (kKeys ? kSecond : 0), e > 0);
+          attn_commit(leader, &sh.done[g]);
           ok = e < kGroups - 1 || second_sum(e - (kGroups - 1));
         }
         for (int e = count - min(kGroups - 1, count); ok && e < count; ++e) ok = second_sum(e);
       }
-      attn_commit(&sh.drained);
+      attn_commit(leader, &sh.drained);
       if (lane == 0) mbar_wait_bounded(&sh.drained, 0, kAttnLimitNs);
     }
   } else if (warp >= 4) {
@@ -856,9 +916,15 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
       // 64 of the columns of dV and dK each
       const bool second = part * 64 >= kD;
       const int c = part * 64 % kD;
+      if (p.splits > 1) {
+        store_row<float, 64>(lanes + kSum1 + part * 64, joined + row * kRow + part * 64, 64, 1.0f, true, count > 0, false);
+      } else {
       T* to = static_cast<T*>(second ? p.dk : p.dv) + (((int64_t)b * p.tk + t) * p.kv_heads + head) * p.d + c;
       store_row<T, 64>(lanes + kSum1 + part * 64, to, p.d - c, second ? p.scale * back : kF16 ? 1.0f / 16384.0f : 1.0f, in, count > 0, false);
+      }
     }
+    if (!ok && kKeys && p.splits > 1)  // a wait ran out: no numbers
+      for (int c = 0; c < 64; ++c) joined[row * kRow + part * 64 + c] = __int_as_float(0x7fc00000);
     if (ok && !kKeys) {
       lacking[part][row] = both(lacks) * back;
       __syncwarp();
@@ -893,6 +959,26 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     }
   }
   attn_end<S::kColumns>(tmem);
+  if (!kKeys || p.splits == 1) return;
+  cluster_meet(p.splits);
+  const float back = kF16 ? ds_power(p.most, -1) : 1.0f;
+  for (int n = threadIdx.x * p.splits + rank; n < min(kTile, p.tk - t0) * (kD / 4); n += S::kBackwardThreads * p.splits) {
+    const int row = n / (kD / 4), column = n % (kD / 4) * 8;  // of dV and dK side by side
+    const bool second = column >= kD;
+    const int c = second ? column - kD : column;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // a pair
+      const uint32_t from = peer_address(joined + row * kRow + column, k);
+      const float4 x = peer_load4(from), y = peer_load4(from + 16);
+      v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+    const float factor = second ? p.scale * back : kF16 ? 1.0f / 16384.0f : 1.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= factor;
+    if (c < p.d) store8(static_cast<T*>(second ? p.dk : p.dv) + (((int64_t)b * p.tk + t0 + row) * p.kv_heads + head) * p.d + c, v);
+  }
+  cluster_meet(p.splits);
 }
 
 }  // namespace dev
@@ -928,7 +1014,8 @@ bool heads_ok(const hc_heads& t, size_t d, size_t length, size_t heads, size_t b
 
 int64_t attn_sms() { return device_info().sms > 0 ? device_info().sms : 1; }
 
-// Into how many CTAs the keys of a tile of queries are shared out, where there are fewer of those than SMs: a CTA costs some three tiles besides its own, joining a part one.
+// Into how many CTAs (a cluster of up to eight) the keys of a tile of queries are shared out where there are fewer tiles than SMs take: a CTA costs some four steps of 64 keys besides its own,
+// joining two more.
 struct Plan {
   int packed, blocks, splits;
 };
@@ -937,19 +1024,43 @@ Plan plan_of(const Sizes& s, size_t window, size_t sinks) {
   const size_t group = s.heads / s.kv_heads;
   p.packed = s.queries * group <= 128 ? (int)(s.queries * group) : 0;
   p.blocks = p.packed ? 1 : (int)((s.queries + 255) / 256);
-  const int64_t ctas = (int64_t)s.batch * (p.packed ? s.kv_heads : s.heads) * p.blocks, sms = attn_sms();
-  const size_t seen = window ? (window + sinks + s.queries < s.keys ? window + sinks + s.queries : s.keys) : s.keys;
-  const int64_t tiles = (int64_t)(seen + 127) / 128;
+  const int64_t ctas = (int64_t)s.batch * (p.packed ? s.kv_heads : s.heads) * p.blocks, slots = attn_sms() * (s.d > 64 ? 1 : 2);
+  const size_t seen = window && window + sinks + 256 < s.keys ? window + sinks + 256 : s.keys;
+  const int64_t steps = (int64_t)(seen + 63) / 64;
   p.splits = 1;
-  int64_t least = (ctas + sms - 1) / sms * (tiles + 3);
-  for (int n = 2; n <= 64 && n <= tiles && ctas < sms * 2; ++n) {
-    const int64_t cost = (ctas * n + sms - 1) / sms * ((tiles + n - 1) / n + 3) + 1 + n / 16;
+  int64_t least = (ctas + slots - 1) / slots * (steps + 4);
+  for (int n = 2; n <= 8 && n <= steps && ctas < slots; n *= 2) {
+    const int64_t cost = (ctas * n + slots - 1) / slots * ((steps + n - 1) / n + 4) + 2;
     if (cost < least) {
       least = cost;
       p.splits = n;
     }
   }
   return p;
+}
+// Whether the query heads that share a tile of keys are shared out to a pair of CTAs: where there are fewer than eight tiles for each place, so that the last ones to end weigh little (16 heads on 4,
+// 8192 positions of 128 values: 1038 us for both passes instead of 1091; with clusters of four, which do not fill the GPU, 1260).
+int kv_splits(const Sizes& s) {
+  const size_t group = s.heads / s.kv_heads, tiles = s.batch * s.kv_heads * ((s.keys + 127) / 128), slots = (size_t)attn_sms() * (s.d > 64 ? 1 : 2);
+  return group % 2 == 0 && tiles < slots * 8 ? 2 : 1;
+}
+
+template <typename K>
+cudaError_t launch_clusters(K kernel, int64_t ctas, int size, int threads, int smem, cudaStream_t stream, const dev::AttnParams& p) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  memset(&attr, 0, sizeof(attr));
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)size;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = size > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 size_t stats_ld(size_t queries) { return up(queries, 128); }
@@ -966,18 +1077,13 @@ void fill_attention(dev::AttnParams* p, const Sizes& s, size_t window, size_t si
 }
 
 template <typename T, int kD>
-cudaError_t run_forward(const dev::AttnParams& p, const Plan& plan, cudaStream_t stream) {
+cudaError_t run_forward(const dev::AttnParams& p, cudaStream_t stream) {
   static unsigned long long allowed = 0;
   constexpr int smem = dev::AttnShape<kD>::kForwardSmem;
-  cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed);
+  const cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t ctas = (int64_t)p.batch * (p.packed ? p.kv_heads : p.heads) * p.blocks * p.splits;
-  dev::hc_attention_kernel<T, kD><<<(unsigned)ctas, dev::AttnShape<kD>::kForwardThreads, smem, stream>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || plan.splits == 1) return e;
-  const int64_t queries = (int64_t)p.batch * p.heads * p.tq;
-  dev::hc_attention_join_kernel<T><<<(unsigned)((queries + 7) / 8), 256, 0, stream>>>(p.part_o, p.part_less, p.splits, queries, p.tq, p.heads, p.d, static_cast<T*>(p.o), p.less, p.less_ld);
-  return cudaGetLastError();
+  return launch_clusters(dev::hc_attention_kernel<T, kD>, ctas, p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, p);
 }
 
 template <typename T, int kD>
@@ -998,20 +1104,16 @@ cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_head
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // dq or not: the keys' pass needs the delta that this one completes
+  const int splits = p.splits;
+  p.splits = 1;
   p.blocks = (p.tq + dev::kTile - 1) / dev::kTile;
-  dev::hc_attention_backward_kernel<T, kD, false><<<(unsigned)((int64_t)p.batch * p.heads * p.blocks), dev::AttnShape<kD>::kBackwardThreads, smem, stream>>>(p);
-  if (p.dk) {
-    p.blocks = (p.tk + dev::kTile - 1) / dev::kTile;
-    dev::hc_attention_backward_kernel<T, kD, true><<<(unsigned)((int64_t)p.batch * p.kv_heads * p.blocks), dev::AttnShape<kD>::kBackwardThreads, smem, stream>>>(p);
-  }
-  return cudaGetLastError();
+  e = launch_clusters(dev::hc_attention_backward_kernel<T, kD, false>, (int64_t)p.batch * p.heads * p.blocks, 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p);
+  if (e != cudaSuccess || !p.dk) return e;
+  p.splits = splits;
+  p.blocks = (p.tk + dev::kTile - 1) / dev::kTile;
+  return launch_clusters(dev::hc_attention_backward_kernel<T, kD, true>, (int64_t)p.batch * p.kv_heads * p.blocks * splits, splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p);
 }
 
-size_t forward_bytes(const Sizes& s, size_t window, size_t sinks) {
-  const Plan plan = plan_of(s, window, sinks);
-  const size_t rows = s.batch * s.heads * s.queries;
-  return plan.splits > 1 ? up(rows * plan.splits * s.d * sizeof(float), 256) + up(rows * plan.splits * sizeof(float), 256) : 0;
-}
 size_t backward_bytes(const Sizes& s) { return up(s.batch * s.heads * stats_ld(s.queries) * sizeof(float), 256) + 256; }
 
 }  // namespace
@@ -1024,13 +1126,8 @@ extern "C" {
 
 size_t hc_attention_stats(size_t batch, size_t heads, size_t queries) { return batch * heads * hc::stats_ld(queries); }
 
-size_t hc_attention_bytes(size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size, size_t window, size_t sinks) {
-  const hc::Sizes s = {batch, heads, kv_heads, queries, keys, head_size};
-  return hc::sizes_ok(s) && batch && queries && keys ? hc::forward_bytes(s, window, sinks) : 0;
-}
-
 int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float* stats, size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size,
-                 size_t window, size_t sinks, float scale, void* scratch, size_t scratch_bytes, hc_stream_t stream) {
+                 size_t window, size_t sinks, float scale, hc_stream_t stream) {
   using namespace hc;
   const Sizes s = {batch, heads, kv_heads, queries, keys, head_size};
   if ((type != kBf16 && type != kF16) || !sizes_ok(s) || !(scale > 0.0f) || !(scale < INFINITY) || !lies_at(out, 16) || !lies_at(stats, 16)) return kErrArgument;
@@ -1042,8 +1139,6 @@ int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float*
   }
   if (!heads_ok(q, head_size, queries, heads, batch) || !heads_ok(k, head_size, keys, kv_heads, batch) || !heads_ok(v, head_size, keys, kv_heads, batch)) return kErrArgument;
   const Plan plan = plan_of(s, window, sinks);
-  const size_t need = forward_bytes(s, window, sinks), rows = batch * heads * queries;
-  if (need && (!scratch || !lies_at(scratch, 256) || scratch_bytes < need)) return kErrArgument;
   dev::AttnParams p;
   fill_attention(&p, s, window, sinks, scale);
   p.packed = plan.packed;
@@ -1051,16 +1146,12 @@ int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float*
   p.splits = plan.splits;
   p.o = out;
   p.less = stats;
-  if (plan.splits > 1) {
-    p.part_o = static_cast<float*>(scratch);
-    p.part_less = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + up(rows * plan.splits * head_size * sizeof(float), 256));
-  }
   if (!make_head_map(&p.q, type, q, head_size, queries, heads, batch, plan.packed ? (int)queries : dev::kTile, plan.packed ? p.group : 1) ||
       !make_head_map(&p.k, type, k, head_size, keys, kv_heads, batch, dev::kStep, 1) || !make_head_map(&p.v, type, v, head_size, keys, kv_heads, batch, dev::kStep, 1))
     return kErrArgument;
   cudaError_t e;
-  if (type == kBf16) e = head_size <= 64 ? run_forward<__nv_bfloat16, 64>(p, plan, stream) : run_forward<__nv_bfloat16, 128>(p, plan, stream);
-  else e = head_size <= 64 ? run_forward<__half, 64>(p, plan, stream) : run_forward<__half, 128>(p, plan, stream);
+  if (type == kBf16) e = head_size <= 64 ? run_forward<__nv_bfloat16, 64>(p, stream) : run_forward<__nv_bfloat16, 128>(p, stream);
+  else e = head_size <= 64 ? run_forward<__half, 64>(p, stream) : run_forward<__half, 128>(p, stream);
   return e == cudaSuccess ? kOk : kErrCuda;
 }
 
@@ -1097,6 +1188,7 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
   p.delta = delta;
   p.most = most;
   p.dq = dq, p.dk = dk, p.dv = dv;
+  p.splits = kv_splits(s);
   const auto map = [&](CUtensorMap* m, const hc_heads& t, size_t length, size_t of, int rows) { return make_head_map(m, type, t, head_size, length, of, batch, rows, 1); };
   if (!map(&p.q, q, queries, heads, dev::kStep) || !map(&p.q_tile, q, queries, heads, dev::kTile) || !map(&p.dout, dout, queries, heads, dev::kStep) ||
       !map(&p.dout_tile, dout, queries, heads, dev::kTile) || !map(&p.k, k, keys, kv_heads, dev::kStep) || !map(&p.k_tile, k, keys, kv_heads, dev::kTile) ||

@@ -93,16 +93,16 @@ int hc_orthogonalize(const void* g, int type, size_t batch, size_t height, size_
 // below 2^24, scale above 0.
 // A tensor's values are adjacent, 16-byte aligned; its strides, multiples of 8 elements and at least head_size, are its own.
 // out and the gradients: (batch, position, head, head_size) without gaps, 16-byte aligned.
-// stats: hc_attention_stats floats for the backward pass, 16-byte aligned, or NULL.  Scratch memory, 256-byte aligned, of hc_attention_bytes (0: none).
+// stats: hc_attention_stats floats for the backward pass, 16-byte aligned, or NULL.
 // A key or value that is not finite may show in any query of its sequence and head, also in one that does not see it.
 typedef struct hc_heads {
   const void* data;
   size_t batch, head, position;  // elements from one to the next
 } hc_heads;
 size_t hc_attention_stats(size_t batch, size_t heads, size_t queries);
-size_t hc_attention_bytes(size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size, size_t window, size_t sinks);
 int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float* stats, size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size,
-                 size_t window, size_t sinks, float scale, void* scratch, size_t scratch_bytes, hc_stream_t stream);
+                 size_t window, size_t sinks, float scale, hc_stream_t stream);
+// Scratch memory of the backward pass: hc_attention_backward_bytes, 256-byte aligned.
 // dq, and dk and dv (both or neither): of `type`, from `out` and `stats` of the forward pass.  Probabilities and their gradients are rounded to `type` for the products.
 size_t hc_attention_backward_bytes(size_t batch, size_t heads, size_t kv_heads, size_t queries, size_t keys, size_t head_size);
 int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k, hc_heads v, int type, const float* stats, void* dq, void* dk, void* dv, size_t batch, size_t heads,

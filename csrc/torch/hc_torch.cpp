@@ -46,7 +46,6 @@ struct Api {
   decltype(&hc_orthogonalize_bytes) orthogonalize_bytes;
   decltype(&hc_orthogonalize) orthogonalize;
   decltype(&hc_attention_stats) attention_stats;
-  decltype(&hc_attention_bytes) attention_bytes;
   decltype(&hc_attention) attention;
   decltype(&hc_attention_backward_bytes) attention_backward_bytes;
   decltype(&hc_attention_backward) attention_backward;
@@ -73,7 +72,6 @@ void bind_all(const std::unordered_map<std::string, uintptr_t>& at) {
   HC_BIND(orthogonalize_bytes);
   HC_BIND(orthogonalize);
   HC_BIND(attention_stats);
-  HC_BIND(attention_bytes);
   HC_BIND(attention);
   HC_BIND(attention_backward_bytes);
   HC_BIND(attention_backward);
@@ -504,10 +502,8 @@ Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, int6
   const int64_t b = q.size(0), h = q.size(1), kv = k.size(1), m = q.size(2), n = k.size(2), d = q.size(3);
   Tensor out = empty_heads(q, q);
   if (stats) *stats = at::empty({(int64_t)api.attention_stats(b, h, m)}, q.options().dtype(at::kFloat));
-  const size_t need = api.attention_bytes(b, h, kv, m, n, d, window, sinks);
-  const Tensor scratch = scratch_of(need, q);
   check(api.attention(heads_at(q), heads_at(k), heads_at(v), type_of(q), out.data_ptr(), stats ? static_cast<float*>(stats->data_ptr()) : nullptr, b, h, kv, m, n, d, window, sinks, (float)scale,
-                      ptr(scratch), need, stream_of(q)),
+                      stream_of(q)),
         "attention");
   return out;
 }

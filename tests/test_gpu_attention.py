@@ -327,7 +327,7 @@ def test_c_entry_points_refuse():
     def at(data=4096, batch=4096, head=1024, position=16):
         return Heads(data, batch, head, position)
 
-    forward = dict(q=at(), k=at(), v=at(), type=1, out=p, stats=p, b=2, h=4, kv=2, m=3, n=5, d=16, w=0, s=0, scale=0.25, scratch=p, bytes=big)
+    forward = dict(q=at(), k=at(), v=at(), type=1, out=p, stats=p, b=2, h=4, kv=2, m=3, n=5, d=16, w=0, s=0, scale=0.25)
     backward = dict(do=at(), out=p, q=at(), k=at(), v=at(), type=1, stats=p, dq=p, dk=p, dv=p, b=2, h=4, kv=2, m=3, n=5, d=16, w=0, s=0, scale=0.25, scratch=p, bytes=big)
     both = [dict(q=at(data=4098)), dict(k=at(data=None)), dict(v=at(position=12)), dict(q=at(position=8)), dict(k=at(head=1028)), dict(v=at(batch=0)), dict(type=0), dict(type=3), dict(out=None), dict(out=some),
             dict(stats=some), dict(h=3), dict(kv=0), dict(m=1 << 24), dict(n=1 << 24), dict(d=12), dict(d=136), dict(d=0), dict(b=1 << 24), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan)]
@@ -337,7 +337,7 @@ def test_c_entry_points_refuse():
         assert lib.hc_attention_backward(*{**backward, **bad}.values(), None) == 4, bad
     assert lib.hc_attention_backward(*{**backward, "dq": None, "dk": None, "dv": None}.values(), None) == 0
     assert lib.hc_attention(*{**forward, "b": 0}.values(), None) == 0 and lib.hc_attention(*{**forward, "m": 0}.values(), None) == 0
-    assert lib.hc_attention_bytes(2, 3, 2, 3, 5, 16, 0, 0) == 0 and lib.hc_attention_stats(2, 4, 129) == 2 * 4 * 256
+    assert lib.hc_attention_backward_bytes(2, 3, 2, 3, 5, 16) == 0 and lib.hc_attention_stats(2, 4, 129) == 2 * 4 * 256
 
 
 @pytest.mark.gpu

@@ -20,7 +20,6 @@ def declare(lib):
         "hc_linear_backward_bytes": [sz, sz, sz, i],
         "hc_orthogonalize_bytes": [sz, sz, sz],
         "hc_attention_stats": [sz, sz, sz],
-        "hc_attention_bytes": [sz] * 8,
         "hc_attention_backward_bytes": [sz] * 6,
         "hc_linear_cross_entropy_bytes": [sz, sz, sz],
         "hc_linear_cross_entropy_backward_bytes": [sz, sz, sz],
@@ -32,7 +31,7 @@ def declare(lib):
         "hc_linear": [vp, sz, vp, sz, i, vp, i, vp, sz, vp, i, sz, vp, sz, i, sz, sz, sz, vp, sz, vp],
         "hc_linear_backward": [vp, i, sz, vp, sz, i, i, vp, sz, vp, sz, i, vp, sz, vp, sz, vp, i, sz, sz, sz, vp, sz, vp],
         "hc_orthogonalize": [vp, i, sz, sz, sz, sz, sz, vp, i, f, f, f, f, vp, sz, vp],
-        "hc_attention": [Heads, Heads, Heads, i, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, f, vp, sz, vp],
+        "hc_attention": [Heads, Heads, Heads, i, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, f, vp],
         "hc_attention_backward": [Heads, vp, Heads, Heads, Heads, i, vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, f, vp, sz, vp],
         "hc_linear_cross_entropy": [vp, sz, vp, sz, i, vp, l, i, vp, vp, sz, sz, sz, vp, sz, vp],
         "hc_linear_cross_entropy_backward": [vp, sz, vp, sz, i, vp, l, i, vp, vp, vp, sz, vp, sz, sz, sz, sz, vp, sz, vp],

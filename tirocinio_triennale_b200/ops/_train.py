@@ -33,7 +33,7 @@ def _load():
             names = ("hc_layer_norm", "hc_layer_norm_backward_bytes", "hc_layer_norm_backward", "hc_token_logprobs", "hc_token_logprobs_backward",
                      "hc_align_rows", "hc_linear_bytes", "hc_linear", "hc_linear_backward_bytes", "hc_linear_backward", "hc_orthogonalize_bytes", "hc_orthogonalize",
                      "hc_adamw", "hc_adamw_values", "hc_linear_cross_entropy_bytes", "hc_linear_cross_entropy", "hc_linear_cross_entropy_backward_bytes",
-                     "hc_linear_cross_entropy_backward", "hc_attention_stats", "hc_attention_bytes", "hc_attention", "hc_attention_backward_bytes", "hc_attention_backward")
+                     "hc_linear_cross_entropy_backward", "hc_attention_stats", "hc_attention", "hc_attention_backward_bytes", "hc_attention_backward")
             module.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in names})
             _module = module
     return _module
