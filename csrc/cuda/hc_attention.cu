@@ -614,66 +614,46 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
-// delta = dO . O of every query and head; eight values a thread, so `kLanes` threads a query
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) hc_attention_delta_kernel(const T* dout, int64_t stride_b, int64_t stride_h, int64_t stride_t, const T* o, int batch, int heads, int tq, int d, float* delta,
-                                                                 int64_t ld, unsigned int* most) {
-  const int64_t total = (int64_t)batch * heads * tq;
-  const int part = threadIdx.x % kLanes;
+// delta = dO . O of every query of a head (kDelta), and the largest square of a norm of dO's (or V's) rows.  Eight values a thread, four rows of a thread on their way together; a block has
+// 4 * 256 / kLanes rows of a head.
+template <typename T, int kLanes, bool kDelta>
+__global__ void __launch_bounds__(256) hc_attention_rows_kernel(const T* rows, int64_t stride_b, int64_t stride_h, int64_t stride_t, const T* o, int heads, int length, int d, int blocks, float* delta,
+                                                                int64_t ld, unsigned int* most) {
+  constexpr int kAtOnce = 4, kApart = 256 / kLanes;
+  const int head_at = blockIdx.x / blocks, b = head_at / heads, h = head_at - b * heads;
+  const int part = threadIdx.x % kLanes, first = (blockIdx.x - head_at * blocks) * (kAtOnce * kApart) + threadIdx.x / kLanes;
+  const bool has = part * 8 < d;
+  const T* from = rows + b * stride_b + h * stride_h + part * 8;
+  uint4 x[kAtOnce], y[kAtOnce];
+#pragma unroll
+  for (int k = 0; k < kAtOnce; ++k) {
+    const int i = first + k * kApart;
+    x[k] = y[k] = make_uint4(0, 0, 0, 0);
+    if (!has || i >= length) continue;
+    x[k] = *reinterpret_cast<const uint4*>(from + i * stride_t);
+    if (kDelta) y[k] = *reinterpret_cast<const uint4*>(o + (((int64_t)b * length + i) * heads + h) * d + part * 8);
+  }
   unsigned int largest = 0;
-  for (int64_t first = blockIdx.x * (256ll / kLanes); first < total; first += gridDim.x * (256ll / kLanes)) {
-    const int64_t n = first + threadIdx.x / kLanes;  // as O lies: head after head of a query
-    float dot = 0.0f, square = 0.0f;
-    int64_t h = 0, b = 0;
-    int i = 0;
-    if (n < total) {
-      h = n % heads;
-      const int64_t r = n / heads;
-      b = r / tq;
-      i = (int)(r - b * tq);
-      if (part * 8 < d) {
-        float x[8], y[8];
-        load8(dout + b * stride_b + h * stride_h + i * stride_t + part * 8, x);
-        load8(o + n * d + part * 8, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          dot = fmaf(x[j], y[j], dot);
-          square = fmaf(x[j], x[j], square);
-        }
-      }
+  for (int k = 0; k < kAtOnce; ++k) {
+    float u[8], v[8], dot = 0.0f, square = 0.0f;
+    unpack2<T>(x[k].x, u[0], u[1]), unpack2<T>(x[k].y, u[2], u[3]), unpack2<T>(x[k].z, u[4], u[5]), unpack2<T>(x[k].w, u[6], u[7]);
+    unpack2<T>(y[k].x, v[0], v[1]), unpack2<T>(y[k].y, v[2], v[3]), unpack2<T>(y[k].z, v[4], v[5]), unpack2<T>(y[k].w, v[6], v[7]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dot = fmaf(u[j], v[j], dot);
+      square = fmaf(u[j], u[j], square);
     }
 #pragma unroll
-    for (int k = kLanes / 2; k > 0; k >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, k);
-      square += __shfl_xor_sync(0xffffffffu, square, k);
+    for (int n = kLanes / 2; n > 0; n >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, n);
+      square += __shfl_xor_sync(0xffffffffu, square, n);
     }
-    if (n < total && part == 0) delta[(b * heads + h) * ld + i] = dot;
+    const int i = first + k * kApart;
+    if (kDelta && part == 0 && i < length) delta[head_at * ld + i] = dot;
     if (square < INFINITY) largest = max(largest, __float_as_uint(square));
   }
   if (!most) return;
-  largest = __reduce_max_sync(0xffffffffu, largest);
-  if ((threadIdx.x & 31) == 0 && largest) atomicMax(most, largest);
-}
-// the largest square of a norm of the rows of V
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) hc_attention_norm_kernel(const T* v, int64_t stride_b, int64_t stride_h, int64_t stride_t, int batch, int heads, int tk, int d, unsigned int* most) {
-  const int64_t total = (int64_t)batch * heads * tk;
-  const int part = threadIdx.x % kLanes;
-  unsigned int largest = 0;
-  for (int64_t first = blockIdx.x * (256ll / kLanes); first < total; first += gridDim.x * (256ll / kLanes)) {
-    const int64_t n = first + threadIdx.x / kLanes;
-    float square = 0.0f;
-    if (n < total && part * 8 < d) {
-      const int64_t h = n % heads, r = n / heads, b = r / tk;
-      float x[8];
-      load8(v + b * stride_b + h * stride_h + (r - b * tk) * stride_t + part * 8, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) square = fmaf(x[j], x[j], square);
-    }
-#pragma unroll
-    for (int k = kLanes / 2; k > 0; k >>= 1) square += __shfl_xor_sync(0xffffffffu, square, k);
-    if (square < INFINITY) largest = max(largest, __float_as_uint(square));
-  }
   largest = __reduce_max_sync(0xffffffffu, largest);
   if ((threadIdx.x & 31) == 0 && largest) atomicMax(most, largest);
 }
@@ -1093,14 +1073,13 @@ cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_head
   cudaError_t e = allow_smem(dev::hc_attention_backward_kernel<T, kD, true>, smem, &allowed_kv);
   if (e == cudaSuccess) e = allow_smem(dev::hc_attention_backward_kernel<T, kD, false>, smem, &allowed_q);
   if (e != cudaSuccess) return e;
-  constexpr int kLanes = kD / 8;
-  const int64_t most_blocks = attn_sms() * 8;
-  const auto blocks_for = [&](int64_t rows) { return (unsigned)((rows + 256 / kLanes - 1) / (256 / kLanes) < most_blocks ? (rows + 256 / kLanes - 1) / (256 / kLanes) : most_blocks); };
-  dev::hc_attention_delta_kernel<T, kLanes><<<blocks_for((int64_t)p.batch * p.heads * p.tq), 256, 0, stream>>>(
-      static_cast<const T*>(dout.data), (int64_t)dout.batch, (int64_t)dout.head, (int64_t)dout.position, static_cast<const T*>(o), p.batch, p.heads, p.tq, p.d, delta, p.less_ld, most);
+  constexpr int kLanes = kD / 8, kRows = 4 * 256 / kLanes;  // of a block
+  const int q_blocks = (p.tq + kRows - 1) / kRows, k_blocks = (p.tk + kRows - 1) / kRows;
+  dev::hc_attention_rows_kernel<T, kLanes, true><<<(unsigned)((int64_t)p.batch * p.heads * q_blocks), 256, 0, stream>>>(
+      static_cast<const T*>(dout.data), (int64_t)dout.batch, (int64_t)dout.head, (int64_t)dout.position, static_cast<const T*>(o), p.heads, p.tq, p.d, q_blocks, delta, p.less_ld, most);
   if (most)
-    dev::hc_attention_norm_kernel<T, kLanes><<<blocks_for((int64_t)p.batch * p.kv_heads * p.tk), 256, 0, stream>>>(
-        static_cast<const T*>(v.data), (int64_t)v.batch, (int64_t)v.head, (int64_t)v.position, p.batch, p.kv_heads, p.tk, p.d, most + 1);
+    dev::hc_attention_rows_kernel<T, kLanes, false><<<(unsigned)((int64_t)p.batch * p.kv_heads * k_blocks), 256, 0, stream>>>(
+        static_cast<const T*>(v.data), (int64_t)v.batch, (int64_t)v.head, (int64_t)v.position, nullptr, p.kv_heads, p.tk, p.d, k_blocks, nullptr, 0, most + 1);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // dq or not: the keys' pass needs the delta that this one completes

@@ -1214,11 +1214,11 @@ int gemm_parts(int64_t m, int64_t n, int64_t k) {
   return best;
 }
 
-int64_t gemm_cost(int64_t m, int64_t n, int64_t k) {
+int64_t gemm_cost(int64_t m, int64_t n, int64_t k, int parts) {
   GemmCall c;
   memset(&c, 0, sizeof(c));
   c.m = m, c.n = n, c.k = k, c.batch = 1;
-  return best_tile<kGemmLinear>(c, 1, sm_count()).cost;
+  return best_tile<kGemmLinear>(c, parts, sm_count()).cost;
 }
 
 int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k) {

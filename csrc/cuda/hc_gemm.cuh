@@ -135,10 +135,12 @@ struct GemmCall {
 
 // Into how many parts the sum of a product is best shared out (1: none).
 int gemm_parts(int64_t m, int64_t n, int64_t k);
-// What a call's time is reckoned to be, in cycles, as a single part.
-int64_t gemm_cost(int64_t m, int64_t n, int64_t k);
+// What a call's time is reckoned to be, in cycles, in so many parts of its sum.
+int64_t gemm_cost(int64_t m, int64_t n, int64_t k, int parts);
 // stretches of columns of kGemmLossSums, two a tile
 int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k);
+// of up to HC_LINEAR_FEW_ROWS rows, which may begin anywhere: sixteen columns a stretch, sums lie [row][stretch]
+cudaError_t launch_few_rows_loss(const GemmCall& call, cudaStream_t stream);
 cudaError_t launch_loss_sums(const GemmCall& call, cudaStream_t stream);
 cudaError_t launch_loss_grad(const GemmCall& call, cudaStream_t stream);
 // act(a b + bias) + residual

@@ -21,6 +21,7 @@ struct FewRowsParams {
   int64_t ldx, ldw, ldr, ldo, ldz;
   int64_t inner, width;
   int rows, out_type, bias_type, activation;
+  GemmLoss loss;  // `sums`: results are logits, of which each row's largest and sum of exponentials over a block's sixteen go to [row][block]
 };
 
 __device__ __forceinline__ float act_value(float z, int kind) {
@@ -130,9 +131,21 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
   for (int i = threadIdx.x; i < N * 128; i += blockDim.x) {
     const int r = i >> 4;
     const int64_t n = first + (i & 15);
-    if (r >= p.rows || n >= p.width) continue;
+    const bool there = r < p.rows && n < p.width;
+    if (!there && !p.loss.sums) continue;
     float z = 0.0f;
     for (int w = 0; w < warps; ++w) z += parts[w][r][i & 15];
+    if (p.loss.sums) {  // over the sixteen lanes of a row
+      float most = there ? z : -INFINITY;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      float sum = there ? exp2f((z - (most == -INFINITY ? 0.0f : most)) * kLog2E) : 0.0f;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((i & 15) == 0 && r < p.rows) p.loss.sums[(int64_t)r * gridDim.x + blockIdx.x] = make_float2(most, sum);
+      if (there && p.loss.tokens[r] == n) p.loss.picked[r] = z;
+      continue;
+    }
     if (p.bias) z += param_at(p.bias, p.bias_type, n);
     if (p.z) static_cast<T*>(p.z)[r * p.ldz + n] = from_float<T>(z);
     z = act_value(z, p.activation);
@@ -372,6 +385,12 @@ void few_rows(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
   else few_rows_of<T, 2>(p, vector, stream);
 }
 
+void run_few_rows(const dev::FewRowsParams& p, int type, cudaStream_t stream) {
+  const bool vector = p.inner % 8 == 0 && gemm_operand_ok(p.x, p.ldx) && gemm_operand_ok(p.w, p.ldw);
+  if (type == kBf16) few_rows<__nv_bfloat16>(p, vector, stream);
+  else few_rows<__half>(p, vector, stream);
+}
+
 template <typename Y, typename T, int kAct>
 void rows_backward_of(const dev::RowsBackwardParams& p, bool vector, cudaStream_t stream) {
   const dim3 grid((unsigned)((p.width + 255) / 256), (unsigned)p.shares);
@@ -438,6 +457,17 @@ BackwardLayout backward_layout(size_t rows, size_t inner, size_t width, int keep
 bool aligned_rows(const void* p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0; }
 
 }  // namespace
+
+cudaError_t launch_few_rows_loss(const GemmCall& c, cudaStream_t stream) {
+  dev::FewRowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = c.a.data, p.w = c.b.data, p.ldx = c.a.ld, p.ldw = c.b.ld;
+  p.inner = c.k, p.width = c.n, p.rows = (int)c.m;
+  p.loss = c.loss;
+  run_few_rows(p, c.type, stream);
+  return cudaGetLastError();
+}
+
 }  // namespace hc
 
 extern "C" {
@@ -474,9 +504,7 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   if (rows <= kFewRows) {
     const dev::FewRowsParams p = {x, weight, bias, residual, out, z, (int64_t)x_stride, (int64_t)weight_stride, (int64_t)residual_stride,
                                   (int64_t)out_stride, (int64_t)z_stride, (int64_t)inner, (int64_t)width, (int)rows, out_type, bias_type, activation};
-    const bool vector = inner % 8 == 0 && aligned_rows(x, x_stride) && aligned_rows(weight, weight_stride);
-    if (type == kBf16) few_rows<__nv_bfloat16>(p, vector, stream);
-    else few_rows<__half>(p, vector, stream);
+    run_few_rows(p, type, stream);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
   }
   if (!gemm_operand_ok(x, x_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;

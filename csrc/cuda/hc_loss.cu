@@ -47,6 +47,47 @@ __global__ void __launch_bounds__(1024) hc_loss_join_kernel(const float2* sums, 
   losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? all - picked[row] : __int_as_float(0x7fc00000);
 }
 
+// The same of few rows, a block each, whose stretches lie one after the other.
+__global__ void __launch_bounds__(1024) hc_loss_join_row_kernel(const float2* sums, int64_t stretches, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse,
+                                                                 float* losses) {
+  __shared__ float tops[32], totals[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
+  constexpr int kAtOnce = 4;
+  float most = -INFINITY, sum = 0.0f;
+  const auto joined = [](float& most, float& sum, float m, float s) {
+    const float top = fmaxf(most, m), ref = top == -INFINITY ? 0.0f : top;
+    sum = sum * exp2f((most - ref) * kLog2E) + s * exp2f((m - ref) * kLog2E);
+    most = top;
+  };
+  for (int64_t i = threadIdx.x; i < stretches; i += 1024 * kAtOnce) {
+    float2 v[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) v[k] = i + k * 1024 < stretches ? sums[row * stretches + i + k * 1024] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) joined(most, sum, v[k].x, v[k].y);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_down_sync(0xffffffffu, most, o), s = __shfl_down_sync(0xffffffffu, sum, o);
+    joined(most, sum, m, s);
+  }
+  if (lane == 0) tops[warp] = most, totals[warp] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+  most = tops[lane], sum = totals[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_down_sync(0xffffffffu, most, o), s = __shfl_down_sync(0xffffffffu, sum, o);
+    joined(most, sum, m, s);
+  }
+  if (lane != 0) return;
+  const float all = sum > 0.0f || sum != sum ? most + logf(sum) : __int_as_float(0x7fc00000);
+  const int64_t token = tokens[row];
+  lse[row] = all;
+  losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? all - picked[row] : __int_as_float(0x7fc00000);
+}
+
 // their sum, or their mean over the rows that have a token, whose number is kept for the backward pass
 __global__ void __launch_bounds__(1024) hc_loss_reduce_kernel(const float* losses, const int64_t* tokens, int64_t ignore, int64_t rows, int reduction, float* loss, float* count) {
   __shared__ double sums[32];
@@ -95,9 +136,9 @@ __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss
   if (most && (threadIdx.x & 31) == 0 && largest) atomicMax(most, largest);
 }
 
-// dx in its own type, from its sum, which is times 2^k (gradient_power)
+// dx in its own type, from the parts of its sum, which is times 2^k (gradient_power)
 template <typename T>
-__global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64_t from_stride, int64_t rows, int64_t width, const unsigned int* most, T* dx, int64_t stride) {
+__global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64_t from_stride, int parts, int64_t rows, int64_t width, const unsigned int* most, T* dx, int64_t stride) {
   const float power = most ? gradient_power(most, -1) : 1.0f;
   const int64_t groups = (width + 7) / 8;
   const bool vector = stride % 8 == 0 && (reinterpret_cast<uintptr_t>(dx) & 15u) == 0;
@@ -105,6 +146,12 @@ __global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64
     const int64_t r = k / groups, c = (k - r * groups) * 8;
     float v[8];
     load8(sum + r * from_stride + c, v);
+    for (int part = 1; part < parts; ++part) {
+      float w[8];
+      load8(sum + (part * rows + r) * from_stride + c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += w[j];
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= power;
     if (vector && c + 8 <= width) {
@@ -129,9 +176,27 @@ constexpr size_t kPieceBytes = (size_t)256 << 20;
 size_t up(size_t v, size_t unit) { return (v + unit - 1) / unit * unit; }
 bool loss_sizes_ok(size_t rows, size_t inner, size_t vocab) { return inner > 0 && vocab > 0 && inner < kMostSide && vocab < kMostSide && rows < kMostSide; }
 
+int64_t stretches_of(size_t rows, size_t inner, size_t vocab) { return rows <= HC_LINEAR_FEW_ROWS ? (int64_t)(vocab + 15) / 16 : gemm_loss_stretches(rows, vocab, inner); }
 size_t forward_bytes(size_t rows, size_t inner, size_t vocab) {
   if (!rows) return 0;
-  return up((size_t)gemm_loss_stretches(rows, vocab, inner) * rows * sizeof(float2), 256) + 2 * up(rows * sizeof(float), 256);
+  return up((size_t)stretches_of(rows, inner, vocab) * rows * sizeof(float2), 256) + 2 * up(rows * sizeof(float), 256);
+}
+
+// Into how many parts the sum of dx's product with a piece is shared out, each of which is summed over the pieces in an array of its own: 96 tiles of 256 x 256 on 74 pairs of SMs leave a third of
+// them idle, 288 thirds of tiles do not.
+constexpr int kMostParts = 4;
+int dx_parts_of(size_t rows, size_t inner, size_t piece) {
+  int best = 1;
+  double least = 0;
+  for (int parts = 1; parts <= kMostParts && piece >= (size_t)parts * 1024; ++parts) {
+    // what a part writes and reads, some 3000 bytes a cycle, passes beside the products but for a quarter of it
+    const double cost = (double)gemm_cost(rows, inner, piece, parts) + (parts - 1) * (rows * inner * 8.0 / 3000.0 * 0.25);
+    if (least == 0 || cost < least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  return best;
 }
 
 // The pieces of the vocabulary: as many columns as the tiles of the three products fill the SMs best with, by their reckoned times.
@@ -142,7 +207,7 @@ size_t piece_of(size_t rows, size_t inner, size_t vocab) {
   size_t best = most;
   double least = 0;
   for (size_t piece = most; piece >= 1024 && piece * 4 > most; piece -= 256) {
-    const auto cost = [&](size_t n) { return (double)(gemm_cost(rows, n, inner) + gemm_cost(rows, inner, n) + gemm_cost(n, inner, rows)); };
+    const auto cost = [&](size_t n) { return (double)(gemm_cost(rows, n, inner, 1) + gemm_cost(rows, inner, n, dx_parts_of(rows, inner, n)) + gemm_cost(n, inner, rows, 1)); };
     const size_t whole = vocab / piece, rest = vocab % piece;
     const double all = whole * (cost(piece) + 15000.0) + (rest ? cost(rest) + 15000.0 : 0.0);
     if (least == 0 || all < least) {
@@ -153,21 +218,23 @@ size_t piece_of(size_t rows, size_t inner, size_t vocab) {
   return best;
 }
 struct LossLayout {
+  int parts;  // of dx
   size_t piece, g, dx, weight, most, total;  // offsets, G at 0
 };
 LossLayout backward_layout(size_t rows, size_t inner, size_t vocab) {
   LossLayout l;
   l.piece = piece_of(rows, inner, vocab);
+  l.parts = dx_parts_of(rows, inner, l.piece);
   l.dx = up(rows * up(l.piece, 8) * 2, 256);
-  l.weight = l.dx + up(rows * up(inner, 8) * sizeof(float), 256);
+  l.weight = l.dx + up((size_t)l.parts * rows * up(inner, 8) * sizeof(float), 256);
   l.most = l.weight + up(rows * sizeof(float), 256);
   l.total = l.most + kMostBytes;
   return l;
 }
 
-bool operands_ok(const void* x, size_t x_stride, const void* weight, size_t weight_stride, size_t inner) {
+bool operands_ok(const void* x, size_t x_stride, const void* weight, size_t weight_stride, size_t inner, bool anywhere) {
   return x && weight && x_stride >= inner && weight_stride >= inner && x_stride < ((size_t)1 << 32) && weight_stride < ((size_t)1 << 32) &&
-         gemm_operand_ok(x, (int64_t)x_stride) && gemm_operand_ok(weight, (int64_t)weight_stride);
+         (anywhere ? lies_at(x, 2) && lies_at(weight, 2) : gemm_operand_ok(x, (int64_t)x_stride) && gemm_operand_ok(weight, (int64_t)weight_stride));
 }
 
 }  // namespace
@@ -184,7 +251,7 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
   if (!lies_at(loss, 4) || !lies_at(stats, 4) || !lies_at(tokens, 8) || (!loss && (rows || reduction)) || !stats) return kErrArgument;
   float *losses = loss, *lse = stats, *count = stats + rows;
   if (rows) {
-    if (!tokens || !operands_ok(x, x_stride, weight, weight_stride, inner)) return kErrArgument;
+    if (!tokens || !operands_ok(x, x_stride, weight, weight_stride, inner, rows <= HC_LINEAR_FEW_ROWS)) return kErrArgument;
     if (!scratch || !lies_at(scratch, 256) || scratch_bytes < forward_bytes(rows, inner, vocab)) return kErrArgument;
     GemmCall c;
     memset(&c, 0, sizeof(c));
@@ -192,7 +259,7 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     c.m = rows, c.n = vocab, c.k = inner, c.batch = 1;
     c.a = {x, (int64_t)x_stride, 0, true};
     c.b = {weight, (int64_t)weight_stride, 0, true};
-    const int64_t stretches = gemm_loss_stretches(rows, vocab, inner);
+    const int64_t stretches = stretches_of(rows, inner, vocab);
     unsigned char* at = static_cast<unsigned char*>(scratch);
     c.loss.sums = reinterpret_cast<float2*>(at);
     at += up((size_t)stretches * rows * sizeof(float2), 256);
@@ -200,7 +267,11 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     if (reduction != dev::kNone) losses = reinterpret_cast<float*>(at + up(rows * sizeof(float), 256));
     c.loss.tokens = tokens;
     c.loss.ignore = ignore;
-    if (launch_loss_sums(c, stream) != cudaSuccess) return kErrCuda;
+    const bool few = rows <= HC_LINEAR_FEW_ROWS;
+    if ((few ? launch_few_rows_loss(c, stream) : launch_loss_sums(c, stream)) != cudaSuccess) return kErrCuda;
+    if (few)
+      dev::hc_loss_join_row_kernel<<<(unsigned)rows, 1024, 0, stream>>>(c.loss.sums, stretches, c.loss.picked, tokens, ignore, (int64_t)vocab, lse, losses);
+    else
     dev::hc_loss_join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(c.loss.sums, stretches, (int64_t)rows, c.loss.picked, tokens, ignore, (int64_t)vocab, lse, losses);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   }
@@ -223,7 +294,7 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
   if (rows == 0)
     return !dweight || cudaMemset2DAsync(dweight, dweight_stride * 2, 0, inner * 2, vocab, stream) == cudaSuccess ? kOk : kErrCuda;
   if (!dx && !dweight) return kOk;
-  if (!tokens || !stats || !dloss || !operands_ok(x, x_stride, weight, weight_stride, inner)) return kErrArgument;
+  if (!tokens || !stats || !dloss || !operands_ok(x, x_stride, weight, weight_stride, inner, false)) return kErrArgument;
   const LossLayout l = backward_layout(rows, inner, vocab);
   if (!scratch || !lies_at(scratch, 256) || scratch_bytes < l.total) return kErrArgument;
   unsigned char* at = static_cast<unsigned char*>(scratch);
@@ -265,7 +336,8 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
       c.a = {at, g_ld, 0, true};
       c.b = {w, (int64_t)weight_stride, 0, false};
       c.out_type = kF32;
-      c.out = {dx_sum, dx_ld, 0};
+      c.out = {dx_sum, dx_ld, (int64_t)rows * dx_ld};
+      c.parts = l.parts;
       c.most = nullptr;
       if (first) c.in = c.out;
       if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
@@ -275,9 +347,9 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
   const size_t dx_blocks = (rows * (up(inner, 8) / 8) + 255) / 256;
   const unsigned grid = (unsigned)(dx_blocks < 2368 ? dx_blocks : 2368);
   if (type == kBf16)
-    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, (int64_t)rows, (int64_t)inner, most, static_cast<__nv_bfloat16*>(dx), (int64_t)dx_stride);
+    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, static_cast<__nv_bfloat16*>(dx), (int64_t)dx_stride);
   else
-    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, (int64_t)rows, (int64_t)inner, most, static_cast<__half*>(dx), (int64_t)dx_stride);
+    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, static_cast<__half*>(dx), (int64_t)dx_stride);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 

@@ -110,7 +110,7 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
 
 // ---- cross entropy from hidden rows ------------------------------------------------------------------------------------
 // loss_i = log sum_v exp(x_i . w_v) - x_i . w_token, without the logits ever being stored: x [rows][inner], weight [vocab][inner], both of `type` (1 or 2), as operands
-// of a product lie (16-byte aligned, strides multiples of 8), sides below 2^26; sums in the tensor core over up to 1024 terms.
+// of a product lie (16-byte aligned, strides multiples of 8; without a backward pass up to HC_LINEAR_FEW_ROWS rows, and their weights, may begin anywhere), sides below 2^26; sums in the tensor core over up to 1024 terms.
 // reduction: 0 none (loss: a value a row), 1 sum, 2 mean over the rows that have a token (loss: one value; NaN where there are none).  A row whose token is `ignore`
 // gives 0 and a gradient of 0, whatever it holds, and enters dweight times 0; a token outside the vocabulary gives NaN, in the gradient in all of dweight.
 // stats: rows + 1 floats for the backward pass.  Scratch memory, 256-byte aligned: hc_linear_cross_entropy_bytes for the current device.
@@ -119,7 +119,7 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
                             float* stats, size_t rows, size_t inner, size_t vocab, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 // dx = G weight and dweight = G^T x (of `type`, each NULL where it is not wanted) with G = a (p - 1[token]); a: dloss (fp32) of the row, or dloss[0], over the count for a mean.
 // G is formed for a piece of the vocabulary at a time, in 16 bits (of fp16 times a power of two that the largest |a| gives), in scratch memory of at most 256 MiB or 1024 columns;
-// dx is summed in fp32.  Where a result's stride is its width rounded up to eight, what lies behind its rows may be overwritten.
+// dx is summed in fp32, in up to four parts.  Where a result's stride is its width rounded up to eight, what lies behind its rows may be overwritten.
 size_t hc_linear_cross_entropy_backward_bytes(size_t rows, size_t inner, size_t vocab);
 int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const int64_t* tokens, int64_t ignore, int reduction,
                                      const float* stats, const float* dloss, void* dx, size_t dx_stride, void* dweight, size_t dweight_stride, size_t rows, size_t inner, size_t vocab,

@@ -637,7 +637,7 @@ Tensor linear_cross_entropy(const Tensor& x_, const Tensor& weight_, const Tenso
   TORCH_CHECK_VALUE(std::max(m, std::max(n, k)) < (1 << 26), "linear_cross_entropy: every side is below 2^26");
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight))) return LinearCrossEntropy::apply(x, weight, tokens, ignore, (int64_t)reduction);
   Tensor stats;
-  return loss_forward(operand(matrix(x, k)), operand(weight), tokens.contiguous(), ignore, reduction, tokens.sizes(), &stats);
+  return loss_forward(for_rows(matrix(x, k), m), for_rows(weight, m), tokens.contiguous(), ignore, reduction, tokens.sizes(), &stats);
 }
 
 // ---- AdamW ------------------------------------------------------------------------------------------------------------

@@ -103,7 +103,7 @@ def test_pieces_of_the_vocabulary():
     leaves = [v.detach().requires_grad_() for v in (x, w)]
     loss = ops.linear_cross_entropy(*leaves, t, reduction="none")
     dx, dw = torch.autograd.grad(loss, leaves, a)
-    assert _lib.cuda().hc_linear_cross_entropy_backward_bytes(40000, 16, 13001) <= (256 << 20) + 40000 * (64 + 4) + 1024
+    assert _lib.cuda().hc_linear_cross_entropy_backward_bytes(40000, 16, 13001) <= (256 << 20) + 40000 * (4 * 64 + 4) + 1024
     h = torch.finfo(BF16).eps / 2
     W = w.double()
     total = torch.zeros(13001, 16, dtype=torch.float64, device="cuda")
@@ -311,6 +311,8 @@ def test_c_entry_points_refuse():
     both = [dict(x=None), dict(x=half), dict(w=half), dict(xs=15), dict(xs=20), dict(ws=20), dict(ws=8), dict(type=0), dict(type=3), dict(red=3), dict(red=-1), dict(t=None), dict(t=some.value + 4), dict(stats=None),
             dict(stats=half), dict(m=1 << 26), dict(k=1 << 26), dict(n=1 << 26), dict(k=0), dict(n=0), dict(scratch=None), dict(scratch=some)]
     for bad in both + [dict(loss=None), dict(loss=half), dict(bytes=10)]:
+        assert lib.hc_linear_cross_entropy(*{**forward, "m": 40, **bad}.values(), None) == 4, bad
+    for bad in (dict(x=odd), dict(w=odd), dict(xs=15), dict(bytes=10)):  # few rows may begin anywhere
         assert lib.hc_linear_cross_entropy(*{**forward, **bad}.values(), None) == 4, bad
     for bad in both + [dict(dl=None), dict(dl=half), dict(dx=odd), dict(dw=odd), dict(dxs=8), dict(dws=15), dict(bytes=10)]:
         assert lib.hc_linear_cross_entropy_backward(*{**backward, **bad}.values(), None) == 4, bad
@@ -322,8 +324,8 @@ def test_scratch_memory_is_bounded():
     lib = _lib.cuda()
     for rows, inner, vocab in ((8192, 768, 50257), (1, 4096, 131072), (100000, 64, 131072), (300000, 8, 5000), (1 << 20, 8, 1025)):
         g = max(256 << 20, rows * 1024 * 2)
-        assert lib.hc_linear_cross_entropy_backward_bytes(rows, inner, vocab) <= g + rows * (inner + 8) * 4 + rows * 4 + 2048
-        assert lib.hc_linear_cross_entropy_bytes(rows, inner, vocab) <= rows * ((vocab + 63) // 64 * 16 + 8) + 2048
+        assert lib.hc_linear_cross_entropy_backward_bytes(rows, inner, vocab) <= g + 4 * rows * (inner + 8) * 4 + rows * 4 + 2048
+        assert lib.hc_linear_cross_entropy_bytes(rows, inner, vocab) <= rows * ((vocab + 63) // 64 * 32 + 8) + 2048
 
 
 @pytest.mark.gpu
