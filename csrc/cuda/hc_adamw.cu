@@ -65,13 +65,42 @@ __device__ __forceinline__ float adam_down() { return __uint_as_float((127u - 11
 __device__ __forceinline__ float adam_up() { return __uint_as_float((127u + 111u) << 23); }
 constexpr uint32_t kLeastBits = (127u - 100u) << 23;  // 2^-100: a block whose largest value is below is held as zeros
 constexpr uint32_t kInfBits = 0x7f800000u;
-
-__device__ __forceinline__ float adam_m_of(uint32_t code, float scale) {
-  const float size = ((__uint_as_float((code & 127u) << 20) * adam_up()) * (float)(1.0 / 0.9375)) * scale;
-  return code & 128u ? -size : size;
+template <typename T>
+__device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
+  unpack2<T>(w, a, b);
 }
-__device__ __forceinline__ float adam_root_of(uint32_t code, float scale) {
-  return ((__uint_as_float(code << 19) * adam_up()) * (float)(1.0 / 0.96875)) * scale;
+template <>
+__device__ __forceinline__ void unpack_pair<float>(uint32_t, float&, float&) {}  // floats are not packed
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  return pack2<T>(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<float>(float, float) {
+  return 0;
+}
+
+// 2^111 over what the largest code stands for: the product is a power of two times the quotient rounded, so nothing is rounded twice
+constexpr float kUpM = (float)(1.0 / 0.9375), kUpV = (float)(1.0 / 0.96875);
+__device__ __forceinline__ float adam_m_of(uint32_t code, float scale) {
+  const float size = (__uint_as_float((code & 127u) << 20) * (adam_up() * kUpM)) * scale;
+  return __uint_as_float(__float_as_uint(size) ^ (code & 128u) << 24);
+}
+__device__ __forceinline__ float adam_root_of(uint32_t code, float scale) { return (__uint_as_float(code << 19) * (adam_up() * kUpV)) * scale; }
+// code number j of a word
+__device__ __forceinline__ uint32_t code_at(uint32_t word, int j, int bit, uint32_t mask) { return (bit >= 8 * j ? word << (bit - 8 * j) : word >> (8 * j - bit)) & mask; }
+// four codes of m and of root(v)
+__device__ __forceinline__ void adam_decode4(uint32_t cm, uint32_t cv, float2 scale, float* m, float* v) {
+  const Pair up_m = pair(adam_up() * kUpM, adam_up() * kUpM), up_v = pair(adam_up() * kUpV, adam_up() * kUpV), sm = pair(scale.x, scale.x), sv = pair(scale.y, scale.y);
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    float a, b;
+    parts((pair(__uint_as_float(code_at(cm, j, 20, 127u << 20)), __uint_as_float(code_at(cm, j + 1, 20, 127u << 20))) * up_m) * sm, a, b);
+    m[j] = __uint_as_float(__float_as_uint(a) ^ code_at(cm, j, 24, 1u << 31));
+    m[j + 1] = __uint_as_float(__float_as_uint(b) ^ code_at(cm, j + 1, 24, 1u << 31));
+    const Pair root = (pair(__uint_as_float(code_at(cv, j, 19, 255u << 19)), __uint_as_float(code_at(cv, j + 1, 19, 255u << 19))) * up_v) * sv;
+    parts(root * root, v[j], v[j + 1]);
+  }
 }
 // the scale that stands for a block's largest value, and one over it, 0 where nothing is held: of zeros (below 2^-100), and of a block
 // with something that is no number or infinite, which becomes NaN as a whole
@@ -95,42 +124,76 @@ __device__ __forceinline__ float adam_update(const P& p, const AdamNow& now, flo
   return x * now.keep - __fdiv_rn(m, root_v * now.root + p.eps) * now.size;
 }
 
-template <typename T, typename G, bool k8, typename P>
+template <typename T, bool kWide>
+__device__ __forceinline__ void adam_load4(const T* p, float* v) {
+  if (!kWide) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = to_float(p[j]);
+  } else if (sizeof(T) == 4) {
+    const float4 w = *reinterpret_cast<const float4*>(p);
+    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    unpack_pair<T>(w.x, v[0], v[1]);
+    unpack_pair<T>(w.y, v[2], v[3]);
+  }
+}
+template <typename T, bool kWide>
+__device__ __forceinline__ void adam_store4(T* p, const float* v) {
+  if (!kWide) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = from_float<T>(v[j]);
+  } else if (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]));
+  }
+}
+
+// A whole block of 256: four neighbours a lane, twice, so that a warp's pieces of each array are adjacent.  kWide: parameter and gradient lie at 16 bytes (the moments do in any case).
+template <typename T, typename G, bool k8, bool kWide, typename P>
 __device__ __forceinline__ void adam_unit_vector(const P& p, const AdamNow& now, const AdamEntry& e, int64_t at) {
   const int lane = threadIdx.x & 31;
-  const int64_t i = at + lane * 8;
-  float x[8], g[8], m[8], v[8];
-  uint2 cm, cv;
+  const int64_t i = at + lane * 4;
+  T* param = static_cast<T*>(e.param) + i;
+  const G* grad = static_cast<const G*>(e.grad) + i;
+  float x[8], g[8], m[8], v[8], r[8];
+  uint32_t cm[2], cv[2];
   float2 scale;
-  load8(static_cast<const T*>(e.param) + i, x);
-  load8(static_cast<const G*>(e.grad) + i, g);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    adam_load4<T, kWide>(param + h * 128, x + h * 4);
+    adam_load4<G, kWide>(grad + h * 128, g + h * 4);
+    if (k8) {
+      cm[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(e.m) + i + h * 128);
+      cv[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(e.v) + i + h * 128);
+    } else {
+      adam_load4<float, true>(static_cast<const float*>(e.m) + i + h * 128, m + h * 4);
+      adam_load4<float, true>(static_cast<const float*>(e.v) + i + h * 128, v + h * 4);
+    }
+  }
   if (k8) {
-    cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(e.m) + i);
-    cv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(e.v) + i);
     scale = e.scales[at / kAdamUnit];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = adam_m_of((j < 4 ? cm.x : cm.y) >> (j % 4 * 8) & 255u, scale.x);
-      const float r = adam_root_of((j < 4 ? cv.x : cv.y) >> (j % 4 * 8) & 255u, scale.y);
-      v[j] = r * r;
-    }
-  } else {
-    load8(static_cast<const float*>(e.m) + i, m);
-    load8(static_cast<const float*>(e.v) + i, v);
+    for (int h = 0; h < 2; ++h) adam_decode4(cm[h], cv[h], scale, m + h * 4, v + h * 4);
   }
-  float r[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = adam_update(p, now, x[j], g[j], m[j], v[j], r[j]);
-  store8(static_cast<T*>(e.param) + i, x);
-  if (!k8) {
-    store8(static_cast<float*>(e.m) + i, m);
-    store8(static_cast<float*>(e.v) + i, v);
-    return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    adam_store4<T, kWide>(param + h * 128, x + h * 4);
+    if (!k8) {
+      adam_store4<float, true>(static_cast<float*>(e.m) + i + h * 128, m + h * 4);
+      adam_store4<float, true>(static_cast<float*>(e.v) + i + h * 128, v + h * 4);
+    }
   }
-  uint32_t most_m = 0, most_v = 0;
+  if (!k8) return;
+  uint32_t most_m = 0, most_v = 0, sign[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    most_m = max(most_m, __float_as_uint(m[j]) & 0x7fffffffu);
+    sign[j] = __float_as_uint(m[j]) >> 24 & 128u;
+    m[j] = fabsf(m[j]);
+    most_m = max(most_m, __float_as_uint(m[j]));
     most_v = max(most_v, __float_as_uint(r[j]) & 0x7fffffffu);
   }
   most_m = __reduce_max_sync(0xffffffffu, most_m);
@@ -138,25 +201,34 @@ __device__ __forceinline__ void adam_unit_vector(const P& p, const AdamNow& now,
   float inverse_m, inverse_v;
   adam_scale(most_m, scale.x, inverse_m);
   adam_scale(most_v, scale.y, inverse_v);
-  const uint32_t key = adam_mixed(now.key + e.number);
-  uint32_t words[4] = {0, 0, 0, 0};
+  const uint32_t first = (uint32_t)i * 0x9E3779B1u + adam_mixed(now.key + e.number);
+  const Pair im = pair(inverse_m, inverse_m), iv = pair(inverse_v, inverse_v), top_m = pair(kTopM, kTopM), top_v = pair(kTopV, kTopV), down = pair(adam_down(), adam_down());
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t h = adam_mixed((uint32_t)(i + j) * 0x9E3779B1u + key);
-    const float y = ((fabsf(m[j]) * inverse_m) * kTopM) * adam_down(), z = ((r[j] * inverse_v) * kTopV) * adam_down();
-    uint32_t a = min((__float_as_uint(y) + ((h & 0xffffu) << 4) + 8u) >> 20, 127u);
-    uint32_t b = min((__float_as_uint(z) + ((h >> 16) << 3) + 4u) >> 19, 255u);
-    a = inverse_m > 0.0f ? a + (m[j] < 0.0f && a > 0u ? 128u : 0u) : 0u;
-    b = inverse_v > 0.0f ? (r[j] > 0.0f ? max(b, 1u) : b) : 0u;
-    words[j / 4] |= a << (j % 4 * 8);
-    words[2 + j / 4] |= b << (j % 4 * 8);
+  for (int h = 0; h < 2; ++h) {
+    uint32_t word_m = 0, word_v = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      float y[2], z[2];
+      parts(((pair(m[h * 4 + j], m[h * 4 + j + 1]) * im) * top_m) * down, y[0], y[1]);
+      parts(((pair(r[h * 4 + j], r[h * 4 + j + 1]) * iv) * top_v) * down, z[0], z[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t random = adam_mixed(first + (uint32_t)(h * 128 + j + k) * 0x9E3779B1u);
+        const uint32_t a = min((__float_as_uint(y[k]) + (random << 4 & 0xffff0u) + 8u) >> 20, 127u);
+        const uint32_t b = min((__float_as_uint(z[k]) + (random >> 13 & 0x7fff8u) + 4u) >> 19, 255u);
+        word_m |= (a | sign[h * 4 + j + k]) << (8 * (j + k));
+        word_v |= max(b, min(__float_as_uint(r[h * 4 + j + k]), 1u)) << (8 * (j + k));  // a root above 0 stays above it
+      }
+    }
+    if (inverse_m == 0.0f) word_m = 0;  // of the whole block
+    if (inverse_v == 0.0f) word_v = 0;
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.m) + i + h * 128) = word_m;
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.v) + i + h * 128) = word_v;
   }
-  *reinterpret_cast<uint2*>(static_cast<uint8_t*>(e.m) + i) = make_uint2(words[0], words[1]);
-  *reinterpret_cast<uint2*>(static_cast<uint8_t*>(e.v) + i) = make_uint2(words[2], words[3]);
   if (lane == 0) e.scales[at / kAdamUnit] = scale;
 }
 
-// The same value by value, for tensors that begin anywhere and for their last values: lane l takes every 32nd.
+// The same value by value, for moments that begin anywhere and for a tensor's last values: lane l takes every 32nd.
 template <typename T, typename G, bool k8, typename P>
 __device__ __forceinline__ void adam_unit_single(const P& p, const AdamNow& now, const AdamEntry& e, int64_t at) {
   const int lane = threadIdx.x & 31;
@@ -209,10 +281,10 @@ __device__ __forceinline__ void adam_unit_single(const P& p, const AdamNow& now,
     if (i >= count) continue;
     const uint32_t h = adam_mixed((uint32_t)(at + i) * 0x9E3779B1u + key);
     const float y = ((fabsf(m[j]) * inverse_m) * kTopM) * adam_down(), z = ((r[j] * inverse_v) * kTopV) * adam_down();
-    uint32_t a = min((__float_as_uint(y) + ((h & 0xffffu) << 4) + 8u) >> 20, 127u);
-    uint32_t b = min((__float_as_uint(z) + ((h >> 16) << 3) + 4u) >> 19, 255u);
-    a = inverse_m > 0.0f ? a + (m[j] < 0.0f && a > 0u ? 128u : 0u) : 0u;
-    b = inverse_v > 0.0f ? (r[j] > 0.0f ? max(b, 1u) : b) : 0u;
+    uint32_t a = min((__float_as_uint(y) + (h << 4 & 0xffff0u) + 8u) >> 20, 127u) | (__float_as_uint(m[j]) >> 24 & 128u);
+    uint32_t b = max(min((__float_as_uint(z) + (h >> 13 & 0x7fff8u) + 4u) >> 19, 255u), min(__float_as_uint(r[j]), 1u));
+    a = inverse_m > 0.0f ? a : 0u;
+    b = inverse_v > 0.0f ? b : 0u;
     static_cast<uint8_t*>(e.m)[at + i] = (uint8_t)a;
     static_cast<uint8_t*>(e.v)[at + i] = (uint8_t)b;
   }
@@ -250,35 +322,42 @@ __global__ void __launch_bounds__(kAdamThreads) hc_adamw_kernel(const __grid_con
     }
     const AdamEntry& e = p.entry[t];
     const int64_t at = (int64_t)(unit - e.first) * kAdamUnit;
-    const uintptr_t places = reinterpret_cast<uintptr_t>(e.param) | reinterpret_cast<uintptr_t>(e.grad) |
-                             (k8 ? (reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v)) << 1 : reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v));
-    if (at + kAdamUnit <= e.n && (places & 15u) == 0) adam_unit_vector<T, G, k8>(p, now, e, at);
-    else adam_unit_single<T, G, k8>(p, now, e, at);
+    const uintptr_t own = reinterpret_cast<uintptr_t>(e.param) | reinterpret_cast<uintptr_t>(e.grad), moments = reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v);
+    if (at + kAdamUnit > e.n || moments & (k8 ? 3u : 15u)) adam_unit_single<T, G, k8>(p, now, e, at);
+    else if (own & 15u) adam_unit_vector<T, G, k8, false>(p, now, e, at);
+    else adam_unit_vector<T, G, k8, true>(p, now, e, at);
   }
 }
 
-// What moments in 8 bits stand for.
+// What moments in 8 bits stand for.  Four neighbours a thread, four times.
 __global__ void __launch_bounds__(256) hc_adamw_values_kernel(const uint8_t* m, const uint8_t* v, const float2* scales, int64_t n, float* m_out, float* v_out, bool vector) {
-  const int64_t groups = (n + 7) / 8;
-  for (int64_t k = blockIdx.x * 256ll + threadIdx.x; k < groups; k += gridDim.x * 256ll) {
-    const int64_t i = k * 8;
-    const float2 scale = scales[i / kAdamUnit];
-    float a[8], b[8];
-    if (vector && i + 8 <= n) {
-      const uint2 cm = *reinterpret_cast<const uint2*>(m + i), cv = *reinterpret_cast<const uint2*>(v + i);
+  constexpr int kAtOnce = 4;
+  for (int64_t first = blockIdx.x * (1024ll * kAtOnce); first < n; first += gridDim.x * (1024ll * kAtOnce)) {
+    uint32_t cm[kAtOnce], cv[kAtOnce];
+    float2 scale[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] = adam_m_of((j < 4 ? cm.x : cm.y) >> (j % 4 * 8) & 255u, scale.x);
-        const float r = adam_root_of((j < 4 ? cv.x : cv.y) >> (j % 4 * 8) & 255u, scale.y);
-        b[j] = r * r;
-      }
-      store8(m_out + i, a);
-      store8(v_out + i, b);
-    } else {
-      for (int j = 0; j < 8 && i + j < n; ++j) {
-        m_out[i + j] = adam_m_of(m[i + j], scale.x);
-        const float r = adam_root_of(v[i + j], scale.y);
-        v_out[i + j] = r * r;
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t i = first + k * 1024 + threadIdx.x * 4;
+      if (!vector || i + 4 > n) continue;
+      cm[k] = *reinterpret_cast<const uint32_t*>(m + i);
+      cv[k] = *reinterpret_cast<const uint32_t*>(v + i);
+      scale[k] = scales[i / kAdamUnit];
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t i = first + k * 1024 + threadIdx.x * 4;
+      if (vector && i + 4 <= n) {
+        float a[4], b[4];
+        adam_decode4(cm[k], cv[k], scale[k], a, b);
+        *reinterpret_cast<float4*>(m_out + i) = make_float4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<float4*>(v_out + i) = make_float4(b[0], b[1], b[2], b[3]);
+      } else {
+        for (int64_t j = i; j < i + 4 && j < n; ++j) {
+          const float2 s = scales[j / kAdamUnit];
+          const float root = adam_root_of(v[j], s.y);
+          m_out[j] = adam_m_of(m[j], s.x);
+          v_out[j] = root * root;
+        }
       }
     }
   }
@@ -380,8 +459,8 @@ int hc_adamw_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const flo
   if (n > (1ull << 39)) return kErrArgument;
   if (n == 0) return kOk;
   if (!exp_avg || !exp_avg_sq || !scales || !m || !v || !lies_at(scales, 8) || !lies_at(m, 4) || !lies_at(v, 4)) return kErrArgument;
-  const bool vector = lies_at(exp_avg, 8) && lies_at(exp_avg_sq, 8) && lies_at(m, 16) && lies_at(v, 16);
-  const size_t blocks = ((n + 7) / 8 + 255) / 256, most = (size_t)(device_info().sms > 0 ? device_info().sms : 1) * 8;
+  const bool vector = lies_at(exp_avg, 4) && lies_at(exp_avg_sq, 4) && lies_at(m, 16) && lies_at(v, 16);
+  const size_t blocks = (n + 4095) / 4096, most = (size_t)(device_info().sms > 0 ? device_info().sms : 1) * 8;
   dev::hc_adamw_values_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(exp_avg, exp_avg_sq, reinterpret_cast<const float2*>(scales), (int64_t)n, m, v,
                                                                                            vector);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
