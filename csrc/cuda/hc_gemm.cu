@@ -51,6 +51,7 @@ struct GemmParams {
   float ca, cb, cc;
   const float* scale;
   const unsigned int* most;
+  const float* factor;
   GemmLoss loss;
   int tma_out, tma_out2, tma_in, tma_in2;              // moved by TMA: rows that begin at 16 bytes
   int wide_boxes;                                      // map_out and map_out2 are of boxes of 32 x 64 values
@@ -214,8 +215,8 @@ __device__ __forceinline__ void gemm_finish(const GemmParams& p, int z, int row0
   const int64_t count = row < p.m ? p.n - col0 : 0;  // columns of this row (may be over 32)
   unsigned char* second = slot + kSlot / 2;
   if (MODE == kGemmLinear) {
-    if (p.most) {
-      const float power = gradient_power(p.most, -1);
+    if (p.most || p.factor) {
+      const float power = (p.most ? gradient_power(p.most, -1) : 1.0f) * (p.factor ? *p.factor : 1.0f);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= power;
     }
@@ -335,8 +336,8 @@ __device__ __forceinline__ void gemm_fetch(const GemmParams& p, int z, int row0,
 __device__ __forceinline__ void gemm_finish_half(const GemmParams& p, float (&v)[32], int half, unsigned char* out, unsigned char* z, float bias,
                                                  float* shared_bias) {
   const int lane = threadIdx.x & 31;
-  if (p.most) {
-    const float power = gradient_power(p.most, -1);
+  if (p.most || p.factor) {
+    const float power = (p.most ? gradient_power(p.most, -1) : 1.0f) * (p.factor ? *p.factor : 1.0f);
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] *= power;
   }
@@ -1067,6 +1068,7 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.cc = c.cc;
   p.scale = c.scale;
   p.most = c.most;
+  p.factor = c.factor;
   p.loss = c.loss;
   if (MODE == kGemmLossSums || MODE == dev::kGemmLossSumsWide) return cudaSuccess;
   if (MODE == kGemmLossGrad) return make_side_map(&p.map_out, c.out, c.type, c, true, false, BN >= 128) ? cudaSuccess : cudaErrorInvalidValue;

@@ -130,6 +130,7 @@ struct GemmCall {
   float ca, cb, cc;
   const float* scale;  // of each matrix of a batch (kGemmPoly, kGemmUpdate): X is that times what is stored
   const unsigned int* most;  // kGemmLinear without anything behind it: see gradient_power, whose inverse the result is taken times; or NULL
+  const float* factor;       // the same: a number that the result is taken times; or NULL
   GemmLoss loss;             // kGemmLossSums, kGemmLossGrad
 };
 

@@ -117,15 +117,17 @@ __global__ void __launch_bounds__(1024) hc_loss_reduce_kernel(const float* losse
   if (reduction != kNone) *loss = (float)(reduction == kMean ? sum / (double)kept : sum);
 }
 
-// Each row's weight in the gradient, and the bits of the largest of them.
+// Each row's weight in the gradient, and the bits of the largest of them.  Where all rows weigh the same G is formed with weights of 1 and the results are taken times `factor`: of a token that a row
+// hardly expects G is then -1 to within p, and what rounding G costs is less.
 __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss, const int64_t* tokens, int64_t ignore, int64_t rows, int64_t vocab, int reduction,
-                                                              const float* count, float* weight, unsigned int* most) {
+                                                              const float* count, float* weight, unsigned int* most, float* factor) {
   unsigned int largest = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && factor) *factor = reduction == kSum ? dloss[0] : *count > 0.0f ? dloss[0] / *count : 0.0f;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows; i += gridDim.x * 256ll) {
     const int64_t token = tokens[i];
     float a = 0.0f;
     if (token != ignore) {
-      a = reduction == kNone ? dloss[i] : reduction == kMean ? dloss[0] / *count : dloss[0];
+      a = reduction == kNone ? dloss[i] : 1.0f;
       if (token < 0 || token >= vocab) a = __int_as_float(0x7fc00000);
     }
     weight[i] = a;
@@ -136,10 +138,11 @@ __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss
   if (most && (threadIdx.x & 31) == 0 && largest) atomicMax(most, largest);
 }
 
-// dx in its own type, from the parts of its sum, which is times 2^k (gradient_power)
+// dx in its own type, from the parts of its sum, which is times 2^k (gradient_power) and, over `factor`, of weights of 1
 template <typename T>
-__global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64_t from_stride, int parts, int64_t rows, int64_t width, const unsigned int* most, T* dx, int64_t stride) {
-  const float power = most ? gradient_power(most, -1) : 1.0f;
+__global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64_t from_stride, int parts, int64_t rows, int64_t width, const unsigned int* most, const float* factor, T* dx,
+                                                         int64_t stride) {
+  const float power = (most ? gradient_power(most, -1) : 1.0f) * (factor ? *factor : 1.0f);
   const int64_t groups = (width + 7) / 8;
   const bool vector = stride % 8 == 0 && (reinterpret_cast<uintptr_t>(dx) & 15u) == 0;
   for (int64_t k = blockIdx.x * 256ll + threadIdx.x; k < rows * groups; k += gridDim.x * 256ll) {
@@ -300,9 +303,10 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
   unsigned char* at = static_cast<unsigned char*>(scratch);
   float *dx_sum = reinterpret_cast<float*>(at + l.dx), *row_weight = reinterpret_cast<float*>(at + l.weight);
   unsigned int* most = type == kF16 ? reinterpret_cast<unsigned int*>(at + l.most) : nullptr;
+  float* factor = reduction != dev::kNone ? reinterpret_cast<float*>(at + l.most + 4) : nullptr;
   if (most && cudaMemsetAsync(most, 0, sizeof(*most), stream) != cudaSuccess) return kErrCuda;
   const size_t blocks = (rows + 255) / 256;
-  dev::hc_loss_weights_kernel<<<(unsigned)(blocks < 256 ? blocks : 256), 256, 0, stream>>>(dloss, tokens, ignore, (int64_t)rows, (int64_t)vocab, reduction, stats + rows, row_weight, most);
+  dev::hc_loss_weights_kernel<<<(unsigned)(blocks < 256 ? blocks : 256), 256, 0, stream>>>(dloss, tokens, ignore, (int64_t)rows, (int64_t)vocab, reduction, stats + rows, row_weight, most, factor);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   const int64_t dx_ld = (int64_t)up(inner, 8);
   for (size_t first = 0; first < vocab; first += l.piece) {
@@ -324,6 +328,7 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
     c.loss.lse = stats;
     c.loss.weight = row_weight;
     if (launch_loss_grad(c, stream) != cudaSuccess) return kErrCuda;
+    c.factor = factor;
     if (dweight) {
       c.m = n, c.n = inner, c.k = rows;
       c.a = {at, g_ld, 0, false};
@@ -339,6 +344,7 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
       c.out = {dx_sum, dx_ld, (int64_t)rows * dx_ld};
       c.parts = l.parts;
       c.most = nullptr;
+      c.factor = nullptr;
       if (first) c.in = c.out;
       if (launch_gemm(c, stream) != cudaSuccess) return kErrCuda;
     }
@@ -347,9 +353,9 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
   const size_t dx_blocks = (rows * (up(inner, 8) / 8) + 255) / 256;
   const unsigned grid = (unsigned)(dx_blocks < 2368 ? dx_blocks : 2368);
   if (type == kBf16)
-    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, static_cast<__nv_bfloat16*>(dx), (int64_t)dx_stride);
+    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, factor, static_cast<__nv_bfloat16*>(dx), (int64_t)dx_stride);
   else
-    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, static_cast<__half*>(dx), (int64_t)dx_stride);
+    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, factor, static_cast<__half*>(dx), (int64_t)dx_stride);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 

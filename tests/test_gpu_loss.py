@@ -91,6 +91,14 @@ def test_rows_with_weights(rows, inner, vocab, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("rows", [1, 7, 8, 9, 16, 17])
+def test_few_rows_over_large_vocabularies(rows, kind):
+    for inner, vocab in ((72, 50257), (8, 20001), (1000, 19003), (33, 30000)):
+        check(*make(rows, inner, vocab, kind, rows + inner))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
 @pytest.mark.parametrize("reduction,upstream", [("sum", 1.0), ("mean", 1.0), ("mean", 4096.0), ("sum", 2.0 ** -20), ("mean", 0.0)])
 def test_reductions(reduction, upstream, kind):
     check(*make(70, 96, 1003, kind, 5), reduction, upstream)
