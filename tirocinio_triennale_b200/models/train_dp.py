@@ -70,7 +70,7 @@ def run(args, compressed: bool, rank: int, world: int, device):
         ck = torch.load("%s.%s.rank%d" % (args.resume, arm, rank), map_location=device, weights_only=False)
         model.load_state_dict(ck["model"])
         opt.load_state_dict(ck["opt"])
-        g.set_state(ck["gen"])
+        g.set_state(ck["gen"].cpu())  # map_location has moved it
         start = int(ck["step"])
     losses = []
     t0 = None
