@@ -1,0 +1,55 @@
+"""Rules that the kernels of attention, the loss from hidden rows and the optimiser's step keep, read off their sources: every wait has a limit, whoever waits leaves in order."""
+import re
+from pathlib import Path
+
+import pytest
+
+CUDA = Path(__file__).resolve().parent.parent / "csrc" / "cuda"
+SOURCES = ["hc_attention.cu", "hc_loss.cu", "hc_adamw.cu", "hc_tensor.cuh"]
+
+
+def _code(name):
+    return re.sub(r"//[^\n]*", "", (CUDA / name).read_text())
+
+
+def _body(code, start):
+    at = code.index(start)
+    depth, i = 0, code.index("{", at)
+    for i in range(i, len(code)):
+        depth += {"{": 1, "}": -1}.get(code[i], 0)
+        if depth == 0:
+            return code[at:i + 1]
+
+
+@pytest.mark.parametrize("name", SOURCES)
+def test_waits_have_a_limit(name):
+    code = _code(name)
+    if name == "hc_attention.cu":
+        wait = _body(code, "bool attn_wait(")
+        assert "kAttnLimitNs" in wait and "gave_up" in wait and "return false" in wait
+        code = code.replace(wait, "")
+        assert all("kAttnLimitNs" in call for call in re.findall(r"mbar_wait_bounded\(([^;]*);", code))
+    assert not re.search(r"mbarrier\.(try_wait|test_wait)|mbar_try_wait|mbar_wait\(", code)
+    assert not re.search(r"ld\.(acquire|volatile|relaxed)\.|atomicCAS|while \(\s*(true|1|!)", code)
+    assert '"bar.sync' not in code
+
+
+def test_clusters_meet_outside_of_the_roles():
+    """A cluster's barrier has no limit: all threads of all CTAs come to it in any case, behind the barrier of the whole CTA that every role ends at."""
+    code = _code("hc_attention.cu")
+    assert len(re.findall(r"barrier\.cluster", code)) == 2  # arrive and wait, in one place
+    for kernel in ("hc_attention_kernel(", "hc_attention_backward_kernel("):
+        body = _body(code[code.index("__global__ void __launch_bounds__(AttnShape<kD>::k" + ("Forward" if kernel == "hc_attention_kernel(" else "Backward")):], kernel)
+        ended = body.split("attn_end<S::kColumns>(tmem);")
+        assert len(ended) == 2 and "cluster_meet" not in ended[0] and ended[1].count("cluster_meet(p.splits);") == 2
+        assert "return;" not in ended[0].split("attn_begin<")[1]
+
+
+def test_no_load_goes_to_several_ctas():
+    assert "multicast" not in _code("hc_attention.cu") and "multicast" not in _code("hc_loss.cu")
+
+
+def test_no_other_sums_are_added_to_by_atomics():
+    """Atomics find the largest of something, which has no order, and set the status."""
+    for name in SOURCES:
+        assert set(re.findall(r"atomic\w+", _code(name))) <= {"atomicMax"}
