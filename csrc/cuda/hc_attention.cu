@@ -671,7 +671,8 @@ __device__ __forceinline__ float ds_power(const unsigned int* most, int sign) {
 //
 // delta from the rounded O, whose probabilities were rounded too, is wrong by some 2^-9 of itself, and all of a row's dS with it: half of the error of dQ and dK (1024 x 1024, 2.8e-3 of dQ's norm, where
 // all other roundings come to 2.5e-3).  The rows of dS sum to 0, so the sum of what they are instead is what delta lacks: r = sum_j P (dP - delta).  The queries' pass finds r on
-// its way, sums P K beside dS K, and gives dQ = scale (dS K - r P K); delta + r goes to the keys' pass, which comes behind it.
+// its way, sums P K beside dS K, and gives dQ = scale (dS K - r P K); delta + r goes to the keys' pass, which comes behind it.  For dQ, r is
+// the sum of the rounded dS, so that of what their rounding adds up to the keys' mean has no part either.
 template <typename T, int kD, bool kKeys>
 __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>::kResident) hc_attention_backward_kernel(const __grid_constant__ AttnParams p) {
   using S = AttnShape<kD>;
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   constexpr bool kF16 = operand_format<T>() == 0;
   extern __shared__ unsigned char raw[];
   __shared__ AttnBarriers sh;
-  __shared__ float lacking[kParts][kTile];
+  __shared__ float2 lacking[kParts][kTile];  // sums of a row's dS, and of the rounded
   unsigned char *tile1 = attn_tiles(raw), *tile2 = tile1 + S::kBytes, *ring = tile2 + S::kBytes;
   float* sides = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // of a step of queries: less, delta
   // what the CTAs of a cluster join lies where the operands were: dV and dK side by side
@@ -790,7 +791,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     const bool in = t < (kKeys ? p.tk : p.tq);
     const int64_t side = ((int64_t)b * p.heads + head) * p.less_ld + t;
     float delta = 0.0f;
-    Pair less = pair(-INFINITY, -INFINITY), delta2 = pair(0.0f, 0.0f), lacks = pair(0.0f, 0.0f);
+    Pair less = pair(-INFINITY, -INFINITY), delta2 = pair(0.0f, 0.0f), lacks = pair(0.0f, 0.0f), rounded = pair(0.0f, 0.0f);
     if (!kKeys && in) {
       delta = p.delta[side];
       less = pair(p.less[side], p.less[side]);
@@ -883,8 +884,12 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
       }
 #pragma unroll
       for (int n = 0; n < 32; n += 2) {
-        if (!kKeys) lacks = lacks + pair(d[n], d[n + 1]);
         words[n / 2] = pack2<T>(d[n], d[n + 1]);
+        if (!kKeys) {
+          lacks = lacks + pair(d[n], d[n + 1]);
+          unpack2<T>(words[n / 2], d[n], d[n + 1]);
+          rounded = rounded + pair(d[n], d[n + 1]);
+        }
       }
       tc_store16(dp_at, words);
       tc_store_wait();
@@ -906,14 +911,17 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     if (!ok && kKeys && p.splits > 1)  // a wait ran out: no numbers
       for (int c = 0; c < 64; ++c) joined[row * kRow + part * 64 + c] = __int_as_float(0x7fc00000);
     if (ok && !kKeys) {
-      lacking[part][row] = both(lacks) * back;
+      lacking[part][row] = make_float2(both(lacks) * back, both(rounded) * back);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.met);
       ok = attn_wait_all(&sh.met, 0, sh);
-      float r = 0.0f;
+      float lack = 0.0f, r = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) r += lacking[k][row];
-      if (ok && in && part == 0) p.delta[side] = delta + r;
+      for (int k = 0; k < kParts; ++k) {
+        lack += lacking[k][row].x;
+        r += lacking[k][row].y;
+      }
+      if (ok && in && part == 0) p.delta[side] = delta + lack;
       tc_fence_after();
       // 32 of the columns each
       static_assert(kParts * 32 == kD, "a part's columns");
