@@ -258,8 +258,9 @@ __device__ __forceinline__ uint32_t ones_below(int n) { return n >= 32 ? 0xfffff
 __device__ __forceinline__ uint32_t seen_bits(int low, int high, int sinks, int at) { return ones_below(high - at) & (~ones_below(low - at) | ones_below(sinks - at)); }
 
 // barriers and tensor memory; by all threads.  `rows`: warps that work on a step, `released`: roles that have to be done with a stage.
-template <int kColumns>
-__device__ __forceinline__ void attn_begin(AttnBarriers& sh, int warps, int rows, int released) {
+// `loads`: by thread 0 as soon as the barriers are there, so that the first copies are on their way meanwhile.
+template <int kColumns, typename F>
+__device__ __forceinline__ void attn_begin(AttnBarriers& sh, int warps, int rows, int released, F loads) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 16; ++i) {
       mbar_init(&sh.full[i], 1);
@@ -280,6 +281,7 @@ __device__ __forceinline__ void attn_begin(AttnBarriers& sh, int warps, int rows
     }
     sh.gave_up = 0;
     fence_mbar_init();
+    loads();
   }
   if (threadIdx.x >> 5 == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(kColumns) : "memory");
@@ -377,22 +379,24 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
   const KeySteps list = key_steps(p, p0[0], max(p1[0], p1[1]));
   const int e0 = (int)((int64_t)list.count * split / p.splits), e1 = (int)((int64_t)list.count * (split + 1) / p.splits);
   // One tile of queries is worked on twice, with every second step of the keys each.
-  attn_begin<S::kColumns>(sh, 8, 4, p.packed ? 1 : 2);
+  attn_begin<S::kColumns>(sh, 8, 4, p.packed ? 1 : 2, [&] {
+    if (e0 >= e1) return;
+    const bool second = !p.packed && first + kTile < p.tq;
+    if (p.packed) {
+      mbar_expect_tx(&sh.first, p.packed * 128 * S::kBoxes);
+      for (int i = 0; i < S::kBoxes; ++i) load_4d(tiles + i * kTile * 128, &p.q, i * 64, 0, head * p.group, b, &sh.first);
+    } else {
+      mbar_expect_tx(&sh.first, second ? 2 * S::kBytes : S::kBytes);
+      load_rows<kD, kTile>(tiles, &p.q, first, head, b, &sh.first);
+      if (second) load_rows<kD, kTile>(tiles + S::kBytes, &p.q, first + kTile, head, b, &sh.first);
+    }
+  });
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   constexpr int kRing = kStages / 2;  // of keys; behind it that of values
   unsigned char* v_ring = ring + kRing * S::kStepBytes;
   if (warp == 0) {
     if (lane == 0 && e0 < e1) {
       Ring<kRing> rk, rv;
-      const bool second = !p.packed && first + kTile < p.tq;
-      if (p.packed) {
-        mbar_expect_tx(&sh.first, p.packed * 128 * S::kBoxes);
-        for (int i = 0; i < S::kBoxes; ++i) load_4d(tiles + i * kTile * 128, &p.q, i * 64, 0, head * p.group, b, &sh.first);
-      } else {
-        mbar_expect_tx(&sh.first, second ? 2 * S::kBytes : S::kBytes);
-        load_rows<kD, kTile>(tiles, &p.q, first, head, b, &sh.first);
-        if (second) load_rows<kD, kTile>(tiles + S::kBytes, &p.q, first + kTile, head, b, &sh.first);
-      }
       for (int e = e0; e < e1; ++e) {
         const int k0 = list.at(e);
         if (!attn_wait(&sh.empty[rk.s], rk.phase ^ 1, sh)) break;
@@ -704,14 +708,16 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   const int p0 = p.off + t0, p1 = p.off + min(t0 + kTile, p.tq) - 1;
   const KeySteps list = kKeys ? KeySteps{0, 0, 0} : key_steps(p, p0, p1);
   const int own_heads = p.group / p.splits, count = kKeys ? q_steps * own_heads : list.count;
-  attn_begin<S::kColumns>(sh, 8 * kGroups, 8, 1);
+  attn_begin<S::kColumns>(sh, 8 * kGroups, 8, 1, [&] {
+    if (!count) return;
+    mbar_expect_tx(&sh.first, 2 * S::kBytes);
+    load_rows<kD, kTile>(tile1, kKeys ? &p.k_tile : &p.q_tile, t0, head, b, &sh.first);
+    load_rows<kD, kTile>(tile2, kKeys ? &p.v_tile : &p.dout_tile, t0, head, b, &sh.first);
+  });
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   if (warp == 0) {
     if (lane == 0 && count) {
       Ring<kStages> r;
-      mbar_expect_tx(&sh.first, 2 * S::kBytes);
-      load_rows<kD, kTile>(tile1, kKeys ? &p.k_tile : &p.q_tile, t0, head, b, &sh.first);
-      load_rows<kD, kTile>(tile2, kKeys ? &p.v_tile : &p.dout_tile, t0, head, b, &sh.first);
       int h = kKeys ? head * p.group + rank * own_heads : head / p.group, step = 0;
       for (int e = 0; e < count; ++e) {
         if (!attn_wait(&sh.empty[r.s], r.phase ^ 1, sh)) break;
