@@ -314,7 +314,7 @@ __device__ __forceinline__ void warp_arrives(uint64_t* bar) {
 // kCount of a row's values, `factor` times what tensor memory has, from `to` on; `d`: how many the row has from there.  `there`, the same for all of a warp: tensor memory has them; `none`: zeros.
 template <typename O, int kCount>
 __device__ __forceinline__ void store_row(uint32_t from, O* to, int d, float factor, bool in, bool there, bool none) {
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < kCount; c += 32) {
     float v[32];
     if (there) {
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
       if (some) {
         // where the registers do not hold all of a row's scores they are read twice
         constexpr int kHeld = kD == 128 ? 2 : 1;
-        float v[kHeld][32], tops[4];
+        float v[kHeld][32];
         const bool whole = all_seen(p, p0[q], p1[q], k0, kStep);
         const int high = position + 1 - k0, low = position - p.window + 1 - k0, sinks = min(p.sinks - k0, high);
         const auto read = [&](int c, float(&w)[32]) {
@@ -495,19 +495,19 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
             for (int j = 0; j < 32; ++j) w[j] = seen >> j & 1 ? w[j] : -INFINITY;
           }
         };
-#pragma unroll
+        float top = -INFINITY;
+#pragma unroll kHeld
         for (int c = 0; c < 2; ++c) {
           float(&w)[32] = v[c % kHeld];
           read(c, w);
+          float tops[2] = {fmaxf(w[0], w[1]), fmaxf(w[16], w[17])};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& m = tops[c * 2 + h];
-            m = fmaxf(w[h * 16], w[h * 16 + 1]);
-#pragma unroll
-            for (int j = 2; j < 16; j += 2) m = max3(m, w[h * 16 + j], w[h * 16 + j + 1]);
+          for (int j = 2; j < 16; j += 2) {
+            tops[0] = max3(tops[0], w[j], w[j + 1]);
+            tops[1] = max3(tops[1], w[16 + j], w[17 + j]);
           }
+          top = max3(top, tops[0], tops[1]);
         }
-        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
         const bool grows = top > most + slack;
         if (__any_sync(0xffffffffu, grows)) {
           float factor = 1.0f;
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
         }
         const Pair scale = pair(p.scale2, p.scale2), less = pair(-ref, -ref);
         Pair total[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
-#pragma unroll
+#pragma unroll kHeld
         for (int c = 0; c < 2; ++c) {
           float(&w)[32] = v[c % kHeld];
           if (kHeld == 1) read(c, w);
