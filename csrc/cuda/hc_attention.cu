@@ -481,78 +481,84 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
       if (!ok) break;
       tc_fence_after();
       if (some) {
-        // where the registers do not hold all of a row's scores they are read twice
-        constexpr int kHeld = kD == 128 ? 2 : 1;
-        float v[kHeld][32];
-        const bool whole = all_seen(p, p0[q], p1[q], k0, kStep);
-        const int high = position + 1 - k0, low = position - p.window + 1 - k0, sinks = min(p.sinks - k0, high);
-        const auto read = [&](int c, float(&w)[32]) {
-          tc_load32(s_at + c * 32, w);
-          tc_load_wait(w);
-          if (!whole) {
-            const uint32_t seen = seen_bits(low, high, sinks, c * 32);
+        // twice, so that the steps that are seen as a whole, most of them, run through no code for the others
+        const auto take = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
+          // where the registers do not hold all of a row's scores they are read twice
+          constexpr int kHeld = kD == 128 ? 2 : 1;
+          float v[kHeld][32];
+          const int high = position + 1 - k0, low = position - p.window + 1 - k0, sinks = min(p.sinks - k0, high);
+          const auto read = [&](int c, float(&w)[32]) {
+            tc_load32(s_at + c * 32, w);
+            tc_load_wait(w);
+            if (kMasked) {
+              const uint32_t seen = seen_bits(low, high, sinks, c * 32);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) w[j] = seen >> j & 1 ? w[j] : -INFINITY;
-          }
-        };
-        float top = -INFINITY;
+              for (int j = 0; j < 32; ++j) w[j] = seen >> j & 1 ? w[j] : -INFINITY;
+            }
+          };
+          float top = -INFINITY;
 #pragma unroll kHeld
-        for (int c = 0; c < 2; ++c) {
-          float(&w)[32] = v[c % kHeld];
-          read(c, w);
-          float tops[2] = {fmaxf(w[0], w[1]), fmaxf(w[16], w[17])};
+          for (int c = 0; c < 2; ++c) {
+            float(&w)[32] = v[c % kHeld];
+            read(c, w);
+            float tops[2] = {fmaxf(w[0], w[1]), fmaxf(w[16], w[17])};
 #pragma unroll
-          for (int j = 2; j < 16; j += 2) {
-            tops[0] = max3(tops[0], w[j], w[j + 1]);
-            tops[1] = max3(tops[1], w[16 + j], w[17 + j]);
+            for (int j = 2; j < 16; j += 2) {
+              tops[0] = max3(tops[0], w[j], w[j + 1]);
+              tops[1] = max3(tops[1], w[16 + j], w[17 + j]);
+            }
+            top = max3(top, tops[0], tops[1]);
           }
-          top = max3(top, tops[0], tops[1]);
-        }
-        const bool grows = top > most + slack;
-        if (__any_sync(0xffffffffu, grows)) {
-          float factor = 1.0f;
-          if (grows) {
-            factor = power2((most - top) * p.scale2);
-            most = top;
-            ref = top * p.scale2 - kBias;
-            sum *= factor;
-          }
-          if (taken) {
-            // O has everything up to the step before
-            ok = attn_wait_all(&sh.done[q * kSlots + (taken - 1) % kSlots], ((taken - 1) / kSlots) & 1, sh);
-            if (!ok) break;
-            tc_fence_after();
+          const bool grows = top > most + slack;
+          if (__any_sync(0xffffffffu, grows)) {
+            float factor = 1.0f;
+            if (grows) {
+              factor = power2((most - top) * p.scale2);
+              most = top;
+              ref = top * p.scale2 - kBias;
+              sum *= factor;
+            }
+            if (taken) {
+              // O has everything up to the step before
+              ok = attn_wait_all(&sh.done[q * kSlots + (taken - 1) % kSlots], ((taken - 1) / kSlots) & 1, sh);
+              if (!ok) return;
+              tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < kD; c += 32) {
-              float o[32];
-              tc_load32(o_at + c, o);
-              tc_load_wait(o);
+              for (int c = 0; c < kD; c += 32) {
+                float o[32];
+                tc_load32(o_at + c, o);
+                tc_load_wait(o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] *= factor;
-              tc_store32(o_at + c, o);
+                for (int j = 0; j < 32; ++j) o[j] *= factor;
+                tc_store32(o_at + c, o);
+              }
             }
           }
-        }
-        const Pair scale = pair(p.scale2, p.scale2), less = pair(-ref, -ref);
-        Pair total[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+          const Pair scale = pair(p.scale2, p.scale2), less = pair(-ref, -ref);
+          Pair total[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll kHeld
-        for (int c = 0; c < 2; ++c) {
-          float(&w)[32] = v[c % kHeld];
-          if (kHeld == 1) read(c, w);
-          uint32_t words[16];
+          for (int c = 0; c < 2; ++c) {
+            float(&w)[32] = v[c % kHeld];
+            if (kHeld == 1) read(c, w);
+            uint32_t words[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float x, y;
-            parts(fma2(pair(w[j], w[j + 1]), scale, less), x, y);
-            x = power2(x);
-            y = power2(y);
-            total[j / 2 % 2] = total[j / 2 % 2] + pair(x, y);
-            words[j / 2] = pack2<T>(x, y);
+            for (int j = 0; j < 32; j += 2) {
+              float x, y;
+              parts(fma2(pair(w[j], w[j + 1]), scale, less), x, y);
+              x = power2(x);
+              y = power2(y);
+              total[j / 2 % 2] = total[j / 2 % 2] + pair(x, y);
+              words[j / 2] = pack2<T>(x, y);
+            }
+            tc_store16(s_at + c * 16, words);
           }
-          tc_store16(s_at + c * 16, words);
-        }
-        sum += both(total[0] + total[1]);
-        tc_store_wait();
+          sum += both(total[0] + total[1]);
+          tc_store_wait();
+        };
+        if (all_seen(p, p0[q], p1[q], k0, kStep)) take(std::false_type());
+        else take(std::true_type());
+        if (!ok) break;
       }
       ++taken;
       warp_arrives(&sh.p_ready[slot]);
