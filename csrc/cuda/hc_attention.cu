@@ -200,6 +200,15 @@ __device__ __forceinline__ void weighted(bool leader, uint32_t d, uint32_t p, in
   for (int i = 0; i < kStep / 16; ++i) attn_mma_from_tmem(leader, d, p + i / 2 * second + i % 2 * 8, b + i * 128, idesc, add || i > 0);
 }
 
+// Registers that the warps with roles, the first four, leave to those with rows.  Together they are no more than the CTA was launched with, or the others would wait for ever.
+constexpr int kRoleRegisters = 48;
+template <int kRegisters, int kThreads, int kLaunched>
+__device__ __forceinline__ void share_registers(bool role) {
+  static_assert(128 * kRoleRegisters + (kThreads - 128) * kRegisters <= kThreads * kLaunched, "what the CTA has");
+  if (role) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegisters));
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+
 // ---- clusters -----------------------------------------------------------------------------------------------------------------
 // All threads of all CTAs of a cluster come to both of these, in any case; `all`: the cluster's size.
 __device__ __forceinline__ void cluster_meet(int all) {
@@ -392,6 +401,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
     }
   });
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  if constexpr (S::kResident == 2) share_registers<96, S::kForwardThreads, 80>(warp < 4);
   constexpr int kRing = kStages / 2;  // of keys; behind it that of values
   unsigned char* v_ring = ring + kRing * S::kStepBytes;
   if (warp == 0) {
@@ -721,6 +731,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     load_rows<kD, kTile>(tile2, kKeys ? &p.v_tile : &p.dout_tile, t0, head, b, &sh.first);
   });
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  share_registers<(S::kResident == 2 ? 96 : 104), S::kBackwardThreads, (S::kResident == 2 ? 80 : 96)>(warp < 4);
   if (warp == 0) {
     if (lane == 0 && count) {
       Ring<kStages> r;
@@ -821,91 +832,98 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
         break;
       }
       tc_fence_after();
-      float v[32];
-      tc_load32(s_at, v);
       // what this row sees, or is seen by
-      bool whole;
-      uint32_t seen;
-      if (kKeys) {
-        const int i0 = (q_first + step) * kStep, pa = p.off + i0;
-        whole = i0 + kStep <= p.tq && all_seen(p, pa, pa + kStep - 1, t0, kTile);
-        const int high = min(p.tq - i0, (int)min((int64_t)kStep, t < p.sinks ? (int64_t)kStep : (int64_t)t + p.window - pa));
-        seen = seen_bits(t - pa, high, 0, half * 32);
-        step += kGroups;
-        while (step >= q_steps) step -= q_steps;
-      } else {
-        const int k0 = list.at(e), position = p.off + t, high = position - k0 + 1;
-        whole = all_seen(p, p0, p1, k0, kStep);
-        seen = seen_bits(position - p.window + 1 - k0, high, min(p.sinks - k0, high), half * 32);
-      }
-      tc_load_wait(v);
+      const int i0 = (q_first + step) * kStep, pa = p.off + i0, k0 = kKeys ? t0 : list.at(e), position = p.off + t;
+      const bool whole = kKeys ? i0 + kStep <= p.tq && all_seen(p, pa, pa + kStep - 1, t0, kTile) : all_seen(p, p0, p1, k0, kStep);
+      // twice, so that the steps that are seen as a whole, most of them, run through no code for the others
+      const auto take = [&](auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
+        float v[32];
+        tc_load32(s_at, v);
+        uint32_t seen = 0xffffffffu;
+        if (kMasked && kKeys) {
+          const int high = min(p.tq - i0, (int)min((int64_t)kStep, t < p.sinks ? (int64_t)kStep : (int64_t)t + p.window - pa));
+          seen = seen_bits(t - pa, high, 0, half * 32);
+        } else if (kMasked) {
+          const int high = position - k0 + 1;
+          seen = seen_bits(position - p.window + 1 - k0, high, min(p.sinks - k0, high), half * 32);
+        }
+        tc_load_wait(v);
 #pragma unroll
-      for (int n = 0; n < 32; n += 4) {
-        Pair l0 = less, l1 = less;
-        if (kKeys) {
-          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(side_at + n);
-          l0 = Pair{l.x};
-          l1 = Pair{l.y};
-          if (kBias) {
-            l0 = l0 + bias;
-            l1 = l1 + bias;
+        for (int n = 0; n < 32; n += 4) {
+          Pair l0 = less, l1 = less;
+          if (kKeys) {
+            const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(side_at + n);
+            l0 = Pair{l.x};
+            l1 = Pair{l.y};
+            if (kBias) {
+              l0 = l0 + bias;
+              l1 = l1 + bias;
+            }
+          }
+          parts(fma2(pair(v[n], v[n + 1]), scale, l0), v[n], v[n + 1]);
+          parts(fma2(pair(v[n + 2], v[n + 3]), scale, l1), v[n + 2], v[n + 3]);
+        }
+#pragma unroll
+        for (int n = 0; n < 32; ++n) v[n] = power2(v[n]);
+        if (kMasked) {
+#pragma unroll
+          for (int n = 0; n < 32; ++n) v[n] = seen >> n & 1 ? v[n] : 0.0f;
+        }
+        uint32_t words[16];
+#pragma unroll
+        for (int n = 0; n < 32; n += 2) words[n / 2] = pack2<T>(v[n], v[n + 1]);
+        tc_store16(s_at, words);
+        tc_store_wait();
+        warp_arrives(&sh.p_ready[g]);
+        if (!attn_wait_all(&sh.dp_full[g], turn, sh)) {
+          ok = false;
+          return;
+        }
+        tc_fence_after();
+        float d[32];
+        tc_load32(dp_at, d);
+        tc_load_wait(d);
+#pragma unroll
+        for (int n = 0; n < 32; n += 4) {
+          Pair l0 = delta2, l1 = delta2;
+          if (kKeys) {
+            const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(side_at + 64 + n);
+            l0 = Pair{l.x};
+            l1 = Pair{l.y};
+          }
+          Pair x = fma2(l0, minus, pair(d[n], d[n + 1])) * pair(v[n], v[n + 1]), y = fma2(l1, minus, pair(d[n + 2], d[n + 3])) * pair(v[n + 2], v[n + 3]);
+          if (kF16) {
+            x = x * gain;
+            y = y * gain;
+          }
+          parts(x, d[n], d[n + 1]);
+          parts(y, d[n + 2], d[n + 3]);
+        }
+        if (kMasked) {  // also where one that is not seen, or a query that is none, has no number
+#pragma unroll
+          for (int n = 0; n < 32; ++n) d[n] = seen >> n & 1 ? d[n] : 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < 32; n += 2) {
+          words[n / 2] = pack2<T>(d[n], d[n + 1]);
+          if (!kKeys) {
+            lacks = lacks + pair(d[n], d[n + 1]);
+            unpack2<T>(words[n / 2], d[n], d[n + 1]);
+            rounded = rounded + pair(d[n], d[n + 1]);
           }
         }
-        parts(fma2(pair(v[n], v[n + 1]), scale, l0), v[n], v[n + 1]);
-        parts(fma2(pair(v[n + 2], v[n + 3]), scale, l1), v[n + 2], v[n + 3]);
+        tc_store16(dp_at, words);
+        tc_store_wait();
+        warp_arrives(&sh.ds_ready[g]);
+      };
+      if (whole) take(std::false_type());
+      else take(std::true_type());
+      if (!ok) break;
+      if (kKeys) {
+        step += kGroups;
+        while (step >= q_steps) step -= q_steps;
       }
-#pragma unroll
-      for (int n = 0; n < 32; ++n) v[n] = power2(v[n]);
-      if (!whole) {
-#pragma unroll
-        for (int n = 0; n < 32; ++n) v[n] = seen >> n & 1 ? v[n] : 0.0f;
-      }
-      uint32_t words[16];
-#pragma unroll
-      for (int n = 0; n < 32; n += 2) words[n / 2] = pack2<T>(v[n], v[n + 1]);
-      tc_store16(s_at, words);
-      tc_store_wait();
-      warp_arrives(&sh.p_ready[g]);
-      if (!attn_wait_all(&sh.dp_full[g], turn, sh)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float d[32];
-      tc_load32(dp_at, d);
-      tc_load_wait(d);
-#pragma unroll
-      for (int n = 0; n < 32; n += 4) {
-        Pair l0 = delta2, l1 = delta2;
-        if (kKeys) {
-          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(side_at + 64 + n);
-          l0 = Pair{l.x};
-          l1 = Pair{l.y};
-        }
-        Pair x = fma2(l0, minus, pair(d[n], d[n + 1])) * pair(v[n], v[n + 1]), y = fma2(l1, minus, pair(d[n + 2], d[n + 3])) * pair(v[n + 2], v[n + 3]);
-        if (kF16) {
-          x = x * gain;
-          y = y * gain;
-        }
-        parts(x, d[n], d[n + 1]);
-        parts(y, d[n + 2], d[n + 3]);
-      }
-      if (!whole) {  // also where one that is not seen, or a query that is none, has no number
-#pragma unroll
-        for (int n = 0; n < 32; ++n) d[n] = seen >> n & 1 ? d[n] : 0.0f;
-      }
-#pragma unroll
-      for (int n = 0; n < 32; n += 2) {
-        words[n / 2] = pack2<T>(d[n], d[n + 1]);
-        if (!kKeys) {
-          lacks = lacks + pair(d[n], d[n + 1]);
-          unpack2<T>(words[n / 2], d[n], d[n + 1]);
-          rounded = rounded + pair(d[n], d[n + 1]);
-        }
-      }
-      tc_store16(dp_at, words);
-      tc_store_wait();
-      warp_arrives(&sh.ds_ready[g]);
     }
     if (ok && count) ok = attn_wait_all(&sh.drained, 0, sh);
     if (ok && kKeys) {
