@@ -4,8 +4,8 @@
 //   S = scale Q K^T,  P = softmax of S over what is seen,  O = P V                (a query that sees nothing: 0)
 //   delta_i = dO_i . O_i,  dS = P (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
 //
-// Tiles of 128 queries by 128 keys; tiles that nobody sees are left out, only tiles at an edge of what is seen are masked.  One thread brings
-// operands in by TMA, one issues the matrix instructions, eight warps have a row of a tile a thread: scores, probabilities and their
+// Tiles of 128 rows, steps of 64 of the other side; steps that nobody sees are left out, only steps at an edge of what is seen are masked.  One thread brings
+// operands in by TMA, two warps issue the matrix instructions, eight or sixteen have a row of a tile a thread: scores, probabilities and their
 // gradients go from tensor memory to registers and back and never anywhere else.  The second product of each pair reads its first operand, in 16 bits, from where the
 // scores lay.  Heads and batch are dimensions of the tensor maps, so a view into a projection's result is read where it lies; several query heads to a key's head read the
 // same keys, and dK and dV of such a head are summed in one CTA.  Every sum has a fixed order.
@@ -14,7 +14,7 @@
 // 64 (16 a cycle and SM).  The reference that exponentials are taken relative to follows a row's largest score when that is more than 2^8 above it; only then is O
 // taken times a factor.  Few queries (with all heads of a key's head at most 128 rows, a new token of each text for one) are one tile, and the keys are shared
 // out to the CTAs of a cluster, which join their results over its shared memory: bound by reading keys and values.
-// Backward: dK and dV in a kernel whose CTA has a tile of keys and goes through the queries, dQ in one whose CTA has a tile of queries.  That forms the scores twice (7 products instead of 5), and
+// Backward: dK and dV in a kernel whose CTA has a tile of keys and goes through the queries, dQ in one whose CTA has a tile of queries.  That forms the scores twice (8 products instead of 5, P K below among them), and
 // needs no atomic additions, whose order would change the result, and no array of partial dQ.
 //
 // In fp16, which has no numbers below 2^-24, P is held times a power of two, and dS times one that 2 max|dO_i| max|V_j| (norms of rows, which bound it) gives.
