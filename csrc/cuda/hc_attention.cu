@@ -60,7 +60,7 @@ struct AttnShape {
 struct AttnParams {
   CUtensorMap q, k, v, dout;                          // in steps of 64 positions (forward, q: tiles)
   CUtensorMap q_tile, k_tile, v_tile, dout_tile;  // in tiles of 128 (backward)
-  void* o;
+  void* o;       // the result (backward: read)
   float* less;      // [batch heads][rows]: minus the logarithm (base 2) of a query's sum of exponentials, for the backward pass
   float* delta;  // as `less`
   void *dq, *dk, *dv;
@@ -634,48 +634,41 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
-// delta = dO . O of every query of a head (kDelta), and the largest square of a norm of dO's (or V's) rows.  Eight values a thread, four rows of a thread on their way together; a block has
+// fp16: the largest square of a norm of dO's rows (the first `blocks[0] * heads[0] * batch` blocks) and of V's.  Eight values a thread, four rows of a thread on their way together; a block has
 // 4 * 256 / kLanes rows of a head.
-template <typename T, int kLanes, bool kDelta>
-__global__ void __launch_bounds__(256) hc_attention_rows_kernel(const T* rows, int64_t stride_b, int64_t stride_h, int64_t stride_t, const T* o, int heads, int length, int d, int blocks, float* delta,
-                                                                int64_t ld, unsigned int* most) {
+struct RowsOf {
+  const void* data[2];
+  int64_t stride_b[2], stride_h[2], stride_t[2];
+  int heads[2], length[2], blocks[2];
+  int64_t first_blocks;
+};
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) hc_attention_rows_kernel(const __grid_constant__ RowsOf of, int d, unsigned int* most) {
   constexpr int kAtOnce = 4, kApart = 256 / kLanes;
-  const int head_at = blockIdx.x / blocks, b = head_at / heads, h = head_at - b * heads;
-  const int part = threadIdx.x % kLanes, first = (blockIdx.x - head_at * blocks) * (kAtOnce * kApart) + threadIdx.x / kLanes;
-  const bool has = part * 8 < d;
-  const T* from = rows + b * stride_b + h * stride_h + part * 8;
-  uint4 x[kAtOnce], y[kAtOnce];
+  const int n = blockIdx.x >= of.first_blocks, block = (int)(blockIdx.x - (n ? of.first_blocks : 0));
+  const int head_at = block / of.blocks[n], b = head_at / of.heads[n], h = head_at - b * of.heads[n];
+  const int part = threadIdx.x % kLanes, first = (block - head_at * of.blocks[n]) * (kAtOnce * kApart) + threadIdx.x / kLanes;
+  const T* from = static_cast<const T*>(of.data[n]) + b * of.stride_b[n] + h * of.stride_h[n] + part * 8;
+  uint4 x[kAtOnce];
 #pragma unroll
   for (int k = 0; k < kAtOnce; ++k) {
     const int i = first + k * kApart;
-    x[k] = y[k] = make_uint4(0, 0, 0, 0);
-    if (!has || i >= length) continue;
-    x[k] = *reinterpret_cast<const uint4*>(from + i * stride_t);
-    if (kDelta) y[k] = *reinterpret_cast<const uint4*>(o + (((int64_t)b * length + i) * heads + h) * d + part * 8);
+    x[k] = part * 8 < d && i < of.length[n] ? *reinterpret_cast<const uint4*>(from + i * of.stride_t[n]) : make_uint4(0, 0, 0, 0);
   }
+  launch_dependents();
   unsigned int largest = 0;
 #pragma unroll
   for (int k = 0; k < kAtOnce; ++k) {
-    float u[8], v[8], dot = 0.0f, square = 0.0f;
+    float u[8], square = 0.0f;
     unpack2<T>(x[k].x, u[0], u[1]), unpack2<T>(x[k].y, u[2], u[3]), unpack2<T>(x[k].z, u[4], u[5]), unpack2<T>(x[k].w, u[6], u[7]);
-    unpack2<T>(y[k].x, v[0], v[1]), unpack2<T>(y[k].y, v[2], v[3]), unpack2<T>(y[k].z, v[4], v[5]), unpack2<T>(y[k].w, v[6], v[7]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      dot = fmaf(u[j], v[j], dot);
-      square = fmaf(u[j], u[j], square);
-    }
+    for (int j = 0; j < 8; ++j) square = fmaf(u[j], u[j], square);
 #pragma unroll
-    for (int n = kLanes / 2; n > 0; n >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, n);
-      square += __shfl_xor_sync(0xffffffffu, square, n);
-    }
-    const int i = first + k * kApart;
-    if (kDelta && part == 0 && i < length) delta[head_at * ld + i] = dot;
+    for (int m = kLanes / 2; m > 0; m >>= 1) square += __shfl_xor_sync(0xffffffffu, square, m);
     if (square < INFINITY) largest = max(largest, __float_as_uint(square));
   }
-  if (!most) return;
   largest = __reduce_max_sync(0xffffffffu, largest);
-  if ((threadIdx.x & 31) == 0 && largest) atomicMax(most, largest);
+  if ((threadIdx.x & 31) == 0 && largest) atomicMax(most + n, largest);
 }
 // The power of two that dS is held times in fp16: 2 max|dO_i| max|V_j|, which |dS| does not exceed, comes to below 2^15 (from the squares of both).
 __device__ __forceinline__ float ds_power(const unsigned int* most, int sign) {
@@ -689,7 +682,8 @@ __device__ __forceinline__ float ds_power(const unsigned int* most, int sign) {
 // two CTAs are on an SM, so that exponentials, multiplications and the tensor cores' work overlap.  One warp issues the products that form scores, one those that sum.
 // Tensor memory: scores of the groups' steps, then dO V^T (P and dS at the beginning of each half's 32 columns), then the two sums.
 //
-// delta from the rounded O, whose probabilities were rounded too, is wrong by some 2^-9 of itself, and all of a row's dS with it: half of the error of dQ and dK (1024 x 1024, 2.8e-3 of dQ's norm, where
+// The queries' pass takes delta from dO and O itself (from a kernel before it all passes took 154 us instead of 151 at 8 x 12 x 1024 x 64, and one us less of 967 at 16 heads
+// on 4, 8192 x 128).  delta from the rounded O, whose probabilities were rounded too, is wrong by some 2^-9 of itself, and all of a row's dS with it: half of the error of dQ and dK (1024 x 1024, 2.8e-3 of dQ's norm, where
 // all other roundings come to 2.5e-3).  The rows of dS sum to 0, so the sum of what they are instead is what delta lacks: r = sum_j P (dP - delta).  The queries' pass finds r on
 // its way, sums P K beside dS K, and gives dQ = scale (dS K - r P K); delta + r goes to the keys' pass, which comes behind it.  For dQ, r is
 // the sum of the rounded dS, so that of what their rounding adds up to the keys' mean has no part either.
@@ -702,6 +696,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   extern __shared__ unsigned char raw[];
   __shared__ AttnBarriers sh;
   __shared__ float2 lacking[kParts][kTile];  // sums of a row's dS, and of the rounded
+  __shared__ float dots[kParts][kTile];      // parts of delta
   unsigned char *tile1 = attn_tiles(raw), *tile2 = tile1 + S::kBytes, *ring = tile2 + S::kBytes;
   float* sides = reinterpret_cast<float*>(ring + kStages * kStageBytes);  // of a step of queries: less, delta
   // what the CTAs of a cluster join lies where the operands were: dV and dK side by side
@@ -724,6 +719,16 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   const int p0 = p.off + t0, p1 = p.off + min(t0 + kTile, p.tq) - 1;
   const KeySteps list = kKeys ? KeySteps{0, 0, 0} : key_steps(p, p0, p1);
   const int own_heads = p.group / p.splits, count = kKeys ? q_steps * own_heads : list.count;
+  // for delta: 32 values of a row of O each, on their way while the CTA begins
+  uint4 y[4];
+  float less1 = 0.0f;
+  if (!kKeys && warp >= 4) {
+    const int row = (warp & 3) * 32 + lane, t = t0 + row, c = ((warp - 4) >> 2) * 32;
+    const T* o = static_cast<const T*>(p.o) + (((int64_t)b * p.tq + t) * p.heads + head) * p.d + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = t < p.tq && c + j * 8 < p.d ? *reinterpret_cast<const uint4*>(o + j * 8) : make_uint4(0, 0, 0, 0);
+    if (t < p.tq) less1 = p.less[((int64_t)b * p.heads + head) * p.less_ld + t];
+  }
   attn_begin<S::kColumns>(sh, 8 * kGroups, 8, 1, [&] {
     if (!count) return;
     mbar_expect_tx(&sh.first, 2 * S::kBytes);
@@ -733,6 +738,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   share_registers<(S::kResident == 2 ? 96 : 104), S::kBackwardThreads, (S::kResident == 2 ? 80 : 96)>(warp < 4);
   if (warp == 0) {
+    if (kKeys && lane == 0) grid_dependency_wait();  // behind the queries' pass, whose delta comes in with the queries; the norms were there when it let this kernel begin
     if (lane == 0 && count) {
       Ring<kStages> r;
       int h = kKeys ? head * p.group + rank * own_heads : head / p.group, step = 0;
@@ -808,6 +814,10 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     const int quarter = warp & 3, part = (warp - 4) >> 2, g = part >> 1, half = part & 1, row = quarter * 32 + lane, t = t0 + row;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + g * kStep + half * 32, dp_at = s_at + kDp;
     constexpr float kBias = kF16 && kKeys ? 14.0f : 0.0f;  // P^T is held times 2^14 in fp16 (what P K is for needs no more than a few bits)
+    if (!kKeys) {
+      if (kF16) grid_dependency_wait();  // behind the largest norms
+      launch_dependents();
+    }
     const float power = kF16 ? ds_power(p.most, 1) : 1.0f, back = kF16 ? ds_power(p.most, -1) : 1.0f;
     const Pair gain = pair(power * (kBias ? 1.0f / 16384.0f : 1.0f), power * (kBias ? 1.0f / 16384.0f : 1.0f));
     const Pair scale = pair(p.scale2, p.scale2), minus = pair(-1.0f, -1.0f), bias = pair(kBias, kBias);
@@ -815,9 +825,29 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     const int64_t side = ((int64_t)b * p.heads + head) * p.less_ld + t;
     float delta = 0.0f;
     Pair less = pair(-INFINITY, -INFINITY), delta2 = pair(0.0f, 0.0f), lacks = pair(0.0f, 0.0f), rounded = pair(0.0f, 0.0f);
-    if (!kKeys && in) {
-      delta = p.delta[side];
-      less = pair(p.less[side], p.less[side]);
+    if (!kKeys && count) {
+      // delta = dO . O, dO's row from the tile
+      const int c = part * 32;
+      if (in) less = pair(less1, less1);
+      attn_wait_all(&sh.first, 0, sh);  // when it runs out, so do the waits below
+      const unsigned char* at = tile2 + c / 64 * (kTile * 128) + row * 128;
+      float dot = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at + ((c % 64 / 8 + j) ^ (row & 7)) * 16);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y[j].x, y[j].y, y[j].z, y[j].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float u[2], w[2];
+          unpack2<T>(xs[k], u[0], u[1]);
+          unpack2<T>(ys[k], w[0], w[1]);
+          dot = fmaf(u[1], w[1], fmaf(u[0], w[0], dot));
+        }
+      }
+      dots[part][row] = dot;
+      asm volatile("bar.sync 1, %0;" ::"n"(256 * kGroups) : "memory");
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) delta += dots[k][row];
       delta2 = pair(delta, delta);
     }
     int step = g;
@@ -1063,21 +1093,29 @@ int kv_splits(const Sizes& s) {
   return group % 2 == 0 && tiles < slots * 8 ? 2 : 1;
 }
 
+// early: beside the kernel before it, whose results the kernel waits for where it needs them (griddepcontrol.wait).  8 x 12 heads of 64, 1024 positions, bf16, all three kernels: 151 us, 155 without.
 template <typename K>
-cudaError_t launch_clusters(K kernel, int64_t ctas, int size, int threads, int smem, cudaStream_t stream, const dev::AttnParams& p) {
+cudaError_t launch_clusters(K kernel, int64_t ctas, int size, int threads, int smem, cudaStream_t stream, const dev::AttnParams& p, bool early = false) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  memset(&attr, 0, sizeof(attr));
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)size;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = size > 1 ? 1 : 0;
+  cudaLaunchAttribute attrs[2];
+  memset(attrs, 0, sizeof(attrs));
+  cfg.attrs = attrs;
+  if (size > 1) {
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = (unsigned)size;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (early) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -1105,30 +1143,35 @@ cudaError_t run_forward(const dev::AttnParams& p, cudaStream_t stream) {
 }
 
 template <typename T, int kD>
-cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_heads& v, const void* o, float* delta, unsigned int* most, cudaStream_t stream) {
+cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_heads& v, unsigned int* most, cudaStream_t stream) {
   static unsigned long long allowed_kv = 0, allowed_q = 0;
   constexpr int smem = dev::AttnShape<kD>::kBackwardSmem;
   cudaError_t e = allow_smem(dev::hc_attention_backward_kernel<T, kD, true>, smem, &allowed_kv);
   if (e == cudaSuccess) e = allow_smem(dev::hc_attention_backward_kernel<T, kD, false>, smem, &allowed_q);
   if (e != cudaSuccess) return e;
-  constexpr int kLanes = kD / 8, kRows = 4 * 256 / kLanes;  // of a block
-  const int q_blocks = (p.tq + kRows - 1) / kRows, k_blocks = (p.tk + kRows - 1) / kRows;
-  dev::hc_attention_rows_kernel<T, kLanes, true><<<(unsigned)((int64_t)p.batch * p.heads * q_blocks), 256, 0, stream>>>(
-      static_cast<const T*>(dout.data), (int64_t)dout.batch, (int64_t)dout.head, (int64_t)dout.position, static_cast<const T*>(o), p.heads, p.tq, p.d, q_blocks, delta, p.less_ld, most);
-  if (most)
-    dev::hc_attention_rows_kernel<T, kLanes, false><<<(unsigned)((int64_t)p.batch * p.kv_heads * k_blocks), 256, 0, stream>>>(
-        static_cast<const T*>(v.data), (int64_t)v.batch, (int64_t)v.head, (int64_t)v.position, nullptr, p.kv_heads, p.tk, p.d, k_blocks, nullptr, 0, most + 1);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (most) {
+    constexpr int kLanes = kD / 8, kRows = 4 * 256 / kLanes;  // of a block
+    const dev::RowsOf of = {{dout.data, v.data},
+                            {(int64_t)dout.batch, (int64_t)v.batch},
+                            {(int64_t)dout.head, (int64_t)v.head},
+                            {(int64_t)dout.position, (int64_t)v.position},
+                            {p.heads, p.kv_heads},
+                            {p.tq, p.tk},
+                            {(p.tq + kRows - 1) / kRows, (p.tk + kRows - 1) / kRows},
+                            (int64_t)p.batch * p.heads * ((p.tq + kRows - 1) / kRows)};
+    dev::hc_attention_rows_kernel<T, kLanes><<<(unsigned)(of.first_blocks + (int64_t)p.batch * p.kv_heads * of.blocks[1]), 256, 0, stream>>>(of, p.d, most);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
   // dq or not: the keys' pass needs the delta that this one completes
   const int splits = p.splits;
   p.splits = 1;
   p.blocks = (p.tq + dev::kTile - 1) / dev::kTile;
-  e = launch_clusters(dev::hc_attention_backward_kernel<T, kD, false>, (int64_t)p.batch * p.heads * p.blocks, 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p);
+  e = launch_clusters(dev::hc_attention_backward_kernel<T, kD, false>, (int64_t)p.batch * p.heads * p.blocks, 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, most != nullptr);
   if (e != cudaSuccess || !p.dk) return e;
   p.splits = splits;
   p.blocks = (p.tk + dev::kTile - 1) / dev::kTile;
-  return launch_clusters(dev::hc_attention_backward_kernel<T, kD, true>, (int64_t)p.batch * p.kv_heads * p.blocks * splits, splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p);
+  return launch_clusters(dev::hc_attention_backward_kernel<T, kD, true>, (int64_t)p.batch * p.kv_heads * p.blocks * splits, splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, true);
 }
 
 size_t backward_bytes(const Sizes& s) { return up(s.batch * s.heads * stats_ld(s.queries) * sizeof(float), 256) + 256; }
@@ -1198,11 +1241,11 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
   if (!scratch || !lies_at(scratch, 256) || scratch_bytes < need) return kErrArgument;
   dev::AttnParams p;
   fill_attention(&p, s, window, sinks, scale);
-  float* delta = static_cast<float*>(scratch);
   unsigned int* most = type == kF16 ? reinterpret_cast<unsigned int*>(static_cast<unsigned char*>(scratch) + need - 256) : nullptr;
   if (most && cudaMemsetAsync(most, 0, 8, stream) != cudaSuccess) return kErrCuda;
   p.less = const_cast<float*>(stats);
-  p.delta = delta;
+  p.delta = static_cast<float*>(scratch);
+  p.o = const_cast<void*>(out);
   p.most = most;
   p.dq = dq, p.dk = dk, p.dv = dv;
   p.splits = kv_splits(s);
@@ -1212,8 +1255,8 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
       !map(&p.v, v, keys, kv_heads, dev::kStep) || !map(&p.v_tile, v, keys, kv_heads, dev::kTile))
     return kErrArgument;
   cudaError_t e;
-  if (type == kBf16) e = head_size <= 64 ? run_backward<__nv_bfloat16, 64>(p, dout, v, out, delta, most, stream) : run_backward<__nv_bfloat16, 128>(p, dout, v, out, delta, most, stream);
-  else e = head_size <= 64 ? run_backward<__half, 64>(p, dout, v, out, delta, most, stream) : run_backward<__half, 128>(p, dout, v, out, delta, most, stream);
+  if (type == kBf16) e = head_size <= 64 ? run_backward<__nv_bfloat16, 64>(p, dout, v, most, stream) : run_backward<__nv_bfloat16, 128>(p, dout, v, most, stream);
+  else e = head_size <= 64 ? run_backward<__half, 64>(p, dout, v, most, stream) : run_backward<__half, 128>(p, dout, v, most, stream);
   return e == cudaSuccess ? kOk : kErrCuda;
 }
 
