@@ -160,6 +160,7 @@ template <typename T, int N>
 __global__ void __launch_bounds__(256, N == 1 ? 3 : 2) hc_few_rows_loss_kernel(const __grid_constant__ FewRowsParams p) {
   constexpr int kSteps = 4;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  launch_dependents();  // the kernel that joins the sums begins and waits
   const int64_t groups = (p.width + 15) / 16, last = p.width - 1;
   const T* x[N];
   int64_t end[N];

@@ -47,13 +47,14 @@ __global__ void __launch_bounds__(1024) hc_loss_join_kernel(const float2* sums, 
   losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? all - picked[row] : __int_as_float(0x7fc00000);
 }
 
-// The same of few rows, a block each, whose stretches lie one after the other.
+// The same of few rows, a block each, whose stretches lie one after the other.  Its launch overlaps the products' (1 row of 768, 50257 tokens: 19.6 us a call, 20.6 without).
 __global__ void __launch_bounds__(1024) hc_loss_join_row_kernel(const float2* sums, int64_t stretches, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse,
                                                                  float* losses) {
   __shared__ float tops[32], totals[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
   constexpr int kAtOnce = 4;
+  grid_dependency_wait();
   float most = -INFINITY, sum = 0.0f;
   const auto joined = [](float& most, float& sum, float m, float s) {
     const float top = fmaxf(most, m), ref = top == -INFINITY ? 0.0f : top;
@@ -272,10 +273,13 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     c.loss.ignore = ignore;
     const bool few = rows <= HC_LINEAR_FEW_ROWS;
     if ((few ? launch_few_rows_loss(c, stream) : launch_loss_sums(c, stream)) != cudaSuccess) return kErrCuda;
-    if (few)
-      dev::hc_loss_join_row_kernel<<<(unsigned)rows, 1024, 0, stream>>>(c.loss.sums, stretches, c.loss.picked, tokens, ignore, (int64_t)vocab, lse, losses);
-    else
-    dev::hc_loss_join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(c.loss.sums, stretches, (int64_t)rows, c.loss.picked, tokens, ignore, (int64_t)vocab, lse, losses);
+    const float2* sums = c.loss.sums;
+    const float* picked = c.loss.picked;
+    if (few) {
+      if (launch_overlapped(dev::hc_loss_join_row_kernel, (int)rows, 1024, 0, stream, sums, stretches, picked, tokens, ignore, (int64_t)vocab, lse, losses) != cudaSuccess) return kErrCuda;
+    } else {
+      dev::hc_loss_join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(sums, stretches, (int64_t)rows, picked, tokens, ignore, (int64_t)vocab, lse, losses);
+    }
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   }
   if (reduction == dev::kNone) return kOk;
