@@ -118,7 +118,7 @@ size_t hc_linear_cross_entropy_bytes(size_t rows, size_t inner, size_t vocab);
 int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const int64_t* tokens, int64_t ignore, int reduction, float* loss,
                             float* stats, size_t rows, size_t inner, size_t vocab, void* scratch, size_t scratch_bytes, hc_stream_t stream);
 // dx = G weight and dweight = G^T x (of `type`, each NULL where it is not wanted) with G = a (p - 1[token]); a: dloss (fp32) of the row, or dloss[0], over the count for a mean.
-// G is formed for a piece of the vocabulary at a time, in 16 bits (of fp16 times a power of two that the largest |a| gives), in scratch memory of at most 256 MiB or 1024 columns;
+// G is formed for a piece of the vocabulary at a time, in 16 bits (of fp16 times a power of two that the largest |a| gives), in scratch memory of at most 384 MiB or 1024 columns;
 // dx is summed in fp32, in up to four parts.  Where a result's stride is its width rounded up to eight, what lies behind its rows may be overwritten.
 size_t hc_linear_cross_entropy_backward_bytes(size_t rows, size_t inner, size_t vocab);
 int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const int64_t* tokens, int64_t ignore, int reduction,

@@ -18,7 +18,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     are infinite, gives NaN, in the gradients in its row of ``x`` and in all of ``weight``.
 
     The backward pass forms the logits again, a piece of the vocabulary at a time, and rounds their gradient to the operands' type for its products (float16 times a power of two
-    that brings the largest of the rows' gradients into range).  It takes at most 256 MiB for a piece, or 1024 columns of it, beside float32 sums of the gradient of ``x`` (up to four of its size).
+    that brings the largest of the rows' gradients into range).  It takes at most 384 MiB for a piece, or 1024 columns of it, beside float32 sums of the gradient of ``x`` (up to four of its size).
     Gradients have their tensors' types; all sums have a fixed order.
 
     Forward-mode derivatives, vmap and recorded (traced) calls raise NotImplementedError."""
