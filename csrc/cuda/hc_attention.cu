@@ -99,14 +99,14 @@ __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, AttnBa
 }
 __device__ __forceinline__ bool attn_wait_all(uint64_t* bar, uint32_t parity, AttnBarriers& sh) { return __all_sync(0xffffffffu, attn_wait(bar, parity, sh)); }
 
-// A place in a ring of N stages
+// A place in a ring of N stages, or of the first of them
 template <int N>
 struct Ring {
   int s = 0, count = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
+  __device__ __forceinline__ void next(int stages = N) {
     ++count;
-    if (++s == N) {
+    if (++s == stages) {
       s = 0;
       phase ^= 1;
     }
@@ -114,10 +114,10 @@ struct Ring {
 };
 // what a ring's last loads bring is there before the CTA leaves
 template <int N>
-__device__ __forceinline__ void ring_end(uint64_t* full, const Ring<N>& r) {
-  for (int back = 0; back < N && back < r.count; ++back) {
+__device__ __forceinline__ void ring_end(uint64_t* full, const Ring<N>& r, int stages = N) {
+  for (int back = 0; back < stages && back < r.count; ++back) {
     const int i = r.count - 1 - back;
-    mbar_wait_bounded(&full[i % N], (i / N) & 1, kAttnLimitNs);
+    mbar_wait_bounded(&full[i % stages], (i / stages) & 1, kAttnLimitNs);
   }
 }
 
@@ -404,6 +404,8 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
   if constexpr (S::kResident == 2) share_registers<96, S::kForwardThreads, 80>(warp < 4);
   constexpr int kRing = kStages / 2;  // of keys; behind it that of values
   unsigned char* v_ring = ring + kRing * S::kStepBytes;
+  // Groups that take the steps in turn need an even number of stages, so that a stage is always of the same group: one that does not wait for each of a barrier's phases cannot tell them apart.
+  const int stages = p.packed ? kRing / 2 * 2 : kRing;
   if (warp == 0) {
     if (lane == 0 && e0 < e1) {
       Ring<kRing> rk, rv;
@@ -412,14 +414,14 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
         if (!attn_wait(&sh.empty[rk.s], rk.phase ^ 1, sh)) break;
         mbar_expect_tx(&sh.full[rk.s], S::kStepBytes);
         load_rows<kD, kStep>(ring + rk.s * S::kStepBytes, &p.k, k0, kv_head, b, &sh.full[rk.s]);
-        rk.next();
+        rk.next(stages);
         if (!attn_wait(&sh.empty[8 + rv.s], rv.phase ^ 1, sh)) break;
         mbar_expect_tx(&sh.full[8 + rv.s], S::kStepBytes);
         load_rows<kD, kStep>(v_ring + rv.s * S::kStepBytes, &p.v, k0, kv_head, b, &sh.full[8 + rv.s]);
-        rv.next();
+        rv.next(stages);
       }
-      ring_end(sh.full, rk);
-      ring_end(sh.full + 8, rv);
+      ring_end(sh.full, rk, stages);
+      ring_end(sh.full + 8, rv, stages);
       mbar_wait_bounded(&sh.first, 0, kAttnLimitNs);
     }
   } else if (warp <= 2) {
@@ -433,8 +435,8 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
       Ring<kRing> rk, rv;
       const int start = p.packed ? e0 + ((e0 ^ q) & 1) : e0;  // its first step
       if (start != e0) {
-        rk.next();
-        rv.next();
+        rk.next(stages);
+        rv.next(stages);
       }
       const auto score = [&](int e) {
         if (!attn_wait_all(&sh.full[rk.s], rk.phase, sh)) return false;
@@ -446,8 +448,8 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
           attn_commit(leader, &sh.s_full[slot]);
         }
         attn_commit(leader, &sh.empty[rk.s]);
-        rk.next();
-        if (by == 2) rk.next();
+        rk.next(stages);
+        if (by == 2) rk.next(stages);
         return true;
       };
       const auto sum = [&](int e) {
@@ -460,8 +462,8 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
           attn_commit(leader, &sh.done[slot]);
         }
         attn_commit(leader, &sh.empty[8 + rv.s]);
-        rv.next();
-        if (by == 2) rv.next();
+        rv.next(stages);
+        if (by == 2) rv.next(stages);
         return true;
       };
       bool ok = attn_wait_all(&sh.first, 0, sh);

@@ -374,3 +374,19 @@ def test_model_with_this_attention(shape):
         scale = q.grad.norm() if not name.endswith("qkv.bias") else fused.blocks[0].qkv.weight.grad.double().norm()
         assert (p.grad.double() - q.grad).norm() <= room * scale, name
     assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,queries,d", [(16, 16, 1, 128), (16, 1, 1, 128), (16, 2, 2, 96), (12, 12, 1, 64), (24, 2, 1, 64)])
+def test_many_calls_give_the_same(heads, kv_heads, queries, d):
+    """Long runs of steps by all of the GPU, again and again: the same bits, and no wait that runs out."""
+    g = torch.Generator("cuda").manual_seed(7)
+    q = torch.randn(32, heads, queries, d, dtype=BF16, device="cuda", generator=g)
+    k, v = (torch.randn(32, kv_heads, 4099, d, dtype=BF16, device="cuda", generator=g) for _ in range(2))
+    first = ops.attention(q, k, v)
+    assert first.isfinite().all()
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(200):
+        differ += (ops.attention(q, k, v) != first).any()
+    assert differ.item() == 0
+    assert ops.train_status() == 0
