@@ -12,7 +12,7 @@
 //
 // Forward: two tiles of queries share their keys, so that the tensor cores work on one while the other's exponentials are taken, which bound it up to heads of
 // 64 (16 a cycle and SM).  The reference that exponentials are taken relative to follows a row's largest score when that is more than 2^8 above it; only then is O
-// taken times a factor.  Few queries (with all heads of a key's head at most 128 rows, a new token of each text for one) are one tile, and the keys are shared
+// taken times a factor.  Few queries (with all heads of a key's head at most 128 rows; up to 8 have a kernel of their own) are one tile, and the keys are shared
 // out to the CTAs of a cluster, which join their results over its shared memory: bound by reading keys and values.
 // Backward: dK and dV in a kernel whose CTA has a tile of keys and goes through the queries, dQ in one whose CTA has a tile of queries.  That forms the scores twice (8 products instead of 5, P K below among them), and
 // needs no atomic additions, whose order would change the result, and no array of partial dQ.
@@ -635,6 +635,215 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
   cluster_meet(p.splits);  // nobody leaves while its shared memory is read
 }
 
+// ---- forward, few rows -------------------------------------------------------------------------------------------------------
+// Up to eight rows (queries times heads of a key's head), a new token for one, where the kernel above mostly waits for its own beginning.  No tensor memory and no mbarriers: a warp loads 16 keys and
+// values at a time from global memory as mma.sync's first operand wants them (S^T = K Q^T, O^T = V^T P^T, so that the rows are its eight columns and no operand is empty), and keeps a maximum, a sum
+// and O of its own keys, which CTA and cluster join.  Bound by reading keys and values, and by latency where they are few.  bf16, times in a graph: 12 heads of 64, 1024 keys 3.9 us (9.1 with
+// the kernel above); 32 heads on 8 of 128, 1024 keys 6.1 us (10.3); 8 x 16 heads on 4 of 128, 4096 keys 16.4 us (21.5); 64 x 12 heads of 64, 1024 keys 38 us, 5.3 TB/s (56); 16 x 16 heads on 4 of 128, 8196
+// keys 53 us (52).  32 keys at a time, with heads up to 64: 5.3 us instead of 4.2; the next keys' loads before the work on these: spills, 73 us instead of 51 at 32 x 16 on 8, 2048 keys of 128.
+struct FewRows {
+  const void *q, *k, *v;
+  int64_t q_batch, q_head, q_position, k_batch, k_head, k_position, v_batch, v_head, v_position;
+  void* o;
+  float* less;
+  int64_t less_ld;
+  int heads, kv_heads, group, tq, d, off, window, sinks, splits, split_bits;  // splits: 2^split_bits
+  unsigned heads_of;  // 2^16 / tq, rounded up
+  float scale2;
+};
+constexpr int kFewWarps = 8, kFewRows = 8, kFewKeys = 16;  // keys of a warp at once
+// eight rows of eight 16-bit values, a row's neighbours 2t and 2t + 1 in lane 4 row + t, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename T, int kD, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 16 ? 1 : kD == 64 ? 3 : 2) hc_attention_few_kernel(const __grid_constant__ FewRows p) {
+  constexpr int kQ = kD / 32, kV = kD / 64;
+  constexpr float kBias = operand_format<T>() ? 0.0f : 14.0f;  // probabilities, and with them sums and O, are held times 2^14 in fp16
+  __shared__ __align__(16) float values[kFewWarps][kFewRows][kD];
+  __shared__ __align__(16) float joined[kFewRows][kD];
+  __shared__ float2 sums[kFewWarps][kFewRows], joined_sums[kFewRows];  // maximum, sum of exponentials
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, rows = p.group * p.tq;
+  const unsigned at = blockIdx.x >> p.split_bits;
+  const int rank = blockIdx.x & (p.splits - 1), b = at / (unsigned)p.kv_heads, head = at - b * p.kv_heads;
+  const auto head_of = [&](int row) { return (int)((unsigned)row * p.heads_of >> 16); };  // row / tq
+  // the keys that some row sees, counted without the gap between the first tokens and the window
+  const int last = p.off + p.tq - 1, from = max(p.off - p.window + 1, 0), sinks = min(p.sinks, from), count = last < 0 ? 0 : sinks + last - from + 1;
+  const T *k = static_cast<const T*>(p.k) + b * p.k_batch + head * p.k_head, *v = static_cast<const T*>(p.v) + b * p.v_batch + head * p.v_head;
+  const auto key_of = [&](int n) { return n < sinks ? n : n - sinks + from; };
+  // eight values of key number n, from 8 c on
+  const auto load = [&](const T* at, int64_t position, int n, int c) { return n < count && c * 8 < p.d ? *reinterpret_cast<const uint4*>(at + key_of(n) * position + c * 8) : make_uint4(0, 0, 0, 0); };
+  uint4 q[kQ];  // of row g
+#pragma unroll
+  for (int i = 0; i < kQ; ++i) {
+    const int c = t + 4 * i;
+    q[i] = make_uint4(0, 0, 0, 0);
+    if (g < rows && c * 8 < p.d) q[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_batch + (head * p.group + head_of(g)) * p.q_head + (g - head_of(g) * p.tq) * p.q_position + c * 8);
+  }
+  float o[kV][4][4];  // of rows 2t (0, 2) and 2t + 1 (1, 3), values 8 (g + 8 i) + 2 u (0, 1) and the next
+#pragma unroll
+  for (int i = 0; i < kV; ++i)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][u][j] = 0.0f;
+  float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  int position[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) position[r] = p.off + 2 * t + r - head_of(2 * t + r) * p.tq;
+  for (int first = (rank * kWarps + warp) * kFewKeys; first < count; first += p.splits * kWarps * kFewKeys) {
+    uint4 x[2][kQ], y[4][kV];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) x[h][i] = load(k, p.k_position, first + h * 8 + g, t + 4 * i);
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int i = 0; i < kV; ++i) y[h][i] = load(v, p.v_position, first + (h >> 1) * 8 + 2 * t + (h & 1), g + 8 * i);
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of keys g (0, 1) and g + 8, rows 2t (0, 2) and 2t + 1
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+      mma_16x8x16<T>(s, x[0][i].x, x[1][i].x, x[0][i].y, x[1][i].y, q[i].x, q[i].y);
+      mma_16x8x16<T>(s, x[0][i].z, x[1][i].z, x[0][i].w, x[1][i].w, q[i].z, q[i].w);
+    }
+    float top[2] = {most[0], most[1]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = first + (j >> 1) * 8 + g, key = key_of(n), at = position[j & 1];
+      const bool seen = n < count && key <= at && (at - key < p.window || key < p.sinks);
+      s[j] = seen ? s[j] * p.scale2 : -INFINITY;
+      top[j & 1] = fmaxf(top[j & 1], s[j]);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int n = 4; n < 32; n <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], n));
+      const float ref = top[r] == -INFINITY ? 0.0f : top[r], before = power2(most[r] - ref);
+      most[r] = top[r];
+      s[r] = power2(s[r] - ref + kBias);
+      s[2 + r] = power2(s[2 + r] - ref + kBias);
+      sum[r] = sum[r] * before + (s[r] + s[2 + r]);
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          o[i][u][r] *= before;
+          o[i][u][2 + r] *= before;
+        }
+    }
+    const uint32_t b0 = transposed(pack2<T>(s[0], s[1])), b1 = transposed(pack2<T>(s[2], s[3]));
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      const auto word = [&](int h, int u) { return u == 0 ? y[h][i].x : u == 1 ? y[h][i].y : u == 2 ? y[h][i].z : y[h][i].w; };
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        mma_16x8x16<T>(o[i][u], __byte_perm(word(0, u), word(1, u), 0x5410), __byte_perm(word(0, u), word(1, u), 0x7632), __byte_perm(word(2, u), word(3, u), 0x5410),
+                       __byte_perm(word(2, u), word(3, u), 0x7632), b0, b1);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int n = 4; n < 32; n <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], n);
+  const auto put = [&](int at) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = 2 * t + r;
+      if (row >= rows) continue;
+      if (g == 0) sums[at][row] = make_float2(most[r], sum[r]);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        float* to = &values[at][row][8 * (g + 8 * i)];
+        *reinterpret_cast<float4*>(to) = make_float4(o[i][0][r], o[i][0][2 + r], o[i][1][r], o[i][1][2 + r]);
+        *reinterpret_cast<float4*>(to + 4) = make_float4(o[i][2][r], o[i][2][2 + r], o[i][3][r], o[i][3][2 + r]);
+      }
+    }
+  };
+  if (kWarps > kFewWarps) {  // the second eight warps' go to the first
+    if (warp >= kFewWarps) put(warp - kFewWarps);
+    __syncthreads();
+    if (warp < kFewWarps) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = 2 * t + r;
+        if (row >= rows) continue;
+        const float2 other = sums[warp][row];
+        const float top = fmaxf(most[r], other.x), ref = top == -INFINITY ? 0.0f : top, a = power2(most[r] - ref), c = power2(other.x - ref);
+        most[r] = top;
+        sum[r] = sum[r] * a + other.y * c;
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float2 w = *reinterpret_cast<const float2*>(&values[warp][row][8 * (g + 8 * i) + 2 * u]);
+            o[i][u][r] = o[i][u][r] * a + w.x * c;
+            o[i][u][2 + r] = o[i][u][2 + r] * a + w.y * c;
+          }
+      }
+      __syncwarp();  // all of it is read
+    }
+  }
+  if (warp < kFewWarps) put(warp);
+  __syncthreads();
+  // of `all` parts: a row's four values, maximum and sum
+  const auto join = [](int all, auto sum_at, auto value_at, float2& total, float4& x) {
+    float2 s[kFewWarps];
+    float4 y[kFewWarps];
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < kFewWarps; ++n) {
+      s[n] = n < all ? sum_at(n) : make_float2(-INFINITY, 0.0f);
+      y[n] = n < all ? value_at(n) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      top = fmaxf(top, s[n].x);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    total = make_float2(top, 0.0f);
+    x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int n = 0; n < kFewWarps; ++n) {
+      const float weight = power2(s[n].x - ref);
+      total.y += weight * s[n].y;
+      x.x += weight * y[n].x, x.y += weight * y[n].y, x.z += weight * y[n].z, x.w += weight * y[n].w;
+    }
+  };
+  const auto store = [&](int r, int col, float2 total, float4 x) {
+    const bool none = total.y == 0.0f;  // (a NaN is not)
+    const float factor = none ? 0.0f : 1.0f / total.y;
+    const int i = r - head_of(r) * p.tq, h = head * p.group + head_of(r);
+    if (col < p.d)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (((int64_t)b * p.tq + i) * p.heads + h) * p.d + col) = make_uint2(pack2<T>(x.x * factor, x.y * factor), pack2<T>(x.z * factor, x.w * factor));
+    if (col == 0 && p.less) p.less[((int64_t)b * p.heads + h) * p.less_ld + i] = none ? -INFINITY : kBias - (total.x + log2f(total.y));
+  };
+  static_assert(kFewRows * (kD / 4) <= 32 * kFewWarps && kMostSplits <= kFewWarps, "a thread's part");
+  const int row = threadIdx.x / (kD / 4), col = threadIdx.x % (kD / 4) * 4;
+  float2 total;
+  float4 x;
+  if (row < rows) {
+    join(kFewWarps, [&](int n) { return sums[n][row]; }, [&](int n) { return *reinterpret_cast<const float4*>(&values[n][row][col]); }, total, x);
+    if (p.splits == 1) store(row, col, total, x);
+  }
+  if (p.splits == 1) return;
+  if (row < rows) {
+    *reinterpret_cast<float4*>(&joined[row][col]) = x;
+    if (col == 0) joined_sums[row] = total;
+  }
+  cluster_meet(p.splits);
+  if (row < rows && threadIdx.x % p.splits == rank) {
+    join(
+        p.splits,
+        [&](int n) {
+          const uint32_t at = peer_address(&joined_sums[row], n);
+          return make_float2(peer_load(at), peer_load(at + 4));
+        },
+        [&](int n) { return peer_load4(peer_address(&joined[row][col], n)); }, total, x);
+    store(row, col, total, x);
+  }
+  cluster_meet(p.splits);  // nobody leaves while its shared memory is read
+}
+
 // ---- backward ----------------------------------------------------------------------------------------------------------------
 // fp16: the largest square of a norm of dO's rows (the first `blocks[0] * heads[0] * batch` blocks) and of V's.  Eight values a thread, four rows of a thread on their way together; a block has
 // 4 * 256 / kLanes rows of a head.
@@ -1096,11 +1305,11 @@ int kv_splits(const Sizes& s) {
 }
 
 // early: beside the kernel before it, whose results the kernel waits for where it needs them (griddepcontrol.wait).  8 x 12 heads of 64, 1024 positions, bf16, all three kernels: 151 us, 155 without.
-template <typename K>
-cudaError_t launch_clusters(K kernel, int64_t ctas, int size, int threads, int smem, cudaStream_t stream, const dev::AttnParams& p, bool early = false) {
+template <typename K, typename P>
+cudaError_t launch_clusters(K kernel, dim3 ctas, int size, int threads, int smem, cudaStream_t stream, const P& p, bool early = false) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.gridDim = ctas;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
@@ -1141,7 +1350,28 @@ cudaError_t run_forward(const dev::AttnParams& p, cudaStream_t stream) {
   const cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t ctas = (int64_t)p.batch * (p.packed ? p.kv_heads : p.heads) * p.blocks * p.splits;
-  return launch_clusters(dev::hc_attention_kernel<T, kD>, ctas, p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, p);
+  return launch_clusters(dev::hc_attention_kernel<T, kD>, dim3((unsigned)ctas), p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, p);
+}
+
+// How the keys of few rows are shared out: CTAs of a cluster, as long as there are fewer than two an SM (4: 59 us instead of 51 at 32 x 16 heads on 8, 2048 keys of 128); sixteen warps a CTA instead of
+// eight where the largest clusters are too few and have more keys than they load at once (12 heads of 64, 32768 keys: 25 us instead of 43; 8 x 16 on 4 of 128, 4096 keys, has enough: 32 instead of 16).
+// No CTAs: they are not that few.
+struct FewPlan {
+  int splits, warps;
+};
+FewPlan few_plan(const Sizes& s, size_t window, size_t sinks) {
+  if (s.heads / s.kv_heads * s.queries > dev::kFewRows) return {0, 0};
+  const size_t reach = window && window + sinks + s.queries < s.keys ? window + sinks + s.queries : s.keys;
+  const int64_t ctas = (int64_t)(s.batch * s.kv_heads), at_once = dev::kFewWarps * dev::kFewKeys;
+  FewPlan p = {1, dev::kFewWarps};
+  while (p.splits < dev::kMostSplits && p.splits * at_once < (int64_t)reach && ctas * p.splits < 2 * attn_sms()) p.splits *= 2;
+  if (p.splits * at_once < (int64_t)reach && ctas * p.splits <= attn_sms()) p.warps *= 2;
+  return p;
+}
+template <typename T, int kD>
+cudaError_t run_few(const dev::FewRows& p, int warps, int batch, cudaStream_t stream) {
+  const auto kernel = warps > dev::kFewWarps ? dev::hc_attention_few_kernel<T, kD, 2 * dev::kFewWarps> : dev::hc_attention_few_kernel<T, kD, dev::kFewWarps>;
+  return launch_clusters(kernel, dim3((unsigned)(batch * p.kv_heads * p.splits)), p.splits, 32 * warps, 0, stream, p);
 }
 
 template <typename T, int kD>
@@ -1169,11 +1399,11 @@ cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_head
   const int splits = p.splits;
   p.splits = 1;
   p.blocks = (p.tq + dev::kTile - 1) / dev::kTile;
-  e = launch_clusters(dev::hc_attention_backward_kernel<T, kD, false>, (int64_t)p.batch * p.heads * p.blocks, 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, most != nullptr);
+  e = launch_clusters(dev::hc_attention_backward_kernel<T, kD, false>, dim3((unsigned)((int64_t)p.batch * p.heads * p.blocks)), 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, most != nullptr);
   if (e != cudaSuccess || !p.dk) return e;
   p.splits = splits;
   p.blocks = (p.tk + dev::kTile - 1) / dev::kTile;
-  return launch_clusters(dev::hc_attention_backward_kernel<T, kD, true>, (int64_t)p.batch * p.kv_heads * p.blocks * splits, splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, true);
+  return launch_clusters(dev::hc_attention_backward_kernel<T, kD, true>, dim3((unsigned)((int64_t)p.batch * p.kv_heads * p.blocks * splits)), splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, true);
 }
 
 size_t backward_bytes(const Sizes& s) { return up(s.batch * s.heads * stats_ld(s.queries) * sizeof(float), 256) + 256; }
@@ -1200,6 +1430,16 @@ int hc_attention(hc_heads q, hc_heads k, hc_heads v, int type, void* out, float*
     return cudaMemsetAsync(out, 0, batch * queries * heads * head_size * 2, stream) == cudaSuccess ? kOk : kErrCuda;
   }
   if (!heads_ok(q, head_size, queries, heads, batch) || !heads_ok(k, head_size, keys, kv_heads, batch) || !heads_ok(v, head_size, keys, kv_heads, batch)) return kErrArgument;
+  if (const FewPlan few = few_plan(s, window, sinks); few.splits) {
+    dev::AttnParams all;
+    fill_attention(&all, s, window, sinks, scale);
+    const int bits = few.splits == 1 ? 0 : few.splits == 2 ? 1 : few.splits == 4 ? 2 : 3;
+    const dev::FewRows p = {q.data, k.data, v.data, (int64_t)q.batch, (int64_t)q.head, (int64_t)q.position, (int64_t)k.batch, (int64_t)k.head, (int64_t)k.position, (int64_t)v.batch,
+                            (int64_t)v.head, (int64_t)v.position, out, stats, all.less_ld, all.heads, all.kv_heads, all.group, all.tq, all.d, all.off, all.window, all.sinks, few.splits, bits,
+                            (unsigned)((65536 + queries - 1) / queries), all.scale2};
+    const auto run = type == kBf16 ? head_size <= 64 ? run_few<__nv_bfloat16, 64> : run_few<__nv_bfloat16, 128> : head_size <= 64 ? run_few<__half, 64> : run_few<__half, 128>;
+    return run(p, few.warps, all.batch, stream) == cudaSuccess ? kOk : kErrCuda;
+  }
   const Plan plan = plan_of(s, window, sinks);
   dev::AttnParams p;
   fill_attention(&p, s, window, sinks, scale);

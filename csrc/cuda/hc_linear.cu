@@ -55,21 +55,6 @@ __device__ __forceinline__ uint4 few_group(const T* row, int64_t k, int64_t end,
   if (!kVector) return any_group(reinterpret_cast<const uint16_t*>(row + k + 8 * t), end - k - 8 * t);
   return k + 8 * t < end ? *reinterpret_cast<const uint4*>(row + k + 8 * t) : make_uint4(0, 0, 0, 0);
 }
-template <typename T>
-__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void few_mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void few_mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 constexpr int kFewWarps = 16;  // at most, of a block
 template <typename T, int N, bool kVector>  // N: eights of rows
 __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __grid_constant__ FewRowsParams p) {
@@ -109,8 +94,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        few_mma<T>(part[n], a[s].x, b[s].x, a[s].y, b[s].y, v[s][n].x, v[s][n].y);
-        few_mma<T>(part[n], a[s].z, b[s].z, a[s].w, b[s].w, v[s][n].z, v[s][n].w);
+        mma_16x8x16<T>(part[n], a[s].x, b[s].x, a[s].y, b[s].y, v[s][n].x, v[s][n].y);
+        mma_16x8x16<T>(part[n], a[s].z, b[s].z, a[s].w, b[s].w, v[s][n].z, v[s][n].w);
       }
     if (++taken == 32 / kSteps || k0 + stride >= p.inner) {
       taken = 0;
@@ -197,8 +182,8 @@ __global__ void __launch_bounds__(256, N == 1 ? 3 : 2) hc_few_rows_loss_kernel(c
         for (int n = 0; n < N; ++n) v[n] = few_group<T, true>(x[n], k0 + s * 32, end[n], t);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          few_mma<T>(part[n], a[s].x, b[s].x, a[s].y, b[s].y, v[n].x, v[n].y);
-          few_mma<T>(part[n], a[s].z, b[s].z, a[s].w, b[s].w, v[n].z, v[n].w);
+          mma_16x8x16<T>(part[n], a[s].x, b[s].x, a[s].y, b[s].y, v[n].x, v[n].y);
+          mma_16x8x16<T>(part[n], a[s].z, b[s].z, a[s].w, b[s].w, v[n].z, v[n].w);
         }
         // the same place of the next stretch is on its way while the others are worked on
         a[s] = few_group<T, true>(w0, k0 + (kSteps + s) * 32, p.inner, t);

@@ -390,3 +390,27 @@ def test_many_calls_give_the_same(heads, kv_heads, queries, d):
         differ += (ops.attention(q, k, v) != first).any()
     assert differ.item() == 0
     assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("d", [8, 64, 72, 128])
+@pytest.mark.parametrize("heads,kv_heads,queries", [(1, 1, 1), (8, 1, 1), (3, 1, 2), (4, 2, 3), (2, 2, 7), (4, 4, 8), (14, 2, 1)])
+def test_up_to_eight_rows(heads, kv_heads, queries, d, kind):
+    """Lengths around what a warp, a CTA and a cluster load at once; queries in front of the first key; windows whose gap begins anywhere."""
+    for n, (keys, window, sinks) in enumerate([(1, None, 0), (3, 2, 1), (16, None, 0), (17, 5, 2), (127, 1, 0), (129, None, 0), (300, 130, 17), (1025, 1000, 3), (1040, 40, 40), (5003, None, 0), (5003, 300, 20)]):
+        q, k, v, dout = make(2, heads, kv_heads, queries, keys, d, kind, n)
+        check(q, k, v, dout, window, sinks, grads=n % 3 == 0)
+
+
+@pytest.mark.gpu
+def test_few_rows_of_many_texts():
+    """More texts and heads than the second dimension of a grid holds."""
+    g = torch.Generator("cuda").manual_seed(3)
+    q, k, v = (torch.randn(70000, 2, n, 8, dtype=BF16, device="cuda", generator=g) for n in (1, 3, 3))
+    p = torch.softmax(q.double() @ k.double().transpose(2, 3) / math.sqrt(8), 3)
+    want = p @ v.double()
+    h = torch.finfo(BF16).eps / 2
+    # a score's sum of 8 in 32 bits moves a probability by less than 2^-18 of itself; it is rounded for the product, and the result once
+    room = (h + 2.0 ** -17) * (p @ v.double().abs()) + h * want.abs() * (1 + 2 * h) + 1e-30
+    assert ((ops.attention(q, k, v).double() - want).abs() <= room).all()
