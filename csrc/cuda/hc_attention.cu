@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
 // values at a time from global memory as mma.sync's first operand wants them (S^T = K Q^T, O^T = V^T P^T, so that the rows are its eight columns and no operand is empty), and keeps a maximum, a sum
 // and O of its own keys, which CTA and cluster join.  Bound by reading keys and values, and by latency where they are few.  bf16, times in a graph: 12 heads of 64, 1024 keys 3.9 us (9.1 with
 // the kernel above); 32 heads on 8 of 128, 1024 keys 6.1 us (10.3); 8 x 16 heads on 4 of 128, 4096 keys 16.4 us (21.5); 64 x 12 heads of 64, 1024 keys 38 us, 5.3 TB/s (56); 16 x 16 heads on 4 of 128, 8196
-// keys 53 us (52).  32 keys at a time, with heads up to 64: 5.3 us instead of 4.2; the next keys' loads before the work on these: spills, 73 us instead of 51 at 32 x 16 on 8, 2048 keys of 128.
+// keys 49 us (52).  32 keys at a time, with heads up to 64: 5.3 us instead of 4.2; the next keys' loads before the work on these: spills, 73 us instead of 51 at 32 x 16 heads on 8, 2048 keys of 128.
 struct FewRows {
   const void *q, *k, *v;
   int64_t q_batch, q_head, q_position, k_batch, k_head, k_position, v_batch, v_head, v_position;
@@ -1353,19 +1353,28 @@ cudaError_t run_forward(const dev::AttnParams& p, cudaStream_t stream) {
   return launch_clusters(dev::hc_attention_kernel<T, kD>, dim3((unsigned)ctas), p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, p);
 }
 
-// How the keys of few rows are shared out: CTAs of a cluster, as long as there are fewer than two an SM (4: 59 us instead of 51 at 32 x 16 heads on 8, 2048 keys of 128); sixteen warps a CTA instead of
-// eight where the largest clusters are too few and have more keys than they load at once (12 heads of 64, 32768 keys: 25 us instead of 43; 8 x 16 on 4 of 128, 4096 keys, has enough: 32 instead of 16).
-// No CTAs: they are not that few.
+// How the keys of few rows are shared out: CTAs of a cluster, and where the largest clusters have more keys than they load at once perhaps sixteen warps a CTA instead of eight, so that their rounds of
+// CTAs and, in each, of loads and two more for beginning and joining are fewest.  16 x 16 heads on 4, 8196 keys of 128: 4 CTAs in one round 49 us, 8 in two 53; 12 heads of 64, 32768 keys:
+// sixteen warps 25 us, eight 43.  Clusters of sixteen CTAs take 45 us instead of 79 for a single key's head with 65536 keys, but 21 instead of 16 for eight with 8192, as they do not all find room at once.
+// No CTAs: the rows are not that few.
 struct FewPlan {
   int splits, warps;
 };
 FewPlan few_plan(const Sizes& s, size_t window, size_t sinks) {
   if (s.heads / s.kv_heads * s.queries > dev::kFewRows) return {0, 0};
   const size_t reach = window && window + sinks + s.queries < s.keys ? window + sinks + s.queries : s.keys;
-  const int64_t ctas = (int64_t)(s.batch * s.kv_heads), at_once = dev::kFewWarps * dev::kFewKeys;
+  const int64_t ctas = (int64_t)(s.batch * s.kv_heads);
   FewPlan p = {1, dev::kFewWarps};
-  while (p.splits < dev::kMostSplits && p.splits * at_once < (int64_t)reach && ctas * p.splits < 2 * attn_sms()) p.splits *= 2;
-  if (p.splits * at_once < (int64_t)reach && ctas * p.splits <= attn_sms()) p.warps *= 2;
+  int64_t least = 0;
+  for (int n = 1; n <= dev::kMostSplits; n *= 2)
+    for (int w = dev::kFewWarps; w <= (n >= dev::kMostSplits ? 2 : 1) * dev::kFewWarps; w *= 2) {
+      const int64_t at_once = (int64_t)n * w * dev::kFewKeys, places = attn_sms() * (w > dev::kFewWarps ? 1 : s.d > 64 ? 2 : 3);
+      const int64_t cost = (ctas * n + places - 1) / places * (((int64_t)reach + at_once - 1) / at_once + 2);
+      if (least == 0 || cost < least) {
+        least = cost;
+        p = {n, w};
+      }
+    }
   return p;
 }
 template <typename T, int kD>
