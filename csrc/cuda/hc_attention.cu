@@ -74,7 +74,7 @@ struct AttnParams {
 };
 
 struct AttnBarriers {
-  uint64_t full[16], empty[16], first, drained, met;
+  uint64_t full[16], empty[16], first, drained, met, dots;
   uint64_t s_full[4], p_ready[4], done[4], dp_full[2], ds_ready[2], ds_done[2];
   uint32_t tmem, gave_up;
 };
@@ -278,6 +278,7 @@ __device__ __forceinline__ void attn_begin(AttnBarriers& sh, int warps, int rows
     mbar_init(&sh.first, 1);
     mbar_init(&sh.drained, 2);
     mbar_init(&sh.met, warps);
+    mbar_init(&sh.dots, warps);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_ready[i], rows);
@@ -1027,7 +1028,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     constexpr float kBias = kF16 && kKeys ? 14.0f : 0.0f;  // P^T is held times 2^14 in fp16 (what P K is for needs no more than a few bits)
     if (!kKeys) {
       if (kF16) grid_dependency_wait();  // behind the largest norms
-      launch_dependents();
+      if (p.dk) launch_dependents();  // the keys' pass; without it, what comes next waits for the end
     }
     const float power = kF16 ? ds_power(p.most, 1) : 1.0f, back = kF16 ? ds_power(p.most, -1) : 1.0f;
     const Pair gain = pair(power * (kBias ? 1.0f / 16384.0f : 1.0f), power * (kBias ? 1.0f / 16384.0f : 1.0f));
@@ -1040,7 +1041,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
       // delta = dO . O, dO's row from the tile
       const int c = part * 32;
       if (in) less = pair(less1, less1);
-      attn_wait_all(&sh.first, 0, sh);  // when it runs out, so do the waits below
+      attn_wait_all(&sh.first, 0, sh);  // when this or the wait for the other parts runs out, so do those below
       const unsigned char* at = tile2 + c / 64 * (kTile * 128) + row * 128;
       float dot = 0.0f;
 #pragma unroll
@@ -1056,7 +1057,9 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
         }
       }
       dots[part][row] = dot;
-      asm volatile("bar.sync 1, %0;" ::"n"(256 * kGroups) : "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.dots);
+      attn_wait_all(&sh.dots, 0, sh);
 #pragma unroll
       for (int k = 0; k < kParts; ++k) delta += dots[k][row];
       delta2 = pair(delta, delta);
@@ -1304,32 +1307,6 @@ int kv_splits(const Sizes& s) {
   return group % 2 == 0 && tiles < slots * 8 ? 2 : 1;
 }
 
-// early: beside the kernel before it, whose results the kernel waits for where it needs them (griddepcontrol.wait).  8 x 12 heads of 64, 1024 positions, bf16, all three kernels: 151 us, 155 without.
-template <typename K, typename P>
-cudaError_t launch_clusters(K kernel, dim3 ctas, int size, int threads, int smem, cudaStream_t stream, const P& p, bool early = false) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = ctas;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attrs[2];
-  memset(attrs, 0, sizeof(attrs));
-  cfg.attrs = attrs;
-  if (size > 1) {
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim.x = (unsigned)size;
-    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  }
-  if (early) {
-    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 size_t stats_ld(size_t queries) { return up(queries, 128); }
 
 void fill_attention(dev::AttnParams* p, const Sizes& s, size_t window, size_t sinks, float scale) {
@@ -1350,7 +1327,7 @@ cudaError_t run_forward(const dev::AttnParams& p, cudaStream_t stream) {
   const cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t ctas = (int64_t)p.batch * (p.packed ? p.kv_heads : p.heads) * p.blocks * p.splits;
-  return launch_clusters(dev::hc_attention_kernel<T, kD>, dim3((unsigned)ctas), p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, p);
+  return launch_with(dev::hc_attention_kernel<T, kD>, ctas, p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, false, p);
 }
 
 // How the keys of few rows are shared out: CTAs of a cluster, and where the largest clusters have more keys than they load at once perhaps sixteen warps a CTA instead of eight, so that their rounds of
@@ -1380,7 +1357,7 @@ FewPlan few_plan(const Sizes& s, size_t window, size_t sinks) {
 template <typename T, int kD>
 cudaError_t run_few(const dev::FewRows& p, int warps, int batch, cudaStream_t stream) {
   const auto kernel = warps > dev::kFewWarps ? dev::hc_attention_few_kernel<T, kD, 2 * dev::kFewWarps> : dev::hc_attention_few_kernel<T, kD, dev::kFewWarps>;
-  return launch_clusters(kernel, dim3((unsigned)(batch * p.kv_heads * p.splits)), p.splits, 32 * warps, 0, stream, p);
+  return launch_with(kernel, batch * p.kv_heads * p.splits, p.splits, 32 * warps, 0, stream, false, p);
 }
 
 template <typename T, int kD>
@@ -1408,11 +1385,12 @@ cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_head
   const int splits = p.splits;
   p.splits = 1;
   p.blocks = (p.tq + dev::kTile - 1) / dev::kTile;
-  e = launch_clusters(dev::hc_attention_backward_kernel<T, kD, false>, dim3((unsigned)((int64_t)p.batch * p.heads * p.blocks)), 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, most != nullptr);
+  e = launch_with(dev::hc_attention_backward_kernel<T, kD, false>, (int64_t)p.batch * p.heads * p.blocks, 1, dev::AttnShape<kD>::kBackwardThreads, smem, stream, most != nullptr, p);
   if (e != cudaSuccess || !p.dk) return e;
   p.splits = splits;
   p.blocks = (p.tk + dev::kTile - 1) / dev::kTile;
-  return launch_clusters(dev::hc_attention_backward_kernel<T, kD, true>, dim3((unsigned)((int64_t)p.batch * p.kv_heads * p.blocks * splits)), splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, p, true);
+  // beside the queries' pass: 8 x 12 heads of 64, 1024 positions, bf16, all three kernels 151 us, 155 without
+  return launch_with(dev::hc_attention_backward_kernel<T, kD, true>, (int64_t)p.batch * p.kv_heads * p.blocks * splits, splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, true, p);
 }
 
 size_t backward_bytes(const Sizes& s) { return up(s.batch * s.heads * stats_ld(s.queries) * sizeof(float), 256) + 256; }

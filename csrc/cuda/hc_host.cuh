@@ -67,6 +67,33 @@ inline DeviceInfo& device_info() {
   return d;
 }
 
+// A launch of clusters of `size` CTAs.  beside: the kernel may begin while the one before it in the stream runs, once all of that one's CTAs have allowed it or ended (griddepcontrol.launch_dependents),
+// and waits for the end of that one where it needs its results (griddepcontrol.wait); some thread of each CTA does, so that it does not end first.
+template <typename... Params, typename... Args>
+cudaError_t launch_with(void (*kernel)(Params...), int64_t ctas, int size, int threads, int smem, cudaStream_t stream, bool beside, const Args&... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  memset(attrs, 0, sizeof(attrs));
+  cfg.attrs = attrs;
+  if (size > 1) {
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = (unsigned)size;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (beside) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <typename K>
 cudaError_t set_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);

@@ -276,7 +276,7 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     const float2* sums = c.loss.sums;
     const float* picked = c.loss.picked;
     if (few) {
-      if (launch_overlapped(dev::hc_loss_join_row_kernel, (int)rows, 1024, 0, stream, sums, stretches, picked, tokens, ignore, (int64_t)vocab, lse, losses) != cudaSuccess) return kErrCuda;
+      if (launch_with(dev::hc_loss_join_row_kernel, (int64_t)rows, 1, 1024, 0, stream, true, sums, stretches, picked, tokens, ignore, (int64_t)vocab, lse, losses) != cudaSuccess) return kErrCuda;
     } else {
       dev::hc_loss_join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(sums, stretches, (int64_t)rows, picked, tokens, ignore, (int64_t)vocab, lse, losses);
     }

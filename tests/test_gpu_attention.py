@@ -247,9 +247,10 @@ def test_against_differences():
 
 
 @pytest.mark.gpu
-def test_captured_and_on_two_streams():
+@pytest.mark.parametrize("kind", [BF16, F16])
+def test_captured_and_on_two_streams(kind):
     """Two graphs replayed at once on other values, each with scratch memory of its own; single tokens and sequences."""
-    sets = [(make(2, 4, 2, 1, 5000, 64, BF16, 10 + i), make(1, 4, 4, 300, 300, 64, BF16, 20 + i)) for i in range(2)]
+    sets = [(make(2, 4, 2, 1, 5000, 64, kind, 10 + i), make(1, 4, 4, 300, 300, 64, kind, 20 + i)) for i in range(2)]
     graphs, outs, held = [], [], []
 
     def call(token, whole):
@@ -414,3 +415,25 @@ def test_few_rows_of_many_texts():
     # a score's sum of 8 in 32 bits moves a probability by less than 2^-18 of itself; it is rounded for the product, and the result once
     room = (h + 2.0 ** -17) * (p @ v.double().abs()) + h * want.abs() * (1 + 2 * h) + 1e-30
     assert ((ops.attention(q, k, v).double() - want).abs() <= room).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,length,d", [(12, 12, 500, 64), (8, 4, 700, 128), (2, 2, 100, 64)])
+def test_many_backward_passes_give_the_same(heads, kv_heads, length, d, kind):
+    """Kernels that begin beside the one before them: the same bits again and again, with other values in the memory that they take and other work before and behind them."""
+    q, k, v, dout = make(4, heads, kv_heads, length, length, d, kind, 9)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    first = [t.clone() for t in torch.autograd.grad(ops.attention(*leaves), leaves, dout)]
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(100):
+        scratch = [torch.full((1 << n,), math.nan, device="cuda") for n in (14, 16, 18, 20)]
+        del scratch
+        if i % 3 == 2:
+            (dq,) = torch.autograd.grad(ops.attention(*leaves), leaves[:1], dout)
+            differ += (dq != first[0]).any()
+            continue
+        for a, b in zip(torch.autograd.grad(ops.attention(*leaves), leaves, dout), first):
+            differ += (a != b).any()
+    assert differ.item() == 0
+    assert ops.train_status() == 0
