@@ -437,3 +437,20 @@ def test_many_backward_passes_give_the_same(heads, kv_heads, length, d, kind):
             differ += (a != b).any()
     assert differ.item() == 0
     assert ops.train_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [2, 12])
+def test_offsets_beyond_32_bits(heads):
+    """The end of a cache of 2^24 - 64 positions of two texts, 2^32 values and more, against its last positions alone: the same bits."""
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs 20 GB")
+    n, m = (1 << 24) - 64, 1024
+    k, v = (torch.zeros(2, 1, n, 128, dtype=BF16, device="cuda") for _ in range(2))
+    g = torch.Generator("cuda").manual_seed(1)
+    q = torch.randn(2, heads, 1, 128, dtype=BF16, device="cuda", generator=g)
+    for t in (k, v):
+        t[:, :, -m:] = torch.randn(2, 1, m, 128, dtype=BF16, device="cuda", generator=g)
+    want = ops.attention(q, k[:, :, -m:].contiguous(), v[:, :, -m:].contiguous(), window=700)
+    assert torch.equal(ops.attention(q, k, v, window=700), want)
+    assert want.norm() > 0
