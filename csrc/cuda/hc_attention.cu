@@ -210,8 +210,9 @@ __device__ __forceinline__ void share_registers(bool role) {
 }
 
 // ---- clusters -----------------------------------------------------------------------------------------------------------------
-// All threads of all CTAs of a cluster come to both of these, in any case; `all`: the cluster's size.
+// All threads of all CTAs of a cluster come to both of these, in any case; `all`: the cluster's size.  The instructions want whole warps, which rows and columns shared out by thread may have split.
 __device__ __forceinline__ void cluster_meet(int all) {
+  __syncwarp();
   if (all > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
@@ -532,6 +533,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
               ref = top * p.scale2 - kBias;
               sum *= factor;
             }
+            __syncwarp();  // tensor memory is read by whole warps
             if (taken) {
               // O has everything up to the step before
               ok = attn_wait_all(&sh.done[q * kSlots + (taken - 1) % kSlots], ((taken - 1) / kSlots) & 1, sh);
@@ -1196,6 +1198,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
         r += lacking[k][row].y;
       }
       if (ok && in && part == 0) p.delta[side] = delta + lack;
+      __syncwarp();
       tc_fence_after();
       // 32 of the columns each
       static_assert(kParts * 32 == kD, "a part's columns");

@@ -639,6 +639,7 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
           float(&v)[32] = sums[0];
+          __syncwarp();
           tc_load32(lanes + st.acc * BN + (c + h) * 32, v);
           tc_load_wait(v);
 #pragma unroll
