@@ -47,6 +47,8 @@ struct AttnShape {
   // Heads of up to 64 values: two CTAs an SM, with half of the tensor memory each.
   static constexpr int kResident = kD == 128 ? 1 : 2;
   static constexpr int kColumns = 512 / kResident;
+  // Registers a thread that share_registers counts on, or 0 where it is not used; a kernel that was built with fewer is not launched.
+  static constexpr int kForwardRegisters = kResident == 2 ? 80 : 0, kBackwardRegisters = kResident == 2 ? 80 : 96;
   static constexpr int kSlots = kD == 128 ? 2 : 1;  // forward: steps of scores of a tile
   static constexpr int kForwardStages = kD == 128 ? 10 : 8;  // steps, half of them of keys and half of values
   static constexpr int kForwardSmem = 2 * kBytes + kForwardStages * kStepBytes + 1024;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kForwardThreads, AttnShape<kD>:
     }
   });
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-  if constexpr (S::kResident == 2) share_registers<96, S::kForwardThreads, 80>(warp < 4);
+  if constexpr (S::kResident == 2) share_registers<96, S::kForwardThreads, S::kForwardRegisters>(warp < 4);
   constexpr int kRing = kStages / 2;  // of keys; behind it that of values
   unsigned char* v_ring = ring + kRing * S::kStepBytes;
   // Groups that take the steps in turn need an even number of stages, so that a stage is always of the same group: one that does not wait for each of a barrier's phases cannot tell them apart.
@@ -950,7 +952,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
     load_rows<kD, kTile>(tile2, kKeys ? &p.v_tile : &p.dout_tile, t0, head, b, &sh.first);
   });
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-  share_registers<(S::kResident == 2 ? 96 : 104), S::kBackwardThreads, (S::kResident == 2 ? 80 : 96)>(warp < 4);
+  share_registers<(S::kResident == 2 ? 96 : 104), S::kBackwardThreads, S::kBackwardRegisters>(warp < 4);
   if (warp == 0) {
     if (kKeys && lane == 0) grid_dependency_wait();  // behind the queries' pass, whose delta comes in with the queries; the norms were there when it let this kernel begin
     if (lane == 0 && count) {
@@ -1327,7 +1329,7 @@ template <typename T, int kD>
 cudaError_t run_forward(const dev::AttnParams& p, cudaStream_t stream) {
   static unsigned long long allowed = 0;
   constexpr int smem = dev::AttnShape<kD>::kForwardSmem;
-  const cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed);
+  const cudaError_t e = allow_smem(dev::hc_attention_kernel<T, kD>, smem, &allowed, dev::AttnShape<kD>::kForwardRegisters);
   if (e != cudaSuccess) return e;
   const int64_t ctas = (int64_t)p.batch * (p.packed ? p.kv_heads : p.heads) * p.blocks * p.splits;
   return launch_with(dev::hc_attention_kernel<T, kD>, ctas, p.splits, dev::AttnShape<kD>::kForwardThreads, smem, stream, false, p);
@@ -1366,9 +1368,9 @@ cudaError_t run_few(const dev::FewRows& p, int warps, int batch, cudaStream_t st
 template <typename T, int kD>
 cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_heads& v, unsigned int* most, cudaStream_t stream) {
   static unsigned long long allowed_kv = 0, allowed_q = 0;
-  constexpr int smem = dev::AttnShape<kD>::kBackwardSmem;
-  cudaError_t e = allow_smem(dev::hc_attention_backward_kernel<T, kD, true>, smem, &allowed_kv);
-  if (e == cudaSuccess) e = allow_smem(dev::hc_attention_backward_kernel<T, kD, false>, smem, &allowed_q);
+  constexpr int smem = dev::AttnShape<kD>::kBackwardSmem, registers = dev::AttnShape<kD>::kBackwardRegisters;
+  cudaError_t e = allow_smem(dev::hc_attention_backward_kernel<T, kD, true>, smem, &allowed_kv, registers);
+  if (e == cudaSuccess) e = allow_smem(dev::hc_attention_backward_kernel<T, kD, false>, smem, &allowed_q, registers);
   if (e != cudaSuccess) return e;
   if (most) {
     constexpr int kLanes = kD / 8, kRows = 4 * 256 / kLanes;  // of a block

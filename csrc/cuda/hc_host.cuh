@@ -122,14 +122,20 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), int grid, int block, in
 }
 
 // The same, asked once for each device: `done` is the kernel's own, one bit a device.  All sizes up to the most that a block may
-// have are allowed then.
+// have are allowed then.  `registers`: what the kernel counts on having a thread; one that was built with fewer is refused.
 template <typename K>
-cudaError_t allow_smem(K kernel, int most, unsigned long long* done) {
+cudaError_t allow_smem(K kernel, int most, unsigned long long* done, int registers = 0) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned long long bit = 1ull << (dev & 63);
   if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return cudaSuccess;
+  if (registers > 0) {
+    cudaFuncAttributes a;
+    e = cudaFuncGetAttributes(&a, kernel);
+    if (e != cudaSuccess) return e;
+    if ((a.numRegs + 7) / 8 * 8 < registers) return cudaErrorInvalidConfiguration;
+  }
   e = set_smem(kernel, most);
   if (e == cudaSuccess) __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
   return e;
