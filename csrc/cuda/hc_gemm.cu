@@ -12,6 +12,7 @@
 // in a bank) and one TMA store takes them; what is added to a result comes in the same way, one piece ahead, and is
 // overwritten by the result in place.  Stored from registers, a row a thread, the projection 8192 x 2304 x 768 took 101 us.
 #include <initializer_list>
+#include <type_traits>
 
 #include "hc_gemm.cuh"
 #include "hc_host.cuh"
@@ -1071,7 +1072,7 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.most = c.most;
   p.factor = c.factor;
   p.loss = c.loss;
-  if (MODE == kGemmLossSums || MODE == dev::kGemmLossSumsWide) return cudaSuccess;
+  if (MODE == kGemmLossSums || MODE == dev::kGemmLossSumsWide) return p.tiles_n * 2ll <= c.loss.stretches ? cudaSuccess : cudaErrorInvalidValue;
   if (MODE == kGemmLossGrad) return make_side_map(&p.map_out, c.out, c.type, c, true, false, BN >= 128) ? cudaSuccess : cudaErrorInvalidValue;
   constexpr bool kLinear = MODE == kGemmLinear || MODE == dev::kGemmLinearWide, kUpdate = MODE == kGemmUpdate;
   if (MODE == kGemmLinear && BN >= 128 && c.out_type != kF32 && !c.in.data && make_side_map(&p.map_out, c.out, c.out_type, c, true, false, true))
@@ -1224,16 +1225,21 @@ int64_t gemm_cost(int64_t m, int64_t n, int64_t k, int parts) {
   return best_tile<kGemmLinear>(c, parts, sm_count()).cost;
 }
 
+// which of the two modes forms logits that are sums over k: for the room as for the launch
+template <typename F>
+auto with_loss_sums_mode(int64_t k, F f) {
+  return k > dev::kChunk * dev::kBK ? f(std::integral_constant<int, dev::kGemmLossSumsWide>()) : f(std::integral_constant<int, kGemmLossSums>());
+}
 int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k) {
   GemmCall c;
   memset(&c, 0, sizeof(c));
   c.m = m, c.n = n, c.k = k, c.batch = 1;
-  const int bn = best_tile<kGemmLossSums>(c, 1, sm_count()).bn;
+  const int bn = with_loss_sums_mode(k, [&](auto mode) { return best_tile<decltype(mode)::value>(c, 1, sm_count()).bn; });
   return (n + bn - 1) / bn * 2;
 }
 
 cudaError_t launch_loss_sums(const GemmCall& c, cudaStream_t stream) {
-  return c.k > dev::kChunk * dev::kBK ? run_gemm_mode<dev::kGemmLossSumsWide>(c, stream) : run_gemm_mode<kGemmLossSums>(c, stream);
+  return with_loss_sums_mode(c.k, [&](auto mode) { return run_gemm_mode<decltype(mode)::value>(c, stream); });
 }
 cudaError_t launch_loss_grad(const GemmCall& c, cudaStream_t stream) { return run_gemm_mode<kGemmLossGrad>(c, stream); }
 

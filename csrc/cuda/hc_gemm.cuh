@@ -111,6 +111,7 @@ struct GemmLoss {
   int64_t ignore;
   int64_t first;       // the vocabulary's number of column 0
   float2* sums;        // [stretch][row]: the largest logit of a stretch of columns and the sum of exp(logit - that); gemm_loss_stretches
+  int64_t stretches;   // for how many there is room in `sums`
   float* picked;       // the token's logit
   const float* lse;    // of a row
   const float* weight;
@@ -138,7 +139,7 @@ struct GemmCall {
 int gemm_parts(int64_t m, int64_t n, int64_t k);
 // What a call's time is reckoned to be, in cycles, in so many parts of its sum.
 int64_t gemm_cost(int64_t m, int64_t n, int64_t k, int parts);
-// stretches of columns of kGemmLossSums, two a tile
+// stretches of columns of kGemmLossSums, two a tile; launch_loss_sums refuses a call with room for fewer
 int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k);
 // of up to HC_LINEAR_FEW_ROWS rows, which may begin anywhere: sixteen columns a stretch, sums lie [row][stretch]
 cudaError_t launch_few_rows_loss(const GemmCall& call, cudaStream_t stream);

@@ -266,6 +266,7 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     const int64_t stretches = stretches_of(rows, inner, vocab);
     unsigned char* at = static_cast<unsigned char*>(scratch);
     c.loss.sums = reinterpret_cast<float2*>(at);
+    c.loss.stretches = stretches;
     at += up((size_t)stretches * rows * sizeof(float2), 256);
     c.loss.picked = reinterpret_cast<float*>(at);
     if (reduction != dev::kNone) losses = reinterpret_cast<float*>(at + up(rows * sizeof(float), 256));

@@ -89,3 +89,14 @@ def test_registers_that_are_shared_out(tmp_path):
         seen += 1
         assert (used + 7) // 8 * 8 >= (80 if kernel.group(2) == "64" else 96), name
     assert seen == 10
+
+
+def test_sums_of_logits_have_room(runtime, tmp_path):
+    """Scratch memory is counted for the tiles that are launched, and a launch that has less is refused."""
+    lib = _build.build_cuda()
+    exe = tmp_path / "loss_room"
+    csrc = _build.CSRC
+    subprocess.run([_build.nvcc_path(), *_build.NVCC_FLAGS, "-I", str(csrc / "include"), "-I", str(csrc / "cuda"), str(Path(__file__).with_name("loss_room.cu")), "-o", str(exe),
+                    str(lib), str(runtime), "-cudart", "shared", "-Xlinker", "-rpath=%s:%s" % (lib.parent, runtime.parent)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120, env={**os.environ, "LD_PRELOAD": str(runtime)})
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
