@@ -21,7 +21,7 @@ struct FewRowsParams {
   int64_t ldx, ldw, ldr, ldo, ldz;
   int64_t inner, width;
   int rows, out_type, bias_type, activation;
-  GemmLoss loss;  // `sums`: results are logits, of which each row's largest and sum of exponentials over a block's sixteen go to [row][block]
+  GemmLoss loss;  // of logits: each row's largest and sum of exponentials over a block's sixteen go to `sums` [row][block]
 };
 
 __device__ __forceinline__ float act_value(float z, int kind) {
@@ -56,7 +56,8 @@ __device__ __forceinline__ uint4 few_group(const T* row, int64_t k, int64_t end,
   return k + 8 * t < end ? *reinterpret_cast<const uint4*>(row + k + 8 * t) : make_uint4(0, 0, 0, 0);
 }
 constexpr int kFewWarps = 16;  // at most, of a block
-template <typename T, int N, bool kVector>  // N: eights of rows
+// N: eights of rows.  kLoss: results are logits, of which p.loss.sums gets what is kept (a branch at run time costs the other form registers: 8 bytes spilled with N = 2).
+template <typename T, int N, bool kVector, bool kLoss>
 __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __grid_constant__ FewRowsParams p) {
   __shared__ float parts[kFewWarps][N * 8][17];
   constexpr int kSteps = 4;  // of 32 along the sum, whose loads are under way together
@@ -117,10 +118,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
     const int r = i >> 4;
     const int64_t n = first + (i & 15);
     const bool there = r < p.rows && n < p.width;
-    if (!there && !p.loss.sums) continue;
+    if (!kLoss && !there) continue;
     float z = 0.0f;
     for (int w = 0; w < warps; ++w) z += parts[w][r][i & 15];
-    if (p.loss.sums) {  // over the sixteen lanes of a row
+    if constexpr (kLoss) {  // over the sixteen lanes of a row
       float most = there ? z : -INFINITY;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -439,25 +440,26 @@ int shares_of(size_t rows, size_t width, int activation) {
   return (int)(shares ? shares : 1);
 }
 
-template <typename T, int N>
+template <typename T, int N, bool kLoss>
 void few_rows_of(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
   // eight warps a block; sixteen where that leaves SMs without a block and each warp has a step to go
   const unsigned grid = (unsigned)((p.width + 15) / 16);
   const unsigned threads = (int)grid <= device_info().sms && p.inner >= 1024 ? 512 : 256;
-  if (vector) dev::hc_few_rows_kernel<T, N, true><<<grid, threads, 0, stream>>>(p);
-  else dev::hc_few_rows_kernel<T, N, false><<<grid, threads, 0, stream>>>(p);
+  if (vector) dev::hc_few_rows_kernel<T, N, true, kLoss><<<grid, threads, 0, stream>>>(p);
+  else dev::hc_few_rows_kernel<T, N, false, kLoss><<<grid, threads, 0, stream>>>(p);
 }
-template <typename T>
+template <typename T, bool kLoss>
 void few_rows(const dev::FewRowsParams& p, bool vector, cudaStream_t stream) {
   static_assert(kFewRows <= 16, "two eights of rows");
-  if (p.rows <= 8) few_rows_of<T, 1>(p, vector, stream);
-  else few_rows_of<T, 2>(p, vector, stream);
+  if (p.rows <= 8) few_rows_of<T, 1, kLoss>(p, vector, stream);
+  else few_rows_of<T, 2, kLoss>(p, vector, stream);
 }
 
+template <bool kLoss>
 void run_few_rows(const dev::FewRowsParams& p, int type, cudaStream_t stream) {
   const bool vector = p.inner % 8 == 0 && gemm_operand_ok(p.x, p.ldx) && gemm_operand_ok(p.w, p.ldw);
-  if (type == kBf16) few_rows<__nv_bfloat16>(p, vector, stream);
-  else few_rows<__half>(p, vector, stream);
+  if (type == kBf16) few_rows<__nv_bfloat16, kLoss>(p, vector, stream);
+  else few_rows<__half, kLoss>(p, vector, stream);
 }
 
 template <typename Y, typename T, int kAct>
@@ -536,7 +538,7 @@ cudaError_t launch_few_rows_loss(const GemmCall& c, cudaStream_t stream) {
   // a warp to sixteen tokens where there are sixteens for most warps that the SMs hold, and 16-byte loads
   const int64_t groups = (c.n + 15) / 16, resident = (int64_t)(device_info().sms > 0 ? device_info().sms : 1) * (c.m <= 8 ? 3 : 2);
   if (groups < resident * 2 || !(c.k % 8 == 0 && gemm_operand_ok(c.a.data, c.a.ld) && gemm_operand_ok(c.b.data, c.b.ld))) {
-    run_few_rows(p, c.type, stream);
+    run_few_rows<true>(p, c.type, stream);
     return cudaGetLastError();
   }
   const unsigned grid = (unsigned)((groups + 7) / 8 < resident ? (groups + 7) / 8 : resident);
@@ -586,7 +588,7 @@ int hc_linear(const void* x, size_t x_stride, const void* weight, size_t weight_
   if (rows <= kFewRows) {
     const dev::FewRowsParams p = {x, weight, bias, residual, out, z, (int64_t)x_stride, (int64_t)weight_stride, (int64_t)residual_stride,
                                   (int64_t)out_stride, (int64_t)z_stride, (int64_t)inner, (int64_t)width, (int)rows, out_type, bias_type, activation};
-    run_few_rows(p, type, stream);
+    run_few_rows<false>(p, type, stream);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
   }
   if (!gemm_operand_ok(x, x_stride) || !gemm_operand_ok(weight, weight_stride)) return kErrArgument;
