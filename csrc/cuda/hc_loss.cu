@@ -20,6 +20,15 @@ namespace dev {
 
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
 
+// What a row's largest logit and sum of exponentials relative to it come to: lse, and its loss, which takes the token's logit from the largest first: of a row that is sure of its token little is
+// left, which lse, rounded at its own size, no longer has.  A row with an infinite logit has a NaN among its sums, one of -inf alone a sum of 0.
+__device__ __forceinline__ void loss_of_row(float most, float sum, int64_t row, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse, float* losses) {
+  const float none = __int_as_float(0x7fc00000), rest = sum > 0.0f || sum != sum ? logf(sum) : none;
+  const int64_t token = tokens[row];
+  lse[row] = most + rest;
+  losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? (most - picked[row]) + rest : none;
+}
+
 // Joins the stretches of 32 rows: warp w takes every 32nd, a lane a row.
 __global__ void __launch_bounds__(1024) hc_loss_join_kernel(const float2* sums, int64_t stretches, int64_t rows, const float* picked, const int64_t* tokens, int64_t ignore,
                                                              int64_t vocab, float* lse, float* losses) {
@@ -40,11 +49,7 @@ __global__ void __launch_bounds__(1024) hc_loss_join_kernel(const float2* sums, 
   __syncthreads();
   if (warp != 0 || row >= rows) return;
   for (int w = 1; w < 32; ++w) take(shared[w][lane]);
-  // a row with an infinite logit has a NaN among its sums, one of -inf alone a sum of 0
-  const float all = sum > 0.0f || sum != sum ? most + logf(sum) : __int_as_float(0x7fc00000);
-  const int64_t token = tokens[row];
-  lse[row] = all;
-  losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? all - picked[row] : __int_as_float(0x7fc00000);
+  loss_of_row(most, sum, row, picked, tokens, ignore, vocab, lse, losses);
 }
 
 // The same of few rows, a block each, whose stretches lie one after the other.  Its launch overlaps the products' (1 row of 768, 50257 tokens: 19.6 us a call, 20.6 without).
@@ -83,10 +88,7 @@ __global__ void __launch_bounds__(1024) hc_loss_join_row_kernel(const float2* su
     joined(most, sum, m, s);
   }
   if (lane != 0) return;
-  const float all = sum > 0.0f || sum != sum ? most + logf(sum) : __int_as_float(0x7fc00000);
-  const int64_t token = tokens[row];
-  lse[row] = all;
-  losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? all - picked[row] : __int_as_float(0x7fc00000);
+  loss_of_row(most, sum, row, picked, tokens, ignore, vocab, lse, losses);
 }
 
 // their sum, or their mean over the rows that have a token, whose number is kept for the backward pass

@@ -1,0 +1,57 @@
+"""Cross entropy from hidden rows where a row is sure of a token: what is left of the loss, and of the gradient at the token, is small beside the logits.
+
+All rows of W are alike but for two of their values, so that logits differ by what these bring: `off` (a whole number) for a token that stands out, over a column of x that is 1, and nothing for the
+column of x that is 0, which carries a token's mark into dx.  The loss is then log1p((vocabulary - 1) exp(-off)) at logits of any size, without rounding.
+
+Tolerances.  u and h are half a step of fp32 and of the operands' type.  The sums of exponentials have their largest term, 1, and are off by u for each addition behind it: 16 and 5 in a
+stretch of columns, 31 and 32 where stretches are joined, twice that for products with powers of two that are 1 only to a step; the others are off by 4 u + 3 u off of themselves.  The sums
+that logits are differ in their last step alone: by 4 whole steps of fp32 at the logit's size, for the instruction's addition and that of a part of the sum."""
+import math
+
+import pytest
+import torch
+
+from tirocinio_triennale_b200 import ops
+
+U = torch.finfo(torch.float32).eps / 2
+BF16, F16 = torch.bfloat16, torch.float16
+ADDITIONS = 2 * (16 + 5 + 31 + 32)
+
+
+def make(rows, inner, vocab, size, off, kind, stands_out, exact=False, seed=0):
+    """x and W of logits of about `size`; of each row token `stands_out` is `off` above the others."""
+    g = torch.Generator().manual_seed(seed + rows + inner)
+    x, w = torch.zeros(rows, inner), torch.zeros(vocab, inner)
+    if exact:  # one product of powers of two, the same in all rows
+        x[:, 0], w[:, 0] = 2.0 ** 4, size / 2.0 ** 4
+    else:  # sums of products that are all positive
+        x[:, :inner - 2] = 0.5 + torch.rand(rows, inner - 2, generator=g)
+        w[:, :inner - 2] = (0.5 + torch.rand(inner - 2, generator=g)) * size / inner
+    x[:, -1] = 1.0
+    w[:, -1] = -off
+    w[stands_out, -1] = 0.0
+    w[stands_out, -2] = 1.0  # where x is 0: dx there is G of that token
+    return x.to(kind).cuda(), w.to(kind).cuda()
+
+
+def room_of(loss, logit, off):
+    """of a loss, relative to itself"""
+    return U * ADDITIONS / loss + U * (8 + 3 * off) + 4 * 2 * U * 2.0 ** math.ceil(math.log2(logit))
+
+
+SIZES = [(1, 64, 16), (5, 3, 7), (16, 1000, 1000), (17, 40, 64), (300, 700, 100), (700, 3001, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("size", [16, 512, 8192])
+@pytest.mark.parametrize("rows,vocab,inner", SIZES)
+def test_small_losses_beside_large_logits(rows, vocab, inner, size, kind):
+    for off in (4, 9, 13):
+        x, w = make(rows, inner, vocab, size, off, kind, vocab // 2, exact=True)
+        t = torch.full((rows,), vocab // 2, device="cuda")
+        want = math.log1p((vocab - 1) * math.exp(-off))
+        room = want * room_of(want, size, off) - want * 8 * U * 2.0 ** math.ceil(math.log2(size))  # these sums are exact
+        for reduction in ("none", "mean", "sum"):
+            loss = ops.linear_cross_entropy(x, w, t, reduction=reduction).double() / (rows if reduction == "sum" else 1)
+            assert ((loss - want).abs() <= 1.01 * room + U * want).all(), (float((loss - want).abs().max()), want)
