@@ -363,8 +363,8 @@ __device__ __forceinline__ void gemm_finish_half(const GemmParams& p, float (&v)
   for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(wide_at(out, lane, half * 4 + i)) = pack8_as(v + i * 8, p.type);
 }
 
-// 32 logits of a row from column `col` on, of which `count` are of the vocabulary, taken up into the row's largest logit and the sum of
-// exponentials relative to it.  A NaN, or an infinite logit, makes the sum NaN; a row of -inf alone has a sum of 0.
+// 32 logits of a row, of which `count` are of the vocabulary and one may be its token's, which goes to `picked`; the others are taken up into their largest and the sum of
+// exponentials relative to it.  A NaN, or an infinite logit, makes the sum NaN; of -inf alone, or nothing, it is 0.
 __device__ __forceinline__ void loss_take(float (&v)[32], int64_t count, int64_t token, float& most, float& sum, float* picked) {
   if (count < 32) {
 #pragma unroll
@@ -380,6 +380,8 @@ __device__ __forceinline__ void loss_take(float (&v)[32], int64_t count, int64_t
 #pragma unroll
       for (int j = 0; j < 16 >> bit; ++j) w[j] = token >> bit & 1 ? w[2 * j + 1] : w[2 * j];
     *picked = w[0];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = j == (int)token ? -INFINITY : v[j];
   }
   float top = fmaxf(v[0], v[1]);
 #pragma unroll

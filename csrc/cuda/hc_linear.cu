@@ -21,7 +21,7 @@ struct FewRowsParams {
   int64_t ldx, ldw, ldr, ldo, ldz;
   int64_t inner, width;
   int rows, out_type, bias_type, activation;
-  GemmLoss loss;  // of logits: each row's largest and sum of exponentials over a block's sixteen go to `sums` [row][block]
+  GemmLoss loss;  // of logits: each row's largest and sum of exponentials over a block's sixteen go to `sums` [row][block], its token's to `picked`
 };
 
 __device__ __forceinline__ float act_value(float z, int kind) {
@@ -122,14 +122,15 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
     float z = 0.0f;
     for (int w = 0; w < warps; ++w) z += parts[w][r][i & 15];
     if constexpr (kLoss) {  // over the sixteen lanes of a row
-      float most = there ? z : -INFINITY;
+      const bool own = there && p.loss.tokens[r] == n, other = there && !own;
+      float most = other ? z : -INFINITY;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      float sum = there ? exp2f((z - (most == -INFINITY ? 0.0f : most)) * kLog2E) : 0.0f;
+      float sum = other ? exp2f((z - (most == -INFINITY ? 0.0f : most)) * kLog2E) : 0.0f;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if ((i & 15) == 0 && r < p.rows) p.loss.sums[(int64_t)r * gridDim.x + blockIdx.x] = make_float2(most, sum);
-      if (there && p.loss.tokens[r] == n) p.loss.picked[r] = z;
+      if (own) p.loss.picked[r] = z;
       continue;
     }
     if (p.bias) z += param_at(p.bias, p.bias_type, n);
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) hc_few_rows_kernel(const __gri
   }
 }
 
-// Logits of a few rows over a vocabulary, of which only each row's largest and sum of exponentials over sixteen tokens are kept ([row][sixteen]).  A warp has sixteen rows of W to itself, all
+// Logits of a few rows over a vocabulary, of which only each row's own token's is kept, and of the others the largest and the sum of exponentials over sixteen tokens ([row][sixteen]).  A warp has sixteen rows of W to itself, all
 // along the sum, so nothing is shared and nothing waits: one row of 768 -> 50257 takes 15 us (5.0 TB/s), 27 with the kernel above, whose blocks have six steps of loads each and meet to add.
 template <typename T, int N>
 __global__ void __launch_bounds__(256, N == 1 ? 3 : 2) hc_few_rows_loss_kernel(const __grid_constant__ FewRowsParams p) {
@@ -207,7 +208,15 @@ __global__ void __launch_bounds__(256, N == 1 ? 3 : 2) hc_few_rows_loss_kernel(c
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = n * 8 + 2 * t + j;
-        const float lower = first + g <= last ? sum[n][j] : -INFINITY, upper = first + g + 8 <= last ? sum[n][j + 2] : -INFINITY;
+        const int64_t token = row < p.rows ? p.loss.tokens[row] - first : -1;
+        float lower = first + g <= last ? sum[n][j] : -INFINITY, upper = first + g + 8 <= last ? sum[n][j + 2] : -INFINITY;
+        if (token == g && first + g <= last) {
+          p.loss.picked[row] = lower;
+          lower = -INFINITY;
+        } else if (token == g + 8 && first + g + 8 <= last) {
+          p.loss.picked[row] = upper;
+          upper = -INFINITY;
+        }
         float most = fmaxf(lower, upper);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -215,11 +224,7 @@ __global__ void __launch_bounds__(256, N == 1 ? 3 : 2) hc_few_rows_loss_kernel(c
         float total = exp2f((lower - ref) * kLog2E) + exp2f((upper - ref) * kLog2E);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (row >= p.rows) continue;
-        if (g == 0) p.loss.sums[row * groups + group] = make_float2(most, total);
-        const int64_t token = p.loss.tokens[row] - first;
-        if (token == g && token + first <= last) p.loss.picked[row] = lower;
-        if (token == g + 8 && token + first <= last) p.loss.picked[row] = upper;
+        if (row < p.rows && g == 0) p.loss.sums[row * groups + group] = make_float2(most, total);
       }
   }
 }

@@ -3,7 +3,7 @@
 //   l_iv = x_i . w_v,  lse_i = log sum_v exp l_iv,  loss_i = lse_i - l_i,token
 //   G_iv = a_i (exp(l_iv - lse_i) - [v = token_i]),  dx = G W,  dW = G^T x         (a: the upstream gradient of a row)
 //
-// Forward, one product whose epilogue keeps each row's largest logit and sum of exponentials over a stretch of columns (hc_gemm.cu): 8 bytes for 32
+// Forward, one product whose epilogue keeps each row's largest logit and sum of exponentials over a stretch of columns (hc_gemm.cu), its token's logit apart: 8 bytes for 32
 // to 128 logits, joined by a second kernel.  Backward, a piece of the vocabulary at a time: its logits are formed again, G leaves the
 // epilogue in 16 bits, and two products take it up: dx is summed over the pieces in fp32, the piece of dW is done.  That is four products where three
 // would do with the logits kept; kept in 16 bits they would be wrong by 2^-9 of themselves, and G by as much times the logit.  G rounded to 16 bits is what any
@@ -20,13 +20,20 @@ namespace dev {
 
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
 
-// What a row's largest logit and sum of exponentials relative to it come to: lse, and its loss, which takes the token's logit from the largest first: of a row that is sure of its token little is
-// left, which lse, rounded at its own size, no longer has.  A row with an infinite logit has a NaN among its sums, one of -inf alone a sum of 0.
+// A row's loss and lse from its token's logit z and what the others come to, their largest and their sum of exponentials relative to it: with d = log sum of the others - z, loss = log(1 + exp d).  The token
+// has no part in the sum: of a row that is sure of its token little is left, which a sum that begins with the token's 1, or lse, rounded at its own size, no longer has.  A row with an infinite logit,
+// or a NaN, has a NaN among its sums (or as z); where all others are -inf their sum is 0.
 __device__ __forceinline__ void loss_of_row(float most, float sum, int64_t row, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse, float* losses) {
-  const float none = __int_as_float(0x7fc00000), rest = sum > 0.0f || sum != sum ? logf(sum) : none;
+  const float none = __int_as_float(0x7fc00000), others = most + logf(sum);
   const int64_t token = tokens[row];
-  lse[row] = most + rest;
-  losses[row] = token == ignore ? 0.0f : token >= 0 && token < vocab ? (most - picked[row]) + rest : none;
+  if (token == ignore || token < 0 || token >= vocab) {
+    lse[row] = sum == 0.0f ? none : others;
+    losses[row] = token == ignore ? 0.0f : none;
+    return;
+  }
+  const float z = picked[row], d = (most - z) + logf(sum), above = log1pf(expf(-fabsf(d)));
+  lse[row] = z < INFINITY ? (d > 0.0f ? others : z) + above : none;
+  losses[row] = z < INFINITY ? d > 0.0f ? d + above : above : none;
 }
 
 // Joins the stretches of 32 rows: warp w takes every 32nd, a lane a row.

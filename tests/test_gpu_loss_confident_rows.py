@@ -55,3 +55,37 @@ def test_small_losses_beside_large_logits(rows, vocab, inner, size, kind):
         for reduction in ("none", "mean", "sum"):
             loss = ops.linear_cross_entropy(x, w, t, reduction=reduction).double() / (rows if reduction == "sum" else 1)
             assert ((loss - want).abs() <= 1.01 * room + U * want).all(), (float((loss - want).abs().max()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("rows,vocab,inner", SIZES + [(16, 50257, 64), (33, 13001, 16)])
+def test_losses_far_below_one(rows, vocab, inner, kind):
+    """Their digits are those of the others' sum, in which the token's own 1 has no part."""
+    for size in (16, 8192):
+        for off in (16, 24, 32):
+            x, w = make(rows, inner, vocab, size, off, kind, vocab - 1, exact=True)
+            want = math.log1p((vocab - 1) * math.exp(-off))
+            loss = ops.linear_cross_entropy(x, w, torch.full((rows,), vocab - 1, device="cuda"), reduction="none").double()
+            assert ((loss - want).abs() <= want * U * (ADDITIONS + 8 + 3 * off)).all(), (float((loss - want).abs().max()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 16, 40])
+def test_logits_that_are_no_numbers(rows):
+    """Of the token itself, or of another one."""
+    inner, vocab = 8, 700
+    for token in (3, 699):
+        for at in (3, 699):
+            for value, want in ((math.inf, math.nan), (math.nan, math.nan), (-math.inf, math.inf if at == token else math.log(vocab - 1))):
+                w = torch.zeros(vocab, inner, dtype=BF16, device="cuda")
+                x = torch.ones(rows, inner, dtype=BF16, device="cuda")
+                w[at, 0] = value
+                loss = ops.linear_cross_entropy(x, w, torch.full((rows,), token, device="cuda"), reduction="none")
+                assert torch.allclose(loss, torch.full_like(loss, want), rtol=1e-5, atol=0, equal_nan=True), (token, at, value)
+        w = torch.full((vocab, inner), -math.inf, dtype=BF16, device="cuda")
+        t = torch.full((rows,), token, device="cuda")
+        assert ops.linear_cross_entropy(x, w, t, reduction="none").isnan().all()
+        w[token] = 1.0  # and no other
+        assert (ops.linear_cross_entropy(x, w, t, reduction="none") == 0).all()
+    assert (ops.linear_cross_entropy(x, w[token:token + 1], torch.zeros_like(t), reduction="none") == 0).all()
