@@ -631,8 +631,11 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
       const int64_t given = in ? p.loss.tokens[row] : p.loss.ignore, token = given - p.loss.first;
       const bool kept = given != p.loss.ignore;
       const float less = kept ? -p.loss.lse[row] : 0.0f;
-      float weight = kept ? p.loss.weight[row] : 0.0f;
-      if (p.most) weight *= gradient_power(p.most, 1);
+      float weight = kept ? p.loss.weight[row] : 0.0f, picked = kept ? p.loss.picked[row] : 0.0f;
+      if (p.most) {
+        weight *= gradient_power(p.most, 1);
+        picked *= gradient_power(p.most, 1);
+      }
       constexpr int kPer = BN >= 128 ? 2 : 1;  // pieces of a box
 #pragma unroll 1
       for (int c = half * kPer; c < pieces; c += 2 * kPer) {
@@ -654,7 +657,7 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
           const int64_t at = token - (col0 + (c + h) * 32);
           if (at >= 0 && at < 32) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = j == (int)at ? v[j] - weight : v[j];
+            for (int j = 0; j < 32; ++j) v[j] = j == (int)at ? picked : v[j];
           }
           if (!kept) {  // also where the row's logits are no numbers
 #pragma unroll

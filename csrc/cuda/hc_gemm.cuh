@@ -13,7 +13,7 @@ enum GemmMode : int {
   kGemmPoly = 2,    // out = b c1 + c acc, symmetric (c1: the operand itself)
   kGemmUpdate = 3,  // x = a (hi + lo / 2048) + acc; out hi and lo again, or bf16
   kGemmLossSums = 6,  // acc are logits: the one of the row's token; of the others the largest and the sum of exponentials, over stretches of columns
-  kGemmLossGrad = 7,  // out = weight (exp(acc - lse) - [the row's token])
+  kGemmLossGrad = 7,  // out = weight exp(acc - lse), at the row's token `picked`
 };
 enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActRelu = 2, kActSilu = 3 };
 
@@ -112,7 +112,7 @@ struct GemmLoss {
   int64_t first;       // the vocabulary's number of column 0
   float2* sums;        // [stretch][row]: the largest logit of a stretch of columns and the sum of exp(logit - that), without the token's; gemm_loss_stretches
   int64_t stretches;   // for how many there is room in `sums`
-  float* picked;       // the token's logit
+  float* picked;       // the token's logit; for kGemmLossGrad what `out` has at the token (read)
   const float* lse;    // of a row
   const float* weight;
 };

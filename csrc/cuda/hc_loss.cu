@@ -23,22 +23,25 @@ enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
 // A row's loss and lse from its token's logit z and what the others come to, their largest and their sum of exponentials relative to it: with d = log sum of the others - z, loss = log(1 + exp d).  The token
 // has no part in the sum: of a row that is sure of its token little is left, which a sum that begins with the token's 1, or lse, rounded at its own size, no longer has.  A row with an infinite logit,
 // or a NaN, has a NaN among its sums (or as z); where all others are -inf their sum is 0.
-__device__ __forceinline__ void loss_of_row(float most, float sum, int64_t row, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse, float* losses) {
+__device__ __forceinline__ void loss_of_row(float most, float sum, int64_t row, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse, float* kept,
+                                            float* losses) {
   const float none = __int_as_float(0x7fc00000), others = most + logf(sum);
   const int64_t token = tokens[row];
   if (token == ignore || token < 0 || token >= vocab) {
     lse[row] = sum == 0.0f ? none : others;
-    losses[row] = token == ignore ? 0.0f : none;
+    kept[row] = token == ignore ? 0.0f : none;
+    if (losses) losses[row] = kept[row];
     return;
   }
   const float z = picked[row], d = (most - z) + logf(sum), above = log1pf(expf(-fabsf(d)));
   lse[row] = z < INFINITY ? (d > 0.0f ? others : z) + above : none;
-  losses[row] = z < INFINITY ? d > 0.0f ? d + above : above : none;
+  kept[row] = z < INFINITY ? d > 0.0f ? d + above : above : none;
+  if (losses) losses[row] = kept[row];
 }
 
 // Joins the stretches of 32 rows: warp w takes every 32nd, a lane a row.
 __global__ void __launch_bounds__(1024) hc_loss_join_kernel(const float2* sums, int64_t stretches, int64_t rows, const float* picked, const int64_t* tokens, int64_t ignore,
-                                                             int64_t vocab, float* lse, float* losses) {
+                                                             int64_t vocab, float* lse, float* kept, float* losses) {
   __shared__ float2 shared[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x * 32ll + lane;
@@ -56,12 +59,12 @@ __global__ void __launch_bounds__(1024) hc_loss_join_kernel(const float2* sums, 
   __syncthreads();
   if (warp != 0 || row >= rows) return;
   for (int w = 1; w < 32; ++w) take(shared[w][lane]);
-  loss_of_row(most, sum, row, picked, tokens, ignore, vocab, lse, losses);
+  loss_of_row(most, sum, row, picked, tokens, ignore, vocab, lse, kept, losses);
 }
 
 // The same of few rows, a block each, whose stretches lie one after the other.  Its launch overlaps the products' (1 row of 768, 50257 tokens: 19.6 us a call, 20.6 without).
 __global__ void __launch_bounds__(1024) hc_loss_join_row_kernel(const float2* sums, int64_t stretches, const float* picked, const int64_t* tokens, int64_t ignore, int64_t vocab, float* lse,
-                                                                 float* losses) {
+                                                                 float* kept, float* losses) {
   __shared__ float tops[32], totals[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(1024) hc_loss_join_row_kernel(const float2* su
     joined(most, sum, m, s);
   }
   if (lane != 0) return;
-  loss_of_row(most, sum, row, picked, tokens, ignore, vocab, lse, losses);
+  loss_of_row(most, sum, row, picked, tokens, ignore, vocab, lse, kept, losses);
 }
 
 // their sum, or their mean over the rows that have a token, whose number is kept for the backward pass
@@ -128,9 +131,10 @@ __global__ void __launch_bounds__(1024) hc_loss_reduce_kernel(const float* losse
 }
 
 // Each row's weight in the gradient, and the bits of the largest of them.  Where all rows weigh the same G is formed with weights of 1 and the results are taken times `factor`: of a token that a row
-// hardly expects G is then -1 to within p, and what rounding G costs is less.
+// hardly expects G is then -1 to within p, and what rounding G costs is less.  G at a row's token, -(1 - p), is made of its loss: exp(logit - lse), which is off by lse's rounding and by what the two passes'
+// sums differ by, has nothing left of 1 - p where the row is sure of its token.
 __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss, const int64_t* tokens, int64_t ignore, int64_t rows, int64_t vocab, int reduction,
-                                                              const float* count, float* weight, unsigned int* most, float* factor) {
+                                                              const float* losses, const float* count, float* weight, float* picked, unsigned int* most, float* factor) {
   unsigned int largest = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0 && factor) *factor = reduction == kSum ? dloss[0] : *count > 0.0f ? dloss[0] / *count : 0.0f;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows; i += gridDim.x * 256ll) {
@@ -141,6 +145,7 @@ __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss
       if (token < 0 || token >= vocab) a = __int_as_float(0x7fc00000);
     }
     weight[i] = a;
+    picked[i] = token != ignore ? a * expm1f(-losses[i]) : 0.0f;
     const unsigned int bits = __float_as_uint(a) & 0x7fffffffu;
     if (bits < 0x7f800000u) largest = max(largest, bits);
   }
@@ -192,7 +197,7 @@ bool loss_sizes_ok(size_t rows, size_t inner, size_t vocab) { return inner > 0 &
 int64_t stretches_of(size_t rows, size_t inner, size_t vocab) { return rows <= HC_LINEAR_FEW_ROWS ? (int64_t)(vocab + 15) / 16 : gemm_loss_stretches(rows, vocab, inner); }
 size_t forward_bytes(size_t rows, size_t inner, size_t vocab) {
   if (!rows) return 0;
-  return up((size_t)stretches_of(rows, inner, vocab) * rows * sizeof(float2), 256) + 2 * up(rows * sizeof(float), 256);
+  return up((size_t)stretches_of(rows, inner, vocab) * rows * sizeof(float2), 256) + up(rows * sizeof(float), 256);
 }
 
 // Into how many parts the sum of dx's product with a piece is shared out, each of which is summed over the pieces in an array of its own: 96 tiles of 256 x 256 on 74 pairs of SMs leave a third of
@@ -232,7 +237,7 @@ size_t piece_of(size_t rows, size_t inner, size_t vocab) {
 }
 struct LossLayout {
   int parts;  // of dx
-  size_t piece, g, dx, weight, most, total;  // offsets, G at 0
+  size_t piece, g, dx, weight, picked, most, total;  // offsets, G at 0
 };
 LossLayout backward_layout(size_t rows, size_t inner, size_t vocab) {
   LossLayout l;
@@ -240,7 +245,8 @@ LossLayout backward_layout(size_t rows, size_t inner, size_t vocab) {
   l.parts = dx_parts_of(rows, inner, l.piece);
   l.dx = up(rows * up(l.piece, 8) * 2, 256);
   l.weight = l.dx + up((size_t)l.parts * rows * up(inner, 8) * sizeof(float), 256);
-  l.most = l.weight + up(rows * sizeof(float), 256);
+  l.picked = l.weight + up(rows * sizeof(float), 256);
+  l.most = l.picked + up(rows * sizeof(float), 256);
   l.total = l.most + kMostBytes;
   return l;
 }
@@ -262,7 +268,7 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
   using namespace hc;
   if ((type != kBf16 && type != kF16) || reduction < 0 || reduction > 2 || !loss_sizes_ok(rows, inner, vocab)) return kErrArgument;
   if (!lies_at(loss, 4) || !lies_at(stats, 4) || !lies_at(tokens, 8) || (!loss && (rows || reduction)) || !stats) return kErrArgument;
-  float *losses = loss, *lse = stats, *count = stats + rows;
+  float *losses = reduction == dev::kNone ? loss : nullptr, *lse = stats, *kept = stats + rows, *count = stats + 2 * rows;
   if (rows) {
     if (!tokens || !operands_ok(x, x_stride, weight, weight_stride, inner, rows <= HC_LINEAR_FEW_ROWS)) return kErrArgument;
     if (!scratch || !lies_at(scratch, 256) || scratch_bytes < forward_bytes(rows, inner, vocab)) return kErrArgument;
@@ -278,7 +284,6 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     c.loss.stretches = stretches;
     at += up((size_t)stretches * rows * sizeof(float2), 256);
     c.loss.picked = reinterpret_cast<float*>(at);
-    if (reduction != dev::kNone) losses = reinterpret_cast<float*>(at + up(rows * sizeof(float), 256));
     c.loss.tokens = tokens;
     c.loss.ignore = ignore;
     const bool few = rows <= HC_LINEAR_FEW_ROWS;
@@ -286,14 +291,14 @@ int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, 
     const float2* sums = c.loss.sums;
     const float* picked = c.loss.picked;
     if (few) {
-      if (launch_with(dev::hc_loss_join_row_kernel, (int64_t)rows, 1, 1024, 0, stream, true, sums, stretches, picked, tokens, ignore, (int64_t)vocab, lse, losses) != cudaSuccess) return kErrCuda;
+      if (launch_with(dev::hc_loss_join_row_kernel, (int64_t)rows, 1, 1024, 0, stream, true, sums, stretches, picked, tokens, ignore, (int64_t)vocab, lse, kept, losses) != cudaSuccess) return kErrCuda;
     } else {
-      dev::hc_loss_join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(sums, stretches, (int64_t)rows, picked, tokens, ignore, (int64_t)vocab, lse, losses);
+      dev::hc_loss_join_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(sums, stretches, (int64_t)rows, picked, tokens, ignore, (int64_t)vocab, lse, kept, losses);
     }
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   }
   if (reduction == dev::kNone) return kOk;
-  dev::hc_loss_reduce_kernel<<<1, 1024, 0, stream>>>(losses, tokens, ignore, (int64_t)rows, reduction, loss, count);
+  dev::hc_loss_reduce_kernel<<<1, 1024, 0, stream>>>(kept, tokens, ignore, (int64_t)rows, reduction, loss, count);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
@@ -315,12 +320,13 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
   const LossLayout l = backward_layout(rows, inner, vocab);
   if (!scratch || !lies_at(scratch, 256) || scratch_bytes < l.total) return kErrArgument;
   unsigned char* at = static_cast<unsigned char*>(scratch);
-  float *dx_sum = reinterpret_cast<float*>(at + l.dx), *row_weight = reinterpret_cast<float*>(at + l.weight);
+  float *dx_sum = reinterpret_cast<float*>(at + l.dx), *row_weight = reinterpret_cast<float*>(at + l.weight), *picked = reinterpret_cast<float*>(at + l.picked);
   unsigned int* most = type == kF16 ? reinterpret_cast<unsigned int*>(at + l.most) : nullptr;
   float* factor = reduction != dev::kNone ? reinterpret_cast<float*>(at + l.most + 4) : nullptr;
   if (most && cudaMemsetAsync(most, 0, sizeof(*most), stream) != cudaSuccess) return kErrCuda;
   const size_t blocks = (rows + 255) / 256;
-  dev::hc_loss_weights_kernel<<<(unsigned)(blocks < 256 ? blocks : 256), 256, 0, stream>>>(dloss, tokens, ignore, (int64_t)rows, (int64_t)vocab, reduction, stats + rows, row_weight, most, factor);
+  dev::hc_loss_weights_kernel<<<(unsigned)(blocks < 256 ? blocks : 256), 256, 0, stream>>>(dloss, tokens, ignore, (int64_t)rows, (int64_t)vocab, reduction, stats + rows, stats + 2 * rows,
+                                                                                     row_weight, picked, most, factor);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   const int64_t dx_ld = (int64_t)up(inner, 8);
   for (size_t first = 0; first < vocab; first += l.piece) {
@@ -341,6 +347,7 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
     c.loss.first = (int64_t)first;
     c.loss.lse = stats;
     c.loss.weight = row_weight;
+    c.loss.picked = picked;
     if (launch_loss_grad(c, stream) != cudaSuccess) return kErrCuda;
     c.factor = factor;
     if (dweight) {

@@ -113,7 +113,7 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
 // of a product lie (16-byte aligned, strides multiples of 8; without a backward pass up to HC_LINEAR_FEW_ROWS rows, and their weights, may begin anywhere), sides below 2^26; sums in the tensor core over up to 1024 terms.
 // reduction: 0 none (loss: a value a row), 1 sum, 2 mean over the rows that have a token (loss: one value; NaN where there are none).  A row whose token is `ignore`
 // gives 0 and a gradient of 0, whatever it holds, and enters dweight times 0; a token outside the vocabulary gives NaN, in the gradient in all of dweight.
-// stats: rows + 1 floats for the backward pass.  Scratch memory, 256-byte aligned: hc_linear_cross_entropy_bytes for the current device.
+// stats: 2 rows + 1 floats for the backward pass (each row's logarithm of its sum, its loss; the number of rows that have a token).  Scratch memory, 256-byte aligned: hc_linear_cross_entropy_bytes for the current device.
 size_t hc_linear_cross_entropy_bytes(size_t rows, size_t inner, size_t vocab);
 int hc_linear_cross_entropy(const void* x, size_t x_stride, const void* weight, size_t weight_stride, int type, const int64_t* tokens, int64_t ignore, int reduction, float* loss,
                             float* stats, size_t rows, size_t inner, size_t vocab, void* scratch, size_t scratch_bytes, hc_stream_t stream);

@@ -577,7 +577,7 @@ Tensor loss_forward(const Tensor& x, const Tensor& weight, const Tensor& tokens,
   const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
   const at::TensorOptions f = x.options().dtype(at::kFloat);
   Tensor loss = reduction == kNone ? at::empty(shape, f) : at::empty({}, f);
-  *stats = at::empty({m + 1}, f);
+  *stats = at::empty({2 * m + 1}, f);
   const size_t need = api.linear_cross_entropy_bytes(m, k, n);
   const Tensor scratch = scratch_of(need, x);
   check(api.linear_cross_entropy(x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), type_of(x), static_cast<int64_t*>(tokens.data_ptr()), ignore, reduction,

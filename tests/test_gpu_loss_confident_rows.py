@@ -89,3 +89,31 @@ def test_logits_that_are_no_numbers(rows):
         w[token] = 1.0  # and no other
         assert (ops.linear_cross_entropy(x, w, t, reduction="none") == 0).all()
     assert (ops.linear_cross_entropy(x, w[token:token + 1], torch.zeros_like(t), reduction="none") == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("rows", [1, 16, 17, 300])
+@pytest.mark.parametrize("inner,size", [(64, 20), (768, 20), (768, 400), (2048, 20), (4096, 20), (4096, 400)])
+def test_gradients_of_small_losses(inner, size, rows, kind):
+    """G at the token is -(1 - p), whatever the logits' size: dx at the token's mark, and the token's row of dW."""
+    h, vocab, off = torch.finfo(kind).eps / 2, 67, 13
+    x, w = make(rows, inner, vocab, size, off, kind, 5)
+    t = torch.full((rows,), 5, device="cuda")
+    rest = (vocab - 1) * math.exp(-off)
+    want = rest / (1 + rest)
+    logit = (x.double() @ w.double()[5]).max().item()
+    for reduction, a in (("none", None), ("sum", 1.0), ("mean", 64.0)):
+        leaves = [v.detach().requires_grad_() for v in (x, w)]
+        got = ops.linear_cross_entropy(*leaves, t, reduction=reduction)
+        weights = torch.linspace(0.5, 2.0, rows, device="cuda") if reduction == "none" else torch.full((rows,), a / (rows if reduction == "mean" else 1), device="cuda")
+        dx, dw = torch.autograd.grad(got, leaves, weights if reduction == "none" else torch.tensor(a, device="cuda"))
+        G = -weights.double() * want
+        # the loss, of which the others' sum is off relative to itself; G, rounded
+        room = U * (ADDITIONS + 12 + 3 * off) + 4 * 2 * U * 2.0 ** math.ceil(math.log2(2 * logit)) + h + 4 * U
+        least = 2.0 ** -24 if kind == F16 else 0.0  # dx and dW have no smaller steps; those of G are 2^-37 of the largest weight
+        lost = 2.0 ** -37 * weights.double().max() if kind == F16 else 0.0
+        assert ((dx[:, -2].double() - G).abs() <= 1.01 * ((room + h) * G.abs() + lost + least)).all(), float(((dx[:, -2].double() - G) / G).abs().max())
+        exact = G @ x.double()
+        size_of = G.abs() @ x.double().abs()
+        assert ((dw[5].double() - exact).abs() <= 1.01 * ((room + (rows / 16 + 20) * 2 * U) * size_of + h * exact.abs() + lost * x.double().abs().sum(0) + least)).all()
