@@ -30,6 +30,9 @@ constexpr int kOperandA = kBM * kBK * 2;
 constexpr int kGemmLinearWide = 4;  // kGemmLinear whose sums are formed in parts
 constexpr int kGemmGramWide = 5;    // kGemmGram, the same
 constexpr int kGemmLossSumsWide = 8;  // kGemmLossSums, the same
+constexpr int kGemmLossGradWide = 9;  // kGemmLossGrad, the same
+template <int MODE>
+constexpr bool kInParts = MODE == kGemmLinearWide || MODE == kGemmGramWide || MODE == kGemmLossSumsWide || MODE == kGemmLossGradWide;
 constexpr uint64_t kGemmLimitNs = 2000ull * 1000 * 1000;
 
 struct GemmParams {
@@ -488,7 +491,7 @@ __device__ __forceinline__ void multiply_tiles(const GemmParams& p, GemmBarriers
   const int total = p.tiles * p.batch;
   for (int t = unit; st.ok && t < total; t += units) {
     for (int begin = 0; begin < p.k_blocks; begin += kChunk) {
-      const int end = MODE == kGemmLinearWide || MODE == kGemmGramWide || MODE == kGemmLossSumsWide ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
+      const int end = kInParts<MODE> ? min(begin + kChunk, p.k_blocks) : p.k_blocks;
       if (!gemm_wait(&sh.acc_empty[st.acc], st.acc_phase ^ 1, sh)) {
         st.ok = false;
         return;
@@ -540,14 +543,15 @@ __device__ __forceinline__ void release_accumulator(GemmBarriers& sh, Storing& s
 template <int BN, int kCtas, int MODE>
 __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& sh, unsigned char* mine, Storing& st, uint32_t tmem, int unit, int units, int rank) {
   using S = GemmShape<BN, kCtas>;
-  constexpr bool kWide = MODE == kGemmLinearWide || MODE == kGemmGramWide || MODE == kGemmLossSumsWide, kLinear = MODE == kGemmLinear || MODE == kGemmLinearWide;
-  constexpr bool kLossSums = MODE == kGemmLossSums || MODE == kGemmLossSumsWide;
+  constexpr bool kWide = kInParts<MODE>, kLinear = MODE == kGemmLinear || MODE == kGemmLinearWide;
+  constexpr bool kLossSums = MODE == kGemmLossSums || MODE == kGemmLossSumsWide, kLossGrad = MODE == kGemmLossGrad || MODE == kGemmLossGradWide;
   constexpr bool kSymmetric = MODE == kGemmGram || MODE == kGemmGramWide || MODE == kGemmPoly;
   constexpr int kMode = MODE == kGemmLinearWide ? kGemmLinear : MODE == kGemmGramWide ? kGemmGram : MODE;
   constexpr int kPieces = kWide ? (BN / 32 + 1) / 2 : 1;  // of a warp
+  constexpr int kPer = kLossGrad && BN >= 128 ? 2 : 1;    // pieces of a box, which are one warp's
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3;      // the rows of tensor memory that this warp can reach
-  const int half = (warp - 2) >> 2;  // every second piece of 32 columns
+  const int half = (warp - 2) >> 2;  // every second piece of 32 columns, or box of them
   const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
   uint64_t* loaded = sh.loaded[warp - 2];
   float* shared_bias = sh.bias[warp - 2];
@@ -571,6 +575,7 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
       if (kLinear && p.bias && col0 + half * 32 + lane < p.n) bias = param_at(p.bias, p.bias_type, col0 + half * 32 + lane);
     }
     float sums[kPieces][32];
+    const auto piece_of = [&](int q) { return (q / kPer * 2 + half) * kPer + q % kPer; };  // of sums[q]
     if (kWide) {
 #pragma unroll
       for (int q = 0; q < kPieces; ++q)
@@ -584,10 +589,10 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
         tc_fence_after();
 #pragma unroll
         for (int q = 0; q < kPieces; ++q) {
-          if (half + 2 * q >= pieces) break;
+          if (piece_of(q) >= pieces) break;
           float v[32];
           __syncwarp();
-          tc_load32(lanes + st.acc * BN + (half + 2 * q) * 32, v);
+          tc_load32(lanes + st.acc * BN + piece_of(q) * 32, v);
           tc_load_wait(v);
 #pragma unroll
           for (int j = 0; j < 32; ++j) sums[q][j] += v[j];
@@ -609,8 +614,8 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
       if constexpr (kWide) {
 #pragma unroll
         for (int q = 0; q < kPieces; ++q) {
-          const int col = col0 + (half + 2 * q) * 32;
-          if (half + 2 * q < pieces) loss_take(sums[q], p.n - col, token - col, most, sum, p.loss.picked + row);
+          const int col = col0 + piece_of(q) * 32;
+          if (piece_of(q) < pieces) loss_take(sums[q], p.n - col, token - col, most, sum, p.loss.picked + row);
         }
       } else {
 #pragma unroll 1
@@ -625,7 +630,7 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
       if (row < p.m) p.loss.sums[(int64_t)(ni * 2 + half) * p.m + row] = make_float2(most, sum);
       continue;
     }
-    if constexpr (MODE == kGemmLossGrad) {
+    if constexpr (kLossGrad) {
       const int64_t row = row0 + lane;
       const bool in = row < p.m;
       const int64_t given = in ? p.loss.tokens[row] : p.loss.ignore, token = given - p.loss.first;
@@ -636,37 +641,31 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
         weight *= gradient_power(p.most, 1);
         picked *= gradient_power(p.most, 1);
       }
-      constexpr int kPer = BN >= 128 ? 2 : 1;  // pieces of a box
-#pragma unroll 1
-      for (int c = half * kPer; c < pieces; c += 2 * kPer) {
-        unsigned char* slot = mine + (st.uses & 1) * kSlot;
+      const auto finish = [&](float(&v)[32], int c, int h, unsigned char* slot) {  // piece c, number h of its box
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          float a, b;
+          parts((pair(v[j], v[j + 1]) + pair(less, less)) * pair(kLog2E, kLog2E), a, b);
+          parts(pair(power2(a), power2(b)) * pair(weight, weight), v[j], v[j + 1]);
+        }
+        const int64_t at = token - (col0 + c * 32);
+        if (at >= 0 && at < 32) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = j == (int)at ? picked : v[j];
+        }
+        if (!kept) {  // also where the row's logits are no numbers
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(kPer == 2 ? reinterpret_cast<uint4*>(wide_at(slot, lane, h * 4 + i)) : half_at(slot, lane, i)) = pack8_as(v + i * 8, p.type);
+      };
+      const auto begin = [&] {
         if (lane == 0) tma_wait_group_read<1>();
         __syncwarp();
-#pragma unroll
-        for (int h = 0; h < kPer; ++h) {
-          float(&v)[32] = sums[0];
-          __syncwarp();
-          tc_load32(lanes + st.acc * BN + (c + h) * 32, v);
-          tc_load_wait(v);
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float a, b;
-            parts((pair(v[j], v[j + 1]) + pair(less, less)) * pair(kLog2E, kLog2E), a, b);
-            parts(pair(power2(a), power2(b)) * pair(weight, weight), v[j], v[j + 1]);
-          }
-          const int64_t at = token - (col0 + (c + h) * 32);
-          if (at >= 0 && at < 32) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = j == (int)at ? picked : v[j];
-          }
-          if (!kept) {  // also where the row's logits are no numbers
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *(kPer == 2 ? reinterpret_cast<uint4*>(wide_at(slot, lane, h * 4 + i)) : half_at(slot, lane, i)) = pack8_as(v + i * 8, p.type);
-        }
+        return mine + (st.uses & 1) * kSlot;
+      };
+      const auto store = [&](int c, unsigned char* slot) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
@@ -674,8 +673,31 @@ __device__ __forceinline__ void store_tiles(const GemmParams& p, GemmBarriers& s
           tma_commit_group();
         }
         ++st.uses;
+      };
+      if constexpr (kWide) {
+#pragma unroll
+        for (int q = 0; q < kPieces; q += kPer) {
+          if (piece_of(q) >= pieces) break;
+          unsigned char* slot = begin();
+#pragma unroll
+          for (int h = 0; h < kPer; ++h) finish(sums[q + h], piece_of(q) + h, h, slot);
+          store(piece_of(q), slot);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = half * kPer; c < pieces; c += 2 * kPer) {
+          unsigned char* slot = begin();
+#pragma unroll
+          for (int h = 0; h < kPer; ++h) {
+            __syncwarp();
+            tc_load32(lanes + st.acc * BN + (c + h) * 32, sums[0]);
+            tc_load_wait(sums[0]);
+            finish(sums[0], c + h, h, slot);
+          }
+          store(c, slot);
+        }
+        release_accumulator<kCtas>(sh, st, rank);
       }
-      release_accumulator<kCtas>(sh, st, rank);
       continue;
     }
     const auto piece = [&](int c, float (&v)[32]) {  // false: a wait ran out
@@ -1078,7 +1100,7 @@ cudaError_t fill_params(const GemmCall& given, dev::GemmParams* out) {
   p.factor = c.factor;
   p.loss = c.loss;
   if (MODE == kGemmLossSums || MODE == dev::kGemmLossSumsWide) return p.tiles_n * 2ll <= c.loss.stretches ? cudaSuccess : cudaErrorInvalidValue;
-  if (MODE == kGemmLossGrad) return make_side_map(&p.map_out, c.out, c.type, c, true, false, BN >= 128) ? cudaSuccess : cudaErrorInvalidValue;
+  if (MODE == kGemmLossGrad || MODE == dev::kGemmLossGradWide) return make_side_map(&p.map_out, c.out, c.type, c, true, false, BN >= 128) ? cudaSuccess : cudaErrorInvalidValue;
   constexpr bool kLinear = MODE == kGemmLinear || MODE == dev::kGemmLinearWide, kUpdate = MODE == kGemmUpdate;
   if (MODE == kGemmLinear && BN >= 128 && c.out_type != kF32 && !c.in.data && make_side_map(&p.map_out, c.out, c.out_type, c, true, false, true))
     p.wide_boxes = !c.out2.data || make_side_map(&p.map_out2, c.out2, c.type, c, true, false, true);
@@ -1246,7 +1268,10 @@ int64_t gemm_loss_stretches(int64_t m, int64_t n, int64_t k) {
 cudaError_t launch_loss_sums(const GemmCall& c, cudaStream_t stream) {
   return with_loss_sums_mode(c.k, [&](auto mode) { return run_gemm_mode<decltype(mode)::value>(c, stream); });
 }
-cudaError_t launch_loss_grad(const GemmCall& c, cudaStream_t stream) { return run_gemm_mode<kGemmLossGrad>(c, stream); }
+// Logits in the same parts as those that lse is made of: what the tensor core loses of a long sum would otherwise be part of every p (8192 terms of one sign and logits of 900: 5 %).
+cudaError_t launch_loss_grad(const GemmCall& c, cudaStream_t stream) {
+  return c.k > dev::kChunk * dev::kBK ? run_gemm_mode<dev::kGemmLossGradWide>(c, stream) : run_gemm_mode<kGemmLossGrad>(c, stream);
+}
 
 cudaError_t launch_gemm(const GemmCall& c, cudaStream_t stream) {
   // sums in parts cost 8 % at 8192 x 4096 x 8192 (392 us with a bf16 result, 403 with fp32, 437 with fp32 sums in parts), 6 % at

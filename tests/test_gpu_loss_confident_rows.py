@@ -117,3 +117,20 @@ def test_gradients_of_small_losses(inner, size, rows, kind):
         exact = G @ x.double()
         size_of = G.abs() @ x.double().abs()
         assert ((dw[5].double() - exact).abs() <= 1.01 * ((room + (rows / 16 + 20) * 2 * U) * size_of + h * exact.abs() + lost * x.double().abs().sum(0) + least)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("rows", [1, 16, 17, 300])
+@pytest.mark.parametrize("inner", [1024, 1025, 4096, 8192, 16384])
+def test_probabilities_belong_to_the_sums(inner, rows, kind):
+    """A token that a row is sure of, and that is not its own: its p is 1, with logits that are long sums of one sign.  Both passes take them from sums of the same parts, so that what the tensor core
+    loses of each, 6.5e-9 of it a term within a part of 1024, is lost in both: what they may differ by is that of one part, where few rows' sums go through another instruction."""
+    h, vocab, off, size = torch.finfo(kind).eps / 2, 67, 40, 900
+    x, w = make(rows, inner, vocab, size, off, kind, 5)
+    t = torch.full((rows,), 6, device="cuda")
+    leaves = [v.detach().requires_grad_() for v in (x, w)]
+    dx, _ = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, reduction="sum"), leaves)
+    logit = (x.double() @ w.double()[5]).max().item()
+    room = 2 * h + 8 * U + 4 * 2 * U * 2.0 ** math.ceil(math.log2(logit)) + (6.5e-9 * 1024 * logit if rows <= 16 else 0.0)
+    assert ((dx[:, -2].double() - 1).abs() <= 1.01 * room).all(), float((dx[:, -2].double() - 1).abs().max())
