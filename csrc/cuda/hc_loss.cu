@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(1024) hc_loss_reduce_kernel(const float* losse
 __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss, const int64_t* tokens, int64_t ignore, int64_t rows, int64_t vocab, int reduction,
                                                               const float* losses, const float* count, float* weight, float* picked, unsigned int* most, float* factor) {
   unsigned int largest = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0 && factor) *factor = reduction == kSum ? dloss[0] : *count > 0.0f ? dloss[0] / *count : 0.0f;
+  // where no row has a token nothing is taken times an upstream gradient, which may be no number
+  if (blockIdx.x == 0 && threadIdx.x == 0 && factor) *factor = *count > 0.0f ? reduction == kSum ? dloss[0] : dloss[0] / *count : 0.0f;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows; i += gridDim.x * 256ll) {
     const int64_t token = tokens[i];
     float a = 0.0f;
@@ -153,10 +154,10 @@ __global__ void __launch_bounds__(256) hc_loss_weights_kernel(const float* dloss
   if (most && (threadIdx.x & 31) == 0 && largest) atomicMax(most, largest);
 }
 
-// dx in its own type, from the parts of its sum, which is times 2^k (gradient_power) and, over `factor`, of weights of 1
+// dx in its own type, from the parts of its sum, which is times 2^k (gradient_power) and, over `factor`, of weights of 1.  Rows without a token get zeros, also where `factor` is no number.
 template <typename T>
-__global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64_t from_stride, int parts, int64_t rows, int64_t width, const unsigned int* most, const float* factor, T* dx,
-                                                         int64_t stride) {
+__global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64_t from_stride, int parts, int64_t rows, int64_t width, const unsigned int* most, const float* factor,
+                                                         const int64_t* tokens, int64_t ignore, T* dx, int64_t stride) {
   const float power = (most ? gradient_power(most, -1) : 1.0f) * (factor ? *factor : 1.0f);
   const int64_t groups = (width + 7) / 8;
   const bool vector = stride % 8 == 0 && (reinterpret_cast<uintptr_t>(dx) & 15u) == 0;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(256) hc_loss_dx_kernel(const float* sum, int64
       for (int j = 0; j < 8; ++j) v[j] += w[j];
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= power;
+    for (int j = 0; j < 8; ++j) v[j] = tokens[r] == ignore ? 0.0f : v[j] * power;
     if (vector && c + 8 <= width) {
       store8(dx + r * stride + c, v);
     } else {
@@ -374,9 +375,9 @@ int hc_linear_cross_entropy_backward(const void* x, size_t x_stride, const void*
   const size_t dx_blocks = (rows * (up(inner, 8) / 8) + 255) / 256;
   const unsigned grid = (unsigned)(dx_blocks < 2368 ? dx_blocks : 2368);
   if (type == kBf16)
-    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, factor, static_cast<__nv_bfloat16*>(dx), (int64_t)dx_stride);
+    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, factor, tokens, ignore, static_cast<__nv_bfloat16*>(dx), (int64_t)dx_stride);
   else
-    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, factor, static_cast<__half*>(dx), (int64_t)dx_stride);
+    dev::hc_loss_dx_kernel<<<grid, 256, 0, stream>>>(dx_sum, dx_ld, l.parts, (int64_t)rows, (int64_t)inner, most, factor, tokens, ignore, static_cast<__half*>(dx), (int64_t)dx_stride);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
