@@ -17,7 +17,8 @@
 // Backward: dK and dV in a kernel whose CTA has a tile of keys and goes through the queries, dQ in one whose CTA has a tile of queries.  That forms the scores twice (8 products instead of 5, P K below among them), and
 // needs no atomic additions, whose order would change the result, and no array of partial dQ.
 //
-// In fp16, which has no numbers below 2^-24, P is held times a power of two, and dS times one that 2 max|dO_i| max|V_j| (norms of rows, which bound it) gives.
+// In fp16, which has no numbers below 2^-24, P is held times a power of two, and dS times one that 2 max|dO_i| max|V_j| (norms of rows, which bound it) gives, over the queries and keys of a
+// sequence's key head: what else is in the batch has no part in it.
 #include <math.h>
 
 #include <type_traits>
@@ -66,7 +67,7 @@ struct AttnParams {
   float* less;      // [batch heads][rows]: minus the logarithm (base 2) of a query's sum of exponentials, for the backward pass
   float* delta;  // as `less`
   void *dq, *dk, *dv;
-  const unsigned int* most;  // bits of max|dO_i|, max|V_j| (fp16)
+  const unsigned int* most;  // [batch][key heads]: bits of the squares of max|dO_i|, max|V_j| (fp16)
   int64_t less_ld;
   int batch, heads, kv_heads, group, tq, tk, d, off, window, sinks;
   int packed;   // rows of the one tile that holds the queries of all heads of a key's head, or 0
@@ -850,7 +851,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 16 ? 1 : kD == 64 ? 3 :
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
-// fp16: the largest square of a norm of dO's rows (the first `blocks[0] * heads[0] * batch` blocks) and of V's.  Eight values a thread, four rows of a thread on their way together; a block has
+// fp16: for each sequence's key head the largest square of a norm of dO's rows (the first `blocks[0] * heads[0] * batch` blocks) and of V's.  Eight values a thread, four rows of a thread on their way together; a block has
 // 4 * 256 / kLanes rows of a head.
 struct RowsOf {
   const void* data[2];
@@ -884,7 +885,7 @@ __global__ void __launch_bounds__(256) hc_attention_rows_kernel(const __grid_con
     if (square < INFINITY) largest = max(largest, __float_as_uint(square));
   }
   largest = __reduce_max_sync(0xffffffffu, largest);
-  if ((threadIdx.x & 31) == 0 && largest) atomicMax(most + n, largest);
+  if ((threadIdx.x & 31) == 0 && largest) atomicMax(most + 2 * ((int64_t)b * of.heads[1] + h / (of.heads[n] / of.heads[1])) + n, largest);
 }
 // The power of two that dS is held times in fp16: 2 max|dO_i| max|V_j|, which |dS| does not exceed, comes to below 2^15 (from the squares of both).
 __device__ __forceinline__ float ds_power(const unsigned int* most, int sign) {
@@ -928,6 +929,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   at /= heads;
   const int b = (int)(at % p.batch), block = kKeys ? (int)(at / p.batch) : p.blocks - 1 - (int)(at / p.batch);
   const int t0 = block * kTile;  // the tile's first row
+  const int64_t most_at = 2 * ((int64_t)b * p.kv_heads + (kKeys ? head : head / p.group));  // of p.most
   // the stream: queries that see one of the keys, head after head; or the keys that the queries see
   const int q_first = max(t0 - p.off, 0) / kStep,
             q_last = t0 < p.sinks ? p.tq - 1 : (int)min((int64_t)p.tq - 1, (int64_t)min(t0 + kTile, p.tk) - 1 + p.window - 1 - p.off);
@@ -1034,7 +1036,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
       if (kF16) grid_dependency_wait();  // behind the largest norms
       if (p.dk) launch_dependents();  // the keys' pass; without it, what comes next waits for the end
     }
-    const float power = kF16 ? ds_power(p.most, 1) : 1.0f, back = kF16 ? ds_power(p.most, -1) : 1.0f;
+    const float power = kF16 ? ds_power(p.most + most_at, 1) : 1.0f, back = kF16 ? ds_power(p.most + most_at, -1) : 1.0f;
     const Pair gain = pair(power * (kBias ? 1.0f / 16384.0f : 1.0f), power * (kBias ? 1.0f / 16384.0f : 1.0f));
     const Pair scale = pair(p.scale2, p.scale2), minus = pair(-1.0f, -1.0f), bias = pair(kBias, kBias);
     const bool in = t < (kKeys ? p.tk : p.tq);
@@ -1228,7 +1230,7 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
   attn_end<S::kColumns>(tmem);
   if (!kKeys || p.splits == 1) return;
   cluster_meet(p.splits);
-  const float back = kF16 ? ds_power(p.most, -1) : 1.0f;
+  const float back = kF16 ? ds_power(p.most + most_at, -1) : 1.0f;
   for (int n = threadIdx.x * p.splits + rank; n < min(kTile, p.tk - t0) * (kD / 4); n += S::kBackwardThreads * p.splits) {
     const int row = n / (kD / 4), column = n % (kD / 4) * 8;  // of dV and dK side by side
     const bool second = column >= kD;
@@ -1398,7 +1400,10 @@ cudaError_t run_backward(dev::AttnParams& p, const hc_heads& dout, const hc_head
   return launch_with(dev::hc_attention_backward_kernel<T, kD, true>, (int64_t)p.batch * p.kv_heads * p.blocks * splits, splits, dev::AttnShape<kD>::kBackwardThreads, smem, stream, true, p);
 }
 
-size_t backward_bytes(const Sizes& s) { return up(s.batch * s.heads * stats_ld(s.queries) * sizeof(float), 256) + 256; }
+// delta, and behind it what fp16's powers of two are made of
+size_t delta_bytes(const Sizes& s) { return up(s.batch * s.heads * stats_ld(s.queries) * sizeof(float), 256); }
+size_t most_bytes(const Sizes& s) { return s.batch * s.kv_heads * 2 * sizeof(unsigned int); }
+size_t backward_bytes(const Sizes& s) { return delta_bytes(s) + up(most_bytes(s), 256); }
 
 }  // namespace
 
@@ -1475,8 +1480,8 @@ int hc_attention_backward(hc_heads dout, const void* out, hc_heads q, hc_heads k
   if (!scratch || !lies_at(scratch, 256) || scratch_bytes < need) return kErrArgument;
   dev::AttnParams p;
   fill_attention(&p, s, window, sinks, scale);
-  unsigned int* most = type == kF16 ? reinterpret_cast<unsigned int*>(static_cast<unsigned char*>(scratch) + need - 256) : nullptr;
-  if (most && cudaMemsetAsync(most, 0, 8, stream) != cudaSuccess) return kErrCuda;
+  unsigned int* most = type == kF16 ? reinterpret_cast<unsigned int*>(static_cast<unsigned char*>(scratch) + delta_bytes(s)) : nullptr;
+  if (most && cudaMemsetAsync(most, 0, most_bytes(s), stream) != cudaSuccess) return kErrCuda;
   p.less = const_cast<float*>(stats);
   p.delta = static_cast<float*>(scratch);
   p.o = const_cast<void*>(out);
