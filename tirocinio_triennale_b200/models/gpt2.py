@@ -63,6 +63,8 @@ class Block(nn.Module):
         self.fused = cfg.fused
         if cfg.attention not in ("torch", "own") or cfg.attention == "own" and not cfg.fused:
             raise ValueError("GPT2: attention is \"torch\", or with fused \"own\"")
+        if cfg.window is not None and cfg.window < 1 or cfg.sinks < 0:
+            raise ValueError("GPT2: a window is of at least one position, sinks are not negative")
         self.own_attention = cfg.attention == "own"
         self.window, self.sinks = cfg.window, cfg.sinks
 
