@@ -17,7 +17,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``bits``: 32, or 8 for moments of a byte each with a scale for every 256 of them; ``seed``: of their random rounding.
     ``capturable``: the step's number is held on the device and counted for a group as a whole, so that a captured step can be replayed; ``lr`` may
-    then be a float32 CUDA tensor of one value, which can be changed between replays."""
+    then be a float32 CUDA tensor of one value, which can be changed between replays.  A step that is captured without it, or that comes before every parameter's state
+    has begun in a step outside, raises RuntimeError."""
 
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, bits: int = 32, seed: int = 0,
                  capturable: bool = False):
@@ -40,6 +41,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if torch.cuda.is_current_stream_capturing():
+            self._check_capture()
         for number, group in enumerate(self.param_groups):
             alike = {}  # a parameter that had no gradient in some step is behind the others
             for p in group["params"]:
@@ -66,6 +69,15 @@ class AdamW(torch.optim.Optimizer):
                                [s["scales"] for s in states] if group["bits"] == 8 else None, step=group["steps"] if group["capturable"] else count, lr=group["lr"],
                                betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"] + 0x1000193 * number)
         return loss
+
+    def _check_capture(self):
+        # what begins in a captured step would begin again at each replay, and a number that the host counts would stay where it is
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if params and not group["capturable"]:
+                raise RuntimeError("AdamW: a step that is captured needs capturable=True")
+            if params and ("steps" not in group or any(not self.state.get(p) for p in params)):
+                raise RuntimeError("AdamW: the state begins in a step before the capture")
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
