@@ -746,16 +746,16 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   if (lr_at) add_stretch(stretches, *lr_at, false);
   if (step_at) add_stretch(stretches, *step_at, false);
   TORCH_CHECK_VALUE(!any_overlap(stretches), "adamw_step: tensors overlap, or one is in the lists twice");
-  for (const Kind& k : kinds)
-    check(api.adamw(k.tensors.data(), k.tensors.size(), k.param, k.grad, scales ? 8 : 32, lr, static_cast<float*>(ptr(lr_at)), beta1, beta2, eps, weight_decay, step,
-                    static_cast<int64_t*>(ptr(step_at)), seed, stream_of(first)),
-          "adamw_step");
-  for (size_t i = 0; i < count; ++i) {  // whoever kept one of them for a backward pass is told
+  for (size_t i = 0; i < count; ++i) {  // whoever kept one of them for a backward pass is told; and what may not be changed here raises before it is
     params[i].unsafeGetTensorImpl()->bump_version();
     exp_avgs[i].unsafeGetTensorImpl()->bump_version();
     exp_avg_sqs[i].unsafeGetTensorImpl()->bump_version();
     if (scales) (*scales)[i].unsafeGetTensorImpl()->bump_version();
   }
+  for (const Kind& k : kinds)
+    check(api.adamw(k.tensors.data(), k.tensors.size(), k.param, k.grad, scales ? 8 : 32, lr, static_cast<float*>(ptr(lr_at)), beta1, beta2, eps, weight_decay, step,
+                    static_cast<int64_t*>(ptr(step_at)), seed, stream_of(first)),
+          "adamw_step");
 }
 
 std::tuple<Tensor, Tensor> adamw_values(const Tensor& exp_avg, const Tensor& exp_avg_sq, const Tensor& scales) {
