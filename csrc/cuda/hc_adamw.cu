@@ -12,9 +12,9 @@
 // stay where it is for ever, so both are rounded up or down at random, in proportion to what is lost.  The random bits are a hash of the
 // value's number, the tensor's number, the step and a seed.  A sqrt(v) above 0 stays above 0, or the next step would divide by eps.
 //
-// Bound by memory: 28 bytes an element with fp32 parameters and gradients, 16 with moments in 8 bits.  A warp takes a block of 256 values, eight
-// neighbours a lane, so a block's largest values are one reduction instruction each and nothing is shared between warps.  The tensors'
-// addresses are arguments of the kernel (a table of 16 or of 448), so that a call copies nothing to the device.
+// With moments in 32 bits bound by memory: 28 bytes an element with fp32 parameters and gradients (124 million: 557 us, 6.25 TB/s).  With moments in 8 bits 16 bytes, and bound by the instructions: 99 an
+// element, 75 % of the issue slots, DRAM 52 % (455 us).  A warp takes a block of 256 values, four neighbours a lane, twice, so a block's largest values are one reduction instruction each and nothing is shared
+// between warps.  The tensors' addresses are arguments of the kernel (a table of 16 or of 448), so that a call copies nothing to the device.
 #include <math.h>
 
 #include "hc_host.cuh"

@@ -17,8 +17,9 @@
 // Backward: dK and dV in a kernel whose CTA has a tile of keys and goes through the queries, dQ in one whose CTA has a tile of queries.  That forms the scores twice (8 products instead of 5, P K below among them), and
 // needs no atomic additions, whose order would change the result, and no array of partial dQ.
 //
-// In fp16, which has no numbers below 2^-24, P is held times a power of two, and dS times one that 2 max|dO_i| max|V_j| (norms of rows, which bound it) gives, over the queries and keys of a
-// sequence's key head: what else is in the batch has no part in it.
+// In fp16, which has no numbers below 2^-24, P is held times 2^6 in the forward pass (its reference may be 2^8 below a row's largest), times 2^14 for few rows and in the keys' pass, and as it is in the
+// queries' pass, where P K needs no more than a few bits; dS times a power that 2 max|dO_i| max|V_j| (norms of rows, which bound it) gives, over the queries and keys of a sequence's key head: what else
+// is in the batch has no part in it.
 #include <math.h>
 
 #include <type_traits>
@@ -1184,8 +1185,8 @@ __global__ void __launch_bounds__(AttnShape<kD>::kBackwardThreads, AttnShape<kD>
       if (p.splits > 1) {
         store_row<float, 64>(lanes + kSum1 + part * 64, joined + row * kRow + part * 64, 64, 1.0f, true, count > 0, false);
       } else {
-      T* to = static_cast<T*>(second ? p.dk : p.dv) + (((int64_t)b * p.tk + t) * p.kv_heads + head) * p.d + c;
-      store_row<T, 64>(lanes + kSum1 + part * 64, to, p.d - c, second ? p.scale * back : kF16 ? 1.0f / 16384.0f : 1.0f, in, count > 0, false);
+        T* to = static_cast<T*>(second ? p.dk : p.dv) + (((int64_t)b * p.tk + t) * p.kv_heads + head) * p.d + c;
+        store_row<T, 64>(lanes + kSum1 + part * 64, to, p.d - c, second ? p.scale * back : kF16 ? 1.0f / 16384.0f : 1.0f, in, count > 0, false);
       }
     }
     if (!ok && kKeys && p.splits > 1)  // a wait ran out: no numbers

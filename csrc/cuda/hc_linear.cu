@@ -540,7 +540,7 @@ cudaError_t launch_few_rows_loss(const GemmCall& c, cudaStream_t stream) {
   p.x = c.a.data, p.w = c.b.data, p.ldx = c.a.ld, p.ldw = c.b.ld;
   p.inner = c.k, p.width = c.n, p.rows = (int)c.m;
   p.loss = c.loss;
-  // a warp to sixteen tokens where there are sixteens for most warps that the SMs hold, and 16-byte loads
+  // a warp to sixteen tokens where there are sixteens for a quarter of the warps that the SMs hold (`resident` blocks of eight), and 16-byte loads
   const int64_t groups = (c.n + 15) / 16, resident = (int64_t)(device_info().sms > 0 ? device_info().sms : 1) * (c.m <= 8 ? 3 : 2);
   if (groups < resident * 2 || !(c.k % 8 == 0 && gemm_operand_ok(c.a.data, c.a.ld) && gemm_operand_ok(c.b.data, c.b.ld))) {
     run_few_rows<true>(p, c.type, stream);

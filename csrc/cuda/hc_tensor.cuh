@@ -1,4 +1,4 @@
-// Tensor memory, for the kernels that feed tcgen05: fences, loads and stores of a warp's 32 rows, operand descriptors.
+// Tensor memory, for the kernels that feed tcgen05: fences, loads and stores of a warp's 32 rows; and two arithmetic helpers of what is done to them.
 #pragma once
 #include "hc_device.cuh"
 #include "hc_train.cuh"
