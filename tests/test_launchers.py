@@ -35,9 +35,6 @@ def attention(heads, kv, queries, keys, d, kind=1, batch=1):
 def attention_backward(heads, kv, queries, keys, d, kind=1, batch=1):
     h = lambda n, t: Heads(at, n * t * d, t * d, d)
     return lambda: lib.hc_attention_backward(h(heads, queries), at, h(heads, queries), h(kv, keys), h(kv, keys), kind, at, at, at, at, batch, heads, kv, queries, keys, d, 0, 0, 1.0, at, big, None)
-
-def linear(rows, inner, width, kind=1, out=1):
-    return lambda: lib.hc_linear(at, inner, at, inner, kind, None, 0, None, 0, at, out, width, None, 0, 0, rows, inner, width, at, big, None)
 """
 
 
